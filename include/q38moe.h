@@ -516,6 +516,65 @@ int q38moe_qsa_attention(const void* q, const void* k, const void* v, const void
                          int64_t B, int32_t S, int32_t H, int32_t KV, int32_t kk, float scale, int32_t dtype,
                          void* stream);
 
+/*
+ * Softmax cross entropy of a linear head without its logits (the training and evaluation loss over the tied head,
+ * modeling:1398-1431; the reference's trainer calls a fused third-party one, q38/train.py:223-224):
+ *   z = x . w^T,  lse[t] = log sum_v exp z[t,v],  loss[t] = lse[t] - z[t, targets[t]]
+ * x [T,h] and w [V,h] in dtype, targets [T] int32 or int64, loss and lse [T] fp32; logits, maxima and sums in fp32.
+ * Rows whose target is ignore_index have loss 0 (whatever their x) and lse 0; a target outside [0, V) makes its
+ * row's loss and lse NaN. reduced (NULL to skip) = {sum of the losses, or with mean their sum over max(1, rows not
+ * ignored); the factor 1 or 1 / max(1, rows not ignored)}. h a multiple of 64 up to 65536, T <= 2^24, V < 2^21.
+ * Backward: with s[t,v] = exp(z[t,v] - lse[t]) - [v = targets[t]] and G[t] = g[0] or, with g_per_row, g[t], times
+ * *row_scale (NULL: 1):  dx = G s . w [T,h] and dw = (G s)^T . x [V,h] in dtype (either may be NULL). Ignored rows
+ * get zeros and count in nothing. The vocabulary is taken in pieces whose s fits 256 MiB of the workspace (at least 256
+ * rows of w each). Workspaces: q38moe_linear_ce_workspace_bytes with needs 0 (forward) or the set of gradients.
+ */
+#define Q38MOE_NEED_LOSS_X 1
+#define Q38MOE_NEED_LOSS_W 2
+int q38moe_linear_ce_workspace_bytes(int64_t T, int32_t h, int32_t V, int32_t needs, int32_t dtype, size_t* bytes);
+int q38moe_linear_ce_forward(const void* x, const void* w, const void* targets, int32_t targets_int64,
+                             int64_t ignore_index, float* loss, float* lse, float* reduced, int32_t mean, int64_t T,
+                             int32_t h, int32_t V, void* workspace, size_t workspace_bytes, int32_t dtype,
+                             void* stream);
+int q38moe_linear_ce_backward(const float* g, int32_t g_per_row, const float* row_scale, const void* x, const void* w,
+                              const void* targets, int32_t targets_int64, int64_t ignore_index, const float* lse,
+                              void* dx, void* dw, int64_t T, int32_t h, int32_t V, void* workspace,
+                              size_t workspace_bytes, int32_t dtype, void* stream);
+
+/*
+ * Global norm of n tensors (gradients; no counterpart in the reference's MoE path): total = (sum |g|^p)^(1/p) over all
+ * of them, p = 1, 2 or infinity, sums in fp64, and clipping: dst_i = g_i * min(1, max_norm / (total + 1e-6)). src,
+ * dst, numel and the dtypes are host arrays of n entries, read before the call returns; the tensors are contiguous,
+ * bf16 or fp32 each, aligned to their elements (16-byte aligned ones are faster). dst_i may be src_i (then of its dtype); no
+ * output may otherwise overlap a tensor or another output. total: fp32, on the device. A NaN or an infinity among
+ * the gradients makes the total one, and clipping by it gives what the formula gives. Workspace:
+ * q38moe_grad_norm_workspace_bytes.
+ */
+#define Q38MOE_NORM_L1 1
+#define Q38MOE_NORM_L2 2
+#define Q38MOE_NORM_INF 3
+int q38moe_grad_norm_workspace_bytes(int32_t n, size_t* bytes);
+int q38moe_grad_norm(const void* const* src, const int64_t* numel, const int32_t* src_dtype, int32_t n, int32_t norm,
+                     float* total, void* workspace, size_t workspace_bytes, void* stream);
+int q38moe_clip_grads(const void* const* src, void* const* dst, const int64_t* numel, const int32_t* src_dtype,
+                      const int32_t* dst_dtype, int32_t n, int32_t norm, float max_norm, float* total, void* workspace,
+                      size_t workspace_bytes, void* stream);
+
+/*
+ * Rows to experts of the caller's own and back, on the permutation of q38moe_permute (pair p = t*k + j of expert-sorted
+ * row inv[p]; pairs whose index lies outside [0, E) have no row). spread: dst[inv[p]] = src[t] (* w[p] unless w is
+ * NULL), zeros in the rows behind the filled ones, and with y [T*k,h] dw[p] = <src[t], y[inv[p]]> (0 for pairs without
+ * a row); dst or dw may be NULL. collect: out[t] = sum_j src[inv[p]] (* w[p] unless w is NULL). src, dst, y and out in
+ * dtype, w and dw [T,k] in w_dtype (dtype or fp32); products and sums fp32, rounded once. Dispatch is spread
+ * without w and its gradient collect without w; combine is collect with w and its gradients spread with w and y.
+ */
+int q38moe_spread_rows(const void* src, const void* w, int32_t w_dtype, const void* y, const void* topk_idx,
+                       int32_t idx_is_int64, const int32_t* inv, const int32_t* starts, const int32_t* counts,
+                       void* dst, void* dw, int64_t T, int32_t h, int32_t E, int32_t k, int32_t dtype, void* stream);
+int q38moe_collect_rows(const void* src, const void* w, int32_t w_dtype, const void* topk_idx, int32_t idx_is_int64,
+                        const int32_t* inv, void* out, int64_t T, int32_t h, int32_t E, int32_t k, int32_t dtype,
+                        void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -5,6 +5,7 @@
 #include <cstdlib>
 #include <cmath>
 #include <cstring>
+#include <algorithm>
 #include <mutex>
 
 #include "q38moe.h"
@@ -1465,6 +1466,279 @@ int q38moe_qsa_attention(const void* q, const void* k, const void* v, const void
   Q38_HIP(q38::launch_qsa_attention(q, k, v, qg, sel, out, B, S, H, KV, kk, scale, dtype == Q38MOE_BF16,
                                     static_cast<hipStream_t>(stream)),
           "qsa attention launch");
+  return Q38MOE_OK;
+}
+
+// ---- a training step around the block: the head's loss, gradient clipping, rows to the caller's experts ----------
+
+static int check_loss(int64_t T, int32_t h, int32_t V, int32_t dtype) {
+  Q38_CHECK(check_dtype(dtype));
+  Q38_CHECK(check_dim(h, "h"));
+  if (h > 65536) return fail(Q38MOE_EINVAL, "h must be <= 65536 (got %d)", h);
+  if (T < 0 || T > (int64_t)1 << 24) return fail(Q38MOE_EINVAL, "T must be in [0, 2^24] (got %lld)", (long long)T);
+  if (V < 1 || V >= 1 << 21) return fail(Q38MOE_EINVAL, "V must be in [1, 2^21) (got %d)", V);
+  return Q38MOE_OK;
+}
+
+int q38moe_linear_ce_workspace_bytes(int64_t T, int32_t h, int32_t V, int32_t needs, int32_t dtype, size_t* bytes) {
+  g_err[0] = 0;
+  if (bytes == nullptr) return fail(Q38MOE_EINVAL, "bytes must not be NULL");
+  Q38_CHECK(check_loss(T, h, V, dtype));
+  if (needs < 0 || needs > 3) return fail(Q38MOE_EINVAL, "needs must be a set of Q38MOE_NEED_LOSS_* (got %d)", needs);
+  *bytes = T == 0 ? 0
+                  : q38::linear_ce_workspace(T, h, V, dtype == Q38MOE_FP32, needs == 0, (needs & 1) != 0,
+                                             (needs & 2) != 0);
+  return Q38MOE_OK;
+}
+
+int q38moe_linear_ce_forward(const void* x, const void* w, const void* targets, int32_t targets_int64,
+                             int64_t ignore_index, float* loss, float* lse, float* reduced, int32_t mean, int64_t T,
+                             int32_t h, int32_t V, void* workspace, size_t workspace_bytes, int32_t dtype,
+                             void* stream) {
+  g_err[0] = 0;
+  Q38_CHECK(check_loss(T, h, V, dtype));
+  if (T == 0) return Q38MOE_OK;
+  Q38_CHECK(check_ptr(x, "x"));
+  Q38_CHECK(check_ptr(w, "w"));
+  if (targets == nullptr || loss == nullptr || lse == nullptr)
+    return fail(Q38MOE_EINVAL, "targets, loss and lse must not be NULL");
+  size_t need = 0;
+  Q38_CHECK(q38moe_linear_ce_workspace_bytes(T, h, V, 0, dtype, &need));
+  if (workspace == nullptr || workspace_bytes < need)
+    return fail(Q38MOE_EWORKSPACE, "workspace needs %zu bytes, got %zu", need, workspace_bytes);
+  Q38_CHECK(check_ptr(workspace, "workspace"));
+  (void)hipGetLastError();
+  Q38_HIP(q38::launch_linear_ce_forward(x, w, targets, targets_int64 != 0, ignore_index, loss, lse, reduced, mean != 0,
+                                        T, h, V, workspace, dtype == Q38MOE_FP32, static_cast<hipStream_t>(stream)),
+          "linear cross entropy launch");
+  return Q38MOE_OK;
+}
+
+int q38moe_linear_ce_backward(const float* g, int32_t g_per_row, const float* row_scale, const void* x, const void* w,
+                              const void* targets, int32_t targets_int64, int64_t ignore_index, const float* lse,
+                              void* dx, void* dw, int64_t T, int32_t h, int32_t V, void* workspace,
+                              size_t workspace_bytes, int32_t dtype, void* stream) {
+  g_err[0] = 0;
+  Q38_CHECK(check_loss(T, h, V, dtype));
+  if (dx == nullptr && dw == nullptr) return Q38MOE_OK;
+  if (T == 0) return fail(Q38MOE_EINVAL, "T must be positive (without rows every gradient is zero)");
+  Q38_CHECK(check_ptr(x, "x"));
+  Q38_CHECK(check_ptr(w, "w"));
+  Q38_CHECK(check_opt_ptr(dx, "dx"));
+  Q38_CHECK(check_opt_ptr(dw, "dw"));
+  if (targets == nullptr || g == nullptr || lse == nullptr)
+    return fail(Q38MOE_EINVAL, "targets, g and lse must not be NULL");
+  size_t need = 0;
+  const int32_t needs = (dx != nullptr ? Q38MOE_NEED_LOSS_X : 0) | (dw != nullptr ? Q38MOE_NEED_LOSS_W : 0);
+  Q38_CHECK(q38moe_linear_ce_workspace_bytes(T, h, V, needs, dtype, &need));
+  if (workspace == nullptr || workspace_bytes < need)
+    return fail(Q38MOE_EWORKSPACE, "workspace needs %zu bytes, got %zu", need, workspace_bytes);
+  Q38_CHECK(check_ptr(workspace, "workspace"));
+  (void)hipGetLastError();
+  Q38_HIP(q38::launch_linear_ce_backward(g, g_per_row != 0, row_scale, x, w, targets, targets_int64 != 0, ignore_index,
+                                         lse, dx, dw, T, h, V, workspace, dtype == Q38MOE_FP32,
+                                         static_cast<hipStream_t>(stream)),
+          "linear cross entropy backward launch");
+  return Q38MOE_OK;
+}
+
+// Fills `t` with the tensors from `i` on, as many as a launch takes (empty ones left out); returns the next one.
+static int32_t clip_table(q38::ClipTable& t, int32_t i, const void* const* src, void* const* dst, const int64_t* numel,
+                          const int32_t* src_dtype, const int32_t* dst_dtype, int32_t n) {
+  t.n = 0;
+  int64_t chunks = 0;
+  const int64_t size = q38::clip_chunk();
+  for (; i < n && t.n < q38::CLIP_TENSORS; ++i) {
+    if (numel[i] == 0) continue;
+    t.src[t.n] = src[i];
+    t.dst[t.n] = dst != nullptr ? dst[i] : nullptr;
+    t.numel[t.n] = numel[i];
+    t.first[t.n] = chunks;
+    t.src_f32[t.n] = src_dtype[i] == Q38MOE_FP32;
+    t.dst_f32[t.n] = dst != nullptr && dst_dtype[i] == Q38MOE_FP32;
+    chunks += (numel[i] + size - 1) / size;
+    ++t.n;
+  }
+  t.first[t.n] = chunks;
+  return i;
+}
+
+static int check_clip(const void* const* src, const int64_t* numel, const int32_t* src_dtype, int32_t n, int32_t norm) {
+  if (n < 0) return fail(Q38MOE_EINVAL, "the number of tensors must be >= 0 (got %d)", n);
+  if (norm != Q38MOE_NORM_L1 && norm != Q38MOE_NORM_L2 && norm != Q38MOE_NORM_INF)
+    return fail(Q38MOE_EINVAL, "unsupported norm %d (Q38MOE_NORM_L1, _L2 or _INF)", norm);
+  if (n > 0 && (src == nullptr || numel == nullptr || src_dtype == nullptr))
+    return fail(Q38MOE_EINVAL, "the tensors' addresses, sizes and dtypes must not be NULL");
+  for (int32_t i = 0; i < n; ++i) {
+    Q38_CHECK(check_dtype(src_dtype[i]));
+    if (numel[i] < 0 || numel[i] >= (int64_t)1 << 40) return fail(Q38MOE_EINVAL, "tensor %d has a bad size", i);
+    if (numel[i] > 0 && (src[i] == nullptr || (uintptr_t)src[i] % elem_size(src_dtype[i]) != 0))
+      return fail(Q38MOE_EINVAL, "tensor %d must not be NULL, and aligned to its elements", i);
+  }
+  return Q38MOE_OK;
+}
+
+int q38moe_grad_norm_workspace_bytes(int32_t n, size_t* bytes) {
+  g_err[0] = 0;
+  if (bytes == nullptr) return fail(Q38MOE_EINVAL, "bytes must not be NULL");
+  if (n < 0) return fail(Q38MOE_EINVAL, "the number of tensors must be >= 0 (got %d)", n);
+  const size_t launches = ((size_t)n + q38::CLIP_TENSORS - 1) / q38::CLIP_TENSORS;
+  *bytes = 8 * (launches > 0 ? launches : 1) * q38::CLIP_BLOCKS;
+  return Q38MOE_OK;
+}
+
+// The norm's partial sums of all tensors; *partials of them.
+static int norm_partials(const void* const* src, const int64_t* numel, const int32_t* src_dtype, int32_t n,
+                         int32_t norm, double* ws, int* partials, hipStream_t st) {
+  q38::ClipTable t;
+  *partials = 0;
+  for (int32_t i = 0; i < n;) {
+    i = clip_table(t, i, src, nullptr, numel, src_dtype, nullptr, n);
+    if (t.n == 0) continue;
+    int blocks = 0;
+    Q38_HIP(q38::launch_norm_partial(t, norm, ws + *partials, &blocks, st), "gradient norm launch");
+    *partials += blocks;
+  }
+  return Q38MOE_OK;
+}
+
+static int check_clip_ws(int32_t n, void* workspace, size_t workspace_bytes) {
+  size_t need = 0;
+  Q38_CHECK(q38moe_grad_norm_workspace_bytes(n, &need));
+  if (workspace == nullptr || workspace_bytes < need)
+    return fail(Q38MOE_EWORKSPACE, "workspace needs %zu bytes, got %zu", need, workspace_bytes);
+  return check_ptr(workspace, "workspace");
+}
+
+int q38moe_grad_norm(const void* const* src, const int64_t* numel, const int32_t* src_dtype, int32_t n, int32_t norm,
+                     float* total, void* workspace, size_t workspace_bytes, void* stream) {
+  g_err[0] = 0;
+  Q38_CHECK(check_clip(src, numel, src_dtype, n, norm));
+  if (total == nullptr) return fail(Q38MOE_EINVAL, "total must not be NULL");
+  Q38_CHECK(check_clip_ws(n, workspace, workspace_bytes));
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  (void)hipGetLastError();
+  double* ws = static_cast<double*>(workspace);
+  int partials = 0;
+  Q38_CHECK(norm_partials(src, numel, src_dtype, n, norm, ws, &partials, st));
+  Q38_HIP(q38::launch_norm_finish(ws, partials, norm, total, st), "gradient norm launch");
+  return Q38MOE_OK;
+}
+
+int q38moe_clip_grads(const void* const* src, void* const* dst, const int64_t* numel, const int32_t* src_dtype,
+                      const int32_t* dst_dtype, int32_t n, int32_t norm, float max_norm, float* total, void* workspace,
+                      size_t workspace_bytes, void* stream) {
+  g_err[0] = 0;
+  Q38_CHECK(check_clip(src, numel, src_dtype, n, norm));
+  if (total == nullptr) return fail(Q38MOE_EINVAL, "total must not be NULL");
+  if (!(max_norm >= 0.0f)) return fail(Q38MOE_EINVAL, "max_norm must be >= 0");
+  Q38_CHECK(check_clip_ws(n, workspace, workspace_bytes));
+  if (n > 0 && (dst == nullptr || dst_dtype == nullptr))
+    return fail(Q38MOE_EINVAL, "the outputs' addresses and dtypes must not be NULL");
+  bool in_place = true;
+  for (int32_t i = 0; i < n; ++i) {
+    Q38_CHECK(check_dtype(dst_dtype[i]));
+    if (numel[i] == 0) continue;
+    if (dst[i] == nullptr || (uintptr_t)dst[i] % elem_size(dst_dtype[i]) != 0)
+      return fail(Q38MOE_EINVAL, "output %d must not be NULL, and aligned to its elements", i);
+    if (dst[i] == src[i] && dst_dtype[i] != src_dtype[i])
+      return fail(Q38MOE_EINVAL, "output %d in place of its tensor must have its dtype", i);
+    in_place = in_place && dst[i] == src[i];
+  }
+  // Blocks write their chunks in any order: an output must not meet another output, nor a tensor that is not its own.
+  if (n > 0) {
+    struct Span {
+      uintptr_t lo, hi;
+      int32_t i;
+      bool out;
+    };
+    Span* spans = static_cast<Span*>(std::malloc(2 * (size_t)n * sizeof(Span)));
+    if (spans == nullptr) return fail(Q38MOE_EINVAL, "out of host memory");
+    size_t m = 0;
+    for (int32_t i = 0; i < n; ++i) {
+      if (numel[i] == 0) continue;
+      const uintptr_t s = (uintptr_t)src[i], d = (uintptr_t)dst[i];
+      spans[m++] = {d, d + (uintptr_t)numel[i] * elem_size(dst_dtype[i]), i, true};
+      if (s != d) spans[m++] = {s, s + (uintptr_t)numel[i] * elem_size(src_dtype[i]), i, false};
+    }
+    std::sort(spans, spans + m, [](const Span& a, const Span& b) { return a.lo < b.lo; });
+    // The farthest end so far, of any span and of outputs: a span that begins before it overlaps that one.
+    uintptr_t any = 0, outs = 0;
+    int32_t any_i = -1, outs_i = -1, bad = -1, with = -1;
+    for (size_t j = 0; j < m && bad < 0; ++j) {
+      if (spans[j].out ? spans[j].lo < any : spans[j].lo < outs) {
+        bad = spans[j].i;
+        with = spans[j].out ? any_i : outs_i;
+      }
+      if (spans[j].hi > any) any = spans[j].hi, any_i = spans[j].i;
+      if (spans[j].out && spans[j].hi > outs) outs = spans[j].hi, outs_i = spans[j].i;
+    }
+    std::free(spans);
+    if (bad >= 0) return fail(Q38MOE_EINVAL, "tensors %d and %d overlap where one is written", with, bad);
+  }
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  (void)hipGetLastError();
+  double* ws = static_cast<double*>(workspace);
+  int partials = 0;
+  Q38_CHECK(norm_partials(src, numel, src_dtype, n, norm, ws, &partials, st));
+  if (partials == 0) {
+    Q38_HIP(q38::launch_norm_finish(ws, 0, norm, total, st), "gradient norm launch");
+    return Q38MOE_OK;
+  }
+  q38::ClipTable t;
+  bool first = true;
+  for (int32_t i = 0; i < n;) {
+    i = clip_table(t, i, src, dst, numel, src_dtype, dst_dtype, n);
+    if (t.n == 0) continue;
+    Q38_HIP(q38::launch_clip_scale(t, ws, partials, norm, max_norm, in_place, first ? total : nullptr, st),
+            "gradient clipping launch");
+    first = false;
+  }
+  return Q38MOE_OK;
+}
+
+static int check_rows_args(int64_t T, int32_t h, int32_t E, int32_t k, int32_t w_dtype, const void* w, int32_t dtype) {
+  Q38_CHECK(check_dtype(dtype));
+  Q38_CHECK(check_routing(T, E, k));
+  Q38_CHECK(check_dim(h, "h"));
+  if (w != nullptr && w_dtype != dtype && w_dtype != Q38MOE_FP32)
+    return fail(Q38MOE_EINVAL, "the weights must have the rows' dtype or be fp32");
+  return Q38MOE_OK;
+}
+
+int q38moe_spread_rows(const void* src, const void* w, int32_t w_dtype, const void* y, const void* topk_idx,
+                       int32_t idx_is_int64, const int32_t* inv, const int32_t* starts, const int32_t* counts,
+                       void* dst, void* dw, int64_t T, int32_t h, int32_t E, int32_t k, int32_t dtype, void* stream) {
+  g_err[0] = 0;
+  Q38_CHECK(check_rows_args(T, h, E, k, w_dtype, w, dtype));
+  if (dw != nullptr && (y == nullptr || w == nullptr)) return fail(Q38MOE_EINVAL, "dw needs y and w");
+  if (T == 0 || (dst == nullptr && dw == nullptr)) return Q38MOE_OK;
+  Q38_CHECK(check_ptr(src, "src"));
+  Q38_CHECK(check_opt_ptr(y, "y"));
+  Q38_CHECK(check_opt_ptr(dst, "dst"));
+  if (topk_idx == nullptr || inv == nullptr || starts == nullptr || counts == nullptr)
+    return fail(Q38MOE_EINVAL, "topk_idx, inv, starts and counts must not be NULL");
+  (void)hipGetLastError();
+  Q38_HIP(q38::launch_spread_rows(src, w, w_dtype == Q38MOE_FP32, dw != nullptr ? y : nullptr, topk_idx,
+                                  idx_is_int64 != 0, inv, starts, counts, dst, dw, T, h, E, k, dtype == Q38MOE_BF16,
+                                  static_cast<hipStream_t>(stream)),
+          "spread rows launch");
+  return Q38MOE_OK;
+}
+
+int q38moe_collect_rows(const void* src, const void* w, int32_t w_dtype, const void* topk_idx, int32_t idx_is_int64,
+                        const int32_t* inv, void* out, int64_t T, int32_t h, int32_t E, int32_t k, int32_t dtype,
+                        void* stream) {
+  g_err[0] = 0;
+  Q38_CHECK(check_rows_args(T, h, E, k, w_dtype, w, dtype));
+  if (T == 0) return Q38MOE_OK;
+  Q38_CHECK(check_ptr(src, "src"));
+  Q38_CHECK(check_ptr(out, "out"));
+  if (topk_idx == nullptr || inv == nullptr) return fail(Q38MOE_EINVAL, "topk_idx and inv must not be NULL");
+  (void)hipGetLastError();
+  Q38_HIP(q38::launch_collect_rows(src, w, w_dtype == Q38MOE_FP32, topk_idx, idx_is_int64 != 0, inv, out, T, h, E, k,
+                                   dtype == Q38MOE_BF16, static_cast<hipStream_t>(stream)),
+          "collect rows launch");
   return Q38MOE_OK;
 }
 

@@ -205,4 +205,43 @@ hipError_t launch_qsa_attention(const void* q, const void* k, const void* v, con
                                 void* out, int64_t B, int S, int H, int KV, int kk, float scale, bool bf16,
                                 hipStream_t stream);
 
+// Tokens to expert-sorted rows and back (q38moe_rows.hip), rows in bf16 or fp32, w and dw in the rows' type or
+// fp32 (w_f32). spread: dst[inv[p]] = src[t] (* w[p]), zeros behind the filled rows, dw[p] = <src[t], y[inv[p]]>; w, y
+// with dw, and dst may be NULL. collect: out[t] = sum_j src[inv[p]] (* w[p]).
+hipError_t launch_spread_rows(const void* src, const void* w, bool w_f32, const void* y, const void* idx, bool idx64,
+                              const int32_t* inv, const int32_t* starts, const int32_t* counts, void* dst, void* dw,
+                              int64_t T, int h, int E, int k, bool bf16, hipStream_t st);
+hipError_t launch_collect_rows(const void* src, const void* w, bool w_f32, const void* idx, bool idx64,
+                               const int32_t* inv, void* out, int64_t T, int h, int E, int k, bool bf16,
+                               hipStream_t st);
+
+// Global norm and clipping (q38moe_clip.hip). A table of up to CLIP_TENSORS tensors, passed by value; first[i] is
+// the chunk (clip_chunk() elements) that tensor i starts at, first[n] the number of chunks.
+constexpr int CLIP_L1 = 1, CLIP_L2 = 2, CLIP_INF = 3;
+constexpr int CLIP_TENSORS = 96;
+constexpr int CLIP_BLOCKS = 2048;  // blocks of a launch at most, a partial sum each
+struct ClipTable {
+  const void* src[CLIP_TENSORS];
+  void* dst[CLIP_TENSORS];
+  int64_t numel[CLIP_TENSORS];
+  int64_t first[CLIP_TENSORS + 1];
+  uint8_t src_f32[CLIP_TENSORS], dst_f32[CLIP_TENSORS];
+  int n;
+};
+int clip_chunk();
+hipError_t launch_norm_partial(const ClipTable& t, int ord, double* partial, int* blocks, hipStream_t st);
+hipError_t launch_norm_finish(const double* partial, int n, int ord, float* norm, hipStream_t st);
+hipError_t launch_clip_scale(const ClipTable& t, const double* partial, int npartial, int ord, float max_norm,
+                             bool in_place, float* norm, hipStream_t st);
+
+// Softmax cross entropy of a linear head (q38moe_loss.hip), operands bf16 or fp32. Workspace of the forward, or of
+// the backward pass for the gradients asked for; targets int32 or int64.
+size_t linear_ce_workspace(int64_t T, int h, int V, bool f32, bool forward, bool need_x, bool need_w);
+hipError_t launch_linear_ce_forward(const void* x, const void* w, const void* targets, bool idx64, int64_t ignore,
+                                    float* loss, float* lse, float* reduced, bool mean, int64_t T, int h, int V,
+                                    void* ws, bool f32, hipStream_t st);
+hipError_t launch_linear_ce_backward(const float* g, bool g_rows, const float* r_scale, const void* x, const void* w,
+                                     const void* targets, bool idx64, int64_t ignore, const float* lse, void* dx,
+                                     void* dw, int64_t T, int h, int V, void* ws, bool f32, hipStream_t st);
+
 }  // namespace q38

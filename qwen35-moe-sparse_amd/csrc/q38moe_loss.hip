@@ -1,0 +1,851 @@
+// Softmax cross entropy of a linear head, without its logits, and its gradient.
+//
+//   z = x W^T,  lse[t] = log sum_v exp z[t,v],  loss[t] = lse[t] - z[t, target[t]]
+//   s[t,v] = exp(z[t,v] - lse[t]) - [v = target[t]],  dx = g (s W),  dW = g (s^T x)
+//
+// The forward pass multiplies tiles of the vocabulary by tiles of tokens and keeps of each only its rows' maximum and
+// sum of exponentials (fp32) and the target's logit. The backward pass takes the vocabulary in pieces whose s [T, piece]
+// fits a bounded workspace: it multiplies again (the logits were not kept), turns the fp32 accumulators into s, and
+// multiplies s by W and by x. s is rounded to the operands' type for the matrix units, before the loss's scalar
+// gradient g, which the outputs' epilogues apply: -1 + p then rounds alike in no two rows, where g (p - 1) would carry
+// one rounding error into every row. (A gradient per row has to go into s.)
+//
+// Rows whose target is the ignored one leave the problem first: a stable partition lists the others, their x is copied
+// next to each other, and the products run over those rows only, so neither the work nor a NaN in a masked row counts.
+//
+// One kernel does the four products. C[m, n] = sum_k A[m, k] B[n, k] on 256 x 256 tiles (128 x 128 where those are few),
+// four waves, each a quarter of the tile in 32x32 blocks: at one wave per SIMD with 128 x 128 elements each operand byte
+// read from LDS is used 128 times, which keeps LDS reads at half of the matrix units' time. An operand is either
+// K-contiguous (KC: rows of 128 bytes per K step) or K-strided (KS: K rows of the tile's columns, fragments by the
+// transposing LDS read in bf16), so s, x and W are used as they lie:
+//     z^T : A = W (KC), B = x (KC);   dx^T : A = W (KS), B = s (KC);   dW^T : A = x (KS), B = s (KS).
+// A K step is 128 bytes of K; two steps lie in LDS, copied there by buffer loads that write LDS directly (out of range reads give zeros: the
+// tails of every dimension). The tokens (or vocabulary rows) are the lanes of the accumulators and the reduced or stored
+// dimension their registers, so the softmax's maxima and sums are in-lane but for one exchange.
+#include "q38moe_common.h"
+#include "q38moe_kernels.h"
+
+namespace q38 {
+namespace {
+
+enum { KC = 0, KS = 1 };
+enum { EPI_LSE = 0, EPI_S = 1, EPI_OUT = 2, EPI_ACC = 3 };
+
+constexpr float LOG2E = 1.4426950408889634f;
+
+typedef short ls_i16x4_t __attribute__((ext_vector_type(4)));
+
+// Copy of 16 bytes per lane from a buffer into LDS at lds + 16 lane. The compiler does not see these loads; the step's
+// barrier waits for them.
+__device__ __forceinline__ void ls_dma(u32x4_t rsrc, uint32_t voff, uint32_t soff, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 1\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(lds), "v"(voff),
+               "s"(rsrc), "s"(soff)
+               : "memory", "m0");
+}
+
+__device__ __forceinline__ uint32_t uniform(uint32_t v) { return __builtin_amdgcn_readfirstlane(v); }
+
+// Buffer resource (raw, no format) over `bytes` bytes at p; nothing where bytes <= 0.
+__device__ __forceinline__ u32x4_t ls_rsrc(const uint8_t* p, int64_t bytes) {
+  const uint64_t a = (uint64_t)(uintptr_t)p;
+  const uint32_t n = bytes <= 0 ? 0u : (bytes >= 0xffffffffll ? 0xffffffffu : (uint32_t)bytes);
+  return (u32x4_t){uniform((uint32_t)a), uniform((uint32_t)(a >> 32) & 0xffffu), uniform(n), 0x00020000u};
+}
+
+__device__ __forceinline__ uint2 ls_read_tr(const uint8_t* p) {
+  const ls_i16x4_t v = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+      (__attribute__((address_space(3))) ls_i16x4_t*)(uintptr_t)((const __attribute__((address_space(3))) uint8_t*)p));
+  return __builtin_bit_cast(uint2, v);
+}
+
+// One tile operand: R rows (KC) or columns (KS) of it, F32 elements or bf16.
+template <bool F32, int R, int L>
+struct Operand {
+  static constexpr int ESZ = F32 ? 4 : 2;
+  static constexpr int BK = 128 / ESZ;        // K elements of a step
+  static constexpr int NDMA = R / 32;         // copies per wave and step
+  static constexpr int PITCH = L == KC ? 128 : R * ESZ;
+  static constexpr int LPR = PITCH / 16;      // lanes per LDS row of a copy
+  static constexpr int NOFF = L == KC ? 4 : R / 64;  // lane offsets of a wave's fragments
+
+  // Offset of copy j's 16 bytes of this lane from the operand's base: rows are ld bytes apart. Chunk c of row r lies at
+  // c ^ swz(r): the 16 lanes that read together then cover the 64 banks.
+  static __device__ __forceinline__ uint32_t voff(int j, int wave, int lane, uint32_t ld) {
+    const int row = wave * (L == KC ? R / 4 : BK / 4) + j * (64 / LPR) + lane / LPR;
+    const int sw = L == KC ? (row >> 1) & 7 : (F32 ? 8 * ((row >> 2) & 1) : 4 * (row & 3));
+    return (uint32_t)row * ld + 16u * (uint32_t)((lane % LPR) ^ sw);
+  }
+
+  // This lane's LDS offset of fragments: of K substep i (KC; block b adds 32 rows) or of block i (KS; substep u adds
+  // rows).
+  static __device__ __forceinline__ int foff(int i, int half, int lane) {
+    const int r0 = half * (R / 2);
+    if constexpr (L == KC) {
+      const int row = r0 + (lane & 31);
+      return row * 128 + 16 * ((2 * i + (lane >> 5)) ^ ((row >> 1) & 7));
+    } else if constexpr (F32) {
+      const int col = r0 + 32 * i + (lane & 31);
+      return 4 * (lane >> 5) * PITCH + 16 * ((col >> 2) ^ (8 * (lane >> 5))) + 4 * (col & 3);
+    } else {
+      const int g = lane >> 4, gi = lane & 15;
+      const int row = 8 * (g >> 1) + (gi >> 2), col = r0 + 32 * i + 16 * (g & 1) + 4 * (gi & 3);
+      return row * PITCH + 16 * ((col >> 3) ^ (4 * (row & 3))) + 2 * (col & 7);
+    }
+  }
+
+  // Fragment of block b, substep u (a quarter of the step's K): 16 bytes of K per lane.
+  static __device__ __forceinline__ u32x4_t frag(const uint8_t* lds, const int (&off)[NOFF], int b, int u) {
+    if constexpr (L == KC) {
+      return ld16(lds + off[u] + b * 32 * 128);
+    } else if constexpr (F32) {
+      const uint8_t* p = lds + off[b] + u * 8 * PITCH;
+      u32x4_t v;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = *reinterpret_cast<const uint32_t*>(p + e * PITCH);
+      return v;
+    } else {
+      const uint8_t* p = lds + off[b] + u * 16 * PITCH;
+      const uint2 a = ls_read_tr(p), c = ls_read_tr(p + 4 * PITCH);
+      return (u32x4_t){a.x, a.y, c.x, c.y};
+    }
+  }
+};
+
+// acc += A B (or = A B): inline asm with the accumulator in its own AGPRs, as the four-wave gate/up kernel does it and
+// for its reasons; the build checks that no VALU write of an operand comes right before one.
+template <bool F32, bool FIRST>
+__device__ __forceinline__ void ls_mfma(f32x16_t& acc, u32x4_t a, u32x4_t b) {
+  if constexpr (F32) {
+    if constexpr (FIRST)
+      asm volatile("s_nop 1\n\tv_mfma_f32_32x32x2_f32 %0, %1, %2, 0" : "=a"(acc) : "v"(a[0]), "v"(b[0]));
+    else
+      asm volatile("s_nop 1\n\tv_mfma_f32_32x32x2_f32 %0, %1, %2, %0" : "+a"(acc) : "v"(a[0]), "v"(b[0]));
+#pragma unroll
+    for (int e = 1; e < 4; ++e)
+      asm volatile("s_nop 1\n\tv_mfma_f32_32x32x2_f32 %0, %1, %2, %0" : "+a"(acc) : "v"(a[e]), "v"(b[e]));
+  } else if constexpr (FIRST) {
+    asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %1, %2, 0" : "=a"(acc) : "v"(a), "v"(b));
+  } else {
+    asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+a"(acc) : "v"(a), "v"(b));
+  }
+}
+// Wait states between the last MFMA and VALU reads of its result (16 passes).
+__device__ __forceinline__ void ls_drain() { asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 7" ::: "memory"); }
+
+__device__ __forceinline__ uint32_t ls_lds_addr(const void* p) {
+  return uniform((uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)p);
+}
+
+struct LsParams {
+  const uint8_t* A;      // KC [M, K], KS [K, M]
+  const uint8_t* B;      // KC [N, K], KS [K, N]
+  const uint8_t* alt;    // the operand that holds tokens where every row counts (the uncopied x)
+  int64_t lda, ldb;      // bytes between rows
+  int64_t M, N, K;       // extents (the tokens' one: an upper bound)
+  int64_t m_rows;        // rows (KC) or columns of A that exist, <= M: the others of M multiply zeros
+  const int32_t* count;  // tokens that count (device), NULL: all
+  int64_t T;             // tokens of the call
+  int parts;             // K split into this many runs of whole steps
+  // epilogues
+  int64_t v0;            // EPI_S: first vocabulary row of the piece
+  float2* part;          // EPI_LSE: {max, sum} [2 ceil(M / BM), T]
+  const int32_t* tgt;    // EPI_LSE, EPI_S: target per counted token
+  float* zt;             // EPI_LSE: the target's logit
+  const int32_t* rows;   // original row of a counted token
+  const float* lse;      // EPI_S: by original row
+  const float* g_row;    // EPI_S: gradient per original row, or NULL
+  void* out;             // EPI_S: s; EPI_OUT: the gradient; EPI_ACC: fp32 [parts, N, M]
+  int64_t ldo;           // elements between rows of out
+  const float* g_scale;  // EPI_OUT: the loss's gradient (NULL: 1)
+  const float* r_scale;  // EPI_OUT: the reduction's factor (NULL: 1)
+  bool scatter;          // EPI_OUT: rows through `rows`
+  bool add;              // EPI_ACC: add to what is there
+  bool out_f32;
+};
+
+// Position of a work item: tile (m0, n0) and its K steps.
+struct LsItem {
+  int m, n, part, k0, nk;
+};
+
+template <bool F32, int BM, int BN, int LA, int LB, int EPI>
+__global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void ls_gemm_kernel(const LsParams p) {
+  using OA = Operand<F32, BM, LA>;
+  using OB = Operand<F32, BN, LB>;
+  constexpr int MB = BM / 64, NB = BN / 64;  // 32x32 blocks of a wave
+  constexpr int SLOT = (BM + BN) * 128;
+  constexpr int BK = OA::BK, ESZ = OA::ESZ;
+  __shared__ __align__(1024) uint8_t lds[2 * SLOT];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = (int)uniform((uint32_t)tid >> 6);
+  const int wm = wave >> 1, wn = wave & 1;
+
+  // Tokens are N of z^T and dx^T, K of dW^T.
+  const int64_t cnt = p.count != nullptr ? (int64_t)load_uniform(p.count) : p.T;
+  const bool all = cnt >= p.T;
+  const bool tok_k = EPI == EPI_ACC ? LB == KS : (EPI == EPI_OUT ? LB == KS : false);
+  const int64_t N = tok_k ? p.N : cnt, K = tok_k ? cnt : p.K;
+  const uint8_t* const A = tok_k && all && p.alt != nullptr ? p.alt : p.A;
+  const uint8_t* const B = !tok_k && all && p.alt != nullptr ? p.alt : p.B;
+  const int ntm = (int)((p.M + BM - 1) / BM), ntn = (int)((N + BN - 1) / BN);
+  const int steps = (int)((K + BK - 1) / BK), per = (steps + p.parts - 1) / p.parts;
+  const int64_t tiles = (int64_t)ntm * ntn, total = tiles * p.parts;
+
+  // Work items of neighbouring blocks on an XCD are neighbouring tiles: 8 tiles of M by as many of N as it has room for.
+  const int G = gridDim.x;
+  const int first = (G & 7) == 0 ? (int)(blockIdx.x & 7) * (G >> 3) + (int)(blockIdx.x >> 3) : (int)blockIdx.x;
+  if (first >= total) return;
+  auto item_of = [&](int64_t L) {
+    LsItem it;
+    it.part = (int)(L / tiles);
+    const int t = (int)(L - (int64_t)it.part * tiles);
+    const int grp = t / (8 * ntn), rem = t - grp * 8 * ntn;
+    const int gm = min(8, ntm - grp * 8);
+    it.n = rem / gm;
+    it.m = grp * 8 + rem - it.n * gm;
+    it.k0 = it.part * per;
+    it.nk = max(1, min(per, steps - it.k0));  // a part without steps multiplies zeros
+    return it;
+  };
+
+  uint32_t va[OA::NDMA], vb[OB::NDMA];
+#pragma unroll
+  for (int j = 0; j < OA::NDMA; ++j) va[j] = OA::voff(j, wave, lane, (uint32_t)p.lda);
+#pragma unroll
+  for (int j = 0; j < OB::NDMA; ++j) vb[j] = OB::voff(j, wave, lane, (uint32_t)p.ldb);
+  int fa[OA::NOFF], fb[OB::NOFF];
+#pragma unroll
+  for (int i = 0; i < OA::NOFF; ++i) fa[i] = OA::foff(i, wm, lane);
+#pragma unroll
+  for (int i = 0; i < OB::NOFF; ++i) fb[i] = BM * 128 + OB::foff(i, wn, lane);
+  const uint32_t lds0 = ls_lds_addr(lds);
+
+  // The stream of K steps over this block's items, as the copies see it.
+  int64_t c_item = first;
+  LsItem c = item_of(c_item);
+  int c_step = 0;
+  u32x4_t ra, rb;
+  auto bases = [&]() {
+    const bool live = c_item < total;
+    const int64_t k = (int64_t)(c.k0 + c_step) * BK;
+    if (LA == KC) {
+      const int64_t r0 = (int64_t)c.m * BM;
+      ra = ls_rsrc(A + r0 * p.lda + k * ESZ,
+                   live && k < K ? min((int64_t)BM, p.m_rows - r0) * p.lda - k * ESZ : 0);
+    } else {
+      const int64_t c0 = (int64_t)c.m * BM * ESZ;
+      ra = ls_rsrc(A + k * p.lda + c0, live ? (K - k) * p.lda - c0 : 0);
+    }
+    if (LB == KC) {
+      const int64_t r0 = (int64_t)c.n * BN;
+      rb = ls_rsrc(B + r0 * p.ldb + k * ESZ, live && k < K ? min((int64_t)BN, N - r0) * p.ldb - k * ESZ : 0);
+    } else {
+      const int64_t c0 = (int64_t)c.n * BN * ESZ;
+      rb = ls_rsrc(B + k * p.ldb + c0, live ? (K - k) * p.ldb - c0 : 0);
+    }
+  };
+  auto advance = [&]() {
+    if (++c_step < c.nk) return;
+    c_step = 0;
+    c_item += G;
+    if (c_item < total) c = item_of(c_item);
+  };
+  auto copy_a = [&](int j, uint32_t slot) {
+    ls_dma(ra, va[j], 0, slot + (uint32_t)wave * (BM * 32) + (uint32_t)j * 1024u);
+  };
+  auto copy_b = [&](int j, uint32_t slot) {
+    ls_dma(rb, vb[j], 0, slot + BM * 128 + (uint32_t)wave * (BN * 32) + (uint32_t)j * 1024u);
+  };
+
+  f32x16_t acc[MB][NB];
+  LsItem it = c;
+  int64_t item = first;
+  int slot = 0;
+#pragma unroll 1
+  for (;;) {
+    for (int s = 0; s < it.nk; ++s) {
+      // Simple form: copy a step, wait, multiply.
+      bases();
+      const uint32_t sl = lds0 + (uint32_t)slot * SLOT;
+#pragma unroll
+      for (int j = 0; j < OA::NDMA; ++j) copy_a(j, sl);
+#pragma unroll
+      for (int j = 0; j < OB::NDMA; ++j) copy_b(j, sl);
+      advance();
+      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      const uint8_t* base = lds + slot * SLOT;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        u32x4_t a[MB], b[NB];
+#pragma unroll
+        for (int i = 0; i < MB; ++i) a[i] = OA::frag(base, fa, i, u);
+#pragma unroll
+        for (int i = 0; i < NB; ++i) b[i] = OB::frag(base, fb, i, u);
+        if (s == 0 && u == 0) {
+#pragma unroll
+          for (int i = 0; i < MB; ++i)
+#pragma unroll
+            for (int j = 0; j < NB; ++j) ls_mfma<F32, true>(acc[i][j], a[i], b[j]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < MB; ++i)
+#pragma unroll
+            for (int j = 0; j < NB; ++j) ls_mfma<F32, false>(acc[i][j], a[i], b[j]);
+        }
+      }
+      slot ^= 1;
+    }
+    ls_drain();
+
+    // acc[i][j][q] of lane l: m = 32 i + 8 (q / 4) + 4 (l / 32) + q % 4 of the wave's rows, n = 32 j + l % 32.
+    const int64_t mw = (int64_t)it.m * BM + wm * (BM / 2), nw = (int64_t)it.n * BN + wn * (BN / 2);
+    const int lh = lane >> 5;
+    const int mleft = (int)min((int64_t)(BM / 2), p.m_rows - mw);  // rows of the wave that exist (may be <= 0)
+#pragma unroll
+    for (int j = 0; j < NB; ++j) {
+      const int64_t n = nw + 32 * j + (lane & 31);
+      const bool n_ok = n < N;
+      if constexpr (EPI == EPI_LSE) {
+        const int rel = n_ok ? p.tgt[n] - (int)mw : -1;
+        float mx = -__builtin_inff();
+#pragma unroll
+        for (int i = 0; i < MB; ++i)
+#pragma unroll
+          for (int q = 0; q < 16; ++q) {
+            const int r = 32 * i + 8 * (q >> 2) + 4 * lh + (q & 3);
+            if (r < mleft) mx = fmaxf(mx, acc[i][j][q]);
+          }
+        mx = fmaxf(mx, __shfl_xor(mx, 32));
+        const float ref = mx == -__builtin_inff() ? 0.0f : mx;
+        float sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < MB; ++i)
+#pragma unroll
+          for (int q = 0; q < 16; ++q) {
+            const int r = 32 * i + 8 * (q >> 2) + 4 * lh + (q & 3);
+            if (r < mleft) sum += __builtin_amdgcn_exp2f((acc[i][j][q] - ref) * LOG2E);
+          }
+        sum += __shfl_xor(sum, 32);
+        if (n_ok && lh == 0) p.part[((int64_t)it.m * 2 + wm) * p.T + n] = make_float2(mx, sum);
+#pragma unroll
+        for (int i = 0; i < MB; ++i) {
+          if (__any((rel >> 5) == i)) {
+#pragma unroll
+            for (int q = 0; q < 16; ++q)
+              if (rel == 32 * i + 8 * (q >> 2) + 4 * lh + (q & 3) && rel < mleft) p.zt[n] = acc[i][j][q];
+          }
+        }
+      } else if constexpr (EPI == EPI_S) {
+        if (!n_ok) continue;
+        const int64_t row = p.rows[n];
+        const float lse = p.lse[row];
+        const float g = p.g_row != nullptr ? p.g_row[row] : 1.0f;
+        const int rel = p.tgt[n] - (int)p.v0 - (int)mw;
+#pragma unroll
+        for (int i = 0; i < MB; ++i)
+#pragma unroll
+          for (int q4 = 0; q4 < 4; ++q4) {
+            const int r0 = 32 * i + 8 * q4 + 4 * lh;
+            float f[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              f[q] = __builtin_amdgcn_exp2f((acc[i][j][4 * q4 + q] - lse) * LOG2E);
+              if (rel == r0 + q) f[q] -= 1.0f;
+              f[q] = r0 + q < mleft ? f[q] * g : 0.0f;
+            }
+            const int64_t at = n * p.ldo + mw + r0;
+            if constexpr (F32)
+              *reinterpret_cast<f32x4_t*>(static_cast<float*>(p.out) + at) = (f32x4_t){f[0], f[1], f[2], f[3]};
+            else
+              *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + at) =
+                  make_uint2(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]));
+          }
+      } else {
+        if (!n_ok) continue;
+        float scale = 1.0f;
+        if (EPI == EPI_OUT) {
+          if (p.g_scale != nullptr) scale *= *p.g_scale;
+          if (p.r_scale != nullptr) scale *= *p.r_scale;
+        }
+        const int64_t row = EPI == EPI_OUT && p.scatter ? (int64_t)p.rows[n]
+                                                        : (EPI == EPI_ACC ? (int64_t)it.part * p.N + n : n);
+#pragma unroll
+        for (int i = 0; i < MB; ++i)
+#pragma unroll
+          for (int q4 = 0; q4 < 4; ++q4) {
+            const int r0 = 32 * i + 8 * q4 + 4 * lh;
+            if (r0 >= mleft) continue;  // M is a multiple of 64
+            f32x4_t f;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) f[q] = acc[i][j][4 * q4 + q] * scale;
+            const int64_t at = row * p.ldo + mw + r0;
+            if constexpr (EPI == EPI_ACC) {
+              f32x4_t* o = reinterpret_cast<f32x4_t*>(static_cast<float*>(p.out) + at);
+              if (p.add) f += *o;
+              *o = f;
+            } else if (p.out_f32) {
+              *reinterpret_cast<f32x4_t*>(static_cast<float*>(p.out) + at) = f;
+            } else {
+              *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + at) =
+                  make_uint2(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]));
+            }
+          }
+      }
+    }
+    item += G;
+    if (item >= total) break;
+    it = item_of(item);
+  }
+}
+
+// Partition of the rows: rows[0 .. n-1] those that count, ascending, rows[n .. T-1] the ignored ones, *count = n, tgt[i]
+// the target of rows[i] (-1: outside the vocabulary). With `keep` (no copy follows) every row stays where it is and an
+// ignored one gets target -2. One block; ballots give a row's place.
+template <typename IdxT>
+__global__ __launch_bounds__(1024) void ls_rows_kernel(const IdxT* __restrict__ targets, int64_t ignore, int64_t T, int V,
+                                                       bool keep, int32_t* __restrict__ rows, int32_t* __restrict__ tgt,
+                                                       int32_t* __restrict__ count) {
+  __shared__ int waves[2][16];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  int64_t kept = 0;  // rows that count, so far
+  int buf = 0;
+  for (int64_t t0 = 0; t0 < T; t0 += 1024, buf ^= 1) {
+    const int64_t t = t0 + tid;
+    const int64_t v = t < T ? (int64_t)targets[t] : ignore;
+    const bool in = t < T && v != ignore;
+    const int32_t place = v >= 0 && v < V ? (int32_t)v : -1;
+    const uint64_t mask = ballot64(in);
+    if (lane == 0) waves[buf][wave] = __popcll(mask);
+    __syncthreads();
+    int before = 0, all = 0;
+#pragma unroll
+    for (int w = 0; w < 16; ++w) {
+      const int c = waves[buf][w];
+      before += w < wave ? c : 0;
+      all += c;
+    }
+    before += __popcll(mask & ((1ull << lane) - 1));
+    if (t < T) {
+      if (keep) {
+        rows[t] = (int32_t)t;
+        tgt[t] = in ? place : -2;
+      } else if (in) {
+        rows[kept + before] = (int32_t)t;
+        tgt[kept + before] = place;
+      } else {
+        rows[T - 1 - (t - (kept + before))] = (int32_t)t;  // from the end
+      }
+    }
+    kept += all;
+  }
+  if (tid == 0) *count = (int32_t)(keep ? T : kept);
+}
+
+// xc[i] = x[rows[i]] for the rows that count, unless all do; zero[rows[i]] = 0 for the others (zero may be NULL). One wave per
+// row, rows of `bytes` bytes.
+__global__ __launch_bounds__(256) void ls_gather_kernel(const uint8_t* __restrict__ x, const int32_t* __restrict__ rows,
+                                                        const int32_t* __restrict__ count, uint8_t* __restrict__ xc,
+                                                        uint8_t* __restrict__ zero, int64_t T, int bytes) {
+  const int64_t n = load_uniform(count);
+  if (n >= T) return;
+  const int64_t i = (int64_t)blockIdx.x * 4 + (int)uniform(threadIdx.x >> 6);
+  if (i >= T || (i >= n && zero == nullptr)) return;
+  const int64_t r = rows[i];
+  for (int c = 16 * (threadIdx.x & 63); c < bytes; c += 1024) {
+    if (i < n) st16(xc + i * bytes + c, ld16(x + r * bytes + c));
+    else st16(zero + r * bytes + c, (u32x4_t){0u, 0u, 0u, 0u});
+  }
+}
+
+__device__ __forceinline__ void lse_join(float& m, float& s, float m2, float s2) {
+  const float top = fmaxf(m, m2);
+  const float ref = top == -__builtin_inff() ? 0.0f : top;
+  s = s * __builtin_amdgcn_exp2f((m - ref) * LOG2E) + s2 * __builtin_amdgcn_exp2f((m2 - ref) * LOG2E);
+  m = top;
+}
+
+// lse and loss of 64 rows per block from their partial maxima and sums (16 waves share the entries), the block's sum of losses
+// and its count. Rows that do not count get loss 0.
+__global__ __launch_bounds__(1024) void ls_finish_kernel(const float2* __restrict__ part, int entries,
+                                                         const float* __restrict__ zt, const int32_t* __restrict__ tgt,
+                                                         const int32_t* __restrict__ rows,
+                                                         const int32_t* __restrict__ count, int64_t T,
+                                                         float* __restrict__ loss, float* __restrict__ lse,
+                                                         double* __restrict__ block_sum, int32_t* __restrict__ block_n) {
+  __shared__ float2 red[16][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t n = load_uniform(count), i = (int64_t)blockIdx.x * 64 + lane;
+  float m = -__builtin_inff(), s = 0.0f;
+  if (i < n) {
+#pragma unroll 4
+    for (int e = wave; e < entries; e += 16) {
+      const float2 v = part[(int64_t)e * T + i];
+      lse_join(m, s, v.x, v.y);
+    }
+  }
+  red[wave][lane] = make_float2(m, s);
+  __syncthreads();
+  if (wave != 0) return;
+#pragma unroll
+  for (int w = 1; w < 16; ++w) lse_join(m, s, red[w][lane].x, red[w][lane].y);
+  double sum = 0.0;
+  int c = 0;
+  if (i < T) {
+    const int64_t r = rows[i];
+    const int tg = i < n ? tgt[i] : -2;
+    float l = 0.0f, z = 0.0f;
+    if (tg != -2) {
+      z = tg < 0 ? __builtin_nanf("") : m + logf(s);  // a target outside the vocabulary shows as NaN
+      l = tg < 0 ? z : z - zt[i];
+      sum = (double)l;
+      c = 1;
+    }
+    loss[r] = l;
+    lse[r] = z;
+  }
+#pragma unroll
+  for (int o = 32; o; o >>= 1) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, sum);
+    const uint32_t lo = __shfl_xor((int)(uint32_t)u, o), hi = __shfl_xor((int)(uint32_t)(u >> 32), o);
+    sum += __builtin_bit_cast(double, ((uint64_t)hi << 32) | lo);
+    c += __shfl_xor(c, o);
+  }
+  if (lane == 0) {
+    block_sum[blockIdx.x] = sum;
+    block_n[blockIdx.x] = c;
+  }
+}
+
+// reduced[0] = the sum of the losses (mean: over the rows that count; 0 where none does), reduced[1] = the factor of every
+// row's gradient.
+__global__ __launch_bounds__(256) void ls_reduce_kernel(const double* __restrict__ block_sum,
+                                                        const int32_t* __restrict__ block_n, int blocks, bool mean,
+                                                        float* __restrict__ reduced) {
+  __shared__ double sums[256];
+  __shared__ int64_t ns[256];
+  double s = 0.0;
+  int64_t n = 0;
+  for (int b = threadIdx.x; b < blocks; b += 256) {
+    s += block_sum[b];
+    n += block_n[b];
+  }
+  sums[threadIdx.x] = s;
+  ns[threadIdx.x] = n;
+  __syncthreads();
+  for (int o = 128; o; o >>= 1) {
+    if ((int)threadIdx.x < o) {
+      sums[threadIdx.x] += sums[threadIdx.x + o];
+      ns[threadIdx.x] += ns[threadIdx.x + o];
+    }
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) {
+    const double d = mean ? (double)(ns[0] > 0 ? ns[0] : 1) : 1.0;
+    reduced[0] = (float)(sums[0] / d);
+    reduced[1] = (float)(1.0 / d);
+  }
+}
+
+// out[row] = scale * sum over the parts of acc [parts, N, M], row = rows[i] (rows NULL: i), i < min(N, *count).
+template <typename E>
+__global__ __launch_bounds__(256) void ls_join_kernel(const float* __restrict__ acc, int parts, int64_t N, int M,
+                                                      const int32_t* __restrict__ count,
+                                                      const int32_t* __restrict__ rows,
+                                                      const float* __restrict__ g_scale,
+                                                      const float* __restrict__ r_scale, E* __restrict__ out) {
+  const int64_t n = count != nullptr ? min(N, (int64_t)load_uniform(count)) : N;
+  const int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x, per = M / 4;
+  const int64_t i = q / per;
+  if (i >= n) return;
+  const int c = (int)(q - i * per) * 4;
+  f32x4_t s = *reinterpret_cast<const f32x4_t*>(acc + i * M + c);
+  for (int p = 1; p < parts; ++p) s += *reinterpret_cast<const f32x4_t*>(acc + ((int64_t)p * N + i) * M + c);
+  float scale = 1.0f;
+  if (g_scale != nullptr) scale *= *g_scale;
+  if (r_scale != nullptr) scale *= *r_scale;
+  s *= scale;
+  E* o = out + (rows != nullptr ? (int64_t)rows[i] : i) * M + c;
+  if constexpr (sizeof(E) == 4) *reinterpret_cast<f32x4_t*>(o) = s;
+  else *reinterpret_cast<uint2*>(o) = make_uint2(pack_bf16x2(s[0], s[1]), pack_bf16x2(s[2], s[3]));
+}
+
+template <bool F32, int BM, int BN, int LA, int LB, int EPI>
+hipError_t ls_gemm(const LsParams& p, hipStream_t st) {
+  const int64_t items = ((p.M + BM - 1) / BM) * ((p.N + BN - 1) / BN) * p.parts;
+  const int64_t most = (int64_t)device_cus() * (BM == 256 ? 1 : 2);
+  const unsigned grid = (unsigned)(items < most ? items : most);
+  if (grid == 0) return hipSuccess;
+  hipLaunchKernelGGL((ls_gemm_kernel<F32, BM, BN, LA, LB, EPI>), dim3(grid), dim3(256), 0, st, p);
+  return hipGetLastError();
+}
+
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// Tiles of 256 x 256 where they fill at least half the CUs, else of 128 x 128.
+bool big_tiles(int64_t M, int64_t N) { return ceil_div(M, 256) * ceil_div(N, 256) * 2 >= device_cus(); }
+
+// Runs that K's steps are split into, so that the tiles fill the CUs.
+int split_parts(int64_t M, int64_t N, int64_t steps) {
+  const bool big = big_tiles(M, N);
+  const int64_t tiles = ceil_div(M, big ? 256 : 128) * ceil_div(N, big ? 256 : 128);
+  const int64_t slots = (int64_t)device_cus() * (big ? 1 : 2);
+  int best = 1;
+  double cost = 0.0;
+  for (int p = 1; p <= 16 && p <= steps; ++p) {
+    const double c = (double)ceil_div(tiles * p, slots) * ((double)ceil_div(steps, p) + 4.0) + (p > 1 ? 2.0 * p : 0.0);
+    if (p == 1 || c < cost) {
+      best = p;
+      cost = c;
+    }
+  }
+  return best;
+}
+
+size_t up(size_t v) { return (v + 255) / 256 * 256; }
+
+struct Layout {
+  size_t rows, tgt, count, xc, part, zt, bsum, bn, s, acc_x, acc_w, end;
+  int entries;             // of the forward's partial sums
+  int64_t piece;           // vocabulary rows of a piece (multiple of 256)
+  int pieces, parts_x, parts_w;
+  bool gather;
+};
+
+constexpr int64_t PIECE_BYTES = (int64_t)256 << 20;
+
+Layout layout(int64_t T, int h, int V, bool f32, bool fwd, bool need_x, bool need_w) {
+  Layout l = {};
+  const size_t esz = f32 ? 4 : 2;
+  size_t off = 0;
+  auto take = [&](size_t n) {
+    const size_t at = off;
+    off = up(off + n);
+    return at;
+  };
+  l.rows = take(4 * T);
+  l.tgt = take(4 * T);
+  l.count = take(4);
+  l.gather = !fwd || T > 256;
+  l.xc = take(l.gather ? esz * T * h : 0);
+  if (fwd) {
+    l.entries = (int)(2 * ceil_div(V, big_tiles(V, T) ? 256 : 128));
+    l.part = take(8 * (size_t)l.entries * T);
+    l.zt = take(4 * T);
+    l.bsum = take(8 * ceil_div(T, 64));
+    l.bn = take(4 * ceil_div(T, 64));
+  } else {
+    const int64_t vt = ceil_div(V, 256);
+    int64_t most = PIECE_BYTES / ((int64_t)esz * T) / 256;
+    if (most < 1) most = 1;
+    l.pieces = (int)ceil_div(vt, most);
+    const int64_t pt = ceil_div(vt, l.pieces);
+    l.pieces = (int)ceil_div(vt, pt);
+    l.piece = pt * 256;
+    l.s = take(esz * (size_t)T * l.piece);
+    l.parts_x = split_parts(h, T, l.piece / (f32 ? 32 : 64));
+    l.parts_w = split_parts(h, l.piece < V ? l.piece : V, ceil_div(T, f32 ? 32 : 64));
+    l.acc_x = take(need_x && (l.parts_x > 1 || l.pieces > 1) ? 4 * (size_t)l.parts_x * T * h : 0);
+    l.acc_w = take(need_w && l.parts_w > 1 ? 4 * (size_t)l.parts_w * l.piece * h : 0);
+  }
+  l.end = off;
+  return l;
+}
+
+template <typename P>
+P* at(void* base, size_t off) {
+  return reinterpret_cast<P*>(static_cast<char*>(base) + off);
+}
+
+#define LS_TRY(e)                       \
+  do {                                  \
+    const hipError_t e_ = (e);          \
+    if (e_ != hipSuccess) return e_;    \
+  } while (0)
+
+hipError_t ls_rows(const void* targets, bool idx64, int64_t ignore, int64_t T, int V, bool keep, int32_t* rows,
+                   int32_t* tgt, int32_t* count, hipStream_t st) {
+  if (idx64)
+    hipLaunchKernelGGL(ls_rows_kernel<int64_t>, dim3(1), dim3(1024), 0, st, (const int64_t*)targets, ignore, T, V, keep,
+                       rows, tgt, count);
+  else
+    hipLaunchKernelGGL(ls_rows_kernel<int32_t>, dim3(1), dim3(1024), 0, st, (const int32_t*)targets, ignore, T, V, keep,
+                       rows, tgt, count);
+  return hipGetLastError();
+}
+
+hipError_t ls_gather(const void* x, const int32_t* rows, const int32_t* count, void* xc, void* zero, int64_t T,
+                     int bytes, hipStream_t st) {
+  hipLaunchKernelGGL(ls_gather_kernel, dim3((unsigned)ceil_div(T, 4)), dim3(256), 0, st, (const uint8_t*)x, rows, count,
+                     (uint8_t*)xc, (uint8_t*)zero, T, bytes);
+  return hipGetLastError();
+}
+
+template <bool F32, int LA, int LB, int EPI>
+hipError_t ls_gemm_any(const LsParams& p, bool big, hipStream_t st) {
+  return big ? ls_gemm<F32, 256, 256, LA, LB, EPI>(p, st) : ls_gemm<F32, 128, 128, LA, LB, EPI>(p, st);
+}
+
+template <bool F32>
+hipError_t ce_forward(const void* x, const void* w, const void* targets, bool idx64, int64_t ignore, float* loss,
+                      float* lse, float* reduced, bool mean, int64_t T, int h, int V, void* ws, hipStream_t st) {
+  const Layout l = layout(T, h, V, F32, true, false, false);
+  int32_t* rows = at<int32_t>(ws, l.rows);
+  int32_t* tgt = at<int32_t>(ws, l.tgt);
+  int32_t* count = at<int32_t>(ws, l.count);
+  const int64_t rb = (int64_t)h * (F32 ? 4 : 2);
+  LS_TRY(ls_rows(targets, idx64, ignore, T, V, !l.gather, rows, tgt, count, st));
+  if (l.gather) LS_TRY(ls_gather(x, rows, count, at<void>(ws, l.xc), nullptr, T, (int)rb, st));
+  LsParams p = {};
+  p.A = static_cast<const uint8_t*>(w);
+  p.B = l.gather ? at<const uint8_t>(ws, l.xc) : static_cast<const uint8_t*>(x);
+  p.alt = static_cast<const uint8_t*>(x);
+  p.lda = p.ldb = rb;
+  p.M = p.m_rows = V;
+  p.N = p.T = T;
+  p.K = h;
+  p.count = count;
+  p.parts = 1;
+  p.part = at<float2>(ws, l.part);
+  p.tgt = tgt;
+  p.zt = at<float>(ws, l.zt);
+  LS_TRY((ls_gemm_any<F32, KC, KC, EPI_LSE>(p, big_tiles(V, T), st)));
+  const int blocks = (int)ceil_div(T, 64);
+  hipLaunchKernelGGL(ls_finish_kernel, dim3(blocks), dim3(1024), 0, st, p.part, l.entries, p.zt, tgt, rows, count, T,
+                     loss, lse, at<double>(ws, l.bsum), at<int32_t>(ws, l.bn));
+  LS_TRY(hipGetLastError());
+  if (reduced != nullptr) {
+    hipLaunchKernelGGL(ls_reduce_kernel, dim3(1), dim3(256), 0, st, at<double>(ws, l.bsum), at<int32_t>(ws, l.bn),
+                       blocks, mean, reduced);
+    LS_TRY(hipGetLastError());
+  }
+  return hipSuccess;
+}
+
+template <bool F32>
+hipError_t ce_backward(const float* g, bool g_rows, const float* r_scale, const void* x, const void* w,
+                       const void* targets, bool idx64, int64_t ignore, const float* lse, void* dx, void* dw, int64_t T,
+                       int h, int V, void* ws, hipStream_t st) {
+  using E = typename std::conditional<F32, float, uint16_t>::type;
+  const Layout l = layout(T, h, V, F32, false, dx != nullptr, dw != nullptr);
+  int32_t* rows = at<int32_t>(ws, l.rows);
+  int32_t* tgt = at<int32_t>(ws, l.tgt);
+  int32_t* count = at<int32_t>(ws, l.count);
+  const int64_t rb = (int64_t)h * (F32 ? 4 : 2);
+  const int64_t esz = F32 ? 4 : 2;
+  LS_TRY(ls_rows(targets, idx64, ignore, T, V, false, rows, tgt, count, st));
+  LS_TRY(ls_gather(x, rows, count, at<void>(ws, l.xc), dx, T, (int)rb, st));
+  const uint8_t* xc = at<const uint8_t>(ws, l.xc);
+  const float* scale = g_rows ? nullptr : g;
+  for (int i = 0; i < l.pieces; ++i) {
+    const int64_t v0 = (int64_t)i * l.piece, n = V - v0 < l.piece ? V - v0 : l.piece;
+    const int64_t pitch = ceil_div(n, 256) * 256;
+    const uint8_t* wp = static_cast<const uint8_t*>(w) + v0 * rb;
+    LsParams p = {};
+    p.T = T;
+    p.count = count;
+    p.rows = rows;
+    p.parts = 1;
+    // s [T, pitch]
+    p.A = wp;
+    p.B = xc;
+    p.alt = static_cast<const uint8_t*>(x);
+    p.lda = p.ldb = rb;
+    p.N = T;
+    p.K = h;
+    p.v0 = v0;
+    p.tgt = tgt;
+    p.lse = lse;
+    p.g_row = g_rows ? g : nullptr;
+    p.out = at<void>(ws, l.s);
+    p.ldo = pitch;
+    p.M = pitch;  // whole tiles: the columns behind the piece become zeros
+    p.m_rows = n;
+    LS_TRY((ls_gemm_any<F32, KC, KC, EPI_S>(p, big_tiles(n, T), st)));
+    if (dx != nullptr) {
+      LsParams q = {};
+      q.A = wp;
+      q.B = at<const uint8_t>(ws, l.s);
+      q.lda = rb;
+      q.ldb = pitch * esz;
+      q.M = q.m_rows = h;
+      q.N = T;
+      q.K = n;
+      q.T = T;
+      q.count = count;
+      q.rows = rows;
+      q.parts = l.parts_x;
+      q.ldo = h;
+      const bool big = big_tiles(h, T);
+      if (l.parts_x > 1 || l.pieces > 1) {
+        q.out = at<void>(ws, l.acc_x);
+        q.add = i > 0;
+        LS_TRY((ls_gemm_any<F32, KS, KC, EPI_ACC>(q, big, st)));
+      } else {
+        q.out = dx;
+        q.out_f32 = F32;
+        q.scatter = true;
+        q.g_scale = scale;
+        q.r_scale = r_scale;
+        LS_TRY((ls_gemm_any<F32, KS, KC, EPI_OUT>(q, big, st)));
+      }
+    }
+    if (dw != nullptr) {
+      LsParams q = {};
+      q.A = xc;
+      q.alt = static_cast<const uint8_t*>(x);
+      q.B = at<const uint8_t>(ws, l.s);
+      q.lda = rb;
+      q.ldb = pitch * esz;
+      q.M = q.m_rows = h;
+      q.N = n;
+      q.K = T;
+      q.T = T;
+      q.count = count;
+      q.parts = l.parts_w;
+      q.ldo = h;
+      E* out = static_cast<E*>(dw) + v0 * h;
+      const bool big = big_tiles(h, l.piece < V ? l.piece : V);
+      if (l.parts_w > 1) {
+        q.out = at<void>(ws, l.acc_w);
+        LS_TRY((ls_gemm_any<F32, KS, KS, EPI_ACC>(q, big, st)));
+        hipLaunchKernelGGL(ls_join_kernel<E>, dim3((unsigned)ceil_div(n * (h / 4), 256)), dim3(256), 0, st,
+                           at<float>(ws, l.acc_w), l.parts_w, n, h, nullptr, nullptr, scale, r_scale, out);
+        LS_TRY(hipGetLastError());
+      } else {
+        q.out = out;
+        q.out_f32 = F32;
+        q.g_scale = scale;
+        q.r_scale = r_scale;
+        LS_TRY((ls_gemm_any<F32, KS, KS, EPI_OUT>(q, big, st)));
+      }
+    }
+  }
+  if (dx != nullptr && (l.parts_x > 1 || l.pieces > 1)) {
+    hipLaunchKernelGGL(ls_join_kernel<E>, dim3((unsigned)ceil_div(T * (h / 4), 256)), dim3(256), 0, st,
+                       at<float>(ws, l.acc_x), l.parts_x, T, h, count, rows, scale, r_scale, static_cast<E*>(dx));
+    LS_TRY(hipGetLastError());
+  }
+  return hipSuccess;
+}
+
+}  // namespace
+
+size_t linear_ce_workspace(int64_t T, int h, int V, bool f32, bool forward, bool need_x, bool need_w) {
+  return layout(T, h, V, f32, forward, need_x, need_w).end;
+}
+
+hipError_t launch_linear_ce_forward(const void* x, const void* w, const void* targets, bool idx64, int64_t ignore,
+                                    float* loss, float* lse, float* reduced, bool mean, int64_t T, int h, int V,
+                                    void* ws, bool f32, hipStream_t st) {
+  return f32 ? ce_forward<true>(x, w, targets, idx64, ignore, loss, lse, reduced, mean, T, h, V, ws, st)
+             : ce_forward<false>(x, w, targets, idx64, ignore, loss, lse, reduced, mean, T, h, V, ws, st);
+}
+
+hipError_t launch_linear_ce_backward(const float* g, bool g_rows, const float* r_scale, const void* x, const void* w,
+                                     const void* targets, bool idx64, int64_t ignore, const float* lse, void* dx,
+                                     void* dw, int64_t T, int h, int V, void* ws, bool f32, hipStream_t st) {
+  return f32 ? ce_backward<true>(g, g_rows, r_scale, x, w, targets, idx64, ignore, lse, dx, dw, T, h, V, ws, st)
+             : ce_backward<false>(g, g_rows, r_scale, x, w, targets, idx64, ignore, lse, dx, dw, T, h, V, ws, st);
+}
+
+}  // namespace q38

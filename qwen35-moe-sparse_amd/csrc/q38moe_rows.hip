@@ -1,0 +1,232 @@
+// Tokens to expert-sorted rows and back (differentiable experts of the caller's own between the two), on the
+// permutation of q38moe_permute.hip: pair p = t*k + j of token t goes to row inv[p]; pairs whose index lies outside
+// [0, E) have no row, and the rows behind the last filled one are theirs to be zero.
+//
+//   spread:   dst[inv[p]] = src[t] (* w[p]),  dst[r] = 0 for r >= filled,  dw[p] = <src[t], y[inv[p]]>
+//   collect:  out[t] = sum_j src[inv[p]] (* w[p])
+//
+// spread without w is the dispatch, collect without w its gradient; collect with w is the combine, spread with
+// w and y its gradients. Products and sums are fp32, each output is rounded once. Both run one wave per token: the
+// token's k rows of a column chunk are loaded before any is used, so k 16-byte loads per lane are in flight, and the
+// token's own row moves once. Both are bound by memory.
+#include <type_traits>
+
+#include "q38moe_common.h"
+#include "q38moe_kernels.h"
+
+namespace q38 {
+namespace {
+
+template <typename E>
+constexpr int VEC = 16 / sizeof(E);  // elements of a 16-byte load
+
+template <typename E>
+__device__ __forceinline__ void unpack16(u32x4_t v, float (&f)[VEC<E>]) {
+  if constexpr (std::is_same<E, float>::value) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[i] = __uint_as_float(v[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) unpack_bf16x2(v[i], f[2 * i], f[2 * i + 1]);
+  }
+}
+
+template <typename E>
+__device__ __forceinline__ u32x4_t pack16(const float (&f)[VEC<E>]) {
+  u32x4_t v;
+  if constexpr (std::is_same<E, float>::value) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = __float_as_uint(f[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = pack_bf16x2(f[2 * i], f[2 * i + 1]);
+  }
+  return v;
+}
+
+__device__ __forceinline__ float weight_of(const void* w, bool f32, int64_t p) {
+  return f32 ? static_cast<const float*>(w)[p] : bf16_to_f32(static_cast<const uint16_t*>(w)[p]);
+}
+
+__device__ __forceinline__ float wave_add(float v) {
+#pragma unroll
+  for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
+  return v;
+}
+
+// The rows of token t's pairs (-1: none), wave-uniform.
+template <typename IdxT, int KT>
+__device__ __forceinline__ void pair_rows(const IdxT* idx, const int32_t* inv, int64_t t, int E, int64_t (&row)[KT]) {
+#pragma unroll
+  for (int j = 0; j < KT; ++j) {
+    const int64_t e = (int64_t)idx[t * KT + j];
+    const bool ok = __builtin_amdgcn_readfirstlane((int)(e >= 0 && e < E)) != 0;
+    row[j] = ok ? (int64_t)__builtin_amdgcn_readfirstlane(inv[t * KT + j]) : (int64_t)-1;
+  }
+}
+
+template <typename E, typename IdxT, int KT>
+__global__ __launch_bounds__(256) void spread_kernel(const E* __restrict__ src, const void* __restrict__ w, bool w_f32,
+                                                     const E* __restrict__ y, const IdxT* __restrict__ idx,
+                                                     const int32_t* __restrict__ inv,
+                                                     const int32_t* __restrict__ starts,
+                                                     const int32_t* __restrict__ counts, E* __restrict__ dst,
+                                                     void* __restrict__ dw, int64_t T, int h, int NE) {
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63;
+  const int64_t t = (int64_t)blockIdx.x * 4 + wave;
+  if (t >= T) return;
+  int64_t row[KT];
+  pair_rows<IdxT, KT>(idx, inv, t, NE, row);
+  float s[KT], acc[KT];
+#pragma unroll
+  for (int j = 0; j < KT; ++j) {
+    s[j] = w != nullptr ? weight_of(w, w_f32, t * KT + j) : 1.0f;
+    acc[j] = 0.0f;
+  }
+  for (int c = lane * VEC<E>; c < h; c += 64 * VEC<E>) {
+    const u32x4_t a = ld16(src + t * h + c);
+    float f[VEC<E>];
+    unpack16<E>(a, f);
+    if (y != nullptr) {
+      u32x4_t b[KT];
+#pragma unroll
+      for (int j = 0; j < KT; ++j) b[j] = row[j] >= 0 ? ld16(y + row[j] * h + c) : (u32x4_t){0u, 0u, 0u, 0u};
+#pragma unroll
+      for (int j = 0; j < KT; ++j) {
+        if (row[j] < 0) continue;
+        float g[VEC<E>];
+        unpack16<E>(b[j], g);
+#pragma unroll
+        for (int i = 0; i < VEC<E>; ++i) acc[j] = fmaf(f[i], g[i], acc[j]);
+      }
+    }
+    if (dst != nullptr) {
+#pragma unroll
+      for (int j = 0; j < KT; ++j) {
+        if (row[j] < 0) continue;
+        u32x4_t v = a;
+        if (w != nullptr) {
+          float g[VEC<E>];
+#pragma unroll
+          for (int i = 0; i < VEC<E>; ++i) g[i] = f[i] * s[j];
+          v = pack16<E>(g);
+        }
+        st16(dst + row[j] * h + c, v);
+      }
+    }
+  }
+  if (dw != nullptr) {
+#pragma unroll
+    for (int j = 0; j < KT; ++j) {
+      const float r = wave_add(acc[j]);
+      if (lane == 0) {
+        if (w_f32) static_cast<float*>(dw)[t * KT + j] = r;
+        else static_cast<uint16_t*>(dw)[t * KT + j] = (uint16_t)f32_to_bf16_rne(r);
+      }
+    }
+  }
+  if (dst != nullptr) {  // of the T*k rows, wave t looks after the zeros among rows t*k .. t*k + k - 1
+    const int64_t filled = (int64_t)starts[NE - 1] + counts[NE - 1];
+#pragma unroll
+    for (int j = 0; j < KT; ++j) {
+      const int64_t r = t * KT + j;
+      if (r < filled) continue;
+      for (int c = lane * VEC<E>; c < h; c += 64 * VEC<E>) st16(dst + r * h + c, (u32x4_t){0u, 0u, 0u, 0u});
+    }
+  }
+}
+
+template <typename E, typename IdxT, int KT>
+__global__ __launch_bounds__(256) void collect_kernel(const E* __restrict__ src, const void* __restrict__ w, bool w_f32,
+                                                      const IdxT* __restrict__ idx, const int32_t* __restrict__ inv,
+                                                      E* __restrict__ out, int64_t T, int h, int NE) {
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63;
+  const int64_t t = (int64_t)blockIdx.x * 4 + wave;
+  if (t >= T) return;
+  int64_t row[KT];
+  pair_rows<IdxT, KT>(idx, inv, t, NE, row);
+  float s[KT];
+#pragma unroll
+  for (int j = 0; j < KT; ++j) s[j] = w != nullptr ? weight_of(w, w_f32, t * KT + j) : 1.0f;
+  for (int c = lane * VEC<E>; c < h; c += 64 * VEC<E>) {
+    u32x4_t b[KT];
+#pragma unroll
+    for (int j = 0; j < KT; ++j) b[j] = row[j] >= 0 ? ld16(src + row[j] * h + c) : (u32x4_t){0u, 0u, 0u, 0u};
+    float a[VEC<E>];
+#pragma unroll
+    for (int i = 0; i < VEC<E>; ++i) a[i] = 0.0f;
+#pragma unroll
+    for (int j = 0; j < KT; ++j) {
+      if (row[j] < 0) continue;  // its weight may be anything
+      float g[VEC<E>];
+      unpack16<E>(b[j], g);
+#pragma unroll
+      for (int i = 0; i < VEC<E>; ++i) a[i] = fmaf(g[i], s[j], a[i]);
+    }
+    st16(out + t * h + c, pack16<E>(a));
+  }
+}
+
+template <typename E, typename IdxT>
+hipError_t spread_k(const void* src, const void* w, bool w_f32, const void* y, const void* idx, const int32_t* inv,
+                    const int32_t* starts, const int32_t* counts, void* dst, void* dw, int64_t T, int h, int NE, int k,
+                    hipStream_t st) {
+  const dim3 grid((unsigned)((T + 3) / 4));
+#define Q38_SPREAD(KT)                                                                                              \
+  case KT:                                                                                                          \
+    hipLaunchKernelGGL((spread_kernel<E, IdxT, KT>), grid, dim3(256), 0, st, (const E*)src, w, w_f32, (const E*)y,  \
+                       (const IdxT*)idx, inv, starts, counts, (E*)dst, dw, T, h, NE);                               \
+    break;
+  switch (k) {
+    Q38_SPREAD(1) Q38_SPREAD(2) Q38_SPREAD(3) Q38_SPREAD(4) Q38_SPREAD(5) Q38_SPREAD(6) Q38_SPREAD(7) Q38_SPREAD(8)
+    default: return hipErrorInvalidValue;
+  }
+#undef Q38_SPREAD
+  return hipGetLastError();
+}
+
+template <typename E, typename IdxT>
+hipError_t collect_k(const void* src, const void* w, bool w_f32, const void* idx, const int32_t* inv, void* out,
+                     int64_t T, int h, int NE, int k, hipStream_t st) {
+  const dim3 grid((unsigned)((T + 3) / 4));
+#define Q38_COLLECT(KT)                                                                                             \
+  case KT:                                                                                                          \
+    hipLaunchKernelGGL((collect_kernel<E, IdxT, KT>), grid, dim3(256), 0, st, (const E*)src, w, w_f32,              \
+                       (const IdxT*)idx, inv, (E*)out, T, h, NE);                                                   \
+    break;
+  switch (k) {
+    Q38_COLLECT(1) Q38_COLLECT(2) Q38_COLLECT(3) Q38_COLLECT(4) Q38_COLLECT(5) Q38_COLLECT(6) Q38_COLLECT(7)
+    Q38_COLLECT(8)
+    default: return hipErrorInvalidValue;
+  }
+#undef Q38_COLLECT
+  return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t launch_spread_rows(const void* src, const void* w, bool w_f32, const void* y, const void* idx, bool idx64,
+                              const int32_t* inv, const int32_t* starts, const int32_t* counts, void* dst, void* dw,
+                              int64_t T, int h, int E, int k, bool bf16, hipStream_t st) {
+  if (T == 0) return hipSuccess;
+  if (bf16)
+    return idx64 ? spread_k<uint16_t, int64_t>(src, w, w_f32, y, idx, inv, starts, counts, dst, dw, T, h, E, k, st)
+                 : spread_k<uint16_t, int32_t>(src, w, w_f32, y, idx, inv, starts, counts, dst, dw, T, h, E, k, st);
+  return idx64 ? spread_k<float, int64_t>(src, w, w_f32, y, idx, inv, starts, counts, dst, dw, T, h, E, k, st)
+               : spread_k<float, int32_t>(src, w, w_f32, y, idx, inv, starts, counts, dst, dw, T, h, E, k, st);
+}
+
+hipError_t launch_collect_rows(const void* src, const void* w, bool w_f32, const void* idx, bool idx64,
+                               const int32_t* inv, void* out, int64_t T, int h, int E, int k, bool bf16,
+                               hipStream_t st) {
+  if (T == 0) return hipSuccess;
+  if (bf16)
+    return idx64 ? collect_k<uint16_t, int64_t>(src, w, w_f32, idx, inv, out, T, h, E, k, st)
+                 : collect_k<uint16_t, int32_t>(src, w, w_f32, idx, inv, out, T, h, E, k, st);
+  return idx64 ? collect_k<float, int64_t>(src, w, w_f32, idx, inv, out, T, h, E, k, st)
+               : collect_k<float, int32_t>(src, w, w_f32, idx, inv, out, T, h, E, k, st);
+}
+
+}  // namespace q38

@@ -1,5 +1,6 @@
 """Differentiable HIP MoE pieces: the routed experts (the training counterpart of
-``ops.experts_forward``), the router and the shared expert.
+``ops.experts_forward``), the router and the shared expert; and what a training step has around them: the
+head's loss (``linear_cross_entropy``) and the way to experts of the caller's own and back (``dispatch``, ``combine``).
 
 The reference's differentiable experts path is ``padded_batched_experts_forward``
 (q38/inference.py:358-384: gather, bmm gate/up, SiLU * up, bmm down, * top_k_weights, scatter-sum);
@@ -29,6 +30,7 @@ are int32/int64 as in the forward.
 """
 import torch
 from torch.autograd import forward_ad
+from torch.autograd.function import once_differentiable
 
 from . import ops
 
@@ -172,3 +174,102 @@ def shared_expert(x, w_gate, w_up, w_down):
     out = experts(x, idx, ones, w_gate_up, w_down.unsqueeze(0))
     # Under autocast the MLP's last nn.Linear returns the autocast dtype, whatever x's dtype.
     return out.to(torch.bfloat16) if _bf16_autocast() else out
+
+
+def _aligned(t):
+    """t contiguous and on a 16-byte boundary (a differentiable copy where it is not)."""
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+class HipLinearCE(torch.autograd.Function):
+    """Forward: maxima and sums of the logits' tiles; kept are the operands and the rows' log-sum-exp. Backward: the tiles again, in
+    pieces of the vocabulary (q38moe_linear_ce_forward, _backward)."""
+
+    @staticmethod
+    def forward(ctx, x, weight, targets, ignore_index, reduction):
+        loss, lse, reduced = ops.linear_ce_forward(x, weight, targets, ignore_index,
+                                                   None if reduction == "none" else reduction)
+        ctx.save_for_backward(x, weight, targets, lse, reduced)
+        ctx.ignore_index = ignore_index
+        return loss if reduced is None else reduced[0].clone()
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        x, weight, targets, lse, reduced = ctx.saved_tensors
+        need_x, need_w = ctx.needs_input_grad[:2]
+        dx, dw = ops.linear_ce_backward(g.contiguous(), x, weight, targets, lse, ctx.ignore_index,
+                                        None if reduced is None else reduced[1:], need_x, need_w)
+        return dx, dw, None, None, None
+
+
+def linear_cross_entropy(x, weight, targets, ignore_index=-100, reduction="mean"):
+    """``F.cross_entropy(F.linear(x, weight).float(), targets)`` with autograd and without the logits: x [..., h],
+    weight [V, h], targets of x's leading shape (int32 or int64); the loss is fp32. reduction "mean" (over the targets
+    that are not ignore_index), "sum" or "none". Gradients flow to x and weight; logits, maxima, sums and the loss are
+    fp32. x and weight share a type, bf16 or fp32 (any float types under bf16 autocast, which casts them as it casts F.linear's
+    operands). A batch whose targets are all ignored has loss 0 under every reduction, where F.cross_entropy's mean is NaN; a row
+    that is ignored may hold anything, NaN too. A target outside the vocabulary makes the loss NaN instead of ending
+    the process."""
+    if reduction not in ("mean", "sum", "none"):
+        raise ValueError(f"reduction must be 'mean', 'sum' or 'none', got {reduction!r}")
+    if tuple(targets.shape) != tuple(x.shape[:-1]):
+        raise ValueError(f"targets {tuple(targets.shape)} do not match x {tuple(x.shape)}")
+    if _bf16_autocast() and x.is_floating_point() and weight.is_floating_point():
+        x, weight = x.to(torch.bfloat16), weight.to(torch.bfloat16)
+    loss = HipLinearCE.apply(_aligned(x.reshape(-1, x.shape[-1])), _aligned(weight), targets.reshape(-1).contiguous(),
+                             ignore_index, reduction)
+    return loss.view(targets.shape) if reduction == "none" else loss
+
+
+class HipDispatch(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, plan):
+        ctx.plan = plan
+        return ops.spread_rows(x, plan)[0]
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, d_rows):
+        return ops.collect_rows(_aligned(d_rows), ctx.plan), None
+
+
+class HipCombine(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, rows, w, plan):
+        ctx.save_for_backward(rows, w)
+        ctx.plan = plan
+        return ops.collect_rows(rows, plan, w)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, d_out):
+        rows, w = ctx.saved_tensors
+        need_rows, need_w = ctx.needs_input_grad[:2]
+        if not (need_rows or need_w):
+            return None, None, None
+        d_rows, dw = ops.spread_rows(_aligned(d_out), ctx.plan, w, rows if need_w else None, need_rows)
+        return d_rows, dw, None
+
+
+def dispatch(x, topk_idx, num_experts):
+    """Tokens x [T,h] (bf16 or fp32) in expert order, for experts of the caller's own: (rows [T*k,h], plan). Expert e's
+    rows are rows[plan.starts[e] : plan.starts[e] + plan.counts[e]], in the order of the pairs; pairs routed outside [0, num_experts)
+    have none, and as many rows at the end are zero. topk_idx [T,k] int32 or int64; num_experts <= 64, k <= 8, h a
+    multiple of 64. Gradients flow to x. ``combine`` with the same plan brings the experts' outputs back."""
+    if x.dim() != 2 or topk_idx.dim() != 2 or topk_idx.shape[0] != x.shape[0]:
+        raise ValueError(f"x must be [T,h] and topk_idx [T,k], got {tuple(x.shape)} and {tuple(topk_idx.shape)}")
+    ops._fdt(x, "x")
+    plan = ops.rows_plan(topk_idx.contiguous(), num_experts)
+    return HipDispatch.apply(_aligned(x), plan), plan
+
+
+def combine(rows, topk_w, plan):
+    """Expert outputs ``rows`` [T*k,h] in ``dispatch``'s order summed per token with the routing weights topk_w [T,k]
+    (the rows' type or fp32): [T,h]. Products and sums are fp32, rounded once. Gradients flow to rows (zero where no
+    pair has the row) and topk_w (zero for pairs without a row)."""
+    dt = ops._fdt(rows, "rows")
+    if dt == torch.float32 and topk_w.dtype == torch.bfloat16:
+        topk_w = topk_w.float()
+    return HipCombine.apply(_aligned(rows), topk_w.contiguous(), plan)

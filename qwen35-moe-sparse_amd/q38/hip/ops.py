@@ -7,7 +7,10 @@ of the reference, computed without intermediate roundings); the activations' dty
 weights must share it. Weights use the reference parameter layouts (experts.gate_up_proj [E,2I,h],
 experts.down_proj [E,h,I], nn.Linear weights [out,in]).
 """
+import contextlib
 import ctypes
+import math
+from typing import NamedTuple
 
 import torch
 
@@ -792,4 +795,270 @@ def qsa_attention(q, k, v, qg, sel, scale):
     out = torch.empty(B, S, H * 64, dtype=dt, device=q.device)
     check(lib.q38moe_qsa_attention(_ptr(q), _ptr(k), _ptr(v), _ptr(qg), _ptr(sel), _ptr(out), B, S, H, KV, kk, scale,
                                    _DTYPES[dt], _stream(q.device)), "q38moe_qsa_attention")
+    return out
+
+
+# ---- a training step around the block: the head's loss, gradient clipping, rows to the caller's experts ----
+
+NEED_LOSS_X, NEED_LOSS_W = 1, 2
+_NORMS = {1.0: 1, 2.0: 2, math.inf: 3}
+
+
+def _on(device):
+    """The tensors' device as the current one, for launches on its stream."""
+    return contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def _loss_args(x, w, targets):
+    dt = _fdt(x, "x")
+    _need(x, "x", dtype=dt, ndim=2)
+    _need(w, "w", dtype=dt, ndim=2)
+    _need(targets, "targets", dtype=None, ndim=1)
+    if targets.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"targets must be int32 or int64, got {targets.dtype}")
+    T, h = x.shape
+    if w.shape[1] != h:
+        raise ValueError(f"w {tuple(w.shape)} does not match hidden {h}")
+    if targets.numel() != T:
+        raise ValueError(f"targets must hold {T} ids, got {targets.numel()}")
+    if w.device != x.device or targets.device != x.device:
+        raise RuntimeError("x, w and targets must be on one device")
+    return dt, T, h, w.shape[0]
+
+
+def _loss_workspace(T, h, V, needs, dt, device):
+    n = ctypes.c_size_t()
+    check(lib.q38moe_linear_ce_workspace_bytes(T, h, V, needs, _DTYPES[dt], ctypes.byref(n)),
+          "q38moe_linear_ce_workspace_bytes")
+    return torch.empty(n.value, dtype=torch.uint8, device=device)
+
+
+def linear_ce_forward(x, w, targets, ignore_index=-100, reduction=None):
+    """Softmax cross entropy of logits x . w^T without the logits (q38moe_linear_ce_forward): (loss [T], lse [T],
+    reduced) fp32, reduced = [sum or mean of the losses, the rows' gradient factor] for reduction "sum" or "mean", else None."""
+    dt, T, h, V = _loss_args(x, w, targets)
+    if reduction not in (None, "sum", "mean"):
+        raise ValueError(f"reduction must be None, 'sum' or 'mean', got {reduction!r}")
+    dev = x.device
+    loss = torch.empty(T, dtype=torch.float32, device=dev)
+    lse = torch.empty(T, dtype=torch.float32, device=dev)
+    reduced = None
+    if reduction is not None:
+        reduced = torch.empty(2, dtype=torch.float32, device=dev) if T else torch.zeros(2, device=dev)
+    with _on(dev):
+        ws = _loss_workspace(T, h, V, 0, dt, dev)
+        check(lib.q38moe_linear_ce_forward(_ptr(x), _ptr(w), _ptr(targets), targets.dtype == torch.int64, ignore_index,
+                                           _ptr(loss), _ptr(lse), _ptr(reduced), reduction == "mean", T, h, V, _ptr(ws),
+                                           ws.numel(), _DTYPES[dt], _stream(dev)), "q38moe_linear_ce_forward")
+    return loss, lse, reduced
+
+
+def linear_ce_backward(g, x, w, targets, lse, ignore_index=-100, row_scale=None, need_x=True, need_w=True):
+    """Gradients (dx [T,h], dw [V,h], None where not needed) of linear_ce_forward's losses for their gradient g, fp32: one
+    element for every row, or [T]; times row_scale (one fp32 element) where given."""
+    dt, T, h, V = _loss_args(x, w, targets)
+    dev = x.device
+    _need(g, "g", dtype=torch.float32)
+    _same(lse, "lse", torch.float32, (T,))
+    if g.dim() > 1 or (g.dim() == 1 and g.numel() != T):
+        raise ValueError(f"g must hold one element or [{T}], got {tuple(g.shape)}")
+    if row_scale is not None:
+        _need(row_scale, "row_scale", dtype=torch.float32)
+    if T == 0:
+        return (torch.zeros_like(x) if need_x else None), (torch.zeros_like(w) if need_w else None)
+    dx = torch.empty_like(x) if need_x else None
+    dw = torch.empty_like(w) if need_w else None
+    with _on(dev):
+        ws = _loss_workspace(T, h, V, NEED_LOSS_X * need_x | NEED_LOSS_W * need_w, dt, dev)
+        check(lib.q38moe_linear_ce_backward(_ptr(g), g.dim() == 1, _ptr(row_scale), _ptr(x), _ptr(w), _ptr(targets),
+                                            targets.dtype == torch.int64, ignore_index, _ptr(lse), _ptr(dx), _ptr(dw),
+                                            T, h, V, _ptr(ws), ws.numel(), _DTYPES[dt], _stream(dev)),
+              "q38moe_linear_ce_backward")
+    return dx, dw
+
+
+def _norm_args(tensors, norm_type):
+    norm = _NORMS.get(float(norm_type))
+    if norm is None:
+        raise ValueError(f"norm_type must be 1, 2 or inf, got {norm_type!r}")
+    dtypes = []
+    dev = None
+    for t in tensors:
+        code = _DTYPES.get(t.dtype) if isinstance(t, torch.Tensor) else None
+        if code is None:
+            raise TypeError(f"gradients must be bf16 or fp32 tensors, got {getattr(t, 'dtype', type(t))}")
+        if t.layout is not torch.strided:
+            raise TypeError(f"gradients must be dense, got {t.layout}")
+        if not t.is_cuda:
+            raise RuntimeError("gradients must be CUDA/HIP tensors")
+        if not t.is_contiguous():
+            raise ValueError(f"gradients must be contiguous, got strides {t.stride()} for {tuple(t.shape)}")
+        if dev is None:
+            dev = t.device
+        elif t.device != dev:
+            raise RuntimeError(f"gradients must be on one device, got {dev} and {t.device}")
+        dtypes.append(code)
+    n = len(dtypes)
+    ptrs = (ctypes.c_void_p * n)(*[t.data_ptr() for t in tensors])
+    sizes = (ctypes.c_int64 * n)(*[t.numel() for t in tensors])
+    return norm, dev, n, ptrs, sizes, (ctypes.c_int32 * n)(*dtypes)
+
+
+def _norm_workspace(n, dev):
+    b = ctypes.c_size_t()
+    check(lib.q38moe_grad_norm_workspace_bytes(n, ctypes.byref(b)), "q38moe_grad_norm_workspace_bytes")
+    return torch.empty(b.value, dtype=torch.uint8, device=dev)
+
+
+def grad_norm(grads, norm_type=2.0):
+    """Global norm (p = 1, 2 or inf) of all elements of the tensors in ``grads`` (bf16 or fp32, contiguous, on one
+    GPU), summed in fp64: an fp32 scalar on their device (q38moe_grad_norm). Without tensors, 0 on the CPU."""
+    grads = list(grads)
+    if not grads:
+        if float(norm_type) not in _NORMS:
+            raise ValueError(f"norm_type must be 1, 2 or inf, got {norm_type!r}")
+        return torch.tensor(0.0)
+    norm, dev, n, ptrs, sizes, dts = _norm_args(grads, norm_type)
+    with _on(dev):
+        total = torch.empty((), dtype=torch.float32, device=dev)
+        ws = _norm_workspace(n, dev)
+        check(lib.q38moe_grad_norm(ptrs, sizes, dts, n, norm, _ptr(total), _ptr(ws), ws.numel(), _stream(dev)),
+              "q38moe_grad_norm")
+    return total
+
+
+def clip_grads(grads, max_norm, norm_type=2.0, out=None):
+    """``grads`` times min(1, max_norm / (N + 1e-6)), N their global norm as in ``grad_norm``: in place, or into the
+    tensors of ``out`` (of the same shapes, bf16 or fp32 each, which no tensor of ``grads`` may overlap unless it is
+    its own). Returns N. Nothing is synchronised (q38moe_clip_grads)."""
+    grads = list(grads)
+    max_norm = float(max_norm)
+    outs = grads if out is None else list(out)
+    if len(outs) != len(grads):
+        raise ValueError(f"out must hold {len(grads)} tensors, got {len(outs)}")
+    if not max_norm >= 0:
+        raise ValueError(f"max_norm must be >= 0, got {max_norm}")
+    if not grads:
+        return grad_norm(grads, norm_type)
+    norm, dev, n, ptrs, sizes, dts = _norm_args(grads, norm_type)
+    optrs, odts = ptrs, dts
+    if out is not None:
+        _, odev, _, optrs, _, odts = _norm_args(outs, norm_type)
+        if odev != dev:
+            raise RuntimeError(f"out must be on {dev}, got {odev}")
+        for g, o in zip(grads, outs):
+            if g.shape != o.shape:
+                raise ValueError(f"out must have the gradients' shapes, got {tuple(o.shape)} for {tuple(g.shape)}")
+    with _on(dev):
+        total = torch.empty((), dtype=torch.float32, device=dev)
+        ws = _norm_workspace(n, dev)
+        check(lib.q38moe_clip_grads(ptrs, optrs, sizes, dts, odts, n, norm, max_norm, _ptr(total), _ptr(ws), ws.numel(),
+                                    _stream(dev)), "q38moe_clip_grads")
+    torch.autograd.graph.increment_version(outs)
+    return total
+
+
+def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False):
+    """``torch.nn.utils.clip_grad_norm_`` in two launches per 96 gradients: the ``.grad`` of ``parameters`` (a tensor
+    or an iterable; those without one are left out, a gradient met twice counts once) clipped in place to a global
+    norm of ``max_norm``. Returns the norm before. ``error_if_nonfinite`` reads it back before anything is changed."""
+    if isinstance(parameters, torch.Tensor):
+        parameters = [parameters]
+    grads = list({id(g): g for g in (p.grad for p in parameters) if g is not None}.values())
+    flat = [g if g.layout is not torch.strided or g.is_contiguous() else g.contiguous() for g in grads]
+    if error_if_nonfinite and flat:
+        total = grad_norm(flat, norm_type)
+        if not bool(torch.isfinite(total)):
+            raise RuntimeError(f"the total norm of order {norm_type} of the gradients is not finite, so they cannot be "
+                               "clipped; nothing was changed")
+    total = clip_grads(flat, max_norm, norm_type)
+    for g, f in zip(grads, flat):
+        if f is not g:
+            g.copy_(f)
+    return total
+
+
+class RowsPlan(NamedTuple):
+    """Where the pairs of a routing [T,k] go: expert e's rows are starts[e] .. starts[e] + counts[e] - 1, row r is pair
+    perm[r] (token perm[r] // k; only rows that are filled), pair p is row inv[p] (only pairs routed inside [0, E))."""
+
+    idx: torch.Tensor
+    counts: torch.Tensor
+    starts: torch.Tensor
+    perm: torch.Tensor
+    inv: torch.Tensor
+    experts: int
+
+
+def rows_plan(topk_idx, experts):
+    """The stable sort of routing indices [T,k] (int32 or int64) by expert (q38moe_histogram, q38moe_permute)."""
+    _need(topk_idx, "topk_idx", dtype=None, ndim=2)
+    flag = _idx_flag(topk_idx)
+    T, k = topk_idx.shape
+    dev = topk_idx.device
+    nb = max((T + 63) // 64, 1)
+    # One allocation, each part on a 16-byte boundary.
+    E4, P4 = -(-experts // 4) * 4, -(-T * k // 4) * 4
+    buf = torch.empty(2 * E4 + 2 * P4 + nb * experts, dtype=torch.int32, device=dev)
+    counts, starts = buf[:experts], buf[E4:E4 + experts]
+    perm, inv = buf[2 * E4:2 * E4 + T * k], buf[2 * E4 + P4:2 * E4 + P4 + T * k]
+    hist = buf[2 * E4 + 2 * P4:]
+    with _on(dev):
+        st = _stream(dev)
+        check(lib.q38moe_histogram(_ptr(topk_idx), flag, _ptr(hist), T, experts, k, st), "q38moe_histogram")
+        check(lib.q38moe_permute(_ptr(topk_idx), flag, _ptr(hist), _ptr(counts), _ptr(starts), _ptr(perm), _ptr(inv),
+                                 None, None, 0, T, experts, k, st), "q38moe_permute")
+    return RowsPlan(topk_idx, counts, starts, perm, inv, experts)
+
+
+def _rows_weights(w, shape, dt):
+    _need(w, "weights", dtype=None, ndim=2)
+    if w.dtype not in (dt, torch.float32):
+        raise TypeError(f"weights must be {dt} or fp32, got {w.dtype}")
+    if w.shape != shape:
+        raise ValueError(f"weights must be {tuple(shape)}, got {tuple(w.shape)}")
+    return w
+
+
+def spread_rows(src, plan, w=None, y=None, need_rows=True):
+    """Rows in expert order from tokens (q38moe_spread_rows): (rows [T*k,h] with rows[inv[p]] = src[t] (* w[p]) and zeros
+    behind the filled ones, dw [T,k] with dw[p] = <src[t], y[inv[p]]>, None without y or need_rows)."""
+    dt = _fdt(src, "src")
+    _need(src, "src", dtype=dt, ndim=2)
+    T, k = plan.idx.shape
+    h = src.shape[1]
+    if src.shape[0] != T:
+        raise ValueError(f"src must hold {T} tokens, got {src.shape[0]}")
+    if w is not None:
+        _rows_weights(w, plan.idx.shape, dt)
+    if y is not None:
+        _same(y, "y", dt, (T * k, h))
+        if w is None:
+            raise ValueError("y needs weights")
+    dst = torch.empty(T * k, h, dtype=dt, device=src.device) if need_rows else None
+    dw = torch.empty_like(w) if y is not None else None
+    with _on(src.device):
+        check(lib.q38moe_spread_rows(_ptr(src), _ptr(w), _DTYPES[dt if w is None else w.dtype], _ptr(y),
+                                     _ptr(plan.idx), _idx_flag(plan.idx), _ptr(plan.inv), _ptr(plan.starts),
+                                     _ptr(plan.counts), _ptr(dst), _ptr(dw), T, h, plan.experts, k, _DTYPES[dt],
+                                     _stream(src.device)), "q38moe_spread_rows")
+    return dst, dw
+
+
+def collect_rows(rows, plan, w=None):
+    """Tokens [T,h] from rows [T*k,h] in expert order (q38moe_collect_rows): sum_j rows[inv[p]] (* w[p]), summed in
+    fp32 and rounded once; pairs without a row add nothing."""
+    dt = _fdt(rows, "rows")
+    T, k = plan.idx.shape
+    _need(rows, "rows", dtype=dt, ndim=2)
+    h = rows.shape[1]
+    if rows.shape[0] != T * k:
+        raise ValueError(f"rows must hold {T * k} rows, got {rows.shape[0]}")
+    if w is not None:
+        _rows_weights(w, plan.idx.shape, dt)
+    out = torch.empty(T, h, dtype=dt, device=rows.device)
+    with _on(rows.device):
+        check(lib.q38moe_collect_rows(_ptr(rows), _ptr(w), _DTYPES[dt if w is None else w.dtype], _ptr(plan.idx),
+                                      _idx_flag(plan.idx), _ptr(plan.inv), _ptr(out), T, h, plan.experts, k,
+                                      _DTYPES[dt], _stream(rows.device)), "q38moe_collect_rows")
     return out
