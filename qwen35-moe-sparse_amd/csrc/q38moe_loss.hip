@@ -132,6 +132,26 @@ __device__ __forceinline__ void ls_mfma(f32x16_t& acc, u32x4_t a, u32x4_t b) {
 // Wait states between the last MFMA and VALU reads of its result (16 passes).
 __device__ __forceinline__ void ls_drain() { asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 7" ::: "memory"); }
 
+// A block's accumulators in VGPRs, at this place of the instruction order (left to itself the compiler moves all of a
+// tile's out at once, and spills).
+__device__ __forceinline__ f32x16_t ls_take(const f32x16_t& a) {
+  f32x16_t v = a;
+  asm volatile("" : "+v"(v));
+  return v;
+}
+
+// v = with where a value's row 32 i + 8 (q / 4) + q % 4 is `left` or beyond. (The comparisons stay at their place: as invariants
+// of the blocks' loop their masks would not fit the SGPRs.)
+template <int MB>
+__device__ __forceinline__ void ls_mask(f32x16_t (&v)[MB], int left, float with) {
+  asm volatile("" : "+v"(left));
+#pragma unroll
+  for (int i = 0; i < MB; ++i)
+#pragma unroll
+    for (int q = 0; q < 16; ++q)
+      if (32 * i + 8 * (q >> 2) + (q & 3) >= left) v[i][q] = with;
+}
+
 __device__ __forceinline__ uint32_t ls_lds_addr(const void* p) {
   return uniform((uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)p);
 }
@@ -160,7 +180,6 @@ struct LsParams {
   const float* r_scale;  // EPI_OUT: the reduction's factor (NULL: 1)
   bool scatter;          // EPI_OUT: rows through `rows`
   bool add;              // EPI_ACC: add to what is there
-  bool out_f32;
 };
 
 // Position of a work item: tile (m0, n0) and its K steps.
@@ -176,6 +195,9 @@ __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void ls_gemm_kernel(const L
   constexpr int SLOT = (BM + BN) * 128;
   constexpr int BK = OA::BK, ESZ = OA::ESZ;
   __shared__ __align__(1024) uint8_t lds[2 * SLOT];
+  // Staging of bf16 outputs, 32 rows of out by BM / 2 columns per wave (beside the slots: copies for the next item run meanwhile).
+  constexpr bool STAGED = !F32 && (EPI == EPI_S || EPI == EPI_OUT);
+  __shared__ __align__(1024) uint8_t stage[STAGED ? 4 * 32 * BM : 16];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = (int)uniform((uint32_t)tid >> 6);
   const int wm = wave >> 1, wn = wave & 1;
@@ -257,41 +279,76 @@ __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void ls_gemm_kernel(const L
     ls_dma(rb, vb[j], 0, slot + BM * 128 + (uint32_t)wave * (BN * 32) + (uint32_t)j * 1024u);
   };
 
+  // Copies of stream position q go to slot q % 2. While step q multiplies, q + 1 lies in the other slot; q + 2 is copied over
+  // q once every wave has read it, during q's last quarter, and has the three quarters of q + 1 to arrive.
+  auto copy = [&](int j, uint32_t slot) {
+    if (j < OA::NDMA) copy_a(j, slot);
+    else copy_b(j - OA::NDMA, slot);
+  };
+  bases();
+#pragma unroll
+  for (int j = 0; j < OA::NDMA + OB::NDMA; ++j) copy(j, lds0);
+  advance();
+  bases();
+#pragma unroll
+  for (int j = 0; j < OA::NDMA + OB::NDMA; ++j) copy(j, lds0 + SLOT);
+  advance();
+  asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+
   f32x16_t acc[MB][NB];
-  LsItem it = c;
+  u32x4_t fr[2][MB + NB];  // fragments of two quarters: A's, then B's
+  auto read = [&](int j, const uint8_t* base, int u) {
+    return j < MB ? OA::frag(base, fa, j, u) : OB::frag(base, fb, j - MB, u);
+  };
+#pragma unroll
+  for (int j = 0; j < MB + NB; ++j) fr[0][j] = read(j, lds, 0);
+  LsItem it = item_of(first);
   int64_t item = first;
   int slot = 0;
 #pragma unroll 1
   for (;;) {
+#pragma unroll 1
     for (int s = 0; s < it.nk; ++s) {
-      // Simple form: copy a step, wait, multiply.
-      bases();
-      const uint32_t sl = lds0 + (uint32_t)slot * SLOT;
-#pragma unroll
-      for (int j = 0; j < OA::NDMA; ++j) copy_a(j, sl);
-#pragma unroll
-      for (int j = 0; j < OB::NDMA; ++j) copy_b(j, sl);
-      advance();
-      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
       const uint8_t* base = lds + slot * SLOT;
+      const uint8_t* next = lds + (slot ^ 1) * SLOT;
+      // Quarter u multiplies fr[u % 2] while the next quarter's fragments are read into the other half, one read after
+      // each of the first MFMAs.
+      if (s == 0) {
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        u32x4_t a[MB], b[NB];
-#pragma unroll
-        for (int i = 0; i < MB; ++i) a[i] = OA::frag(base, fa, i, u);
-#pragma unroll
-        for (int i = 0; i < NB; ++i) b[i] = OB::frag(base, fb, i, u);
-        if (s == 0 && u == 0) {
-#pragma unroll
-          for (int i = 0; i < MB; ++i)
-#pragma unroll
-            for (int j = 0; j < NB; ++j) ls_mfma<F32, true>(acc[i][j], a[i], b[j]);
-        } else {
-#pragma unroll
-          for (int i = 0; i < MB; ++i)
-#pragma unroll
-            for (int j = 0; j < NB; ++j) ls_mfma<F32, false>(acc[i][j], a[i], b[j]);
+        for (int q = 0; q < MB * NB; ++q) {
+          ls_mfma<F32, true>(acc[q / NB][q % NB], fr[0][q / NB], fr[0][MB + q % NB]);
+          if (q < MB + NB) fr[1][q] = read(q, base, 1);
         }
+      } else {
+#pragma unroll
+        for (int q = 0; q < MB * NB; ++q) {
+          ls_mfma<F32, false>(acc[q / NB][q % NB], fr[0][q / NB], fr[0][MB + q % NB]);
+          if (q < MB + NB) fr[1][q] = read(q, base, 1);
+        }
+      }
+#pragma unroll
+      for (int q = 0; q < MB * NB; ++q) {
+        ls_mfma<F32, false>(acc[q / NB][q % NB], fr[1][q / NB], fr[1][MB + q % NB]);
+        if (q < MB + NB) fr[0][q] = read(q, base, 2);
+      }
+#pragma unroll
+      for (int q = 0; q < MB * NB; ++q) {
+        ls_mfma<F32, false>(acc[q / NB][q % NB], fr[0][q / NB], fr[0][MB + q % NB]);
+        if (q < MB + NB) fr[1][q] = read(q, base, 3);
+      }
+      bases();
+      advance();
+      // Every wave's reads of this slot are done (its own by lgkmcnt) and the next step's copies have landed.
+      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      const uint32_t here = lds0 + (uint32_t)slot * SLOT;
+#pragma unroll
+      for (int q = 0; q < MB * NB; ++q) {
+        ls_mfma<F32, false>(acc[q / NB][q % NB], fr[1][q / NB], fr[1][MB + q % NB]);
+        constexpr int PER = (OA::NDMA + OB::NDMA) / (MB * NB);
+        static_assert(PER * MB * NB == OA::NDMA + OB::NDMA, "copies go evenly between the MFMAs");
+#pragma unroll
+        for (int e = 0; e < PER; ++e) copy(q * PER + e, here);
+        if (q < MB + NB) fr[0][q] = read(q, next, 0);
       }
       slot ^= 1;
     }
@@ -301,101 +358,121 @@ __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void ls_gemm_kernel(const L
     const int64_t mw = (int64_t)it.m * BM + wm * (BM / 2), nw = (int64_t)it.n * BN + wn * (BN / 2);
     const int lh = lane >> 5;
     const int mleft = (int)min((int64_t)(BM / 2), p.m_rows - mw);  // rows of the wave that exist (may be <= 0)
+    float scale = 1.0f;
+    if (EPI == EPI_OUT) {
+      if (p.g_scale != nullptr) scale *= *p.g_scale;
+      if (p.r_scale != nullptr) scale *= *p.r_scale;
+    }
 #pragma unroll
     for (int j = 0; j < NB; ++j) {
       const int64_t n = nw + 32 * j + (lane & 31);
       const bool n_ok = n < N;
+      f32x16_t v[MB];
+#pragma unroll
+      for (int i = 0; i < MB; ++i) v[i] = ls_take(acc[i][j]);
       if constexpr (EPI == EPI_LSE) {
         const int rel = n_ok ? p.tgt[n] - (int)mw : -1;
+        if (mleft < BM / 2) ls_mask(v, mleft - 4 * lh, -__builtin_inff());
         float mx = -__builtin_inff();
 #pragma unroll
         for (int i = 0; i < MB; ++i)
 #pragma unroll
-          for (int q = 0; q < 16; ++q) {
-            const int r = 32 * i + 8 * (q >> 2) + 4 * lh + (q & 3);
-            if (r < mleft) mx = fmaxf(mx, acc[i][j][q]);
-          }
+          for (int q = 0; q < 16; ++q) mx = fmaxf(mx, v[i][q]);
         mx = fmaxf(mx, __shfl_xor(mx, 32));
         const float ref = mx == -__builtin_inff() ? 0.0f : mx;
-        float sum = 0.0f;
+        float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int i = 0; i < MB; ++i)
 #pragma unroll
-          for (int q = 0; q < 16; ++q) {
-            const int r = 32 * i + 8 * (q >> 2) + 4 * lh + (q & 3);
-            if (r < mleft) sum += __builtin_amdgcn_exp2f((acc[i][j][q] - ref) * LOG2E);
-          }
-        sum += __shfl_xor(sum, 32);
-        if (n_ok && lh == 0) p.part[((int64_t)it.m * 2 + wm) * p.T + n] = make_float2(mx, sum);
+          for (int q = 0; q < 16; ++q) sum[q & 3] += __builtin_amdgcn_exp2f((v[i][q] - ref) * LOG2E);
+        float all_sum = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        all_sum += __shfl_xor(all_sum, 32);
+        if (n_ok && lh == 0) p.part[((int64_t)it.m * 2 + wm) * p.T + n] = make_float2(mx, all_sum);
 #pragma unroll
         for (int i = 0; i < MB; ++i) {
           if (__any((rel >> 5) == i)) {
 #pragma unroll
             for (int q = 0; q < 16; ++q)
-              if (rel == 32 * i + 8 * (q >> 2) + 4 * lh + (q & 3) && rel < mleft) p.zt[n] = acc[i][j][q];
+              if (rel == 32 * i + 8 * (q >> 2) + 4 * lh + (q & 3)) p.zt[n] = v[i][q];
           }
         }
-      } else if constexpr (EPI == EPI_S) {
-        if (!n_ok) continue;
-        const int64_t row = p.rows[n];
-        const float lse = p.lse[row];
-        const float g = p.g_row != nullptr ? p.g_row[row] : 1.0f;
-        const int rel = p.tgt[n] - (int)p.v0 - (int)mw;
-#pragma unroll
-        for (int i = 0; i < MB; ++i)
-#pragma unroll
-          for (int q4 = 0; q4 < 4; ++q4) {
-            const int r0 = 32 * i + 8 * q4 + 4 * lh;
-            float f[4];
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              f[q] = __builtin_amdgcn_exp2f((acc[i][j][4 * q4 + q] - lse) * LOG2E);
-              if (rel == r0 + q) f[q] -= 1.0f;
-              f[q] = r0 + q < mleft ? f[q] * g : 0.0f;
-            }
-            const int64_t at = n * p.ldo + mw + r0;
-            if constexpr (F32)
-              *reinterpret_cast<f32x4_t*>(static_cast<float*>(p.out) + at) = (f32x4_t){f[0], f[1], f[2], f[3]};
-            else
-              *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + at) =
-                  make_uint2(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]));
-          }
       } else {
-        if (!n_ok) continue;
-        float scale = 1.0f;
-        if (EPI == EPI_OUT) {
-          if (p.g_scale != nullptr) scale *= *p.g_scale;
-          if (p.r_scale != nullptr) scale *= *p.r_scale;
+        if constexpr (EPI == EPI_S) {
+          const int64_t row = n_ok ? p.rows[n] : 0;
+          const float lse = n_ok ? p.lse[row] : 0.0f;
+          const float g = p.g_row != nullptr && n_ok ? p.g_row[row] : 1.0f;
+          const int rel = n_ok ? p.tgt[n] - (int)p.v0 - (int)mw : -1;
+#pragma unroll
+          for (int i = 0; i < MB; ++i) {
+#pragma unroll
+            for (int q = 0; q < 16; ++q) v[i][q] = __builtin_amdgcn_exp2f((v[i][q] - lse) * LOG2E);
+            if (__any((rel >> 5) == i)) {
+#pragma unroll
+              for (int q = 0; q < 16; ++q)
+                if (rel == 32 * i + 8 * (q >> 2) + 4 * lh + (q & 3)) v[i][q] -= 1.0f;
+            }
+            if (p.g_row != nullptr) v[i] *= g;
+          }
+          if (mleft < BM / 2) ls_mask(v, mleft - 4 * lh, 0.0f);
+        } else if (EPI == EPI_OUT) {
+#pragma unroll
+          for (int i = 0; i < MB; ++i) v[i] *= scale;
         }
-        const int64_t row = EPI == EPI_OUT && p.scatter ? (int64_t)p.rows[n]
-                                                        : (EPI == EPI_ACC ? (int64_t)it.part * p.N + n : n);
+        const int mstore = EPI == EPI_S ? BM / 2 : mleft;  // s: whole tiles, the others' rows are a multiple of 64
+        if constexpr (F32 || EPI == EPI_ACC) {
+          if (n_ok) {
+            const int64_t row = EPI == EPI_ACC ? (int64_t)it.part * p.N + n
+                                               : (EPI == EPI_OUT && p.scatter ? (int64_t)p.rows[n] : n);
 #pragma unroll
-        for (int i = 0; i < MB; ++i)
+            for (int i = 0; i < MB; ++i)
 #pragma unroll
-          for (int q4 = 0; q4 < 4; ++q4) {
-            const int r0 = 32 * i + 8 * q4 + 4 * lh;
-            if (r0 >= mleft) continue;  // M is a multiple of 64
-            f32x4_t f;
+              for (int q4 = 0; q4 < 4; ++q4) {
+                const int r0 = 32 * i + 8 * q4 + 4 * lh;
+                if (r0 >= mstore) continue;
+                f32x4_t f = {v[i][4 * q4], v[i][4 * q4 + 1], v[i][4 * q4 + 2], v[i][4 * q4 + 3]};
+                f32x4_t* o = reinterpret_cast<f32x4_t*>(static_cast<float*>(p.out) + row * p.ldo + mw + r0);
+                if (EPI == EPI_ACC && p.add) f += *o;
+                *o = f;
+              }
+          }
+        } else {
+          // Through the wave's staging area, 32 rows of out by BM / 2 columns, so that stores write whole lines: 16-byte chunk
+          // c of row r at c ^ r.
+          constexpr int PITCH = BM, CH = BM / 16;  // bytes and chunks of a row
+          uint8_t* const st = stage + wave * 32 * PITCH;
+          const int r = lane & 31;
 #pragma unroll
-            for (int q = 0; q < 4; ++q) f[q] = acc[i][j][4 * q4 + q] * scale;
-            const int64_t at = row * p.ldo + mw + r0;
-            if constexpr (EPI == EPI_ACC) {
-              f32x4_t* o = reinterpret_cast<f32x4_t*>(static_cast<float*>(p.out) + at);
-              if (p.add) f += *o;
-              *o = f;
-            } else if (p.out_f32) {
-              *reinterpret_cast<f32x4_t*>(static_cast<float*>(p.out) + at) = f;
-            } else {
-              *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + at) =
-                  make_uint2(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]));
+          for (int i = 0; i < MB; ++i)
+#pragma unroll
+            for (int q4 = 0; q4 < 4; ++q4)
+              *reinterpret_cast<uint2*>(st + r * PITCH + 16 * ((4 * i + q4) ^ (r & (CH - 1))) + 8 * lh) =
+                  make_uint2(pack_bf16x2(v[i][4 * q4], v[i][4 * q4 + 1]),
+                             pack_bf16x2(v[i][4 * q4 + 2], v[i][4 * q4 + 3]));
+          constexpr int RPI = 64 / CH;  // rows of a store
+          const int c = lane % CH;
+          u32x4_t w[32 / RPI];
+#pragma unroll
+          for (int k = 0; k < 32 / RPI; ++k) {
+            const int rr = k * RPI + lane / CH;
+            w[k] = ld16(st + rr * PITCH + 16 * (c ^ (rr & (CH - 1))));
+          }
+#pragma unroll
+          for (int k = 0; k < 32 / RPI; ++k) {
+            const int64_t nn = nw + 32 * j + k * RPI + lane / CH;
+            if (nn < N && 8 * c < mstore) {
+              const int64_t row = EPI == EPI_OUT && p.scatter ? (int64_t)p.rows[nn] : nn;
+              st16(static_cast<uint16_t*>(p.out) + row * p.ldo + mw + 8 * c, w[k]);
             }
           }
+        }
       }
     }
     item += G;
     if (item >= total) break;
     it = item_of(item);
   }
+  // The last copies (of nothing) complete before the block's LDS is released.
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 }
 
 // Partition of the rows: rows[0 .. n-1] those that count, ascending, rows[n .. T-1] the ignored ones, *count = n, tgt[i]
@@ -782,7 +859,6 @@ hipError_t ce_backward(const float* g, bool g_rows, const float* r_scale, const 
         LS_TRY((ls_gemm_any<F32, KS, KC, EPI_ACC>(q, big, st)));
       } else {
         q.out = dx;
-        q.out_f32 = F32;
         q.scatter = true;
         q.g_scale = scale;
         q.r_scale = r_scale;
@@ -813,7 +889,6 @@ hipError_t ce_backward(const float* g, bool g_rows, const float* r_scale, const 
         LS_TRY(hipGetLastError());
       } else {
         q.out = out;
-        q.out_f32 = F32;
         q.g_scale = scale;
         q.r_scale = r_scale;
         LS_TRY((ls_gemm_any<F32, KS, KS, EPI_OUT>(q, big, st)));
