@@ -35,22 +35,17 @@ constexpr float LOG2E = 1.4426950408889634f;
 
 typedef short ls_i16x4_t __attribute__((ext_vector_type(4)));
 
-// Copy of 16 bytes per lane from a buffer into LDS at lds + 16 lane. The compiler does not see these loads; the step's
-// barrier waits for them.
-__device__ __forceinline__ void ls_dma(u32x4_t rsrc, uint32_t voff, uint32_t soff, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 1\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(lds), "v"(voff),
-               "s"(rsrc), "s"(soff)
-               : "memory", "m0");
-}
-
 __device__ __forceinline__ uint32_t uniform(uint32_t v) { return __builtin_amdgcn_readfirstlane(v); }
 
-// Buffer resource (raw, no format) over `bytes` bytes at p; nothing where bytes <= 0.
-__device__ __forceinline__ u32x4_t ls_rsrc(const uint8_t* p, int64_t bytes) {
-  const uint64_t a = (uint64_t)(uintptr_t)p;
-  const uint32_t n = bytes <= 0 ? 0u : (bytes >= 0xffffffffll ? 0xffffffffu : (uint32_t)bytes);
-  return (u32x4_t){uniform((uint32_t)a), uniform((uint32_t)(a >> 32) & 0xffffu), uniform(n), 0x00020000u};
+// 16 bytes at p + voff + soff, zeros where voff (+ soff) reaches `bytes` (raw buffer, no format).
+__device__ __forceinline__ u32x4_t ls_load(const uint8_t* p, int64_t bytes, uint32_t voff, uint32_t soff) {
+  const int n = bytes <= 0 ? 0 : (bytes >= 0xffffffffll ? -1 : (int)(uint32_t)bytes);
+  const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(p), (short)0, n, 0x00020000);
+  return __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(r, (int)voff, (int)soff, 0));
 }
+
+// This wave's LDS operations are done, and so are the others'.
+__device__ __forceinline__ void ls_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
 __device__ __forceinline__ uint2 ls_read_tr(const uint8_t* p) {
   const ls_i16x4_t v = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
@@ -111,23 +106,22 @@ struct Operand {
   }
 };
 
-// acc += A B (or = A B): inline asm with the accumulator in its own AGPRs, as the four-wave gate/up kernel does it and
-// for its reasons; the build checks that no VALU write of an operand comes right before one.
-template <bool F32, bool FIRST>
+// acc += A B: inline asm with the accumulator in its own AGPRs, as the four-wave gate/up kernel does it and for its
+// reasons; two wait states cover a VALU write of an operand right before it.
+template <bool F32>
 __device__ __forceinline__ void ls_mfma(f32x16_t& acc, u32x4_t a, u32x4_t b) {
   if constexpr (F32) {
-    if constexpr (FIRST)
-      asm volatile("s_nop 1\n\tv_mfma_f32_32x32x2_f32 %0, %1, %2, 0" : "=a"(acc) : "v"(a[0]), "v"(b[0]));
-    else
-      asm volatile("s_nop 1\n\tv_mfma_f32_32x32x2_f32 %0, %1, %2, %0" : "+a"(acc) : "v"(a[0]), "v"(b[0]));
 #pragma unroll
-    for (int e = 1; e < 4; ++e)
+    for (int e = 0; e < 4; ++e)
       asm volatile("s_nop 1\n\tv_mfma_f32_32x32x2_f32 %0, %1, %2, %0" : "+a"(acc) : "v"(a[e]), "v"(b[e]));
-  } else if constexpr (FIRST) {
-    asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %1, %2, 0" : "=a"(acc) : "v"(a), "v"(b));
   } else {
     asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+a"(acc) : "v"(a), "v"(b));
   }
+}
+// acc = 0 by the matrix unit, which has nothing else to do between two tiles (16 VALU writes would cost the epilogue their time).
+__device__ __forceinline__ void ls_zero(f32x16_t& acc) {
+  const u32x4_t z = {0u, 0u, 0u, 0u};
+  asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %1, %1, 0" : "+a"(acc) : "v"(z));
 }
 // Wait states between the last MFMA and VALU reads of its result (16 passes).
 __device__ __forceinline__ void ls_drain() { asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 7" ::: "memory"); }
@@ -140,20 +134,21 @@ __device__ __forceinline__ f32x16_t ls_take(const f32x16_t& a) {
   return v;
 }
 
-// v = with where a value's row 32 i + 8 (q / 4) + q % 4 is `left` or beyond. (The comparisons stay at their place: as invariants
-// of the blocks' loop their masks would not fit the SGPRs.)
-template <int MB>
-__device__ __forceinline__ void ls_mask(f32x16_t (&v)[MB], int left, float with) {
+// v = with where a value's row 8 (q / 4) + q % 4 of the block is `left` or beyond. (The comparisons stay at their place: as
+// invariants of the blocks' loop their masks would not fit the SGPRs.)
+__device__ __forceinline__ void ls_mask(f32x16_t& v, int left, float with) {
   asm volatile("" : "+v"(left));
 #pragma unroll
-  for (int i = 0; i < MB; ++i)
-#pragma unroll
-    for (int q = 0; q < 16; ++q)
-      if (32 * i + 8 * (q >> 2) + (q & 3) >= left) v[i][q] = with;
+  for (int q = 0; q < 16; ++q)
+    if (8 * (q >> 2) + (q & 3) >= left) v[q] = with;
 }
 
-__device__ __forceinline__ uint32_t ls_lds_addr(const void* p) {
-  return uniform((uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)p);
+// {m, s} of two sets of values as one.
+__device__ __forceinline__ void lse_join(float& m, float& s, float m2, float s2) {
+  const float top = fmaxf(m, m2);
+  const float ref = top == -__builtin_inff() ? 0.0f : top;
+  s = s * __builtin_amdgcn_exp2f((m - ref) * LOG2E) + s2 * __builtin_amdgcn_exp2f((m2 - ref) * LOG2E);
+  m = top;
 }
 
 struct LsParams {
@@ -198,9 +193,12 @@ __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void ls_gemm_kernel(const L
   // Staging of bf16 outputs, 32 rows of out by BM / 2 columns per wave (beside the slots: copies for the next item run meanwhile).
   constexpr bool STAGED = !F32 && (EPI == EPI_S || EPI == EPI_OUT);
   __shared__ __align__(1024) uint8_t stage[STAGED ? 4 * 32 * BM : 16];
+  constexpr int CH = BM / 16, RPI = 64 / CH;  // 16-byte chunks of a staged row, rows of a store
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = (int)uniform((uint32_t)tid >> 6);
   const int wm = wave >> 1, wn = wave & 1;
+
+  uint8_t* const stw = stage + (STAGED ? wave * 32 * BM : 0);
 
   // Tokens are N of z^T and dx^T, K of dW^T.
   const int64_t cnt = p.count != nullptr ? (int64_t)load_uniform(p.count) : p.T;
@@ -209,22 +207,22 @@ __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void ls_gemm_kernel(const L
   const int64_t N = tok_k ? p.N : cnt, K = tok_k ? cnt : p.K;
   const uint8_t* const A = tok_k && all && p.alt != nullptr ? p.alt : p.A;
   const uint8_t* const B = !tok_k && all && p.alt != nullptr ? p.alt : p.B;
-  const int ntm = (int)((p.M + BM - 1) / BM), ntn = (int)((N + BN - 1) / BN);
+  const uint32_t ntm = (uint32_t)((p.M + BM - 1) / BM), ntn = (uint32_t)((N + BN - 1) / BN);
   const int steps = (int)((K + BK - 1) / BK), per = (steps + p.parts - 1) / p.parts;
-  const int64_t tiles = (int64_t)ntm * ntn, total = tiles * p.parts;
+  const uint32_t tiles = ntm * ntn, total = tiles * (uint32_t)p.parts;  // < 2^31: the callers' limits on T and V
 
   // Work items of neighbouring blocks on an XCD are neighbouring tiles: 8 tiles of M by as many of N as it has room for.
-  const int G = gridDim.x;
-  const int first = (G & 7) == 0 ? (int)(blockIdx.x & 7) * (G >> 3) + (int)(blockIdx.x >> 3) : (int)blockIdx.x;
+  const uint32_t G = gridDim.x;
+  const uint32_t first = (G & 7) == 0 ? (blockIdx.x & 7) * (G >> 3) + (blockIdx.x >> 3) : blockIdx.x;
   if (first >= total) return;
-  auto item_of = [&](int64_t L) {
+  auto item_of = [&](uint32_t L) {
     LsItem it;
-    it.part = (int)(L / tiles);
-    const int t = (int)(L - (int64_t)it.part * tiles);
-    const int grp = t / (8 * ntn), rem = t - grp * 8 * ntn;
-    const int gm = min(8, ntm - grp * 8);
-    it.n = rem / gm;
-    it.m = grp * 8 + rem - it.n * gm;
+    const uint32_t part = L / tiles, t = L - part * tiles;
+    const uint32_t grp = t / (8u * ntn), rem = t - grp * 8u * ntn;
+    const uint32_t gm = min(8u, ntm - grp * 8u), n = rem / gm;
+    it.part = (int)part;
+    it.n = (int)n;
+    it.m = (int)(grp * 8u + rem - n * gm);
     it.k0 = it.part * per;
     it.nk = max(1, min(per, steps - it.k0));  // a part without steps multiplies zeros
     return it;
@@ -240,62 +238,82 @@ __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void ls_gemm_kernel(const L
   for (int i = 0; i < OA::NOFF; ++i) fa[i] = OA::foff(i, wm, lane);
 #pragma unroll
   for (int i = 0; i < OB::NOFF; ++i) fb[i] = BM * 128 + OB::foff(i, wn, lane);
-  const uint32_t lds0 = ls_lds_addr(lds);
 
-  // The stream of K steps over this block's items, as the copies see it.
-  int64_t c_item = first;
+  // The stream of K steps over this block's items, as the loads see it: `c` and its step, the operands' resources and the
+  // K offset of a KC operand's rows (a KS operand's base moves instead: its end has to bound the step's K rows).
+  uint32_t c_item = first;
   LsItem c = item_of(c_item);
   int c_step = 0;
-  u32x4_t ra, rb;
-  auto bases = [&]() {
+  uint32_t c_soff = 0;
+  const uint8_t *pa, *pb;
+  int64_t na, nb;  // bytes from pa, pb to the operands' ends
+  auto enter = [&]() {
     const bool live = c_item < total;
-    const int64_t k = (int64_t)(c.k0 + c_step) * BK;
+    const int64_t k = (int64_t)c.k0 * BK, ma = (int64_t)c.m * BM, mb = (int64_t)c.n * BN;
+    c_soff = 0;
     if (LA == KC) {
-      const int64_t r0 = (int64_t)c.m * BM;
-      ra = ls_rsrc(A + r0 * p.lda + k * ESZ,
-                   live && k < K ? min((int64_t)BM, p.m_rows - r0) * p.lda - k * ESZ : 0);
+      pa = A + ma * p.lda + k * ESZ;
+      na = live && k < K ? min((int64_t)BM, p.m_rows - ma) * p.lda - k * ESZ : 0;
     } else {
-      const int64_t c0 = (int64_t)c.m * BM * ESZ;
-      ra = ls_rsrc(A + k * p.lda + c0, live ? (K - k) * p.lda - c0 : 0);
+      pa = A + k * p.lda + ma * ESZ;
+      na = live ? (K - k) * p.lda - ma * ESZ : 0;
     }
     if (LB == KC) {
-      const int64_t r0 = (int64_t)c.n * BN;
-      rb = ls_rsrc(B + r0 * p.ldb + k * ESZ, live && k < K ? min((int64_t)BN, N - r0) * p.ldb - k * ESZ : 0);
+      pb = B + mb * p.ldb + k * ESZ;
+      nb = live && k < K ? min((int64_t)BN, N - mb) * p.ldb - k * ESZ : 0;
     } else {
-      const int64_t c0 = (int64_t)c.n * BN * ESZ;
-      rb = ls_rsrc(B + k * p.ldb + c0, live ? (K - k) * p.ldb - c0 : 0);
+      pb = B + k * p.ldb + mb * ESZ;
+      nb = live ? (K - k) * p.ldb - mb * ESZ : 0;
     }
   };
   auto advance = [&]() {
-    if (++c_step < c.nk) return;
+    if (++c_step < c.nk) {
+      c_soff += 128;
+      if (LA == KS) pa += BK * p.lda, na -= BK * p.lda;
+      if (LB == KS) pb += BK * p.ldb, nb -= BK * p.ldb;
+      return;
+    }
     c_step = 0;
     c_item += G;
     if (c_item < total) c = item_of(c_item);
-  };
-  auto copy_a = [&](int j, uint32_t slot) {
-    ls_dma(ra, va[j], 0, slot + (uint32_t)wave * (BM * 32) + (uint32_t)j * 1024u);
-  };
-  auto copy_b = [&](int j, uint32_t slot) {
-    ls_dma(rb, vb[j], 0, slot + BM * 128 + (uint32_t)wave * (BN * 32) + (uint32_t)j * 1024u);
+    enter();
   };
 
-  // Copies of stream position q go to slot q % 2. While step q multiplies, q + 1 lies in the other slot; q + 2 is copied over
-  // q once every wave has read it, during q's last quarter, and has the three quarters of q + 1 to arrive.
-  auto copy = [&](int j, uint32_t slot) {
-    if (j < OA::NDMA) copy_a(j, slot);
-    else copy_b(j - OA::NDMA, slot);
+  // Loads of stream position q + 3 are issued, in registers, while q multiplies: each of a wave's NC loads of a step waits a
+  // whole step, then its 16 bytes go to LDS and the register takes the next position's. Of position q + 1, in slot
+  // (q + 1) % 2, the first quarter of the stores runs during the last quarter of q - 1 (which frees the slot), the others
+  // during the first three quarters of q.
+  constexpr int NC = OA::NDMA + OB::NDMA, Q = MB * NB;
+  u32x4_t st[NC];
+  auto load = [&](int j) {
+    if (j < OA::NDMA) st[j] = ls_load(pa, na, va[j], LA == KC ? c_soff : 0u);
+    else st[j] = ls_load(pb, nb, vb[j - OA::NDMA], LB == KC ? c_soff : 0u);
   };
-  bases();
+  uint8_t* const wr = lds + 16 * lane;
+  auto store = [&](int j, int slot) {
+    const int at = j < OA::NDMA ? wave * (BM * 32) + j * 1024 : BM * 128 + wave * (BN * 32) + (j - OA::NDMA) * 1024;
+    st16(wr + slot * SLOT + at, st[j]);
+  };
+  enter();
 #pragma unroll
-  for (int j = 0; j < OA::NDMA + OB::NDMA; ++j) copy(j, lds0);
+  for (int j = 0; j < NC; ++j) load(j);
   advance();
-  bases();
 #pragma unroll
-  for (int j = 0; j < OA::NDMA + OB::NDMA; ++j) copy(j, lds0 + SLOT);
+  for (int j = 0; j < NC; ++j) {
+    store(j, 0);
+    load(j);
+  }
   advance();
-  asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+#pragma unroll
+  for (int j = 0; j < NC / 4; ++j) {
+    store(j, 1);
+    load(j);
+  }
+  ls_barrier();
 
   f32x16_t acc[MB][NB];
+#pragma unroll
+  for (int q = 0; q < MB * NB; ++q) ls_zero(acc[q / NB][q % NB]);
   u32x4_t fr[2][MB + NB];  // fragments of two quarters: A's, then B's
   auto read = [&](int j, const uint8_t* base, int u) {
     return j < MB ? OA::frag(base, fa, j, u) : OB::frag(base, fb, j - MB, u);
@@ -303,7 +321,7 @@ __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void ls_gemm_kernel(const L
 #pragma unroll
   for (int j = 0; j < MB + NB; ++j) fr[0][j] = read(j, lds, 0);
   LsItem it = item_of(first);
-  int64_t item = first;
+  uint32_t item = first;
   int slot = 0;
 #pragma unroll 1
   for (;;) {
@@ -311,45 +329,32 @@ __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void ls_gemm_kernel(const L
     for (int s = 0; s < it.nk; ++s) {
       const uint8_t* base = lds + slot * SLOT;
       const uint8_t* next = lds + (slot ^ 1) * SLOT;
-      // Quarter u multiplies fr[u % 2] while the next quarter's fragments are read into the other half, one read after
-      // each of the first MFMAs.
-      if (s == 0) {
+      // A quarter multiplies fr[half], reads fragments u of src into the other half after the first MFMAs, in the order of
+      // their use, and stores and reloads quarter `part` of the loads after the others.
+      auto quarter = [&](int half, const uint8_t* src, int u, int part, int to) {
 #pragma unroll
-        for (int q = 0; q < MB * NB; ++q) {
-          ls_mfma<F32, true>(acc[q / NB][q % NB], fr[0][q / NB], fr[0][MB + q % NB]);
-          if (q < MB + NB) fr[1][q] = read(q, base, 1);
+        for (int q = 0; q < Q; ++q) {
+          ls_mfma<F32>(acc[q / NB][q % NB], fr[half][q / NB], fr[half][MB + q % NB]);
+#pragma unroll
+          for (int e = 0; e < MB + NB; ++e)
+            if (e * Q / (MB + NB) / 2 == q) {
+              const int j = e == 0 ? 0 : (e <= NB ? MB + e - 1 : e - NB);
+              fr[half ^ 1][j] = read(j, src, u);
+            }
+#pragma unroll
+          for (int e = 0; e < NC / 4; ++e)
+            if (Q / 2 + e * Q / (NC / 2) == q) {
+              store(part * (NC / 4) + e, to);
+              load(part * (NC / 4) + e);
+            }
         }
-      } else {
-#pragma unroll
-        for (int q = 0; q < MB * NB; ++q) {
-          ls_mfma<F32, false>(acc[q / NB][q % NB], fr[0][q / NB], fr[0][MB + q % NB]);
-          if (q < MB + NB) fr[1][q] = read(q, base, 1);
-        }
-      }
-#pragma unroll
-      for (int q = 0; q < MB * NB; ++q) {
-        ls_mfma<F32, false>(acc[q / NB][q % NB], fr[1][q / NB], fr[1][MB + q % NB]);
-        if (q < MB + NB) fr[0][q] = read(q, base, 2);
-      }
-#pragma unroll
-      for (int q = 0; q < MB * NB; ++q) {
-        ls_mfma<F32, false>(acc[q / NB][q % NB], fr[0][q / NB], fr[0][MB + q % NB]);
-        if (q < MB + NB) fr[1][q] = read(q, base, 3);
-      }
-      bases();
+      };
+      quarter(0, base, 1, 1, slot ^ 1);
+      quarter(1, base, 2, 2, slot ^ 1);
+      quarter(0, base, 3, 3, slot ^ 1);
       advance();
-      // Every wave's reads of this slot are done (its own by lgkmcnt) and the next step's copies have landed.
-      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-      const uint32_t here = lds0 + (uint32_t)slot * SLOT;
-#pragma unroll
-      for (int q = 0; q < MB * NB; ++q) {
-        ls_mfma<F32, false>(acc[q / NB][q % NB], fr[1][q / NB], fr[1][MB + q % NB]);
-        constexpr int PER = (OA::NDMA + OB::NDMA) / (MB * NB);
-        static_assert(PER * MB * NB == OA::NDMA + OB::NDMA, "copies go evenly between the MFMAs");
-#pragma unroll
-        for (int e = 0; e < PER; ++e) copy(q * PER + e, here);
-        if (q < MB + NB) fr[0][q] = read(q, next, 0);
-      }
+      ls_barrier();  // every wave has read this slot and stored the next
+      quarter(1, next, 0, 0, slot);
       slot ^= 1;
     }
     ls_drain();
@@ -367,102 +372,93 @@ __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void ls_gemm_kernel(const L
     for (int j = 0; j < NB; ++j) {
       const int64_t n = nw + 32 * j + (lane & 31);
       const bool n_ok = n < N;
-      f32x16_t v[MB];
-#pragma unroll
-      for (int i = 0; i < MB; ++i) v[i] = ls_take(acc[i][j]);
+      // Per token: where its target lies among the wave's rows, and what the softmax needs.
+      int rel = -1;
+      float lse = 0.0f, g = 1.0f, mx = -__builtin_inff(), sum = 0.0f;
+      int64_t row = n;
       if constexpr (EPI == EPI_LSE) {
-        const int rel = n_ok ? p.tgt[n] - (int)mw : -1;
-        if (mleft < BM / 2) ls_mask(v, mleft - 4 * lh, -__builtin_inff());
-        float mx = -__builtin_inff();
+        if (n_ok) rel = p.tgt[n] - (int)mw;
+      } else if constexpr (EPI == EPI_S) {
+        if (n_ok) {
+          const int64_t r = p.rows[n];
+          rel = p.tgt[n] - (int)p.v0 - (int)mw;
+          lse = p.lse[r];
+          if (p.g_row != nullptr) g = p.g_row[r];
+        }
+      } else if constexpr (F32 && EPI == EPI_OUT) {
+        if (n_ok && p.scatter) row = p.rows[n];
+      }
 #pragma unroll
-        for (int i = 0; i < MB; ++i)
+      for (int i = 0; i < MB; ++i) {
+        f32x16_t v = ls_take(acc[i][j]);
+        ls_zero(acc[i][j]);
+        if constexpr (EPI == EPI_LSE) {
+          if (mleft < BM / 2) ls_mask(v, mleft - 4 * lh - 32 * i, -__builtin_inff());
+          float top = mx;
 #pragma unroll
-          for (int q = 0; q < 16; ++q) mx = fmaxf(mx, v[i][q]);
-        mx = fmaxf(mx, __shfl_xor(mx, 32));
-        const float ref = mx == -__builtin_inff() ? 0.0f : mx;
-        float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+          for (int q = 0; q < 16; ++q) top = fmaxf(top, v[q]);
+          const float ref = top == -__builtin_inff() ? 0.0f : top;
+          float part[2] = {sum * __builtin_amdgcn_exp2f((mx - ref) * LOG2E), 0.0f};
 #pragma unroll
-        for (int i = 0; i < MB; ++i)
-#pragma unroll
-          for (int q = 0; q < 16; ++q) sum[q & 3] += __builtin_amdgcn_exp2f((v[i][q] - ref) * LOG2E);
-        float all_sum = (sum[0] + sum[1]) + (sum[2] + sum[3]);
-        all_sum += __shfl_xor(all_sum, 32);
-        if (n_ok && lh == 0) p.part[((int64_t)it.m * 2 + wm) * p.T + n] = make_float2(mx, all_sum);
-#pragma unroll
-        for (int i = 0; i < MB; ++i) {
+          for (int q = 0; q < 16; ++q) part[q & 1] += __builtin_amdgcn_exp2f((v[q] - ref) * LOG2E);
+          mx = top;
+          sum = part[0] + part[1];
           if (__any((rel >> 5) == i)) {
 #pragma unroll
             for (int q = 0; q < 16; ++q)
-              if (rel == 32 * i + 8 * (q >> 2) + 4 * lh + (q & 3)) p.zt[n] = v[i][q];
+              if (rel == 32 * i + 8 * (q >> 2) + 4 * lh + (q & 3)) p.zt[n] = v[q];
           }
-        }
-      } else {
-        if constexpr (EPI == EPI_S) {
-          const int64_t row = n_ok ? p.rows[n] : 0;
-          const float lse = n_ok ? p.lse[row] : 0.0f;
-          const float g = p.g_row != nullptr && n_ok ? p.g_row[row] : 1.0f;
-          const int rel = n_ok ? p.tgt[n] - (int)p.v0 - (int)mw : -1;
+        } else {
+          if constexpr (EPI == EPI_S) {
 #pragma unroll
-          for (int i = 0; i < MB; ++i) {
-#pragma unroll
-            for (int q = 0; q < 16; ++q) v[i][q] = __builtin_amdgcn_exp2f((v[i][q] - lse) * LOG2E);
+            for (int q = 0; q < 16; ++q) v[q] = __builtin_amdgcn_exp2f((v[q] - lse) * LOG2E);
             if (__any((rel >> 5) == i)) {
 #pragma unroll
               for (int q = 0; q < 16; ++q)
-                if (rel == 32 * i + 8 * (q >> 2) + 4 * lh + (q & 3)) v[i][q] -= 1.0f;
+                if (rel == 32 * i + 8 * (q >> 2) + 4 * lh + (q & 3)) v[q] -= 1.0f;
             }
-            if (p.g_row != nullptr) v[i] *= g;
+            if (p.g_row != nullptr) v *= g;
+            if (mleft < BM / 2) ls_mask(v, mleft - 4 * lh - 32 * i, 0.0f);
+          } else if (EPI == EPI_OUT) {
+            v *= scale;
           }
-          if (mleft < BM / 2) ls_mask(v, mleft - 4 * lh, 0.0f);
-        } else if (EPI == EPI_OUT) {
-#pragma unroll
-          for (int i = 0; i < MB; ++i) v[i] *= scale;
-        }
-        const int mstore = EPI == EPI_S ? BM / 2 : mleft;  // s: whole tiles, the others' rows are a multiple of 64
-        if constexpr (F32 || EPI == EPI_ACC) {
-          if (n_ok) {
-            const int64_t row = EPI == EPI_ACC ? (int64_t)it.part * p.N + n
-                                               : (EPI == EPI_OUT && p.scatter ? (int64_t)p.rows[n] : n);
-#pragma unroll
-            for (int i = 0; i < MB; ++i)
+          const int mstore = EPI == EPI_S ? BM / 2 : mleft;  // s: whole tiles; the others' rows are a multiple of 64
+          if constexpr (F32 || EPI == EPI_ACC) {
+            if (n_ok && 32 * i < mstore) {
+              const int64_t r = EPI == EPI_ACC ? (int64_t)it.part * p.N + n : row;
 #pragma unroll
               for (int q4 = 0; q4 < 4; ++q4) {
-                const int r0 = 32 * i + 8 * q4 + 4 * lh;
-                if (r0 >= mstore) continue;
-                f32x4_t f = {v[i][4 * q4], v[i][4 * q4 + 1], v[i][4 * q4 + 2], v[i][4 * q4 + 3]};
-                f32x4_t* o = reinterpret_cast<f32x4_t*>(static_cast<float*>(p.out) + row * p.ldo + mw + r0);
+                f32x4_t f = {v[4 * q4], v[4 * q4 + 1], v[4 * q4 + 2], v[4 * q4 + 3]};
+                f32x4_t* o = reinterpret_cast<f32x4_t*>(static_cast<float*>(p.out) + r * p.ldo + mw + 32 * i + 8 * q4 + 4 * lh);
                 if (EPI == EPI_ACC && p.add) f += *o;
                 *o = f;
               }
-          }
-        } else {
-          // Through the wave's staging area, 32 rows of out by BM / 2 columns, so that stores write whole lines: 16-byte chunk
-          // c of row r at c ^ r.
-          constexpr int PITCH = BM, CH = BM / 16;  // bytes and chunks of a row
-          uint8_t* const st = stage + wave * 32 * PITCH;
-          const int r = lane & 31;
-#pragma unroll
-          for (int i = 0; i < MB; ++i)
+            }
+          } else {
+            // Through the wave's staging area, 32 rows of out by BM / 2 columns, so that stores write whole lines: 16-byte
+            // chunk c of row r at c ^ r.
+            const int r = lane & 31;
 #pragma unroll
             for (int q4 = 0; q4 < 4; ++q4)
-              *reinterpret_cast<uint2*>(st + r * PITCH + 16 * ((4 * i + q4) ^ (r & (CH - 1))) + 8 * lh) =
-                  make_uint2(pack_bf16x2(v[i][4 * q4], v[i][4 * q4 + 1]),
-                             pack_bf16x2(v[i][4 * q4 + 2], v[i][4 * q4 + 3]));
-          constexpr int RPI = 64 / CH;  // rows of a store
-          const int c = lane % CH;
-          u32x4_t w[32 / RPI];
-#pragma unroll
-          for (int k = 0; k < 32 / RPI; ++k) {
-            const int rr = k * RPI + lane / CH;
-            w[k] = ld16(st + rr * PITCH + 16 * (c ^ (rr & (CH - 1))));
+              *reinterpret_cast<uint2*>(stw + r * BM + 16 * ((4 * i + q4) ^ (r & (CH - 1))) + 8 * lh) =
+                  make_uint2(pack_bf16x2(v[4 * q4], v[4 * q4 + 1]), pack_bf16x2(v[4 * q4 + 2], v[4 * q4 + 3]));
           }
+        }
+      }
+      if constexpr (EPI == EPI_LSE) {
+        const float mx2 = __shfl_xor(mx, 32), sum2 = __shfl_xor(sum, 32);
+        lse_join(mx, sum, mx2, sum2);
+        if (n_ok && lh == 0) p.part[((int64_t)it.m * 2 + wm) * p.T + n] = make_float2(mx, sum);
+      } else if constexpr (STAGED) {
+        const int mstore = EPI == EPI_S ? BM / 2 : mleft, c = lane % CH;
 #pragma unroll
-          for (int k = 0; k < 32 / RPI; ++k) {
-            const int64_t nn = nw + 32 * j + k * RPI + lane / CH;
-            if (nn < N && 8 * c < mstore) {
-              const int64_t row = EPI == EPI_OUT && p.scatter ? (int64_t)p.rows[nn] : nn;
-              st16(static_cast<uint16_t*>(p.out) + row * p.ldo + mw + 8 * c, w[k]);
-            }
+        for (int k = 0; k < 32 / RPI; ++k) {
+          const int rr = k * RPI + lane / CH;
+          const u32x4_t w = ld16(stw + rr * BM + 16 * (c ^ (rr & (CH - 1))));
+          const int64_t nn = nw + 32 * j + rr;
+          if (nn < N && 8 * c < mstore) {
+            const int64_t r = EPI == EPI_OUT && p.scatter ? (int64_t)p.rows[nn] : nn;
+            st16(static_cast<uint16_t*>(p.out) + r * p.ldo + mw + 8 * c, w);
           }
         }
       }
@@ -471,8 +467,6 @@ __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void ls_gemm_kernel(const L
     if (item >= total) break;
     it = item_of(item);
   }
-  // The last copies (of nothing) complete before the block's LDS is released.
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 }
 
 // Partition of the rows: rows[0 .. n-1] those that count, ascending, rows[n .. T-1] the ignored ones, *count = n, tgt[i]
@@ -532,13 +526,6 @@ __global__ __launch_bounds__(256) void ls_gather_kernel(const uint8_t* __restric
     if (i < n) st16(xc + i * bytes + c, ld16(x + r * bytes + c));
     else st16(zero + r * bytes + c, (u32x4_t){0u, 0u, 0u, 0u});
   }
-}
-
-__device__ __forceinline__ void lse_join(float& m, float& s, float m2, float s2) {
-  const float top = fmaxf(m, m2);
-  const float ref = top == -__builtin_inff() ? 0.0f : top;
-  s = s * __builtin_amdgcn_exp2f((m - ref) * LOG2E) + s2 * __builtin_amdgcn_exp2f((m2 - ref) * LOG2E);
-  m = top;
 }
 
 // lse and loss of 64 rows per block from their partial maxima and sums (16 waves share the entries), the block's sum of losses
