@@ -29,7 +29,7 @@ namespace q38 {
 namespace {
 
 enum { KC = 0, KS = 1 };
-enum { EPI_LSE = 0, EPI_S = 1, EPI_OUT = 2, EPI_ACC = 3 };
+enum { EPI_LSE = 0, EPI_S = 1, EPI_OUT = 2 };
 
 constexpr float LOG2E = 1.4426950408889634f;
 
@@ -44,6 +44,15 @@ __device__ __forceinline__ u32x4_t ls_load(const uint8_t* p, int64_t bytes, uint
   return __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(r, (int)voff, (int)soff, 0));
 }
 
+__device__ __forceinline__ void ls_dma(const uint8_t* p, int64_t bytes, uint32_t voff, uint32_t soff, uint32_t lds) {
+  const uint64_t a = (uint64_t)(uintptr_t)p;
+  const uint32_t n = bytes <= 0 ? 0u : (bytes >= 0xffffffffll ? 0xffffffffu : (uint32_t)bytes);
+  const u32x4_t r = {uniform((uint32_t)a), uniform((uint32_t)(a >> 32) & 0xffffu), uniform(n), 0x00020000u};
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(lds), "v"(voff), "s"(r), "s"(soff) : "memory", "m0");
+}
+__device__ __forceinline__ uint32_t ls_lds_addr(const void* p) {
+  return uniform((uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)p);
+}
 // This wave's LDS operations are done, and so are the others'.
 __device__ __forceinline__ void ls_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
@@ -158,29 +167,69 @@ struct LsParams {
   int64_t lda, ldb;      // bytes between rows
   int64_t M, N, K;       // extents (the tokens' one: an upper bound)
   int64_t m_rows;        // rows (KC) or columns of A that exist, <= M: the others of M multiply zeros
-  const int32_t* count;  // tokens that count (device), NULL: all
+  const int32_t* count;  // tokens that count (device)
   int64_t T;             // tokens of the call
-  int parts;             // K split into this many runs of whole steps
-  // epilogues
-  int64_t v0;            // EPI_S: first vocabulary row of the piece
-  float2* part;          // EPI_LSE: {max, sum} [2 ceil(M / BM), T]
-  const int32_t* tgt;    // EPI_LSE, EPI_S: target per counted token
-  float* zt;             // EPI_LSE: the target's logit
   const int32_t* rows;   // original row of a counted token
-  const float* lse;      // EPI_S: by original row
-  const float* g_row;    // EPI_S: gradient per original row, or NULL
-  void* out;             // EPI_S: s; EPI_OUT: the gradient; EPI_ACC: fp32 [parts, N, M]
+  // EPI_LSE, EPI_S
+  int64_t v0;            // first vocabulary row of the piece
+  float2* part;          // {max, sum} [2 ceil(M / BM), T]
+  const int32_t* tgt;    // target per counted token
+  float* zt;             // the target's logit
+  const float* lse;      // by original row
+  const float* g_row;    // gradient per original row, or NULL
+  // EPI_S, EPI_OUT
+  void* out;             // s, or the gradient
   int64_t ldo;           // elements between rows of out
-  const float* g_scale;  // EPI_OUT: the loss's gradient (NULL: 1)
-  const float* r_scale;  // EPI_OUT: the reduction's factor (NULL: 1)
-  bool scatter;          // EPI_OUT: rows through `rows`
-  bool add;              // EPI_ACC: add to what is there
+  const float* g_scale;  // the loss's gradient (NULL: 1)
+  const float* r_scale;  // the reduction's factor (NULL: 1)
+  bool scatter;          // rows of out through `rows`
+  float* acc;            // tiles' sums over the pieces so far (fp32, in the accumulators' own order), or NULL
+  bool first, last;      // piece: acc holds nothing yet; out is written (else acc)
+  float* split;          // partial sums of split tiles, a tile after another
+  uint32_t slots;        // workgroups that run at once
 };
 
-// Position of a work item: tile (m0, n0) and its K steps.
+// How a product's tiles are dealt to `slots` workgroups: whole rounds of them take their tile over all of K; the `rest` of a last,
+// partial round is split over K into `parts` runs, so that it ends when about as many workgroups are done. In steps' time
+// (1.7 us on 256 x 256): an item costs 3 beside its own, a partial sum of a tile 6 to write and, with the others, 10 to join.
+struct LsPlan {
+  uint32_t full, rest;
+  int parts, per;  // per: steps of a part
+};
+constexpr int LS_PARTS = 8;  // and rest * parts at most twice the slots: the size of the partial sums' buffer
+__host__ __device__ inline LsPlan ls_plan(uint32_t tiles, int steps, uint32_t slots) {
+  LsPlan pl = {tiles, 0, 1, steps};
+  const uint32_t rest = tiles % slots;
+  if (rest == 0) return pl;
+  uint32_t best = 0;
+  for (int p = 1; p <= LS_PARTS && p <= steps && (p == 1 || rest * p <= 2 * slots); ++p) {
+    const uint32_t per = (uint32_t)(steps + p - 1) / p, load = rest * p;
+    const uint32_t cost = (load + slots - 1) / slots * (per + 3) + (p > 1 ? 4 + 16 * load / slots : 0);
+    if (p == 1 || cost < best) {
+      best = cost;
+      pl.parts = p;
+      pl.per = (int)per;
+    }
+  }
+  if (pl.parts > 1) {
+    pl.full = tiles - rest;
+    pl.rest = rest;
+  }
+  return pl;
+}
+
+// Position of a work item: tile (m, n) and its K steps; part: its index among the split tiles' partial sums, or -1.
 struct LsItem {
   int m, n, part, k0, nk;
+  uint32_t tile;
 };
+
+__device__ __forceinline__ void ls_tile(uint32_t t, uint32_t ntm, uint32_t ntn, int& m, int& n) {
+  const uint32_t grp = t / (8u * ntn), rem = t - grp * 8u * ntn;
+  const uint32_t gm = min(8u, ntm - grp * 8u), q = rem / gm;
+  n = (int)q;
+  m = (int)(grp * 8u + rem - q * gm);
+}
 
 template <bool F32, int BM, int BN, int LA, int LB, int EPI>
 __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void ls_gemm_kernel(const LsParams p) {
@@ -201,30 +250,32 @@ __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void ls_gemm_kernel(const L
   uint8_t* const stw = stage + (STAGED ? wave * 32 * BM : 0);
 
   // Tokens are N of z^T and dx^T, K of dW^T.
-  const int64_t cnt = p.count != nullptr ? (int64_t)load_uniform(p.count) : p.T;
+  const int64_t cnt = (int64_t)load_uniform(p.count);
   const bool all = cnt >= p.T;
-  const bool tok_k = EPI == EPI_ACC ? LB == KS : (EPI == EPI_OUT ? LB == KS : false);
+  constexpr bool tok_k = LB == KS;
   const int64_t N = tok_k ? p.N : cnt, K = tok_k ? cnt : p.K;
   const uint8_t* const A = tok_k && all && p.alt != nullptr ? p.alt : p.A;
   const uint8_t* const B = !tok_k && all && p.alt != nullptr ? p.alt : p.B;
   const uint32_t ntm = (uint32_t)((p.M + BM - 1) / BM), ntn = (uint32_t)((N + BN - 1) / BN);
-  const int steps = (int)((K + BK - 1) / BK), per = (steps + p.parts - 1) / p.parts;
-  const uint32_t tiles = ntm * ntn, total = tiles * (uint32_t)p.parts;  // < 2^31: the callers' limits on T and V
+  const int steps = (int)((K + BK - 1) / BK);
+  const uint32_t tiles = ntm * ntn;  // < 2^31: the callers' limits on T and V
 
   // Work items of neighbouring blocks on an XCD are neighbouring tiles: 8 tiles of M by as many of N as it has room for.
   const uint32_t G = gridDim.x;
   const uint32_t first = (G & 7) == 0 ? (blockIdx.x & 7) * (G >> 3) + (blockIdx.x >> 3) : blockIdx.x;
+  const LsPlan pl = EPI == EPI_OUT ? ls_plan(tiles, steps, p.slots) : LsPlan{tiles, 0, 1, steps};
+  const uint32_t total = pl.full + pl.rest * pl.parts;
   if (first >= total) return;
   auto item_of = [&](uint32_t L) {
-    LsItem it;
-    const uint32_t part = L / tiles, t = L - part * tiles;
-    const uint32_t grp = t / (8u * ntn), rem = t - grp * 8u * ntn;
-    const uint32_t gm = min(8u, ntm - grp * 8u), n = rem / gm;
-    it.part = (int)part;
-    it.n = (int)n;
-    it.m = (int)(grp * 8u + rem - n * gm);
-    it.k0 = it.part * per;
-    it.nk = max(1, min(per, steps - it.k0));  // a part without steps multiplies zeros
+    LsItem it = {0, 0, -1, 0, max(1, steps), L};  // no step at all: one of zeros
+    if (EPI == EPI_OUT && L >= pl.full) {
+      const uint32_t q = L - pl.full, part = q / pl.rest;
+      it.part = (int)q;
+      it.tile = pl.full + q - part * pl.rest;
+      it.k0 = (int)part * pl.per;
+      it.nk = max(1, min(pl.per, steps - it.k0));
+    }
+    ls_tile(it.tile, ntm, ntn, it.m, it.n);
     return it;
   };
 
@@ -279,37 +330,26 @@ __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void ls_gemm_kernel(const L
     enter();
   };
 
-  // Loads of stream position q + 3 are issued, in registers, while q multiplies: each of a wave's NC loads of a step waits a
-  // whole step, then its 16 bytes go to LDS and the register takes the next position's. Of position q + 1, in slot
-  // (q + 1) % 2, the first quarter of the stores runs during the last quarter of q - 1 (which frees the slot), the others
-  // during the first three quarters of q.
+  // Position q of the stream lies in slot q % 2. Its slot is free once every wave has read its last fragments: in the
+  // last quarter of q the first half of position q + 2 is copied over it, in the first quarter of q + 1 the second,
+  // and both have at least two quarters to arrive. (All in one quarter is 5 % slower, over three or four quarters 2 %
+  // slower; the same loads through registers, a whole step ahead of their LDS stores, 2 % slower: at full rate the chip's
+  // power decides, and the registers' way costs more of it.)
   constexpr int NC = OA::NDMA + OB::NDMA, Q = MB * NB;
-  u32x4_t st[NC];
-  auto load = [&](int j) {
-    if (j < OA::NDMA) st[j] = ls_load(pa, na, va[j], LA == KC ? c_soff : 0u);
-    else st[j] = ls_load(pb, nb, vb[j - OA::NDMA], LB == KC ? c_soff : 0u);
-  };
-  uint8_t* const wr = lds + 16 * lane;
-  auto store = [&](int j, int slot) {
-    const int at = j < OA::NDMA ? wave * (BM * 32) + j * 1024 : BM * 128 + wave * (BN * 32) + (j - OA::NDMA) * 1024;
-    st16(wr + slot * SLOT + at, st[j]);
+  constexpr int C3 = NC / 2, C0 = NC - C3;
+  const uint32_t lds0 = ls_lds_addr(lds);
+  auto copy = [&](int j, int slot) {
+    const uint32_t to = lds0 + (uint32_t)slot * SLOT;
+    if (j < OA::NDMA) ls_dma(pa, na, va[j], LA == KC ? c_soff : 0u, to + wave * (BM * 32) + j * 1024);
+    else ls_dma(pb, nb, vb[j - OA::NDMA], LB == KC ? c_soff : 0u, to + BM * 128 + wave * (BN * 32) + (j - OA::NDMA) * 1024);
   };
   enter();
 #pragma unroll
-  for (int j = 0; j < NC; ++j) load(j);
+  for (int j = 0; j < NC; ++j) copy(j, 0);
   advance();
 #pragma unroll
-  for (int j = 0; j < NC; ++j) {
-    store(j, 0);
-    load(j);
-  }
-  advance();
-#pragma unroll
-  for (int j = 0; j < NC / 4; ++j) {
-    store(j, 1);
-    load(j);
-  }
-  ls_barrier();
+  for (int j = 0; j < C3; ++j) copy(j, 1);
+  asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(C3) : "memory");
 
   f32x16_t acc[MB][NB];
 #pragma unroll
@@ -331,7 +371,7 @@ __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void ls_gemm_kernel(const L
       const uint8_t* next = lds + (slot ^ 1) * SLOT;
       // A quarter multiplies fr[half], reads fragments u of src into the other half after the first MFMAs, in the order of
       // their use, and stores and reloads quarter `part` of the loads after the others.
-      auto quarter = [&](int half, const uint8_t* src, int u, int part, int to) {
+      auto quarter = [&](int half, const uint8_t* src, int u, int from, int cn, int to) {
 #pragma unroll
         for (int q = 0; q < Q; ++q) {
           ls_mfma<F32>(acc[q / NB][q % NB], fr[half][q / NB], fr[half][MB + q % NB]);
@@ -342,19 +382,16 @@ __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void ls_gemm_kernel(const L
               fr[half ^ 1][j] = read(j, src, u);
             }
 #pragma unroll
-          for (int e = 0; e < NC / 4; ++e)
-            if (Q / 2 + e * Q / (NC / 2) == q) {
-              store(part * (NC / 4) + e, to);
-              load(part * (NC / 4) + e);
-            }
+          for (int e = cn * q / Q; e < cn * (q + 1) / Q; ++e) copy(from + e, to);
         }
       };
-      quarter(0, base, 1, 1, slot ^ 1);
-      quarter(1, base, 2, 2, slot ^ 1);
-      quarter(0, base, 3, 3, slot ^ 1);
+      quarter(0, base, 1, C3, C0, slot ^ 1);
+      quarter(1, base, 2, 0, 0, slot ^ 1);
+      quarter(0, base, 3, 0, 0, slot ^ 1);
       advance();
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       ls_barrier();  // every wave has read this slot and stored the next
-      quarter(1, next, 0, 0, slot);
+      quarter(1, next, 0, 0, C3, slot);
       slot ^= 1;
     }
     ls_drain();
@@ -364,7 +401,8 @@ __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void ls_gemm_kernel(const L
     const int lh = lane >> 5;
     const int mleft = (int)min((int64_t)(BM / 2), p.m_rows - mw);  // rows of the wave that exist (may be <= 0)
     float scale = 1.0f;
-    if (EPI == EPI_OUT) {
+    const bool to_out = EPI != EPI_OUT || (it.part < 0 && p.last);  // else to the partial sums or the pieces' sums
+    if (EPI == EPI_OUT && to_out) {
       if (p.g_scale != nullptr) scale *= *p.g_scale;
       if (p.r_scale != nullptr) scale *= *p.r_scale;
     }
@@ -419,20 +457,35 @@ __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void ls_gemm_kernel(const L
             }
             if (p.g_row != nullptr) v *= g;
             if (mleft < BM / 2) ls_mask(v, mleft - 4 * lh - 32 * i, 0.0f);
-          } else if (EPI == EPI_OUT) {
+          } else {
+            // The accumulators' own order: block (i, j) of wave w at 1024 ((w MB + i) NB + j), its quarters 256 apart, 4 per lane.
+            const int64_t at = (((int64_t)wave * MB + i) * NB + j) * 1024 + 4 * lane;
+            if (it.part < 0 && !p.first) {
+              const float* a = p.acc + (int64_t)it.tile * (BM * BN) + at;
+#pragma unroll
+              for (int q4 = 0; q4 < 4; ++q4) {
+                const f32x4_t f = *reinterpret_cast<const f32x4_t*>(a + 256 * q4);
+#pragma unroll
+                for (int q = 0; q < 4; ++q) v[4 * q4 + q] += f[q];
+              }
+            }
+            if (!to_out) {
+              float* a = (it.part < 0 ? p.acc + (int64_t)it.tile * (BM * BN) : p.split + (int64_t)it.part * (BM * BN)) + at;
+#pragma unroll
+              for (int q4 = 0; q4 < 4; ++q4)
+                *reinterpret_cast<f32x4_t*>(a + 256 * q4) =
+                    (f32x4_t){v[4 * q4], v[4 * q4 + 1], v[4 * q4 + 2], v[4 * q4 + 3]};
+              continue;
+            }
             v *= scale;
           }
           const int mstore = EPI == EPI_S ? BM / 2 : mleft;  // s: whole tiles; the others' rows are a multiple of 64
-          if constexpr (F32 || EPI == EPI_ACC) {
+          if constexpr (F32) {
             if (n_ok && 32 * i < mstore) {
-              const int64_t r = EPI == EPI_ACC ? (int64_t)it.part * p.N + n : row;
 #pragma unroll
-              for (int q4 = 0; q4 < 4; ++q4) {
-                f32x4_t f = {v[4 * q4], v[4 * q4 + 1], v[4 * q4 + 2], v[4 * q4 + 3]};
-                f32x4_t* o = reinterpret_cast<f32x4_t*>(static_cast<float*>(p.out) + r * p.ldo + mw + 32 * i + 8 * q4 + 4 * lh);
-                if (EPI == EPI_ACC && p.add) f += *o;
-                *o = f;
-              }
+              for (int q4 = 0; q4 < 4; ++q4)
+                *reinterpret_cast<f32x4_t*>(static_cast<float*>(p.out) + row * p.ldo + mw + 32 * i + 8 * q4 + 4 * lh) =
+                    (f32x4_t){v[4 * q4], v[4 * q4 + 1], v[4 * q4 + 2], v[4 * q4 + 3]};
             }
           } else {
             // Through the wave's staging area, 32 rows of out by BM / 2 columns, so that stores write whole lines: 16-byte
@@ -450,6 +503,7 @@ __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void ls_gemm_kernel(const L
         lse_join(mx, sum, mx2, sum2);
         if (n_ok && lh == 0) p.part[((int64_t)it.m * 2 + wm) * p.T + n] = make_float2(mx, sum);
       } else if constexpr (STAGED) {
+        if (!to_out) continue;
         const int mstore = EPI == EPI_S ? BM / 2 : mleft, c = lane % CH;
 #pragma unroll
         for (int k = 0; k < 32 / RPI; ++k) {
@@ -467,6 +521,7 @@ __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void ls_gemm_kernel(const L
     if (item >= total) break;
     it = item_of(item);
   }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 }
 
 // Partition of the rows: rows[0 .. n-1] those that count, ascending, rows[n .. T-1] the ignored ones, *count = n, tgt[i]
@@ -610,68 +665,103 @@ __global__ __launch_bounds__(256) void ls_reduce_kernel(const double* __restrict
   }
 }
 
-// out[row] = scale * sum over the parts of acc [parts, N, M], row = rows[i] (rows NULL: i), i < min(N, *count).
-template <typename E>
-__global__ __launch_bounds__(256) void ls_join_kernel(const float* __restrict__ acc, int parts, int64_t N, int M,
-                                                      const int32_t* __restrict__ count,
-                                                      const int32_t* __restrict__ rows,
-                                                      const float* __restrict__ g_scale,
-                                                      const float* __restrict__ r_scale, E* __restrict__ out) {
-  const int64_t n = count != nullptr ? min(N, (int64_t)load_uniform(count)) : N;
-  const int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x, per = M / 4;
-  const int64_t i = q / per;
-  if (i >= n) return;
-  const int c = (int)(q - i * per) * 4;
-  f32x4_t s = *reinterpret_cast<const f32x4_t*>(acc + i * M + c);
-  for (int p = 1; p < parts; ++p) s += *reinterpret_cast<const f32x4_t*>(acc + ((int64_t)p * N + i) * M + c);
+// The split tiles of a product (ls_gemm_kernel with the same parameters): their parts in order and the earlier pieces' sums,
+// to out or to the pieces' sums. A thread takes 32 consecutive m of one n, in the accumulators' order 4 at a time.
+template <typename E, int BM, int BN, bool TOK_K>
+__global__ __launch_bounds__(256) void ls_join_kernel(const LsParams p) {
+  constexpr int BK = 128 / sizeof(E), NB = BN / 64, PER = BM * BN / 32;  // threads of a tile
+  const int64_t cnt = (int64_t)load_uniform(p.count);
+  const int64_t N = TOK_K ? p.N : cnt, K = TOK_K ? cnt : p.K;
+  const uint32_t ntm = (uint32_t)((p.M + BM - 1) / BM), ntn = (uint32_t)((N + BN - 1) / BN);
+  const LsPlan pl = ls_plan(ntm * ntn, (int)((K + BK - 1) / BK), p.slots);
   float scale = 1.0f;
-  if (g_scale != nullptr) scale *= *g_scale;
-  if (r_scale != nullptr) scale *= *r_scale;
-  s *= scale;
-  E* o = out + (rows != nullptr ? (int64_t)rows[i] : i) * M + c;
-  if constexpr (sizeof(E) == 4) *reinterpret_cast<f32x4_t*>(o) = s;
-  else *reinterpret_cast<uint2*>(o) = make_uint2(pack_bf16x2(s[0], s[1]), pack_bf16x2(s[2], s[3]));
-}
-
-template <bool F32, int BM, int BN, int LA, int LB, int EPI>
-hipError_t ls_gemm(const LsParams& p, hipStream_t st) {
-  const int64_t items = ((p.M + BM - 1) / BM) * ((p.N + BN - 1) / BN) * p.parts;
-  const int64_t most = (int64_t)device_cus() * (BM == 256 ? 1 : 2);
-  const unsigned grid = (unsigned)(items < most ? items : most);
-  if (grid == 0) return hipSuccess;
-  hipLaunchKernelGGL((ls_gemm_kernel<F32, BM, BN, LA, LB, EPI>), dim3(grid), dim3(256), 0, st, p);
-  return hipGetLastError();
+  if (p.last && p.g_scale != nullptr) scale *= *p.g_scale;
+  if (p.last && p.r_scale != nullptr) scale *= *p.r_scale;
+  for (uint32_t id = blockIdx.x * 256 + threadIdx.x; id < pl.rest * PER; id += gridDim.x * 256) {
+    const uint32_t q = id / PER, in = id - q * PER;
+    const int ln = in & 31, blk = in >> 5;  // block (w MB + i) NB + j
+    int tm, tn;
+    ls_tile(pl.full + q, ntm, ntn, tm, tn);
+    const int j = blk % NB, i = blk / NB % (BM / 64), w = blk / NB / (BM / 64);
+    const int64_t m = (int64_t)tm * BM + (w >> 1) * (BM / 2) + 32 * i, n = (int64_t)tn * BN + (w & 1) * (BN / 2) + 32 * j + ln;
+    if (m >= p.M || n >= N) continue;
+    f32x4_t v[8];  // m = 8 (k / 2) + 4 (k % 2)
+    const int64_t at = (int64_t)blk * 1024 + 4 * ln;
+    const float* a = p.split + (int64_t)q * (BM * BN) + at;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = *reinterpret_cast<const f32x4_t*>(a + 256 * (k >> 1) + 128 * (k & 1));
+    for (int part = 1; part < pl.parts; ++part) {
+      a += (int64_t)pl.rest * (BM * BN);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] += *reinterpret_cast<const f32x4_t*>(a + 256 * (k >> 1) + 128 * (k & 1));
+    }
+    float* const c = p.acc + (int64_t)(pl.full + q) * (BM * BN) + at;
+    if (!p.first) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] += *reinterpret_cast<const f32x4_t*>(c + 256 * (k >> 1) + 128 * (k & 1));
+    }
+    if (!p.last) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) *reinterpret_cast<f32x4_t*>(c + 256 * (k >> 1) + 128 * (k & 1)) = v[k];
+      continue;
+    }
+    E* const o = static_cast<E*>(p.out) + (p.scatter ? (int64_t)p.rows[n] : n) * p.ldo + m;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      v[k] *= scale;
+      if constexpr (sizeof(E) == 4) *reinterpret_cast<f32x4_t*>(o + 4 * k) = v[k];
+      else if (k & 1)
+        st16(o + 4 * (k - 1), (u32x4_t){pack_bf16x2(v[k - 1][0], v[k - 1][1]), pack_bf16x2(v[k - 1][2], v[k - 1][3]),
+                                        pack_bf16x2(v[k][0], v[k][1]), pack_bf16x2(v[k][2], v[k][3])});
+    }
+  }
 }
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// Tiles of 256 x 256 where they fill at least half the CUs, else of 128 x 128.
+uint32_t ls_slots(bool big) { return (uint32_t)device_cus() * (big ? 1 : 2); }
+
+template <bool F32, int BM, int BN, int LA, int LB, int EPI>
+hipError_t ls_gemm(LsParams p, hipStream_t st) {
+  p.slots = ls_slots(BM == 256);
+  const int64_t tiles = ceil_div(p.M, BM) * ceil_div(p.N, BN);
+  const int64_t items = EPI == EPI_OUT ? tiles * LS_PARTS : tiles;
+  const unsigned grid = (unsigned)(items < p.slots ? items : p.slots);
+  if (grid == 0) return hipSuccess;
+  hipLaunchKernelGGL((ls_gemm_kernel<F32, BM, BN, LA, LB, EPI>), dim3(grid), dim3(256), 0, st, p);
+  const hipError_t e = hipGetLastError();
+  if (EPI != EPI_OUT || e != hipSuccess) return e;
+  using E = typename std::conditional<F32, float, uint16_t>::type;
+  hipLaunchKernelGGL((ls_join_kernel<E, BM, BN, LB == KS>), dim3(1024), dim3(256), 0, st, p);
+  return hipGetLastError();
+}
+
+// Products over the vocabulary: tiles of 256 x 256 where they fill at least half the CUs, else of 128 x 128.
 bool big_tiles(int64_t M, int64_t N) { return ceil_div(M, 256) * ceil_div(N, 256) * 2 >= device_cus(); }
 
-// Runs that K's steps are split into, so that the tiles fill the CUs.
-int split_parts(int64_t M, int64_t N, int64_t steps) {
-  const bool big = big_tiles(M, N);
-  const int64_t tiles = ceil_div(M, big ? 256 : 128) * ceil_div(N, big ? 256 : 128);
-  const int64_t slots = (int64_t)device_cus() * (big ? 1 : 2);
-  int best = 1;
-  double cost = 0.0;
-  for (int p = 1; p <= 16 && p <= steps; ++p) {
-    const double c = (double)ceil_div(tiles * p, slots) * ((double)ceil_div(steps, p) + 4.0) + (p > 1 ? 2.0 * p : 0.0);
-    if (p == 1 || c < cost) {
-      best = p;
-      cost = c;
-    }
-  }
-  return best;
+// Gradients, whose tiles can be split over K: large tiles where each CU has at least 12 steps of them.
+bool big_tiles_k(int64_t M, int64_t N, int64_t steps) {
+  return ceil_div(M, 256) * ceil_div(N, 256) * steps >= (int64_t)12 * device_cus();
+}
+
+// Tiles of partial sums that a product may need, and of its running sums.
+size_t split_bytes(int64_t M, int64_t N, bool big) {
+  const int64_t b = big ? 256 : 128, tiles = ceil_div(M, b) * ceil_div(N, b), most = 2 * (int64_t)ls_slots(big);
+  return 4 * (size_t)(b * b) * (size_t)(tiles * LS_PARTS < most ? tiles * LS_PARTS : most);
+}
+size_t acc_bytes(int64_t M, int64_t N, bool big) {
+  const int64_t b = big ? 256 : 128;
+  return 4 * (size_t)(b * b) * (size_t)(ceil_div(M, b) * ceil_div(N, b));
 }
 
 size_t up(size_t v) { return (v + 255) / 256 * 256; }
 
 struct Layout {
-  size_t rows, tgt, count, xc, part, zt, bsum, bn, s, acc_x, acc_w, end;
+  size_t rows, tgt, count, xc, part, zt, bsum, bn, s, acc, split, end;
   int entries;             // of the forward's partial sums
   int64_t piece;           // vocabulary rows of a piece (multiple of 256)
-  int pieces, parts_x, parts_w;
+  int pieces;
+  bool big_x, big_w;       // tiles of dx's and dw's products
   bool gather;
 };
 
@@ -706,10 +796,12 @@ Layout layout(int64_t T, int h, int V, bool f32, bool fwd, bool need_x, bool nee
     l.pieces = (int)ceil_div(vt, pt);
     l.piece = pt * 256;
     l.s = take(esz * (size_t)T * l.piece);
-    l.parts_x = split_parts(h, T, l.piece / (f32 ? 32 : 64));
-    l.parts_w = split_parts(h, l.piece < V ? l.piece : V, ceil_div(T, f32 ? 32 : 64));
-    l.acc_x = take(need_x && (l.parts_x > 1 || l.pieces > 1) ? 4 * (size_t)l.parts_x * T * h : 0);
-    l.acc_w = take(need_w && l.parts_w > 1 ? 4 * (size_t)l.parts_w * l.piece * h : 0);
+    const int64_t bk = f32 ? 32 : 64;
+    l.big_x = big_tiles_k(h, T, l.piece / bk);
+    l.big_w = big_tiles_k(h, l.piece, ceil_div(T, bk));
+    l.acc = take(need_x && l.pieces > 1 ? acc_bytes(h, T, l.big_x) : 0);
+    const size_t sx = need_x ? split_bytes(h, T, l.big_x) : 0, sw = need_w ? split_bytes(h, l.piece, l.big_w) : 0;
+    l.split = take(sx > sw ? sx : sw);
   }
   l.end = off;
   return l;
@@ -768,7 +860,6 @@ hipError_t ce_forward(const void* x, const void* w, const void* targets, bool id
   p.N = p.T = T;
   p.K = h;
   p.count = count;
-  p.parts = 1;
   p.part = at<float2>(ws, l.part);
   p.tgt = tgt;
   p.zt = at<float>(ws, l.zt);
@@ -789,7 +880,6 @@ template <bool F32>
 hipError_t ce_backward(const float* g, bool g_rows, const float* r_scale, const void* x, const void* w,
                        const void* targets, bool idx64, int64_t ignore, const float* lse, void* dx, void* dw, int64_t T,
                        int h, int V, void* ws, hipStream_t st) {
-  using E = typename std::conditional<F32, float, uint16_t>::type;
   const Layout l = layout(T, h, V, F32, false, dx != nullptr, dw != nullptr);
   int32_t* rows = at<int32_t>(ws, l.rows);
   int32_t* tgt = at<int32_t>(ws, l.tgt);
@@ -808,7 +898,6 @@ hipError_t ce_backward(const float* g, bool g_rows, const float* r_scale, const 
     p.T = T;
     p.count = count;
     p.rows = rows;
-    p.parts = 1;
     // s [T, pitch]
     p.A = wp;
     p.B = xc;
@@ -825,67 +914,39 @@ hipError_t ce_backward(const float* g, bool g_rows, const float* r_scale, const 
     p.M = pitch;  // whole tiles: the columns behind the piece become zeros
     p.m_rows = n;
     LS_TRY((ls_gemm_any<F32, KC, KC, EPI_S>(p, big_tiles(n, T), st)));
+    LsParams q = {};
+    q.B = at<const uint8_t>(ws, l.s);
+    q.lda = rb;
+    q.ldb = pitch * esz;
+    q.M = q.m_rows = h;
+    q.T = T;
+    q.count = count;
+    q.rows = rows;
+    q.ldo = h;
+    q.g_scale = scale;
+    q.r_scale = r_scale;
+    q.split = at<float>(ws, l.split);
     if (dx != nullptr) {
-      LsParams q = {};
       q.A = wp;
-      q.B = at<const uint8_t>(ws, l.s);
-      q.lda = rb;
-      q.ldb = pitch * esz;
-      q.M = q.m_rows = h;
       q.N = T;
       q.K = n;
-      q.T = T;
-      q.count = count;
-      q.rows = rows;
-      q.parts = l.parts_x;
-      q.ldo = h;
-      const bool big = big_tiles(h, T);
-      if (l.parts_x > 1 || l.pieces > 1) {
-        q.out = at<void>(ws, l.acc_x);
-        q.add = i > 0;
-        LS_TRY((ls_gemm_any<F32, KS, KC, EPI_ACC>(q, big, st)));
-      } else {
-        q.out = dx;
-        q.scatter = true;
-        q.g_scale = scale;
-        q.r_scale = r_scale;
-        LS_TRY((ls_gemm_any<F32, KS, KC, EPI_OUT>(q, big, st)));
-      }
+      q.out = dx;
+      q.scatter = true;
+      q.acc = at<float>(ws, l.acc);
+      q.first = i == 0;
+      q.last = i == l.pieces - 1;
+      LS_TRY((ls_gemm_any<F32, KS, KC, EPI_OUT>(q, l.big_x, st)));
     }
     if (dw != nullptr) {
-      LsParams q = {};
       q.A = xc;
       q.alt = static_cast<const uint8_t*>(x);
-      q.B = at<const uint8_t>(ws, l.s);
-      q.lda = rb;
-      q.ldb = pitch * esz;
-      q.M = q.m_rows = h;
       q.N = n;
       q.K = T;
-      q.T = T;
-      q.count = count;
-      q.parts = l.parts_w;
-      q.ldo = h;
-      E* out = static_cast<E*>(dw) + v0 * h;
-      const bool big = big_tiles(h, l.piece < V ? l.piece : V);
-      if (l.parts_w > 1) {
-        q.out = at<void>(ws, l.acc_w);
-        LS_TRY((ls_gemm_any<F32, KS, KS, EPI_ACC>(q, big, st)));
-        hipLaunchKernelGGL(ls_join_kernel<E>, dim3((unsigned)ceil_div(n * (h / 4), 256)), dim3(256), 0, st,
-                           at<float>(ws, l.acc_w), l.parts_w, n, h, nullptr, nullptr, scale, r_scale, out);
-        LS_TRY(hipGetLastError());
-      } else {
-        q.out = out;
-        q.g_scale = scale;
-        q.r_scale = r_scale;
-        LS_TRY((ls_gemm_any<F32, KS, KS, EPI_OUT>(q, big, st)));
-      }
+      q.out = static_cast<uint8_t*>(dw) + v0 * rb;
+      q.scatter = false;
+      q.first = q.last = true;
+      LS_TRY((ls_gemm_any<F32, KS, KS, EPI_OUT>(q, l.big_w, st)));
     }
-  }
-  if (dx != nullptr && (l.parts_x > 1 || l.pieces > 1)) {
-    hipLaunchKernelGGL(ls_join_kernel<E>, dim3((unsigned)ceil_div(T * (h / 4), 256)), dim3(256), 0, st,
-                       at<float>(ws, l.acc_x), l.parts_x, T, h, count, rows, scale, r_scale, static_cast<E*>(dx));
-    LS_TRY(hipGetLastError());
   }
   return hipSuccess;
 }
