@@ -189,36 +189,41 @@ struct LsParams {
   uint32_t slots;        // workgroups that run at once
 };
 
-// How a product's tiles are dealt to `slots` workgroups: whole rounds of them take their tile over all of K; the `rest` of a last,
-// partial round is split over K into `parts` runs, so that it ends when about as many workgroups are done. In steps' time
-// (1.7 us on 256 x 256): an item costs 3 beside its own, a partial sum of a tile 6 to write and, with the others, 10 to join.
+// How a product's tiles are dealt to `slots` workgroups: whole rounds of them take their tile over all of K. The `rest` of a
+// last, partial round is split over K, where that pays, and the partial sums are joined afterwards, in one of two ways:
+//   parts > 0: every tile into `parts` runs of `per` steps, run by run, so that workgroups that share rows of the operands
+//              read them at the same time (at most two items per workgroup);
+//   parts = 0: all steps of the rest evenly, `per` neighbouring ones to a workgroup, which reach over at most two tiles, a
+//              tile cut at most 17-fold.
+// In steps' time (1.7 us on 256 x 256): an item costs 3 beside its own; equal parts 4 and 16 for each round of partial sums,
+// even runs 42. Measured: 80 tiles of 256 steps 164 us in 3 parts and 197 in even runs, 136 tiles of 392 steps 500 and 425.
 struct LsPlan {
-  uint32_t full, rest;
-  int parts, per;  // per: steps of a part
+  uint32_t full, rest, steps, per, parts;
 };
-constexpr int LS_PARTS = 8;  // and rest * parts at most twice the slots: the size of the partial sums' buffer
-__host__ __device__ inline LsPlan ls_plan(uint32_t tiles, int steps, uint32_t slots) {
-  LsPlan pl = {tiles, 0, 1, steps};
+constexpr uint32_t LS_CUTS = 16;
+__host__ __device__ inline LsPlan ls_plan(uint32_t tiles, uint32_t steps, uint32_t slots) {
   const uint32_t rest = tiles % slots;
+  LsPlan pl = {tiles, 0, steps, steps, 1};
   if (rest == 0) return pl;
-  uint32_t best = 0;
-  for (int p = 1; p <= LS_PARTS && p <= steps && (p == 1 || rest * p <= 2 * slots); ++p) {
-    const uint32_t per = (uint32_t)(steps + p - 1) / p, load = rest * p;
-    const uint32_t cost = (load + slots - 1) / slots * (per + 3) + (p > 1 ? 4 + 16 * load / slots : 0);
-    if (p == 1 || cost < best) {
-      best = cost;
-      pl.parts = p;
-      pl.per = (int)per;
-    }
+  const uint64_t even = ((uint64_t)rest * steps + slots - 1) / slots;
+  const uint32_t least = (steps + LS_CUTS - 1) / LS_CUTS, run = even > least ? (uint32_t)even : least;
+  uint32_t best = steps + 3;
+  if (run + 42 < best) {
+    best = run + 42;
+    pl = LsPlan{tiles - rest, rest, steps, run, 0};
   }
-  if (pl.parts > 1) {
-    pl.full = tiles - rest;
-    pl.rest = rest;
+  for (uint32_t q = 2; q <= 8 && q <= steps && rest * q <= 2 * slots; ++q) {
+    const uint32_t per = (steps + q - 1) / q, parts = (steps + per - 1) / per, load = rest * parts;
+    const uint32_t cost = (load + slots - 1) / slots * (per + 3) + 4 + 16 * load / slots;
+    if (cost < best) {
+      best = cost;
+      pl = LsPlan{tiles - rest, rest, steps, per, parts};
+    }
   }
   return pl;
 }
 
-// Position of a work item: tile (m, n) and its K steps; part: its index among the split tiles' partial sums, or -1.
+// Position of a work item: tile (m, n) and its K steps; part: its index among the partial sums, or -1 for a whole tile.
 struct LsItem {
   int m, n, part, k0, nk;
   uint32_t tile;
@@ -263,17 +268,41 @@ __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void ls_gemm_kernel(const L
   // Work items of neighbouring blocks on an XCD are neighbouring tiles: 8 tiles of M by as many of N as it has room for.
   const uint32_t G = gridDim.x;
   const uint32_t first = (G & 7) == 0 ? (blockIdx.x & 7) * (G >> 3) + (blockIdx.x >> 3) : blockIdx.x;
-  const LsPlan pl = EPI == EPI_OUT ? ls_plan(tiles, steps, p.slots) : LsPlan{tiles, 0, 1, steps};
-  const uint32_t total = pl.full + pl.rest * pl.parts;
-  if (first >= total) return;
-  auto item_of = [&](uint32_t L) {
-    LsItem it = {0, 0, -1, 0, max(1, steps), L};  // no step at all: one of zeros
-    if (EPI == EPI_OUT && L >= pl.full) {
-      const uint32_t q = L - pl.full, part = q / pl.rest;
-      it.part = (int)q;
-      it.tile = pl.full + q - part * pl.rest;
-      it.k0 = (int)part * pl.per;
-      it.nk = max(1, min(pl.per, steps - it.k0));
+  const LsPlan pl = EPI == EPI_OUT ? ls_plan(tiles, (uint32_t)steps, p.slots)
+                                   : LsPlan{tiles, 0, (uint32_t)steps, (uint32_t)steps, 1};
+  // This block's items: its tiles of the whole rounds, then (with the grid of p.slots blocks) its share of the rest.
+  const uint32_t rounds = first < pl.full ? (pl.full - first - 1) / G + 1 : 0;
+  uint32_t lo = 0, cut = 0, hi = 0;  // even runs: steps lo .. cut - 1 of its first tile, cut .. hi - 1 of the next
+  uint32_t total = rounds;
+  if (EPI == EPI_OUT && pl.rest != 0) {
+    if (pl.parts != 0) {
+      total += (first < pl.rest * pl.parts ? 1 : 0) + (first + G < pl.rest * pl.parts ? 1 : 0);
+    } else {
+      const uint32_t units = pl.rest * pl.steps;  // < 2^29
+      lo = min(first * pl.per, units);
+      hi = min(lo + pl.per, units);
+      cut = hi > lo ? min((lo / pl.steps + 1) * pl.steps, hi) : lo;
+      total += (hi > lo ? 1 : 0) + (hi > cut ? 1 : 0);
+    }
+  }
+  if (total == 0) return;
+  auto item_of = [&](uint32_t r) {
+    LsItem it = {0, 0, -1, 0, max(1, steps), first + r * G};  // no step at all: one of zeros
+    if (EPI == EPI_OUT && r >= rounds) {
+      const uint32_t s = r - rounds;
+      if (pl.parts != 0) {
+        const uint32_t q = first + s * G, part = q / pl.rest;
+        it.tile = pl.full + q - part * pl.rest;
+        it.k0 = (int)(part * pl.per);
+        it.nk = (int)min(pl.per, pl.steps - part * pl.per);
+        it.part = (int)q;
+      } else {
+        const uint32_t from = s == 0 ? lo : cut, to = s == 0 ? cut : hi, q = from / pl.steps;
+        it.tile = pl.full + q;
+        it.k0 = (int)(from - q * pl.steps);
+        it.nk = (int)(to - from);
+        if (to - from < pl.steps) it.part = (int)(2 * first + s);
+      }
     }
     ls_tile(it.tile, ntm, ntn, it.m, it.n);
     return it;
@@ -292,7 +321,7 @@ __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void ls_gemm_kernel(const L
 
   // The stream of K steps over this block's items, as the loads see it: `c` and its step, the operands' resources and the
   // K offset of a KC operand's rows (a KS operand's base moves instead: its end has to bound the step's K rows).
-  uint32_t c_item = first;
+  uint32_t c_item = 0;
   LsItem c = item_of(c_item);
   int c_step = 0;
   uint32_t c_soff = 0;
@@ -325,8 +354,7 @@ __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void ls_gemm_kernel(const L
       return;
     }
     c_step = 0;
-    c_item += G;
-    if (c_item < total) c = item_of(c_item);
+    if (++c_item < total) c = item_of(c_item);
     enter();
   };
 
@@ -360,8 +388,8 @@ __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void ls_gemm_kernel(const L
   };
 #pragma unroll
   for (int j = 0; j < MB + NB; ++j) fr[0][j] = read(j, lds, 0);
-  LsItem it = item_of(first);
-  uint32_t item = first;
+  LsItem it = item_of(0);
+  uint32_t item = 0;
   int slot = 0;
 #pragma unroll 1
   for (;;) {
@@ -517,8 +545,7 @@ __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void ls_gemm_kernel(const L
         }
       }
     }
-    item += G;
-    if (item >= total) break;
+    if (++item >= total) break;
     it = item_of(item);
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -673,12 +700,16 @@ __global__ __launch_bounds__(256) void ls_join_kernel(const LsParams p) {
   const int64_t cnt = (int64_t)load_uniform(p.count);
   const int64_t N = TOK_K ? p.N : cnt, K = TOK_K ? cnt : p.K;
   const uint32_t ntm = (uint32_t)((p.M + BM - 1) / BM), ntn = (uint32_t)((N + BN - 1) / BN);
-  const LsPlan pl = ls_plan(ntm * ntn, (int)((K + BK - 1) / BK), p.slots);
+  const LsPlan pl = ls_plan(ntm * ntn, (uint32_t)((K + BK - 1) / BK), p.slots);
   float scale = 1.0f;
   if (p.last && p.g_scale != nullptr) scale *= *p.g_scale;
   if (p.last && p.r_scale != nullptr) scale *= *p.r_scale;
   for (uint32_t id = blockIdx.x * 256 + threadIdx.x; id < pl.rest * PER; id += gridDim.x * 256) {
     const uint32_t q = id / PER, in = id - q * PER;
+    // Its partial sums: one per part, or one per workgroup whose run of steps meets the tile (one alone has written it).
+    const uint32_t lo = q * pl.steps;
+    const uint32_t c0 = pl.parts != 0 ? 0 : lo / pl.per, c1 = pl.parts != 0 ? pl.parts - 1 : (lo + pl.steps - 1) / pl.per;
+    if (c0 == c1) continue;
     const int ln = in & 31, blk = in >> 5;  // block (w MB + i) NB + j
     int tm, tn;
     ls_tile(pl.full + q, ntm, ntn, tm, tn);
@@ -687,11 +718,12 @@ __global__ __launch_bounds__(256) void ls_join_kernel(const LsParams p) {
     if (m >= p.M || n >= N) continue;
     f32x4_t v[8];  // m = 8 (k / 2) + 4 (k % 2)
     const int64_t at = (int64_t)blk * 1024 + 4 * ln;
-    const float* a = p.split + (int64_t)q * (BM * BN) + at;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] = *reinterpret_cast<const f32x4_t*>(a + 256 * (k >> 1) + 128 * (k & 1));
-    for (int part = 1; part < pl.parts; ++part) {
-      a += (int64_t)pl.rest * (BM * BN);
+    for (int k = 0; k < 8; ++k) v[k] = (f32x4_t){0.0f, 0.0f, 0.0f, 0.0f};
+    for (uint32_t c = c0; c <= c1; ++c) {
+      // Even runs: the tile is the second of the workgroup's, or the first.
+      const uint32_t part = pl.parts != 0 ? c * pl.rest + q : 2 * c + (c * pl.per < lo ? 1 : 0);
+      const float* a = p.split + (int64_t)part * (BM * BN) + at;
 #pragma unroll
       for (int k = 0; k < 8; ++k) v[k] += *reinterpret_cast<const f32x4_t*>(a + 256 * (k >> 1) + 128 * (k & 1));
     }
@@ -725,9 +757,7 @@ template <bool F32, int BM, int BN, int LA, int LB, int EPI>
 hipError_t ls_gemm(LsParams p, hipStream_t st) {
   p.slots = ls_slots(BM == 256);
   const int64_t tiles = ceil_div(p.M, BM) * ceil_div(p.N, BN);
-  const int64_t items = EPI == EPI_OUT ? tiles * LS_PARTS : tiles;
-  const unsigned grid = (unsigned)(items < p.slots ? items : p.slots);
-  if (grid == 0) return hipSuccess;
+  const unsigned grid = EPI == EPI_OUT || tiles > p.slots ? p.slots : (unsigned)tiles;
   hipLaunchKernelGGL((ls_gemm_kernel<F32, BM, BN, LA, LB, EPI>), dim3(grid), dim3(256), 0, st, p);
   const hipError_t e = hipGetLastError();
   if (EPI != EPI_OUT || e != hipSuccess) return e;
@@ -746,8 +776,8 @@ bool big_tiles_k(int64_t M, int64_t N, int64_t steps) {
 
 // Tiles of partial sums that a product may need, and of its running sums.
 size_t split_bytes(int64_t M, int64_t N, bool big) {
-  const int64_t b = big ? 256 : 128, tiles = ceil_div(M, b) * ceil_div(N, b), most = 2 * (int64_t)ls_slots(big);
-  return 4 * (size_t)(b * b) * (size_t)(tiles * LS_PARTS < most ? tiles * LS_PARTS : most);
+  const int64_t b = big ? 256 : 128, most = 2 * (int64_t)ls_slots(big), cuts = ceil_div(M, b) * ceil_div(N, b) * LS_CUTS * 2;
+  return 4 * (size_t)(b * b) * (size_t)(cuts < most ? cuts : most);
 }
 size_t acc_bytes(int64_t M, int64_t N, bool big) {
   const int64_t b = big ? 256 : 128;
