@@ -522,8 +522,9 @@ int q38moe_qsa_attention(const void* q, const void* k, const void* v, const void
  *   z = x . w^T,  lse[t] = log sum_v exp z[t,v],  loss[t] = lse[t] - z[t, targets[t]]
  * x [T,h] and w [V,h] in dtype, targets [T] int32 or int64, loss and lse [T] fp32; logits, maxima and sums in fp32.
  * Rows whose target is ignore_index have loss 0 (whatever their x) and lse 0; a target outside [0, V) makes its
- * row's loss and lse NaN. reduced (NULL to skip) = {sum of the losses, or with mean their sum over max(1, rows not
- * ignored); the factor 1 or 1 / max(1, rows not ignored)}. h a multiple of 64 up to 65536, T <= 2^24, V < 2^21.
+ * row's loss and lse NaN. lse may be NULL (no backward pass follows). *reduced (NULL to skip) = the sum of the losses, or
+ * with mean their sum over max(1, rows not ignored); *row_scale (NULL to skip) = 1 or 1 / max(1, rows not ignored),
+ * every row's factor in the reduction's gradient. h a multiple of 64 up to 65536, T <= 2^24, V < 2^21.
  * Backward: with s[t,v] = exp(z[t,v] - lse[t]) - [v = targets[t]] and G[t] = g[0] or, with g_per_row, g[t], times
  * *row_scale (NULL: 1):  dx = G s . w [T,h] and dw = (G s)^T . x [V,h] in dtype (either may be NULL). Ignored rows
  * get zeros and count in nothing. The vocabulary is taken in pieces whose s fits 256 MiB of the workspace (at least 256
@@ -533,8 +534,8 @@ int q38moe_qsa_attention(const void* q, const void* k, const void* v, const void
 #define Q38MOE_NEED_LOSS_W 2
 int q38moe_linear_ce_workspace_bytes(int64_t T, int32_t h, int32_t V, int32_t needs, int32_t dtype, size_t* bytes);
 int q38moe_linear_ce_forward(const void* x, const void* w, const void* targets, int32_t targets_int64,
-                             int64_t ignore_index, float* loss, float* lse, float* reduced, int32_t mean, int64_t T,
-                             int32_t h, int32_t V, void* workspace, size_t workspace_bytes, int32_t dtype,
+                             int64_t ignore_index, float* loss, float* lse, float* reduced, float* row_scale,
+                             int32_t mean, int64_t T, int32_t h, int32_t V, void* workspace, size_t workspace_bytes, int32_t dtype,
                              void* stream);
 int q38moe_linear_ce_backward(const float* g, int32_t g_per_row, const float* row_scale, const void* x, const void* w,
                               const void* targets, int32_t targets_int64, int64_t ignore_index, const float* lse,

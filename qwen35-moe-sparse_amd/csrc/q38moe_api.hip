@@ -1492,24 +1492,24 @@ int q38moe_linear_ce_workspace_bytes(int64_t T, int32_t h, int32_t V, int32_t ne
 }
 
 int q38moe_linear_ce_forward(const void* x, const void* w, const void* targets, int32_t targets_int64,
-                             int64_t ignore_index, float* loss, float* lse, float* reduced, int32_t mean, int64_t T,
-                             int32_t h, int32_t V, void* workspace, size_t workspace_bytes, int32_t dtype,
+                             int64_t ignore_index, float* loss, float* lse, float* reduced, float* row_scale,
+                             int32_t mean, int64_t T, int32_t h, int32_t V, void* workspace, size_t workspace_bytes, int32_t dtype,
                              void* stream) {
   g_err[0] = 0;
   Q38_CHECK(check_loss(T, h, V, dtype));
   if (T == 0) return Q38MOE_OK;
   Q38_CHECK(check_ptr(x, "x"));
   Q38_CHECK(check_ptr(w, "w"));
-  if (targets == nullptr || loss == nullptr || lse == nullptr)
-    return fail(Q38MOE_EINVAL, "targets, loss and lse must not be NULL");
+  if (targets == nullptr || loss == nullptr) return fail(Q38MOE_EINVAL, "targets and loss must not be NULL");
+  if (row_scale != nullptr && reduced == nullptr) return fail(Q38MOE_EINVAL, "row_scale needs reduced");
   size_t need = 0;
   Q38_CHECK(q38moe_linear_ce_workspace_bytes(T, h, V, 0, dtype, &need));
   if (workspace == nullptr || workspace_bytes < need)
     return fail(Q38MOE_EWORKSPACE, "workspace needs %zu bytes, got %zu", need, workspace_bytes);
   Q38_CHECK(check_ptr(workspace, "workspace"));
   (void)hipGetLastError();
-  Q38_HIP(q38::launch_linear_ce_forward(x, w, targets, targets_int64 != 0, ignore_index, loss, lse, reduced, mean != 0,
-                                        T, h, V, workspace, dtype == Q38MOE_FP32, static_cast<hipStream_t>(stream)),
+  Q38_HIP(q38::launch_linear_ce_forward(x, w, targets, targets_int64 != 0, ignore_index, loss, lse, reduced,
+                                        row_scale, mean != 0, T, h, V, workspace, dtype == Q38MOE_FP32, static_cast<hipStream_t>(stream)),
           "linear cross entropy launch");
   return Q38MOE_OK;
 }

@@ -238,8 +238,8 @@ hipError_t launch_clip_scale(const ClipTable& t, const double* partial, int npar
 // the backward pass for the gradients asked for; targets int32 or int64.
 size_t linear_ce_workspace(int64_t T, int h, int V, bool f32, bool forward, bool need_x, bool need_w);
 hipError_t launch_linear_ce_forward(const void* x, const void* w, const void* targets, bool idx64, int64_t ignore,
-                                    float* loss, float* lse, float* reduced, bool mean, int64_t T, int h, int V,
-                                    void* ws, bool f32, hipStream_t st);
+                                    float* loss, float* lse, float* reduced, float* row_scale, bool mean, int64_t T,
+                                    int h, int V, void* ws, bool f32, hipStream_t st);
 hipError_t launch_linear_ce_backward(const float* g, bool g_rows, const float* r_scale, const void* x, const void* w,
                                      const void* targets, bool idx64, int64_t ignore, const float* lse, void* dx,
                                      void* dw, int64_t T, int h, int V, void* ws, bool f32, hipStream_t st);

@@ -76,9 +76,12 @@ struct Operand {
   // c ^ swz(r): the 16 lanes that read together then cover the 64 banks.
   static __device__ __forceinline__ uint32_t voff(int j, int wave, int lane, uint32_t ld) {
     const int row = wave * (L == KC ? R / 4 : BK / 4) + j * (64 / LPR) + lane / LPR;
-    const int sw = L == KC ? (row >> 1) & 7 : (F32 ? 8 * ((row >> 2) & 1) : 4 * (row & 3));
+    const int sw = L == KC ? (row >> 1) & 7 : (F32 ? 8 * ((row >> 2) & 1) : ks_swz(row));
     return (uint32_t)row * ld + 16u * (uint32_t)((lane % LPR) ^ sw);
   }
+
+  // KS, bf16: the four K rows that a half-wave's transposing read takes 64 bytes of lie in different banks.
+  static __device__ __forceinline__ int ks_swz(int row) { return R == 64 ? 4 * ((row >> 1) & 1) : 4 * (row & 3); }
 
   // This lane's LDS offset of fragments: of K substep i (KC; block b adds 32 rows) or of block i (KS; substep u adds
   // rows).
@@ -93,7 +96,7 @@ struct Operand {
     } else {
       const int g = lane >> 4, gi = lane & 15;
       const int row = 8 * (g >> 1) + (gi >> 2), col = r0 + 32 * i + 16 * (g & 1) + 4 * (gi & 3);
-      return row * PITCH + 16 * ((col >> 3) ^ (4 * (row & 3))) + 2 * (col & 7);
+      return row * PITCH + 16 * ((col >> 3) ^ ks_swz(row)) + 2 * (col & 7);
     }
   }
 
@@ -174,7 +177,10 @@ struct LsParams {
   int64_t v0;            // first vocabulary row of the piece
   float2* part;          // {max, sum} [2 ceil(M / BM), T]
   const int32_t* tgt;    // target per counted token
+  const void* raw;       // EPI_LSE without a list of rows: the targets as they are (count NULL: all T)
+  bool raw64;
   float* zt;             // the target's logit
+  uint32_t* done;        // EPI_LSE: cleared for ls_finish_kernel
   const float* lse;      // by original row
   const float* g_row;    // gradient per original row, or NULL
   // EPI_S, EPI_OUT
@@ -223,6 +229,13 @@ __host__ __device__ inline LsPlan ls_plan(uint32_t tiles, uint32_t steps, uint32
   return pl;
 }
 
+// A target id as an int, -1 where it lies outside of one's range.
+__device__ __forceinline__ int32_t raw_target(const void* targets, bool idx64, int64_t t) {
+  if (!idx64) return static_cast<const int32_t*>(targets)[t];
+  const int64_t v = static_cast<const int64_t*>(targets)[t];
+  return v < 0 || v > 0x7fffffff ? -1 : (int32_t)v;
+}
+
 // Position of a work item: tile (m, n) and its K steps; part: its index among the partial sums, or -1 for a whole tile.
 struct LsItem {
   int m, n, part, k0, nk;
@@ -237,13 +250,14 @@ __device__ __forceinline__ void ls_tile(uint32_t t, uint32_t ntm, uint32_t ntn, 
 }
 
 template <bool F32, int BM, int BN, int LA, int LB, int EPI>
-__global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void ls_gemm_kernel(const LsParams p) {
+__global__ __launch_bounds__(256, BM == 128 ? 2 : 1) void ls_gemm_kernel(const LsParams p) {
   using OA = Operand<F32, BM, LA>;
   using OB = Operand<F32, BN, LB>;
   constexpr int MB = BM / 64, NB = BN / 64;  // 32x32 blocks of a wave
   constexpr int SLOT = (BM + BN) * 128;
+  constexpr int NS = BM == 64 ? 8 : 2;  // steps in LDS: few tiles wait for memory, many for the matrix units
   constexpr int BK = OA::BK, ESZ = OA::ESZ;
-  __shared__ __align__(1024) uint8_t lds[2 * SLOT];
+  __shared__ __align__(1024) uint8_t lds[NS * SLOT];
   // Staging of bf16 outputs, 32 rows of out by BM / 2 columns per wave (beside the slots: copies for the next item run meanwhile).
   constexpr bool STAGED = !F32 && (EPI == EPI_S || EPI == EPI_OUT);
   __shared__ __align__(1024) uint8_t stage[STAGED ? 4 * 32 * BM : 16];
@@ -254,8 +268,10 @@ __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void ls_gemm_kernel(const L
 
   uint8_t* const stw = stage + (STAGED ? wave * 32 * BM : 0);
 
+  if (EPI == EPI_LSE && blockIdx.x == 0 && tid == 0) *p.done = 0;
+
   // Tokens are N of z^T and dx^T, K of dW^T.
-  const int64_t cnt = (int64_t)load_uniform(p.count);
+  const int64_t cnt = p.count != nullptr ? (int64_t)load_uniform(p.count) : p.T;
   const bool all = cnt >= p.T;
   constexpr bool tok_k = LB == KS;
   const int64_t N = tok_k ? p.N : cnt, K = tok_k ? cnt : p.K;
@@ -358,11 +374,11 @@ __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void ls_gemm_kernel(const L
     enter();
   };
 
-  // Position q of the stream lies in slot q % 2. Its slot is free once every wave has read its last fragments: in the
-  // last quarter of q the first half of position q + 2 is copied over it, in the first quarter of q + 1 the second,
-  // and both have at least two quarters to arrive. (All in one quarter is 5 % slower, over three or four quarters 2 %
-  // slower; the same loads through registers, a whole step ahead of their LDS stores, 2 % slower: at full rate the chip's
-  // power decides, and the registers' way costs more of it.)
+  // Position q of the stream lies in slot q % NS. Its slot is free once every wave has read its last fragments: in the
+  // last quarter of q the first half of position q + NS is copied over it, in the first quarter of q + 1 the second,
+  // and with two slots both have at least two quarters to arrive. (All in one quarter is 5 % slower, over three or four
+  // quarters 2 % slower; the same loads through registers, a whole step ahead of their LDS stores, 2 % slower: at full
+  // rate the chip's power decides, and the registers' way costs more of it.)
   constexpr int NC = OA::NDMA + OB::NDMA, Q = MB * NB;
   constexpr int C3 = NC / 2, C0 = NC - C3;
   const uint32_t lds0 = ls_lds_addr(lds);
@@ -372,12 +388,15 @@ __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void ls_gemm_kernel(const L
     else ls_dma(pb, nb, vb[j - OA::NDMA], LB == KC ? c_soff : 0u, to + BM * 128 + wave * (BN * 32) + (j - OA::NDMA) * 1024);
   };
   enter();
+#pragma unroll 1
+  for (int q = 0; q < NS - 1; ++q) {
 #pragma unroll
-  for (int j = 0; j < NC; ++j) copy(j, 0);
-  advance();
+    for (int j = 0; j < NC; ++j) copy(j, q);
+    advance();
+  }
 #pragma unroll
-  for (int j = 0; j < C3; ++j) copy(j, 1);
-  asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(C3) : "memory");
+  for (int j = 0; j < C3; ++j) copy(j, NS - 1);
+  asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((NS - 2) * NC + C3) : "memory");
 
   f32x16_t acc[MB][NB];
 #pragma unroll
@@ -395,8 +414,9 @@ __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void ls_gemm_kernel(const L
   for (;;) {
 #pragma unroll 1
     for (int s = 0; s < it.nk; ++s) {
+      const int then = slot + 1 < NS ? slot + 1 : 0, before = slot > 0 ? slot - 1 : NS - 1;
       const uint8_t* base = lds + slot * SLOT;
-      const uint8_t* next = lds + (slot ^ 1) * SLOT;
+      const uint8_t* next = lds + then * SLOT;
       // A quarter multiplies fr[half], reads fragments u of src into the other half after the first MFMAs, in the order of
       // their use, and stores and reloads quarter `part` of the loads after the others.
       auto quarter = [&](int half, const uint8_t* src, int u, int from, int cn, int to) {
@@ -413,14 +433,16 @@ __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void ls_gemm_kernel(const L
           for (int e = cn * q / Q; e < cn * (q + 1) / Q; ++e) copy(from + e, to);
         }
       };
-      quarter(0, base, 1, C3, C0, slot ^ 1);
-      quarter(1, base, 2, 0, 0, slot ^ 1);
-      quarter(0, base, 3, 0, 0, slot ^ 1);
+      quarter(0, base, 1, C3, C0, before);
+      quarter(1, base, 2, 0, 0, slot);
+      quarter(0, base, 3, 0, 0, slot);
       advance();
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-      ls_barrier();  // every wave has read this slot and stored the next
+      // This wave's copies of the next step have landed (those of the NS - 2 positions behind it may be under way), its reads of
+      // this slot are done, and so are the others'.
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NS - 2) * NC) : "memory");
+      ls_barrier();
       quarter(1, next, 0, 0, C3, slot);
-      slot ^= 1;
+      slot = then;
     }
     ls_drain();
 
@@ -443,7 +465,7 @@ __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void ls_gemm_kernel(const L
       float lse = 0.0f, g = 1.0f, mx = -__builtin_inff(), sum = 0.0f;
       int64_t row = n;
       if constexpr (EPI == EPI_LSE) {
-        if (n_ok) rel = p.tgt[n] - (int)mw;
+        if (n_ok) rel = (p.raw != nullptr ? raw_target(p.raw, p.raw64, n) : p.tgt[n]) - (int)mw;
       } else if constexpr (EPI == EPI_S) {
         if (n_ok) {
           const int64_t r = p.rows[n];
@@ -552,46 +574,59 @@ __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void ls_gemm_kernel(const L
 }
 
 // Partition of the rows: rows[0 .. n-1] those that count, ascending, rows[n .. T-1] the ignored ones, *count = n, tgt[i]
-// the target of rows[i] (-1: outside the vocabulary). With `keep` (no copy follows) every row stays where it is and an
-// ignored one gets target -2. One block; ballots give a row's place.
+// the target of rows[i] (-1: outside the vocabulary). One block; ballots give a row's place, 8192 rows at a time (16384 rows:
+// 4.5 us, 14.5 with 1024 at a time).
 template <typename IdxT>
 __global__ __launch_bounds__(1024) void ls_rows_kernel(const IdxT* __restrict__ targets, int64_t ignore, int64_t T, int V,
-                                                       bool keep, int32_t* __restrict__ rows, int32_t* __restrict__ tgt,
+                                                       int32_t* __restrict__ rows, int32_t* __restrict__ tgt,
                                                        int32_t* __restrict__ count) {
-  __shared__ int waves[2][16];
+  constexpr int E = 8;  // runs of 1024 rows
+  __shared__ int sums[E * 16 + 1];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   int64_t kept = 0;  // rows that count, so far
-  int buf = 0;
-  for (int64_t t0 = 0; t0 < T; t0 += 1024, buf ^= 1) {
-    const int64_t t = t0 + tid;
-    const int64_t v = t < T ? (int64_t)targets[t] : ignore;
-    const bool in = t < T && v != ignore;
-    const int32_t place = v >= 0 && v < V ? (int32_t)v : -1;
-    const uint64_t mask = ballot64(in);
-    if (lane == 0) waves[buf][wave] = __popcll(mask);
-    __syncthreads();
-    int before = 0, all = 0;
+  for (int64_t t0 = 0; t0 < T; t0 += E * 1024) {
+    int64_t v[E];
+    uint64_t mask[E];
 #pragma unroll
-    for (int w = 0; w < 16; ++w) {
-      const int c = waves[buf][w];
-      before += w < wave ? c : 0;
-      all += c;
+    for (int e = 0; e < E; ++e) {
+      const int64_t t = t0 + e * 1024 + tid;
+      v[e] = t < T ? (int64_t)targets[t] : ignore;
     }
-    before += __popcll(mask & ((1ull << lane) - 1));
-    if (t < T) {
-      if (keep) {
-        rows[t] = (int32_t)t;
-        tgt[t] = in ? place : -2;
-      } else if (in) {
-        rows[kept + before] = (int32_t)t;
-        tgt[kept + before] = place;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      mask[e] = ballot64(v[e] != ignore);  // the places behind T hold ignore
+      if (lane == 0) sums[e * 16 + wave] = __popcll(mask[e]);
+    }
+    __syncthreads();
+    if (wave == 0) {  // exclusive prefix sums of the E * 16 counts
+      const int a = sums[2 * lane], b = sums[2 * lane + 1];
+      int s = a + b;
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) {
+        const int u = __shfl_up(s, o);
+        if (lane >= o) s += u;
+      }
+      sums[2 * lane] = s - a - b;
+      sums[2 * lane + 1] = s - b;
+      if (lane == 63) sums[E * 16] = s;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const int64_t t = t0 + e * 1024 + tid;
+      if (t >= T) break;
+      const int64_t before = kept + sums[e * 16 + wave] + __popcll(mask[e] & ((1ull << lane) - 1));
+      if (v[e] != ignore) {
+        rows[before] = (int32_t)t;
+        tgt[before] = v[e] >= 0 && v[e] < V ? (int32_t)v[e] : -1;
       } else {
-        rows[T - 1 - (t - (kept + before))] = (int32_t)t;  // from the end
+        rows[T - 1 - (t - before)] = (int32_t)t;  // from the end
       }
     }
-    kept += all;
+    kept += sums[E * 16];
+    __syncthreads();
   }
-  if (tid == 0) *count = (int32_t)(keep ? T : kept);
+  if (tid == 0) *count = (int32_t)kept;
 }
 
 // xc[i] = x[rows[i]] for the rows that count, unless all do; zero[rows[i]] = 0 for the others (zero may be NULL). One wave per
@@ -610,17 +645,22 @@ __global__ __launch_bounds__(256) void ls_gather_kernel(const uint8_t* __restric
   }
 }
 
-// lse and loss of 64 rows per block from their partial maxima and sums (16 waves share the entries), the block's sum of losses
-// and its count. Rows that do not count get loss 0.
+// lse and loss of 64 rows per block from their partial maxima and sums (16 waves share the entries); rows that do not count get
+// loss 0. Rows are those of the list, or with `raw` the call's own. Then *reduced = the sum of all losses (mean: over
+// the rows that count; 0 where none does), *row_scale = the factor of every row's gradient: by the block that is done last, from
+// the blocks' sums in their order (*done is 0 before and after).
 __global__ __launch_bounds__(1024) void ls_finish_kernel(const float2* __restrict__ part, int entries,
                                                          const float* __restrict__ zt, const int32_t* __restrict__ tgt,
                                                          const int32_t* __restrict__ rows,
-                                                         const int32_t* __restrict__ count, int64_t T,
-                                                         float* __restrict__ loss, float* __restrict__ lse,
-                                                         double* __restrict__ block_sum, int32_t* __restrict__ block_n) {
+                                                         const int32_t* __restrict__ count, const void* raw, bool raw64,
+                                                         int64_t ignore, int V, int64_t T, float* __restrict__ loss,
+                                                         float* __restrict__ lse, bool mean, double* block_sum,
+                                                         int32_t* block_n, uint32_t* done, float* __restrict__ reduced,
+                                                         float* __restrict__ row_scale) {
   __shared__ float2 red[16][64];
+  __shared__ bool last;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t n = load_uniform(count), i = (int64_t)blockIdx.x * 64 + lane;
+  const int64_t n = raw != nullptr ? T : (int64_t)load_uniform(count), i = (int64_t)blockIdx.x * 64 + lane;
   float m = -__builtin_inff(), s = 0.0f;
   if (i < n) {
 #pragma unroll 4
@@ -631,54 +671,62 @@ __global__ __launch_bounds__(1024) void ls_finish_kernel(const float2* __restric
   }
   red[wave][lane] = make_float2(m, s);
   __syncthreads();
-  if (wave != 0) return;
+  if (wave == 0) {
 #pragma unroll
-  for (int w = 1; w < 16; ++w) lse_join(m, s, red[w][lane].x, red[w][lane].y);
-  double sum = 0.0;
-  int c = 0;
-  if (i < T) {
-    const int64_t r = rows[i];
-    const int tg = i < n ? tgt[i] : -2;
-    float l = 0.0f, z = 0.0f;
-    if (tg != -2) {
-      z = tg < 0 ? __builtin_nanf("") : m + logf(s);  // a target outside the vocabulary shows as NaN
-      l = tg < 0 ? z : z - zt[i];
-      sum = (double)l;
-      c = 1;
+    for (int w = 1; w < 16; ++w) lse_join(m, s, red[w][lane].x, red[w][lane].y);
+    double sum = 0.0;
+    int c = 0;
+    if (i < T) {
+      const int64_t r = raw != nullptr ? i : (int64_t)rows[i];
+      int tg = -1;
+      bool in = i < n;
+      if (raw != nullptr) {
+        const int64_t v = raw64 ? static_cast<const int64_t*>(raw)[i] : (int64_t)static_cast<const int32_t*>(raw)[i];
+        in = v != ignore;
+        tg = v >= 0 && v < V ? (int)v : -1;
+      } else if (in) {
+        tg = tgt[i];
+      }
+      float l = 0.0f, z = 0.0f;
+      if (in) {
+        z = tg < 0 ? __builtin_nanf("") : m + logf(s);  // a target outside the vocabulary shows as NaN
+        l = tg < 0 ? z : z - zt[i];
+        sum = (double)l;
+        c = 1;
+      }
+      loss[r] = l;
+      if (lse != nullptr) lse[r] = z;
     }
-    loss[r] = l;
-    lse[r] = z;
-  }
+    if (reduced != nullptr) {
 #pragma unroll
-  for (int o = 32; o; o >>= 1) {
-    const uint64_t u = __builtin_bit_cast(uint64_t, sum);
-    const uint32_t lo = __shfl_xor((int)(uint32_t)u, o), hi = __shfl_xor((int)(uint32_t)(u >> 32), o);
-    sum += __builtin_bit_cast(double, ((uint64_t)hi << 32) | lo);
-    c += __shfl_xor(c, o);
+      for (int o = 32; o; o >>= 1) {
+        const uint64_t u = __builtin_bit_cast(uint64_t, sum);
+        const uint32_t lo = __shfl_xor((int)(uint32_t)u, o), hi = __shfl_xor((int)(uint32_t)(u >> 32), o);
+        sum += __builtin_bit_cast(double, ((uint64_t)hi << 32) | lo);
+        c += __shfl_xor(c, o);
+      }
+      if (lane == 0) {
+        __hip_atomic_store(block_sum + blockIdx.x, sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        __hip_atomic_store(block_n + blockIdx.x, c, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        last = __hip_atomic_fetch_add(done, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == gridDim.x - 1;
+      }
+    }
   }
-  if (lane == 0) {
-    block_sum[blockIdx.x] = sum;
-    block_n[blockIdx.x] = c;
-  }
-}
-
-// reduced[0] = the sum of the losses (mean: over the rows that count; 0 where none does), reduced[1] = the factor of every
-// row's gradient.
-__global__ __launch_bounds__(256) void ls_reduce_kernel(const double* __restrict__ block_sum,
-                                                        const int32_t* __restrict__ block_n, int blocks, bool mean,
-                                                        float* __restrict__ reduced) {
-  __shared__ double sums[256];
-  __shared__ int64_t ns[256];
-  double s = 0.0;
-  int64_t n = 0;
-  for (int b = threadIdx.x; b < blocks; b += 256) {
-    s += block_sum[b];
-    n += block_n[b];
-  }
-  sums[threadIdx.x] = s;
-  ns[threadIdx.x] = n;
+  if (reduced == nullptr) return;
   __syncthreads();
-  for (int o = 128; o; o >>= 1) {
+  if (!last) return;
+  __shared__ double sums[1024];
+  __shared__ int64_t ns[1024];
+  double a = 0.0;
+  int64_t k = 0;
+  for (int b = threadIdx.x; b < (int)gridDim.x; b += 1024) {
+    a += __hip_atomic_load(block_sum + b, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    k += __hip_atomic_load(block_n + b, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  sums[threadIdx.x] = a;
+  ns[threadIdx.x] = k;
+  __syncthreads();
+  for (int o = 512; o; o >>= 1) {
     if ((int)threadIdx.x < o) {
       sums[threadIdx.x] += sums[threadIdx.x + o];
       ns[threadIdx.x] += ns[threadIdx.x + o];
@@ -687,8 +735,9 @@ __global__ __launch_bounds__(256) void ls_reduce_kernel(const double* __restrict
   }
   if (threadIdx.x == 0) {
     const double d = mean ? (double)(ns[0] > 0 ? ns[0] : 1) : 1.0;
-    reduced[0] = (float)(sums[0] / d);
-    reduced[1] = (float)(1.0 / d);
+    *reduced = (float)(sums[0] / d);
+    if (row_scale != nullptr) *row_scale = (float)(1.0 / d);
+    *done = 0;
   }
 }
 
@@ -751,11 +800,12 @@ __global__ __launch_bounds__(256) void ls_join_kernel(const LsParams p) {
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-uint32_t ls_slots(bool big) { return (uint32_t)device_cus() * (big ? 1 : 2); }
+// Workgroups that run at once: two of 128 x 128 tiles share a CU.
+uint32_t ls_slots(int bm) { return (uint32_t)device_cus() * (bm == 128 ? 2 : 1); }
 
 template <bool F32, int BM, int BN, int LA, int LB, int EPI>
 hipError_t ls_gemm(LsParams p, hipStream_t st) {
-  p.slots = ls_slots(BM == 256);
+  p.slots = ls_slots(BM);
   const int64_t tiles = ceil_div(p.M, BM) * ceil_div(p.N, BN);
   const unsigned grid = EPI == EPI_OUT || tiles > p.slots ? p.slots : (unsigned)tiles;
   hipLaunchKernelGGL((ls_gemm_kernel<F32, BM, BN, LA, LB, EPI>), dim3(grid), dim3(256), 0, st, p);
@@ -766,33 +816,36 @@ hipError_t ls_gemm(LsParams p, hipStream_t st) {
   return hipGetLastError();
 }
 
-// Products over the vocabulary: tiles of 256 x 256 where they fill at least half the CUs, else of 128 x 128.
-bool big_tiles(int64_t M, int64_t N) { return ceil_div(M, 256) * ceil_div(N, 256) * 2 >= device_cus(); }
-
-// Gradients, whose tiles can be split over K: large tiles where each CU has at least 12 steps of them.
-bool big_tiles_k(int64_t M, int64_t N, int64_t steps) {
-  return ceil_div(M, 256) * ceil_div(N, 256) * steps >= (int64_t)12 * device_cus();
+// Tile side of the products over the vocabulary, whose tiles stay whole: 256 where such tiles fill at least half the CUs, 64 (with
+// eight steps in LDS) where tiles of 128 leave half the CUs without one, else 128.
+int tile_z(int64_t M, int64_t N) {
+  if (ceil_div(M, 256) * ceil_div(N, 256) * 2 >= device_cus()) return 256;
+  return ceil_div(M, 128) * ceil_div(N, 128) * 2 < device_cus() ? 64 : 128;
 }
 
-// Tiles of partial sums that a product may need, and of its running sums.
-size_t split_bytes(int64_t M, int64_t N, bool big) {
-  const int64_t b = big ? 256 : 128, most = 2 * (int64_t)ls_slots(big), cuts = ceil_div(M, b) * ceil_div(N, b) * LS_CUTS * 2;
+// Of the gradients' products, whose tiles can be split over K: 256 where each CU has at least 12 steps of such tiles, 128 where
+// each has 6 of those.
+int tile_k(int64_t M, int64_t N, int64_t steps) {
+  if (ceil_div(M, 256) * ceil_div(N, 256) * steps >= (int64_t)12 * device_cus()) return 256;
+  return ceil_div(M, 128) * ceil_div(N, 128) * steps >= (int64_t)6 * device_cus() ? 128 : 64;
+}
+
+// Bytes of a product's partial sums, and of its running sums.
+size_t split_bytes(int64_t M, int64_t N, int b) {
+  const int64_t most = 2 * (int64_t)ls_slots(b), cuts = ceil_div(M, b) * ceil_div(N, b) * LS_CUTS * 2;
   return 4 * (size_t)(b * b) * (size_t)(cuts < most ? cuts : most);
 }
-size_t acc_bytes(int64_t M, int64_t N, bool big) {
-  const int64_t b = big ? 256 : 128;
-  return 4 * (size_t)(b * b) * (size_t)(ceil_div(M, b) * ceil_div(N, b));
-}
+size_t acc_bytes(int64_t M, int64_t N, int b) { return 4 * (size_t)(b * b) * (size_t)(ceil_div(M, b) * ceil_div(N, b)); }
 
 size_t up(size_t v) { return (v + 255) / 256 * 256; }
 
 struct Layout {
-  size_t rows, tgt, count, xc, part, zt, bsum, bn, s, acc, split, end;
+  size_t rows, tgt, count, xc, part, zt, bsum, bn, done, s, acc, split, end;
   int entries;             // of the forward's partial sums
   int64_t piece;           // vocabulary rows of a piece (multiple of 256)
   int pieces;
-  bool big_x, big_w;       // tiles of dx's and dw's products
-  bool gather;
+  int tile_s, tile_x, tile_w;  // tile sides of the forward's or s's, dx's and dw's products
+  bool raw;                // forward: no list of rows, every row's logits
 };
 
 constexpr int64_t PIECE_BYTES = (int64_t)256 << 20;
@@ -806,17 +859,19 @@ Layout layout(int64_t T, int h, int V, bool f32, bool fwd, bool need_x, bool nee
     off = up(off + n);
     return at;
   };
-  l.rows = take(4 * T);
-  l.tgt = take(4 * T);
+  l.raw = fwd && T <= 256;  // one tile of tokens: nothing to skip, and two launches fewer
+  l.rows = take(l.raw ? 0 : 4 * T);
+  l.tgt = take(l.raw ? 0 : 4 * T);
   l.count = take(4);
-  l.gather = !fwd || T > 256;
-  l.xc = take(l.gather ? esz * T * h : 0);
+  l.xc = take(l.raw ? 0 : esz * T * h);
+  l.tile_s = tile_z(V, T);
   if (fwd) {
-    l.entries = (int)(2 * ceil_div(V, big_tiles(V, T) ? 256 : 128));
+    l.entries = (int)(2 * ceil_div(V, l.tile_s));
     l.part = take(8 * (size_t)l.entries * T);
     l.zt = take(4 * T);
     l.bsum = take(8 * ceil_div(T, 64));
     l.bn = take(4 * ceil_div(T, 64));
+    l.done = take(4);
   } else {
     const int64_t vt = ceil_div(V, 256);
     int64_t most = PIECE_BYTES / ((int64_t)esz * T) / 256;
@@ -826,11 +881,12 @@ Layout layout(int64_t T, int h, int V, bool f32, bool fwd, bool need_x, bool nee
     l.pieces = (int)ceil_div(vt, pt);
     l.piece = pt * 256;
     l.s = take(esz * (size_t)T * l.piece);
-    const int64_t bk = f32 ? 32 : 64;
-    l.big_x = big_tiles_k(h, T, l.piece / bk);
-    l.big_w = big_tiles_k(h, l.piece, ceil_div(T, bk));
-    l.acc = take(need_x && l.pieces > 1 ? acc_bytes(h, T, l.big_x) : 0);
-    const size_t sx = need_x ? split_bytes(h, T, l.big_x) : 0, sw = need_w ? split_bytes(h, l.piece, l.big_w) : 0;
+    const int64_t bk = f32 ? 32 : 64, n = l.piece < V ? l.piece : V;
+    l.tile_s = tile_z(n, T);
+    l.tile_x = tile_k(h, T, ceil_div(n, bk));
+    l.tile_w = tile_k(h, n, ceil_div(T, bk));
+    l.acc = take(need_x && l.pieces > 1 ? acc_bytes(h, T, l.tile_x) : 0);
+    const size_t sx = need_x ? split_bytes(h, T, l.tile_x) : 0, sw = need_w ? split_bytes(h, n, l.tile_w) : 0;
     l.split = take(sx > sw ? sx : sw);
   }
   l.end = off;
@@ -848,14 +904,14 @@ P* at(void* base, size_t off) {
     if (e_ != hipSuccess) return e_;    \
   } while (0)
 
-hipError_t ls_rows(const void* targets, bool idx64, int64_t ignore, int64_t T, int V, bool keep, int32_t* rows,
-                   int32_t* tgt, int32_t* count, hipStream_t st) {
+hipError_t ls_rows(const void* targets, bool idx64, int64_t ignore, int64_t T, int V, int32_t* rows, int32_t* tgt,
+                   int32_t* count, hipStream_t st) {
   if (idx64)
-    hipLaunchKernelGGL(ls_rows_kernel<int64_t>, dim3(1), dim3(1024), 0, st, (const int64_t*)targets, ignore, T, V, keep,
-                       rows, tgt, count);
+    hipLaunchKernelGGL(ls_rows_kernel<int64_t>, dim3(1), dim3(1024), 0, st, (const int64_t*)targets, ignore, T, V, rows,
+                       tgt, count);
   else
-    hipLaunchKernelGGL(ls_rows_kernel<int32_t>, dim3(1), dim3(1024), 0, st, (const int32_t*)targets, ignore, T, V, keep,
-                       rows, tgt, count);
+    hipLaunchKernelGGL(ls_rows_kernel<int32_t>, dim3(1), dim3(1024), 0, st, (const int32_t*)targets, ignore, T, V, rows,
+                       tgt, count);
   return hipGetLastError();
 }
 
@@ -867,43 +923,44 @@ hipError_t ls_gather(const void* x, const int32_t* rows, const int32_t* count, v
 }
 
 template <bool F32, int LA, int LB, int EPI>
-hipError_t ls_gemm_any(const LsParams& p, bool big, hipStream_t st) {
-  return big ? ls_gemm<F32, 256, 256, LA, LB, EPI>(p, st) : ls_gemm<F32, 128, 128, LA, LB, EPI>(p, st);
+hipError_t ls_gemm_any(const LsParams& p, int tile, hipStream_t st) {
+  if (tile == 64) return ls_gemm<F32, 64, 64, LA, LB, EPI>(p, st);
+  return tile == 256 ? ls_gemm<F32, 256, 256, LA, LB, EPI>(p, st) : ls_gemm<F32, 128, 128, LA, LB, EPI>(p, st);
 }
 
 template <bool F32>
 hipError_t ce_forward(const void* x, const void* w, const void* targets, bool idx64, int64_t ignore, float* loss,
-                      float* lse, float* reduced, bool mean, int64_t T, int h, int V, void* ws, hipStream_t st) {
+                      float* lse, float* reduced, float* row_scale, bool mean, int64_t T, int h, int V, void* ws,
+                      hipStream_t st) {
   const Layout l = layout(T, h, V, F32, true, false, false);
   int32_t* rows = at<int32_t>(ws, l.rows);
   int32_t* tgt = at<int32_t>(ws, l.tgt);
   int32_t* count = at<int32_t>(ws, l.count);
   const int64_t rb = (int64_t)h * (F32 ? 4 : 2);
-  LS_TRY(ls_rows(targets, idx64, ignore, T, V, !l.gather, rows, tgt, count, st));
-  if (l.gather) LS_TRY(ls_gather(x, rows, count, at<void>(ws, l.xc), nullptr, T, (int)rb, st));
+  if (!l.raw) {
+    LS_TRY(ls_rows(targets, idx64, ignore, T, V, rows, tgt, count, st));
+    LS_TRY(ls_gather(x, rows, count, at<void>(ws, l.xc), nullptr, T, (int)rb, st));
+  }
   LsParams p = {};
   p.A = static_cast<const uint8_t*>(w);
-  p.B = l.gather ? at<const uint8_t>(ws, l.xc) : static_cast<const uint8_t*>(x);
+  p.B = l.raw ? static_cast<const uint8_t*>(x) : at<const uint8_t>(ws, l.xc);
   p.alt = static_cast<const uint8_t*>(x);
   p.lda = p.ldb = rb;
   p.M = p.m_rows = V;
   p.N = p.T = T;
   p.K = h;
-  p.count = count;
+  p.count = l.raw ? nullptr : count;
+  p.raw = l.raw ? targets : nullptr;
+  p.raw64 = idx64;
   p.part = at<float2>(ws, l.part);
   p.tgt = tgt;
   p.zt = at<float>(ws, l.zt);
-  LS_TRY((ls_gemm_any<F32, KC, KC, EPI_LSE>(p, big_tiles(V, T), st)));
-  const int blocks = (int)ceil_div(T, 64);
-  hipLaunchKernelGGL(ls_finish_kernel, dim3(blocks), dim3(1024), 0, st, p.part, l.entries, p.zt, tgt, rows, count, T,
-                     loss, lse, at<double>(ws, l.bsum), at<int32_t>(ws, l.bn));
-  LS_TRY(hipGetLastError());
-  if (reduced != nullptr) {
-    hipLaunchKernelGGL(ls_reduce_kernel, dim3(1), dim3(256), 0, st, at<double>(ws, l.bsum), at<int32_t>(ws, l.bn),
-                       blocks, mean, reduced);
-    LS_TRY(hipGetLastError());
-  }
-  return hipSuccess;
+  p.done = at<uint32_t>(ws, l.done);
+  LS_TRY((ls_gemm_any<F32, KC, KC, EPI_LSE>(p, l.tile_s, st)));
+  hipLaunchKernelGGL(ls_finish_kernel, dim3((unsigned)ceil_div(T, 64)), dim3(1024), 0, st, p.part, l.entries, p.zt, tgt,
+                     rows, count, p.raw, idx64, ignore, V, T, loss, lse, mean, at<double>(ws, l.bsum),
+                     at<int32_t>(ws, l.bn), p.done, reduced, row_scale);
+  return hipGetLastError();
 }
 
 template <bool F32>
@@ -916,7 +973,7 @@ hipError_t ce_backward(const float* g, bool g_rows, const float* r_scale, const 
   int32_t* count = at<int32_t>(ws, l.count);
   const int64_t rb = (int64_t)h * (F32 ? 4 : 2);
   const int64_t esz = F32 ? 4 : 2;
-  LS_TRY(ls_rows(targets, idx64, ignore, T, V, false, rows, tgt, count, st));
+  LS_TRY(ls_rows(targets, idx64, ignore, T, V, rows, tgt, count, st));
   LS_TRY(ls_gather(x, rows, count, at<void>(ws, l.xc), dx, T, (int)rb, st));
   const uint8_t* xc = at<const uint8_t>(ws, l.xc);
   const float* scale = g_rows ? nullptr : g;
@@ -943,7 +1000,7 @@ hipError_t ce_backward(const float* g, bool g_rows, const float* r_scale, const 
     p.ldo = pitch;
     p.M = pitch;  // whole tiles: the columns behind the piece become zeros
     p.m_rows = n;
-    LS_TRY((ls_gemm_any<F32, KC, KC, EPI_S>(p, big_tiles(n, T), st)));
+    LS_TRY((ls_gemm_any<F32, KC, KC, EPI_S>(p, l.tile_s, st)));
     LsParams q = {};
     q.B = at<const uint8_t>(ws, l.s);
     q.lda = rb;
@@ -965,7 +1022,7 @@ hipError_t ce_backward(const float* g, bool g_rows, const float* r_scale, const 
       q.acc = at<float>(ws, l.acc);
       q.first = i == 0;
       q.last = i == l.pieces - 1;
-      LS_TRY((ls_gemm_any<F32, KS, KC, EPI_OUT>(q, l.big_x, st)));
+      LS_TRY((ls_gemm_any<F32, KS, KC, EPI_OUT>(q, l.tile_x, st)));
     }
     if (dw != nullptr) {
       q.A = xc;
@@ -975,7 +1032,7 @@ hipError_t ce_backward(const float* g, bool g_rows, const float* r_scale, const 
       q.out = static_cast<uint8_t*>(dw) + v0 * rb;
       q.scatter = false;
       q.first = q.last = true;
-      LS_TRY((ls_gemm_any<F32, KS, KS, EPI_OUT>(q, l.big_w, st)));
+      LS_TRY((ls_gemm_any<F32, KS, KS, EPI_OUT>(q, l.tile_w, st)));
     }
   }
   return hipSuccess;
@@ -988,10 +1045,10 @@ size_t linear_ce_workspace(int64_t T, int h, int V, bool f32, bool forward, bool
 }
 
 hipError_t launch_linear_ce_forward(const void* x, const void* w, const void* targets, bool idx64, int64_t ignore,
-                                    float* loss, float* lse, float* reduced, bool mean, int64_t T, int h, int V,
-                                    void* ws, bool f32, hipStream_t st) {
-  return f32 ? ce_forward<true>(x, w, targets, idx64, ignore, loss, lse, reduced, mean, T, h, V, ws, st)
-             : ce_forward<false>(x, w, targets, idx64, ignore, loss, lse, reduced, mean, T, h, V, ws, st);
+                                    float* loss, float* lse, float* reduced, float* row_scale, bool mean, int64_t T,
+                                    int h, int V, void* ws, bool f32, hipStream_t st) {
+  return f32 ? ce_forward<true>(x, w, targets, idx64, ignore, loss, lse, reduced, row_scale, mean, T, h, V, ws, st)
+             : ce_forward<false>(x, w, targets, idx64, ignore, loss, lse, reduced, row_scale, mean, T, h, V, ws, st);
 }
 
 hipError_t launch_linear_ce_backward(const float* g, bool g_rows, const float* r_scale, const void* x, const void* w,

@@ -86,8 +86,8 @@ SIGNATURES = {
     "q38moe_gdn_delta": (_c_int, [_vp] * 8 + [_c_i64, _c_i32, _c_i32, _c_i32, ctypes.c_float, _vp, _c_size, _c_i32,
                                               _vp]),
     "q38moe_linear_ce_workspace_bytes": (_c_int, [_c_i64, _c_i32, _c_i32, _c_i32, _c_i32, ctypes.POINTER(_c_size)]),
-    "q38moe_linear_ce_forward": (_c_int, [_vp] * 3 + [_c_i32, _c_i64, _vp, _vp, _vp, _c_i32, _c_i64, _c_i32, _c_i32, _vp,
-                                          _c_size, _c_i32, _vp]),
+    "q38moe_linear_ce_forward": (_c_int, [_vp] * 3 + [_c_i32, _c_i64] + [_vp] * 4 + [_c_i32, _c_i64, _c_i32, _c_i32, _vp,
+                                                                                     _c_size, _c_i32, _vp]),
     "q38moe_linear_ce_backward": (_c_int, [_vp, _c_i32] + [_vp] * 4 + [_c_i32, _c_i64, _vp, _vp, _vp, _c_i64, _c_i32,
                                                                        _c_i32, _vp, _c_size, _c_i32, _vp]),
     "q38moe_grad_norm_workspace_bytes": (_c_int, [_c_i32, ctypes.POINTER(_c_size)]),

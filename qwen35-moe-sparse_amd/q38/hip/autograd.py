@@ -188,19 +188,19 @@ class HipLinearCE(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, weight, targets, ignore_index, reduction):
-        loss, lse, reduced = ops.linear_ce_forward(x, weight, targets, ignore_index,
-                                                   None if reduction == "none" else reduction)
-        ctx.save_for_backward(x, weight, targets, lse, reduced)
+        loss, lse, reduced, row_scale = ops.linear_ce_forward(x, weight, targets, ignore_index,
+                                                              None if reduction == "none" else reduction)
+        ctx.save_for_backward(x, weight, targets, lse, row_scale)
         ctx.ignore_index = ignore_index
-        return loss if reduced is None else reduced[0].clone()
+        return loss if reduced is None else reduced
 
     @staticmethod
     @once_differentiable
     def backward(ctx, g):
-        x, weight, targets, lse, reduced = ctx.saved_tensors
+        x, weight, targets, lse, row_scale = ctx.saved_tensors
         need_x, need_w = ctx.needs_input_grad[:2]
-        dx, dw = ops.linear_ce_backward(g.contiguous(), x, weight, targets, lse, ctx.ignore_index,
-                                        None if reduced is None else reduced[1:], need_x, need_w)
+        dx, dw = ops.linear_ce_backward(g.contiguous(), x, weight, targets, lse, ctx.ignore_index, row_scale, need_x,
+                                        need_w)
         return dx, dw, None, None, None
 
 
@@ -218,8 +218,13 @@ def linear_cross_entropy(x, weight, targets, ignore_index=-100, reduction="mean"
         raise ValueError(f"targets {tuple(targets.shape)} do not match x {tuple(x.shape)}")
     if _bf16_autocast() and x.is_floating_point() and weight.is_floating_point():
         x, weight = x.to(torch.bfloat16), weight.to(torch.bfloat16)
-    loss = HipLinearCE.apply(_aligned(x.reshape(-1, x.shape[-1])), _aligned(weight), targets.reshape(-1).contiguous(),
-                             ignore_index, reduction)
+    args = (_aligned(x.reshape(-1, x.shape[-1])), _aligned(weight), targets.reshape(-1).contiguous(), ignore_index)
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
+        loss = HipLinearCE.apply(*args, reduction)
+    elif reduction == "none":
+        loss = ops.linear_ce_forward(*args, want_lse=False)[0]
+    else:
+        loss = ops.linear_ce_forward(*args, reduction, want_lse=False)[2]
     return loss.view(targets.shape) if reduction == "none" else loss
 
 

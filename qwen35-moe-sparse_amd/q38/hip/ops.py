@@ -9,6 +9,7 @@ experts.down_proj [E,h,I], nn.Linear weights [out,in]).
 """
 import contextlib
 import ctypes
+import functools
 import math
 from typing import NamedTuple
 
@@ -826,31 +827,36 @@ def _loss_args(x, w, targets):
     return dt, T, h, w.shape[0]
 
 
-def _loss_workspace(T, h, V, needs, dt, device):
+@functools.lru_cache(maxsize=512)
+def _loss_workspace_bytes(T, h, V, needs, dt, device):
     n = ctypes.c_size_t()
     check(lib.q38moe_linear_ce_workspace_bytes(T, h, V, needs, _DTYPES[dt], ctypes.byref(n)),
           "q38moe_linear_ce_workspace_bytes")
-    return torch.empty(n.value, dtype=torch.uint8, device=device)
+    return n.value
 
 
-def linear_ce_forward(x, w, targets, ignore_index=-100, reduction=None):
-    """Softmax cross entropy of logits x . w^T without the logits (q38moe_linear_ce_forward): (loss [T], lse [T],
-    reduced) fp32, reduced = [sum or mean of the losses, the rows' gradient factor] for reduction "sum" or "mean", else None."""
+def linear_ce_forward(x, w, targets, ignore_index=-100, reduction=None, want_lse=True):
+    """Softmax cross entropy of logits x . w^T without the logits (q38moe_linear_ce_forward): (loss [T], lse [T] or
+    None, reduced, row_scale) fp32; reduced is the sum or mean of the losses and row_scale every row's factor in it, for
+    reduction "sum" or "mean", else None."""
     dt, T, h, V = _loss_args(x, w, targets)
     if reduction not in (None, "sum", "mean"):
         raise ValueError(f"reduction must be None, 'sum' or 'mean', got {reduction!r}")
     dev = x.device
     loss = torch.empty(T, dtype=torch.float32, device=dev)
-    lse = torch.empty(T, dtype=torch.float32, device=dev)
-    reduced = None
+    lse = torch.empty(T, dtype=torch.float32, device=dev) if want_lse else None
+    reduced = row_scale = None
     if reduction is not None:
-        reduced = torch.empty(2, dtype=torch.float32, device=dev) if T else torch.zeros(2, device=dev)
+        make = torch.empty if T else torch.zeros
+        reduced = make((), dtype=torch.float32, device=dev)
+        row_scale = make((), dtype=torch.float32, device=dev) if want_lse else None
     with _on(dev):
-        ws = _loss_workspace(T, h, V, 0, dt, dev)
+        ws = torch.empty(_loss_workspace_bytes(T, h, V, 0, dt, dev), dtype=torch.uint8, device=dev)
         check(lib.q38moe_linear_ce_forward(_ptr(x), _ptr(w), _ptr(targets), targets.dtype == torch.int64, ignore_index,
-                                           _ptr(loss), _ptr(lse), _ptr(reduced), reduction == "mean", T, h, V, _ptr(ws),
-                                           ws.numel(), _DTYPES[dt], _stream(dev)), "q38moe_linear_ce_forward")
-    return loss, lse, reduced
+                                           _ptr(loss), _ptr(lse), _ptr(reduced), _ptr(row_scale), reduction == "mean",
+                                           T, h, V, _ptr(ws), ws.numel(), _DTYPES[dt], _stream(dev)),
+              "q38moe_linear_ce_forward")
+    return loss, lse, reduced, row_scale
 
 
 def linear_ce_backward(g, x, w, targets, lse, ignore_index=-100, row_scale=None, need_x=True, need_w=True):
@@ -869,7 +875,8 @@ def linear_ce_backward(g, x, w, targets, lse, ignore_index=-100, row_scale=None,
     dx = torch.empty_like(x) if need_x else None
     dw = torch.empty_like(w) if need_w else None
     with _on(dev):
-        ws = _loss_workspace(T, h, V, NEED_LOSS_X * need_x | NEED_LOSS_W * need_w, dt, dev)
+        ws = torch.empty(_loss_workspace_bytes(T, h, V, NEED_LOSS_X * need_x | NEED_LOSS_W * need_w, dt, dev),
+                         dtype=torch.uint8, device=dev)
         check(lib.q38moe_linear_ce_backward(_ptr(g), g.dim() == 1, _ptr(row_scale), _ptr(x), _ptr(w), _ptr(targets),
                                             targets.dtype == torch.int64, ignore_index, _ptr(lse), _ptr(dx), _ptr(dw),
                                             T, h, V, _ptr(ws), ws.numel(), _DTYPES[dt], _stream(dev)),

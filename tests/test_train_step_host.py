@@ -43,8 +43,8 @@ def test_loss_shapes(T, h, V, dtype, msg):
 def test_loss_abi_arguments():
     m = _lib()
     lib, p = m.lib, ctypes.c_void_p(1 << 20)
-    fwd = lambda x, t, ws, n, T=4: lib.q38moe_linear_ce_forward(x, p, t, 1, -100, p, p, None, 0, T, 64, 10, ws, n,  # noqa: E731
-                                                                1, None)
+    fwd = lambda x, t, ws, n, T=4: lib.q38moe_linear_ce_forward(x, p, t, 1, -100, p, p, None, None, 0, T, 64, 10,  # noqa: E731
+                                                                ws, n, 1, None)
     assert fwd(None, p, p, 1 << 30) == -1 and "x must not be NULL" in lib.q38moe_last_error().decode()
     assert fwd(ctypes.c_void_p(8), p, p, 1 << 30) == -1 and "aligned" in lib.q38moe_last_error().decode()
     assert fwd(p, None, p, 1 << 30) == -1 and "targets" in lib.q38moe_last_error().decode()
