@@ -816,18 +816,25 @@ hipError_t ls_gemm(LsParams p, hipStream_t st) {
   return hipGetLastError();
 }
 
-// Tile side of the products over the vocabulary, whose tiles stay whole: 256 where such tiles fill at least half the CUs, 64 (with
-// eight steps in LDS) where tiles of 128 leave half the CUs without one, else 128.
-int tile_z(int64_t M, int64_t N) {
-  if (ceil_div(M, 256) * ceil_div(N, 256) * 2 >= device_cus()) return 256;
-  return ceil_div(M, 128) * ceil_div(N, 128) * 2 < device_cus() ? 64 : 128;
+// Tile side of the products over the vocabulary, whose tiles stay whole. bf16: a round of 256 x 256 tiles takes 30 us at h = 1024
+// and one of 128 x 128, two to a CU, 17 (16384 x 1024 x 10112: 302 and 350 us; 1777 tokens: 60 and 51; 300: 30 and 17; 64 x 64
+// tiles are never faster). fp32 multiplies at a sixteenth of the rate, so that a large tile's reuse is worth nothing and a
+// few tiles leave CUs without work: 64 where tiles of 128 reach at most half the CUs (61 x 1024 x 10112: 37 and 75 us with
+// the rest of the call; 300 tokens: 112 and 84), else 128.
+int tile_z(int64_t M, int64_t N, bool f32) {
+  const int64_t cus = device_cus(), n128 = ceil_div(M, 128) * ceil_div(N, 128);
+  if (f32) return 2 * n128 <= cus ? 64 : 128;
+  return 7 * ceil_div(ceil_div(M, 256) * ceil_div(N, 256), cus) <= 4 * ceil_div(n128, 2 * cus) ? 256 : 128;
 }
 
-// Of the gradients' products, whose tiles can be split over K: 256 where each CU has at least 12 steps of such tiles, 128 where
-// each has 6 of those.
-int tile_k(int64_t M, int64_t N, int64_t steps) {
-  if (ceil_div(M, 256) * ceil_div(N, 256) * steps >= (int64_t)12 * device_cus()) return 256;
-  return ceil_div(M, 128) * ceil_div(N, 128) * steps >= (int64_t)6 * device_cus() ? 128 : 64;
+// Of the gradients' products, whose tiles can be split over K. 64 (with eight steps in LDS) for few tiles of 128, or
+// for less than every CU's and little K (dx of 61 x 1024 x 10112: 37 and 49 us with the rest of the call, of 600 tokens
+// 88 and 63; dw of 1000 x 512 x 2000: 27 and 47). bf16: 256 where each CU has at least 12 steps of such tiles (dx of 300 x
+// 2048 x 50021: 231 us, with 128 292; of 1000 x 1024 x 10112 96 and 83); fp32 has no use for them.
+int tile_k(int64_t M, int64_t N, int64_t steps, bool f32) {
+  const int64_t cus = device_cus(), n128 = ceil_div(M, 128) * ceil_div(N, 128);
+  if (8 * n128 <= cus || (n128 < cus && n128 * steps < (f32 ? 16 : 8) * cus)) return 64;
+  return !f32 && ceil_div(M, 256) * ceil_div(N, 256) * steps >= 12 * cus ? 256 : 128;
 }
 
 // Bytes of a product's partial sums, and of its running sums.
@@ -864,7 +871,7 @@ Layout layout(int64_t T, int h, int V, bool f32, bool fwd, bool need_x, bool nee
   l.tgt = take(l.raw ? 0 : 4 * T);
   l.count = take(4);
   l.xc = take(l.raw ? 0 : esz * T * h);
-  l.tile_s = tile_z(V, T);
+  l.tile_s = tile_z(V, T, f32);
   if (fwd) {
     l.entries = (int)(2 * ceil_div(V, l.tile_s));
     l.part = take(8 * (size_t)l.entries * T);
@@ -882,9 +889,9 @@ Layout layout(int64_t T, int h, int V, bool f32, bool fwd, bool need_x, bool nee
     l.piece = pt * 256;
     l.s = take(esz * (size_t)T * l.piece);
     const int64_t bk = f32 ? 32 : 64, n = l.piece < V ? l.piece : V;
-    l.tile_s = tile_z(n, T);
-    l.tile_x = tile_k(h, T, ceil_div(n, bk));
-    l.tile_w = tile_k(h, n, ceil_div(T, bk));
+    l.tile_s = tile_z(n, T, f32);
+    l.tile_x = tile_k(h, T, ceil_div(n, bk), f32);
+    l.tile_w = tile_k(h, n, ceil_div(T, bk), f32);
     l.acc = take(need_x && l.pieces > 1 ? acc_bytes(h, T, l.tile_x) : 0);
     const size_t sx = need_x ? split_bytes(h, T, l.tile_x) : 0, sw = need_w ? split_bytes(h, n, l.tile_w) : 0;
     l.split = take(sx > sw ? sx : sw);
@@ -924,8 +931,11 @@ hipError_t ls_gather(const void* x, const int32_t* rows, const int32_t* count, v
 
 template <bool F32, int LA, int LB, int EPI>
 hipError_t ls_gemm_any(const LsParams& p, int tile, hipStream_t st) {
-  if (tile == 64) return ls_gemm<F32, 64, 64, LA, LB, EPI>(p, st);
-  return tile == 256 ? ls_gemm<F32, 256, 256, LA, LB, EPI>(p, st) : ls_gemm<F32, 128, 128, LA, LB, EPI>(p, st);
+  if constexpr (F32 || EPI == EPI_OUT)
+    if (tile == 64) return ls_gemm<F32, 64, 64, LA, LB, EPI>(p, st);
+  if constexpr (!F32)
+    if (tile == 256) return ls_gemm<F32, 256, 256, LA, LB, EPI>(p, st);
+  return ls_gemm<F32, 128, 128, LA, LB, EPI>(p, st);
 }
 
 template <bool F32>
