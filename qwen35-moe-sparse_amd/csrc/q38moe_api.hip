@@ -1706,9 +1706,50 @@ static int check_rows_args(int64_t T, int32_t h, int32_t E, int32_t k, int32_t w
   return Q38MOE_OK;
 }
 
+// Parts of a plan (see q38moe.h).
+struct RowsPlan {
+  int64_t E4, P4;
+  int64_t starts() const { return E4; }
+  int64_t perm() const { return 2 * E4; }
+  int64_t inv() const { return 2 * E4 + P4; }
+  int64_t hist() const { return 2 * E4 + 2 * P4; }
+};
+
+static RowsPlan rows_plan(int64_t T, int32_t E, int32_t k) { return {(E + 3) / 4 * 4, (T * k + 3) / 4 * 4}; }
+
+int64_t q38moe_rows_plan_ints(int64_t T, int32_t E, int32_t k) {
+  g_err[0] = 0;
+  if (check_routing(T, E, k) != Q38MOE_OK) return -1;
+  return rows_plan(T, E, k).hist() + (hist_blocks(T) > 0 ? hist_blocks(T) : 1) * E;
+}
+
+int q38moe_dispatch_rows(const void* x, const void* topk_idx, int32_t idx_is_int64, int32_t* plan, void* dst, int64_t T,
+                         int32_t h, int32_t E, int32_t k, int32_t dtype, void* stream) {
+  g_err[0] = 0;
+  Q38_CHECK(check_rows_args(T, h, E, k, dtype, nullptr, dtype));
+  if (plan == nullptr) return fail(Q38MOE_EINVAL, "plan must not be NULL");
+  if (T > 0) {
+    Q38_CHECK(check_ptr(x, "x"));
+    Q38_CHECK(check_ptr(dst, "dst"));
+    if (topk_idx == nullptr) return fail(Q38MOE_EINVAL, "topk_idx must not be NULL");
+  }
+  const RowsPlan L = rows_plan(T, E, k);
+  const bool idx64 = idx_is_int64 != 0;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  (void)hipGetLastError();
+  if (T > 0) Q38_HIP(q38::launch_histogram(topk_idx, idx64, plan + L.hist(), T, E, k, st), "histogram launch");
+  Q38_HIP(q38::launch_permute(topk_idx, idx64, plan + L.hist(), plan, plan + L.starts(), plan + L.perm(), plan + L.inv(),
+                              nullptr, nullptr, q38::gemm_block_m(), 0, 0, T, E, k, st),
+          "permute launch");
+  Q38_HIP(q38::launch_spread_rows(x, nullptr, false, nullptr, topk_idx, idx64, plan + L.inv(), plan + L.starts(), plan,
+                                  dst, nullptr, T, h, E, k, dtype == Q38MOE_BF16, st),
+          "dispatch rows launch");
+  return Q38MOE_OK;
+}
+
 int q38moe_spread_rows(const void* src, const void* w, int32_t w_dtype, const void* y, const void* topk_idx,
-                       int32_t idx_is_int64, const int32_t* inv, const int32_t* starts, const int32_t* counts,
-                       void* dst, void* dw, int64_t T, int32_t h, int32_t E, int32_t k, int32_t dtype, void* stream) {
+                       int32_t idx_is_int64, const int32_t* plan, void* dst, void* dw, int64_t T, int32_t h, int32_t E,
+                       int32_t k, int32_t dtype, void* stream) {
   g_err[0] = 0;
   Q38_CHECK(check_rows_args(T, h, E, k, w_dtype, w, dtype));
   if (dw != nullptr && (y == nullptr || w == nullptr)) return fail(Q38MOE_EINVAL, "dw needs y and w");
@@ -1716,28 +1757,29 @@ int q38moe_spread_rows(const void* src, const void* w, int32_t w_dtype, const vo
   Q38_CHECK(check_ptr(src, "src"));
   Q38_CHECK(check_opt_ptr(y, "y"));
   Q38_CHECK(check_opt_ptr(dst, "dst"));
-  if (topk_idx == nullptr || inv == nullptr || starts == nullptr || counts == nullptr)
-    return fail(Q38MOE_EINVAL, "topk_idx, inv, starts and counts must not be NULL");
+  if (topk_idx == nullptr || plan == nullptr) return fail(Q38MOE_EINVAL, "topk_idx and plan must not be NULL");
+  const RowsPlan L = rows_plan(T, E, k);
   (void)hipGetLastError();
   Q38_HIP(q38::launch_spread_rows(src, w, w_dtype == Q38MOE_FP32, dw != nullptr ? y : nullptr, topk_idx,
-                                  idx_is_int64 != 0, inv, starts, counts, dst, dw, T, h, E, k, dtype == Q38MOE_BF16,
-                                  static_cast<hipStream_t>(stream)),
+                                  idx_is_int64 != 0, plan + L.inv(), plan + L.starts(), plan, dst, dw, T, h, E, k,
+                                  dtype == Q38MOE_BF16, static_cast<hipStream_t>(stream)),
           "spread rows launch");
   return Q38MOE_OK;
 }
 
 int q38moe_collect_rows(const void* src, const void* w, int32_t w_dtype, const void* topk_idx, int32_t idx_is_int64,
-                        const int32_t* inv, void* out, int64_t T, int32_t h, int32_t E, int32_t k, int32_t dtype,
+                        const int32_t* plan, void* out, int64_t T, int32_t h, int32_t E, int32_t k, int32_t dtype,
                         void* stream) {
   g_err[0] = 0;
   Q38_CHECK(check_rows_args(T, h, E, k, w_dtype, w, dtype));
   if (T == 0) return Q38MOE_OK;
   Q38_CHECK(check_ptr(src, "src"));
   Q38_CHECK(check_ptr(out, "out"));
-  if (topk_idx == nullptr || inv == nullptr) return fail(Q38MOE_EINVAL, "topk_idx and inv must not be NULL");
+  if (topk_idx == nullptr || plan == nullptr) return fail(Q38MOE_EINVAL, "topk_idx and plan must not be NULL");
   (void)hipGetLastError();
-  Q38_HIP(q38::launch_collect_rows(src, w, w_dtype == Q38MOE_FP32, topk_idx, idx_is_int64 != 0, inv, out, T, h, E, k,
-                                   dtype == Q38MOE_BF16, static_cast<hipStream_t>(stream)),
+  Q38_HIP(q38::launch_collect_rows(src, w, w_dtype == Q38MOE_FP32, topk_idx, idx_is_int64 != 0,
+                                   plan + rows_plan(T, E, k).inv(), out, T, h, E, k, dtype == Q38MOE_BF16,
+                                   static_cast<hipStream_t>(stream)),
           "collect rows launch");
   return Q38MOE_OK;
 }

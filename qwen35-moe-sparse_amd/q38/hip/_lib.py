@@ -93,7 +93,9 @@ SIGNATURES = {
     "q38moe_grad_norm_workspace_bytes": (_c_int, [_c_i32, ctypes.POINTER(_c_size)]),
     "q38moe_grad_norm": (_c_int, [_vp, _vp, _vp, _c_i32, _c_i32, _vp, _vp, _c_size, _vp]),
     "q38moe_clip_grads": (_c_int, [_vp] * 5 + [_c_i32, _c_i32, ctypes.c_float, _vp, _vp, _c_size, _vp]),
-    "q38moe_spread_rows": (_c_int, [_vp, _vp, _c_i32, _vp, _vp, _c_i32] + [_vp] * 5 +
+    "q38moe_rows_plan_ints": (_c_i64, [_c_i64, _c_i32, _c_i32]),
+    "q38moe_dispatch_rows": (_c_int, [_vp, _vp, _c_i32, _vp, _vp, _c_i64, _c_i32, _c_i32, _c_i32, _c_i32, _vp]),
+    "q38moe_spread_rows": (_c_int, [_vp, _vp, _c_i32, _vp, _vp, _c_i32] + [_vp] * 3 +
                            [_c_i64, _c_i32, _c_i32, _c_i32, _c_i32, _vp]),
     "q38moe_collect_rows": (_c_int, [_vp, _vp, _c_i32, _vp, _c_i32, _vp, _vp, _c_i64, _c_i32, _c_i32, _c_i32, _c_i32,
                                      _vp]),

@@ -232,7 +232,7 @@ class HipDispatch(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, plan):
         ctx.plan = plan
-        return ops.spread_rows(x, plan)[0]
+        return ops.dispatch_rows(x, plan)
 
     @staticmethod
     @once_differentiable
@@ -266,8 +266,9 @@ def dispatch(x, topk_idx, num_experts):
     if x.dim() != 2 or topk_idx.dim() != 2 or topk_idx.shape[0] != x.shape[0]:
         raise ValueError(f"x must be [T,h] and topk_idx [T,k], got {tuple(x.shape)} and {tuple(topk_idx.shape)}")
     ops._fdt(x, "x")
-    plan = ops.rows_plan(topk_idx.contiguous(), num_experts)
-    return HipDispatch.apply(_aligned(x), plan), plan
+    plan = ops.RowsPlan(topk_idx.contiguous(), num_experts)
+    x = _aligned(x)
+    return (HipDispatch.apply(x, plan) if torch.is_grad_enabled() and x.requires_grad else ops.dispatch_rows(x, plan)), plan
 
 
 def combine(rows, topk_w, plan):
@@ -277,4 +278,7 @@ def combine(rows, topk_w, plan):
     dt = ops._fdt(rows, "rows")
     if dt == torch.float32 and topk_w.dtype == torch.bfloat16:
         topk_w = topk_w.float()
-    return HipCombine.apply(_aligned(rows), topk_w.contiguous(), plan)
+    rows, topk_w = _aligned(rows), topk_w.contiguous()
+    if torch.is_grad_enabled() and (rows.requires_grad or topk_w.requires_grad):
+        return HipCombine.apply(rows, topk_w, plan)
+    return ops.collect_rows(rows, plan, topk_w)

@@ -11,7 +11,6 @@ import contextlib
 import ctypes
 import functools
 import math
-from typing import NamedTuple
 
 import torch
 
@@ -805,6 +804,11 @@ NEED_LOSS_X, NEED_LOSS_W = 1, 2
 _NORMS = {1.0: 1, 2.0: 2, math.inf: 3}
 
 
+# The current stream's handle on a GPU of this index, without the Stream object that torch.cuda.current_stream makes (2 us).
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
 def _on(device):
     """The tensors' device as the current one, for launches on its stream."""
     return contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
@@ -852,9 +856,12 @@ def linear_ce_forward(x, w, targets, ignore_index=-100, reduction=None, want_lse
         row_scale = make((), dtype=torch.float32, device=dev) if want_lse else None
     with _on(dev):
         ws = torch.empty(_loss_workspace_bytes(T, h, V, 0, dt, dev), dtype=torch.uint8, device=dev)
-        check(lib.q38moe_linear_ce_forward(_ptr(x), _ptr(w), _ptr(targets), targets.dtype == torch.int64, ignore_index,
-                                           _ptr(loss), _ptr(lse), _ptr(reduced), _ptr(row_scale), reduction == "mean",
-                                           T, h, V, _ptr(ws), ws.numel(), _DTYPES[dt], _stream(dev)),
+        check(lib.q38moe_linear_ce_forward(x.data_ptr(), w.data_ptr(), targets.data_ptr(),
+                                           targets.dtype == torch.int64, ignore_index, loss.data_ptr(),
+                                           None if lse is None else lse.data_ptr(),
+                                           None if reduced is None else reduced.data_ptr(),
+                                           None if row_scale is None else row_scale.data_ptr(), reduction == "mean",
+                                           T, h, V, ws.data_ptr(), ws.numel(), _DTYPES[dt], _raw_stream(dev.index)),
               "q38moe_linear_ce_forward")
     return loss, lse, reduced, row_scale
 
@@ -877,60 +884,70 @@ def linear_ce_backward(g, x, w, targets, lse, ignore_index=-100, row_scale=None,
     with _on(dev):
         ws = torch.empty(_loss_workspace_bytes(T, h, V, NEED_LOSS_X * need_x | NEED_LOSS_W * need_w, dt, dev),
                          dtype=torch.uint8, device=dev)
-        check(lib.q38moe_linear_ce_backward(_ptr(g), g.dim() == 1, _ptr(row_scale), _ptr(x), _ptr(w), _ptr(targets),
-                                            targets.dtype == torch.int64, ignore_index, _ptr(lse), _ptr(dx), _ptr(dw),
-                                            T, h, V, _ptr(ws), ws.numel(), _DTYPES[dt], _stream(dev)),
-              "q38moe_linear_ce_backward")
+        check(lib.q38moe_linear_ce_backward(g.data_ptr(), g.dim() == 1,
+                                            None if row_scale is None else row_scale.data_ptr(), x.data_ptr(),
+                                            w.data_ptr(), targets.data_ptr(), targets.dtype == torch.int64,
+                                            ignore_index, lse.data_ptr(), dx.data_ptr() if need_x else None,
+                                            dw.data_ptr() if need_w else None, T, h, V, ws.data_ptr(), ws.numel(),
+                                            _DTYPES[dt], _raw_stream(dev.index)), "q38moe_linear_ce_backward")
     return dx, dw
 
 
-def _norm_args(tensors, norm_type):
-    norm = _NORMS.get(float(norm_type))
-    if norm is None:
-        raise ValueError(f"norm_type must be 1, 2 or inf, got {norm_type!r}")
-    dtypes = []
-    dev = None
+def _norm_args(tensors):
+    """The tensors' device and, as C arrays, their addresses, sizes and dtypes. (Whole lists at a time: a loop over the
+    tensors' attributes costs the host 1 us a tensor.)"""
     for t in tensors:
-        code = _DTYPES.get(t.dtype) if isinstance(t, torch.Tensor) else None
-        if code is None:
-            raise TypeError(f"gradients must be bf16 or fp32 tensors, got {getattr(t, 'dtype', type(t))}")
-        if t.layout is not torch.strided:
-            raise TypeError(f"gradients must be dense, got {t.layout}")
-        if not t.is_cuda:
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"gradients must be bf16 or fp32 tensors, got {type(t)}")
+    dtypes = [t.dtype for t in tensors]
+    for dt in set(dtypes):
+        if dt not in _DTYPES:
+            raise TypeError(f"gradients must be bf16 or fp32 tensors, got {dt}")
+    for layout in {t.layout for t in tensors}:
+        if layout is not torch.strided:
+            raise TypeError(f"gradients must be dense, got {layout}")
+    devices = {t.device for t in tensors}
+    dev = tensors[0].device
+    if dev.type != "cuda" or len(devices) > 1:
+        if any(d.type != "cuda" for d in devices):
             raise RuntimeError("gradients must be CUDA/HIP tensors")
-        if not t.is_contiguous():
-            raise ValueError(f"gradients must be contiguous, got strides {t.stride()} for {tuple(t.shape)}")
-        if dev is None:
-            dev = t.device
-        elif t.device != dev:
-            raise RuntimeError(f"gradients must be on one device, got {dev} and {t.device}")
-        dtypes.append(code)
-    n = len(dtypes)
-    ptrs = (ctypes.c_void_p * n)(*[t.data_ptr() for t in tensors])
-    sizes = (ctypes.c_int64 * n)(*[t.numel() for t in tensors])
-    return norm, dev, n, ptrs, sizes, (ctypes.c_int32 * n)(*dtypes)
+        raise RuntimeError(f"gradients must be on one device, got {sorted(map(str, devices))}")
+    if not all(map(torch.Tensor.is_contiguous, tensors)):
+        bad = next(t for t in tensors if not t.is_contiguous())
+        raise ValueError(f"gradients must be contiguous, got strides {bad.stride()} for {tuple(bad.shape)}")
+    n = len(tensors)
+    return (dev, (ctypes.c_void_p * n)(*map(torch.Tensor.data_ptr, tensors)),
+            (ctypes.c_int64 * n)(*map(torch.Tensor.numel, tensors)), (ctypes.c_int32 * n)(*map(_DTYPES.get, dtypes)))
 
 
-def _norm_workspace(n, dev):
+def _norm_code(norm_type):
+    code = _NORMS.get(float(norm_type))
+    if code is None:
+        raise ValueError(f"norm_type must be 1, 2 or inf, got {norm_type!r}")
+    return code
+
+
+@functools.lru_cache(maxsize=64)
+def _norm_workspace_bytes(n):
     b = ctypes.c_size_t()
     check(lib.q38moe_grad_norm_workspace_bytes(n, ctypes.byref(b)), "q38moe_grad_norm_workspace_bytes")
-    return torch.empty(b.value, dtype=torch.uint8, device=dev)
+    return b.value
 
 
 def grad_norm(grads, norm_type=2.0):
     """Global norm (p = 1, 2 or inf) of all elements of the tensors in ``grads`` (bf16 or fp32, contiguous, on one
     GPU), summed in fp64: an fp32 scalar on their device (q38moe_grad_norm). Without tensors, 0 on the CPU."""
     grads = list(grads)
+    norm = _norm_code(norm_type)
     if not grads:
-        if float(norm_type) not in _NORMS:
-            raise ValueError(f"norm_type must be 1, 2 or inf, got {norm_type!r}")
         return torch.tensor(0.0)
-    norm, dev, n, ptrs, sizes, dts = _norm_args(grads, norm_type)
+    dev, ptrs, sizes, dts = _norm_args(grads)
+    n = len(grads)
     with _on(dev):
         total = torch.empty((), dtype=torch.float32, device=dev)
-        ws = _norm_workspace(n, dev)
-        check(lib.q38moe_grad_norm(ptrs, sizes, dts, n, norm, _ptr(total), _ptr(ws), ws.numel(), _stream(dev)),
-              "q38moe_grad_norm")
+        ws = torch.empty(_norm_workspace_bytes(n), dtype=torch.uint8, device=dev)
+        check(lib.q38moe_grad_norm(ptrs, sizes, dts, n, norm, total.data_ptr(), ws.data_ptr(), ws.numel(),
+                                   _raw_stream(dev.index)), "q38moe_grad_norm")
     return total
 
 
@@ -945,22 +962,24 @@ def clip_grads(grads, max_norm, norm_type=2.0, out=None):
         raise ValueError(f"out must hold {len(grads)} tensors, got {len(outs)}")
     if not max_norm >= 0:
         raise ValueError(f"max_norm must be >= 0, got {max_norm}")
+    norm = _norm_code(norm_type)
     if not grads:
-        return grad_norm(grads, norm_type)
-    norm, dev, n, ptrs, sizes, dts = _norm_args(grads, norm_type)
+        return torch.tensor(0.0)
+    dev, ptrs, sizes, dts = _norm_args(grads)
+    n = len(grads)
     optrs, odts = ptrs, dts
     if out is not None:
-        _, odev, _, optrs, _, odts = _norm_args(outs, norm_type)
+        odev, optrs, _, odts = _norm_args(outs)
         if odev != dev:
             raise RuntimeError(f"out must be on {dev}, got {odev}")
-        for g, o in zip(grads, outs):
-            if g.shape != o.shape:
-                raise ValueError(f"out must have the gradients' shapes, got {tuple(o.shape)} for {tuple(g.shape)}")
+        if [g.shape for g in grads] != [o.shape for o in outs]:
+            g, o = next((g, o) for g, o in zip(grads, outs) if g.shape != o.shape)
+            raise ValueError(f"out must have the gradients' shapes, got {tuple(o.shape)} for {tuple(g.shape)}")
     with _on(dev):
         total = torch.empty((), dtype=torch.float32, device=dev)
-        ws = _norm_workspace(n, dev)
-        check(lib.q38moe_clip_grads(ptrs, optrs, sizes, dts, odts, n, norm, max_norm, _ptr(total), _ptr(ws), ws.numel(),
-                                    _stream(dev)), "q38moe_clip_grads")
+        ws = torch.empty(_norm_workspace_bytes(n), dtype=torch.uint8, device=dev)
+        check(lib.q38moe_clip_grads(ptrs, optrs, sizes, dts, odts, n, norm, max_norm, total.data_ptr(), ws.data_ptr(),
+                                    ws.numel(), _raw_stream(dev.index)), "q38moe_clip_grads")
     torch.autograd.graph.increment_version(outs)
     return total
 
@@ -985,37 +1004,50 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
     return total
 
 
-class RowsPlan(NamedTuple):
-    """Where the pairs of a routing [T,k] go: expert e's rows are starts[e] .. starts[e] + counts[e] - 1, row r is pair
-    perm[r] (token perm[r] // k; only rows that are filled), pair p is row inv[p] (only pairs routed inside [0, E))."""
+class RowsPlan:
+    """Where the pairs of a routing idx [T,k] go: expert e's rows are starts[e] .. starts[e] + counts[e] - 1, row r is pair
+    perm[r] (token perm[r] // k; only rows that are filled), pair p is row inv[p] (only pairs routed inside [0, experts)).
+    ``dispatch_rows`` fills it."""
 
-    idx: torch.Tensor
-    counts: torch.Tensor
-    starts: torch.Tensor
-    perm: torch.Tensor
-    inv: torch.Tensor
-    experts: int
+    __slots__ = ("idx", "experts", "buffer")
+
+    def __init__(self, topk_idx, experts):
+        _need(topk_idx, "topk_idx", dtype=None, ndim=2)
+        _idx_flag(topk_idx)
+        n = lib.q38moe_rows_plan_ints(*topk_idx.shape[:1], experts, topk_idx.shape[1])
+        check(min(n, 0), "q38moe_rows_plan_ints")
+        self.idx, self.experts = topk_idx, experts
+        self.buffer = torch.empty(n, dtype=torch.int32, device=topk_idx.device)
+
+    def _part(self, i):
+        E4, P = -(-self.experts // 4) * 4, self.idx.numel()
+        start = (0, E4, 2 * E4, 2 * E4 + -(-P // 4) * 4)[i]
+        return self.buffer[start:start + (self.experts if i < 2 else P)]
+
+    counts = property(lambda self: self._part(0))
+    starts = property(lambda self: self._part(1))
+    perm = property(lambda self: self._part(2))
+    inv = property(lambda self: self._part(3))
 
 
-def rows_plan(topk_idx, experts):
-    """The stable sort of routing indices [T,k] (int32 or int64) by expert (q38moe_histogram, q38moe_permute)."""
-    _need(topk_idx, "topk_idx", dtype=None, ndim=2)
-    flag = _idx_flag(topk_idx)
-    T, k = topk_idx.shape
-    dev = topk_idx.device
-    nb = max((T + 63) // 64, 1)
-    # One allocation, each part on a 16-byte boundary.
-    E4, P4 = -(-experts // 4) * 4, -(-T * k // 4) * 4
-    buf = torch.empty(2 * E4 + 2 * P4 + nb * experts, dtype=torch.int32, device=dev)
-    counts, starts = buf[:experts], buf[E4:E4 + experts]
-    perm, inv = buf[2 * E4:2 * E4 + T * k], buf[2 * E4 + P4:2 * E4 + P4 + T * k]
-    hist = buf[2 * E4 + 2 * P4:]
+def dispatch_rows(x, plan):
+    """Fills the plan (the stable sort of its indices by expert) and returns the tokens x [T,h] in expert order, [T*k,h]
+    with zeros behind the filled rows (q38moe_dispatch_rows)."""
+    dt = _fdt(x, "x")
+    _need(x, "x", dtype=dt, ndim=2)
+    T, h = x.shape
+    k = plan.idx.shape[1]
+    if plan.idx.shape[0] != T:
+        raise ValueError(f"x must hold {plan.idx.shape[0]} tokens, got {T}")
+    dev = x.device
+    if plan.buffer.device != dev:
+        raise RuntimeError("x and the routing must be on one device")
+    dst = torch.empty(T * k, h, dtype=dt, device=dev)
     with _on(dev):
-        st = _stream(dev)
-        check(lib.q38moe_histogram(_ptr(topk_idx), flag, _ptr(hist), T, experts, k, st), "q38moe_histogram")
-        check(lib.q38moe_permute(_ptr(topk_idx), flag, _ptr(hist), _ptr(counts), _ptr(starts), _ptr(perm), _ptr(inv),
-                                 None, None, 0, T, experts, k, st), "q38moe_permute")
-    return RowsPlan(topk_idx, counts, starts, perm, inv, experts)
+        check(lib.q38moe_dispatch_rows(x.data_ptr(), plan.idx.data_ptr(), _idx_flag(plan.idx), plan.buffer.data_ptr(),
+                                       dst.data_ptr(), T, h, plan.experts, k, _DTYPES[dt], _raw_stream(dev.index)),
+              "q38moe_dispatch_rows")
+    return dst
 
 
 def _rows_weights(w, shape, dt):
@@ -1024,7 +1056,7 @@ def _rows_weights(w, shape, dt):
         raise TypeError(f"weights must be {dt} or fp32, got {w.dtype}")
     if w.shape != shape:
         raise ValueError(f"weights must be {tuple(shape)}, got {tuple(w.shape)}")
-    return w
+    return w.data_ptr()
 
 
 def spread_rows(src, plan, w=None, y=None, need_rows=True):
@@ -1034,21 +1066,24 @@ def spread_rows(src, plan, w=None, y=None, need_rows=True):
     _need(src, "src", dtype=dt, ndim=2)
     T, k = plan.idx.shape
     h = src.shape[1]
+    dev = src.device
     if src.shape[0] != T:
         raise ValueError(f"src must hold {T} tokens, got {src.shape[0]}")
-    if w is not None:
-        _rows_weights(w, plan.idx.shape, dt)
+    if plan.buffer.device != dev:
+        raise RuntimeError("src and the plan must be on one device")
+    pw = None if w is None else _rows_weights(w, plan.idx.shape, dt)
     if y is not None:
         _same(y, "y", dt, (T * k, h))
         if w is None:
             raise ValueError("y needs weights")
-    dst = torch.empty(T * k, h, dtype=dt, device=src.device) if need_rows else None
+    dst = torch.empty(T * k, h, dtype=dt, device=dev) if need_rows else None
     dw = torch.empty_like(w) if y is not None else None
-    with _on(src.device):
-        check(lib.q38moe_spread_rows(_ptr(src), _ptr(w), _DTYPES[dt if w is None else w.dtype], _ptr(y),
-                                     _ptr(plan.idx), _idx_flag(plan.idx), _ptr(plan.inv), _ptr(plan.starts),
-                                     _ptr(plan.counts), _ptr(dst), _ptr(dw), T, h, plan.experts, k, _DTYPES[dt],
-                                     _stream(src.device)), "q38moe_spread_rows")
+    with _on(dev):
+        check(lib.q38moe_spread_rows(src.data_ptr(), pw, _DTYPES[dt if w is None else w.dtype],
+                                     None if y is None else y.data_ptr(), plan.idx.data_ptr(), _idx_flag(plan.idx),
+                                     plan.buffer.data_ptr(), dst.data_ptr() if need_rows else None,
+                                     None if dw is None else dw.data_ptr(), T, h, plan.experts, k, _DTYPES[dt],
+                                     _raw_stream(dev.index)), "q38moe_spread_rows")
     return dst, dw
 
 
@@ -1059,13 +1094,15 @@ def collect_rows(rows, plan, w=None):
     T, k = plan.idx.shape
     _need(rows, "rows", dtype=dt, ndim=2)
     h = rows.shape[1]
+    dev = rows.device
     if rows.shape[0] != T * k:
         raise ValueError(f"rows must hold {T * k} rows, got {rows.shape[0]}")
-    if w is not None:
-        _rows_weights(w, plan.idx.shape, dt)
-    out = torch.empty(T, h, dtype=dt, device=rows.device)
-    with _on(rows.device):
-        check(lib.q38moe_collect_rows(_ptr(rows), _ptr(w), _DTYPES[dt if w is None else w.dtype], _ptr(plan.idx),
-                                      _idx_flag(plan.idx), _ptr(plan.inv), _ptr(out), T, h, plan.experts, k,
-                                      _DTYPES[dt], _stream(rows.device)), "q38moe_collect_rows")
+    if plan.buffer.device != dev:
+        raise RuntimeError("rows and the plan must be on one device")
+    pw = None if w is None else _rows_weights(w, plan.idx.shape, dt)
+    out = torch.empty(T, h, dtype=dt, device=dev)
+    with _on(dev):
+        check(lib.q38moe_collect_rows(rows.data_ptr(), pw, _DTYPES[dt if w is None else w.dtype], plan.idx.data_ptr(),
+                                      _idx_flag(plan.idx), plan.buffer.data_ptr(), out.data_ptr(), T, h, plan.experts,
+                                      k, _DTYPES[dt], _raw_stream(dev.index)), "q38moe_collect_rows")
     return out

@@ -161,8 +161,8 @@ def test_captured_and_on_another_stream(gpu):
     x, idx, w, y, _, d_out = _inputs(200, 128, 16, 4, torch.bfloat16, gpu, 0.1)
 
     def step():
-        plan = ops.rows_plan(idx, 16)
-        return (ops.spread_rows(x, plan)[0], ops.collect_rows(y, plan, w), plan.counts,
+        plan = ops.RowsPlan(idx, 16)
+        return (ops.dispatch_rows(x, plan), ops.collect_rows(y, plan, w), plan.counts,
                 *ops.spread_rows(d_out, plan, w, y))
 
     eager = [t.clone() for t in step()]
