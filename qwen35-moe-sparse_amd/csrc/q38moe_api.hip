@@ -1681,18 +1681,17 @@ int q38moe_clip_grads(const void* const* src, void* const* dst, const int64_t* n
   double* ws = static_cast<double*>(workspace);
   int partials = 0;
   Q38_CHECK(norm_partials(src, numel, src_dtype, n, norm, ws, &partials, st));
-  if (partials == 0) {
-    Q38_HIP(q38::launch_norm_finish(ws, 0, norm, total, st), "gradient norm launch");
-    return Q38MOE_OK;
+  // One launch's partial sums are summed by the blocks that use them, more (or none) once beforehand.
+  if (partials > q38::CLIP_BLOCKS || partials == 0) {
+    Q38_HIP(q38::launch_norm_finish(ws, partials, norm, total, st), "gradient norm launch");
+    if (partials == 0) return Q38MOE_OK;
+    partials = 0;
   }
   q38::ClipTable t;
-  bool first = true;
   for (int32_t i = 0; i < n;) {
     i = clip_table(t, i, src, dst, numel, src_dtype, dst_dtype, n);
     if (t.n == 0) continue;
-    Q38_HIP(q38::launch_clip_scale(t, ws, partials, norm, max_norm, in_place, first ? total : nullptr, st),
-            "gradient clipping launch");
-    first = false;
+    Q38_HIP(q38::launch_clip_scale(t, ws, partials, norm, max_norm, in_place, total, st), "gradient clipping launch");
   }
   return Q38MOE_OK;
 }

@@ -163,43 +163,46 @@ __global__ __launch_bounds__(256) void norm_finish_kernel(const double* __restri
   if (threadIdx.x == 0) *norm = v;
 }
 
+// 4 elements as floats, and back: 8 or 16 bytes per lane, a wave's instruction whole lines either way.
+__device__ __forceinline__ f32x4_t load4(const float* p) {
+  return __builtin_nontemporal_load(reinterpret_cast<const f32x4_t*>(p));
+}
+typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ f32x4_t load4(const uint16_t* p) {
+  const u32x2_t v = __builtin_nontemporal_load(reinterpret_cast<const u32x2_t*>(p));
+  f32x4_t f;
+  float a, b;
+  unpack_bf16x2(v[0], a, b);
+  f[0] = a;
+  f[1] = b;
+  unpack_bf16x2(v[1], a, b);
+  f[2] = a;
+  f[3] = b;
+  return f;
+}
+__device__ __forceinline__ void store4(float* p, f32x4_t f) {
+  __builtin_nontemporal_store(f, reinterpret_cast<f32x4_t*>(p));
+}
+__device__ __forceinline__ void store4(uint16_t* p, f32x4_t f) {
+  __builtin_nontemporal_store((u32x2_t){pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3])},
+                              reinterpret_cast<u32x2_t*>(p));
+}
+
 template <typename S, typename D>
 __device__ __forceinline__ void chunk_scale(const S* p, D* o, int n, float c) {
   const int tid = threadIdx.x;
   int i = 0;
-  if (((reinterpret_cast<uintptr_t>(p) | reinterpret_cast<uintptr_t>(o)) & 15) == 0) {
-    for (; i + 8 * tid + 8 <= n; i += 2048) {
-      const int at = i + 8 * tid;
-      float f[8];
-      if constexpr (sizeof(S) == 2) {
-        const u32x4_t v = ld16(p + at);
+  if ((reinterpret_cast<uintptr_t>(p) & (4 * sizeof(S) - 1)) == 0 &&
+      (reinterpret_cast<uintptr_t>(o) & (4 * sizeof(D) - 1)) == 0) {
+    for (; i + 4096 <= n; i += 4096) {
+      f32x4_t f[4];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) unpack_bf16x2(v[q], f[2 * q], f[2 * q + 1]);
-      } else {
-        const u32x4_t v = ld16(p + at), w = ld16(p + at + 4);
+      for (int u = 0; u < 4; ++u) f[u] = load4(p + i + 1024 * u + 4 * tid);
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          f[q] = __uint_as_float(v[q]);
-          f[4 + q] = __uint_as_float(w[q]);
-        }
-      }
-#pragma unroll
-      for (int q = 0; q < 8; ++q) f[q] *= c;
-      if constexpr (sizeof(D) == 2) {
-        st16(o + at, (u32x4_t){pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]),
-                               pack_bf16x2(f[6], f[7])});
-      } else {
-        u32x4_t v, w;
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          v[q] = __float_as_uint(f[q]);
-          w[q] = __float_as_uint(f[4 + q]);
-        }
-        st16(o + at, v);
-        st16(o + at + 4, w);
-      }
+      for (int u = 0; u < 4; ++u) store4(o + i + 1024 * u + 4 * tid, f[u] * c);
     }
-    i = n & ~7;
+    for (; i + 4 * tid + 4 <= n; i += 1024) store4(o + i + 4 * tid, load4(p + i + 4 * tid) * c);
+    i = n & ~3;
   }
   for (int j = i + tid; j < n; j += 256) {
     float f;
@@ -211,14 +214,21 @@ __device__ __forceinline__ void chunk_scale(const S* p, D* o, int n, float c) {
   }
 }
 
-// out = g * coefficient; the norm comes from all launches' partials, summed by every block for itself, and block 0 of the
-// first launch stores it. In place with a coefficient of 1 nothing is written (the tensors already hold the result).
+// out = g * coefficient. The norm comes from the partials, summed by every block for itself, and block 0 stores it in *norm; or from
+// *norm where there are none (more than one launch's partials are summed once instead). A block takes the chunks of its
+// run backwards: the last ones that the first pass read are still in the caches. In place with a coefficient of 1
+// nothing is written (the tensors already hold the result).
 __global__ __launch_bounds__(256) void clip_scale_kernel(const ClipTable t, const double* __restrict__ partial,
                                                          int npartial, int ord, float max_norm, bool in_place,
                                                          float* __restrict__ norm) {
   __shared__ double lds[4];
-  const float N = norm_of(partial, npartial, ord, lds);
-  if (blockIdx.x == 0 && threadIdx.x == 0 && norm != nullptr) *norm = N;
+  float N;
+  if (npartial > 0) {
+    N = norm_of(partial, npartial, ord, lds);
+    if (blockIdx.x == 0 && threadIdx.x == 0) *norm = N;
+  } else {
+    N = *norm;
+  }
   const float ratio = max_norm / (N + 1e-6f);
   const float c = ratio > 1.0f ? 1.0f : ratio;  // a NaN stays one
   if (in_place && c == 1.0f) return;
@@ -226,9 +236,9 @@ __global__ __launch_bounds__(256) void clip_scale_kernel(const ClipTable t, cons
   const int64_t per = (chunks + gridDim.x - 1) / gridDim.x;
   const int64_t c0 = (int64_t)blockIdx.x * per, c1 = min(c0 + per, chunks);
   if (c0 >= c1) return;
-  int i = tensor_of(t, c0);
-  for (int64_t k = c0; k < c1; ++k) {
-    while (k >= t.first[i + 1]) ++i;
+  int i = tensor_of(t, c1 - 1);
+  for (int64_t k = c1 - 1; k >= c0; --k) {
+    while (k < t.first[i]) --i;
     const int64_t at = (k - t.first[i]) * CLIP_CHUNK;
     const int n = (int)min((int64_t)CLIP_CHUNK, t.numel[i] - at);
     if (t.src_f32[i]) {

@@ -6,9 +6,11 @@
 //   collect:  out[t] = sum_j src[inv[p]] (* w[p])
 //
 // spread without w is the dispatch, collect without w its gradient; collect with w is the combine, spread with
-// w and y its gradients. Products and sums are fp32, each output is rounded once. Both run one wave per token: the
-// token's k rows of a column chunk are loaded before any is used, so k 16-byte loads per lane are in flight, and the
-// token's own row moves once. Both are bound by memory.
+// w and y its gradients. Products and sums are fp32, each output is rounded once. Both run one wave per token: a wave's
+// instruction covers 1 KiB of a row, and the loads of two such pieces of all k rows are issued before any is used. Both are bound
+// by memory: 16384 tokens of 1024 bf16 by 5 take 36 us there (201 MB, 5.6 TB/s), 35 back, and 68 for both gradients of the
+// combine (369 MB, 5.4 TB/s). Rows are written past the caches, which the next reader's 168 MB would not find there anyway:
+// through them the four passes take 195 us together instead of 174.
 #include <type_traits>
 
 #include "q38moe_common.h"
@@ -84,38 +86,50 @@ __global__ __launch_bounds__(256) void spread_kernel(const E* __restrict__ src, 
     s[j] = w != nullptr ? weight_of(w, w_f32, t * KT + j) : 1.0f;
     acc[j] = 0.0f;
   }
-  for (int c = lane * VEC<E>; c < h; c += 64 * VEC<E>) {
-    const u32x4_t a = ld16(src + t * h + c);
-    float f[VEC<E>];
-    unpack16<E>(a, f);
-    if (y != nullptr) {
-      u32x4_t b[KT];
+  // U pieces of the row at c, c + 64 VEC, ...
+  auto piece = [&](auto pieces, int c) {
+    constexpr int U = decltype(pieces)::value, P = 64 * VEC<E>;
+    u32x4_t a[U], b[U][KT];
 #pragma unroll
-      for (int j = 0; j < KT; ++j) b[j] = row[j] >= 0 ? ld16(y + row[j] * h + c) : (u32x4_t){0u, 0u, 0u, 0u};
+    for (int u = 0; u < U; ++u) {
+      a[u] = ld16(src + t * h + c + u * P);
+      if (y != nullptr) {
 #pragma unroll
-      for (int j = 0; j < KT; ++j) {
-        if (row[j] < 0) continue;
-        float g[VEC<E>];
-        unpack16<E>(b[j], g);
-#pragma unroll
-        for (int i = 0; i < VEC<E>; ++i) acc[j] = fmaf(f[i], g[i], acc[j]);
+        for (int j = 0; j < KT; ++j)
+          b[u][j] = row[j] >= 0 ? ld16_stream(y + row[j] * h + c + u * P) : (u32x4_t){0u, 0u, 0u, 0u};
       }
     }
-    if (dst != nullptr) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      float f[VEC<E>];
+      unpack16<E>(a[u], f);
 #pragma unroll
       for (int j = 0; j < KT; ++j) {
         if (row[j] < 0) continue;
-        u32x4_t v = a;
-        if (w != nullptr) {
+        if (y != nullptr) {
           float g[VEC<E>];
+          unpack16<E>(b[u][j], g);
 #pragma unroll
-          for (int i = 0; i < VEC<E>; ++i) g[i] = f[i] * s[j];
-          v = pack16<E>(g);
+          for (int i = 0; i < VEC<E>; ++i) acc[j] = fmaf(f[i], g[i], acc[j]);
         }
-        st16(dst + row[j] * h + c, v);
+        if (dst != nullptr) {
+          u32x4_t v = a[u];
+          if (w != nullptr) {
+            float g[VEC<E>];
+#pragma unroll
+            for (int i = 0; i < VEC<E>; ++i) g[i] = f[i] * s[j];
+            v = pack16<E>(g);
+          }
+          st16_stream(dst + row[j] * h + c + u * P, v);
+        }
       }
     }
-  }
+  };
+  // (Two pieces of y's rows at a time cost more registers than they hide: both gradients 75 us against 67.)
+  int c = lane * VEC<E>;
+  if (y == nullptr)
+    for (; c + 64 * VEC<E> < h; c += 128 * VEC<E>) piece(std::integral_constant<int, 2>{}, c);
+  for (; c < h; c += 64 * VEC<E>) piece(std::integral_constant<int, 1>{}, c);
   if (dw != nullptr) {
 #pragma unroll
     for (int j = 0; j < KT; ++j) {
@@ -150,23 +164,33 @@ __global__ __launch_bounds__(256) void collect_kernel(const E* __restrict__ src,
   float s[KT];
 #pragma unroll
   for (int j = 0; j < KT; ++j) s[j] = w != nullptr ? weight_of(w, w_f32, t * KT + j) : 1.0f;
-  for (int c = lane * VEC<E>; c < h; c += 64 * VEC<E>) {
-    u32x4_t b[KT];
+  auto piece = [&](auto pieces, int c) {
+    constexpr int U = decltype(pieces)::value, P = 64 * VEC<E>;
+    u32x4_t b[U][KT];
 #pragma unroll
-    for (int j = 0; j < KT; ++j) b[j] = row[j] >= 0 ? ld16(src + row[j] * h + c) : (u32x4_t){0u, 0u, 0u, 0u};
-    float a[VEC<E>];
+    for (int u = 0; u < U; ++u)
 #pragma unroll
-    for (int i = 0; i < VEC<E>; ++i) a[i] = 0.0f;
+      for (int j = 0; j < KT; ++j)
+        b[u][j] = row[j] >= 0 ? ld16_stream(src + row[j] * h + c + u * P) : (u32x4_t){0u, 0u, 0u, 0u};
 #pragma unroll
-    for (int j = 0; j < KT; ++j) {
-      if (row[j] < 0) continue;  // its weight may be anything
-      float g[VEC<E>];
-      unpack16<E>(b[j], g);
+    for (int u = 0; u < U; ++u) {
+      float a[VEC<E>];
 #pragma unroll
-      for (int i = 0; i < VEC<E>; ++i) a[i] = fmaf(g[i], s[j], a[i]);
+      for (int i = 0; i < VEC<E>; ++i) a[i] = 0.0f;
+#pragma unroll
+      for (int j = 0; j < KT; ++j) {
+        if (row[j] < 0) continue;  // its weight may be anything
+        float g[VEC<E>];
+        unpack16<E>(b[u][j], g);
+#pragma unroll
+        for (int i = 0; i < VEC<E>; ++i) a[i] = fmaf(g[i], s[j], a[i]);
+      }
+      st16(out + t * h + c + u * P, pack16<E>(a));
     }
-    st16(out + t * h + c, pack16<E>(a));
-  }
+  };
+  int c = lane * VEC<E>;
+  for (; c + 64 * VEC<E> < h; c += 128 * VEC<E>) piece(std::integral_constant<int, 2>{}, c);
+  if (c < h) piece(std::integral_constant<int, 1>{}, c);
 }
 
 template <typename E, typename IdxT>
