@@ -227,7 +227,10 @@ class Qwen3_8MoeForCausalLM(Qwen3_8MoePreTrainedModel):
     """Causal LM head over the Q38 trunk for uncached packed prefill (modeling:1358-1433): the same
     module tree and parameter names as the reference (``model.*``, tied ``lm_head``), the MoE blocks
     on the fused HIP block. ``forward(input_ids, output_router_logits=None, logits_to_keep=0)``
-    returns logits (and with router logits, the load-balancing loss) in a MoeCausalLMOutputWithPast."""
+    returns logits (and with router logits, the load-balancing loss) in a MoeCausalLMOutputWithPast.
+    With ``labels`` [B,S] (-100 where nothing counts) it returns the next-token loss too, taken from the
+    hidden states without logits; ``router_aux_loss_coef`` times the load-balancing loss is added where
+    that is made. ``logits_to_keep=None`` with labels makes no logits at all."""
 
     _tied_weights_keys = {"lm_head.weight": "model.embed_tokens.weight"}
 
@@ -247,18 +250,27 @@ class Qwen3_8MoeForCausalLM(Qwen3_8MoePreTrainedModel):
     def _moe(self, block, x, with_router):
         return hip_moe_block_forward_with_router(block, x) if with_router else block(x)
 
-    def forward(self, input_ids=None, output_router_logits=None, logits_to_keep=0, **kwargs):
+    def forward(self, input_ids=None, output_router_logits=None, logits_to_keep=0, labels=None, **kwargs):
         if input_ids is None or kwargs.get("past_key_values") is not None or kwargs.get("attention_mask") is not None:
             raise ValueError("Q38 supports uncached packed prefill from input_ids without attention_mask")
+        if labels is not None and labels.shape != input_ids.shape:
+            raise ValueError(f"labels {tuple(labels.shape)} do not match input_ids {tuple(input_ids.shape)}")
         want = self.config.output_router_logits if output_router_logits is None else output_router_logits
         router = [] if want else None
         cfg = self.prefill_config
         with torch.no_grad():
             hs = _prefill.trunk_forward(self.model, cfg, input_ids, self._moe, router)
-            keep = slice(-logits_to_keep, None) if isinstance(logits_to_keep, int) else logits_to_keep
-            logits = self.lm_head(hs[:, keep, :])
+            logits = loss = None
+            if labels is None or logits_to_keep is not None:
+                keep = slice(-logits_to_keep, None) if isinstance(logits_to_keep, int) else logits_to_keep
+                logits = self.lm_head(hs[:, keep, :])
             aux = _prefill.load_balancing_loss(router, cfg.experts, cfg.topk) if want else None
-        return MoeCausalLMOutputWithPast(logits=logits, aux_loss=aux, router_logits=tuple(router) if want else None)
+            if labels is not None:
+                loss = _prefill.next_token_loss(hs, self.lm_head.weight, labels.to(hs.device))
+                if want:
+                    loss = loss + self.config.router_aux_loss_coef * aux
+        return MoeCausalLMOutputWithPast(loss=loss, aux_loss=aux, logits=logits,
+                                         router_logits=tuple(router) if want else None)
 
 
 __all__ = ["Qwen3_8MoeMLP", "Qwen3_8MoeExperts", "Qwen3_8MoeTopKRouter", "Qwen3_8MoeSparseMoeBlock",

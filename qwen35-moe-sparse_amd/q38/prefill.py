@@ -685,6 +685,18 @@ def load_balancing_loss(router_logits, num_experts, top_k):
     return torch.sum((counts / rows) * (probs / rows)) * num_experts
 
 
+def next_token_loss(hs, head, labels, ignore_index=-100, reduction="mean"):
+    """Cross entropy of each position's next label (int32 or int64 [B, S]) under hs [B, S, h] and the head [V, h],
+    without the logits (q38.hip.autograd.linear_cross_entropy: bf16 or fp32 on the GPU, fp32 loss). The last position
+    has no next label and counts as ignored, in loss and mean alike; with reduction "none" its entry is 0."""
+    from .hip import autograd
+
+    if tuple(labels.shape) != tuple(hs.shape[:-1]):
+        raise ValueError(f"labels {tuple(labels.shape)} do not match the tokens {tuple(hs.shape[:-1])}")
+    nxt = F.pad(labels[:, 1:], (0, 1), value=ignore_index)
+    return autograd.linear_cross_entropy(hs, head, nxt, ignore_index, reduction)
+
+
 @dataclass
 class PrefillOutput:
     """The fields of MoeCausalLMOutputWithPast the packed prefill fills (modeling:1425-1433)."""
@@ -735,6 +747,16 @@ class Q38Prefill(nn.Module):
         if router is None:
             return logits
         return PrefillOutput(logits, load_balancing_loss(router, self.cfg.experts, self.cfg.topk), tuple(router))
+
+    @torch.no_grad()
+    def loss(self, ids, labels=None, ignore_index=-100, reduction="mean"):
+        """Next-token cross entropy of ids [B,S] (or of ``labels`` [B,S], where ignore_index marks what does not
+        count) in fp32, from the hidden states and without the logits' [B,S,vocab]: "mean", "sum" or "none" [B,S]."""
+        if labels is not None and labels.shape != ids.shape:  # before the trunk's work
+            raise ValueError(f"labels {tuple(labels.shape)} do not match the tokens {tuple(ids.shape)}")
+        hs = trunk_forward(self.model, self.cfg, ids, self._moe)
+        return next_token_loss(hs, self.model.embed_tokens.weight, ids if labels is None else labels, ignore_index,
+                               reduction)
 
     def _moe(self, block, x, with_router):
         if not with_router:

@@ -167,3 +167,18 @@ def test_rows_abi_arguments():
     assert lib.q38moe_collect_rows(None, None, 1, p, 1, p, p, 4, 64, 8, 2, 1, None) == -1 and says("src")
     assert lib.q38moe_collect_rows(p, None, 1, None, 1, p, p, 4, 64, 8, 2, 1, None) == -1 and says("topk_idx")
     assert lib.q38moe_collect_rows(None, None, 1, None, 1, None, None, 0, 64, 8, 2, 1, None) == 0
+
+
+def test_model_loss_refuses_other_labels():
+    """Before the trunk runs (it could not: the blocks have no CPU path)."""
+    from q38 import prefill as P
+    from q38.models.qwen3_8_moe import Qwen3_8MoeForCausalLM, Qwen3_8MoeTextConfig
+    ids = torch.zeros(2, 8, dtype=torch.long)
+    with torch.device("meta"):
+        model = Qwen3_8MoeForCausalLM(Qwen3_8MoeTextConfig())
+    with pytest.raises(ValueError, match="labels"):
+        model(input_ids=ids, labels=ids[:, 1:])
+    with pytest.raises(ValueError, match="labels"):
+        P.Q38Prefill(P.PrefillConfig()).loss(ids, ids[:1])
+    with pytest.raises(ValueError, match="labels"):
+        P.next_token_loss(torch.zeros(2, 8, 64), torch.zeros(10, 64), ids[:, 1:])
