@@ -13,15 +13,23 @@
 // Rows whose target is the ignored one leave the problem first: a stable partition lists the others, their x is copied
 // next to each other, and the products run over those rows only, so neither the work nor a NaN in a masked row counts.
 //
-// One kernel does the four products. C[m, n] = sum_k A[m, k] B[n, k] on 256 x 256 tiles (128 x 128 where those are few),
-// four waves, each a quarter of the tile in 32x32 blocks: at one wave per SIMD with 128 x 128 elements each operand byte
+// One kernel does the four products. C[m, n] = sum_k A[m, k] B[n, k] on 256 x 256 tiles (128 x 128 or 64 x 64 where those are
+// few), four waves, each a quarter of the tile in 32x32 blocks: at one wave per SIMD with 128 x 128 elements each operand byte
 // read from LDS is used 128 times, which keeps LDS reads at half of the matrix units' time. An operand is either
 // K-contiguous (KC: rows of 128 bytes per K step) or K-strided (KS: K rows of the tile's columns, fragments by the
 // transposing LDS read in bf16), so s, x and W are used as they lie:
 //     z^T : A = W (KC), B = x (KC);   dx^T : A = W (KS), B = s (KC);   dW^T : A = x (KS), B = s (KS).
-// A K step is 128 bytes of K; two steps lie in LDS, copied there by buffer loads that write LDS directly (out of range reads give zeros: the
-// tails of every dimension). The tokens (or vocabulary rows) are the lanes of the accumulators and the reduced or stored
-// dimension their registers, so the softmax's maxima and sums are in-lane but for one exchange.
+// A K step is 128 bytes of K. Two steps lie in LDS (four or eight with 64 x 64 tiles, whose products wait for memory), copied
+// there by buffer loads that write LDS directly; reads out of range give zeros, which are the tails of every dimension. The
+// tokens (or vocabulary rows) are the lanes of the accumulators and the reduced or stored dimension their registers, so the
+// softmax's maxima and sums are in-lane but for one exchange.
+//
+// What bounds it. The matrix units need 2051 clocks for a step of a 256 x 256 tile. With all CUs at work on random bf16 data the
+// chip lowers its clock to 1.7 - 1.9 GHz: MFMAs alone take 1.09 us a step, with their LDS reads 1.23, with the copies to
+// LDS out of the L2 1.33 (all zeros: 0.94, 0.96, 1.04), and with a stream of its own per CU 1.94; this kernel, whose
+// tiles share the streams eight by four, takes 1.7. 16384 x 1024 x 10112: z 302 us (1120 TFLOP/s), s 2 x 172, dx 2 x 155, dW
+// 2 x 165. 4099 x 2048 x 50021: z 700 us (1200), s 2 x 400, dx 2 x 430, dW 2 x 408. Few tokens are bound by the latency of W's
+// way into LDS: 61 x 1024 x 10112 z 10 us for 20.7 MB.
 #include "q38moe_common.h"
 #include "q38moe_kernels.h"
 
@@ -37,13 +45,7 @@ typedef short ls_i16x4_t __attribute__((ext_vector_type(4)));
 
 __device__ __forceinline__ uint32_t uniform(uint32_t v) { return __builtin_amdgcn_readfirstlane(v); }
 
-// 16 bytes at p + voff + soff, zeros where voff (+ soff) reaches `bytes` (raw buffer, no format).
-__device__ __forceinline__ u32x4_t ls_load(const uint8_t* p, int64_t bytes, uint32_t voff, uint32_t soff) {
-  const int n = bytes <= 0 ? 0 : (bytes >= 0xffffffffll ? -1 : (int)(uint32_t)bytes);
-  const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(p), (short)0, n, 0x00020000);
-  return __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(r, (int)voff, (int)soff, 0));
-}
-
+// 16 bytes per lane from p + voff + soff to LDS at lds + 16 lane, zeros where voff + soff reaches `bytes` (raw buffer, no format).
 __device__ __forceinline__ void ls_dma(const uint8_t* p, int64_t bytes, uint32_t voff, uint32_t soff, uint32_t lds) {
   const uint64_t a = (uint64_t)(uintptr_t)p;
   const uint32_t n = bytes <= 0 ? 0u : (bytes >= 0xffffffffll ? 0xffffffffu : (uint32_t)bytes);
@@ -229,6 +231,9 @@ __host__ __device__ inline LsPlan ls_plan(uint32_t tiles, uint32_t steps, uint32
   return pl;
 }
 
+// Workgroups that share a CU.
+constexpr int ls_per_cu(int bm, int epi) { return bm == 128 || (bm == 64 && epi != EPI_OUT) ? 2 : 1; }
+
 // A target id as an int, -1 where it lies outside of one's range.
 __device__ __forceinline__ int32_t raw_target(const void* targets, bool idx64, int64_t t) {
   if (!idx64) return static_cast<const int32_t*>(targets)[t];
@@ -250,12 +255,12 @@ __device__ __forceinline__ void ls_tile(uint32_t t, uint32_t ntm, uint32_t ntn, 
 }
 
 template <bool F32, int BM, int BN, int LA, int LB, int EPI>
-__global__ __launch_bounds__(256, BM == 128 ? 2 : 1) void ls_gemm_kernel(const LsParams p) {
+__global__ __launch_bounds__(256, ls_per_cu(BM, EPI)) void ls_gemm_kernel(const LsParams p) {
   using OA = Operand<F32, BM, LA>;
   using OB = Operand<F32, BN, LB>;
   constexpr int MB = BM / 64, NB = BN / 64;  // 32x32 blocks of a wave
   constexpr int SLOT = (BM + BN) * 128;
-  constexpr int NS = BM == 64 ? 8 : 2;  // steps in LDS: few tiles wait for memory, many for the matrix units
+  constexpr int NS = BM != 64 ? 2 : EPI == EPI_OUT ? 8 : 4;  // steps in LDS: few tiles wait for memory, many for the matrix units
   constexpr int BK = OA::BK, ESZ = OA::ESZ;
   __shared__ __align__(1024) uint8_t lds[NS * SLOT];
   // Staging of bf16 outputs, 32 rows of out by BM / 2 columns per wave (beside the slots: copies for the next item run meanwhile).
@@ -645,10 +650,12 @@ __global__ __launch_bounds__(256) void ls_gather_kernel(const uint8_t* __restric
   }
 }
 
-// lse and loss of 64 rows per block from their partial maxima and sums (16 waves share the entries); rows that do not count get
-// loss 0. Rows are those of the list, or with `raw` the call's own. Then *reduced = the sum of all losses (mean: over
-// the rows that count; 0 where none does), *row_scale = the factor of every row's gradient: by the block that is done last, from
-// the blocks' sums in their order (*done is 0 before and after).
+// lse and loss of LS_FIN rows per block from their partial maxima and sums, which its 64 groups of lanes share (a block's few
+// loads each wait for memory: 61 rows of 316 entries take 3.8 us, with 64 rows to a block and a wave per entry 5.7); rows that
+// do not count get loss 0. Rows are those of the list, or with `raw` the call's own. Then *reduced = the sum of all losses (mean:
+// over the rows that count; 0 where none does), *row_scale = the factor of every row's gradient: by the block that is done
+// last, from the blocks' sums in their order (*done is 0 before and after).
+constexpr int LS_FIN = 16;
 __global__ __launch_bounds__(1024) void ls_finish_kernel(const float2* __restrict__ part, int entries,
                                                          const float* __restrict__ zt, const int32_t* __restrict__ tgt,
                                                          const int32_t* __restrict__ rows,
@@ -657,26 +664,37 @@ __global__ __launch_bounds__(1024) void ls_finish_kernel(const float2* __restric
                                                          float* __restrict__ lse, bool mean, double* block_sum,
                                                          int32_t* block_n, uint32_t* done, float* __restrict__ reduced,
                                                          float* __restrict__ row_scale) {
-  __shared__ float2 red[16][64];
+  __shared__ float2 red[16][LS_FIN];
   __shared__ bool last;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t n = raw != nullptr ? T : (int64_t)load_uniform(count), i = (int64_t)blockIdx.x * 64 + lane;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, group = threadIdx.x / LS_FIN;
+  const int64_t n = raw != nullptr ? T : (int64_t)load_uniform(count);
+  const int64_t i = (int64_t)blockIdx.x * LS_FIN + (lane & (LS_FIN - 1));
   float m = -__builtin_inff(), s = 0.0f;
+  auto join_lanes = [&]() {  // the wave's groups, each lane with all of its row's
+#pragma unroll
+    for (int o = LS_FIN; o < 64; o <<= 1) lse_join(m, s, __shfl_xor(m, o), __shfl_xor(s, o));
+  };
   if (i < n) {
 #pragma unroll 4
-    for (int e = wave; e < entries; e += 16) {
+    for (int e = group; e < entries; e += 1024 / LS_FIN) {
       const float2 v = part[(int64_t)e * T + i];
       lse_join(m, s, v.x, v.y);
     }
   }
-  red[wave][lane] = make_float2(m, s);
+  join_lanes();
+  if (lane < LS_FIN) red[wave][lane] = make_float2(m, s);
   __syncthreads();
   if (wave == 0) {
+    m = -__builtin_inff(), s = 0.0f;
 #pragma unroll
-    for (int w = 1; w < 16; ++w) lse_join(m, s, red[w][lane].x, red[w][lane].y);
+    for (int w = 0; w < 16; w += 64 / LS_FIN) {
+      const float2 v = red[w + lane / LS_FIN][lane & (LS_FIN - 1)];
+      lse_join(m, s, v.x, v.y);
+    }
+    join_lanes();
     double sum = 0.0;
     int c = 0;
-    if (i < T) {
+    if (i < T && lane < LS_FIN) {
       const int64_t r = raw != nullptr ? i : (int64_t)rows[i];
       int tg = -1;
       bool in = i < n;
@@ -800,12 +818,11 @@ __global__ __launch_bounds__(256) void ls_join_kernel(const LsParams p) {
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// Workgroups that run at once: two of 128 x 128 tiles share a CU.
-uint32_t ls_slots(int bm) { return (uint32_t)device_cus() * (bm == 128 ? 2 : 1); }
+uint32_t ls_slots(int bm, int epi) { return (uint32_t)(device_cus() * ls_per_cu(bm, epi)); }
 
 template <bool F32, int BM, int BN, int LA, int LB, int EPI>
 hipError_t ls_gemm(LsParams p, hipStream_t st) {
-  p.slots = ls_slots(BM);
+  p.slots = ls_slots(BM, EPI);
   const int64_t tiles = ceil_div(p.M, BM) * ceil_div(p.N, BN);
   const unsigned grid = EPI == EPI_OUT || tiles > p.slots ? p.slots : (unsigned)tiles;
   hipLaunchKernelGGL((ls_gemm_kernel<F32, BM, BN, LA, LB, EPI>), dim3(grid), dim3(256), 0, st, p);
@@ -816,14 +833,17 @@ hipError_t ls_gemm(LsParams p, hipStream_t st) {
   return hipGetLastError();
 }
 
-// Tile side of the products over the vocabulary, whose tiles stay whole. bf16: a round of 256 x 256 tiles takes 30 us at h = 1024
-// and one of 128 x 128, two to a CU, 17 (16384 x 1024 x 10112: 302 and 350 us; 1777 tokens: 60 and 51; 300: 30 and 17; 64 x 64
-// tiles are never faster). fp32 multiplies at a sixteenth of the rate, so that a large tile's reuse is worth nothing and a
-// few tiles leave CUs without work: 64 where tiles of 128 reach at most half the CUs (61 x 1024 x 10112: 37 and 75 us with
-// the rest of the call; 300 tokens: 112 and 84), else 128.
+// Tile side of the products over the vocabulary, whose tiles stay whole. bf16: 64 where one round of such tiles, two to a CU, is
+// all (61 x 1024 x 10112 forward and dx: 15.6 and 36 us, with 128 18.5 and 42; 128 tokens 17.1 and 38, 18.5 and 42; 2 rounds, 200
+// tokens: 25.5 and 51, 18.8 and 47). Else a round of 256 x 256 tiles takes 30 us at h = 1024 and one of 128 x 128, two to a CU, 17
+// (16384 x 1024 x 10112: 302 and 350 us; 1777 tokens: 60 and 51; 300: 30 and 17). fp32 multiplies at a sixteenth of the rate, so
+// that a large tile's reuse is worth nothing, and the work on the busiest CU decides: 64 where it gets fewer than three times as
+// many of those as of 128 (of 64 tokens the larger tile is half empty: 61 x 2048 x 50021 forward 158 and 247 us, 100 x 1024 x
+// 10112 46 and 60; 200 tokens, three for one, 80 and 74; 600, seven for two, 155 and 134).
 int tile_z(int64_t M, int64_t N, bool f32) {
-  const int64_t cus = device_cus(), n128 = ceil_div(M, 128) * ceil_div(N, 128);
-  if (f32) return 2 * n128 <= cus ? 64 : 128;
+  const int64_t cus = device_cus(), n64 = ceil_div(M, 64) * ceil_div(N, 64), n128 = ceil_div(M, 128) * ceil_div(N, 128);
+  if (f32) return ceil_div(n64, cus) < 3 * ceil_div(n128, cus) ? 64 : 128;
+  if (n64 <= 2 * cus) return 64;
   return 7 * ceil_div(ceil_div(M, 256) * ceil_div(N, 256), cus) <= 4 * ceil_div(n128, 2 * cus) ? 256 : 128;
 }
 
@@ -839,7 +859,7 @@ int tile_k(int64_t M, int64_t N, int64_t steps, bool f32) {
 
 // Bytes of a product's partial sums, and of its running sums.
 size_t split_bytes(int64_t M, int64_t N, int b) {
-  const int64_t most = 2 * (int64_t)ls_slots(b), cuts = ceil_div(M, b) * ceil_div(N, b) * LS_CUTS * 2;
+  const int64_t most = 2 * (int64_t)ls_slots(b, EPI_OUT), cuts = ceil_div(M, b) * ceil_div(N, b) * LS_CUTS * 2;
   return 4 * (size_t)(b * b) * (size_t)(cuts < most ? cuts : most);
 }
 size_t acc_bytes(int64_t M, int64_t N, int b) { return 4 * (size_t)(b * b) * (size_t)(ceil_div(M, b) * ceil_div(N, b)); }
@@ -876,8 +896,8 @@ Layout layout(int64_t T, int h, int V, bool f32, bool fwd, bool need_x, bool nee
     l.entries = (int)(2 * ceil_div(V, l.tile_s));
     l.part = take(8 * (size_t)l.entries * T);
     l.zt = take(4 * T);
-    l.bsum = take(8 * ceil_div(T, 64));
-    l.bn = take(4 * ceil_div(T, 64));
+    l.bsum = take(8 * ceil_div(T, LS_FIN));
+    l.bn = take(4 * ceil_div(T, LS_FIN));
     l.done = take(4);
   } else {
     const int64_t vt = ceil_div(V, 256);
@@ -931,8 +951,7 @@ hipError_t ls_gather(const void* x, const int32_t* rows, const int32_t* count, v
 
 template <bool F32, int LA, int LB, int EPI>
 hipError_t ls_gemm_any(const LsParams& p, int tile, hipStream_t st) {
-  if constexpr (F32 || EPI == EPI_OUT)
-    if (tile == 64) return ls_gemm<F32, 64, 64, LA, LB, EPI>(p, st);
+  if (tile == 64) return ls_gemm<F32, 64, 64, LA, LB, EPI>(p, st);
   if constexpr (!F32)
     if (tile == 256) return ls_gemm<F32, 256, 256, LA, LB, EPI>(p, st);
   return ls_gemm<F32, 128, 128, LA, LB, EPI>(p, st);
@@ -967,7 +986,7 @@ hipError_t ce_forward(const void* x, const void* w, const void* targets, bool id
   p.zt = at<float>(ws, l.zt);
   p.done = at<uint32_t>(ws, l.done);
   LS_TRY((ls_gemm_any<F32, KC, KC, EPI_LSE>(p, l.tile_s, st)));
-  hipLaunchKernelGGL(ls_finish_kernel, dim3((unsigned)ceil_div(T, 64)), dim3(1024), 0, st, p.part, l.entries, p.zt, tgt,
+  hipLaunchKernelGGL(ls_finish_kernel, dim3((unsigned)ceil_div(T, LS_FIN)), dim3(1024), 0, st, p.part, l.entries, p.zt, tgt,
                      rows, count, p.raw, idx64, ignore, V, T, loss, lse, mean, at<double>(ws, l.bsum),
                      at<int32_t>(ws, l.bn), p.done, reduced, row_scale);
   return hipGetLastError();

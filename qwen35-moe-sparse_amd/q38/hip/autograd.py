@@ -218,14 +218,17 @@ def linear_cross_entropy(x, weight, targets, ignore_index=-100, reduction="mean"
         raise ValueError(f"targets {tuple(targets.shape)} do not match x {tuple(x.shape)}")
     if _bf16_autocast() and x.is_floating_point() and weight.is_floating_point():
         x, weight = x.to(torch.bfloat16), weight.to(torch.bfloat16)
-    args = (_aligned(x.reshape(-1, x.shape[-1])), _aligned(weight), targets.reshape(-1).contiguous(), ignore_index)
+    flat = x.dim() == 2
+    if not flat:
+        x = x.reshape(-1, x.shape[-1])
+    args = (_aligned(x), _aligned(weight), (targets if flat else targets.reshape(-1)).contiguous(), ignore_index)
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
         loss = HipLinearCE.apply(*args, reduction)
     elif reduction == "none":
         loss = ops.linear_ce_forward(*args, want_lse=False)[0]
     else:
         loss = ops.linear_ce_forward(*args, reduction, want_lse=False)[2]
-    return loss.view(targets.shape) if reduction == "none" else loss
+    return loss if flat or reduction != "none" else loss.view(targets.shape)
 
 
 class HipDispatch(torch.autograd.Function):

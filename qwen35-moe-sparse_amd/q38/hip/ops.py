@@ -809,9 +809,12 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
     lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
+_HERE = contextlib.nullcontext()
+
+
 def _on(device):
     """The tensors' device as the current one, for launches on its stream."""
-    return contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
 def _loss_args(x, w, targets):
@@ -877,6 +880,10 @@ def linear_ce_backward(g, x, w, targets, lse, ignore_index=-100, row_scale=None,
         raise ValueError(f"g must hold one element or [{T}], got {tuple(g.shape)}")
     if row_scale is not None:
         _need(row_scale, "row_scale", dtype=torch.float32)
+        if row_scale.numel() != 1:
+            raise ValueError(f"row_scale must hold one element, got {tuple(row_scale.shape)}")
+    if any(t is not None and t.device != dev for t in (g, lse, row_scale)):
+        raise RuntimeError("g, lse, row_scale and x must be on one device")
     if T == 0:
         return (torch.zeros_like(x) if need_x else None), (torch.zeros_like(w) if need_w else None)
     dx = torch.empty_like(x) if need_x else None
