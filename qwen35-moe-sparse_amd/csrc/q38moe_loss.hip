@@ -650,12 +650,13 @@ __global__ __launch_bounds__(256) void ls_gather_kernel(const uint8_t* __restric
   }
 }
 
-// lse and loss of LS_FIN rows per block from their partial maxima and sums, which its 64 groups of lanes share (a block's few
-// loads each wait for memory: 61 rows of 316 entries take 3.8 us, with 64 rows to a block and a wave per entry 5.7); rows that
-// do not count get loss 0. Rows are those of the list, or with `raw` the call's own. Then *reduced = the sum of all losses (mean:
+// lse and loss of R rows per block from their partial maxima and sums, which its 1024 / R groups of lanes share; rows that do not
+// count get loss 0. Few rows wait for the groups' loads, many for the blocks' sums to reach the last one: 16 rows to a block up
+// to 2048 rows, else 64 (61 rows of 316 entries 3.8 and 5.7 us; 1777 7.2 and 7.4; with the mean of 4099 13.9 and 10.8, of 16384 27 and
+// 10). Rows are those of the list, or with `raw` the call's own. Then *reduced = the sum of all losses (mean:
 // over the rows that count; 0 where none does), *row_scale = the factor of every row's gradient: by the block that is done
 // last, from the blocks' sums in their order (*done is 0 before and after).
-constexpr int LS_FIN = 16;
+template <int R>
 __global__ __launch_bounds__(1024) void ls_finish_kernel(const float2* __restrict__ part, int entries,
                                                          const float* __restrict__ zt, const int32_t* __restrict__ tgt,
                                                          const int32_t* __restrict__ rows,
@@ -664,37 +665,37 @@ __global__ __launch_bounds__(1024) void ls_finish_kernel(const float2* __restric
                                                          float* __restrict__ lse, bool mean, double* block_sum,
                                                          int32_t* block_n, uint32_t* done, float* __restrict__ reduced,
                                                          float* __restrict__ row_scale) {
-  __shared__ float2 red[16][LS_FIN];
+  __shared__ float2 red[16][R];
   __shared__ bool last;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, group = threadIdx.x / LS_FIN;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, group = threadIdx.x / R;
   const int64_t n = raw != nullptr ? T : (int64_t)load_uniform(count);
-  const int64_t i = (int64_t)blockIdx.x * LS_FIN + (lane & (LS_FIN - 1));
+  const int64_t i = (int64_t)blockIdx.x * R + (lane & (R - 1));
   float m = -__builtin_inff(), s = 0.0f;
   auto join_lanes = [&]() {  // the wave's groups, each lane with all of its row's
 #pragma unroll
-    for (int o = LS_FIN; o < 64; o <<= 1) lse_join(m, s, __shfl_xor(m, o), __shfl_xor(s, o));
+    for (int o = R; o < 64; o <<= 1) lse_join(m, s, __shfl_xor(m, o), __shfl_xor(s, o));
   };
   if (i < n) {
 #pragma unroll 4
-    for (int e = group; e < entries; e += 1024 / LS_FIN) {
+    for (int e = group; e < entries; e += 1024 / R) {
       const float2 v = part[(int64_t)e * T + i];
       lse_join(m, s, v.x, v.y);
     }
   }
   join_lanes();
-  if (lane < LS_FIN) red[wave][lane] = make_float2(m, s);
+  if (lane < R) red[wave][lane] = make_float2(m, s);
   __syncthreads();
   if (wave == 0) {
     m = -__builtin_inff(), s = 0.0f;
 #pragma unroll
-    for (int w = 0; w < 16; w += 64 / LS_FIN) {
-      const float2 v = red[w + lane / LS_FIN][lane & (LS_FIN - 1)];
+    for (int w = 0; w < 16; w += 64 / R) {
+      const float2 v = red[w + lane / R][lane & (R - 1)];
       lse_join(m, s, v.x, v.y);
     }
     join_lanes();
     double sum = 0.0;
     int c = 0;
-    if (i < T && lane < LS_FIN) {
+    if (i < T && lane < R) {
       const int64_t r = raw != nullptr ? i : (int64_t)rows[i];
       int tg = -1;
       bool in = i < n;
@@ -857,6 +858,8 @@ int tile_k(int64_t M, int64_t N, int64_t steps, bool f32) {
   return !f32 && ceil_div(M, 256) * ceil_div(N, 256) * steps >= 12 * cus ? 256 : 128;
 }
 
+int ls_finish_rows(int64_t T) { return T <= 2048 ? 16 : 64; }
+
 // Bytes of a product's partial sums, and of its running sums.
 size_t split_bytes(int64_t M, int64_t N, int b) {
   const int64_t most = 2 * (int64_t)ls_slots(b, EPI_OUT), cuts = ceil_div(M, b) * ceil_div(N, b) * LS_CUTS * 2;
@@ -896,8 +899,8 @@ Layout layout(int64_t T, int h, int V, bool f32, bool fwd, bool need_x, bool nee
     l.entries = (int)(2 * ceil_div(V, l.tile_s));
     l.part = take(8 * (size_t)l.entries * T);
     l.zt = take(4 * T);
-    l.bsum = take(8 * ceil_div(T, LS_FIN));
-    l.bn = take(4 * ceil_div(T, LS_FIN));
+    l.bsum = take(8 * ceil_div(T, ls_finish_rows(T)));
+    l.bn = take(4 * ceil_div(T, ls_finish_rows(T)));
     l.done = take(4);
   } else {
     const int64_t vt = ceil_div(V, 256);
@@ -986,9 +989,10 @@ hipError_t ce_forward(const void* x, const void* w, const void* targets, bool id
   p.zt = at<float>(ws, l.zt);
   p.done = at<uint32_t>(ws, l.done);
   LS_TRY((ls_gemm_any<F32, KC, KC, EPI_LSE>(p, l.tile_s, st)));
-  hipLaunchKernelGGL(ls_finish_kernel, dim3((unsigned)ceil_div(T, LS_FIN)), dim3(1024), 0, st, p.part, l.entries, p.zt, tgt,
-                     rows, count, p.raw, idx64, ignore, V, T, loss, lse, mean, at<double>(ws, l.bsum),
-                     at<int32_t>(ws, l.bn), p.done, reduced, row_scale);
+  const int per = ls_finish_rows(T);
+  hipLaunchKernelGGL(per == 16 ? ls_finish_kernel<16> : ls_finish_kernel<64>, dim3((unsigned)ceil_div(T, per)), dim3(1024), 0, st,
+                     p.part, l.entries, p.zt, tgt, rows, count, p.raw, idx64, ignore, V, T, loss, lse, mean,
+                     at<double>(ws, l.bsum), at<int32_t>(ws, l.bn), p.done, reduced, row_scale);
   return hipGetLastError();
 }
 

@@ -103,6 +103,8 @@ def _grad_of(reduction, T, gen, dev):
     (1300, 128, 2049, 0.6),
     (100, 4096, 300, 0.1),   # 64 steps of K: the eight slots of small tiles go round
     (700, 1344, 200, 0.0),
+    (2048, 64, 130, 0.3),    # the last size with 16 rows to a finishing block
+    (2049, 64, 130, 0.3),
 ])
 def test_small(gpu, dtype, T, h, V, ignored):
     x, w, t, g = _data(T, h, V, dtype, gpu, ignored=ignored)
