@@ -565,8 +565,8 @@ int q38moe_clip_grads(const void* const* src, void* const* dst, const int64_t* n
  * Rows to experts of the caller's own and back. A plan is the permutation of q38moe_permute (pair p = t*k + j of
  * expert-sorted row inv[p]; pairs whose index lies outside [0, E) have no row) in one int32 buffer of
  * q38moe_rows_plan_ints(T, E, k) entries: counts [E], starts [E], perm [T*k] and inv [T*k] from entries 0, E4, 2 E4 and
- * 2 E4 + P4 on (E4 and P4: E and T*k up to a multiple of 4), then scratch. dispatch makes the plan and dst[inv[p]] = x[t]; spread
- * uses it: dst[inv[p]] = src[t] (* w[p] unless w is NULL), and with y [T*k,h] dw[p] = <src[t], y[inv[p]]> (0 for pairs
+ * 2 E4 + P4 on (E4 and P4: E and T*k up to a multiple of 4), then scratch. dispatch makes the plan (inv is -1 for
+ * pairs without a row) and dst[inv[p]] = x[t]; the others look at the plan alone. spread: dst[inv[p]] = src[t] (* w[p] unless w is NULL), and with y [T*k,h] dw[p] = <src[t], y[inv[p]]> (0 for pairs
  * without a row); dst or dw may be NULL. Both fill the rows behind the last filled one with zeros. collect: out[t] =
  * sum_j src[inv[p]] (* w[p] unless w is NULL). x, src, dst, y and out in dtype, w and dw [T,k] in w_dtype (dtype or
  * fp32); products and sums fp32, rounded once. The gradient of dispatch is collect without w; combine is collect
@@ -575,12 +575,10 @@ int q38moe_clip_grads(const void* const* src, void* const* dst, const int64_t* n
 int64_t q38moe_rows_plan_ints(int64_t T, int32_t E, int32_t k);
 int q38moe_dispatch_rows(const void* x, const void* topk_idx, int32_t idx_is_int64, int32_t* plan, void* dst, int64_t T,
                          int32_t h, int32_t E, int32_t k, int32_t dtype, void* stream);
-int q38moe_spread_rows(const void* src, const void* w, int32_t w_dtype, const void* y, const void* topk_idx,
-                       int32_t idx_is_int64, const int32_t* plan, void* dst, void* dw, int64_t T, int32_t h, int32_t E,
-                       int32_t k, int32_t dtype, void* stream);
-int q38moe_collect_rows(const void* src, const void* w, int32_t w_dtype, const void* topk_idx, int32_t idx_is_int64,
-                        const int32_t* plan, void* out, int64_t T, int32_t h, int32_t E, int32_t k, int32_t dtype,
-                        void* stream);
+int q38moe_spread_rows(const void* src, const void* w, int32_t w_dtype, const void* y, const int32_t* plan, void* dst,
+                       void* dw, int64_t T, int32_t h, int32_t E, int32_t k, int32_t dtype, void* stream);
+int q38moe_collect_rows(const void* src, const void* w, int32_t w_dtype, const int32_t* plan, void* out, int64_t T,
+                        int32_t h, int32_t E, int32_t k, int32_t dtype, void* stream);
 
 #ifdef __cplusplus
 }

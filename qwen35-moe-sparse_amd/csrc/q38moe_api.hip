@@ -1746,9 +1746,8 @@ int q38moe_dispatch_rows(const void* x, const void* topk_idx, int32_t idx_is_int
   return Q38MOE_OK;
 }
 
-int q38moe_spread_rows(const void* src, const void* w, int32_t w_dtype, const void* y, const void* topk_idx,
-                       int32_t idx_is_int64, const int32_t* plan, void* dst, void* dw, int64_t T, int32_t h, int32_t E,
-                       int32_t k, int32_t dtype, void* stream) {
+int q38moe_spread_rows(const void* src, const void* w, int32_t w_dtype, const void* y, const int32_t* plan, void* dst,
+                       void* dw, int64_t T, int32_t h, int32_t E, int32_t k, int32_t dtype, void* stream) {
   g_err[0] = 0;
   Q38_CHECK(check_rows_args(T, h, E, k, w_dtype, w, dtype));
   if (dw != nullptr && (y == nullptr || w == nullptr)) return fail(Q38MOE_EINVAL, "dw needs y and w");
@@ -1756,29 +1755,28 @@ int q38moe_spread_rows(const void* src, const void* w, int32_t w_dtype, const vo
   Q38_CHECK(check_ptr(src, "src"));
   Q38_CHECK(check_opt_ptr(y, "y"));
   Q38_CHECK(check_opt_ptr(dst, "dst"));
-  if (topk_idx == nullptr || plan == nullptr) return fail(Q38MOE_EINVAL, "topk_idx and plan must not be NULL");
+  if (plan == nullptr) return fail(Q38MOE_EINVAL, "plan must not be NULL");
   const RowsPlan L = rows_plan(T, E, k);
   (void)hipGetLastError();
-  Q38_HIP(q38::launch_spread_rows(src, w, w_dtype == Q38MOE_FP32, dw != nullptr ? y : nullptr, topk_idx,
-                                  idx_is_int64 != 0, plan + L.inv(), plan + L.starts(), plan, dst, dw, T, h, E, k,
-                                  dtype == Q38MOE_BF16, static_cast<hipStream_t>(stream)),
+  Q38_HIP(q38::launch_spread_rows(src, w, w_dtype == Q38MOE_FP32, dw != nullptr ? y : nullptr, nullptr, false,
+                                  const_cast<int32_t*>(plan) + L.inv(),  // written by dispatch only
+                                  plan + L.starts(), plan, dst, dw, T, h, E, k, dtype == Q38MOE_BF16,
+                                  static_cast<hipStream_t>(stream)),
           "spread rows launch");
   return Q38MOE_OK;
 }
 
-int q38moe_collect_rows(const void* src, const void* w, int32_t w_dtype, const void* topk_idx, int32_t idx_is_int64,
-                        const int32_t* plan, void* out, int64_t T, int32_t h, int32_t E, int32_t k, int32_t dtype,
-                        void* stream) {
+int q38moe_collect_rows(const void* src, const void* w, int32_t w_dtype, const int32_t* plan, void* out, int64_t T, int32_t h,
+                        int32_t E, int32_t k, int32_t dtype, void* stream) {
   g_err[0] = 0;
   Q38_CHECK(check_rows_args(T, h, E, k, w_dtype, w, dtype));
   if (T == 0) return Q38MOE_OK;
   Q38_CHECK(check_ptr(src, "src"));
   Q38_CHECK(check_ptr(out, "out"));
-  if (topk_idx == nullptr || plan == nullptr) return fail(Q38MOE_EINVAL, "topk_idx and plan must not be NULL");
+  if (plan == nullptr) return fail(Q38MOE_EINVAL, "plan must not be NULL");
   (void)hipGetLastError();
-  Q38_HIP(q38::launch_collect_rows(src, w, w_dtype == Q38MOE_FP32, topk_idx, idx_is_int64 != 0,
-                                   plan + rows_plan(T, E, k).inv(), out, T, h, E, k, dtype == Q38MOE_BF16,
-                                   static_cast<hipStream_t>(stream)),
+  Q38_HIP(q38::launch_collect_rows(src, w, w_dtype == Q38MOE_FP32, plan + rows_plan(T, E, k).inv(), out, T, h, k,
+                                   dtype == Q38MOE_BF16, static_cast<hipStream_t>(stream)),
           "collect rows launch");
   return Q38MOE_OK;
 }

@@ -207,13 +207,12 @@ hipError_t launch_qsa_attention(const void* q, const void* k, const void* v, con
 
 // Tokens to expert-sorted rows and back (q38moe_rows.hip), rows in bf16 or fp32, w and dw in the rows' type or
 // fp32 (w_f32). spread: dst[inv[p]] = src[t] (* w[p]), zeros behind the filled rows, dw[p] = <src[t], y[inv[p]]>; w, y
-// with dw, and dst may be NULL. collect: out[t] = sum_j src[inv[p]] (* w[p]).
+// with dw, and dst may be NULL; with idx (dispatch) inv becomes -1 for the pairs without a row, else it says so. collect: out[t] = sum_j src[inv[p]] (* w[p]).
 hipError_t launch_spread_rows(const void* src, const void* w, bool w_f32, const void* y, const void* idx, bool idx64,
-                              const int32_t* inv, const int32_t* starts, const int32_t* counts, void* dst, void* dw,
-                              int64_t T, int h, int E, int k, bool bf16, hipStream_t st);
-hipError_t launch_collect_rows(const void* src, const void* w, bool w_f32, const void* idx, bool idx64,
-                               const int32_t* inv, void* out, int64_t T, int h, int E, int k, bool bf16,
-                               hipStream_t st);
+                              int32_t* inv, const int32_t* starts, const int32_t* counts, void* dst, void* dw, int64_t T,
+                              int h, int E, int k, bool bf16, hipStream_t st);
+hipError_t launch_collect_rows(const void* src, const void* w, bool w_f32, const int32_t* inv, void* out, int64_t T, int h,
+                               int k, bool bf16, hipStream_t st);
 
 // Global norm and clipping (q38moe_clip.hip). A table of up to CLIP_TENSORS tensors, passed by value; first[i] is
 // the chunk (clip_chunk() elements) that tensor i starts at, first[n] the number of chunks.

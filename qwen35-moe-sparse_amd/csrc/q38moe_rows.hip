@@ -56,21 +56,29 @@ __device__ __forceinline__ float wave_add(float v) {
   return v;
 }
 
-// The rows of token t's pairs (-1: none), wave-uniform.
-template <typename IdxT, int KT>
-__device__ __forceinline__ void pair_rows(const IdxT* idx, const int32_t* inv, int64_t t, int E, int64_t (&row)[KT]) {
+// The rows of token t's pairs (-1: none), wave-uniform. Dispatch takes them from its indices and leaves -1 in the plan for the
+// pairs that have none; everything after it looks at the plan alone, so that indices changed since reach nothing, and a plan
+// that does not hold rows (below P = T*k) leads to none.
+template <int KT, typename IdxT>
+__device__ __forceinline__ void pair_rows(const IdxT* idx, int32_t* inv, int64_t t, int NE, int64_t P, int64_t (&row)[KT]) {
 #pragma unroll
   for (int j = 0; j < KT; ++j) {
-    const int64_t e = (int64_t)idx[t * KT + j];
-    const bool ok = __builtin_amdgcn_readfirstlane((int)(e >= 0 && e < E)) != 0;
-    row[j] = ok ? (int64_t)__builtin_amdgcn_readfirstlane(inv[t * KT + j]) : (int64_t)-1;
+    bool ok = true;
+    if constexpr (!std::is_void<IdxT>::value) {
+      const int64_t e = (int64_t)idx[t * KT + j];
+      ok = __builtin_amdgcn_readfirstlane((int)(e >= 0 && e < NE)) != 0;
+    }
+    const int64_t r = (int64_t)__builtin_amdgcn_readfirstlane(inv[t * KT + j]);
+    row[j] = ok && r >= 0 && r < P ? r : (int64_t)-1;
+    if constexpr (!std::is_void<IdxT>::value)
+      if (!ok && (threadIdx.x & 63) == 0) inv[t * KT + j] = -1;
   }
 }
 
 template <typename E, typename IdxT, int KT>
 __global__ __launch_bounds__(256) void spread_kernel(const E* __restrict__ src, const void* __restrict__ w, bool w_f32,
                                                      const E* __restrict__ y, const IdxT* __restrict__ idx,
-                                                     const int32_t* __restrict__ inv,
+                                                     int32_t* __restrict__ inv,
                                                      const int32_t* __restrict__ starts,
                                                      const int32_t* __restrict__ counts, E* __restrict__ dst,
                                                      void* __restrict__ dw, int64_t T, int h, int NE) {
@@ -79,7 +87,7 @@ __global__ __launch_bounds__(256) void spread_kernel(const E* __restrict__ src, 
   const int64_t t = (int64_t)blockIdx.x * 4 + wave;
   if (t >= T) return;
   int64_t row[KT];
-  pair_rows<IdxT, KT>(idx, inv, t, NE, row);
+  pair_rows<KT, IdxT>(idx, inv, t, NE, T * KT, row);
   float s[KT], acc[KT];
 #pragma unroll
   for (int j = 0; j < KT; ++j) {
@@ -151,16 +159,15 @@ __global__ __launch_bounds__(256) void spread_kernel(const E* __restrict__ src, 
   }
 }
 
-template <typename E, typename IdxT, int KT>
+template <typename E, int KT>
 __global__ __launch_bounds__(256) void collect_kernel(const E* __restrict__ src, const void* __restrict__ w, bool w_f32,
-                                                      const IdxT* __restrict__ idx, const int32_t* __restrict__ inv,
-                                                      E* __restrict__ out, int64_t T, int h, int NE) {
+                                                      int32_t* __restrict__ inv, E* __restrict__ out, int64_t T, int h) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lane = threadIdx.x & 63;
   const int64_t t = (int64_t)blockIdx.x * 4 + wave;
   if (t >= T) return;
   int64_t row[KT];
-  pair_rows<IdxT, KT>(idx, inv, t, NE, row);
+  pair_rows<KT, void>(nullptr, inv, t, 0, T * KT, row);
   float s[KT];
 #pragma unroll
   for (int j = 0; j < KT; ++j) s[j] = w != nullptr ? weight_of(w, w_f32, t * KT + j) : 1.0f;
@@ -194,7 +201,7 @@ __global__ __launch_bounds__(256) void collect_kernel(const E* __restrict__ src,
 }
 
 template <typename E, typename IdxT>
-hipError_t spread_k(const void* src, const void* w, bool w_f32, const void* y, const void* idx, const int32_t* inv,
+hipError_t spread_k(const void* src, const void* w, bool w_f32, const void* y, const void* idx, int32_t* inv,
                     const int32_t* starts, const int32_t* counts, void* dst, void* dw, int64_t T, int h, int NE, int k,
                     hipStream_t st) {
   const dim3 grid((unsigned)((T + 3) / 4));
@@ -211,14 +218,13 @@ hipError_t spread_k(const void* src, const void* w, bool w_f32, const void* y, c
   return hipGetLastError();
 }
 
-template <typename E, typename IdxT>
-hipError_t collect_k(const void* src, const void* w, bool w_f32, const void* idx, const int32_t* inv, void* out,
-                     int64_t T, int h, int NE, int k, hipStream_t st) {
+template <typename E>
+hipError_t collect_k(const void* src, const void* w, bool w_f32, int32_t* inv, void* out, int64_t T, int h, int k,
+                     hipStream_t st) {
   const dim3 grid((unsigned)((T + 3) / 4));
 #define Q38_COLLECT(KT)                                                                                             \
   case KT:                                                                                                          \
-    hipLaunchKernelGGL((collect_kernel<E, IdxT, KT>), grid, dim3(256), 0, st, (const E*)src, w, w_f32,              \
-                       (const IdxT*)idx, inv, (E*)out, T, h, NE);                                                   \
+    hipLaunchKernelGGL((collect_kernel<E, KT>), grid, dim3(256), 0, st, (const E*)src, w, w_f32, inv, (E*)out, T, h); \
     break;
   switch (k) {
     Q38_COLLECT(1) Q38_COLLECT(2) Q38_COLLECT(3) Q38_COLLECT(4) Q38_COLLECT(5) Q38_COLLECT(6) Q38_COLLECT(7)
@@ -229,28 +235,31 @@ hipError_t collect_k(const void* src, const void* w, bool w_f32, const void* idx
   return hipGetLastError();
 }
 
+template <typename E>
+hipError_t spread_any(const void* src, const void* w, bool w_f32, const void* y, const void* idx, bool idx64, int32_t* inv,
+                      const int32_t* starts, const int32_t* counts, void* dst, void* dw, int64_t T, int h, int NE, int k,
+                      hipStream_t st) {
+  if (idx == nullptr) return spread_k<E, void>(src, w, w_f32, y, idx, inv, starts, counts, dst, dw, T, h, NE, k, st);
+  if (idx64) return spread_k<E, int64_t>(src, w, w_f32, y, idx, inv, starts, counts, dst, dw, T, h, NE, k, st);
+  return spread_k<E, int32_t>(src, w, w_f32, y, idx, inv, starts, counts, dst, dw, T, h, NE, k, st);
+}
+
 }  // namespace
 
 hipError_t launch_spread_rows(const void* src, const void* w, bool w_f32, const void* y, const void* idx, bool idx64,
-                              const int32_t* inv, const int32_t* starts, const int32_t* counts, void* dst, void* dw,
-                              int64_t T, int h, int E, int k, bool bf16, hipStream_t st) {
+                              int32_t* inv, const int32_t* starts, const int32_t* counts, void* dst, void* dw, int64_t T,
+                              int h, int E, int k, bool bf16, hipStream_t st) {
   if (T == 0) return hipSuccess;
-  if (bf16)
-    return idx64 ? spread_k<uint16_t, int64_t>(src, w, w_f32, y, idx, inv, starts, counts, dst, dw, T, h, E, k, st)
-                 : spread_k<uint16_t, int32_t>(src, w, w_f32, y, idx, inv, starts, counts, dst, dw, T, h, E, k, st);
-  return idx64 ? spread_k<float, int64_t>(src, w, w_f32, y, idx, inv, starts, counts, dst, dw, T, h, E, k, st)
-               : spread_k<float, int32_t>(src, w, w_f32, y, idx, inv, starts, counts, dst, dw, T, h, E, k, st);
+  return bf16 ? spread_any<uint16_t>(src, w, w_f32, y, idx, idx64, inv, starts, counts, dst, dw, T, h, E, k, st)
+              : spread_any<float>(src, w, w_f32, y, idx, idx64, inv, starts, counts, dst, dw, T, h, E, k, st);
 }
 
-hipError_t launch_collect_rows(const void* src, const void* w, bool w_f32, const void* idx, bool idx64,
-                               const int32_t* inv, void* out, int64_t T, int h, int E, int k, bool bf16,
-                               hipStream_t st) {
+hipError_t launch_collect_rows(const void* src, const void* w, bool w_f32, const int32_t* inv, void* out, int64_t T, int h,
+                               int k, bool bf16, hipStream_t st) {
   if (T == 0) return hipSuccess;
-  if (bf16)
-    return idx64 ? collect_k<uint16_t, int64_t>(src, w, w_f32, idx, inv, out, T, h, E, k, st)
-                 : collect_k<uint16_t, int32_t>(src, w, w_f32, idx, inv, out, T, h, E, k, st);
-  return idx64 ? collect_k<float, int64_t>(src, w, w_f32, idx, inv, out, T, h, E, k, st)
-               : collect_k<float, int32_t>(src, w, w_f32, idx, inv, out, T, h, E, k, st);
+  int32_t* const plan = const_cast<int32_t*>(inv);  // only read without indices
+  return bf16 ? collect_k<uint16_t>(src, w, w_f32, plan, out, T, h, k, st)
+              : collect_k<float>(src, w, w_f32, plan, out, T, h, k, st);
 }
 
 }  // namespace q38

@@ -95,10 +95,8 @@ SIGNATURES = {
     "q38moe_clip_grads": (_c_int, [_vp] * 5 + [_c_i32, _c_i32, ctypes.c_float, _vp, _vp, _c_size, _vp]),
     "q38moe_rows_plan_ints": (_c_i64, [_c_i64, _c_i32, _c_i32]),
     "q38moe_dispatch_rows": (_c_int, [_vp, _vp, _c_i32, _vp, _vp, _c_i64, _c_i32, _c_i32, _c_i32, _c_i32, _vp]),
-    "q38moe_spread_rows": (_c_int, [_vp, _vp, _c_i32, _vp, _vp, _c_i32] + [_vp] * 3 +
-                           [_c_i64, _c_i32, _c_i32, _c_i32, _c_i32, _vp]),
-    "q38moe_collect_rows": (_c_int, [_vp, _vp, _c_i32, _vp, _c_i32, _vp, _vp, _c_i64, _c_i32, _c_i32, _c_i32, _c_i32,
-                                     _vp]),
+    "q38moe_spread_rows": (_c_int, [_vp, _vp, _c_i32] + [_vp] * 4 + [_c_i64, _c_i32, _c_i32, _c_i32, _c_i32, _vp]),
+    "q38moe_collect_rows": (_c_int, [_vp, _vp, _c_i32, _vp, _vp, _c_i64, _c_i32, _c_i32, _c_i32, _c_i32, _vp]),
 }
 
 

@@ -182,6 +182,11 @@ def _aligned(t):
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
+def _recorded(*tensors):
+    """True where a gradient of the call may be asked for, or a tangent carried through it (which these operators refuse)."""
+    return (torch.is_grad_enabled() and any(t.requires_grad for t in tensors)) or forward_ad._current_level >= 0
+
+
 class HipLinearCE(torch.autograd.Function):
     """Forward: maxima and sums of the logits' tiles; kept are the operands and the rows' log-sum-exp. Backward: the tiles again, in
     pieces of the vocabulary (q38moe_linear_ce_forward, _backward)."""
@@ -222,7 +227,7 @@ def linear_cross_entropy(x, weight, targets, ignore_index=-100, reduction="mean"
     if not flat:
         x = x.reshape(-1, x.shape[-1])
     args = (_aligned(x), _aligned(weight), (targets if flat else targets.reshape(-1)).contiguous(), ignore_index)
-    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
+    if _recorded(x, weight):
         loss = HipLinearCE.apply(*args, reduction)
     elif reduction == "none":
         loss = ops.linear_ce_forward(*args, want_lse=False)[0]
@@ -264,14 +269,14 @@ class HipCombine(torch.autograd.Function):
 def dispatch(x, topk_idx, num_experts):
     """Tokens x [T,h] (bf16 or fp32) in expert order, for experts of the caller's own: (rows [T*k,h], plan). Expert e's
     rows are rows[plan.starts[e] : plan.starts[e] + plan.counts[e]], in the order of the pairs; pairs routed outside [0, num_experts)
-    have none, and as many rows at the end are zero. topk_idx [T,k] int32 or int64; num_experts <= 64, k <= 8, h a
-    multiple of 64. Gradients flow to x. ``combine`` with the same plan brings the experts' outputs back."""
+    have none, and as many rows at the end are zero. topk_idx [T,k] int32 or int64, which may change afterwards; num_experts
+    <= 64, k <= 8, h a multiple of 64. Gradients flow to x. ``combine`` with the same plan brings the experts' outputs back."""
     if x.dim() != 2 or topk_idx.dim() != 2 or topk_idx.shape[0] != x.shape[0]:
         raise ValueError(f"x must be [T,h] and topk_idx [T,k], got {tuple(x.shape)} and {tuple(topk_idx.shape)}")
     ops._fdt(x, "x")
     plan = ops.RowsPlan(topk_idx.contiguous(), num_experts)
     x = _aligned(x)
-    return (HipDispatch.apply(x, plan) if torch.is_grad_enabled() and x.requires_grad else ops.dispatch_rows(x, plan)), plan
+    return (HipDispatch.apply(x, plan) if _recorded(x) else ops.dispatch_rows(x, plan)), plan
 
 
 def combine(rows, topk_w, plan):
@@ -282,6 +287,6 @@ def combine(rows, topk_w, plan):
     if dt == torch.float32 and topk_w.dtype == torch.bfloat16:
         topk_w = topk_w.float()
     rows, topk_w = _aligned(rows), topk_w.contiguous()
-    if torch.is_grad_enabled() and (rows.requires_grad or topk_w.requires_grad):
+    if _recorded(rows, topk_w):
         return HipCombine.apply(rows, topk_w, plan)
     return ops.collect_rows(rows, plan, topk_w)

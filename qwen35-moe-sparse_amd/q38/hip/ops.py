@@ -1013,17 +1013,17 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
 
 class RowsPlan:
     """Where the pairs of a routing idx [T,k] go: expert e's rows are starts[e] .. starts[e] + counts[e] - 1, row r is pair
-    perm[r] (token perm[r] // k; only rows that are filled), pair p is row inv[p] (only pairs routed inside [0, experts)).
-    ``dispatch_rows`` fills it."""
+    perm[r] (token perm[r] // k; only rows that are filled), pair p is row inv[p] (-1 for pairs routed outside
+    [0, experts)). ``dispatch_rows`` fills it; the indices are not looked at again."""
 
-    __slots__ = ("idx", "experts", "buffer")
+    __slots__ = ("idx", "experts", "buffer", "filled")
 
     def __init__(self, topk_idx, experts):
         _need(topk_idx, "topk_idx", dtype=None, ndim=2)
         _idx_flag(topk_idx)
         n = lib.q38moe_rows_plan_ints(*topk_idx.shape[:1], experts, topk_idx.shape[1])
         check(min(n, 0), "q38moe_rows_plan_ints")
-        self.idx, self.experts = topk_idx, experts
+        self.idx, self.experts, self.filled = topk_idx, experts, False
         self.buffer = torch.empty(n, dtype=torch.int32, device=topk_idx.device)
 
     def _part(self, i):
@@ -1054,11 +1054,21 @@ def dispatch_rows(x, plan):
         check(lib.q38moe_dispatch_rows(x.data_ptr(), plan.idx.data_ptr(), _idx_flag(plan.idx), plan.buffer.data_ptr(),
                                        dst.data_ptr(), T, h, plan.experts, k, _DTYPES[dt], _raw_stream(dev.index)),
               "q38moe_dispatch_rows")
+    plan.filled = True
     return dst
 
 
-def _rows_weights(w, shape, dt):
+def _filled(plan, dev, name):
+    if not plan.filled:
+        raise RuntimeError("the plan is empty: dispatch_rows fills it")
+    if plan.buffer.device != dev:
+        raise RuntimeError(f"{name} and the plan must be on one device")
+
+
+def _rows_weights(w, shape, dt, dev):
     _need(w, "weights", dtype=None, ndim=2)
+    if w.device != dev:
+        raise RuntimeError(f"weights must be on {dev}, got {w.device}")
     if w.dtype not in (dt, torch.float32):
         raise TypeError(f"weights must be {dt} or fp32, got {w.dtype}")
     if w.shape != shape:
@@ -1076,21 +1086,21 @@ def spread_rows(src, plan, w=None, y=None, need_rows=True):
     dev = src.device
     if src.shape[0] != T:
         raise ValueError(f"src must hold {T} tokens, got {src.shape[0]}")
-    if plan.buffer.device != dev:
-        raise RuntimeError("src and the plan must be on one device")
-    pw = None if w is None else _rows_weights(w, plan.idx.shape, dt)
+    _filled(plan, dev, "src")
+    pw = None if w is None else _rows_weights(w, plan.idx.shape, dt, dev)
     if y is not None:
         _same(y, "y", dt, (T * k, h))
+        if y.device != dev:
+            raise RuntimeError(f"y must be on {dev}, got {y.device}")
         if w is None:
             raise ValueError("y needs weights")
     dst = torch.empty(T * k, h, dtype=dt, device=dev) if need_rows else None
     dw = torch.empty_like(w) if y is not None else None
     with _on(dev):
         check(lib.q38moe_spread_rows(src.data_ptr(), pw, _DTYPES[dt if w is None else w.dtype],
-                                     None if y is None else y.data_ptr(), plan.idx.data_ptr(), _idx_flag(plan.idx),
-                                     plan.buffer.data_ptr(), dst.data_ptr() if need_rows else None,
-                                     None if dw is None else dw.data_ptr(), T, h, plan.experts, k, _DTYPES[dt],
-                                     _raw_stream(dev.index)), "q38moe_spread_rows")
+                                     None if y is None else y.data_ptr(), plan.buffer.data_ptr(),
+                                     dst.data_ptr() if need_rows else None, None if dw is None else dw.data_ptr(), T, h,
+                                     plan.experts, k, _DTYPES[dt], _raw_stream(dev.index)), "q38moe_spread_rows")
     return dst, dw
 
 
@@ -1104,12 +1114,11 @@ def collect_rows(rows, plan, w=None):
     dev = rows.device
     if rows.shape[0] != T * k:
         raise ValueError(f"rows must hold {T * k} rows, got {rows.shape[0]}")
-    if plan.buffer.device != dev:
-        raise RuntimeError("rows and the plan must be on one device")
-    pw = None if w is None else _rows_weights(w, plan.idx.shape, dt)
+    _filled(plan, dev, "rows")
+    pw = None if w is None else _rows_weights(w, plan.idx.shape, dt, dev)
     out = torch.empty(T, h, dtype=dt, device=dev)
     with _on(dev):
-        check(lib.q38moe_collect_rows(rows.data_ptr(), pw, _DTYPES[dt if w is None else w.dtype], plan.idx.data_ptr(),
-                                      _idx_flag(plan.idx), plan.buffer.data_ptr(), out.data_ptr(), T, h, plan.experts,
-                                      k, _DTYPES[dt], _raw_stream(dev.index)), "q38moe_collect_rows")
+        check(lib.q38moe_collect_rows(rows.data_ptr(), pw, _DTYPES[dt if w is None else w.dtype], plan.buffer.data_ptr(),
+                                      out.data_ptr(), T, h, plan.experts, k, _DTYPES[dt], _raw_stream(dev.index)),
+              "q38moe_collect_rows")
     return out

@@ -183,3 +183,42 @@ def test_captured_and_on_another_stream(gpu):
         torch.cuda.synchronize()
         got = [t.clone() for t in outs]
         assert all(torch.equal(a, b) for a, b in zip(got, step()))
+
+
+def test_indices_may_change_after_dispatch(gpu):
+    """Combine and the gradients follow the plan: indices overwritten since dispatch, dropped pairs made valid among them, reach
+    nothing."""
+    from q38.hip import autograd, ops
+    x, idx, w, y, d_rows, d_out = _inputs(77, 128, 16, 4, torch.bfloat16, gpu, dropped=0.5)
+
+    def run(spoil):
+        mine = idx.clone()
+        leaves = [a.clone().requires_grad_(True) for a in (x, w, y)]
+        rows, plan = autograd.dispatch(leaves[0], mine, 16)
+        assert bool(((plan.inv >= 0) == ((idx >= 0) & (idx < 16)).reshape(-1)).all())
+        if spoil:
+            mine.copy_(torch.arange(77 * 4, device=gpu).view(77, 4) % 16)
+        out = autograd.combine(leaves[2], leaves[1], plan)
+        return [rows, out, *torch.autograd.grad((rows, out), leaves, (d_rows, d_out))]
+
+    for a, b in zip(run(False), run(True)):
+        assert torch.equal(a, b)
+    with pytest.raises(RuntimeError, match="plan is empty"):
+        ops.collect_rows(y, ops.RowsPlan(idx, 16))
+    with pytest.raises(RuntimeError, match="plan is empty"):
+        ops.spread_rows(x, ops.RowsPlan(idx, 16))
+
+
+def test_forward_mode_is_refused(gpu):
+    """A tangent is not dropped silently."""
+    import torch.autograd.forward_ad as fwad
+    from q38.hip import autograd
+    x, idx, w, y, _, _ = _inputs(8, 64, 4, 2, torch.float32, gpu)
+    _, plan = autograd.dispatch(x, idx, 4)
+    head, t = torch.randn(10, 64, device=gpu), torch.zeros(8, dtype=torch.int64, device=gpu)
+    with fwad.dual_level():
+        dual = fwad.make_dual(x, torch.ones_like(x))
+        for f in (lambda: autograd.dispatch(dual, idx, 4), lambda: autograd.linear_cross_entropy(dual, head, t),
+                  lambda: autograd.combine(fwad.make_dual(y, torch.ones_like(y)), w, plan)):
+            with pytest.raises(Exception, match="jvp|forward mode"):
+                f()

@@ -145,8 +145,8 @@ def test_rows_abi_arguments():
     m = _lib()
     lib, p = m.lib, ctypes.c_void_p(1 << 20)
 
-    def spread(src=p, w=None, w_dtype=1, y=None, idx=p, plan=p, dst=p, dw=None, T=4, h=64, E=8, k=2, dtype=1):
-        return lib.q38moe_spread_rows(src, w, w_dtype, y, idx, 1, plan, dst, dw, T, h, E, k, dtype, None)
+    def spread(src=p, w=None, w_dtype=1, y=None, plan=p, dst=p, dw=None, T=4, h=64, E=8, k=2, dtype=1):
+        return lib.q38moe_spread_rows(src, w, w_dtype, y, plan, dst, dw, T, h, E, k, dtype, None)
 
     def says(text):
         return text in lib.q38moe_last_error().decode()
@@ -164,9 +164,10 @@ def test_rows_abi_arguments():
     assert lib.q38moe_dispatch_rows(None, p, 1, p, p, 4, 64, 8, 2, 1, None) == -1 and says("x must not")
     assert lib.q38moe_dispatch_rows(p, p, 1, p, p, 4, 100, 8, 2, 1, None) == -1 and says("h must be")
     assert spread(T=0) == 0 and spread(dst=None) == 0
-    assert lib.q38moe_collect_rows(None, None, 1, p, 1, p, p, 4, 64, 8, 2, 1, None) == -1 and says("src")
-    assert lib.q38moe_collect_rows(p, None, 1, None, 1, p, p, 4, 64, 8, 2, 1, None) == -1 and says("topk_idx")
-    assert lib.q38moe_collect_rows(None, None, 1, None, 1, None, None, 0, 64, 8, 2, 1, None) == 0
+    assert lib.q38moe_dispatch_rows(p, None, 1, p, p, 4, 64, 8, 2, 1, None) == -1 and says("topk_idx")
+    assert lib.q38moe_collect_rows(None, None, 1, p, p, 4, 64, 8, 2, 1, None) == -1 and says("src")
+    assert lib.q38moe_collect_rows(p, None, 1, None, p, 4, 64, 8, 2, 1, None) == -1 and says("plan")
+    assert lib.q38moe_collect_rows(None, None, 1, None, None, 0, 64, 8, 2, 1, None) == 0
 
 
 def test_model_loss_refuses_other_labels():
