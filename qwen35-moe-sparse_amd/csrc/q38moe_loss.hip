@@ -27,8 +27,8 @@
 // What bounds it. The matrix units need 2051 clocks for a step of a 256 x 256 tile. With all CUs at work on random bf16 data the
 // chip lowers its clock to 1.7 - 1.9 GHz: MFMAs alone take 1.09 us a step, with their LDS reads 1.23, with the copies to
 // LDS out of the L2 1.33 (all zeros: 0.94, 0.96, 1.04), and with a stream of its own per CU 1.94; this kernel, whose
-// tiles share the streams eight by four, takes 1.7. 16384 x 1024 x 10112: z 302 us (1120 TFLOP/s), s 2 x 172, dx 2 x 155, dW
-// 2 x 165. 4099 x 2048 x 50021: z 700 us (1200), s 2 x 400, dx 2 x 430, dW 2 x 408. Few tokens are bound by the latency of W's
+// tiles share the streams eight by four, takes 1.7. 16384 x 1024 x 10112: z 302 us (1120 TFLOP/s), s 2 x 168, dx 2 x 158, dW
+// 2 x 165. 4099 x 2048 x 50021: z 700 us (1190), s 2 x 391, dx 2 x 426, dW 2 x 410. Few tokens are bound by the latency of W's
 // way into LDS: 61 x 1024 x 10112 z 10 us for 20.7 MB.
 #include "q38moe_common.h"
 #include "q38moe_kernels.h"
@@ -183,14 +183,13 @@ struct LsParams {
   bool raw64;
   float* zt;             // the target's logit
   uint32_t* done;        // EPI_LSE: cleared for ls_finish_kernel
-  const float* lse;      // by original row
-  const float* g_row;    // gradient per original row, or NULL
+  const float* lse;      // EPI_S: per counted token
+  const float* g_row;    // its gradient, or NULL
   // EPI_S, EPI_OUT
   void* out;             // s, or the gradient
   int64_t ldo;           // elements between rows of out
   const float* g_scale;  // the loss's gradient (NULL: 1)
   const float* r_scale;  // the reduction's factor (NULL: 1)
-  bool scatter;          // rows of out through `rows`
   float* acc;            // tiles' sums over the pieces so far (fp32, in the accumulators' own order), or NULL
   bool first, last;      // piece: acc holds nothing yet; out is written (else acc)
   float* split;          // partial sums of split tiles, a tile after another
@@ -415,6 +414,33 @@ __global__ __launch_bounds__(256, ls_per_cu(BM, EPI)) void ls_gemm_kernel(const 
   LsItem it = item_of(0);
   uint32_t item = 0;
   int slot = 0;
+  // What a tile's tokens bring to its epilogue: the target, lse and gradient, or the row of out; lane l holds token 32 j + l % 32's.
+  // Read at the tile's start: in the epilogue each read would wait for memory, and for the copies under way before it.
+  int32_t tk[NB];
+  float tl[NB], tg[NB];
+  auto tokens = [&]() {
+#pragma unroll
+    for (int j = 0; j < NB; ++j) {
+      const int64_t n = (int64_t)it.n * BN + wn * (BN / 2) + 32 * j + (lane & 31);
+      const bool ok = n < N;
+      tk[j] = -1;
+      if constexpr (EPI == EPI_LSE) {
+        if (ok) tk[j] = p.raw != nullptr ? raw_target(p.raw, p.raw64, n) : p.tgt[n];
+      } else if constexpr (EPI == EPI_S) {
+        tl[j] = 0.0f;
+        tg[j] = 1.0f;
+        if (ok) {
+          tk[j] = p.tgt[n];
+          tl[j] = p.lse[n];
+          if (p.g_row != nullptr) tg[j] = p.g_row[n];
+        }
+      } else if (LB == KC) {
+        tk[j] = (int32_t)n;
+        if (!all && ok) tk[j] = p.rows[n];
+      }
+    }
+  };
+  tokens();
 #pragma unroll 1
   for (;;) {
 #pragma unroll 1
@@ -446,6 +472,13 @@ __global__ __launch_bounds__(256, ls_per_cu(BM, EPI)) void ls_gemm_kernel(const 
       // this slot are done, and so are the others'.
       asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NS - 2) * NC) : "memory");
       ls_barrier();
+      if constexpr (NS == 2) {  // the tokens' reads have landed with the copies: no wait for them later
+#pragma unroll
+        for (int j = 0; j < NB; ++j) {
+          asm volatile("" : "+v"(tk[j]));
+          if constexpr (EPI == EPI_S) asm volatile("" : "+v"(tl[j]), "+v"(tg[j]));
+        }
+      }
       quarter(1, next, 0, 0, C3, slot);
       slot = then;
     }
@@ -465,22 +498,11 @@ __global__ __launch_bounds__(256, ls_per_cu(BM, EPI)) void ls_gemm_kernel(const 
     for (int j = 0; j < NB; ++j) {
       const int64_t n = nw + 32 * j + (lane & 31);
       const bool n_ok = n < N;
-      // Per token: where its target lies among the wave's rows, and what the softmax needs.
-      int rel = -1;
-      float lse = 0.0f, g = 1.0f, mx = -__builtin_inff(), sum = 0.0f;
-      int64_t row = n;
-      if constexpr (EPI == EPI_LSE) {
-        if (n_ok) rel = (p.raw != nullptr ? raw_target(p.raw, p.raw64, n) : p.tgt[n]) - (int)mw;
-      } else if constexpr (EPI == EPI_S) {
-        if (n_ok) {
-          const int64_t r = p.rows[n];
-          rel = p.tgt[n] - (int)p.v0 - (int)mw;
-          lse = p.lse[r];
-          if (p.g_row != nullptr) g = p.g_row[r];
-        }
-      } else if constexpr (F32 && EPI == EPI_OUT) {
-        if (n_ok && p.scatter) row = p.rows[n];
-      }
+      // Where the token's target lies among the wave's rows, and what the softmax needs.
+      const int rel = EPI == EPI_OUT ? -1 : tk[j] - (EPI == EPI_S ? (int)p.v0 : 0) - (int)mw;
+      const float lse = EPI == EPI_S ? tl[j] : 0.0f, g = EPI == EPI_S ? tg[j] : 1.0f;
+      const int64_t row = LB == KC && EPI == EPI_OUT ? (int64_t)tk[j] : n;
+      float mx = -__builtin_inff(), sum = 0.0f;
 #pragma unroll
       for (int i = 0; i < MB; ++i) {
         f32x16_t v = ls_take(acc[i][j]);
@@ -565,8 +587,8 @@ __global__ __launch_bounds__(256, ls_per_cu(BM, EPI)) void ls_gemm_kernel(const 
           const int rr = k * RPI + lane / CH;
           const u32x4_t w = ld16(stw + rr * BM + 16 * (c ^ (rr & (CH - 1))));
           const int64_t nn = nw + 32 * j + rr;
+          const int64_t r = EPI == EPI_OUT && LB == KC ? (int64_t)__shfl(tk[j], rr) : nn;
           if (nn < N && 8 * c < mstore) {
-            const int64_t r = EPI == EPI_OUT && p.scatter ? (int64_t)p.rows[nn] : nn;
             st16(static_cast<uint16_t*>(p.out) + r * p.ldo + mw + 8 * c, w);
           }
         }
@@ -574,28 +596,34 @@ __global__ __launch_bounds__(256, ls_per_cu(BM, EPI)) void ls_gemm_kernel(const 
     }
     if (++item >= total) break;
     it = item_of(item);
+    tokens();
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 }
 
 // Partition of the rows: rows[0 .. n-1] those that count, ascending, rows[n .. T-1] the ignored ones, *count = n, tgt[i]
-// the target of rows[i] (-1: outside the vocabulary). One block; ballots give a row's place, 8192 rows at a time (16384 rows:
+// the target of rows[i] (-1: outside the vocabulary), and where given lse_c[i] = lse[rows[i]], g_c[i] = g[rows[i]]. One block; ballots give a row's place, 8192 rows at a time (16384 rows:
 // 4.5 us, 14.5 with 1024 at a time).
 template <typename IdxT>
 __global__ __launch_bounds__(1024) void ls_rows_kernel(const IdxT* __restrict__ targets, int64_t ignore, int64_t T, int V,
                                                        int32_t* __restrict__ rows, int32_t* __restrict__ tgt,
-                                                       int32_t* __restrict__ count) {
+                                                       int32_t* __restrict__ count, const float* __restrict__ lse,
+                                                       float* __restrict__ lse_c, const float* __restrict__ g,
+                                                       float* __restrict__ g_c) {
   constexpr int E = 8;  // runs of 1024 rows
   __shared__ int sums[E * 16 + 1];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   int64_t kept = 0;  // rows that count, so far
   for (int64_t t0 = 0; t0 < T; t0 += E * 1024) {
     int64_t v[E];
+    float l[E], r[E];
     uint64_t mask[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) {
       const int64_t t = t0 + e * 1024 + tid;
       v[e] = t < T ? (int64_t)targets[t] : ignore;
+      l[e] = lse != nullptr && t < T ? lse[t] : 0.0f;
+      r[e] = g != nullptr && t < T ? g[t] : 0.0f;
     }
 #pragma unroll
     for (int e = 0; e < E; ++e) {
@@ -624,6 +652,8 @@ __global__ __launch_bounds__(1024) void ls_rows_kernel(const IdxT* __restrict__ 
       if (v[e] != ignore) {
         rows[before] = (int32_t)t;
         tgt[before] = v[e] >= 0 && v[e] < V ? (int32_t)v[e] : -1;
+        if (lse != nullptr) lse_c[before] = l[e];
+        if (g != nullptr) g_c[before] = r[e];
       } else {
         rows[T - 1 - (t - before)] = (int32_t)t;  // from the end
       }
@@ -805,7 +835,7 @@ __global__ __launch_bounds__(256) void ls_join_kernel(const LsParams p) {
       for (int k = 0; k < 8; ++k) *reinterpret_cast<f32x4_t*>(c + 256 * (k >> 1) + 128 * (k & 1)) = v[k];
       continue;
     }
-    E* const o = static_cast<E*>(p.out) + (p.scatter ? (int64_t)p.rows[n] : n) * p.ldo + m;
+    E* const o = static_cast<E*>(p.out) + (TOK_K || cnt >= p.T ? n : (int64_t)p.rows[n]) * p.ldo + m;
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
       v[k] *= scale;
@@ -870,7 +900,7 @@ size_t acc_bytes(int64_t M, int64_t N, int b) { return 4 * (size_t)(b * b) * (si
 size_t up(size_t v) { return (v + 255) / 256 * 256; }
 
 struct Layout {
-  size_t rows, tgt, count, xc, part, zt, bsum, bn, done, s, acc, split, end;
+  size_t rows, tgt, count, xc, part, zt, bsum, bn, done, lse, g, s, acc, split, end;
   int entries;             // of the forward's partial sums
   int64_t piece;           // vocabulary rows of a piece (multiple of 256)
   int pieces;
@@ -910,6 +940,8 @@ Layout layout(int64_t T, int h, int V, bool f32, bool fwd, bool need_x, bool nee
     const int64_t pt = ceil_div(vt, l.pieces);
     l.pieces = (int)ceil_div(vt, pt);
     l.piece = pt * 256;
+    l.lse = take(4 * T);
+    l.g = take(4 * T);
     l.s = take(esz * (size_t)T * l.piece);
     const int64_t bk = f32 ? 32 : 64, n = l.piece < V ? l.piece : V;
     l.tile_s = tile_z(n, T, f32);
@@ -935,13 +967,13 @@ P* at(void* base, size_t off) {
   } while (0)
 
 hipError_t ls_rows(const void* targets, bool idx64, int64_t ignore, int64_t T, int V, int32_t* rows, int32_t* tgt,
-                   int32_t* count, hipStream_t st) {
+                   int32_t* count, const float* lse, float* lse_c, const float* g, float* g_c, hipStream_t st) {
   if (idx64)
     hipLaunchKernelGGL(ls_rows_kernel<int64_t>, dim3(1), dim3(1024), 0, st, (const int64_t*)targets, ignore, T, V, rows,
-                       tgt, count);
+                       tgt, count, lse, lse_c, g, g_c);
   else
     hipLaunchKernelGGL(ls_rows_kernel<int32_t>, dim3(1), dim3(1024), 0, st, (const int32_t*)targets, ignore, T, V, rows,
-                       tgt, count);
+                       tgt, count, lse, lse_c, g, g_c);
   return hipGetLastError();
 }
 
@@ -970,7 +1002,7 @@ hipError_t ce_forward(const void* x, const void* w, const void* targets, bool id
   int32_t* count = at<int32_t>(ws, l.count);
   const int64_t rb = (int64_t)h * (F32 ? 4 : 2);
   if (!l.raw) {
-    LS_TRY(ls_rows(targets, idx64, ignore, T, V, rows, tgt, count, st));
+    LS_TRY(ls_rows(targets, idx64, ignore, T, V, rows, tgt, count, nullptr, nullptr, nullptr, nullptr, st));
     LS_TRY(ls_gather(x, rows, count, at<void>(ws, l.xc), nullptr, T, (int)rb, st));
   }
   LsParams p = {};
@@ -1006,7 +1038,8 @@ hipError_t ce_backward(const float* g, bool g_rows, const float* r_scale, const 
   int32_t* count = at<int32_t>(ws, l.count);
   const int64_t rb = (int64_t)h * (F32 ? 4 : 2);
   const int64_t esz = F32 ? 4 : 2;
-  LS_TRY(ls_rows(targets, idx64, ignore, T, V, rows, tgt, count, st));
+  LS_TRY(ls_rows(targets, idx64, ignore, T, V, rows, tgt, count, lse, at<float>(ws, l.lse), g_rows ? g : nullptr,
+                 at<float>(ws, l.g), st));
   LS_TRY(ls_gather(x, rows, count, at<void>(ws, l.xc), dx, T, (int)rb, st));
   const uint8_t* xc = at<const uint8_t>(ws, l.xc);
   const float* scale = g_rows ? nullptr : g;
@@ -1017,7 +1050,6 @@ hipError_t ce_backward(const float* g, bool g_rows, const float* r_scale, const 
     LsParams p = {};
     p.T = T;
     p.count = count;
-    p.rows = rows;
     // s [T, pitch]
     p.A = wp;
     p.B = xc;
@@ -1027,8 +1059,8 @@ hipError_t ce_backward(const float* g, bool g_rows, const float* r_scale, const 
     p.K = h;
     p.v0 = v0;
     p.tgt = tgt;
-    p.lse = lse;
-    p.g_row = g_rows ? g : nullptr;
+    p.lse = at<float>(ws, l.lse);
+    p.g_row = g_rows ? at<float>(ws, l.g) : nullptr;
     p.out = at<void>(ws, l.s);
     p.ldo = pitch;
     p.M = pitch;  // whole tiles: the columns behind the piece become zeros
@@ -1051,7 +1083,6 @@ hipError_t ce_backward(const float* g, bool g_rows, const float* r_scale, const 
       q.N = T;
       q.K = n;
       q.out = dx;
-      q.scatter = true;
       q.acc = at<float>(ws, l.acc);
       q.first = i == 0;
       q.last = i == l.pieces - 1;
@@ -1063,7 +1094,6 @@ hipError_t ce_backward(const float* g, bool g_rows, const float* r_scale, const 
       q.N = n;
       q.K = T;
       q.out = static_cast<uint8_t*>(dw) + v0 * rb;
-      q.scatter = false;
       q.first = q.last = true;
       LS_TRY((ls_gemm_any<F32, KS, KS, EPI_OUT>(q, l.tile_w, st)));
     }
