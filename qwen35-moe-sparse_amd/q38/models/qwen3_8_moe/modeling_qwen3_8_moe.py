@@ -263,7 +263,9 @@ class Qwen3_8MoeForCausalLM(Qwen3_8MoePreTrainedModel):
             logits = loss = None
             if labels is None or logits_to_keep is not None:
                 keep = slice(-logits_to_keep, None) if isinstance(logits_to_keep, int) else logits_to_keep
-                logits = self.lm_head(hs[:, keep, :])
+                # Contiguous: of a strided batch torch makes a bf16 batched product with a transposed right operand, which
+                # has given wrong values and faults on this GPU.
+                logits = self.lm_head(hs[:, keep, :].contiguous())
             aux = _prefill.load_balancing_loss(router, cfg.experts, cfg.topk) if want else None
             if labels is not None:
                 loss = _prefill.next_token_loss(hs, self.lm_head.weight, labels.to(hs.device))

@@ -278,6 +278,9 @@ def test_causal_lm_labels(gpu):
     assert plain.loss is None and torch.equal(out.logits, plain.logits)
     last = model(input_ids=ids, labels=labels, logits_to_keep=1)
     assert torch.equal(last.loss, out.loss) and last.logits.shape[1] == 1
+    # The same rows of the same product, but for the order of its sums over 128 terms and its rounding.
+    z = plain.logits[:, -1:].float()
+    assert bool(((last.logits.float() - z).abs() <= 2 * 2.0 ** -8 * z.abs() + 1e-3).all())
     none = model(input_ids=ids, labels=labels, logits_to_keep=None)
     assert none.logits is None and torch.equal(none.loss, out.loss)
     aux = model(input_ids=ids, labels=labels.cpu(), output_router_logits=True)
