@@ -52,6 +52,13 @@ __device__ __forceinline__ void ls_dma(const uint8_t* p, int64_t bytes, uint32_t
   const u32x4_t r = {uniform((uint32_t)a), uniform((uint32_t)(a >> 32) & 0xffffu), uniform(n), 0x00020000u};
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(lds), "v"(voff), "s"(r), "s"(soff) : "memory", "m0");
 }
+// 16 bytes to p + off (p uniform), through the XCD's L2 (scope sc1): what a kernel leaves there has to be written back before the
+// next one starts. For whole lines: s of 1024 x 1024 x 10112 36 -> 34 us, of 1024 x 1024 x 5056 21.3 -> 19.6, dW 47 -> 44.8; fp32, whose
+// lanes store parts of lines, 43.6 -> 47. Past it (non-temporal) s is not found by its readers either (dx 32.7 -> 41 us).
+__device__ __forceinline__ void ls_store_through(void* p, uint32_t off, u32x4_t v) {
+  const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(p, (short)0, -1, 0x00020000);
+  __builtin_amdgcn_raw_buffer_store_b128(v, r, (int)off, 0, 16);
+}
 __device__ __forceinline__ uint32_t ls_lds_addr(const void* p) {
   return uniform((uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)p);
 }
@@ -265,7 +272,9 @@ __global__ __launch_bounds__(256, ls_per_cu(BM, EPI)) void ls_gemm_kernel(const 
   // Staging of bf16 outputs, 32 rows of out by BM / 2 columns per wave (beside the slots: copies for the next item run meanwhile).
   constexpr bool STAGED = !F32 && (EPI == EPI_S || EPI == EPI_OUT);
   __shared__ __align__(1024) uint8_t stage[STAGED ? 4 * 32 * BM : 16];
+  constexpr bool TO_ROWS = EPI == EPI_OUT && LB == KC;  // dx: rows of out through `rows`
   constexpr int CH = BM / 16, RPI = 64 / CH;  // 16-byte chunks of a staged row, rows of a store
+  constexpr int KB = 32 / RPI < 4 ? 32 / RPI : 4;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = (int)uniform((uint32_t)tid >> 6);
   const int wm = wave >> 1, wn = wave & 1;
@@ -434,7 +443,7 @@ __global__ __launch_bounds__(256, ls_per_cu(BM, EPI)) void ls_gemm_kernel(const 
           tl[j] = p.lse[n];
           if (p.g_row != nullptr) tg[j] = p.g_row[n];
         }
-      } else if (LB == KC) {
+      } else if (TO_ROWS) {
         tk[j] = (int32_t)n;
         if (!all && ok) tk[j] = p.rows[n];
       }
@@ -501,7 +510,7 @@ __global__ __launch_bounds__(256, ls_per_cu(BM, EPI)) void ls_gemm_kernel(const 
       // Where the token's target lies among the wave's rows, and what the softmax needs.
       const int rel = EPI == EPI_OUT ? -1 : tk[j] - (EPI == EPI_S ? (int)p.v0 : 0) - (int)mw;
       const float lse = EPI == EPI_S ? tl[j] : 0.0f, g = EPI == EPI_S ? tg[j] : 1.0f;
-      const int64_t row = LB == KC && EPI == EPI_OUT ? (int64_t)tk[j] : n;
+      const int64_t row = TO_ROWS ? (int64_t)tk[j] : n;
       float mx = -__builtin_inff(), sum = 0.0f;
 #pragma unroll
       for (int i = 0; i < MB; ++i) {
@@ -583,13 +592,23 @@ __global__ __launch_bounds__(256, ls_per_cu(BM, EPI)) void ls_gemm_kernel(const 
         if (!to_out) continue;
         const int mstore = EPI == EPI_S ? BM / 2 : mleft, c = lane % CH;
 #pragma unroll
-        for (int k = 0; k < 32 / RPI; ++k) {
-          const int rr = k * RPI + lane / CH;
-          const u32x4_t w = ld16(stw + rr * BM + 16 * (c ^ (rr & (CH - 1))));
-          const int64_t nn = nw + 32 * j + rr;
-          const int64_t r = EPI == EPI_OUT && LB == KC ? (int64_t)__shfl(tk[j], rr) : nn;
-          if (nn < N && 8 * c < mstore) {
-            st16(static_cast<uint16_t*>(p.out) + r * p.ldo + mw + 8 * c, w);
+        for (int k0 = 0; k0 < 32 / RPI; k0 += KB) {  // several reads under way: one at a time the tile's 32 would wait for one another
+          u32x4_t w[KB];
+#pragma unroll
+          for (int k = 0; k < KB; ++k) {
+            const int rr = (k0 + k) * RPI + lane / CH;
+            w[k] = ld16(stw + rr * BM + 16 * (c ^ (rr & (CH - 1))));
+          }
+#pragma unroll
+          for (int k = 0; k < KB; ++k) {
+            const int rr = (k0 + k) * RPI + lane / CH;
+            const int64_t nn = nw + 32 * j + rr;
+            const int r = TO_ROWS ? __shfl(tk[j], rr) : 32 * j + rr;
+            if (nn < N && 8 * c < mstore) {
+              if constexpr (TO_ROWS) st16(static_cast<uint16_t*>(p.out) + r * p.ldo + mw + 8 * c, w[k]);
+              else ls_store_through(static_cast<uint16_t*>(p.out) + nw * p.ldo + mw,
+                                    2u * ((uint32_t)r * (uint32_t)p.ldo + 8u * (uint32_t)c), w[k]);
+            }
           }
         }
       }
