@@ -210,28 +210,32 @@ struct LsParams {
 //   parts = 0: all steps of the rest evenly, `per` neighbouring ones to a workgroup, which reach over at most two tiles, a
 //              tile cut at most 17-fold.
 // In steps' time (1.7 us on 256 x 256): an item costs 3 beside its own; equal parts 4 and 16 for each round of partial sums,
-// even runs 42. Measured: 80 tiles of 256 steps 164 us in 3 parts and 197 in even runs, 136 tiles of 392 steps 500 and 425.
+// even runs 42. Measured: 80 tiles of 256 steps 164 us in 3 parts and 197 in even runs, 136 tiles of 392 steps 500 and 425. Even runs
+// share no operand rows: bf16 tiles of 128 x 128 (`eager`), whose step takes half as long, then wait for memory, 2.5 times as long
+// (376 tiles of 158 steps: 257 us in even runs, 160 whole).
 struct LsPlan {
   uint32_t full, rest, steps, per, parts;
+  uint32_t cost;  // of the last, partial round
 };
 constexpr uint32_t LS_CUTS = 16;
-__host__ __device__ inline LsPlan ls_plan(uint32_t tiles, uint32_t steps, uint32_t slots) {
+__host__ __device__ inline LsPlan ls_plan(uint32_t tiles, uint32_t steps, uint32_t slots, bool eager) {
   const uint32_t rest = tiles % slots;
-  LsPlan pl = {tiles, 0, steps, steps, 1};
+  LsPlan pl = {tiles, 0, steps, steps, 1, rest != 0 ? steps + 3 : 0};
   if (rest == 0) return pl;
   const uint64_t even = ((uint64_t)rest * steps + slots - 1) / slots;
   const uint32_t least = (steps + LS_CUTS - 1) / LS_CUTS, run = even > least ? (uint32_t)even : least;
   uint32_t best = steps + 3;
-  if (run + 42 < best) {
-    best = run + 42;
-    pl = LsPlan{tiles - rest, rest, steps, run, 0};
+  const uint32_t run_cost = (eager ? run * 5 / 2 : run) + 42;
+  if (run_cost < best) {
+    best = run_cost;
+    pl = LsPlan{tiles - rest, rest, steps, run, 0, best};
   }
   for (uint32_t q = 2; q <= 8 && q <= steps && rest * q <= 2 * slots; ++q) {
     const uint32_t per = (steps + q - 1) / q, parts = (steps + per - 1) / per, load = rest * parts;
     const uint32_t cost = (load + slots - 1) / slots * (per + 3) + 4 + 16 * load / slots;
     if (cost < best) {
       best = cost;
-      pl = LsPlan{tiles - rest, rest, steps, per, parts};
+      pl = LsPlan{tiles - rest, rest, steps, per, parts, best};
     }
   }
   return pl;
@@ -297,8 +301,8 @@ __global__ __launch_bounds__(256, ls_per_cu(BM, EPI)) void ls_gemm_kernel(const 
   // Work items of neighbouring blocks on an XCD are neighbouring tiles: 8 tiles of M by as many of N as it has room for.
   const uint32_t G = gridDim.x;
   const uint32_t first = (G & 7) == 0 ? (blockIdx.x & 7) * (G >> 3) + (blockIdx.x >> 3) : blockIdx.x;
-  const LsPlan pl = EPI == EPI_OUT ? ls_plan(tiles, (uint32_t)steps, p.slots)
-                                   : LsPlan{tiles, 0, (uint32_t)steps, (uint32_t)steps, 1};
+  const LsPlan pl = EPI == EPI_OUT ? ls_plan(tiles, (uint32_t)steps, p.slots, !F32 && BM == 128)
+                                   : LsPlan{tiles, 0, (uint32_t)steps, (uint32_t)steps, 1, 0};
   // This block's items: its tiles of the whole rounds, then (with the grid of p.slots blocks) its share of the rest.
   const uint32_t rounds = first < pl.full ? (pl.full - first - 1) / G + 1 : 0;
   uint32_t lo = 0, cut = 0, hi = 0;  // even runs: steps lo .. cut - 1 of its first tile, cut .. hi - 1 of the next
@@ -817,7 +821,7 @@ __global__ __launch_bounds__(256) void ls_join_kernel(const LsParams p) {
   const int64_t cnt = (int64_t)load_uniform(p.count);
   const int64_t N = TOK_K ? p.N : cnt, K = TOK_K ? cnt : p.K;
   const uint32_t ntm = (uint32_t)((p.M + BM - 1) / BM), ntn = (uint32_t)((N + BN - 1) / BN);
-  const LsPlan pl = ls_plan(ntm * ntn, (uint32_t)((K + BK - 1) / BK), p.slots);
+  const LsPlan pl = ls_plan(ntm * ntn, (uint32_t)((K + BK - 1) / BK), p.slots, sizeof(E) == 2 && BM == 128);
   float scale = 1.0f;
   if (p.last && p.g_scale != nullptr) scale *= *p.g_scale;
   if (p.last && p.r_scale != nullptr) scale *= *p.r_scale;
@@ -897,14 +901,22 @@ int tile_z(int64_t M, int64_t N, bool f32) {
   return 7 * ceil_div(ceil_div(M, 256) * ceil_div(N, 256), cus) <= 4 * ceil_div(n128, 2 * cus) ? 256 : 128;
 }
 
-// Of the gradients' products, whose tiles can be split over K. 64 (with eight steps in LDS) for few tiles of 128, or
-// for less than every CU's and little K (dx of 61 x 1024 x 10112: 37 and 49 us with the rest of the call, of 600 tokens
-// 88 and 63; dw of 1000 x 512 x 2000: 27 and 47). bf16: 256 where each CU has at least 12 steps of such tiles (dx of 300 x
-// 2048 x 50021: 231 us, with 128 292; of 1000 x 1024 x 10112 96 and 83); fp32 has no use for them.
+// A product's time over K that may be split, in steps of its tiles.
+uint64_t ls_cost(int64_t M, int64_t N, int64_t steps, int b) {
+  const uint32_t tiles = (uint32_t)(ceil_div(M, b) * ceil_div(N, b)), slots = ls_slots(b, EPI_OUT);
+  return (uint64_t)(tiles / slots) * (uint64_t)(steps + 3) + ls_plan(tiles, (uint32_t)steps, slots, b == 128).cost;
+}
+
+// Of the gradients' products, whose tiles can be split over K. 64 (with eight steps in LDS) for few tiles of 128, or for less than
+// every CU's and little K (dx of 61 x 1024 x 10112: 37 and 49 us with the rest of the call, of 600 tokens 88 and 63, of 400 x
+// 1024 x 30000, 32 tiles, 173 and 116; dw of 2600 x 512 x 2000 39 and 47). Else bf16 takes 128 or 256 by the time that the plan
+// gives either, a step of 256 being worth 1.6 (two of 128 to a CU): dx of 1280 x 1024 x 10112 88 and 100 us, of 1536 x 2048 x
+// 50021 762 and 648; dw of 6000 x 1024 x 10112 290 and 321, of 1536 x 2048 x 50021 727 and 667. fp32 has no use for 256.
 int tile_k(int64_t M, int64_t N, int64_t steps, bool f32) {
   const int64_t cus = device_cus(), n128 = ceil_div(M, 128) * ceil_div(N, 128);
-  if (8 * n128 <= cus || (n128 < cus && n128 * steps < (f32 ? 16 : 8) * cus)) return 64;
-  return !f32 && ceil_div(M, 256) * ceil_div(N, 256) * steps >= 12 * cus ? 256 : 128;
+  if (f32) return 8 * n128 <= cus || (n128 < cus && n128 * steps < 16 * cus) ? 64 : 128;
+  if (8 * n128 < cus || (n128 < cus && n128 * steps < 12 * cus)) return 64;
+  return 8 * ls_cost(M, N, steps, 256) <= 5 * ls_cost(M, N, steps, 128) ? 256 : 128;
 }
 
 int ls_finish_rows(int64_t T) { return T <= 2048 ? 16 : 64; }
