@@ -303,13 +303,23 @@ __global__ __launch_bounds__(256, ls_per_cu(BM, EPI)) void ls_gemm_kernel(const 
   const uint32_t first = (G & 7) == 0 ? (blockIdx.x & 7) * (G >> 3) + (blockIdx.x >> 3) : blockIdx.x;
   const LsPlan pl = EPI == EPI_OUT ? ls_plan(tiles, (uint32_t)steps, p.slots, !F32 && BM == 128)
                                    : LsPlan{tiles, 0, (uint32_t)steps, (uint32_t)steps, 1, 0};
+  // Of n items that are fewer than the blocks: this block's, or n. Each XCD has an eighth, neighbours, for its first blocks (dealt
+  // like whole rounds, they would all go to the first XCDs: dW of 1777 x 1024 x 10112 with the rest of the call 106 us, so 119; the
+  // fp32 forward of 1024 x 512 x 10112 106 and 134).
+  auto partial = [&](uint32_t n) -> uint32_t {
+    if ((G & 7) != 0) return min((uint32_t)blockIdx.x, n);
+    const uint32_t share = (n + 7) >> 3, i = blockIdx.x >> 3, at = (blockIdx.x & 7) * share + i;
+    return i < share ? min(at, n) : n;
+  };
   // This block's items: its tiles of the whole rounds, then (with the grid of p.slots blocks) its share of the rest.
-  const uint32_t rounds = first < pl.full ? (pl.full - first - 1) / G + 1 : 0;
+  const uint32_t whole = pl.full / G, left = pl.full - whole * G, last_tile = partial(left);
+  const uint32_t rounds = whole + (last_tile < left ? 1 : 0);
+  const uint32_t load = pl.rest * pl.parts, load1 = load / G, load_left = load - load1 * G, last_part = partial(load_left);
   uint32_t lo = 0, cut = 0, hi = 0;  // even runs: steps lo .. cut - 1 of its first tile, cut .. hi - 1 of the next
   uint32_t total = rounds;
   if (EPI == EPI_OUT && pl.rest != 0) {
     if (pl.parts != 0) {
-      total += (first < pl.rest * pl.parts ? 1 : 0) + (first + G < pl.rest * pl.parts ? 1 : 0);
+      total += load1 + (last_part < load_left ? 1 : 0);
     } else {
       const uint32_t units = pl.rest * pl.steps;  // < 2^29
       lo = min(first * pl.per, units);
@@ -320,11 +330,11 @@ __global__ __launch_bounds__(256, ls_per_cu(BM, EPI)) void ls_gemm_kernel(const 
   }
   if (total == 0) return;
   auto item_of = [&](uint32_t r) {
-    LsItem it = {0, 0, -1, 0, max(1, steps), first + r * G};  // no step at all: one of zeros
+    LsItem it = {0, 0, -1, 0, max(1, steps), r < whole ? first + r * G : whole * G + last_tile};  // no step at all: one of zeros
     if (EPI == EPI_OUT && r >= rounds) {
       const uint32_t s = r - rounds;
       if (pl.parts != 0) {
-        const uint32_t q = first + s * G, part = q / pl.rest;
+        const uint32_t q = s < load1 ? first + s * G : load1 * G + last_part, part = q / pl.rest;
         it.tile = pl.full + q - part * pl.rest;
         it.k0 = (int)(part * pl.per);
         it.nk = (int)min(pl.per, pl.steps - part * pl.per);
