@@ -214,3 +214,19 @@ def test_captured_and_on_another_stream(gpu):
         got, clipped = norm.clone(), [t.clone() for t in out]
         assert torch.equal(got, ops.clip_grads(grads, 1.0, out=out))
         assert all(torch.equal(a, b) for a, b in zip(out, clipped))
+
+
+def test_more_than_2_31_elements(gpu):
+    from q38.hip import ops
+    n = 2 ** 31 + 12345
+    t = torch.zeros(n, dtype=torch.bfloat16, device=gpu)
+    spots = [(0, 100_000), (2 ** 31 - 50_000, 2 ** 31 + 12345)]
+    g = torch.Generator(device=gpu).manual_seed(1)
+    for a, b in spots:
+        t[a:b] = torch.randn(b - a, generator=g, device=gpu).to(torch.bfloat16)
+    before = [t[a:b].clone() for a, b in spots]
+    n64 = float(torch.cat([v.double() for v in before]).norm())
+    got = ops.clip_grads([t], 1.0)
+    assert abs(float(got) - n64) <= n64 * (U + 1e-12)
+    _check_scaled(before, [t[a:b] for a, b in spots], n64, 1.0)
+    assert not bool(t[200_000:2 ** 31 - 60_000].any())

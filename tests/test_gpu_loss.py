@@ -315,3 +315,36 @@ def test_close_to_torch(gpu):
     theirs.backward()
     for a, b in ((leaves[0], leaves[2]), (leaves[1], leaves[3])):
         assert float((a.grad - b.grad).norm() / b.grad.norm()) < 1e-5
+
+
+def test_offsets_past_32_bits(gpu):
+    """x, its copy and dx of more than 4 GiB. x is zero but for 3000 rows, at both ends and around element 2^31, so that dw
+    sums (and rounds) 3000 terms."""
+    from q38.hip import autograd
+    T, h, V = 2_200_000, 1024, 70
+    g = torch.Generator(device=gpu).manual_seed(3)
+    x = torch.zeros(T, h, dtype=torch.bfloat16, device=gpu)
+    for i in (0, 2 ** 31 // h - 500, T - 1000):
+        x[i:i + 1000] = torch.randn(1000, h, generator=g, device=gpu).to(torch.bfloat16)
+    w = (torch.randn(V, h, generator=g, device=gpu) * h ** -0.5).to(torch.bfloat16)
+    t = torch.randint(0, V, (T,), generator=g, device=gpu)
+    t[5] = t[T // 2] = t[T - 3] = -100  # a copy of x is made, and zeros are written
+    x.requires_grad_(True)
+    w.requires_grad_(True)
+    print("loss past 32 bits", flush=True)
+    loss = autograd.linear_cross_entropy(x, w, t, reduction="sum")
+    dx, dw = torch.autograd.grad(loss, (x, w))
+    x, w = x.detach(), w.detach()
+    v, total, size = 2.0 ** -8, 0.0, 0.0
+    want, bound = torch.zeros(V, h, dtype=torch.float64, device=gpu), torch.zeros(V, h, dtype=torch.float64, device=gpu)
+    for i in range(0, T, 100_000):
+        rows, _, s, p, dz, xd, wd, keep = _oracle(x[i:i + 100_000], w, t[i:i + 100_000])
+        total, size = total + float(rows.sum()), size + float((2 * dz + 420 * U).sum())
+        e = s.abs() * (v + 8 * U) + p * (2 * dz + 440 * U)[:, None]
+        want += s.t().contiguous() @ xd
+        bound += (e + 2 * (3000 + 20) * U * s.abs()).t().contiguous() @ xd.abs()
+        exact, b = s @ wd, (e + 2 * (V + 20) * U * s.abs()) @ wd.abs()
+        err = (dx[i:i + 100_000].double() - exact).abs()
+        assert bool((err <= b + v * (exact.abs() + b) + 1e-38).all()), i
+    assert abs(float(loss) - total) <= size + 2 * U * total
+    assert bool(((dw.double() - want).abs() <= bound + v * (want.abs() + bound)).all())

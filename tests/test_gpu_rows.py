@@ -222,3 +222,25 @@ def test_forward_mode_is_refused(gpu):
                   lambda: autograd.combine(fwad.make_dual(y, torch.ones_like(y)), w, plan)):
             with pytest.raises(Exception, match="jvp|forward mode"):
                 f()
+
+
+def test_offsets_past_32_bits(gpu):
+    """Rows of more than 4 GiB: copies there and the sums back, checked in pieces."""
+    from q38.hip import autograd
+    T, h, E, k = 450_000, 1024, 64, 5
+    g = torch.Generator(device=gpu).manual_seed(5)
+    x = torch.empty(T, h, dtype=torch.bfloat16, device=gpu)
+    for i in range(0, T, 50_000):
+        x[i:i + 50_000] = torch.randn(50_000, h, generator=g, device=gpu).to(torch.bfloat16)
+    idx = torch.topk(torch.rand(T, E, generator=g, device=gpu), k, dim=1).indices
+    w = torch.rand(T, k, generator=g, device=gpu).to(torch.bfloat16)
+    print("rows past 32 bits", flush=True)
+    rows, plan = autograd.dispatch(x, idx, E)
+    out = autograd.combine(rows, w, plan)
+    inv = plan.inv.view(T, k).long()
+    assert int(plan.counts.sum()) == T * k and bool((torch.sort(inv.reshape(-1)).values == torch.arange(T * k, device=gpu)).all())
+    for i in range(0, T, 50_000):
+        xd, wd = x[i:i + 50_000], w[i:i + 50_000].double()
+        assert torch.equal(rows[inv[i:i + 50_000]], xd[:, None].expand(-1, k, -1))
+        exact = xd.double() * wd.sum(1, keepdim=True)
+        _near(out[i:i + 50_000], exact, xd.double().abs() * wd.sum(1, keepdim=True), 10, f"out {i}")

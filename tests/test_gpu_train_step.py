@@ -291,3 +291,33 @@ def test_causal_lm_labels(gpu):
     assert abs(float(out.loss) - float(want)) <= 2 * 2.0 ** -8 * float(z.abs().max()) * 1.01 + 1e-5
     with pytest.raises(ValueError, match="labels"):
         model(input_ids=ids, labels=labels[:, 1:])
+
+
+def test_two_streams_at_once(gpu):
+    """Steps under way on two streams at the same time give the bits that they give alone."""
+    from q38.hip import ops
+    sets = [[a.requires_grad_(a.is_floating_point()) if isinstance(a, torch.Tensor) else a
+             for a in _params(torch.bfloat16, gpu, T=400 + 9 * s, seed=s)] for s in range(2)]
+
+    def run(args):
+        x, w_r, up, head, t, k = args
+        from q38.hip import autograd
+        logits, w, idx = autograd.router(x, w_r, k)
+        rows, plan = autograd.dispatch(x, idx, up.shape[0])
+        hidden = x + autograd.combine(rows, w, plan)
+        loss = autograd.linear_cross_entropy(hidden, head, t)
+        grads = torch.autograd.grad(loss, (x, w_r, head))
+        return [loss.detach(), ops.clip_grads(list(grads), 0.1), *grads]
+
+    alone = [run(a) for a in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sets]
+    got = [[], []]
+    for _ in range(4):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(run(sets[i]))
+    torch.cuda.synchronize()
+    for want, many in zip(alone, got):
+        for one in many:
+            assert all(torch.equal(a, b) for a, b in zip(want, one))
