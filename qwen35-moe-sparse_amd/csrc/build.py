@@ -30,7 +30,7 @@ FLAGS = [
 
 # Sources whose kernels issue MFMAs from inline asm: the compiler's hazard recognizer does not see
 # them, so their generated code is kept (-save-temps) and checked by mfma_operand_hazards.
-ASM_MFMA_SOURCES = ["q38moe_gemm4w.hip"]
+ASM_MFMA_SOURCES = ["q38moe_gemm4w.hip", "q38moe_loss.hip"]
 
 
 def mfma_operand_hazards(asm_text):
