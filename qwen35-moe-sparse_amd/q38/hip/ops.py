@@ -903,28 +903,35 @@ def linear_ce_backward(g, x, w, targets, lse, ignore_index=-100, row_scale=None,
 def _norm_args(tensors):
     """The tensors' device and, as C arrays, their addresses, sizes and dtypes. (Whole lists at a time: a loop over the
     tensors' attributes costs the host 1 us a tensor.)"""
+    try:
+        codes = [_DTYPES[t.dtype] for t in tensors]
+        indices = set(map(torch.Tensor.get_device, tensors))
+        if len(indices) == 1 and min(indices) >= 0 and all(map(torch.Tensor.is_contiguous, tensors)):
+            n = len(tensors)
+            return (tensors[0].device, (ctypes.c_void_p * n)(*map(torch.Tensor.data_ptr, tensors)),
+                    (ctypes.c_int64 * n)(*map(torch.Tensor.numel, tensors)), (ctypes.c_int32 * n)(*codes))
+    except (AttributeError, KeyError, NotImplementedError, RuntimeError, TypeError):
+        pass
+    raise _norm_refusal(tensors)
+
+
+def _norm_refusal(tensors):
     for t in tensors:
         if not isinstance(t, torch.Tensor):
-            raise TypeError(f"gradients must be bf16 or fp32 tensors, got {type(t)}")
-    dtypes = [t.dtype for t in tensors]
-    for dt in set(dtypes):
-        if dt not in _DTYPES:
-            raise TypeError(f"gradients must be bf16 or fp32 tensors, got {dt}")
-    for layout in {t.layout for t in tensors}:
-        if layout is not torch.strided:
-            raise TypeError(f"gradients must be dense, got {layout}")
-    devices = {t.device for t in tensors}
-    dev = tensors[0].device
-    if dev.type != "cuda" or len(devices) > 1:
-        if any(d.type != "cuda" for d in devices):
-            raise RuntimeError("gradients must be CUDA/HIP tensors")
-        raise RuntimeError(f"gradients must be on one device, got {sorted(map(str, devices))}")
-    if not all(map(torch.Tensor.is_contiguous, tensors)):
-        bad = next(t for t in tensors if not t.is_contiguous())
-        raise ValueError(f"gradients must be contiguous, got strides {bad.stride()} for {tuple(bad.shape)}")
-    n = len(tensors)
-    return (dev, (ctypes.c_void_p * n)(*map(torch.Tensor.data_ptr, tensors)),
-            (ctypes.c_int64 * n)(*map(torch.Tensor.numel, tensors)), (ctypes.c_int32 * n)(*map(_DTYPES.get, dtypes)))
+            return TypeError(f"gradients must be bf16 or fp32 tensors, got {type(t)}")
+        if t.dtype not in _DTYPES:
+            return TypeError(f"gradients must be bf16 or fp32 tensors, got {t.dtype}")
+        if t.layout is not torch.strided:
+            return TypeError(f"gradients must be dense, got {t.layout}")
+        if t.device.type != "cuda":
+            return RuntimeError("gradients must be CUDA/HIP tensors")
+    devices = {str(t.device) for t in tensors}
+    if len(devices) > 1:
+        return RuntimeError(f"gradients must be on one device, got {sorted(devices)}")
+    for t in tensors:
+        if not t.is_contiguous():
+            return ValueError(f"gradients must be contiguous, got strides {t.stride()} for {tuple(t.shape)}")
+    return RuntimeError("gradients must be plain tensors in memory")
 
 
 def _norm_code(norm_type):
@@ -1011,6 +1018,13 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
     return total
 
 
+@functools.lru_cache(maxsize=512)
+def _plan_ints(T, experts, k):
+    n = lib.q38moe_rows_plan_ints(T, experts, k)
+    check(min(n, 0), "q38moe_rows_plan_ints")
+    return n
+
+
 class RowsPlan:
     """Where the pairs of a routing idx [T,k] go: expert e's rows are starts[e] .. starts[e] + counts[e] - 1, row r is pair
     perm[r] (token perm[r] // k; only rows that are filled), pair p is row inv[p] (-1 for pairs routed outside
@@ -1021,8 +1035,7 @@ class RowsPlan:
     def __init__(self, topk_idx, experts):
         _need(topk_idx, "topk_idx", dtype=None, ndim=2)
         _idx_flag(topk_idx)
-        n = lib.q38moe_rows_plan_ints(*topk_idx.shape[:1], experts, topk_idx.shape[1])
-        check(min(n, 0), "q38moe_rows_plan_ints")
+        n = _plan_ints(topk_idx.shape[0], experts, topk_idx.shape[1])
         self.idx, self.experts, self.filled = topk_idx, experts, False
         self.buffer = torch.empty(n, dtype=torch.int32, device=topk_idx.device)
 
