@@ -1736,6 +1736,12 @@ int q38moe_dispatch_rows(const void* x, const void* topk_idx, int32_t idx_is_int
   const bool idx64 = idx_is_int64 != 0;
   hipStream_t st = static_cast<hipStream_t>(stream);
   (void)hipGetLastError();
+  if (q38::dispatch_is_small(T, k)) {
+    Q38_HIP(q38::launch_dispatch_small(x, topk_idx, idx64, plan, plan + L.starts(), plan + L.perm(), plan + L.inv(), dst, T,
+                                       h, E, k, dtype == Q38MOE_BF16, st),
+            "dispatch rows launch");
+    return Q38MOE_OK;
+  }
   if (T > 0) Q38_HIP(q38::launch_histogram(topk_idx, idx64, plan + L.hist(), T, E, k, st), "histogram launch");
   Q38_HIP(q38::launch_permute(topk_idx, idx64, plan + L.hist(), plan, plan + L.starts(), plan + L.perm(), plan + L.inv(),
                               nullptr, nullptr, q38::gemm_block_m(), 0, 0, T, E, k, st),

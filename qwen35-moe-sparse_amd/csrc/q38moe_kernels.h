@@ -211,6 +211,11 @@ hipError_t launch_qsa_attention(const void* q, const void* k, const void* v, con
 hipError_t launch_spread_rows(const void* src, const void* w, bool w_f32, const void* y, const void* idx, bool idx64,
                               int32_t* inv, const int32_t* starts, const int32_t* counts, void* dst, void* dw, int64_t T,
                               int h, int E, int k, bool bf16, hipStream_t st);
+// Dispatch in one launch, the whole plan included, for few pairs (dispatch_is_small).
+bool dispatch_is_small(int64_t T, int k);
+hipError_t launch_dispatch_small(const void* src, const void* idx, bool idx64, int32_t* counts, int32_t* starts,
+                                 int32_t* perm, int32_t* inv, void* dst, int64_t T, int h, int E, int k, bool bf16,
+                                 hipStream_t st);
 hipError_t launch_collect_rows(const void* src, const void* w, bool w_f32, const int32_t* inv, void* out, int64_t T, int h,
                                int k, bool bf16, hipStream_t st);
 

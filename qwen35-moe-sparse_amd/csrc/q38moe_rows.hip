@@ -22,6 +22,8 @@ namespace {
 template <typename E>
 constexpr int VEC = 16 / sizeof(E);  // elements of a 16-byte load
 
+constexpr int ROWS_SMALL = 4096;  // pairs of a dispatch in one launch
+
 template <typename E>
 __device__ __forceinline__ void unpack16(u32x4_t v, float (&f)[VEC<E>]) {
   if constexpr (std::is_same<E, float>::value) {
@@ -159,6 +161,84 @@ __global__ __launch_bounds__(256) void spread_kernel(const E* __restrict__ src, 
   }
 }
 
+// Dispatch of up to ROWS_SMALL pairs in one launch instead of three (histogram, permutation, spread): every block takes all
+// pairs' experts into LDS and counts them, and a wave finds its token's rows as starts[e] + the earlier pairs of the same expert, 64
+// at a time by ballots, which is the stable order of the permutation. Between them the blocks write the whole plan. 305 pairs take 5.4
+// us on the GPU and 9.5 with the host's part, in three launches 8.7 and 16; 2560 pairs 8.8 and 9.6, 10.1 and 16.5; at 4096 the ballots
+// cost as much as the launches (k = 2: 9.1 and 9.2 us on the GPU; k = 8: 11.9 and 10.4, but 11.6 and 16 with the host).
+template <typename E, typename IdxT, int KT>
+__global__ __launch_bounds__(256) void dispatch_small_kernel(const E* __restrict__ src, const IdxT* __restrict__ idx,
+                                                             int32_t* __restrict__ counts, int32_t* __restrict__ starts,
+                                                             int32_t* __restrict__ perm, int32_t* __restrict__ inv,
+                                                             E* __restrict__ dst, int64_t T, int h, int NE) {
+  constexpr int NONE = 255;
+  __shared__ uint8_t ids[ROWS_SMALL];
+  __shared__ int cnt[64];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int P = (int)T * KT;
+  if (threadIdx.x < 64) cnt[threadIdx.x] = 0;
+  __syncthreads();
+  for (int p = threadIdx.x; p < P; p += 256) {
+    const int64_t e = (int64_t)idx[p];
+    const bool ok = e >= 0 && e < NE;
+    ids[p] = ok ? (uint8_t)e : (uint8_t)NONE;
+    if (ok) atomicAdd(&cnt[e], 1);
+  }
+  __syncthreads();
+  const int c = cnt[lane];  // lane = expert; none beyond NE
+  int end = c;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int u = __shfl_up(end, o);
+    if (lane >= o) end += u;
+  }
+  const int start = end - c, filled = __shfl(end, 63);
+  if (blockIdx.x == 0 && wave == 0 && lane < NE) {
+    counts[lane] = c;
+    starts[lane] = start;
+  }
+  const int t = (int)blockIdx.x * 4 + wave;
+  if (t >= T) return;
+  int e[KT], row[KT];
+#pragma unroll
+  for (int j = 0; j < KT; ++j) {
+    e[j] = __builtin_amdgcn_readfirstlane((int)ids[t * KT + j]);
+    row[j] = 0;
+  }
+  int p0 = 0;
+  for (; p0 + 256 <= t * KT; p0 += 256) {  // all before the token's own pairs
+    int v[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) v[u] = ids[p0 + 64 * u + lane];
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+#pragma unroll
+      for (int j = 0; j < KT; ++j) row[j] += __popcll(ballot64(v[u] == e[j]));
+  }
+  for (; p0 < t * KT + KT; p0 += 64) {
+    const int p = p0 + lane, v = p < P ? (int)ids[p] : NONE;
+#pragma unroll
+    for (int j = 0; j < KT; ++j) row[j] += __popcll(ballot64(v == e[j] && p < t * KT + j));
+  }
+#pragma unroll
+  for (int j = 0; j < KT; ++j) {
+    row[j] = e[j] == NONE ? -1 : row[j] + __shfl(start, e[j] & 63);
+    row[j] = __builtin_amdgcn_readfirstlane(row[j]);
+    if (lane == 0) {
+      inv[t * KT + j] = row[j];
+      if (row[j] >= 0) perm[row[j]] = t * KT + j;
+    }
+  }
+  for (int k = lane * VEC<E>; k < h; k += 64 * VEC<E>) {
+    const u32x4_t v = ld16(src + (int64_t)t * h + k);
+#pragma unroll
+    for (int j = 0; j < KT; ++j) {
+      if (row[j] >= 0) st16(dst + (int64_t)row[j] * h + k, v);
+      if (t * KT + j >= filled) st16(dst + (int64_t)(t * KT + j) * h + k, (u32x4_t){0u, 0u, 0u, 0u});
+    }
+  }
+}
+
 template <typename E, int KT>
 __global__ __launch_bounds__(256) void collect_kernel(const E* __restrict__ src, const void* __restrict__ w, bool w_f32,
                                                       int32_t* __restrict__ inv, E* __restrict__ out, int64_t T, int h) {
@@ -218,6 +298,24 @@ hipError_t spread_k(const void* src, const void* w, bool w_f32, const void* y, c
   return hipGetLastError();
 }
 
+template <typename E, typename IdxT>
+hipError_t dispatch_small_k(const void* src, const void* idx, int32_t* counts, int32_t* starts, int32_t* perm, int32_t* inv,
+                            void* dst, int64_t T, int h, int NE, int k, hipStream_t st) {
+  const dim3 grid((unsigned)((T + 3) / 4));
+#define Q38_DISPATCH(KT)                                                                                          \
+  case KT:                                                                                                        \
+    hipLaunchKernelGGL((dispatch_small_kernel<E, IdxT, KT>), grid, dim3(256), 0, st, (const E*)src,               \
+                       (const IdxT*)idx, counts, starts, perm, inv, (E*)dst, T, h, NE);                           \
+    break;
+  switch (k) {
+    Q38_DISPATCH(1) Q38_DISPATCH(2) Q38_DISPATCH(3) Q38_DISPATCH(4) Q38_DISPATCH(5) Q38_DISPATCH(6) Q38_DISPATCH(7)
+    Q38_DISPATCH(8)
+    default: return hipErrorInvalidValue;
+  }
+#undef Q38_DISPATCH
+  return hipGetLastError();
+}
+
 template <typename E>
 hipError_t collect_k(const void* src, const void* w, bool w_f32, int32_t* inv, void* out, int64_t T, int h, int k,
                      hipStream_t st) {
@@ -252,6 +350,19 @@ hipError_t launch_spread_rows(const void* src, const void* w, bool w_f32, const 
   if (T == 0) return hipSuccess;
   return bf16 ? spread_any<uint16_t>(src, w, w_f32, y, idx, idx64, inv, starts, counts, dst, dw, T, h, E, k, st)
               : spread_any<float>(src, w, w_f32, y, idx, idx64, inv, starts, counts, dst, dw, T, h, E, k, st);
+}
+
+bool dispatch_is_small(int64_t T, int k) { return T > 0 && T * k <= ROWS_SMALL; }
+
+hipError_t launch_dispatch_small(const void* src, const void* idx, bool idx64, int32_t* counts, int32_t* starts,
+                                 int32_t* perm, int32_t* inv, void* dst, int64_t T, int h, int E, int k, bool bf16,
+                                 hipStream_t st) {
+  if (!dispatch_is_small(T, k)) return hipErrorInvalidValue;
+  if (bf16)
+    return idx64 ? dispatch_small_k<uint16_t, int64_t>(src, idx, counts, starts, perm, inv, dst, T, h, E, k, st)
+                 : dispatch_small_k<uint16_t, int32_t>(src, idx, counts, starts, perm, inv, dst, T, h, E, k, st);
+  return idx64 ? dispatch_small_k<float, int64_t>(src, idx, counts, starts, perm, inv, dst, T, h, E, k, st)
+               : dispatch_small_k<float, int32_t>(src, idx, counts, starts, perm, inv, dst, T, h, E, k, st);
 }
 
 hipError_t launch_collect_rows(const void* src, const void* w, bool w_f32, const int32_t* inv, void* out, int64_t T, int h,

@@ -51,6 +51,10 @@ def _near(got, exact, terms, sums, name):
     (1000, 64, 64, 6, 0.95),
     (77, 192, 5, 2, 1.0),      # no pair has a row
     (50, 2048, 7, 7, 0.2),
+    (512, 64, 16, 8, 0.1),     # the last pairs that one launch dispatches
+    (513, 64, 16, 8, 0.1),     # the first that three do
+    (1500, 320, 60, 5, 0.3),
+    (900, 192, 9, 7, 1.0),
 ])
 def test_rows(gpu, dtype, w_dtype, idx_dtype, T, h, E, k, dropped):
     from q38.hip import autograd
