@@ -105,6 +105,8 @@ def _grad_of(reduction, T, gen, dev):
     (700, 1344, 200, 0.0),
     (2048, 64, 130, 0.3),    # the last size with 16 rows to a finishing block
     (2049, 64, 130, 0.3),
+    (8192, 64, 70, 0.3),     # the last size whose list and copies are one launch
+    (8193, 64, 70, 0.3),
 ])
 def test_small(gpu, dtype, T, h, V, ignored):
     x, w, t, g = _data(T, h, V, dtype, gpu, ignored=ignored)
