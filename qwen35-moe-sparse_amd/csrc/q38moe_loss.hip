@@ -209,36 +209,72 @@ struct LsParams {
 //              read them at the same time (at most two items per workgroup);
 //   parts = 0: all steps of the rest evenly, `per` neighbouring ones to a workgroup, which reach over at most two tiles, a
 //              tile cut at most 17-fold.
-// In steps' time (1.7 us on 256 x 256): an item costs 3 beside its own; equal parts 4 and 16 for each round of partial sums,
-// even runs 42. Measured: 80 tiles of 256 steps 164 us in 3 parts and 197 in even runs, 136 tiles of 392 steps 500 and 425. Even runs
-// share no operand rows: bf16 tiles of 128 x 128 (`eager`), whose step takes half as long, then wait for memory, 2.5 times as long
+// In steps' time (1.7 us on 256 x 256): an item costs 3 beside its own; equal parts (up to 8) 4 and 16 for each round of partial
+// sums, even runs 42. 64 x 64 tiles have a sixteenth of the partial sums, 5 a round, but their joining waits once for each part, 1 in
+// bf16 and 0.5 in fp32, and may have 16 (dx of 16 x 256 x 10112 in fp32 with the rest of the call: 42 us, with 8 parts 50). Measured: 80 tiles of 256 steps 164 us in 3 parts and 197 in even runs, 136 tiles of 392 steps 500 and 425. Even runs
+// share no operand rows: bf16 tiles of 128 x 128, whose step takes half as long, then wait for memory, 2.5 times as long
 // (376 tiles of 158 steps: 257 us in even runs, 160 whole).
 struct LsPlan {
   uint32_t full, rest, steps, per, parts;
   uint32_t cost;  // of the last, partial round
 };
 constexpr uint32_t LS_CUTS = 16;
-__host__ __device__ inline LsPlan ls_plan(uint32_t tiles, uint32_t steps, uint32_t slots, bool eager) {
+
+// The time of `rest` tiles in about q equal parts each, and those.
+template <bool F32, int BM>
+__host__ __device__ inline uint32_t ls_parts(uint32_t rest, uint32_t steps, uint32_t slots, uint32_t q, uint32_t& per,
+                                             uint32_t& parts) {
+  per = (steps + q - 1) / q;
+  parts = (steps + per - 1) / per;
+  const uint32_t load = rest * parts;
+  const uint32_t join = BM == 64 ? 5 * load / slots + (F32 ? parts / 2 : parts) : 4 + 16 * load / slots;
+  return (load + slots - 1) / slots * (per + 3) + join;
+}
+template <int BM>
+__host__ __device__ inline bool ls_may(uint32_t rest, uint32_t steps, uint32_t slots, uint32_t q) {
+  return q <= (BM == 64 ? LS_CUTS : 8) && q <= steps && rest * q <= 2 * slots;
+}
+
+// The plan but for equal parts.
+template <bool F32, int BM>
+__host__ __device__ inline LsPlan ls_unparted(uint32_t tiles, uint32_t steps, uint32_t slots) {
   const uint32_t rest = tiles % slots;
-  LsPlan pl = {tiles, 0, steps, steps, 1, rest != 0 ? steps + 3 : 0};
-  if (rest == 0) return pl;
-  const uint64_t even = ((uint64_t)rest * steps + slots - 1) / slots;
-  const uint32_t least = (steps + LS_CUTS - 1) / LS_CUTS, run = even > least ? (uint32_t)even : least;
-  uint32_t best = steps + 3;
-  const uint32_t run_cost = (eager ? run * 5 / 2 : run) + 42;
-  if (run_cost < best) {
-    best = run_cost;
-    pl = LsPlan{tiles - rest, rest, steps, run, 0, best};
-  }
-  for (uint32_t q = 2; q <= 8 && q <= steps && rest * q <= 2 * slots; ++q) {
-    const uint32_t per = (steps + q - 1) / q, parts = (steps + per - 1) / per, load = rest * parts;
-    const uint32_t cost = (load + slots - 1) / slots * (per + 3) + 4 + 16 * load / slots;
-    if (cost < best) {
-      best = cost;
-      pl = LsPlan{tiles - rest, rest, steps, per, parts, best};
-    }
+  if (rest == 0) return LsPlan{tiles, 0, steps, steps, 1, 0};
+  const uint32_t even = (uint32_t)(((uint64_t)rest * steps + slots - 1) / slots);
+  const uint32_t least = (steps + LS_CUTS - 1) / LS_CUTS, run = even > least ? even : least;
+  const uint32_t run_cost = (!F32 && BM == 128 ? run * 5 / 2 : run) + 42;
+  if (run_cost < steps + 3) return LsPlan{tiles - rest, rest, steps, run, 0, run_cost};
+  return LsPlan{tiles, 0, steps, steps, 1, steps + 3};
+}
+
+template <bool F32, int BM>
+LsPlan ls_plan(uint32_t tiles, uint32_t steps, uint32_t slots) {
+  LsPlan pl = ls_unparted<F32, BM>(tiles, steps, slots);
+  const uint32_t rest = tiles % slots;
+  for (uint32_t q = 2; rest != 0 && ls_may<BM>(rest, steps, slots, q); ++q) {
+    uint32_t per, parts;
+    const uint32_t cost = ls_parts<F32, BM>(rest, steps, slots, q, per, parts);
+    if (cost < pl.cost) pl = LsPlan{tiles - rest, rest, steps, per, parts, cost};
   }
   return pl;
+}
+
+// The same by a wave, a lane for each q: one after another their divisions take 2 us a kernel and 4 with 16 of them (dx of 1 x 256
+// x 1000, a product and its joining: 21 and 27 us with the rest of the call, so 18.6).
+template <bool F32, int BM>
+__device__ __forceinline__ LsPlan ls_plan_wave(uint32_t tiles, uint32_t steps, uint32_t slots) {
+  const LsPlan pl = ls_unparted<F32, BM>(tiles, steps, slots);
+  const uint32_t rest = tiles % slots, q = 2 + (threadIdx.x & 15);
+  if (rest == 0 || steps < 2) return pl;
+  uint32_t per = 0, parts = 0, key = 0xffffffffu;
+  if (ls_may<BM>(rest, steps, slots, q)) key = ls_parts<F32, BM>(rest, steps, slots, q, per, parts) << 5 | q;  // < 2^26
+#pragma unroll
+  for (int o = 1; o < 16; o <<= 1) key = min(key, (uint32_t)__shfl_xor((int)key, o));
+  key = uniform(key);
+  if ((key >> 5) >= pl.cost) return pl;
+  const int at = (int)(key & 31) - 2;
+  return LsPlan{tiles - rest, rest, steps, uniform((uint32_t)__shfl((int)per, at)), uniform((uint32_t)__shfl((int)parts, at)),
+                key >> 5};
 }
 
 // Workgroups that share a CU.
@@ -270,7 +306,7 @@ __global__ __launch_bounds__(256, ls_per_cu(BM, EPI)) void ls_gemm_kernel(const 
   using OB = Operand<F32, BN, LB>;
   constexpr int MB = BM / 64, NB = BN / 64;  // 32x32 blocks of a wave
   constexpr int SLOT = (BM + BN) * 128;
-  constexpr int NS = BM != 64 ? 2 : EPI == EPI_OUT ? 8 : 4;  // steps in LDS: few tiles wait for memory, many for the matrix units
+  constexpr int NS = BM != 64 ? 2 : ls_per_cu(BM, EPI) == 1 ? 8 : 4;  // steps in LDS: few tiles wait for memory, many for the matrix units
   constexpr int BK = OA::BK, ESZ = OA::ESZ;
   __shared__ __align__(1024) uint8_t lds[NS * SLOT];
   // Staging of bf16 outputs, 32 rows of out by BM / 2 columns per wave (beside the slots: copies for the next item run meanwhile).
@@ -301,7 +337,7 @@ __global__ __launch_bounds__(256, ls_per_cu(BM, EPI)) void ls_gemm_kernel(const 
   // Work items of neighbouring blocks on an XCD are neighbouring tiles: 8 tiles of M by as many of N as it has room for.
   const uint32_t G = gridDim.x;
   const uint32_t first = (G & 7) == 0 ? (blockIdx.x & 7) * (G >> 3) + (blockIdx.x >> 3) : blockIdx.x;
-  const LsPlan pl = EPI == EPI_OUT ? ls_plan(tiles, (uint32_t)steps, p.slots, !F32 && BM == 128)
+  const LsPlan pl = EPI == EPI_OUT ? ls_plan_wave<F32, BM>(tiles, (uint32_t)steps, p.slots)
                                    : LsPlan{tiles, 0, (uint32_t)steps, (uint32_t)steps, 1, 0};
   // Of n items that are fewer than the blocks: this block's, or n. Each XCD has an eighth, neighbours, for its first blocks (dealt
   // like whole rounds, they would all go to the first XCDs: dW of 1777 x 1024 x 10112 with the rest of the call 106 us, so 119; the
@@ -867,7 +903,7 @@ __global__ __launch_bounds__(256) void ls_join_kernel(const LsParams p) {
   const int64_t cnt = (int64_t)load_uniform(p.count);
   const int64_t N = TOK_K ? p.N : cnt, K = TOK_K ? cnt : p.K;
   const uint32_t ntm = (uint32_t)((p.M + BM - 1) / BM), ntn = (uint32_t)((N + BN - 1) / BN);
-  const LsPlan pl = ls_plan(ntm * ntn, (uint32_t)((K + BK - 1) / BK), p.slots, sizeof(E) == 2 && BM == 128);
+  const LsPlan pl = ls_plan_wave<sizeof(E) == 4, BM>(ntm * ntn, (uint32_t)((K + BK - 1) / BK), p.slots);
   float scale = 1.0f;
   if (p.last && p.g_scale != nullptr) scale *= *p.g_scale;
   if (p.last && p.r_scale != nullptr) scale *= *p.r_scale;
@@ -947,10 +983,11 @@ int tile_z(int64_t M, int64_t N, bool f32) {
   return 7 * ceil_div(ceil_div(M, 256) * ceil_div(N, 256), cus) <= 4 * ceil_div(n128, 2 * cus) ? 256 : 128;
 }
 
-// A product's time over K that may be split, in steps of its tiles.
-uint64_t ls_cost(int64_t M, int64_t N, int64_t steps, int b) {
-  const uint32_t tiles = (uint32_t)(ceil_div(M, b) * ceil_div(N, b)), slots = ls_slots(b, EPI_OUT);
-  return (uint64_t)(tiles / slots) * (uint64_t)(steps + 3) + ls_plan(tiles, (uint32_t)steps, slots, b == 128).cost;
+// A bf16 product's time over K that may be split, in steps of its tiles.
+template <int B>
+uint64_t ls_cost(int64_t M, int64_t N, int64_t steps) {
+  const uint32_t tiles = (uint32_t)(ceil_div(M, B) * ceil_div(N, B)), slots = ls_slots(B, EPI_OUT);
+  return (uint64_t)(tiles / slots) * (uint64_t)(steps + 3) + ls_plan<false, B>(tiles, (uint32_t)steps, slots).cost;
 }
 
 // Of the gradients' products, whose tiles can be split over K. 64 (with eight steps in LDS) for few tiles of 128, or for less than
@@ -962,7 +999,7 @@ int tile_k(int64_t M, int64_t N, int64_t steps, bool f32) {
   const int64_t cus = device_cus(), n128 = ceil_div(M, 128) * ceil_div(N, 128);
   if (f32) return 8 * n128 <= cus || (n128 < cus && n128 * steps < 16 * cus) ? 64 : 128;
   if (8 * n128 < cus || (n128 < cus && n128 * steps < 12 * cus)) return 64;
-  return 8 * ls_cost(M, N, steps, 256) <= 5 * ls_cost(M, N, steps, 128) ? 256 : 128;
+  return 8 * ls_cost<256>(M, N, steps) <= 5 * ls_cost<128>(M, N, steps) ? 256 : 128;
 }
 
 int ls_finish_rows(int64_t T) { return T <= 2048 ? 16 : 64; }
