@@ -973,12 +973,12 @@ hipError_t ls_gemm(LsParams p, hipStream_t st) {
 // all (61 x 1024 x 10112 forward and dx: 15.6 and 36 us, with 128 18.5 and 42; 128 tokens 17.1 and 38, 18.5 and 42; 2 rounds, 200
 // tokens: 25.5 and 51, 18.8 and 47). Else a round of 256 x 256 tiles takes 30 us at h = 1024 and one of 128 x 128, two to a CU, 17
 // (16384 x 1024 x 10112: 302 and 350 us; 1777 tokens: 60 and 51; 300: 30 and 17). fp32 multiplies at a sixteenth of the rate, so
-// that a large tile's reuse is worth nothing, and the work on the busiest CU decides: 64 where it gets fewer than three times as
-// many of those as of 128 (of 64 tokens the larger tile is half empty: 61 x 2048 x 50021 forward 158 and 247 us, 100 x 1024 x
-// 10112 46 and 60; 200 tokens, three for one, 80 and 74; 600, seven for two, 155 and 134).
+// that a large tile's reuse is worth nothing, and the work on the busiest CU decides: 64 where it gets at most three times as many of
+// those as of 128 (of 64 tokens the larger tile is half empty: 61 x 2048 x 50021 forward 155 and 244 us; 100 x 1024 x 10112 45 and 71;
+// three for one, 200 tokens, 69 and 72, 2600 x 512 x 2000 67 and 72; seven for two, 700 tokens, 137 and 129).
 int tile_z(int64_t M, int64_t N, bool f32) {
   const int64_t cus = device_cus(), n64 = ceil_div(M, 64) * ceil_div(N, 64), n128 = ceil_div(M, 128) * ceil_div(N, 128);
-  if (f32) return ceil_div(n64, cus) < 3 * ceil_div(n128, cus) ? 64 : 128;
+  if (f32) return ceil_div(n64, cus) <= 3 * ceil_div(n128, cus) ? 64 : 128;
   if (n64 <= 2 * cus) return 64;
   return 7 * ceil_div(ceil_div(M, 256) * ceil_div(N, 256), cus) <= 4 * ceil_div(n128, 2 * cus) ? 256 : 128;
 }
