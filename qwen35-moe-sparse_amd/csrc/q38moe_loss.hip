@@ -987,18 +987,20 @@ int tile_z(int64_t M, int64_t N, bool f32) {
 template <int B>
 uint64_t ls_cost(int64_t M, int64_t N, int64_t steps) {
   const uint32_t tiles = (uint32_t)(ceil_div(M, B) * ceil_div(N, B)), slots = ls_slots(B, EPI_OUT);
-  return (uint64_t)(tiles / slots) * (uint64_t)(steps + 3) + ls_plan<false, B>(tiles, (uint32_t)steps, slots).cost;
+  return (uint64_t)(tiles / slots) * (uint64_t)(steps + 3) + ls_plan<false, B>(tiles, (uint32_t)steps, slots).cost +
+         (B == 256 ? 2 * ((tiles + slots - 1) / slots) : 0);  // its longer epilogue
 }
 
-// Of the gradients' products, whose tiles can be split over K. 64 (with eight steps in LDS) for few tiles of 128, or for less than
-// every CU's and little K (dx of 61 x 1024 x 10112: 37 and 49 us with the rest of the call, of 600 tokens 88 and 63, of 400 x
-// 1024 x 30000, 32 tiles, 173 and 116; dw of 2600 x 512 x 2000 39 and 47). Else bf16 takes 128 or 256 by the time that the plan
-// gives either, a step of 256 being worth 1.6 (two of 128 to a CU): dx of 1280 x 1024 x 10112 88 and 100 us, of 1536 x 2048 x
-// 50021 762 and 648; dw of 6000 x 1024 x 10112 290 and 321, of 1536 x 2048 x 50021 727 and 667. fp32 has no use for 256.
+// Of the gradients' products, whose tiles can be split over K. 64 (with eight steps in LDS) for few tiles of 128, or for at most one
+// per two CUs and little K (dx of 61 x 1024 x 10112: 37 and 49 us with the rest of the call; of 400 x 1024 x 30000, 32 tiles, 173
+// and 116, in fp32 of 400 x 1024 x 10112 224 and 192; dw of 2600 x 512 x 2000 39 and 47, of 1500 x 1024 x 2000, 128 tiles of 24
+// steps, 42 and 47, of 700 x 256 x 10112, 158 tiles, 35 and 28). Else bf16 takes 128 or 256 by the time that the plan gives either, a
+// step of 256 being worth 1.6 (two of 128 to a CU): dx of 1280 x 1024 x 10112 88 and 100 us, of 1536 x 2048 x 50021 762 and 648; dw of
+// 100 x 1024 x 10112 28 and 30, of 6000 x 1024 x 10112 290 and 321, of 1536 x 2048 x 50021 727 and 667. fp32 has no use for 256.
 int tile_k(int64_t M, int64_t N, int64_t steps, bool f32) {
   const int64_t cus = device_cus(), n128 = ceil_div(M, 128) * ceil_div(N, 128);
-  if (f32) return 8 * n128 <= cus || (n128 < cus && n128 * steps < 16 * cus) ? 64 : 128;
-  if (8 * n128 < cus || (n128 < cus && n128 * steps < 12 * cus)) return 64;
+  if (8 * n128 < cus || (2 * n128 <= cus && n128 * steps <= (f32 ? 16 : 12) * cus)) return 64;
+  if (f32) return 128;
   return 8 * ls_cost<256>(M, N, steps) <= 5 * ls_cost<128>(M, N, steps) ? 256 : 128;
 }
 
