@@ -350,3 +350,34 @@ def test_offsets_past_32_bits(gpu):
         assert bool((err <= b + v * (exact.abs() + b) + 1e-38).all()), i
     assert abs(float(loss) - total) <= size + 2 * U * total
     assert bool(((dw.double() - want).abs() <= bound + v * (want.abs() + bound)).all())
+
+
+@pytest.mark.parametrize("dtype,T,h,V,ignored,reduction", [
+    # Sides of the gradients' tiles and ways of their last, partial round, on 256 CUs.
+    (torch.bfloat16, 300, 1024, 8200, 0.0, "mean"),     # dw: 256, whole
+    (torch.bfloat16, 4099, 2048, 300, 0.2, "mean"),     # dx: 256, whole
+    (torch.bfloat16, 1500, 2048, 8200, 0.1, "sum"),     # dx: 256, equal parts
+    (torch.bfloat16, 5000, 2048, 2049, 0.0, "none"),    # dw: 256, equal parts
+    (torch.bfloat16, 3000, 2048, 20001, 0.0, "mean"),   # dx: 256, even runs
+    (torch.bfloat16, 12000, 1024, 10112, 0.0, "mean"),  # dw: 256, even runs
+    (torch.bfloat16, 16400, 256, 8200, 0.1, "mean"),    # dx: 256, equal parts, two pieces
+    (torch.bfloat16, 3000, 512, 50021, 0.0, "mean"),    # dw: 256, whole, two pieces
+    (torch.bfloat16, 16400, 64, 300, 0.0, "mean"),      # dx: 128, whole
+    (torch.bfloat16, 12000, 64, 2049, 0.3, "none"),     # dx: 128, equal parts
+    (torch.bfloat16, 20000, 256, 8200, 0.0, "sum"),     # dx: 128, whole, two pieces
+    (torch.bfloat16, 6500, 64, 4100, 0.0, "mean"),      # dw: 128, equal parts
+    (torch.bfloat16, 2100, 128, 50021, 0.0, "mean"),    # dx: 64, even runs
+    (torch.bfloat16, 3000, 64, 50021, 0.1, "mean"),     # dx: 64, equal parts, two pieces
+    (torch.float32, 2100, 128, 30011, 0.0, "mean"),     # dx: 64, even runs
+    (torch.float32, 1500, 64, 50021, 0.0, "none"),      # dx: 64, equal parts, two pieces
+    (torch.float32, 16400, 128, 8200, 0.1, "mean"),     # dw: 64, even runs, two pieces
+    (torch.float32, 16400, 64, 300, 0.0, "mean"),       # dx: 128, whole
+    (torch.float32, 1000, 512, 20001, 0.0, "mean"),     # dx: 128, even runs
+    (torch.float32, 4099, 64, 30011, 0.1, "sum"),       # dx: 128, even runs, two pieces
+    (torch.float32, 16400, 512, 1000, 0.0, "mean"),     # dw: 128, even runs
+    (torch.float32, 300, 64, 20001, 0.0, "mean"),       # dw: 128, whole
+])
+def test_plans(gpu, dtype, T, h, V, ignored, reduction):
+    x, w, t, g = _data(T, h, V, dtype, gpu, ignored=ignored)
+    print(f"loss T={T} h={h} V={V} {dtype} {reduction}", flush=True)
+    _check(x, w, t, reduction, _grad_of(reduction, T, g, gpu))
