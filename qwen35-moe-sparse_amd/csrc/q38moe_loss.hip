@@ -24,12 +24,12 @@
 // tokens (or vocabulary rows) are the lanes of the accumulators and the reduced or stored dimension their registers, so the
 // softmax's maxima and sums are in-lane but for one exchange.
 //
-// What bounds it. The matrix units need 2051 clocks for a step of a 256 x 256 tile. With all CUs at work on random bf16 data the
-// chip lowers its clock to 1.7 - 1.9 GHz: MFMAs alone take 1.09 us a step, with their LDS reads 1.23, with the copies to
-// LDS out of the L2 1.33 (all zeros: 0.94, 0.96, 1.04), and with a stream of its own per CU 1.94; this kernel, whose
-// tiles share the streams eight by four, takes 1.7. 16384 x 1024 x 10112: z 302 us (1120 TFLOP/s), s 2 x 168, dx 2 x 158, dW
-// 2 x 165. 4099 x 2048 x 50021: z 700 us (1190), s 2 x 391, dx 2 x 426, dW 2 x 410. Few tokens are bound by the latency of W's
-// way into LDS: 61 x 1024 x 10112 z 10 us for 20.7 MB.
+// What bounds it. The matrix units need 2051 clocks for a step of a 256 x 256 tile. With all CUs at work on random bf16
+// data the chip lowers its clock to 1.7 - 1.9 GHz: MFMAs alone take 1.09 us a step, with their LDS reads 1.23, with the
+// copies to LDS out of the L2 1.33 (all zeros: 0.94, 0.96, 1.04), and with a stream of its own per CU 1.94; this kernel,
+// whose tiles share the streams eight by four, takes 1.7. 16384 x 1024 x 10112: z 302 us (1120 TFLOP/s), s 2 x 168, dx 2 x
+// 158, dW 2 x 165. 4099 x 2048 x 50021: z 700 us (1190), s 2 x 391, dx 2 x 426, dW 2 x 410. Few tokens are bound by the
+// latency of W's way into LDS: 61 x 1024 x 10112 z 10 us for 20.7 MB.
 #include "q38moe_common.h"
 #include "q38moe_kernels.h"
 
@@ -45,16 +45,18 @@ typedef short ls_i16x4_t __attribute__((ext_vector_type(4)));
 
 __device__ __forceinline__ uint32_t uniform(uint32_t v) { return __builtin_amdgcn_readfirstlane(v); }
 
-// 16 bytes per lane from p + voff + soff to LDS at lds + 16 lane, zeros where voff + soff reaches `bytes` (raw buffer, no format).
+// 16 bytes per lane from p + voff + soff to LDS at lds + 16 lane, zeros where voff + soff reaches `bytes` (raw buffer, no
+// format).
 __device__ __forceinline__ void ls_dma(const uint8_t* p, int64_t bytes, uint32_t voff, uint32_t soff, uint32_t lds) {
   const uint64_t a = (uint64_t)(uintptr_t)p;
   const uint32_t n = bytes <= 0 ? 0u : (bytes >= 0xffffffffll ? 0xffffffffu : (uint32_t)bytes);
   const u32x4_t r = {uniform((uint32_t)a), uniform((uint32_t)(a >> 32) & 0xffffu), uniform(n), 0x00020000u};
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(lds), "v"(voff), "s"(r), "s"(soff) : "memory", "m0");
 }
-// 16 bytes to p + off (p uniform), through the XCD's L2 (scope sc1): what a kernel leaves there has to be written back before the
-// next one starts. For whole lines: s of 1024 x 1024 x 10112 36 -> 34 us, of 1024 x 1024 x 5056 21.3 -> 19.6, dW 47 -> 44.8; fp32, whose
-// lanes store parts of lines, 43.6 -> 47. Past it (non-temporal) s is not found by its readers either (dx 32.7 -> 41 us).
+// 16 bytes to p + off (p uniform), through the XCD's L2 (scope sc1): what a kernel leaves there has to be written back
+// before the next one starts. For whole lines: s of 1024 x 1024 x 10112 36 -> 34 us, of 1024 x 1024 x 5056 21.3 -> 19.6, dW
+// 47 -> 44.8; fp32, whose lanes store parts of lines, 43.6 -> 47. Past it (non-temporal) s is not found by its readers
+// either (dx 32.7 -> 41 us).
 __device__ __forceinline__ void ls_store_through(void* p, uint32_t off, u32x4_t v) {
   const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(p, (short)0, -1, 0x00020000);
   __builtin_amdgcn_raw_buffer_store_b128(v, r, (int)off, 0, 16);
@@ -139,7 +141,8 @@ __device__ __forceinline__ void ls_mfma(f32x16_t& acc, u32x4_t a, u32x4_t b) {
     asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+a"(acc) : "v"(a), "v"(b));
   }
 }
-// acc = 0 by the matrix unit, which has nothing else to do between two tiles (16 VALU writes would cost the epilogue their time).
+// acc = 0 by the matrix unit, which has nothing else to do between two tiles (16 VALU writes would cost the epilogue their
+// time).
 __device__ __forceinline__ void ls_zero(f32x16_t& acc) {
   const u32x4_t z = {0u, 0u, 0u, 0u};
   asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %1, %1, 0" : "+a"(acc) : "v"(z));
@@ -203,17 +206,18 @@ struct LsParams {
   uint32_t slots;        // workgroups that run at once
 };
 
-// How a product's tiles are dealt to `slots` workgroups: whole rounds of them take their tile over all of K. The `rest` of a
-// last, partial round is split over K, where that pays, and the partial sums are joined afterwards, in one of two ways:
+// How a product's tiles are dealt to `slots` workgroups: whole rounds of them take their tile over all of K. The `rest` of
+// a last, partial round is split over K, where that pays, and the partial sums are joined afterwards, in one of two ways:
 //   parts > 0: every tile into `parts` runs of `per` steps, run by run, so that workgroups that share rows of the operands
 //              read them at the same time (at most two items per workgroup);
 //   parts = 0: all steps of the rest evenly, `per` neighbouring ones to a workgroup, which reach over at most two tiles, a
 //              tile cut at most 17-fold.
-// In steps' time (1.7 us on 256 x 256): an item costs 3 beside its own; equal parts (up to 8) 4 and 16 for each round of partial
-// sums, even runs 42. 64 x 64 tiles have a sixteenth of the partial sums, 5 a round, but their joining waits once for each part, 1 in
-// bf16 and 0.5 in fp32, and may have 16 (dx of 16 x 256 x 10112 in fp32 with the rest of the call: 42 us, with 8 parts 50). Measured: 80 tiles of 256 steps 164 us in 3 parts and 197 in even runs, 136 tiles of 392 steps 500 and 425. Even runs
-// share no operand rows: bf16 tiles of 128 x 128, whose step takes half as long, then wait for memory, 2.5 times as long
-// (376 tiles of 158 steps: 257 us in even runs, 160 whole).
+// In steps' time (1.7 us on 256 x 256): an item costs 3 beside its own; equal parts (up to 8) 4 and 16 for each round of
+// partial sums, even runs 42. 64 x 64 tiles have a sixteenth of the partial sums, 5 a round, but their joining waits once
+// for each part, 1 in bf16 and 0.5 in fp32, and may have 16 (dx of 16 x 256 x 10112 in fp32 with the rest of the call: 42
+// us, with 8 parts 50). Measured: 80 tiles of 256 steps 164 us in 3 parts and 197 in even runs, 136 tiles of 392 steps 500
+// and 425. Even runs share no operand rows: bf16 tiles of 128 x 128, whose step takes half as long, then wait for memory,
+// 2.5 times as long (376 tiles of 158 steps: 257 us in even runs, 160 whole).
 struct LsPlan {
   uint32_t full, rest, steps, per, parts;
   uint32_t cost;  // of the last, partial round
@@ -259,8 +263,8 @@ LsPlan ls_plan(uint32_t tiles, uint32_t steps, uint32_t slots) {
   return pl;
 }
 
-// The same by a wave, a lane for each q: one after another their divisions take 2 us a kernel and 4 with 16 of them (dx of 1 x 256
-// x 1000, a product and its joining: 21 and 27 us with the rest of the call, so 18.6).
+// The same by a wave, a lane for each q: one after another their divisions take 2 us a kernel and 4 with 16 of them (dx of
+// 1 x 256 x 1000, a product and its joining: 21 and 27 us with the rest of the call, so 18.6).
 template <bool F32, int BM>
 __device__ __forceinline__ LsPlan ls_plan_wave(uint32_t tiles, uint32_t steps, uint32_t slots) {
   const LsPlan pl = ls_unparted<F32, BM>(tiles, steps, slots);
@@ -309,7 +313,8 @@ __global__ __launch_bounds__(256, ls_per_cu(BM, EPI)) void ls_gemm_kernel(const 
   constexpr int NS = BM != 64 ? 2 : ls_per_cu(BM, EPI) == 1 ? 8 : 4;  // steps in LDS: few tiles wait for memory, many for the matrix units
   constexpr int BK = OA::BK, ESZ = OA::ESZ;
   __shared__ __align__(1024) uint8_t lds[NS * SLOT];
-  // Staging of bf16 outputs, 32 rows of out by BM / 2 columns per wave (beside the slots: copies for the next item run meanwhile).
+  // Staging of bf16 outputs, 32 rows of out by BM / 2 columns per wave (beside the slots: copies for the next item run
+  // meanwhile).
   constexpr bool STAGED = !F32 && (EPI == EPI_S || EPI == EPI_OUT);
   __shared__ __align__(1024) uint8_t stage[STAGED ? 4 * 32 * BM : 16];
   constexpr bool TO_ROWS = EPI == EPI_OUT && LB == KC;  // dx: rows of out through `rows`
@@ -339,9 +344,9 @@ __global__ __launch_bounds__(256, ls_per_cu(BM, EPI)) void ls_gemm_kernel(const 
   const uint32_t first = (G & 7) == 0 ? (blockIdx.x & 7) * (G >> 3) + (blockIdx.x >> 3) : blockIdx.x;
   const LsPlan pl = EPI == EPI_OUT ? ls_plan_wave<F32, BM>(tiles, (uint32_t)steps, p.slots)
                                    : LsPlan{tiles, 0, (uint32_t)steps, (uint32_t)steps, 1, 0};
-  // Of n items that are fewer than the blocks: this block's, or n. Each XCD has an eighth, neighbours, for its first blocks (dealt
-  // like whole rounds, they would all go to the first XCDs: dW of 1777 x 1024 x 10112 with the rest of the call 106 us, so 119; the
-  // fp32 forward of 1024 x 512 x 10112 106 and 134).
+  // Of n items that are fewer than the blocks: this block's, or n. Each XCD has an eighth, neighbours, for its first blocks
+  // (dealt like whole rounds, they would all go to the first XCDs: dW of 1777 x 1024 x 10112 with the rest of the call 106
+  // us, so 119; the fp32 forward of 1024 x 512 x 10112 106 and 134).
   auto partial = [&](uint32_t n) -> uint32_t {
     if ((G & 7) != 0) return min((uint32_t)blockIdx.x, n);
     const uint32_t share = (n + 7) >> 3, i = blockIdx.x >> 3, at = (blockIdx.x & 7) * share + i;
@@ -473,8 +478,9 @@ __global__ __launch_bounds__(256, ls_per_cu(BM, EPI)) void ls_gemm_kernel(const 
   LsItem it = item_of(0);
   uint32_t item = 0;
   int slot = 0;
-  // What a tile's tokens bring to its epilogue: the target, lse and gradient, or the row of out; lane l holds token 32 j + l % 32's.
-  // Read at the tile's start: in the epilogue each read would wait for memory, and for the copies under way before it.
+  // What a tile's tokens bring to its epilogue: the target, lse and gradient, or the row of out; lane l holds token 32 j +
+  // l % 32's. Read at the tile's start: in the epilogue each read would wait for memory, and for the copies under way
+  // before it.
   int32_t tk[NB];
   float tl[NB], tg[NB];
   auto tokens = [&]() {
@@ -527,8 +533,8 @@ __global__ __launch_bounds__(256, ls_per_cu(BM, EPI)) void ls_gemm_kernel(const 
       quarter(1, base, 2, 0, 0, slot);
       quarter(0, base, 3, 0, 0, slot);
       advance();
-      // This wave's copies of the next step have landed (those of the NS - 2 positions behind it may be under way), its reads of
-      // this slot are done, and so are the others'.
+      // This wave's copies of the next step have landed (those of the NS - 2 positions behind it may be under way), its
+      // reads of this slot are done, and so are the others'.
       asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NS - 2) * NC) : "memory");
       ls_barrier();
       if constexpr (NS == 2) {  // the tokens' reads have landed with the copies: no wait for them later
@@ -594,7 +600,8 @@ __global__ __launch_bounds__(256, ls_per_cu(BM, EPI)) void ls_gemm_kernel(const 
             if (p.g_row != nullptr) v *= g;
             if (mleft < BM / 2) ls_mask(v, mleft - 4 * lh - 32 * i, 0.0f);
           } else {
-            // The accumulators' own order: block (i, j) of wave w at 1024 ((w MB + i) NB + j), its quarters 256 apart, 4 per lane.
+            // The accumulators' own order: block (i, j) of wave w at 1024 ((w MB + i) NB + j), its quarters 256 apart, 4
+            // per lane.
             const int64_t at = (((int64_t)wave * MB + i) * NB + j) * 1024 + 4 * lane;
             if (it.part < 0 && !p.first) {
               const float* a = p.acc + (int64_t)it.tile * (BM * BN) + at;
@@ -681,8 +688,8 @@ struct LsList {
 };
 constexpr int LS_RUNS = 8, LS_LIST = LS_RUNS * 1024;  // rows that a block of 1024 lists at a time, in runs of 1024
 
-// Places of rows t0 .. t0 + LS_LIST - 1, of which `kept` before them count, by ballots and a scan of the waves' counts: place(t, i, v) for
-// each, i its place in the list and v its target. Returns how many of them count.
+// Places of rows t0 .. t0 + LS_LIST - 1, of which `kept` before them count, by ballots and a scan of the waves' counts:
+// place(t, i, v) for each, i its place in the list and v its target. Returns how many of them count.
 template <typename IdxT, typename F>
 __device__ __forceinline__ int ls_places(const IdxT* targets, int64_t ignore, int64_t T, int64_t t0, int64_t kept, int* sums,
                                          F place) {
@@ -733,7 +740,7 @@ __device__ __forceinline__ void ls_put(const LsList& l, int64_t t, int64_t i, in
   if (l.g != nullptr) l.g_c[i] = l.g[t];
 }
 
-// The list by one block (16384 rows: 4.5 us, 14.5 with 1024 rows at a time).
+// The list by one block (16384 rows: 4.5 us with the targets in the caches, 9 without; with 1024 rows at a time 14.5).
 template <typename IdxT>
 __global__ __launch_bounds__(1024) void ls_rows_kernel(const IdxT* __restrict__ targets, int64_t ignore, int64_t T, int V,
                                                        LsList l) {
@@ -753,9 +760,9 @@ __device__ __forceinline__ void ls_copy_row(const uint8_t* x, uint8_t* xc, uint8
   }
 }
 
-// Up to LS_LIST rows: the list and ls_gather_kernel's copies in one launch. Every block makes the list, the first one stores it,
-// and each copies the 16 rows of its places: 2 us a call less than two launches at 61 to 4096 rows (1777 rows, 40 % ignored: 5
-// and 7.5 with the gap between), 0.5 to 1 at 8192.
+// Up to LS_LIST rows: the list and ls_gather_kernel's copies in one launch. Every block makes the list, the first one
+// stores it, and each copies the 16 rows of its places: 2 us a call less than two launches at 61 to 4096 rows (1777 rows,
+// 40 % ignored: 5 and 7.5 with the gap between), 0.5 to 1 at 8192.
 template <typename IdxT>
 __global__ __launch_bounds__(1024) void ls_list_kernel(const IdxT* __restrict__ targets, int64_t ignore, int64_t T, int V,
                                                        LsList l, const uint8_t* __restrict__ x, uint8_t* __restrict__ xc,
@@ -785,12 +792,12 @@ __global__ __launch_bounds__(256) void ls_gather_kernel(const uint8_t* __restric
   ls_copy_row(x, xc, zero, i, (int64_t)rows[i], i < n, bytes);
 }
 
-// lse and loss of R rows per block from their partial maxima and sums, which its 1024 / R groups of lanes share; rows that do not
-// count get loss 0. Few rows wait for the groups' loads, many for the blocks' sums to reach the last one: 16 rows to a block up
-// to 2048 rows, else 64 (61 rows of 316 entries 3.8 and 5.7 us; 1777 7.2 and 7.4; with the mean of 4099 13.9 and 10.8, of 16384 27 and
-// 10). Rows are those of the list, or with `raw` the call's own. Then *reduced = the sum of all losses (mean:
-// over the rows that count; 0 where none does), *row_scale = the factor of every row's gradient: by the block that is done
-// last, from the blocks' sums in their order (*done is 0 before and after).
+// lse and loss of R rows per block from their partial maxima and sums, which its 1024 / R groups of lanes share; rows that
+// do not count get loss 0. Few rows wait for the groups' loads, many for the blocks' sums to reach the last one: 16 rows to
+// a block up to 2048 rows, else 64 (61 rows of 316 entries 3.8 and 5.7 us; 1777 7.2 and 7.4; with the mean of 4099 13.9 and
+// 10.8, of 16384 27 and 10). Rows are those of the list, or with `raw` the call's own. Then *reduced = the sum of all
+// losses (mean: over the rows that count; 0 where none does), *row_scale = the factor of every row's gradient: by the block
+// that is done last, from the blocks' sums in their order (*done is 0 before and after).
 template <int R>
 __global__ __launch_bounds__(1024) void ls_finish_kernel(const float2* __restrict__ part, int entries,
                                                          const float* __restrict__ zt, const int32_t* __restrict__ tgt,
@@ -969,13 +976,14 @@ hipError_t ls_gemm(LsParams p, hipStream_t st) {
   return hipGetLastError();
 }
 
-// Tile side of the products over the vocabulary, whose tiles stay whole. bf16: 64 where one round of such tiles, two to a CU, is
-// all (61 x 1024 x 10112 forward and dx: 15.6 and 36 us, with 128 18.5 and 42; 128 tokens 17.1 and 38, 18.5 and 42; 2 rounds, 200
-// tokens: 25.5 and 51, 18.8 and 47). Else a round of 256 x 256 tiles takes 30 us at h = 1024 and one of 128 x 128, two to a CU, 17
-// (16384 x 1024 x 10112: 302 and 350 us; 1777 tokens: 60 and 51; 300: 30 and 17). fp32 multiplies at a sixteenth of the rate, so
-// that a large tile's reuse is worth nothing, and the work on the busiest CU decides: 64 where it gets at most three times as many of
-// those as of 128 (of 64 tokens the larger tile is half empty: 61 x 2048 x 50021 forward 155 and 244 us; 100 x 1024 x 10112 45 and 71;
-// three for one, 200 tokens, 69 and 72, 2600 x 512 x 2000 67 and 72; seven for two, 700 tokens, 137 and 129).
+// Tile side of the products over the vocabulary, whose tiles stay whole. bf16: 64 where one round of such tiles, two to a
+// CU, is all (61 x 1024 x 10112 forward and dx: 15.6 and 36 us, with 128 18.5 and 42; 128 tokens 17.1 and 38, 18.5 and 42;
+// 2 rounds, 200 tokens: 25.5 and 51, 18.8 and 47). Else a round of 256 x 256 tiles takes 30 us at h = 1024 and one of 128 x
+// 128, two to a CU, 17 (16384 x 1024 x 10112: 302 and 350 us; 1777 tokens: 60 and 51; 300: 30 and 17). fp32 multiplies at a
+// sixteenth of the rate, so that a large tile's reuse is worth nothing, and the work on the busiest CU decides: 64 where it
+// gets at most three times as many of those as of 128 (of 64 tokens the larger tile is half empty: 61 x 2048 x 50021
+// forward 155 and 244 us; 100 x 1024 x 10112 45 and 71; three for one, 200 tokens, 69 and 72, 2600 x 512 x 2000 67 and 72;
+// seven for two, 700 tokens, 137 and 129).
 int tile_z(int64_t M, int64_t N, bool f32) {
   const int64_t cus = device_cus(), n64 = ceil_div(M, 64) * ceil_div(N, 64), n128 = ceil_div(M, 128) * ceil_div(N, 128);
   if (f32) return ceil_div(n64, cus) <= 3 * ceil_div(n128, cus) ? 64 : 128;
@@ -991,12 +999,13 @@ uint64_t ls_cost(int64_t M, int64_t N, int64_t steps) {
          (B == 256 ? 2 * ((tiles + slots - 1) / slots) : 0);  // its longer epilogue
 }
 
-// Of the gradients' products, whose tiles can be split over K. 64 (with eight steps in LDS) for few tiles of 128, or for at most one
-// per two CUs and little K (dx of 61 x 1024 x 10112: 37 and 49 us with the rest of the call; of 400 x 1024 x 30000, 32 tiles, 173
-// and 116, in fp32 of 400 x 1024 x 10112 224 and 192; dw of 2600 x 512 x 2000 39 and 47, of 1500 x 1024 x 2000, 128 tiles of 24
-// steps, 42 and 47, of 700 x 256 x 10112, 158 tiles, 35 and 28). Else bf16 takes 128 or 256 by the time that the plan gives either, a
-// step of 256 being worth 1.6 (two of 128 to a CU): dx of 1280 x 1024 x 10112 88 and 100 us, of 1536 x 2048 x 50021 762 and 648; dw of
-// 100 x 1024 x 10112 28 and 30, of 6000 x 1024 x 10112 290 and 321, of 1536 x 2048 x 50021 727 and 667. fp32 has no use for 256.
+// Of the gradients' products, whose tiles can be split over K. 64 (with eight steps in LDS) for few tiles of 128, or for at
+// most one per two CUs and little K (dx of 61 x 1024 x 10112: 37 and 49 us with the rest of the call; of 400 x 1024 x
+// 30000, 32 tiles, 173 and 116, in fp32 of 400 x 1024 x 10112 224 and 192; dw of 2600 x 512 x 2000 39 and 47, of 1500 x
+// 1024 x 2000, 128 tiles of 24 steps, 42 and 47, of 700 x 256 x 10112, 158 tiles, 35 and 28). Else bf16 takes 128 or 256 by
+// the time that the plan gives either, a step of 256 being worth 1.6 (two of 128 to a CU): dx of 1280 x 1024 x 10112 88 and
+// 100 us, of 1536 x 2048 x 50021 762 and 648; dw of 100 x 1024 x 10112 28 and 30, of 6000 x 1024 x 10112 290 and 321, of
+// 1536 x 2048 x 50021 727 and 667. fp32 has no use for 256.
 int tile_k(int64_t M, int64_t N, int64_t steps, bool f32) {
   const int64_t cus = device_cus(), n128 = ceil_div(M, 128) * ceil_div(N, 128);
   if (8 * n128 < cus || (2 * n128 <= cus && n128 * steps <= (f32 ? 16 : 12) * cus)) return 64;

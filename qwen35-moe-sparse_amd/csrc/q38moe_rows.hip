@@ -5,10 +5,10 @@
 //   spread:   dst[inv[p]] = src[t] (* w[p]),  dst[r] = 0 for r >= filled,  dw[p] = <src[t], y[inv[p]]>
 //   collect:  out[t] = sum_j src[inv[p]] (* w[p])
 //
-// spread without w is the dispatch, collect without w its gradient; collect with w is the combine, spread with
-// w and y its gradients. Products and sums are fp32, each output is rounded once. Both run one wave per token: a wave's
-// instruction covers 1 KiB of a row, and the loads of two such pieces of all k rows are issued before any is used. Both are bound
-// by memory: 16384 tokens of 1024 bf16 by 5 take 36 us there (201 MB, 5.6 TB/s), 35 back, and 68 for both gradients of the
+// spread without w is the dispatch, collect without w its gradient; collect with w is the combine, spread with w and y its
+// gradients. Products and sums are fp32, each output is rounded once. Both run one wave per token: a wave's instruction
+// covers 1 KiB of a row, and the loads of two such pieces of all k rows are issued before any is used. Both are bound by
+// memory: 16384 tokens of 1024 bf16 by 5 take 36 us there (201 MB, 5.6 TB/s), 35 back, and 68 for both gradients of the
 // combine (369 MB, 5.4 TB/s). Rows are written past the caches, which the next reader's 168 MB would not find there anyway:
 // through them the four passes take 195 us together instead of 174.
 #include <type_traits>
@@ -162,10 +162,11 @@ __global__ __launch_bounds__(256) void spread_kernel(const E* __restrict__ src, 
 }
 
 // Dispatch of up to ROWS_SMALL pairs in one launch instead of three (histogram, permutation, spread): every block takes all
-// pairs' experts into LDS and counts them, and a wave finds its token's rows as starts[e] + the earlier pairs of the same expert, 64
-// at a time by ballots, which is the stable order of the permutation. Between them the blocks write the whole plan. 305 pairs take 5.4
-// us on the GPU and 9.5 with the host's part, in three launches 8.7 and 16; 2560 pairs 8.8 and 9.6, 10.1 and 16.5; at 4096 the ballots
-// cost as much as the launches (k = 2: 9.1 and 9.2 us on the GPU; k = 8: 11.9 and 10.4, but 11.6 and 16 with the host).
+// pairs' experts into LDS and counts them, and a wave finds its token's rows as starts[e] + the earlier pairs of the same
+// expert, 64 at a time by ballots, which is the stable order of the permutation. Between them the blocks write the whole
+// plan. 305 pairs take 5.4 us on the GPU and 9.5 with the host's part, in three launches 8.7 and 16; 2560 pairs 8.8 and
+// 9.6, 10.1 and 16.5; at 4096 the ballots cost as much as the launches (k = 2: 9.1 and 9.2 us on the GPU; k = 8: 11.9 and
+// 10.4, but 11.6 and 16 with the host).
 template <typename E, typename IdxT, int KT>
 __global__ __launch_bounds__(256) void dispatch_small_kernel(const E* __restrict__ src, const IdxT* __restrict__ idx,
                                                              int32_t* __restrict__ counts, int32_t* __restrict__ starts,
