@@ -535,8 +535,8 @@ int q38moe_qsa_attention(const void* q, const void* k, const void* v, const void
 int q38moe_linear_ce_workspace_bytes(int64_t T, int32_t h, int32_t V, int32_t needs, int32_t dtype, size_t* bytes);
 int q38moe_linear_ce_forward(const void* x, const void* w, const void* targets, int32_t targets_int64,
                              int64_t ignore_index, float* loss, float* lse, float* reduced, float* row_scale,
-                             int32_t mean, int64_t T, int32_t h, int32_t V, void* workspace, size_t workspace_bytes, int32_t dtype,
-                             void* stream);
+                             int32_t mean, int64_t T, int32_t h, int32_t V, void* workspace, size_t workspace_bytes,
+                             int32_t dtype, void* stream);
 int q38moe_linear_ce_backward(const float* g, int32_t g_per_row, const float* row_scale, const void* x, const void* w,
                               const void* targets, int32_t targets_int64, int64_t ignore_index, const float* lse,
                               void* dx, void* dw, int64_t T, int32_t h, int32_t V, void* workspace,
@@ -565,12 +565,12 @@ int q38moe_clip_grads(const void* const* src, void* const* dst, const int64_t* n
  * Rows to experts of the caller's own and back. A plan is the permutation of q38moe_permute (pair p = t*k + j of
  * expert-sorted row inv[p]; pairs whose index lies outside [0, E) have no row) in one int32 buffer of
  * q38moe_rows_plan_ints(T, E, k) entries: counts [E], starts [E], perm [T*k] and inv [T*k] from entries 0, E4, 2 E4 and
- * 2 E4 + P4 on (E4 and P4: E and T*k up to a multiple of 4), then scratch. dispatch makes the plan (inv is -1 for
- * pairs without a row) and dst[inv[p]] = x[t]; the others look at the plan alone. spread: dst[inv[p]] = src[t] (* w[p] unless w is NULL), and with y [T*k,h] dw[p] = <src[t], y[inv[p]]> (0 for pairs
- * without a row); dst or dw may be NULL. Both fill the rows behind the last filled one with zeros. collect: out[t] =
- * sum_j src[inv[p]] (* w[p] unless w is NULL). x, src, dst, y and out in dtype, w and dw [T,k] in w_dtype (dtype or
- * fp32); products and sums fp32, rounded once. The gradient of dispatch is collect without w; combine is collect
- * with w and its gradients spread with w and y.
+ * 2 E4 + P4 on (E4 and P4: E and T*k up to a multiple of 4), then scratch. dispatch makes the plan (inv is -1 for pairs
+ * without a row) and dst[inv[p]] = x[t]; the others look at the plan alone. spread: dst[inv[p]] = src[t] (* w[p] unless w
+ * is NULL), and with y [T*k,h] dw[p] = <src[t], y[inv[p]]> (0 for pairs without a row); dst or dw may be NULL. Both fill
+ * the rows behind the last filled one with zeros. collect: out[t] = sum_j src[inv[p]] (* w[p] unless w is NULL). x, src,
+ * dst, y and out in dtype, w and dw [T,k] in w_dtype (dtype or fp32); products and sums fp32, rounded once. The gradient
+ * of dispatch is collect without w; combine is collect with w and its gradients spread with w and y.
  */
 int64_t q38moe_rows_plan_ints(int64_t T, int32_t E, int32_t k);
 int q38moe_dispatch_rows(const void* x, const void* topk_idx, int32_t idx_is_int64, int32_t* plan, void* dst, int64_t T,
