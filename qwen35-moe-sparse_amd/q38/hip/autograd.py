@@ -204,8 +204,11 @@ class HipLinearCE(torch.autograd.Function):
     def backward(ctx, g):
         x, weight, targets, lse, row_scale = ctx.saved_tensors
         need_x, need_w = ctx.needs_input_grad[:2]
-        dx, dw = ops.linear_ce_backward(g.contiguous(), x, weight, targets, lse, ctx.ignore_index, row_scale, need_x,
-                                        need_w)
+        if not (need_x or need_w):
+            return None, None, None, None, None
+        # g has the loss's type, shape and device: autograd sees to that, and the forward has looked at the rest.
+        dx, dw = ops._linear_ce_backward(g.contiguous(), x, weight, targets, lse, ctx.ignore_index, row_scale, need_x,
+                                         need_w)
         return dx, dw, None, None, None
 
 
@@ -245,7 +248,7 @@ class HipDispatch(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, d_rows):
-        return ops.collect_rows(_aligned(d_rows), ctx.plan), None
+        return ops._collect_rows(_aligned(d_rows), ctx.plan, None, None), None
 
 
 class HipCombine(torch.autograd.Function):
@@ -262,7 +265,7 @@ class HipCombine(torch.autograd.Function):
         need_rows, need_w = ctx.needs_input_grad[:2]
         if not (need_rows or need_w):
             return None, None, None
-        d_rows, dw = ops.spread_rows(_aligned(d_out), ctx.plan, w, rows if need_w else None, need_rows)
+        d_rows, dw = ops._spread_rows(_aligned(d_out), ctx.plan, w, w.data_ptr(), rows if need_w else None, need_rows)
         return d_rows, dw, None
 
 

@@ -810,11 +810,12 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
 
 
 _HERE = contextlib.nullcontext()
+_device_index = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
 def _on(device):
     """The tensors' device as the current one, for launches on its stream."""
-    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+    return _HERE if device.index == _device_index() else torch.cuda.device(device)
 
 
 def _loss_args(x, w, targets):
@@ -884,6 +885,12 @@ def linear_ce_backward(g, x, w, targets, lse, ignore_index=-100, row_scale=None,
             raise ValueError(f"row_scale must hold one element, got {tuple(row_scale.shape)}")
     if any(t is not None and t.device != dev for t in (g, lse, row_scale)):
         raise RuntimeError("g, lse, row_scale and x must be on one device")
+    return _linear_ce_backward(g, x, w, targets, lse, ignore_index, row_scale, need_x, need_w)
+
+
+def _linear_ce_backward(g, x, w, targets, lse, ignore_index, row_scale, need_x, need_w):
+    """linear_ce_backward of operands that its forward has looked at."""
+    (T, h), V, dt, dev = x.shape, w.shape[0], x.dtype, x.device
     if T == 0:
         return (torch.zeros_like(x) if need_x else None), (torch.zeros_like(w) if need_w else None)
     dx = torch.empty_like(x) if need_x else None
@@ -1107,6 +1114,12 @@ def spread_rows(src, plan, w=None, y=None, need_rows=True):
             raise RuntimeError(f"y must be on {dev}, got {y.device}")
         if w is None:
             raise ValueError("y needs weights")
+    return _spread_rows(src, plan, w, pw, y, need_rows)
+
+
+def _spread_rows(src, plan, w, pw, y, need_rows):
+    """spread_rows of operands that have been looked at (pw: w's address)."""
+    (T, h), k, dt, dev = src.shape, plan.idx.shape[1], src.dtype, src.device
     dst = torch.empty(T * k, h, dtype=dt, device=dev) if need_rows else None
     dw = torch.empty_like(w) if y is not None else None
     with _on(dev):
@@ -1128,7 +1141,12 @@ def collect_rows(rows, plan, w=None):
     if rows.shape[0] != T * k:
         raise ValueError(f"rows must hold {T * k} rows, got {rows.shape[0]}")
     _filled(plan, dev, "rows")
-    pw = None if w is None else _rows_weights(w, plan.idx.shape, dt, dev)
+    return _collect_rows(rows, plan, w, None if w is None else _rows_weights(w, plan.idx.shape, dt, dev))
+
+
+def _collect_rows(rows, plan, w, pw):
+    """collect_rows of operands that have been looked at (pw: w's address)."""
+    (T, k), h, dt, dev = plan.idx.shape, rows.shape[1], rows.dtype, rows.device
     out = torch.empty(T, h, dtype=dt, device=dev)
     with _on(dev):
         check(lib.q38moe_collect_rows(rows.data_ptr(), pw, _DTYPES[dt if w is None else w.dtype], plan.buffer.data_ptr(),
