@@ -204,6 +204,7 @@ struct LsParams {
   bool first, last;      // piece: acc holds nothing yet; out is written (else acc)
   float* split;          // partial sums of split tiles, a tile after another
   uint32_t slots;        // workgroups that run at once
+  bool whole;            // no tile is split
 };
 
 // How a product's tiles are dealt to `slots` workgroups: whole rounds of them take their tile over all of K. The `rest` of
@@ -342,8 +343,8 @@ __global__ __launch_bounds__(256, ls_per_cu(BM, EPI)) void ls_gemm_kernel(const 
   // Work items of neighbouring blocks on an XCD are neighbouring tiles: 8 tiles of M by as many of N as it has room for.
   const uint32_t G = gridDim.x;
   const uint32_t first = (G & 7) == 0 ? (blockIdx.x & 7) * (G >> 3) + (blockIdx.x >> 3) : blockIdx.x;
-  const LsPlan pl = EPI == EPI_OUT ? ls_plan_wave<F32, BM>(tiles, (uint32_t)steps, p.slots)
-                                   : LsPlan{tiles, 0, (uint32_t)steps, (uint32_t)steps, 1, 0};
+  const LsPlan pl = EPI == EPI_OUT && !p.whole ? ls_plan_wave<F32, BM>(tiles, (uint32_t)steps, p.slots)
+                                               : LsPlan{tiles, 0, (uint32_t)steps, (uint32_t)steps, 1, 0};
   // Of n items that are fewer than the blocks: this block's, or n. Each XCD has an eighth, neighbours, for its first blocks
   // (dealt like whole rounds, they would all go to the first XCDs: dW of 1777 x 1024 x 10112 with the rest of the call 106
   // us, so 119; the fp32 forward of 1024 x 512 x 10112 106 and 134).
@@ -966,11 +967,16 @@ uint32_t ls_slots(int bm, int epi) { return (uint32_t)(device_cus() * ls_per_cu(
 template <bool F32, int BM, int BN, int LA, int LB, int EPI>
 hipError_t ls_gemm(LsParams p, hipStream_t st) {
   p.slots = ls_slots(BM, EPI);
+  // dW's tiles do not depend on the rows that count, and fewer of those (fewer steps) make splitting no better: where T rows
+  // leave the tiles whole there is nothing to join (1777 x 1024 x 10112: 4 us).
+  if (EPI == EPI_OUT && LB == KS)
+    p.whole = ls_plan<F32, BM>((uint32_t)(ceil_div(p.M, BM) * ceil_div(p.N, BN)),
+                               (uint32_t)ceil_div(p.K, 128 / (F32 ? 4 : 2)), p.slots).rest == 0;
   const int64_t tiles = ceil_div(p.M, BM) * ceil_div(p.N, BN);
   const unsigned grid = EPI == EPI_OUT || tiles > p.slots ? p.slots : (unsigned)tiles;
   hipLaunchKernelGGL((ls_gemm_kernel<F32, BM, BN, LA, LB, EPI>), dim3(grid), dim3(256), 0, st, p);
   const hipError_t e = hipGetLastError();
-  if (EPI != EPI_OUT || e != hipSuccess) return e;
+  if (EPI != EPI_OUT || p.whole || e != hipSuccess) return e;
   using E = typename std::conditional<F32, float, uint16_t>::type;
   hipLaunchKernelGGL((ls_join_kernel<E, BM, BN, LB == KS>), dim3(1024), dim3(256), 0, st, p);
   return hipGetLastError();
