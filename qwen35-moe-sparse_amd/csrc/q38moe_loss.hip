@@ -904,10 +904,11 @@ __global__ __launch_bounds__(1024) void ls_finish_kernel(const float2* __restric
 }
 
 // The split tiles of a product (ls_gemm_kernel with the same parameters): their parts in order and the earlier pieces' sums,
-// to out or to the pieces' sums. A thread takes 32 consecutive m of one n, in the accumulators' order 4 at a time.
+// to out or to the pieces' sums. A thread takes 8 consecutive m of one n, in the accumulators' order 4 at a time (32 of them
+// leave too few loads under way: 80 tiles of 256 x 256 in 3 parts 16.5 us, so 18.1; 36 of 64 x 64 in fp32 5.9 and 7.2).
 template <typename E, int BM, int BN, bool TOK_K>
 __global__ __launch_bounds__(256) void ls_join_kernel(const LsParams p) {
-  constexpr int BK = 128 / sizeof(E), NB = BN / 64, PER = BM * BN / 32;  // threads of a tile
+  constexpr int BK = 128 / sizeof(E), NB = BN / 64, W = 2, PER = BM * BN / (4 * W);  // groups of four values of a thread, threads of a tile
   const int64_t cnt = (int64_t)load_uniform(p.count);
   const int64_t N = TOK_K ? p.N : cnt, K = TOK_K ? cnt : p.K;
   const uint32_t ntm = (uint32_t)((p.M + BM - 1) / BM), ntn = (uint32_t)((N + BN - 1) / BN);
@@ -921,36 +922,36 @@ __global__ __launch_bounds__(256) void ls_join_kernel(const LsParams p) {
     const uint32_t lo = q * pl.steps;
     const uint32_t c0 = pl.parts != 0 ? 0 : lo / pl.per, c1 = pl.parts != 0 ? pl.parts - 1 : (lo + pl.steps - 1) / pl.per;
     if (c0 == c1) continue;
-    const int ln = in & 31, blk = in >> 5;  // block (w MB + i) NB + j
+    const int ln = in & 31, k0 = (int)(in >> 5) % (8 / W) * W, blk = (int)(in >> 5) / (8 / W);  // block (w MB + i) NB + j
     int tm, tn;
     ls_tile(pl.full + q, ntm, ntn, tm, tn);
     const int j = blk % NB, i = blk / NB % (BM / 64), w = blk / NB / (BM / 64);
     const int64_t m = (int64_t)tm * BM + (w >> 1) * (BM / 2) + 32 * i, n = (int64_t)tn * BN + (w & 1) * (BN / 2) + 32 * j + ln;
     if (m >= p.M || n >= N) continue;
-    f32x4_t v[8];  // m = 8 (k / 2) + 4 (k % 2)
+    f32x4_t v[W];  // m = 4 (k0 + k)
     const int64_t at = (int64_t)blk * 1024 + 4 * ln;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] = (f32x4_t){0.0f, 0.0f, 0.0f, 0.0f};
+    for (int k = 0; k < W; ++k) v[k] = (f32x4_t){0.0f, 0.0f, 0.0f, 0.0f};
     for (uint32_t c = c0; c <= c1; ++c) {
       // Even runs: the tile is the second of the workgroup's, or the first.
       const uint32_t part = pl.parts != 0 ? c * pl.rest + q : 2 * c + (c * pl.per < lo ? 1 : 0);
       const float* a = p.split + (int64_t)part * (BM * BN) + at;
 #pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] += *reinterpret_cast<const f32x4_t*>(a + 256 * (k >> 1) + 128 * (k & 1));
+      for (int k = 0; k < W; ++k) v[k] += *reinterpret_cast<const f32x4_t*>(a + 128 * (k0 + k));
     }
     float* const c = p.acc + (int64_t)(pl.full + q) * (BM * BN) + at;
     if (!p.first) {
 #pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] += *reinterpret_cast<const f32x4_t*>(c + 256 * (k >> 1) + 128 * (k & 1));
+      for (int k = 0; k < W; ++k) v[k] += *reinterpret_cast<const f32x4_t*>(c + 128 * (k0 + k));
     }
     if (!p.last) {
 #pragma unroll
-      for (int k = 0; k < 8; ++k) *reinterpret_cast<f32x4_t*>(c + 256 * (k >> 1) + 128 * (k & 1)) = v[k];
+      for (int k = 0; k < W; ++k) *reinterpret_cast<f32x4_t*>(c + 128 * (k0 + k)) = v[k];
       continue;
     }
-    E* const o = static_cast<E*>(p.out) + (TOK_K || cnt >= p.T ? n : (int64_t)p.rows[n]) * p.ldo + m;
+    E* const o = static_cast<E*>(p.out) + (TOK_K || cnt >= p.T ? n : (int64_t)p.rows[n]) * p.ldo + m + 4 * k0;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
+    for (int k = 0; k < W; ++k) {
       v[k] *= scale;
       if constexpr (sizeof(E) == 4) *reinterpret_cast<f32x4_t*>(o + 4 * k) = v[k];
       else if (k & 1)
