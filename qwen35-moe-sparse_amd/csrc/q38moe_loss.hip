@@ -6,9 +6,14 @@
 // The forward pass multiplies tiles of the vocabulary by tiles of tokens and keeps of each only its rows' maximum and
 // sum of exponentials (fp32) and the target's logit. The backward pass takes the vocabulary in pieces whose s [T, piece]
 // fits a bounded workspace: it multiplies again (the logits were not kept), turns the fp32 accumulators into s, and
-// multiplies s by W and by x. s is rounded to the operands' type for the matrix units, before the loss's scalar
-// gradient g, which the outputs' epilogues apply: -1 + p then rounds alike in no two rows, where g (p - 1) would carry
-// one rounding error into every row. (A gradient per row has to go into s.)
+// multiplies s by W and by x. s is rounded to the operands' type for the matrix units (bf16: by up to 2^-8 of each
+// value), before the loss's scalar gradient g, which the outputs' epilogues apply: the target's -1 + p, most of s's norm,
+// then is -1 where p is below half a step, 2^-9, and loses only that p (1e-4 of the gradient at a vocabulary of 4000),
+// where g (-1 + p) would carry the rounding of g, the same one, into every row. A gradient per row has to go into s, since
+// dW sums over rows. What the rows' gradients share is taken out of them first: u, the largest without its power of two, so that
+// one that all rows have rounds as the scalar does (1777 x 256 x 4096 against float64, g = 0.5637 in every row: dx and dW are
+// off by 0.0017 of their norm; with g whole in s 0.0026, of which 0.0019 lie in the result's own direction). Where g / u is
+// no power of two the target's entry rounds too, once as every other (random g: 0.0022). In fp32 g stays whole.
 //
 // Rows whose target is the ignored one leave the problem first: a stable partition lists the others, their x is copied
 // next to each other, and the products run over those rows only, so neither the work nor a NaN in a masked row counts.
@@ -195,10 +200,11 @@ struct LsParams {
   uint32_t* done;        // EPI_LSE: cleared for ls_finish_kernel
   const float* lse;      // EPI_S: per counted token
   const float* g_row;    // its gradient, or NULL
+  const float* g_unit;   // bf16: what is taken out of it before s is rounded, or NULL
   // EPI_S, EPI_OUT
   void* out;             // s, or the gradient
   int64_t ldo;           // elements between rows of out
-  const float* g_scale;  // the loss's gradient (NULL: 1)
+  const float* g_scale;  // the loss's gradient, or the unit of the rows' (NULL: 1)
   const float* r_scale;  // the reduction's factor (NULL: 1)
   float* acc;            // tiles' sums over the pieces so far (fp32, in the accumulators' own order), or NULL
   bool first, last;      // piece: acc holds nothing yet; out is written (else acc)
@@ -353,6 +359,7 @@ __global__ __launch_bounds__(256, ls_per_cu(BM, EPI)) void ls_gemm_kernel(const 
     const uint32_t share = (n + 7) >> 3, i = blockIdx.x >> 3, at = (blockIdx.x & 7) * share + i;
     return i < share ? min(at, n) : n;
   };
+  const float unit = EPI == EPI_S && p.g_unit != nullptr ? load_uniform(p.g_unit) : 1.0f;
   // This block's items: its tiles of the whole rounds, then (with the grid of p.slots blocks) its share of the rest.
   const uint32_t whole = pl.full / G, left = pl.full - whole * G, last_tile = partial(left);
   const uint32_t rounds = whole + (last_tile < left ? 1 : 0);
@@ -566,7 +573,9 @@ __global__ __launch_bounds__(256, ls_per_cu(BM, EPI)) void ls_gemm_kernel(const 
       const bool n_ok = n < N;
       // Where the token's target lies among the wave's rows, and what the softmax needs.
       const int rel = EPI == EPI_OUT ? -1 : tk[j] - (EPI == EPI_S ? (int)p.v0 : 0) - (int)mw;
-      const float lse = EPI == EPI_S ? tl[j] : 0.0f, g = EPI == EPI_S ? tg[j] : 1.0f;
+      const float lse = EPI == EPI_S ? tl[j] : 0.0f;
+      float g = EPI == EPI_S ? tg[j] : 1.0f;
+      if (EPI == EPI_S && !F32 && p.g_row != nullptr) g /= unit;
       const int64_t row = TO_ROWS ? (int64_t)tk[j] : n;
       float mx = -__builtin_inff(), sum = 0.0f;
 #pragma unroll
@@ -679,13 +688,15 @@ __global__ __launch_bounds__(256, ls_per_cu(BM, EPI)) void ls_gemm_kernel(const 
 }
 
 // Partition of the rows: rows[0 .. n-1] those that count, ascending, rows[n .. T-1] the ignored ones, *count = n, tgt[i]
-// the target of rows[i] (-1: outside the vocabulary), and where given lse_c[i] = lse[rows[i]], g_c[i] = g[rows[i]].
+// the target of rows[i] (-1: outside the vocabulary), and where given lse_c[i] = lse[rows[i]], g_c[i] = g[rows[i]], *unit the
+// unit of those g.
 struct LsList {
   int32_t *rows, *tgt, *count;
   const float* lse;
   float* lse_c;
   const float* g;
   float* g_c;
+  float* unit;
 };
 constexpr int LS_RUNS = 8, LS_LIST = LS_RUNS * 1024;  // rows that a block of 1024 lists at a time, in runs of 1024
 
@@ -733,12 +744,36 @@ __device__ __forceinline__ int ls_places(const IdxT* targets, int64_t ignore, in
   return n;
 }
 
-__device__ __forceinline__ void ls_put(const LsList& l, int64_t t, int64_t i, int64_t v, int64_t ignore, int V) {
+// top: the largest finite g and -g so far.
+__device__ __forceinline__ void ls_put(const LsList& l, int64_t t, int64_t i, int64_t v, int64_t ignore, int V,
+                                       float (&top)[2]) {
   l.rows[i] = (int32_t)t;
   if (v == ignore) return;
   l.tgt[i] = v >= 0 && v < V ? (int32_t)v : -1;
   if (l.lse != nullptr) l.lse_c[i] = l.lse[t];
-  if (l.g != nullptr) l.g_c[i] = l.g[t];
+  if (l.g == nullptr) return;
+  const float g = l.g[t];
+  l.g_c[i] = g;
+  if (fabsf(g) < __builtin_inff()) top[0] = fmaxf(top[0], g), top[1] = fmaxf(top[1], -g);
+}
+
+// *unit = the finite g of the largest size without its power of two, in [1, 2) with g's sign (1 where it is zero or
+// subnormal; the positive one of two that are as large): by a block of 1024, of whose threads each has met `top`. Of the
+// rows' g only this is taken out before s is rounded, so that their range stays what it is; with the sign, because the
+// matrix unit's sums of -a are not exactly those of a.
+__device__ __forceinline__ void ls_store_unit(float* unit, float (&top)[2], float (*red)[2]) {
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+#pragma unroll
+    for (int o = 32; o; o >>= 1) top[e] = fmaxf(top[e], __shfl_xor(top[e], o));
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6][e] = top[e];
+  }
+  __syncthreads();
+  if (threadIdx.x != 0) return;
+#pragma unroll
+  for (int w = 1; w < 16; ++w) top[0] = fmaxf(top[0], red[w][0]), top[1] = fmaxf(top[1], red[w][1]);
+  const float g = top[1] > top[0] ? -top[1] : top[0];
+  *unit = fabsf(g) < 0x1p-126f ? 1.0f : __uint_as_float((__float_as_uint(g) & 0x807fffffu) | 0x3f800000u);
 }
 
 // The list by one block (16384 rows: 4.5 us with the targets in the caches, 9 without; with 1024 rows at a time 14.5).
@@ -746,11 +781,14 @@ template <typename IdxT>
 __global__ __launch_bounds__(1024) void ls_rows_kernel(const IdxT* __restrict__ targets, int64_t ignore, int64_t T, int V,
                                                        LsList l) {
   __shared__ int sums[LS_RUNS * 16 + 1];
+  __shared__ float red[16][2];
   int64_t kept = 0;  // rows that count, so far
+  float top[2] = {0.0f, 0.0f};
   for (int64_t t0 = 0; t0 < T; t0 += LS_LIST)
     kept += ls_places(targets, ignore, T, t0, kept, sums,
-                      [&](int64_t t, int64_t i, int64_t v) { ls_put(l, t, i, v, ignore, V); });
+                      [&](int64_t t, int64_t i, int64_t v) { ls_put(l, t, i, v, ignore, V, top); });
   if (threadIdx.x == 0) *l.count = (int32_t)kept;
+  if (l.unit != nullptr) ls_store_unit(l.unit, top, red);
 }
 
 __device__ __forceinline__ void ls_copy_row(const uint8_t* x, uint8_t* xc, uint8_t* zero, int64_t i, int64_t r, bool counts,
@@ -770,11 +808,14 @@ __global__ __launch_bounds__(1024) void ls_list_kernel(const IdxT* __restrict__ 
                                                        uint8_t* __restrict__ zero, int bytes) {
   __shared__ int sums[LS_RUNS * 16 + 1];
   __shared__ int own[16];
+  __shared__ float red[16][2];
+  float top[2] = {0.0f, 0.0f};
   const int n = ls_places(targets, ignore, T, 0, 0, sums, [&](int64_t t, int64_t i, int64_t v) {
-    if (blockIdx.x == 0) ls_put(l, t, i, v, ignore, V);
+    if (blockIdx.x == 0) ls_put(l, t, i, v, ignore, V, top);
     if ((int)(i >> 4) == (int)blockIdx.x) own[i & 15] = (int)t;
   });
   if (blockIdx.x == 0 && threadIdx.x == 0) *l.count = n;
+  if (blockIdx.x == 0 && l.unit != nullptr) ls_store_unit(l.unit, top, red);
   const int wave = (int)uniform(threadIdx.x >> 6);
   const int64_t i = (int64_t)blockIdx.x * 16 + wave;
   if (n >= T || i >= T || (i >= n && zero == nullptr)) return;
@@ -1032,7 +1073,7 @@ size_t acc_bytes(int64_t M, int64_t N, int b) { return 4 * (size_t)(b * b) * (si
 size_t up(size_t v) { return (v + 255) / 256 * 256; }
 
 struct Layout {
-  size_t rows, tgt, count, xc, part, zt, bsum, bn, done, lse, g, s, acc, split, end;
+  size_t rows, tgt, count, xc, part, zt, bsum, bn, done, lse, g, unit, s, acc, split, end;
   int entries;             // of the forward's partial sums
   int64_t piece;           // vocabulary rows of a piece (multiple of 256)
   int pieces;
@@ -1074,6 +1115,7 @@ Layout layout(int64_t T, int h, int V, bool f32, bool fwd, bool need_x, bool nee
     l.piece = pt * 256;
     l.lse = take(4 * T);
     l.g = take(4 * T);
+    l.unit = take(4);
     l.s = take(esz * (size_t)T * l.piece);
     const int64_t bk = f32 ? 32 : 64, n = l.piece < V ? l.piece : V;
     l.tile_s = tile_z(n, T, f32);
@@ -1140,7 +1182,7 @@ hipError_t ce_forward(const void* x, const void* w, const void* targets, bool id
   int32_t* count = at<int32_t>(ws, l.count);
   const int64_t rb = (int64_t)h * (F32 ? 4 : 2);
   if (!l.raw) {
-    const LsList list = {rows, tgt, count, nullptr, nullptr, nullptr, nullptr};
+    const LsList list = {rows, tgt, count, nullptr, nullptr, nullptr, nullptr, nullptr};
     LS_TRY(ls_rows_any(targets, idx64, ignore, T, V, list, x, at<void>(ws, l.xc), nullptr, (int)rb, st));
   }
   LsParams p = {};
@@ -1176,10 +1218,11 @@ hipError_t ce_backward(const float* g, bool g_rows, const float* r_scale, const 
   int32_t* count = at<int32_t>(ws, l.count);
   const int64_t rb = (int64_t)h * (F32 ? 4 : 2);
   const int64_t esz = F32 ? 4 : 2;
-  const LsList list = {rows, tgt, count, lse, at<float>(ws, l.lse), g_rows ? g : nullptr, at<float>(ws, l.g)};
+  float* unit = g_rows && !F32 ? at<float>(ws, l.unit) : nullptr;
+  const LsList list = {rows, tgt, count, lse, at<float>(ws, l.lse), g_rows ? g : nullptr, at<float>(ws, l.g), unit};
   LS_TRY(ls_rows_any(targets, idx64, ignore, T, V, list, x, at<void>(ws, l.xc), dx, (int)rb, st));
   const uint8_t* xc = at<const uint8_t>(ws, l.xc);
-  const float* scale = g_rows ? nullptr : g;
+  const float* scale = g_rows ? unit : g;
   for (int i = 0; i < l.pieces; ++i) {
     const int64_t v0 = (int64_t)i * l.piece, n = V - v0 < l.piece ? V - v0 : l.piece;
     const int64_t pitch = ceil_div(n, 256) * 256;
@@ -1198,6 +1241,7 @@ hipError_t ce_backward(const float* g, bool g_rows, const float* r_scale, const 
     p.tgt = tgt;
     p.lse = at<float>(ws, l.lse);
     p.g_row = g_rows ? at<float>(ws, l.g) : nullptr;
+    p.g_unit = unit;
     p.out = at<void>(ws, l.s);
     p.ldo = pitch;
     p.M = pitch;  // whole tiles: the columns behind the piece become zeros
