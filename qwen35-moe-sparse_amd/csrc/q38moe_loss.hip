@@ -32,9 +32,10 @@
 // What bounds it. The matrix units need 2051 clocks for a step of a 256 x 256 tile. With all CUs at work on random bf16
 // data the chip lowers its clock to 1.7 - 1.9 GHz: MFMAs alone take 1.09 us a step, with their LDS reads 1.23, with the
 // copies to LDS out of the L2 1.33 (all zeros: 0.94, 0.96, 1.04), and with a stream of its own per CU 1.94; this kernel,
-// whose tiles share the streams eight by four, takes 1.7. 16384 x 1024 x 10112: z 302 us (1120 TFLOP/s), s 2 x 168, dx 2 x
-// 158, dW 2 x 165. 4099 x 2048 x 50021: z 700 us (1190), s 2 x 391, dx 2 x 426, dW 2 x 410. Few tokens are bound by the
-// latency of W's way into LDS: 61 x 1024 x 10112 z 10 us for 20.7 MB.
+// whose tiles share the streams eight by four, takes 1.7, in dx, whose s comes from memory, 2.1 and more. Smallest and
+// median time of nine steps in a row: 16384 x 1024 x 10112 z 311 and 326 us (1090 and 1041 TFLOP/s), s 2 x 169 and 180, dx
+// 2 x 163 and 194, dW 2 x 168 and 182; 4099 x 2048 x 50021 z 703 and 732 (1195 and 1147), s 2 x 381 and 397, dx 2 x 425 and
+// 450, dW 2 x 403 and 423. Few tokens are bound by the latency of W's way into LDS: 61 x 1024 x 10112 z 10 us for 20.7 MB.
 #include "q38moe_common.h"
 #include "q38moe_kernels.h"
 
@@ -1092,7 +1093,7 @@ Layout layout(int64_t T, int h, int V, bool f32, bool fwd, bool need_x, bool nee
     off = up(off + n);
     return at;
   };
-  l.raw = fwd && T <= 256;  // one tile of tokens: nothing to skip, and two launches fewer
+  l.raw = fwd && T <= 256;  // few tokens: skipping rows would save less than the launch that lists them costs
   l.rows = take(l.raw ? 0 : 4 * T);
   l.tgt = take(l.raw ? 0 : 4 * T);
   l.count = take(4);
