@@ -273,7 +273,8 @@ def dispatch(x, topk_idx, num_experts):
     """Tokens x [T,h] (bf16 or fp32) in expert order, for experts of the caller's own: (rows [T*k,h], plan). Expert e's
     rows are rows[plan.starts[e] : plan.starts[e] + plan.counts[e]], in the order of the pairs; pairs routed outside [0, num_experts)
     have none, and as many rows at the end are zero. topk_idx [T,k] int32 or int64, which may change afterwards; num_experts
-    <= 64, k <= 8, h a multiple of 64. Gradients flow to x. ``combine`` with the same plan brings the experts' outputs back."""
+    <= 64, k <= min(8, num_experts), h a multiple of 64. Gradients flow to x. ``combine`` with the same plan brings the
+    experts' outputs back."""
     if x.dim() != 2 or topk_idx.dim() != 2 or topk_idx.shape[0] != x.shape[0]:
         raise ValueError(f"x must be [T,h] and topk_idx [T,k], got {tuple(x.shape)} and {tuple(topk_idx.shape)}")
     ops._fdt(x, "x")
