@@ -580,6 +580,57 @@ int q38moe_spread_rows(const void* src, const void* w, int32_t w_dtype, const vo
 int q38moe_collect_rows(const void* src, const void* w, int32_t w_dtype, const int32_t* plan, void* out, int64_t T,
                         int32_t h, int32_t E, int32_t k, int32_t dtype, void* stream);
 
+/*
+ * A token mixer with a carried state (no counterpart in the reference, whose mixers are the delta rule and QSA above).
+ *
+ * Norms of query and key heads and their rotation by position, one pass over q [T,H,d] and k [T,KV,d]:
+ *   n = x * rsqrt(mean(x^2) + eps) * w', w' = 1 + w with plus1, else w (n = x where the norm's weight is NULL)
+ *   y[i] = n[i] cos a_i - n[i + rot/2] sin a_i, y[i + rot/2] = n[i + rot/2] cos a_i + n[i] sin a_i for i < rot/2, the rest as
+ *   it is; a_i = positions[axis_of[i]][t] * inv_freq[i], a product in 64 bits; fp32 otherwise, one rounding.
+ * positions [n_axes,T] int32 or int64 (n_axes <= 4), axis_of [rot/2] (NULL: axis 0; an axis outside the positions makes the results
+ * that turn by it NaN), inv_freq [rot/2] fp32. strides (host): token and head stride of q, then of k, in elements, each a
+ * multiple of 16 bytes; outputs contiguous. d a multiple of 8 up to 256, rot a multiple of 8 up to d. Backward: gradients of
+ * both inputs (contiguous) and, where not NULL, of the weights; workspace for those (arbitrary contents).
+ */
+int q38moe_qk_norm_rope(const void* q, const void* k, const int64_t* strides, const void* q_norm, const void* k_norm,
+                        int32_t plus1, const void* positions, int32_t pos_int64, const int32_t* axis_of, int32_t n_axes,
+                        const float* inv_freq, void* q_out, void* k_out, int64_t T, int32_t H, int32_t KV, int32_t d,
+                        int32_t rot, float eps, int32_t dtype, void* stream);
+int q38moe_qk_norm_rope_workspace_bytes(int64_t T, int32_t H, int32_t KV, int32_t d, int32_t rot, size_t* bytes);
+int q38moe_qk_norm_rope_backward(const void* d_q_out, const void* d_k_out, const void* q, const void* k, const int64_t* strides,
+                                 const void* q_norm, const void* k_norm, int32_t plus1, const void* positions,
+                                 int32_t pos_int64, const int32_t* axis_of, int32_t n_axes, const float* inv_freq, void* dq,
+                                 void* dk, void* d_q_norm, void* d_k_norm, int64_t T, int32_t H, int32_t KV, int32_t d,
+                                 int32_t rot, float eps, void* workspace, size_t workspace_bytes, int32_t dtype, void* stream);
+
+/*
+ * Linear attention with a decay for each head: S_t = e^log_decay[h] S_{t-1} + k_t v_t^T, o_t = scale S_t^T q_t, over q [N,S,H,dk],
+ * k [N,S,Hk,dk] and v [N,S,Hk,dv] (head h reads k and v of head h / (H / Hk)), S fp32 [dk,dv] per sequence and head, initial_state
+ * and final_state [N,H,dk,dv] (NULL: zero, not wanted); out [N,S,H,dv] contiguous. With cu_seqlens (device int32 [N+1]) the S
+ * tokens of one row hold N sequences, n the tokens [cu[n], cu[n+1]) (offsets out of order or range are brought into both);
+ * tokens of no sequence get zeros. strides (host): sequence, token and head strides of q, k, v in elements, multiples of 16
+ * bytes (the sequences' unused with cu_seqlens). dk and dv multiples of 8 up to 128. Backward: from d_out (contiguous) and
+ * d_final_state (NULL: zero) the gradients that are not NULL, contiguous; d_initial_state only with dv. A token's NaN or
+ * infinity may reach the outputs of its chunk, up to 63 tokens before it. Workspace contents arbitrary.
+ * step: one token of B sequences, q [B,H,dk], k [B,Hk,dk], v [B,Hk,dv] (strides: sequence and head of each), states updated in
+ * place: state [pool,H,dk,dv], sequence b in slots[b] (NULL: b). A slot outside [0, pool) is none: out is zero. No slot may occur
+ * twice. out [B,H,dv].
+ */
+int q38moe_linear_attention_workspace_bytes(int64_t N, int64_t S, int32_t H, int32_t Hk, int32_t dk, int32_t dv, int32_t packed,
+                                            int32_t backward, size_t* bytes);
+int q38moe_linear_attention_forward(const void* q, const void* k, const void* v, const int64_t* strides, const float* log_decay,
+                                    float scale, const float* initial_state, const int32_t* cu_seqlens, void* out,
+                                    float* final_state, int64_t N, int64_t S, int32_t H, int32_t Hk, int32_t dk, int32_t dv,
+                                    void* workspace, size_t workspace_bytes, int32_t dtype, void* stream);
+int q38moe_linear_attention_backward(const void* d_out, const float* d_final_state, const void* q, const void* k, const void* v,
+                                     const int64_t* strides, const float* log_decay, float scale, const float* initial_state,
+                                     const int32_t* cu_seqlens, void* dq, void* dk_out, void* dv_out, float* d_initial_state,
+                                     int64_t N, int64_t S, int32_t H, int32_t Hk, int32_t dk, int32_t dv, void* workspace,
+                                     size_t workspace_bytes, int32_t dtype, void* stream);
+int q38moe_linear_attention_step(const void* q, const void* k, const void* v, const int64_t* strides, const float* log_decay,
+                                 float scale, float* state, const int32_t* slots, void* out, int64_t B, int64_t pool, int32_t H,
+                                 int32_t Hk, int32_t dk, int32_t dv, int32_t dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1787,4 +1787,293 @@ int q38moe_collect_rows(const void* src, const void* w, int32_t w_dtype, const i
   return Q38MOE_OK;
 }
 
+// ---- a token mixer with a carried state: normed and rotated heads, linear attention, its step -------------------------
+
+static int check_rope(int64_t T, int32_t H, int32_t KV, int32_t d, int32_t rot, int32_t n_axes, int32_t dtype) {
+  Q38_CHECK(check_dtype(dtype));
+  if (T < 0 || T >= (int64_t)1 << 31) return fail(Q38MOE_EINVAL, "T must be in [0, 2^31) (got %lld)", (long long)T);
+  if (H < 1 || KV < 1 || H + (int64_t)KV > 4096)
+    return fail(Q38MOE_EINVAL, "H and KV must be positive, at most 4096 together (got H=%d, KV=%d)", H, KV);
+  if (d < 8 || d > 256 || d % 8 != 0) return fail(Q38MOE_EINVAL, "d must be a multiple of 8 in [8, 256] (got %d)", d);
+  if (rot < 0 || rot > d || rot % 8 != 0) return fail(Q38MOE_EINVAL, "rot must be a multiple of 8 in [0, d] (got %d)", rot);
+  if (n_axes < 1 || n_axes > 4) return fail(Q38MOE_EINVAL, "n_axes must be in [1, 4] (got %d)", n_axes);
+  return Q38MOE_OK;
+}
+
+// Strides in elements: whole 16 bytes.
+static int check_strides(const int64_t* strides, int n, int32_t dtype) {
+  if (strides == nullptr) return fail(Q38MOE_EINVAL, "strides must not be NULL");
+  for (int i = 0; i < n; ++i)
+    if (strides[i] < 0 || strides[i] * (int64_t)elem_size(dtype) % 16 != 0)
+      return fail(Q38MOE_EINVAL, "stride %d must be a multiple of 16 bytes, not negative (got %lld elements)", i,
+                  (long long)strides[i]);
+  return Q38MOE_OK;
+}
+
+static int rope_args(q38::RopeArgs& p, const void* q, const void* k, const int64_t* strides, const void* q_norm,
+                     const void* k_norm, int32_t plus1, const void* positions, int32_t pos_int64, const int32_t* axis_of,
+                     int32_t n_axes, const float* inv_freq, void* q_out, void* k_out, int64_t T, int32_t H, int32_t KV,
+                     int32_t d, int32_t rot, float eps, int32_t dtype) {
+  Q38_CHECK(check_rope(T, H, KV, d, rot, n_axes, dtype));
+  Q38_CHECK(check_strides(strides, 4, dtype));
+  Q38_CHECK(check_opt_ptr(q_norm, "q_norm"));
+  Q38_CHECK(check_opt_ptr(k_norm, "k_norm"));
+  if (T > 0) {
+    Q38_CHECK(check_ptr(q, "q"));
+    Q38_CHECK(check_ptr(k, "k"));
+    Q38_CHECK(check_ptr(q_out, "q_out"));
+    Q38_CHECK(check_ptr(k_out, "k_out"));
+    if (rot > 0 && positions == nullptr) return fail(Q38MOE_EINVAL, "positions must not be NULL");
+    if (rot > 0 && inv_freq == nullptr) return fail(Q38MOE_EINVAL, "inv_freq must not be NULL");
+  }
+  p = {q, k, q_norm, k_norm, positions, strides[0], strides[1], strides[2], strides[3], T, axis_of, inv_freq, q_out, k_out,
+       eps, H, KV, d, rot, n_axes, 0, pos_int64 != 0, plus1 != 0};
+  return Q38MOE_OK;
+}
+
+int q38moe_qk_norm_rope(const void* q, const void* k, const int64_t* strides, const void* q_norm, const void* k_norm,
+                        int32_t plus1, const void* positions, int32_t pos_int64, const int32_t* axis_of, int32_t n_axes,
+                        const float* inv_freq, void* q_out, void* k_out, int64_t T, int32_t H, int32_t KV, int32_t d,
+                        int32_t rot, float eps, int32_t dtype, void* stream) {
+  g_err[0] = 0;
+  q38::RopeArgs p;
+  Q38_CHECK(rope_args(p, q, k, strides, q_norm, k_norm, plus1, positions, pos_int64, axis_of, n_axes, inv_freq, q_out, k_out,
+                      T, H, KV, d, rot, eps, dtype));
+  (void)hipGetLastError();
+  Q38_HIP(q38::launch_rope(p, dtype == Q38MOE_BF16, static_cast<hipStream_t>(stream)), "norm and rotation launch");
+  return Q38MOE_OK;
+}
+
+int q38moe_qk_norm_rope_workspace_bytes(int64_t T, int32_t H, int32_t KV, int32_t d, int32_t rot, size_t* bytes) {
+  g_err[0] = 0;
+  if (bytes == nullptr) return fail(Q38MOE_EINVAL, "bytes must not be NULL");
+  Q38_CHECK(check_rope(T, H, KV, d, rot, 1, Q38MOE_BF16));
+  q38::RopeArgs p = {};
+  p.T = T, p.H = H, p.KV = KV, p.d = d, p.rot = rot;
+  *bytes = sizeof(float) * 2 * (size_t)d * (size_t)std::max(1, q38::rope_backward_blocks(p));
+  return Q38MOE_OK;
+}
+
+int q38moe_qk_norm_rope_backward(const void* d_q_out, const void* d_k_out, const void* q, const void* k, const int64_t* strides,
+                                 const void* q_norm, const void* k_norm, int32_t plus1, const void* positions,
+                                 int32_t pos_int64, const int32_t* axis_of, int32_t n_axes, const float* inv_freq, void* dq,
+                                 void* dk, void* d_q_norm, void* d_k_norm, int64_t T, int32_t H, int32_t KV, int32_t d,
+                                 int32_t rot, float eps, void* workspace, size_t workspace_bytes, int32_t dtype,
+                                 void* stream) {
+  g_err[0] = 0;
+  q38::RopeArgs p;
+  Q38_CHECK(rope_args(p, q, k, strides, q_norm, k_norm, plus1, positions, pos_int64, axis_of, n_axes, inv_freq, dq, dk, T, H,
+                      KV, d, rot, eps, dtype));
+  if ((d_q_norm != nullptr && q_norm == nullptr) || (d_k_norm != nullptr && k_norm == nullptr))
+    return fail(Q38MOE_EINVAL, "a weight's gradient needs the weight");
+  if (T > 0) {
+    Q38_CHECK(check_ptr(d_q_out, "d_q_out"));
+    Q38_CHECK(check_ptr(d_k_out, "d_k_out"));
+  }
+  const bool dw = d_q_norm != nullptr || d_k_norm != nullptr;
+  if (dw) {
+    size_t need = 0;
+    Q38_CHECK(q38moe_qk_norm_rope_workspace_bytes(T, H, KV, d, rot, &need));
+    Q38_CHECK(check_ptr(workspace, "workspace"));
+    if (workspace_bytes < need) return fail(Q38MOE_EWORKSPACE, "workspace needs %zu bytes, got %zu", need, workspace_bytes);
+  }
+  (void)hipGetLastError();
+  Q38_HIP(q38::launch_rope_backward(p, d_q_out, d_k_out, dw ? static_cast<float*>(workspace) : nullptr, d_q_norm, d_k_norm,
+                                    dtype == Q38MOE_BF16, static_cast<hipStream_t>(stream)),
+          "norm and rotation backward launch");
+  return Q38MOE_OK;
+}
+
+static int check_linattn(int64_t N, int64_t S, int32_t H, int32_t Hk, int32_t dk, int32_t dv, int32_t dtype) {
+  Q38_CHECK(check_dtype(dtype));
+  if (N < 0 || N > (1 << 24)) return fail(Q38MOE_EINVAL, "N must be in [0, 2^24] (got %lld)", (long long)N);
+  if (S < 0 || S > (1 << 30)) return fail(Q38MOE_EINVAL, "S must be in [0, 2^30] (got %lld)", (long long)S);
+  if (H < 1 || Hk < 1 || H % Hk != 0) return fail(Q38MOE_EINVAL, "H must be a multiple of Hk (got H=%d, Hk=%d)", H, Hk);
+  if (dk < 8 || dk > 128 || dk % 8 != 0) return fail(Q38MOE_EINVAL, "dk must be a multiple of 8 in [8, 128] (got %d)", dk);
+  if (dv < 8 || dv > 128 || dv % 8 != 0) return fail(Q38MOE_EINVAL, "dv must be a multiple of 8 in [8, 128] (got %d)", dv);
+  return Q38MOE_OK;
+}
+
+// How a call's sequences are cut, and the parts of its workspace: the plan (packed), the states between segments, and (backwards,
+// shared heads) one fp32 gradient for each head.
+struct LinattnPlan {
+  int L, nseg;
+  int64_t tokens, segs;
+  size_t mid, grouped, bytes;
+};
+static int linattn_plan(LinattnPlan& p, int64_t N, int64_t S, int32_t H, int32_t Hk, int32_t dk, int32_t dv, bool packed,
+                        bool backward) {
+  p.tokens = packed ? S : N * S;
+  p.L = q38::la_segment_tokens(p.tokens, N, H);
+  p.nseg = packed ? 0 : (int)std::max<int64_t>(1, (S + p.L - 1) / p.L);
+  p.segs = packed ? S / p.L + N : N * p.nseg;
+  if (p.segs * H >= (int64_t)1 << 31) return fail(Q38MOE_EINVAL, "too many sequences and heads for one launch");
+  const size_t states = sizeof(float) * (size_t)(p.segs - N) * H * (size_t)q38::la_padded_state(dk, dv);
+  const bool grouped = backward && H != Hk;
+  p.mid = packed ? align_up(sizeof(int32_t) * (size_t)(3 * N + 1)) : 0;
+  p.grouped = p.mid + align_up(states);
+  p.bytes = p.grouped + (grouped ? sizeof(float) * (size_t)p.tokens * H * std::max(dk, dv) : 0);
+  return Q38MOE_OK;
+}
+
+int q38moe_linear_attention_workspace_bytes(int64_t N, int64_t S, int32_t H, int32_t Hk, int32_t dk, int32_t dv, int32_t packed,
+                                            int32_t backward, size_t* bytes) {
+  g_err[0] = 0;
+  if (bytes == nullptr) return fail(Q38MOE_EINVAL, "bytes must not be NULL");
+  Q38_CHECK(check_linattn(N, S, H, Hk, dk, dv, Q38MOE_BF16));
+  LinattnPlan p;
+  Q38_CHECK(linattn_plan(p, N, S, H, Hk, dk, dv, packed != 0, backward != 0));
+  *bytes = p.bytes;
+  return Q38MOE_OK;
+}
+
+// Checks, the plan, and what every pass over the tokens shares.
+static int linattn_start(LinattnPlan& p, q38::LaArgs& a, const float* log_decay, const int32_t* cu_seqlens, int64_t N, int64_t S,
+                         int32_t H, int32_t Hk, int32_t dk, int32_t dv, bool backward, void* workspace,
+                         size_t workspace_bytes, int32_t dtype, hipStream_t st) {
+  Q38_CHECK(check_linattn(N, S, H, Hk, dk, dv, dtype));
+  if (log_decay == nullptr) return fail(Q38MOE_EINVAL, "log_decay must not be NULL");
+  Q38_CHECK(linattn_plan(p, N, S, H, Hk, dk, dv, cu_seqlens != nullptr, backward));
+  if (p.bytes > 0) {
+    Q38_CHECK(check_ptr(workspace, "workspace"));
+    if (workspace_bytes < p.bytes)
+      return fail(Q38MOE_EWORKSPACE, "workspace needs %zu bytes, got %zu", p.bytes, workspace_bytes);
+  }
+  a = {};
+  a.g = log_decay;
+  a.mid = reinterpret_cast<float*>(static_cast<char*>(workspace) + p.mid);
+  a.N = (int)N, a.S = (int)S, a.H = H, a.L = p.L, a.nseg = p.nseg;
+  (void)hipGetLastError();
+  if (cu_seqlens != nullptr) {
+    a.plan = static_cast<const int32_t*>(workspace);
+    Q38_HIP(q38::launch_la_plan(cu_seqlens, static_cast<int32_t*>(workspace), (int)N, (int)S, p.L, st), "segments launch");
+  }
+  return Q38MOE_OK;
+}
+
+static q38::LaTensor la_tensor(const void* p, const int64_t* strides, int div) { return {p, strides[0], strides[1], strides[2], div}; }
+
+int q38moe_linear_attention_forward(const void* q, const void* k, const void* v, const int64_t* strides, const float* log_decay,
+                                    float scale, const float* initial_state, const int32_t* cu_seqlens, void* out,
+                                    float* final_state, int64_t N, int64_t S, int32_t H, int32_t Hk, int32_t dk, int32_t dv,
+                                    void* workspace, size_t workspace_bytes, int32_t dtype, void* stream) {
+  g_err[0] = 0;
+  Q38_CHECK(check_strides(strides, 9, dtype));
+  LinattnPlan p;
+  q38::LaArgs a;
+  if (N == 0 && check_linattn(N, S, H, Hk, dk, dv, dtype) == Q38MOE_OK && (cu_seqlens == nullptr || S == 0)) return Q38MOE_OK;
+  if (N == 0 && cu_seqlens != nullptr) return fail(Q38MOE_EINVAL, "packed tokens need a sequence");
+  if (N > 0 && S > 0) {
+    Q38_CHECK(check_ptr(q, "q"));
+    Q38_CHECK(check_ptr(k, "k"));
+    Q38_CHECK(check_ptr(v, "v"));
+    Q38_CHECK(check_ptr(out, "out"));
+  }
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  Q38_CHECK(linattn_start(p, a, log_decay, cu_seqlens, N, S, H, Hk, dk, dv, false, workspace, workspace_bytes, dtype, st));
+  const int G = H / Hk;
+  a.q = la_tensor(q, strides, 1);
+  a.k = la_tensor(k, strides + 3, G);
+  a.v = la_tensor(v, strides + 6, G);
+  a.o = out, a.oh = dv, a.ot = (int64_t)H * dv, a.ob = S * a.ot;
+  a.o_f32 = dtype == Q38MOE_FP32;
+  a.s0 = initial_state, a.s1 = final_state, a.turned = false;
+  a.intra = a.inter = scale, a.gain = 1.0f, a.lag = 0;
+  a.dk = dk, a.dv = dv;
+  const bool bf16 = dtype == Q38MOE_BF16;
+  Q38_HIP(q38::launch_la(a, p.segs, false, bf16, st), "linear attention launch");
+  if (a.plan != nullptr && S > 0)
+    Q38_HIP(q38::launch_la_gap(out, a.plan, (int)N, S, H * dv * (int)elem_size(dtype), st), "linear attention launch");
+  return Q38MOE_OK;
+}
+
+int q38moe_linear_attention_backward(const void* d_out, const float* d_final_state, const void* q, const void* k, const void* v,
+                                     const int64_t* strides, const float* log_decay, float scale, const float* initial_state,
+                                     const int32_t* cu_seqlens, void* dq, void* dk_out, void* dv_out, float* d_initial_state,
+                                     int64_t N, int64_t S, int32_t H, int32_t Hk, int32_t dk, int32_t dv, void* workspace,
+                                     size_t workspace_bytes, int32_t dtype, void* stream) {
+  g_err[0] = 0;
+  Q38_CHECK(check_strides(strides, 9, dtype));
+  LinattnPlan p;
+  q38::LaArgs a;
+  if (N == 0 && check_linattn(N, S, H, Hk, dk, dv, dtype) == Q38MOE_OK && (cu_seqlens == nullptr || S == 0)) return Q38MOE_OK;
+  if (N == 0 && cu_seqlens != nullptr) return fail(Q38MOE_EINVAL, "packed tokens need a sequence");
+  if (N > 0 && S > 0) {
+    Q38_CHECK(check_ptr(q, "q"));
+    Q38_CHECK(check_ptr(k, "k"));
+    Q38_CHECK(check_ptr(v, "v"));
+    Q38_CHECK(check_ptr(d_out, "d_out"));
+    Q38_CHECK(check_opt_ptr(dq, "dq"));
+    Q38_CHECK(check_opt_ptr(dk_out, "dk"));
+    Q38_CHECK(check_opt_ptr(dv_out, "dv"));
+  }
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  Q38_CHECK(linattn_start(p, a, log_decay, cu_seqlens, N, S, H, Hk, dk, dv, true, workspace, workspace_bytes, dtype, st));
+  const int G = H / Hk;
+  const bool bf16 = dtype == Q38MOE_BF16;
+  float* per_head = reinterpret_cast<float*>(static_cast<char*>(workspace) + p.grouped);
+  const int64_t do_strides[3] = {S * (int64_t)H * dv, (int64_t)H * dv, dv};
+  const q38::LaTensor tq = la_tensor(q, strides, 1), tk = la_tensor(k, strides + 3, G), tv = la_tensor(v, strides + 6, G),
+                      tdo = la_tensor(d_out, do_strides, 1);
+  // One pass with its results in `out`, the heads that share one added where it has Hk of them.
+  auto pass = [&](void* out, int d, bool shared, bool backwards) -> int {
+    const bool grouped = shared && G > 1;
+    a.o = grouped ? per_head : out;
+    a.o_f32 = grouped || !bf16;
+    a.oh = d, a.ot = (int64_t)H * d, a.ob = S * a.ot;
+    Q38_HIP(q38::launch_la(a, p.segs, backwards, bf16, st), "linear attention backward launch");
+    if (grouped) Q38_HIP(q38::launch_la_group(per_head, out, p.tokens * Hk, G, d, bf16, st), "linear attention backward launch");
+    if (a.plan != nullptr && S > 0)
+      Q38_HIP(q38::launch_la_gap(out, a.plan, (int)N, S, (shared ? Hk : H) * d * (int)elem_size(dtype), st),
+              "linear attention backward launch");
+    return Q38MOE_OK;
+  };
+  if (dq != nullptr) {
+    a.q = tdo, a.k = tv, a.v = tk, a.dk = dv, a.dv = dk;
+    a.s0 = initial_state, a.s1 = nullptr, a.turned = true;
+    a.intra = a.inter = scale, a.gain = 1.0f, a.lag = 0;
+    Q38_CHECK(pass(dq, dk, false, false));
+  }
+  a.intra = a.gain = scale, a.inter = 1.0f, a.lag = 1;
+  a.s0 = d_final_state;
+  if (dk_out != nullptr) {
+    a.q = tv, a.k = tdo, a.v = tq, a.dk = dv, a.dv = dk;
+    a.s1 = nullptr, a.turned = true;
+    Q38_CHECK(pass(dk_out, dk, true, true));
+  }
+  if (dv_out != nullptr || (p.tokens == 0 && d_initial_state != nullptr)) {
+    a.q = tk, a.k = tq, a.v = tdo, a.dk = dk, a.dv = dv;
+    a.s1 = d_initial_state, a.turned = false;
+    Q38_CHECK(pass(dv_out, dv, true, true));
+  } else if (d_initial_state != nullptr) {
+    return fail(Q38MOE_EINVAL, "the initial state's gradient comes with dv");
+  }
+  return Q38MOE_OK;
+}
+
+int q38moe_linear_attention_step(const void* q, const void* k, const void* v, const int64_t* strides, const float* log_decay,
+                                 float scale, float* state, const int32_t* slots, void* out, int64_t B, int64_t pool, int32_t H,
+                                 int32_t Hk, int32_t dk, int32_t dv, int32_t dtype, void* stream) {
+  g_err[0] = 0;
+  Q38_CHECK(check_linattn(B, 1, H, Hk, dk, dv, dtype));
+  Q38_CHECK(check_strides(strides, 6, dtype));
+  if (B * H * ((dv + 31) / 32) >= (int64_t)1 << 31) return fail(Q38MOE_EINVAL, "too many sequences and heads for one launch");
+  if (pool < 0) return fail(Q38MOE_EINVAL, "pool must be >= 0 (got %lld)", (long long)pool);
+  if (slots == nullptr && B > pool)
+    return fail(Q38MOE_EINVAL, "without slots the pool must hold every sequence (B=%lld, pool=%lld)", (long long)B, (long long)pool);
+  if (B == 0) return Q38MOE_OK;
+  Q38_CHECK(check_ptr(q, "q"));
+  Q38_CHECK(check_ptr(k, "k"));
+  Q38_CHECK(check_ptr(v, "v"));
+  Q38_CHECK(check_ptr(out, "out"));
+  if (pool > 0) Q38_CHECK(check_ptr(state, "state"));
+  if (log_decay == nullptr) return fail(Q38MOE_EINVAL, "log_decay must not be NULL");
+  const int G = H / Hk;
+  const q38::LaStepArgs a = {{q, 0, strides[0], strides[1], 1}, {k, 0, strides[2], strides[3], G}, {v, 0, strides[4], strides[5], G},
+                             log_decay, state, slots, out, scale, B, pool, H, dk, dv};
+  (void)hipGetLastError();
+  Q38_HIP(q38::launch_la_step(a, dtype == Q38MOE_BF16, static_cast<hipStream_t>(stream)), "linear attention step launch");
+  return Q38MOE_OK;
+}
+
 }  // extern "C"

@@ -248,4 +248,63 @@ hipError_t launch_linear_ce_backward(const float* g, bool g_rows, const float* r
                                      const void* targets, bool idx64, int64_t ignore, const float* lse, void* dx,
                                      void* dw, int64_t T, int h, int V, void* ws, bool f32, hipStream_t st);
 
+// Norms and rotation of query and key heads (q38moe_rope.hip). Element strides; q_out and k_out (the gradients, backwards) are
+// [T, H, d] and [T, KV, d]; pos [axes, T], axis_of [rot / 2] or NULL (all the first); wq, wk may be NULL (no norm); tokens is
+// the launch's own.
+struct RopeArgs {
+  const void *q, *k, *wq, *wk, *pos;
+  int64_t q_token, q_head, k_token, k_head, T;
+  const int32_t* axis_of;
+  const float* inv_freq;
+  void *q_out, *k_out;
+  float eps;
+  int H, KV, d, rot, axes, tokens;
+  bool pos64, plus1;
+};
+hipError_t launch_rope(RopeArgs p, bool bf16, hipStream_t st);
+// Blocks of the backward pass, each with 2 d fp32 values of `partial` (NULL: no weights' gradients).
+int rope_backward_blocks(const RopeArgs& p);
+hipError_t launch_rope_backward(RopeArgs p, const void* dyq, const void* dyk, float* partial, void* dwq, void* dwk, bool bf16,
+                                hipStream_t st);
+
+// Linear attention with a decay for each head (q38moe_linattn.hip). Element strides of sequence, token and head; div heads
+// of the call share one of the tensor's.
+struct LaTensor {
+  const void* p;
+  int64_t sb, st, sh;
+  int div;
+};
+// One pass: o_i = intra sum_{j <= i} e^{g (i - j)} (q_i . k_j) v_j + inter e^{g (i + 1 - lag)} S^T q_i and S = e^{g L} S + gain
+// sum_j e^{g (L - 1 - j + lag)} k_j v_j^T, tokens taken forwards or backwards. s0, s1 (may be NULL): the caller's states [N, H, dk, dv],
+// turned: [N, H, dv, dk]. mid: a state per segment of L tokens. plan (packed sequences) or NULL (N sequences of S tokens, nseg
+// segments each).
+struct LaArgs {
+  LaTensor q, k, v;
+  void* o;
+  int64_t ob, ot, oh;
+  const float *g, *s0;
+  float *s1, *mid;
+  const int32_t* plan;
+  float intra, inter, gain;
+  int lag, N, S, H, dk, dv, L, nseg;
+  bool o_f32, turned;
+};
+struct LaStepArgs {
+  LaTensor q, k, v;
+  const float* g;
+  float* state;
+  const int32_t* slots;
+  void* out;
+  float scale;
+  int64_t B, pool;
+  int H, dk, dv;
+};
+int la_segment_tokens(int64_t T, int64_t N, int H);
+int64_t la_padded_state(int dk, int dv);  // elements of a state in mid
+hipError_t launch_la_plan(const int32_t* cu, int32_t* plan, int N, int S, int L, hipStream_t st);
+hipError_t launch_la_gap(void* o, const int32_t* plan, int N, int64_t T, int row_bytes, hipStream_t st);
+hipError_t launch_la(const LaArgs& a, int64_t segs, bool backwards, bool bf16, hipStream_t st);
+hipError_t launch_la_group(const float* x, void* out, int64_t rows, int G, int d, bool bf16, hipStream_t st);
+hipError_t launch_la_step(const LaStepArgs& a, bool bf16, hipStream_t st);
+
 }  // namespace q38

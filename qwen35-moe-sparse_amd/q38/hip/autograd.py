@@ -294,3 +294,83 @@ def combine(rows, topk_w, plan):
     if _recorded(rows, topk_w):
         return HipCombine.apply(rows, topk_w, plan)
     return ops.collect_rows(rows, plan, topk_w)
+
+
+class HipQkNormRope(torch.autograd.Function):
+    """Kept are the operands alone: the backward pass makes the norms and the turns again (q38moe_qk_norm_rope, _backward)."""
+
+    @staticmethod
+    def forward(ctx, q, k, q_norm, k_norm, positions, inv_freq, axes, eps, unit_offset):
+        ctx.save_for_backward(q, k, q_norm, k_norm, positions, inv_freq, axes)
+        ctx.rest = eps, unit_offset
+        return ops.qk_norm_rope(q, k, q_norm, k_norm, positions, inv_freq, axes, eps, unit_offset)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, d_q_out, d_k_out):
+        grads = ops.qk_norm_rope_backward(d_q_out.contiguous(), d_k_out.contiguous(), *ctx.saved_tensors, *ctx.rest,
+                                          need_norms=ctx.needs_input_grad[2:4])
+        return *(g if need else None for g, need in zip(grads, ctx.needs_input_grad)), None, None, None, None, None
+
+
+def qk_norm_rope(q, k, q_norm, k_norm, positions, inv_freq, axes=None, eps=1e-6, unit_offset=True):
+    """RMS norms of query and key heads and their rotation by position, in one pass with autograd: q [..., H, d], k [..., KV, d]
+    (bf16 or fp32, views of a projection as they are where their rows start on 16-byte boundaries), q_norm and k_norm [d] or
+    None (no norm); unit_offset: the norms scale by 1 + weight, else by the weight. The first r = 2 len(inv_freq) features
+    of a head turn, feature i with feature i + r / 2, by the angle position * inv_freq[i] (inv_freq fp32; the product is made in 64
+    bits, so far positions keep their angles). positions: int32 or int64 of q's leading shape, or, with axes (int32
+    [len(inv_freq)], see ``ops.rope_axis_map``), [number of axes, ...] with frequency i turning by axis axes[i]: time, height and
+    width of images and video. fp32 throughout and one rounding. Returns (q, k), contiguous; gradients flow to q, k and the
+    weights. Under bf16 autocast q, k and the weights are cast to bf16."""
+    if _bf16_autocast():
+        q, k, q_norm, k_norm = (t if t is None else t.to(torch.bfloat16) for t in (q, k, q_norm, k_norm))
+    positions = positions.contiguous()
+    if _recorded(*(t for t in (q, k, q_norm, k_norm) if t is not None)):
+        return HipQkNormRope.apply(q, k, q_norm, k_norm, positions, inv_freq, axes, eps, unit_offset)
+    return ops.qk_norm_rope(q, k, q_norm, k_norm, positions, inv_freq, axes, eps, unit_offset)
+
+
+class HipLinearAttention(torch.autograd.Function):
+    """Kept are the operands; the backward pass makes the states again (q38moe_linear_attention_forward, _backward)."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, log_decay, scale, initial_state, cu_seqlens, return_state):
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(q, k, v, log_decay, initial_state, cu_seqlens)
+        ctx.scale = scale
+        return ops.linear_attention(q, k, v, log_decay, scale, initial_state, cu_seqlens, return_state)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, d_out, d_state):
+        q, k, v, g, S0, cu = ctx.saved_tensors
+        needs = ctx.needs_input_grad
+        if (d_out is None and d_state is None) or not any(needs):
+            return (None,) * 8
+        d_out = (torch.zeros(*q.shape[:3], v.shape[3], dtype=q.dtype, device=q.device) if d_out is None
+                 else d_out.contiguous())
+        dq, dk, dv, ds = ops.linear_attention_backward(d_out, None if d_state is None else d_state.contiguous(), q, k, v, g,
+                                                       ctx.scale, S0, cu, need_state=needs[5])
+        return (dq if needs[0] else None, dk if needs[1] else None, dv if needs[2] else None, None, None, ds, None, None)
+
+
+def linear_attention(q, k, v, log_decay, scale=None, initial_state=None, cu_seqlens=None, return_state=False):
+    """Linear attention with a decay for each head, with autograd: S_t = e^log_decay[h] S_(t-1) + k_t v_t^T and out_t = scale S_t^T
+    q_t for q [B,S,H,dk], k [B,S,Hk,dk], v [B,S,Hk,dv] (bf16 or fp32, views of a projection as they are where their rows start
+    on 16-byte boundaries), log_decay fp32 [H]; query head h reads key and value head h // (H // Hk). dk and dv are multiples of
+    8 up to 128, scale is dk^-1/2 unless given. initial_state fp32 [N,H,dk,dv] (zero unless given) is what a sequence goes on
+    from, and with return_state the states after the last tokens come back: (out [B,S,H,dv], state or None). N is B, or, with
+    cu_seqlens (int32 [N+1] on the GPU, B = 1), the row holds N sequences one behind the other, n being the tokens
+    cu_seqlens[n] to cu_seqlens[n+1]; tokens of no sequence come out zero, a sequence without tokens keeps its state. States are fp32
+    throughout; bf16 operands of the matrix units are rounded once (scores, and the state as queries read it). Gradients flow
+    to q, k, v and initial_state, not to log_decay. ``ops.linear_attention_step`` goes on one token at a time. A NaN or infinity
+    at a token may reach up to 63 tokens before it. Under bf16 autocast q, k and v are cast to bf16."""
+    if log_decay.requires_grad and torch.is_grad_enabled():
+        raise ValueError("log_decay has no gradient here: pass log_decay.detach()")
+    if _bf16_autocast():
+        q, k, v = (t.to(torch.bfloat16) for t in (q, k, v))
+    if initial_state is not None:
+        initial_state = initial_state.contiguous()
+    if _recorded(*((q, k, v) if initial_state is None else (q, k, v, initial_state))):
+        return HipLinearAttention.apply(q, k, v, log_decay, scale, initial_state, cu_seqlens, return_state)
+    return ops.linear_attention(q, k, v, log_decay, scale, initial_state, cu_seqlens, return_state)

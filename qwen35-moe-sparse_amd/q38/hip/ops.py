@@ -1153,3 +1153,286 @@ def _collect_rows(rows, plan, w, pw):
                                       out.data_ptr(), T, h, plan.experts, k, _DTYPES[dt], _raw_stream(dev.index)),
               "q38moe_collect_rows")
     return out
+
+
+# ---- a token mixer with a carried state: normed and rotated heads, linear attention, its step ----------------------
+
+def _rows16(t, lead):
+    """t with its first ``lead`` dimensions in place, or a copy of it, whose last dimension is dense and whose rows start on
+    16-byte boundaries."""
+    size = t.element_size()
+    if t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(s * size % 16 == 0 for s in t.stride()[:lead]):
+        return t
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def _heads(t, name, dt, dev, dims=None):
+    if not isinstance(t, torch.Tensor) or t.dtype != dt:
+        raise TypeError(f"{name} must be {dt}, got {getattr(t, 'dtype', type(t))}")
+    if t.device != dev:
+        raise RuntimeError(f"{name} must be on {dev}, got {t.device}")
+    if dims is not None and t.dim() != dims:
+        raise ValueError(f"{name} must have {dims} dims, got shape {tuple(t.shape)}")
+    return t
+
+
+def _head_dim(d, name, most):
+    if d < 8 or d > most or d % 8:
+        raise ValueError(f"{name} must be a multiple of 8 up to {most}, got {d}")
+
+
+def _on_gpu(t, name):
+    if t.device.type != "cuda":
+        raise RuntimeError(f"{name} must be a CUDA/HIP tensor")
+    return t.device
+
+
+def rope_axis_map(sections, interleaved=True, device=None):
+    """The axis of every rotated frequency, int32 [sum(sections)], for ``qk_norm_rope``: sections[a] frequencies turn by the
+    positions of axis a. interleaved: the axes take turns (frequency i belongs to axis i % n while that axis has
+    frequencies left, to axis 0 otherwise); else one section follows the other."""
+    sections = [int(c) for c in sections]
+    n, half = len(sections), sum(sections)
+    if not 1 <= n <= 4 or min(sections) < 0:
+        raise ValueError(f"sections must be one to four counts, got {sections}")
+    if interleaved:
+        found = [i % n if i < n * sections[i % n] else 0 for i in range(half)]
+    else:
+        found = [a for a, c in enumerate(sections) for _ in range(c)]
+    if [found.count(a) for a in range(n)] != sections:
+        raise ValueError(f"sections {sections} cannot be interleaved")
+    return torch.tensor(found, dtype=torch.int32, device=device)
+
+
+class _Rope:
+    """The checked operands of a rotation: q [T,H,d] and k [T,KV,d] (views where they can be), the rest of the C call."""
+
+    __slots__ = ("q", "k", "T", "H", "KV", "d", "rot", "dt", "dev", "strides", "head", "tail")
+
+    def __init__(self, q, k, q_norm, k_norm, positions, inv_freq, axes, eps, unit_offset):
+        dt = self.dt = _fdt(q, "q")
+        dev = self.dev = _on_gpu(q, "q")
+        _heads(k, "k", dt, dev)
+        if q.dim() < 2 or k.dim() != q.dim() or k.shape[:-2] != q.shape[:-2] or k.shape[-1] != q.shape[-1]:
+            raise ValueError(f"q [..., H, d] and k [..., KV, d] do not match: {tuple(q.shape)} and {tuple(k.shape)}")
+        lead = q.shape[:-2]
+        H, d = q.shape[-2:]
+        KV = k.shape[-2]
+        _head_dim(d, "the head width", 256)
+        self.T, self.H, self.KV, self.d = math.prod(lead), H, KV, d
+        for w, name in ((q_norm, "q_norm"), (k_norm, "k_norm")):
+            if w is not None:
+                _same(w, name, dt, (d,))
+                _heads(w, name, dt, dev)
+        _need(inv_freq, "inv_freq", dtype=torch.float32, ndim=1)
+        rot = self.rot = 2 * inv_freq.shape[0]
+        if rot > d or rot % 8:
+            raise ValueError(f"inv_freq must hold a multiple of 4 frequencies up to {d // 2}, got {inv_freq.shape[0]}")
+        _need(positions, "positions", dtype=None)
+        if positions.dtype not in (torch.int32, torch.int64):
+            raise TypeError(f"positions must be int32 or int64, got {positions.dtype}")
+        n = 1
+        if axes is None:
+            if positions.shape != lead:
+                raise ValueError(f"positions must be {tuple(lead)}, got {tuple(positions.shape)}")
+        else:
+            _same(axes, "axes", torch.int32, (rot // 2,))
+            if positions.dim() != q.dim() - 1 or positions.shape[1:] != lead or not 1 <= positions.shape[0] <= 4:
+                raise ValueError(f"positions must be [1 to 4 axes, {', '.join(map(str, lead))}], got {tuple(positions.shape)}")
+            n = positions.shape[0]
+        if inv_freq.device != dev or positions.device != dev or (axes is not None and axes.device != dev):
+            raise RuntimeError("q, positions, inv_freq and axes must be on one device")
+        q, k = (_rows16(t.reshape(self.T, t.shape[-2], d), 2) for t in (q, k))
+        self.q, self.k = q, k
+        self.strides = (ctypes.c_int64 * 4)(q.stride(0), q.stride(1), k.stride(0), k.stride(1))
+        self.head = (q.data_ptr(), k.data_ptr(), self.strides, None if q_norm is None else q_norm.data_ptr(),
+                     None if k_norm is None else k_norm.data_ptr(), bool(unit_offset), positions.data_ptr(),
+                     positions.dtype == torch.int64, None if axes is None else axes.data_ptr(), n, inv_freq.data_ptr())
+        self.tail = (self.T, H, KV, d, rot, eps)
+
+
+def _norm_weight(w):
+    """A norm's weight (or None) as the kernels take it."""
+    return w if w is None or (w.is_contiguous() and w.data_ptr() % 16 == 0) else w.contiguous().clone()
+
+
+def qk_norm_rope(q, k, q_norm, k_norm, positions, inv_freq, axes=None, eps=1e-6, unit_offset=True):
+    """RMS norm of every query and key head and rotation by position in one pass (q38moe_qk_norm_rope): see
+    ``autograd.qk_norm_rope``. Returns contiguous (q [..., H, d], k [..., KV, d])."""
+    q_norm, k_norm = _norm_weight(q_norm), _norm_weight(k_norm)
+    p = _Rope(q, k, q_norm, k_norm, positions, inv_freq, axes, eps, unit_offset)
+    qo, ko = torch.empty(q.shape, dtype=p.dt, device=p.dev), torch.empty(k.shape, dtype=p.dt, device=p.dev)
+    with _on(p.dev):
+        check(lib.q38moe_qk_norm_rope(*p.head, qo.data_ptr(), ko.data_ptr(), *p.tail, _DTYPES[p.dt],
+                                      _raw_stream(p.dev.index)), "q38moe_qk_norm_rope")
+    return qo, ko
+
+
+@functools.lru_cache(maxsize=512)
+def _rope_workspace_bytes(T, H, KV, d, rot, device):
+    n = ctypes.c_size_t()
+    check(lib.q38moe_qk_norm_rope_workspace_bytes(T, H, KV, d, rot, ctypes.byref(n)),
+          "q38moe_qk_norm_rope_workspace_bytes")
+    return n.value
+
+
+def qk_norm_rope_backward(d_q_out, d_k_out, q, k, q_norm, k_norm, positions, inv_freq, axes=None, eps=1e-6,
+                          unit_offset=True, need_norms=(True, True)):
+    """Gradients (dq, dk, d q_norm, d k_norm) of ``qk_norm_rope``'s outputs for theirs; the weights' are None where there is no
+    weight or need_norms says so."""
+    q_norm, k_norm = _norm_weight(q_norm), _norm_weight(k_norm)
+    p = _Rope(q, k, q_norm, k_norm, positions, inv_freq, axes, eps, unit_offset)
+    for g, t, name in ((d_q_out, q, "d_q_out"), (d_k_out, k, "d_k_out")):
+        _heads(_same(g, name, p.dt, t.shape), name, p.dt, p.dev)
+    d_q_out, d_k_out = (g if g.data_ptr() % 16 == 0 else g.clone() for g in (d_q_out, d_k_out))
+    dq, dk = torch.empty(q.shape, dtype=p.dt, device=p.dev), torch.empty(k.shape, dtype=p.dt, device=p.dev)
+    dwq = torch.empty_like(q_norm) if q_norm is not None and need_norms[0] else None
+    dwk = torch.empty_like(k_norm) if k_norm is not None and need_norms[1] else None
+    with _on(p.dev):
+        ws, n = None, 0
+        if dwq is not None or dwk is not None:
+            n = _rope_workspace_bytes(p.T, p.H, p.KV, p.d, p.rot, p.dev)
+            ws = torch.empty(n, dtype=torch.uint8, device=p.dev)
+        check(lib.q38moe_qk_norm_rope_backward(d_q_out.data_ptr(), d_k_out.data_ptr(), *p.head, dq.data_ptr(), dk.data_ptr(),
+                                               None if dwq is None else dwq.data_ptr(),
+                                               None if dwk is None else dwk.data_ptr(), *p.tail,
+                                               None if ws is None else ws.data_ptr(), n, _DTYPES[p.dt],
+                                               _raw_stream(p.dev.index)), "q38moe_qk_norm_rope_backward")
+    return dq, dk, dwq, dwk
+
+
+class _LinearAttention:
+    """The checked operands of a linear attention call."""
+
+    __slots__ = ("q", "k", "v", "g", "cu", "shape", "dt", "dev", "scale", "strides", "S0", "packed")
+
+    def __init__(self, q, k, v, log_decay, scale, initial_state, cu_seqlens):
+        dt = self.dt = _fdt(q, "q")
+        dev = self.dev = _on_gpu(q, "q")
+        _heads(q, "q", dt, dev, 4)
+        _heads(k, "k", dt, dev, 4)
+        _heads(v, "v", dt, dev, 4)
+        B, S, H, dk = q.shape
+        Hk, dv = v.shape[2:]
+        if k.shape != (B, S, Hk, dk) or v.shape[:2] != (B, S) or Hk < 1 or H % Hk:
+            raise ValueError(f"q [B,S,H,dk], k [B,S,Hk,dk], v [B,S,Hk,dv] do not match: {tuple(q.shape)}, {tuple(k.shape)}, "
+                             f"{tuple(v.shape)}")
+        _head_dim(dk, "dk", 128)
+        _head_dim(dv, "dv", 128)
+        self.packed = cu_seqlens is not None
+        N = B
+        if self.packed:
+            _heads(_need(cu_seqlens, "cu_seqlens", dtype=torch.int32, ndim=1), "cu_seqlens", torch.int32, dev)
+            N = cu_seqlens.shape[0] - 1
+            if B != 1 or N < 1:
+                raise ValueError(f"packed sequences are one row of tokens and at least two offsets, got {B} rows and "
+                                 f"{cu_seqlens.shape[0]} offsets")
+        self.g, self.cu = _decay(log_decay, H, dev), cu_seqlens
+        self.scale = dk ** -0.5 if scale is None else float(scale)
+        self.shape = (N, S, H, Hk, dk, dv)
+        self.S0 = _state(initial_state, "initial_state", (N, H, dk, dv), dev)
+        q, k, v = self.q, self.k, self.v = _rows16(q, 3), _rows16(k, 3), _rows16(v, 3)
+        self.strides = (ctypes.c_int64 * 9)(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3])
+
+    def call(self):
+        return (self.q.data_ptr(), self.k.data_ptr(), self.v.data_ptr(), self.strides, self.g.data_ptr(), self.scale,
+                None if self.S0 is None else self.S0.data_ptr(), self.cu.data_ptr() if self.packed else None)
+
+    def workspace(self, backward):
+        n = _linear_attention_workspace_bytes(*self.shape, self.packed, backward, self.dev)
+        return torch.empty(n, dtype=torch.uint8, device=self.dev)
+
+
+def _decay(log_decay, H, dev):
+    _same(log_decay, "log_decay", torch.float32, (H,))
+    return _heads(log_decay, "log_decay", torch.float32, dev)
+
+
+def _state(t, name, shape, dev):
+    return None if t is None else _heads(_same(t, name, torch.float32, shape), name, torch.float32, dev)
+
+
+@functools.lru_cache(maxsize=512)
+def _linear_attention_workspace_bytes(N, S, H, Hk, dk, dv, packed, backward, device):
+    n = ctypes.c_size_t()
+    check(lib.q38moe_linear_attention_workspace_bytes(N, S, H, Hk, dk, dv, packed, backward, ctypes.byref(n)),
+          "q38moe_linear_attention_workspace_bytes")
+    return n.value
+
+
+def linear_attention(q, k, v, log_decay, scale=None, initial_state=None, cu_seqlens=None, return_state=False):
+    """Linear attention with a decay for each head (q38moe_linear_attention_forward): see ``autograd.linear_attention``.
+    Returns (out [B,S,H,dv], final state [N,H,dk,dv] fp32 or None)."""
+    a = _LinearAttention(q, k, v, log_decay, scale, initial_state, cu_seqlens)
+    N, S, H, _, dk, dv = a.shape
+    out = torch.empty(q.shape[0], S, H, dv, dtype=a.dt, device=a.dev)
+    state = torch.empty(N, H, dk, dv, dtype=torch.float32, device=a.dev) if return_state else None
+    with _on(a.dev):
+        ws = a.workspace(False)
+        check(lib.q38moe_linear_attention_forward(*a.call(), out.data_ptr(), None if state is None else state.data_ptr(),
+                                                  *a.shape, ws.data_ptr(), ws.numel(), _DTYPES[a.dt],
+                                                  _raw_stream(a.dev.index)), "q38moe_linear_attention_forward")
+    return out, state
+
+
+def linear_attention_backward(d_out, d_final_state, q, k, v, log_decay, scale=None, initial_state=None, cu_seqlens=None,
+                              need_state=False):
+    """Gradients (dq, dk, dv, d initial_state or None) of ``linear_attention`` for those of its output and its final state
+    (None: zero)."""
+    a = _LinearAttention(q, k, v, log_decay, scale, initial_state, cu_seqlens)
+    N, S, H, Hk, dk, dv = a.shape
+    B = q.shape[0]
+    _heads(_same(d_out, "d_out", a.dt, (B, S, H, dv)), "d_out", a.dt, a.dev)
+    d_out = d_out if d_out.data_ptr() % 16 == 0 else d_out.clone()
+    _state(d_final_state, "d_final_state", (N, H, dk, dv), a.dev)
+    dq, dk_, dv_ = (torch.empty(B, S, h, d, dtype=a.dt, device=a.dev) for h, d in ((H, dk), (Hk, dk), (Hk, dv)))
+    ds = torch.empty(N, H, dk, dv, dtype=torch.float32, device=a.dev) if need_state else None
+    with _on(a.dev):
+        ws = a.workspace(True)
+        check(lib.q38moe_linear_attention_backward(d_out.data_ptr(),
+                                                   None if d_final_state is None else d_final_state.data_ptr(), *a.call(),
+                                                   dq.data_ptr(), dk_.data_ptr(), dv_.data_ptr(),
+                                                   None if ds is None else ds.data_ptr(), *a.shape, ws.data_ptr(),
+                                                   ws.numel(), _DTYPES[a.dt], _raw_stream(a.dev.index)),
+              "q38moe_linear_attention_backward")
+    return dq, dk_, dv_, ds
+
+
+def linear_attention_step(q, k, v, state, log_decay, scale=None, slots=None):
+    """One token of every sequence through ``linear_attention`` (q38moe_linear_attention_step): q [B,H,dk], k [B,Hk,dk], v
+    [B,Hk,dv] (bf16 or fp32), the states [pool,H,dk,dv] (fp32, contiguous) updated in place. Sequence b has the state
+    slots[b] (int32 [B]; without slots the state b); a slot outside the pool is none: nothing is updated and the output is zero.
+    No slot may occur twice. scale: dk^-1/2 unless given. Returns out [B,H,dv]; no gradients."""
+    dt = _fdt(q, "q")
+    dev = _on_gpu(q, "q")
+    _heads(q, "q", dt, dev, 3)
+    _heads(k, "k", dt, dev, 3)
+    _heads(v, "v", dt, dev, 3)
+    B, H, dk = q.shape
+    Hk, dv = v.shape[1:]
+    if k.shape != (B, Hk, dk) or v.shape[0] != B or Hk < 1 or H % Hk:
+        raise ValueError(f"q [B,H,dk], k [B,Hk,dk], v [B,Hk,dv] do not match: {tuple(q.shape)}, {tuple(k.shape)}, "
+                         f"{tuple(v.shape)}")
+    _head_dim(dk, "dk", 128)
+    _head_dim(dv, "dv", 128)
+    _heads(_need(state, "state", dtype=torch.float32, ndim=4), "state", torch.float32, dev)
+    pool = state.shape[0]
+    if state.shape[1:] != (H, dk, dv):
+        raise ValueError(f"state must be [pool,{H},{dk},{dv}], got {tuple(state.shape)}")
+    if slots is not None:
+        _heads(_same(slots, "slots", torch.int32, (B,)), "slots", torch.int32, dev)
+    elif pool < B:
+        raise ValueError(f"without slots state must hold {B} sequences, got {pool}")
+    g = _decay(log_decay, H, dev)
+    q, k, v = _rows16(q, 2), _rows16(k, 2), _rows16(v, 2)
+    out = torch.empty(B, H, dv, dtype=dt, device=dev)
+    strides = (ctypes.c_int64 * 6)(*q.stride()[:2], *k.stride()[:2], *v.stride()[:2])
+    with _on(dev):
+        check(lib.q38moe_linear_attention_step(q.data_ptr(), k.data_ptr(), v.data_ptr(), strides, g.data_ptr(),
+                                               dk ** -0.5 if scale is None else float(scale), state.data_ptr(),
+                                               None if slots is None else slots.data_ptr(), out.data_ptr(), B, pool, H, Hk,
+                                               dk, dv, _DTYPES[dt], _raw_stream(dev.index)),
+              "q38moe_linear_attention_step")
+    torch.autograd.graph.increment_version(state)
+    return out
