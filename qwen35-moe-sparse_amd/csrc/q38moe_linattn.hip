@@ -37,9 +37,11 @@ __device__ __forceinline__ f32x4_t mfma16x16x4(float a, float b, f32x4_t c) {
   return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
 }
 
-// Byte of 16-byte column `col` of row `row` in a tile of rows of `bytes` bytes: the low three bits of the column are mixed with
-// the row's, so that 8 rows' same column lies in 8 different bank groups.
-__device__ __forceinline__ int la_at(int row, int col, int bytes) { return row * bytes + ((col ^ (row & 7)) << 4); }
+// Byte of 16-byte column `col` of row `row` in a tile of rows of `bytes` bytes. The low three bits of the column are mixed with
+// the row's, so that 8 rows' same column, and 4 rows' same pair of columns, lie in different banks.
+__device__ __forceinline__ int la_at(int row, int col, int bytes) {
+  return row * bytes + ((col ^ (((row & 3) << 1) | ((row >> 2) & 1))) << 4);
+}
 
 // e^{g n} to 24 + 24 bits.
 __device__ __forceinline__ float2 la_decay2(double g, int64_t n) {
@@ -150,250 +152,266 @@ __global__ __launch_bounds__(256) void la_gap_kernel(void* o, const int32_t* __r
   }
 }
 
-// 64 rows of up to D features on their way from memory to LDS, zero behind the last row and the last feature.
-template <int BYTES>  // of a row of the tile
+// 64 rows of features on their way from memory to LDS, zero behind the last row and the last feature.
+template <int BYTES, int THREADS>  // of a row of the tile
 struct LaStage {
-  static constexpr int COLS = BYTES / 16, N = LA_C * COLS / 256;
+  static constexpr int COLS = BYTES / 16, N = LA_C * COLS / THREADS, ROWS = THREADS / COLS;
   u32x4_t r[N];
-  template <bool REV>
-  __device__ __forceinline__ void load(const uint8_t* base, int64_t stride, int len, int j0, int rows, int bytes) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int c = (int)threadIdx.x + 256 * i, row = c / COLS, col = c % COLS, j = j0 + row;
-      r[i] = u32x4_t{0, 0, 0, 0};
-      if (row < rows && 16 * col < bytes) r[i] = ld16(base + (int64_t)(REV ? len - 1 - j : j) * stride + 16 * col);
-    }
+  const uint8_t* at;  // the thread's first piece of the next 64 rows
+  int64_t step;       // bytes from row to row, negative backwards
+  __device__ __forceinline__ void start(const uint8_t* base, int64_t stride, int j0) {
+    step = stride;
+    at = base + (j0 + (int)threadIdx.x / COLS) * stride + 16 * ((int)threadIdx.x % COLS);
   }
-  __device__ __forceinline__ void store(uint8_t* lds) const {
+  __device__ __forceinline__ void load(int tid, int rows, int bytes) {
+    const int row = tid / COLS, col = tid % COLS;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int c = (int)threadIdx.x + 256 * i;
-      *reinterpret_cast<u32x4_t*>(lds + la_at(c / COLS, c % COLS, BYTES)) = r[i];
+      r[i] = u32x4_t{0, 0, 0, 0};
+      if (row + ROWS * i < rows && 16 * col < bytes) r[i] = ld16(at + ROWS * i * step);
+    }
+    at += LA_C * step;
+  }
+  __device__ __forceinline__ void store(int tid, uint8_t* lds) const {
+    const int row = tid / COLS, col = tid % COLS;
+#pragma unroll
+    for (int i = 0; i < N; ++i) *reinterpret_cast<u32x4_t*>(lds + la_at(row + ROWS * i, col, BYTES)) = r[i];
+  }
+  // bf16: column 4 u + m of the tile gets features 32 u + 4 m .. and 32 u + 16 + 4 m .. (4 each).
+  __device__ __forceinline__ void store_paired(int tid, uint8_t* lds) const {
+    const int row = tid / COLS, col = tid % COLS, m = (col & ~3) + 2 * (col & 1), half = 4 * (col & 2);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      *reinterpret_cast<uint2*>(lds + la_at(row + ROWS * i, m, BYTES) + half) = make_uint2(r[i][0], r[i][1]);
+      *reinterpret_cast<uint2*>(lds + la_at(row + ROWS * i, m + 1, BYTES) + half) = make_uint2(r[i][2], r[i][3]);
     }
   }
 };
 
-// acc += rows of the tile (16 of them, the lane's is `row`) times the lane's column q, contiguous features.
-template <bool BF16, int BYTES>
-__device__ __forceinline__ f32x4_t la_dot(const uint8_t* tile, int row, int lq, const u32x4_t* q, f32x4_t acc) {
-#pragma unroll
-  for (int s = 0; s < BYTES / 64; ++s) {
-    const u32x4_t x = *reinterpret_cast<const u32x4_t*>(tile + la_at(row, 4 * s + lq, BYTES));
-    if constexpr (BF16) {
-      acc = mfma16x16x32(x, q[s], acc);
-    } else {
-      const f32x4_t xf = __builtin_bit_cast(f32x4_t, x), qf = __builtin_bit_cast(f32x4_t, q[s]);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) acc = mfma16x16x4(xf[e], qf[e], acc);
-    }
-  }
-  return acc;
-}
-
-// bf16: features 16 t .. of tokens 32 u + {4 lq + e, 16 + 4 lq + e} of a row-major tile, feature 16 t + lr in this lane.
+// Two pieces of 4 tokens (rows `row` + {0, 16}) of one feature, transposed out of a row-major bf16 tile: the lane addresses 4
+// features at byte `at` of its row (lr / 4 of the 4 rows) and gets feature lr of the 16 that its group addresses.
 template <int BYTES>
-__device__ __forceinline__ u32x4_t la_column(const uint8_t* tile, int u, int t, int lr, int lq) {
-  const int row = 32 * u + 4 * lq + (lr >> 2);
-  const uint8_t* at = tile + la_at(row, 2 * t + ((lr & 3) >> 1), BYTES) + 8 * (lr & 1);
+__device__ __forceinline__ u32x4_t la_column(const uint8_t* at) {
   const uint2 x = la_read_tr(at), y = la_read_tr(at + 16 * BYTES);
   return u32x4_t{x.x, x.y, y.x, y.y};
 }
-// fp32: feature 16 t + lr of token `row`.
-template <int BYTES>
-__device__ __forceinline__ float la_value(const uint8_t* tile, int row, int t, int lr) {
-  return *reinterpret_cast<const float*>(tile + la_at(row, 4 * t + (lr >> 2), BYTES) + 4 * (lr & 3));
+
+__device__ __forceinline__ u32x4_t la_pack(f32x4_t x, f32x4_t y) {
+  return u32x4_t{pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3])};
 }
 
-// One segment of one head. Wave w has queries 16 w .. of each chunk (scores as [key, query] tiles, outputs as [feature,
-// query] tiles, so that scores go from accumulators to operands within a lane) and the state's columns w DV / 4 .. .
-template <bool BF16, int DK, int DV, bool REV, bool OUT>
-__global__ __launch_bounds__(256) void la_kernel(LaArgs a) {
-  constexpr int ES = BF16 ? 2 : 4, KB = DK * ES, VB = DV * ES, NA = DK / 16, NB = DV / 64, NT = DV / 16;
+// x, but not as the compiler knows it: what follows from it is made again in every chunk rather than kept in registers that
+// the loop lacks.
+__device__ __forceinline__ int afresh(int x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
+
+// Waves on a SIMD that the LDS of la_kernel's workgroups allows, at most 4: the limit of its registers.
+constexpr int la_waves(bool bf16, int dk, int dv, bool out) {
+  return bf16 ? (out && dk == 128 && dv == 64 ? 3 : 4) : out && dk == 128 && dv == 64 ? 1 : 2;
+}
+
+// One segment of one head; DV / 16 waves. Wave w has columns 16 w .. of the state and of the outputs for all 64 queries of a
+// chunk (outputs as [column, query] tiles), and some of the scores' six [32 keys, 16 queries] units, which go through LDS. The
+// state stays in accumulators; rounded, they are the operand that queries read as they lie, since an accumulator's lane holds 4
+// rows of a column and an operand's lane 8 of one: the queries' features are stored in the order that this gives (store_paired).
+// A column's tokens come out of the transposing LDS read in the same order, once for the outputs and for the state.
+// Two barriers a chunk: tiles and scores are read behind one, scores and the next tiles written behind the other.
+template <bool BF16, int DK, int DV, int PARTS, bool REV, bool OUT>
+__global__ __launch_bounds__(4 * DV, la_waves(BF16, DK, DV, OUT)) void la_kernel(LaArgs a) {
+  constexpr int ES = BF16 ? 2 : 4, KB = DK * ES, VB = DV * ES, NA = DK / 16, W = DV / 16, THREADS = 4 * DV;
   __shared__ __attribute__((aligned(16))) uint8_t Ks[LA_C * KB];
   __shared__ __attribute__((aligned(16))) uint8_t Vs[LA_C * VB];
-  __shared__ __attribute__((aligned(16))) uint8_t Ss[OUT ? DV * KB : 16];  // the state as operand: [dv][dk]
-  __shared__ float tab[LA_C + 1];
+  __shared__ __attribute__((aligned(16))) uint8_t Qs[OUT ? LA_C * KB : 16];
+  __shared__ __attribute__((aligned(16))) uint8_t Ps[OUT ? 16 * LA_C * 4 * ES : 16];  // [query tile][key tiles][lane]
+  __shared__ float2 tab[LA_C + 1];  // e^{g n} to 48 bits
+  __shared__ float put[2 * LA_C];   // what a token adds to the state with: of a chunk's 64, then zeros
   const int tid = threadIdx.x, lane = tid & 63, lr = lane & 15, lq = lane >> 4;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int seg = (int)(blockIdx.x / a.H), h = (int)(blockIdx.x % a.H);
   const LaPlace p = la_place<OUT>(a, seg);
   if (!p.there) return;
   const double g = (double)a.g[h];
-  if (tid <= LA_C) tab[tid] = la_decay2(g, tid).x;
-  const float2 whole = la_decay2(g, LA_C);
+  if (tid <= LA_C) tab[tid] = la_decay2(g, tid);
+  if (tid < 2 * LA_C) put[tid] = tid < LA_C ? a.gain * la_decay2(g, LA_C - 1 - tid + a.lag).x : 0.0f;
   const int64_t first = a.plan == nullptr ? 0 : p.start;
   const int64_t sb = a.plan == nullptr ? p.seq : 0;
-  auto at = [&](const LaTensor& t) {
-    return static_cast<const uint8_t*>(t.p) + ES * (sb * t.sb + first * t.st + (int64_t)(h / t.div) * t.sh);
+  auto start = [&](auto& stage, const LaTensor& t, int j0) {
+    const uint8_t* base = static_cast<const uint8_t*>(t.p) + ES * (sb * t.sb + first * t.st + (int64_t)(h / t.div) * t.sh);
+    if (REV) stage.start(base + (int64_t)(p.len - 1) * t.st * ES, -t.st * ES, j0);
+    else stage.start(base, t.st * ES, j0);
   };
-  const uint8_t *qp = at(a.q), *kp = at(a.k), *vp = at(a.v);
-  const int64_t qs = a.q.st * ES, ks = a.k.st * ES, vs = a.v.st * ES;
   const int begin = p.s * a.L, end = min(p.len, begin + a.L);
   const bool last = p.s == p.nseg - 1, keep = !OUT || (last && a.s1 != nullptr);
 
-  // The state the segment starts with.
-  f32x4_t S[NA][NB];
+  f32x4_t S[NA];  // rows 16 i + 4 lq .., column 16 w + lr
   const int64_t slot = la_slot(a, p.seq) + p.s;
-  auto mid = [&](int64_t s, int i, int b) {
-    return reinterpret_cast<f32x4_t*>(a.mid + (s * a.H + h) * (DK * DV) + (((w * NA + i) * NB + b) * 64 + lane) * 4);
+  auto mid = [&](int64_t s, int i) {
+    return reinterpret_cast<f32x4_t*>(a.mid + (s * a.H + h) * (DK * DV) + ((w * NA + i) * 64 + lane) * 4);
   };
-  auto user = [&](int i, int b, int e) {  // of the caller's state
-    const int dk = 16 * i + 4 * lq + e, dv = 16 * (w * NB + b) + lr;
-    return dk < a.dk && dv < a.dv ? ((int64_t)p.seq * a.H + h) * a.dk * a.dv + (a.turned ? dv * a.dk + dk : dk * a.dv + dv) : -1;
-  };
+  // Row and column of the caller's state, whose rows may lie as columns.
+  const int64_t user = ((int64_t)p.seq * a.H + h) * a.dk * a.dv + (16 * w + lr) * (a.turned ? a.dk : 1);
+  const int user_row = a.turned ? 1 : a.dv;
 #pragma unroll
-  for (int i = 0; i < NA; ++i)
+  for (int i = 0; i < NA; ++i) {
+    S[i] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    if (!OUT) continue;
+    if (p.s > 0) {
+      S[i] = *mid(slot - 1, i);
+    } else if (a.s0 != nullptr) {
 #pragma unroll
-    for (int b = 0; b < NB; ++b) {
-      S[i][b] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-      if (!OUT) continue;
-      if (p.s > 0) {
-        S[i][b] = *mid(slot - 1, i, b);
-      } else if (a.s0 != nullptr) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int64_t u = user(i, b, e);
-          if (u >= 0) S[i][b][e] = a.s0[u];
-        }
+      for (int e = 0; e < 4; ++e) {
+        const int row = 16 * i + 4 * lq + e;
+        if (row < a.dk && 16 * w + lr < a.dv) S[i][e] = a.s0[user + row * user_row];
       }
     }
-  auto publish = [&]() {
-#pragma unroll
-    for (int i = 0; i < NA; ++i)
-#pragma unroll
-      for (int b = 0; b < NB; ++b) {
-        const int row = 16 * (w * NB + b) + lr;
-        if constexpr (BF16) {
-          uint8_t* to = Ss + la_at(row, 2 * i + (lq >> 1), KB) + 8 * (lq & 1);
-          *reinterpret_cast<uint2*>(to) = make_uint2(pack_bf16x2(S[i][b][0], S[i][b][1]), pack_bf16x2(S[i][b][2], S[i][b][3]));
-        } else {
-          *reinterpret_cast<f32x4_t*>(Ss + la_at(row, 4 * i + lq, KB)) = S[i][b];
-        }
-      }
+  }
+  LaStage<KB, THREADS> kst, qst;
+  LaStage<VB, THREADS> vst;
+  start(kst, a.k, begin);
+  start(vst, a.v, begin);
+  if (OUT) start(qst, a.q, begin);
+  auto fetch = [&](int rows) {
+    const int tid = afresh((int)threadIdx.x);
+    kst.load(tid, rows, a.dk * ES);
+    vst.load(tid, rows, a.dv * ES);
+    if (OUT) qst.load(tid, rows, a.dk * ES);
   };
-  LaStage<KB> kst;
-  LaStage<VB> vst;
-  u32x4_t q[KB / 64], qn[KB / 64];
-  auto fetch = [&](int j0) {
-    const int rows = min(LA_C, end - j0);
-    kst.template load<REV>(kp, ks, p.len, j0, rows, a.dk * ES);
-    vst.template load<REV>(vp, vs, p.len, j0, rows, a.dv * ES);
-    if (OUT) {
-      const int j = j0 + 16 * w + lr;
-#pragma unroll
-      for (int s = 0; s < KB / 64; ++s) {
-        qn[s] = u32x4_t{0, 0, 0, 0};
-        if (j < end && 64 * s + 16 * lq < a.dk * ES)
-          qn[s] = ld16(qp + (int64_t)(REV ? p.len - 1 - j : j) * qs + 64 * s + 16 * lq);
-      }
+  auto stage = [&]() {
+    const int tid = afresh((int)threadIdx.x);
+    kst.store(tid, Ks);
+    vst.store(tid, Vs);
+    if constexpr (OUT) {
+      if constexpr (BF16) qst.store_paired(tid, Qs);
+      else qst.store(tid, Qs);
     }
   };
   if (begin < end) {
-    fetch(begin);
-    kst.store(Ks);
-    vst.store(Vs);
+    fetch(min(LA_C, end - begin));
+    stage();
   }
-  if (OUT) publish();
   for (int j0 = begin; j0 < end; j0 += LA_C) {
     const int rows = min(LA_C, end - j0);
     const bool more = j0 + LA_C < end;
     __syncthreads();
-    if (OUT) {
+    if (more) fetch(min(LA_C, end - j0 - LA_C));
+    const int lane = afresh(tid & 63), lr = lane & 15, lq = lane >> 4;
+    // Row 16 t + lr, column 4 s + lq of a tile of KB bytes a row: row_at[s & 1] + 128 (s >> 1) + 16 KB t.
+    const int row_at[2] = {la_at(lr, lq, KB), la_at(lr, 4 + lq, KB)};
+    // Rows 4 lq + lr / 4, features 16 i + 4 (lr % 4) ..: column_at[i & 3] + 128 (i >> 2), bf16.
+    int column_at[4];
+  #pragma unroll
+    for (int i = 0; i < 4; ++i) column_at[i] = la_at(4 * lq + (lr >> 2), 2 * i + ((lr & 3) >> 1), KB) + 8 * (lr & 1);
+    const int value_at = la_at(4 * lq + (lr >> 2), 2 * w + ((lr & 3) >> 1), VB) + 8 * (lr & 1);
+    f32x4_t o[4];  // [query tile]
+    if constexpr (OUT) {
+      // Scores of queries 16 t + lr with keys 32 u + {4 lq .., 16 + 4 lq ..}, weighted: units (t, u) = (3, 0), (3, 1), (2, 0),
+      // (1, 0), (0, 0), (2, 1).
+      for (int unit = w; unit < 6; unit += W) {
+        const int t = (0x201233 >> (4 * unit)) & 15, u = (0x22 >> unit) & 1;
+        f32x4_t P[2];
+        P[0] = P[1] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-      for (int s = 0; s < KB / 64; ++s) q[s] = qn[s];
+        for (int s = 0; s < KB / 64; ++s) {
+          const uint8_t* x = Ks + row_at[s & 1] + 128 * (s >> 1) + 32 * KB * u;
+          if constexpr (BF16) {
+            const int m = 2 * (lq & 1), half = 4 * (lq & 2);
+            const uint2 c = *reinterpret_cast<const uint2*>(Qs + la_at(16 * t + lr, 4 * s + m, KB) + half);
+            const uint2 d = *reinterpret_cast<const uint2*>(Qs + la_at(16 * t + lr, 4 * s + m + 1, KB) + half);
+            const u32x4_t q = {c.x, c.y, d.x, d.y};
+            P[0] = mfma16x16x32(*reinterpret_cast<const u32x4_t*>(x), q, P[0]);
+            if (2 * u + 1 <= t) P[1] = mfma16x16x32(*reinterpret_cast<const u32x4_t*>(x + 16 * KB), q, P[1]);
+          } else {
+            const f32x4_t q = *reinterpret_cast<const f32x4_t*>(Qs + row_at[s & 1] + 128 * (s >> 1) + 16 * KB * t);
+            const f32x4_t c = *reinterpret_cast<const f32x4_t*>(x), d = *reinterpret_cast<const f32x4_t*>(x + 16 * KB);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              P[0] = mfma16x16x4(c[e], q[e], P[0]);
+              P[1] = mfma16x16x4(d[e], q[e], P[1]);
+            }
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int n = 16 * (t - 2 * u - k) + lr - 4 * lq - e;  // tokens between key and query
+            P[k][e] = n >= 0 ? P[k][e] * (a.intra * tab[max(n, 0)].x) : 0.0f;
+          }
+        if constexpr (BF16) {
+          *reinterpret_cast<u32x4_t*>(Ps + ((2 * t + u) * 64 + lane) * 16) = la_pack(P[0], P[1]);
+        } else {
+          *reinterpret_cast<f32x4_t*>(Ps + ((4 * t + 2 * u) * 64 + lane) * 16) = P[0];
+          *reinterpret_cast<f32x4_t*>(Ps + ((4 * t + 2 * u + 1) * 64 + lane) * 16) = P[1];
+        }
+      }
+      // What the queries read from the state.
+#pragma unroll
+      for (int t = 0; t < 4; ++t) o[t] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int s = 0; s < KB / 64; ++s) {
+        u32x4_t x;
+        if constexpr (BF16) x = la_pack(S[2 * s], S[2 * s + 1]);
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          const u32x4_t y = *reinterpret_cast<const u32x4_t*>(Qs + row_at[s & 1] + 128 * (s >> 1) + 16 * KB * t);
+          if constexpr (BF16) {
+            o[t] = mfma16x16x32(x, y, o[t]);
+          } else {
+            const f32x4_t yf = __builtin_bit_cast(f32x4_t, y);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[t] = mfma16x16x4(S[s][e], yf[e], o[t]);
+          }
+        }
+      }
+#pragma unroll
+      for (int t = 0; t < 4; ++t) o[t] = o[t] * (a.inter * tab[16 * t + lr + 1 - a.lag].x);
     }
-    if (more) fetch(j0 + LA_C);
-    if (OUT) {
-      f32x4_t o[NT], P[4];
-      const float read = a.inter * tab[16 * w + lr + 1 - a.lag];
+    // The wave's columns of the values: bf16 as operands, tokens 32 u + {4 lq .., 16 + 4 lq ..}; fp32 tokens 16 t + 4 lq .. .
+    u32x4_t v[2];
+    f32x4_t vf[4];
+    if constexpr (BF16) {
 #pragma unroll
-      for (int t = 0; t < NT; ++t)
-        o[t] = la_dot<BF16, KB>(Ss, 16 * t + lr, lq, q, f32x4_t{0.0f, 0.0f, 0.0f, 0.0f}) * read;
+      for (int u = 0; u < 2; ++u) v[u] = la_column<VB>(Vs + value_at + 32 * VB * u);
+    } else {
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        P[t] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-        if (t > w) continue;
-        P[t] = la_dot<BF16, KB>(Ks, 16 * t + lr, lq, q, P[t]);
+      for (int t = 0; t < 4; ++t)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int n = 16 * (w - t) + lr - 4 * lq - e;  // tokens between key and query
-          P[t][e] = n >= 0 ? P[t][e] * (a.intra * tab[n < 0 ? 0 : n]) : 0.0f;
-        }
-      }
-      if constexpr (BF16) {
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          if (2 * u > w) continue;
-          const f32x4_t x = P[2 * u], y = P[2 * u + 1];
-          const u32x4_t f = {pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3])};
-#pragma unroll
-          for (int t = 0; t < NT; ++t) o[t] = mfma16x16x32(la_column<VB>(Vs, u, t, lr, lq), f, o[t]);
-        }
-      } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          if (j > w) continue;
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-#pragma unroll
-            for (int t = 0; t < NT; ++t) o[t] = mfma16x16x4(la_value<VB>(Vs, 16 * j + 4 * lq + e, t, lr), P[j][e], o[t]);
-        }
-      }
-      // Lane: features 16 t + 4 lq .. + 3 of query 16 w + lr.
-      const int j = j0 + 16 * w + lr;
-      if (j < end) {
-        const int64_t to = sb * a.ob + (first + (REV ? p.len - 1 - j : j)) * a.ot + (int64_t)h * a.oh;
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          const int c = 16 * t + 4 * lq;
-          if (c >= a.dv) continue;
-          if (BF16 && !a.o_f32)
-            *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.o) + to + c) =
-                make_uint2(pack_bf16x2(o[t][0], o[t][1]), pack_bf16x2(o[t][2], o[t][3]));
-          else
-            *reinterpret_cast<f32x4_t*>(static_cast<float*>(a.o) + to + c) = o[t];
-        }
-      }
+        for (int e = 0; e < 4; ++e)
+          vf[t][e] = *reinterpret_cast<const float*>(Vs + la_at(16 * t + 4 * lq + e, 4 * w + (lr >> 2), VB) + 4 * (lr & 3));
     }
     if (more || keep) {
-      const float2 full = rows == LA_C ? whole : la_decay2(g, rows);
+      const float2 full = tab[rows];
+      const float* add = put + LA_C - rows;  // zero behind the last row
 #pragma unroll
       for (int i = 0; i < NA; ++i)
 #pragma unroll
-        for (int b = 0; b < NB; ++b)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) S[i][b][e] = fmaf(S[i][b][e], full.x, S[i][b][e] * full.y);
-      const int gap = rows - 1 + a.lag;
+        for (int e = 0; e < 4; ++e) S[i][e] = fmaf(S[i][e], full.x, S[i][e] * full.y);
       if constexpr (BF16) {
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-          u32x4_t part[NB][3];
+          u32x4_t part[PARTS];
 #pragma unroll
-          for (int b = 0; b < NB; ++b) {
-            const u32x4_t v = la_column<VB>(Vs, u, w * NB + b, lr, lq);
+          for (int z = 0; z < 4; ++z) {
+            const int n = 32 * u + 16 * (z >> 1) + 4 * lq + 2 * (z & 1);  // token of the first of the two
+            float x0, x1;
+            unpack_bf16x2(v[u][z], x0, x1);
+            x0 *= add[n];
+            x1 *= add[n + 1];
 #pragma unroll
-            for (int z = 0; z < 4; ++z) {
-              const int n = 32 * u + 16 * (z >> 1) + 4 * lq + 2 * (z & 1);  // token of the first of the two
-              float x0, x1;
-              unpack_bf16x2(v[z], x0, x1);
-              x0 = n < rows ? x0 * (a.gain * tab[gap - min(n, gap)]) : 0.0f;
-              x1 = n + 1 < rows ? x1 * (a.gain * tab[gap - min(n + 1, gap)]) : 0.0f;
-#pragma unroll
-              for (int y = 0; y < 3; ++y) {
-                const uint32_t b0 = __float_as_uint(x0), b1 = __float_as_uint(x1);
-                part[b][y][z] = __builtin_amdgcn_perm(b1, b0, 0x07060302u);  // the high halves
-                x0 -= __uint_as_float(b0 & 0xffff0000u);
-                x1 -= __uint_as_float(b1 & 0xffff0000u);
-              }
+            for (int y = 0; y < PARTS; ++y) {
+              const uint32_t b0 = __float_as_uint(x0), b1 = __float_as_uint(x1);
+              part[y][z] = __builtin_amdgcn_perm(b1, b0, 0x07060302u);  // the high halves
+              x0 -= __uint_as_float(b0 & 0xffff0000u);
+              x1 -= __uint_as_float(b1 & 0xffff0000u);
             }
           }
 #pragma unroll
           for (int i = 0; i < NA; ++i) {
-            const u32x4_t k = la_column<KB>(Ks, u, i, lr, lq);
+            const u32x4_t k = la_column<KB>(Ks + column_at[i & 3] + 128 * (i >> 2) + 32 * KB * u);
 #pragma unroll
-            for (int b = 0; b < NB; ++b)
-#pragma unroll
-              for (int y = 0; y < 3; ++y) S[i][b] = mfma16x16x32(k, part[b][y], S[i][b]);
+            for (int y = 0; y < PARTS; ++y) S[i] = mfma16x16x32(k, part[y], S[i]);
           }
         }
       } else {
@@ -402,40 +420,55 @@ __global__ __launch_bounds__(256) void la_kernel(LaArgs a) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const int n = 16 * t + 4 * lq + e;
-            float v[NB];
+            const float x = vf[t][e] * add[n];
 #pragma unroll
-            for (int b = 0; b < NB; ++b)
-              v[b] = n < rows ? la_value<VB>(Vs, n, w * NB + b, lr) * (a.gain * tab[gap - min(n, gap)]) : 0.0f;
-#pragma unroll
-            for (int i = 0; i < NA; ++i) {
-              const float k = la_value<KB>(Ks, n, i, lr);
-#pragma unroll
-              for (int b = 0; b < NB; ++b) S[i][b] = mfma16x16x4(k, v[b], S[i][b]);
-            }
+            for (int i = 0; i < NA; ++i)
+              S[i] = mfma16x16x4(*reinterpret_cast<const float*>(Ks + la_at(n, 4 * i + (lr >> 2), KB) + 4 * (lr & 3)), x, S[i]);
           }
       }
     }
-    if (!more) break;
     __syncthreads();
-    kst.store(Ks);
-    vst.store(Vs);
-    if (OUT) publish();
+    if (more) stage();
+    if constexpr (OUT) {
+      const int c = 16 * w + 4 * lq;
+      const int64_t out = sb * a.ob + (first + (REV ? p.len - 1 - j0 - lr : j0 + lr)) * a.ot + (int64_t)h * a.oh + c;
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        if constexpr (BF16) {
+#pragma unroll
+          for (int u = 0; u <= t / 2; ++u)
+            o[t] = mfma16x16x32(v[u], *reinterpret_cast<const u32x4_t*>(Ps + ((2 * t + u) * 64 + lane) * 16), o[t]);
+        } else {
+#pragma unroll
+          for (int k = 0; k <= t; ++k) {
+            const f32x4_t s = *reinterpret_cast<const f32x4_t*>(Ps + ((4 * t + k) * 64 + lane) * 16);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[t] = mfma16x16x4(vf[k][e], s[e], o[t]);
+          }
+        }
+        if (j0 + 16 * t + lr >= end || c >= a.dv) continue;
+        const int64_t to = out + (int64_t)(REV ? -(16 * t) : 16 * t) * a.ot;
+        if (BF16 && !a.o_f32)
+          *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.o) + to) =
+              make_uint2(pack_bf16x2(o[t][0], o[t][1]), pack_bf16x2(o[t][2], o[t][3]));
+        else
+          *reinterpret_cast<f32x4_t*>(static_cast<float*>(a.o) + to) = o[t];
+      }
+    }
   }
   if (!keep) return;
 #pragma unroll
-  for (int i = 0; i < NA; ++i)
+  for (int i = 0; i < NA; ++i) {
+    if (!OUT) {
+      *mid(slot, i) = S[i];
+    } else {
 #pragma unroll
-    for (int b = 0; b < NB; ++b) {
-      if (!OUT) {
-        *mid(slot, i, b) = S[i][b];
-      } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int64_t u = user(i, b, e);
-          if (u >= 0) a.s1[u] = S[i][b][e];
-        }
+      for (int e = 0; e < 4; ++e) {
+        const int row = 16 * i + 4 * lq + e;
+        if (row < a.dk && 16 * w + lr < a.dv) a.s1[user + row * user_row] = S[i][e];
       }
     }
+  }
 }
 
 // mid[s] = e^{g L} (the state before segment s) + mid[s]: the state behind every segment but a sequence's last. A thread has 4
@@ -443,7 +476,7 @@ __global__ __launch_bounds__(256) void la_kernel(LaArgs a) {
 constexpr int LA_AHEAD = 8;
 template <int DK, int DV>
 __global__ __launch_bounds__(256) void la_carry_kernel(LaArgs a) {
-  constexpr int NA = DK / 16, NB = DV / 64;
+  constexpr int NA = DK / 16;
   const int seq = (int)(blockIdx.x / a.H), h = (int)(blockIdx.x % a.H);
   const int idx = (int)(blockIdx.y * 256 + threadIdx.x);
   const int n = (a.plan == nullptr ? a.nseg : a.plan[seq + 1] - a.plan[seq]) - 1;
@@ -452,8 +485,7 @@ __global__ __launch_bounds__(256) void la_carry_kernel(LaArgs a) {
   const float2 whole = la_decay2((double)a.g[h], a.L);
   f32x4_t S = {0.0f, 0.0f, 0.0f, 0.0f};
   if (a.s0 != nullptr) {
-    const int lane = idx & 63, b = (idx >> 6) % NB, i = (idx >> 6) / NB % NA, w = (idx >> 6) / NB / NA;
-    const int dv = 16 * (w * NB + b) + (lane & 15);
+    const int lane = idx & 63, i = (idx >> 6) % NA, dv = 16 * ((idx >> 6) / NA) + (lane & 15);
     const int64_t base = ((int64_t)seq * a.H + h) * a.dk * a.dv;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
@@ -551,34 +583,42 @@ __global__ __launch_bounds__(256) void la_step_kernel(LaStepArgs a) {
   }
 }
 
-template <bool BF16, int DK, int DV, bool REV>
+template <bool BF16, int DK, int DV, int PARTS, bool REV>
 hipError_t la_run(const LaArgs& a, int64_t segs, hipStream_t st) {
   const int64_t inner = segs - a.N;  // segments with another behind them, at most
   if (inner > 0) {
-    hipLaunchKernelGGL((la_kernel<BF16, DK, DV, REV, false>), dim3((unsigned)(inner * a.H)), dim3(256), 0, st, a);
+    hipLaunchKernelGGL((la_kernel<BF16, DK, DV, PARTS, REV, false>), dim3((unsigned)(inner * a.H)), dim3(4 * DV), 0, st, a);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     hipLaunchKernelGGL((la_carry_kernel<DK, DV>), dim3((unsigned)(a.N * a.H), DK * DV / 1024), dim3(256), 0, st, a);
     e = hipGetLastError();
     if (e != hipSuccess) return e;
   }
-  hipLaunchKernelGGL((la_kernel<BF16, DK, DV, REV, true>), dim3((unsigned)(segs * a.H)), dim3(256), 0, st, a);
+  hipLaunchKernelGGL((la_kernel<BF16, DK, DV, PARTS, REV, true>), dim3((unsigned)(segs * a.H)), dim3(4 * DV), 0, st, a);
   return hipGetLastError();
 }
 
-template <bool BF16, bool REV>
+template <bool BF16, int PARTS, bool REV>
 hipError_t la_run_d(const LaArgs& a, int64_t segs, hipStream_t st) {
-  if (a.dk <= 64) return a.dv <= 64 ? la_run<BF16, 64, 64, REV>(a, segs, st) : la_run<BF16, 64, 128, REV>(a, segs, st);
-  return a.dv <= 64 ? la_run<BF16, 128, 64, REV>(a, segs, st) : la_run<BF16, 128, 128, REV>(a, segs, st);
+  if (a.dk <= 64)
+    return a.dv <= 64 ? la_run<BF16, 64, 64, PARTS, REV>(a, segs, st) : la_run<BF16, 64, 128, PARTS, REV>(a, segs, st);
+  return a.dv <= 64 ? la_run<BF16, 128, 64, PARTS, REV>(a, segs, st) : la_run<BF16, 128, 128, PARTS, REV>(a, segs, st);
+}
+
+// A state that is an output is made of three bf16 parts (24 bits); one that only queries read, rounded to 8 bits, of two.
+template <bool REV>
+hipError_t la_run_p(const LaArgs& a, int64_t segs, bool bf16, hipStream_t st) {
+  if (!bf16) return la_run_d<false, 1, REV>(a, segs, st);
+  return la_run_d<true, 3, REV>(a, segs, st);
 }
 
 }  // namespace
 
 int la_segment_tokens(int64_t T, int64_t N, int H) {
-  // Segments of at least 8 chunks, as many as give every CU two workgroups.
+  // As many segments as give every CU two workgroups.
   const int64_t want = std::max<int64_t>(1, 2 * (int64_t)device_cus() / H);
   const int64_t chunks = (T + LA_C * want - 1) / (LA_C * want);
-  return (int)std::min<int64_t>(std::max<int64_t>(chunks, 8), 1 << 20) * LA_C;
+  return (int)std::min<int64_t>(std::max<int64_t>(chunks, 1), 1 << 20) * LA_C;
 }
 
 int64_t la_padded_state(int dk, int dv) { return (int64_t)(dk <= 64 ? 64 : 128) * (dv <= 64 ? 64 : 128); }
@@ -594,8 +634,7 @@ hipError_t launch_la_gap(void* o, const int32_t* plan, int N, int64_t T, int row
 }
 
 hipError_t launch_la(const LaArgs& a, int64_t segs, bool backwards, bool bf16, hipStream_t st) {
-  if (backwards) return bf16 ? la_run_d<true, true>(a, segs, st) : la_run_d<false, true>(a, segs, st);
-  return bf16 ? la_run_d<true, false>(a, segs, st) : la_run_d<false, false>(a, segs, st);
+  return backwards ? la_run_p<true>(a, segs, bf16, st) : la_run_p<false>(a, segs, bf16, st);
 }
 
 hipError_t launch_la_group(const float* x, void* out, int64_t rows, int G, int d, bool bf16, hipStream_t st) {
