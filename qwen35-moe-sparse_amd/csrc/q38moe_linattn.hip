@@ -172,19 +172,27 @@ struct LaStage {
     }
     at += LA_C * step;
   }
+  // SWAP: with the 8-byte halves of odd rows' columns exchanged.
+  template <bool SWAP>
   __device__ __forceinline__ void store(int tid, uint8_t* lds) const {
     const int row = tid / COLS, col = tid % COLS;
+    static_assert(ROWS % 2 == 0, "the rows of a thread are all even or all odd");
+    const bool swap = SWAP && (row & 1);
 #pragma unroll
-    for (int i = 0; i < N; ++i) *reinterpret_cast<u32x4_t*>(lds + la_at(row + ROWS * i, col, BYTES)) = r[i];
+    for (int i = 0; i < N; ++i)
+      *reinterpret_cast<u32x4_t*>(lds + la_at(row + ROWS * i, col, BYTES)) =
+          swap ? u32x4_t{r[i][2], r[i][3], r[i][0], r[i][1]} : r[i];
   }
-  // bf16: column 4 u + m of the tile gets features 32 u + 4 m .. and 32 u + 16 + 4 m .. (4 each).
-  __device__ __forceinline__ void store_paired(int tid, uint8_t* lds) const {
-    const int row = tid / COLS, col = tid % COLS, m = (col & ~3) + 2 * (col & 1), half = 4 * (col & 2);
+  // The next 64 rows straight into a tile, asynchronously. Places behind the last row or feature get others of the same kind,
+  // since a copy cannot leave zeros: rows that are not stored, and features that meet zeros of the state and of the keys.
+  __device__ __forceinline__ void copy(int tid, uint8_t* lds, int rows, int bytes) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      *reinterpret_cast<uint2*>(lds + la_at(row + ROWS * i, m, BYTES) + half) = make_uint2(r[i][0], r[i][1]);
-      *reinterpret_cast<uint2*>(lds + la_at(row + ROWS * i, m + 1, BYTES) + half) = make_uint2(r[i][2], r[i][3]);
+      const int row = tid / COLS + ROWS * i, col = la_at(row, tid % COLS, 0) >> 4;
+      load_lds16(at + (min(row, rows - 1) - tid / COLS) * step + 16 * (min(col, bytes / 16 - 1) - tid % COLS),
+                 lds + 16 * (THREADS * i + (tid & ~63)));
     }
+    at += LA_C * step;
   }
 };
 
@@ -209,22 +217,34 @@ __device__ __forceinline__ int afresh(int x) {
 
 // Waves on a SIMD that the LDS of la_kernel's workgroups allows, at most 4: the limit of its registers.
 constexpr int la_waves(bool bf16, int dk, int dv, bool out) {
-  return bf16 ? (out && dk == 128 && dv == 64 ? 3 : 4) : out && dk == 128 && dv == 64 ? 1 : 2;
+  return bf16 ? (out && dk == 128 && dv == 64 ? 2 : 4) : out && dk == 128 && dv == 64 ? 1 : 2;
+}
+
+// The scores of a chunk: units of 32 keys (32 u ..) and 16 queries (16 t ..), those with a key at or before a query.
+constexpr int LA_UNITS = 6;
+__device__ __forceinline__ int la_unit_queries(int unit) { return (0x201233 >> (4 * unit)) & 15; }
+__device__ __forceinline__ int la_unit_keys(int unit) { return (0x22 >> unit) & 1; }
+constexpr int la_unit(int t, int u) { return t == 3 ? u : t == 2 ? 2 + 3 * u : 4 - t; }
+
+// First of the 4 rows of the state that accumulator tile i has in lanes 16 q .. : bf16 tiles 2 u and 2 u + 1 share groups of 8
+// rows, so that a lane's rows of both, rounded, are 8 features in a row: an operand against the queries as they lie.
+template <bool BF16>
+__device__ __forceinline__ int la_row(int i, int q) {
+  return BF16 ? 32 * (i >> 1) + 8 * q + 4 * (i & 1) : 16 * i + 4 * q;
 }
 
 // One segment of one head; DV / 16 waves. Wave w has columns 16 w .. of the state and of the outputs for all 64 queries of a
 // chunk (outputs as [column, query] tiles), and some of the scores' six [32 keys, 16 queries] units, which go through LDS. The
-// state stays in accumulators; rounded, they are the operand that queries read as they lie, since an accumulator's lane holds 4
-// rows of a column and an operand's lane 8 of one: the queries' features are stored in the order that this gives (store_paired).
-// A column's tokens come out of the transposing LDS read in the same order, once for the outputs and for the state.
+// state stays in accumulators, which, rounded, are the operand that queries read (la_row). A column's tokens come out of the
+// transposing LDS read in the order in which an accumulator holds the scores' keys, once for the outputs and for the state.
 // Two barriers a chunk: tiles and scores are read behind one, scores and the next tiles written behind the other.
 template <bool BF16, int DK, int DV, int PARTS, bool REV, bool OUT>
 __global__ __launch_bounds__(4 * DV, la_waves(BF16, DK, DV, OUT)) void la_kernel(LaArgs a) {
   constexpr int ES = BF16 ? 2 : 4, KB = DK * ES, VB = DV * ES, NA = DK / 16, W = DV / 16, THREADS = 4 * DV;
   __shared__ __attribute__((aligned(16))) uint8_t Ks[LA_C * KB];
   __shared__ __attribute__((aligned(16))) uint8_t Vs[LA_C * VB];
-  __shared__ __attribute__((aligned(16))) uint8_t Qs[OUT ? LA_C * KB : 16];
-  __shared__ __attribute__((aligned(16))) uint8_t Ps[OUT ? 16 * LA_C * 4 * ES : 16];  // [query tile][key tiles][lane]
+  __shared__ __attribute__((aligned(16))) uint8_t Qs[2][OUT ? LA_C * KB : 16];
+  __shared__ __attribute__((aligned(16))) uint8_t Ps[OUT ? LA_UNITS * 512 * ES : 16];
   __shared__ float2 tab[LA_C + 1];  // e^{g n} to 48 bits
   __shared__ float put[2 * LA_C];   // what a token adds to the state with: of a chunk's 64, then zeros
   const int tid = threadIdx.x, lane = tid & 63, lr = lane & 15, lq = lane >> 4;
@@ -245,7 +265,8 @@ __global__ __launch_bounds__(4 * DV, la_waves(BF16, DK, DV, OUT)) void la_kernel
   const int begin = p.s * a.L, end = min(p.len, begin + a.L);
   const bool last = p.s == p.nseg - 1, keep = !OUT || (last && a.s1 != nullptr);
 
-  f32x4_t S[NA];  // rows 16 i + 4 lq .., column 16 w + lr
+  // Rows la_row(i, lq) .. + 3, column 16 w + lr.
+  f32x4_t S[NA];
   const int64_t slot = la_slot(a, p.seq) + p.s;
   auto mid = [&](int64_t s, int i) {
     return reinterpret_cast<f32x4_t*>(a.mid + (s * a.H + h) * (DK * DV) + ((w * NA + i) * 64 + lane) * 4);
@@ -262,7 +283,7 @@ __global__ __launch_bounds__(4 * DV, la_waves(BF16, DK, DV, OUT)) void la_kernel
     } else if (a.s0 != nullptr) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const int row = 16 * i + 4 * lq + e;
+        const int row = la_row<BF16>(i, lq) + e;
         if (row < a.dk && 16 * w + lr < a.dv) S[i][e] = a.s0[user + row * user_row];
       }
     }
@@ -272,58 +293,56 @@ __global__ __launch_bounds__(4 * DV, la_waves(BF16, DK, DV, OUT)) void la_kernel
   start(kst, a.k, begin);
   start(vst, a.v, begin);
   if (OUT) start(qst, a.q, begin);
-  auto fetch = [&](int rows) {
+  auto fetch = [&](int rows, uint8_t* queries) {
     const int tid = afresh((int)threadIdx.x);
+    if (OUT) qst.copy(tid, queries, rows, a.dk * ES);  // first: done when the others are
     kst.load(tid, rows, a.dk * ES);
     vst.load(tid, rows, a.dv * ES);
-    if (OUT) qst.load(tid, rows, a.dk * ES);
   };
   auto stage = [&]() {
     const int tid = afresh((int)threadIdx.x);
-    kst.store(tid, Ks);
-    vst.store(tid, Vs);
-    if constexpr (OUT) {
-      if constexpr (BF16) qst.store_paired(tid, Qs);
-      else qst.store(tid, Qs);
-    }
+    kst.template store<BF16>(tid, Ks);
+    vst.template store<false>(tid, Vs);
+    wait_vmcnt0();  // the queries' copy
   };
   if (begin < end) {
-    fetch(min(LA_C, end - begin));
+    fetch(min(LA_C, end - begin), Qs[0]);
     stage();
   }
-  for (int j0 = begin; j0 < end; j0 += LA_C) {
+  for (int j0 = begin, par = 0; j0 < end; j0 += LA_C, par ^= 1) {
     const int rows = min(LA_C, end - j0);
     const bool more = j0 + LA_C < end;
     __syncthreads();
-    if (more) fetch(min(LA_C, end - j0 - LA_C));
+    if (more) fetch(min(LA_C, end - j0 - LA_C), Qs[par ^ 1]);
+    const uint8_t* const Q = Qs[par];
     const int lane = afresh(tid & 63), lr = lane & 15, lq = lane >> 4;
     // Row 16 t + lr, column 4 s + lq of a tile of KB bytes a row: row_at[s & 1] + 128 (s >> 1) + 16 KB t.
     const int row_at[2] = {la_at(lr, lq, KB), la_at(lr, 4 + lq, KB)};
-    // Rows 4 lq + lr / 4, features 16 i + 4 (lr % 4) ..: column_at[i & 3] + 128 (i >> 2), bf16.
-    int column_at[4];
-  #pragma unroll
-    for (int i = 0; i < 4; ++i) column_at[i] = la_at(4 * lq + (lr >> 2), 2 * i + ((lr & 3) >> 1), KB) + 8 * (lr & 1);
+    // bf16: rows 4 lq + lr / 4, features row_of(i, lr / 4, 0) for lr % 4: column_at[i / 2 % 2] ^ 8 (i % 2), + 128 (i / 4).
+    int column_at[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) column_at[i] = la_at(4 * lq + (lr >> 2), 4 * i + (lr & 3), KB) + 8 * ((lr >> 2) & 1);
     const int value_at = la_at(4 * lq + (lr >> 2), 2 * w + ((lr & 3) >> 1), VB) + 8 * (lr & 1);
     f32x4_t o[4];  // [query tile]
     if constexpr (OUT) {
-      // Scores of queries 16 t + lr with keys 32 u + {4 lq .., 16 + 4 lq ..}, weighted: units (t, u) = (3, 0), (3, 1), (2, 0),
-      // (1, 0), (0, 0), (2, 1).
-      for (int unit = w; unit < 6; unit += W) {
-        const int t = (0x201233 >> (4 * unit)) & 15, u = (0x22 >> unit) & 1;
+      // Scores of queries 16 t + lr with keys 32 u + {4 lq .., 16 + 4 lq ..}, weighted.
+      for (int unit = w; unit < LA_UNITS; unit += W) {
+        const int t = la_unit_queries(unit), u = la_unit_keys(unit);
         f32x4_t P[2];
         P[0] = P[1] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int s = 0; s < KB / 64; ++s) {
           const uint8_t* x = Ks + row_at[s & 1] + 128 * (s >> 1) + 32 * KB * u;
           if constexpr (BF16) {
-            const int m = 2 * (lq & 1), half = 4 * (lq & 2);
-            const uint2 c = *reinterpret_cast<const uint2*>(Qs + la_at(16 * t + lr, 4 * s + m, KB) + half);
-            const uint2 d = *reinterpret_cast<const uint2*>(Qs + la_at(16 * t + lr, 4 * s + m + 1, KB) + half);
-            const u32x4_t q = {c.x, c.y, d.x, d.y};
-            P[0] = mfma16x16x32(*reinterpret_cast<const u32x4_t*>(x), q, P[0]);
-            if (2 * u + 1 <= t) P[1] = mfma16x16x32(*reinterpret_cast<const u32x4_t*>(x + 16 * KB), q, P[1]);
+            const u32x4_t q = *reinterpret_cast<const u32x4_t*>(Q + row_at[s & 1] + 128 * (s >> 1) + 16 * KB * t);
+            auto key = [&](const uint8_t* at) {  // odd rows lie with their halves exchanged
+              const u32x4_t k = *reinterpret_cast<const u32x4_t*>(at);
+              return lr & 1 ? u32x4_t{k[2], k[3], k[0], k[1]} : k;
+            };
+            P[0] = mfma16x16x32(key(x), q, P[0]);
+            if (2 * u + 1 <= t) P[1] = mfma16x16x32(key(x + 16 * KB), q, P[1]);
           } else {
-            const f32x4_t q = *reinterpret_cast<const f32x4_t*>(Qs + row_at[s & 1] + 128 * (s >> 1) + 16 * KB * t);
+            const f32x4_t q = *reinterpret_cast<const f32x4_t*>(Q + row_at[s & 1] + 128 * (s >> 1) + 16 * KB * t);
             const f32x4_t c = *reinterpret_cast<const f32x4_t*>(x), d = *reinterpret_cast<const f32x4_t*>(x + 16 * KB);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
@@ -340,10 +359,10 @@ __global__ __launch_bounds__(4 * DV, la_waves(BF16, DK, DV, OUT)) void la_kernel
             P[k][e] = n >= 0 ? P[k][e] * (a.intra * tab[max(n, 0)].x) : 0.0f;
           }
         if constexpr (BF16) {
-          *reinterpret_cast<u32x4_t*>(Ps + ((2 * t + u) * 64 + lane) * 16) = la_pack(P[0], P[1]);
+          *reinterpret_cast<u32x4_t*>(Ps + (unit * 64 + lane) * 16) = la_pack(P[0], P[1]);
         } else {
-          *reinterpret_cast<f32x4_t*>(Ps + ((4 * t + 2 * u) * 64 + lane) * 16) = P[0];
-          *reinterpret_cast<f32x4_t*>(Ps + ((4 * t + 2 * u + 1) * 64 + lane) * 16) = P[1];
+          *reinterpret_cast<f32x4_t*>(Ps + (2 * unit * 64 + lane) * 16) = P[0];
+          *reinterpret_cast<f32x4_t*>(Ps + ((2 * unit + 1) * 64 + lane) * 16) = P[1];
         }
       }
       // What the queries read from the state.
@@ -355,7 +374,7 @@ __global__ __launch_bounds__(4 * DV, la_waves(BF16, DK, DV, OUT)) void la_kernel
         if constexpr (BF16) x = la_pack(S[2 * s], S[2 * s + 1]);
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
-          const u32x4_t y = *reinterpret_cast<const u32x4_t*>(Qs + row_at[s & 1] + 128 * (s >> 1) + 16 * KB * t);
+          const u32x4_t y = *reinterpret_cast<const u32x4_t*>(Q + row_at[s & 1] + 128 * (s >> 1) + 16 * KB * t);
           if constexpr (BF16) {
             o[t] = mfma16x16x32(x, y, o[t]);
           } else {
@@ -391,6 +410,7 @@ __global__ __launch_bounds__(4 * DV, la_waves(BF16, DK, DV, OUT)) void la_kernel
       if constexpr (BF16) {
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
+          __builtin_amdgcn_sched_barrier(0);
           u32x4_t part[PARTS];
 #pragma unroll
           for (int z = 0; z < 4; ++z) {
@@ -409,7 +429,8 @@ __global__ __launch_bounds__(4 * DV, la_waves(BF16, DK, DV, OUT)) void la_kernel
           }
 #pragma unroll
           for (int i = 0; i < NA; ++i) {
-            const u32x4_t k = la_column<KB>(Ks + column_at[i & 3] + 128 * (i >> 2) + 32 * KB * u);
+            if (i % 4 == 0) __builtin_amdgcn_sched_barrier(0);
+            const u32x4_t k = la_column<KB>(Ks + (column_at[(i >> 1) & 1] ^ (8 * (i & 1))) + 128 * (i >> 2) + 32 * KB * u);
 #pragma unroll
             for (int y = 0; y < PARTS; ++y) S[i] = mfma16x16x32(k, part[y], S[i]);
           }
@@ -437,11 +458,11 @@ __global__ __launch_bounds__(4 * DV, la_waves(BF16, DK, DV, OUT)) void la_kernel
         if constexpr (BF16) {
 #pragma unroll
           for (int u = 0; u <= t / 2; ++u)
-            o[t] = mfma16x16x32(v[u], *reinterpret_cast<const u32x4_t*>(Ps + ((2 * t + u) * 64 + lane) * 16), o[t]);
+            o[t] = mfma16x16x32(v[u], *reinterpret_cast<const u32x4_t*>(Ps + (la_unit(t, u) * 64 + lane) * 16), o[t]);
         } else {
 #pragma unroll
           for (int k = 0; k <= t; ++k) {
-            const f32x4_t s = *reinterpret_cast<const f32x4_t*>(Ps + ((4 * t + k) * 64 + lane) * 16);
+            const f32x4_t s = *reinterpret_cast<const f32x4_t*>(Ps + ((2 * la_unit(t, k / 2) + k % 2) * 64 + lane) * 16);
 #pragma unroll
             for (int e = 0; e < 4; ++e) o[t] = mfma16x16x4(vf[k][e], s[e], o[t]);
           }
@@ -464,7 +485,7 @@ __global__ __launch_bounds__(4 * DV, la_waves(BF16, DK, DV, OUT)) void la_kernel
     } else {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const int row = 16 * i + 4 * lq + e;
+        const int row = la_row<BF16>(i, lq) + e;
         if (row < a.dk && 16 * w + lr < a.dv) a.s1[user + row * user_row] = S[i][e];
       }
     }
@@ -474,7 +495,7 @@ __global__ __launch_bounds__(4 * DV, la_waves(BF16, DK, DV, OUT)) void la_kernel
 // mid[s] = e^{g L} (the state before segment s) + mid[s]: the state behind every segment but a sequence's last. A thread has 4
 // elements of one state; reads run LA_AHEAD segments ahead.
 constexpr int LA_AHEAD = 8;
-template <int DK, int DV>
+template <bool BF16, int DK, int DV>
 __global__ __launch_bounds__(256) void la_carry_kernel(LaArgs a) {
   constexpr int NA = DK / 16;
   const int seq = (int)(blockIdx.x / a.H), h = (int)(blockIdx.x % a.H);
@@ -489,7 +510,7 @@ __global__ __launch_bounds__(256) void la_carry_kernel(LaArgs a) {
     const int64_t base = ((int64_t)seq * a.H + h) * a.dk * a.dv;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const int dk = 16 * i + 4 * (lane >> 4) + e;
+      const int dk = la_row<BF16>(i, lane >> 4) + e;
       if (dk < a.dk && dv < a.dv) S[e] = a.s0[base + (a.turned ? dv * a.dk + dk : dk * a.dv + dv)];
     }
   }
@@ -590,7 +611,7 @@ hipError_t la_run(const LaArgs& a, int64_t segs, hipStream_t st) {
     hipLaunchKernelGGL((la_kernel<BF16, DK, DV, PARTS, REV, false>), dim3((unsigned)(inner * a.H)), dim3(4 * DV), 0, st, a);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL((la_carry_kernel<DK, DV>), dim3((unsigned)(a.N * a.H), DK * DV / 1024), dim3(256), 0, st, a);
+    hipLaunchKernelGGL((la_carry_kernel<BF16, DK, DV>), dim3((unsigned)(a.N * a.H), DK * DV / 1024), dim3(256), 0, st, a);
     e = hipGetLastError();
     if (e != hipSuccess) return e;
   }
