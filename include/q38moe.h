@@ -611,20 +611,22 @@ int q38moe_qk_norm_rope_backward(const void* d_q_out, const void* d_k_out, const
  * tokens of no sequence get zeros. strides (host): sequence, token and head strides of q, k, v in elements, multiples of 16
  * bytes (the sequences' unused with cu_seqlens). dk and dv multiples of 8 up to 128. Backward: from d_out (contiguous) and
  * d_final_state (NULL: zero) the gradients that are not NULL, contiguous; d_initial_state only with dv. A token's NaN or
- * infinity may reach the outputs of its chunk, up to 63 tokens before it. Workspace contents arbitrary.
+ * infinity may reach the outputs of its chunk, up to 63 tokens before it. Workspace contents arbitrary. saved (NULL: not kept):
+ * saved_bytes of states that the forward pass leaves and the backward pass of the same call takes (NULL: it makes them again).
  * step: one token of B sequences, q [B,H,dk], k [B,Hk,dk], v [B,Hk,dv] (strides: sequence and head of each), states updated in
  * place: state [pool,H,dk,dv], sequence b in slots[b] (NULL: b). A slot outside [0, pool) is none: out is zero. No slot may occur
  * twice. out [B,H,dv].
  */
 int q38moe_linear_attention_workspace_bytes(int64_t N, int64_t S, int32_t H, int32_t Hk, int32_t dk, int32_t dv, int32_t packed,
-                                            int32_t backward, size_t* bytes);
+                                            int32_t backward, size_t* bytes, size_t* saved_bytes);
 int q38moe_linear_attention_forward(const void* q, const void* k, const void* v, const int64_t* strides, const float* log_decay,
                                     float scale, const float* initial_state, const int32_t* cu_seqlens, void* out,
-                                    float* final_state, int64_t N, int64_t S, int32_t H, int32_t Hk, int32_t dk, int32_t dv,
-                                    void* workspace, size_t workspace_bytes, int32_t dtype, void* stream);
+                                    float* final_state, void* saved, size_t saved_bytes, int64_t N, int64_t S, int32_t H,
+                                    int32_t Hk, int32_t dk, int32_t dv, void* workspace, size_t workspace_bytes, int32_t dtype,
+                                    void* stream);
 int q38moe_linear_attention_backward(const void* d_out, const float* d_final_state, const void* q, const void* k, const void* v,
                                      const int64_t* strides, const float* log_decay, float scale, const float* initial_state,
-                                     const int32_t* cu_seqlens, void* dq, void* dk_out, void* dv_out, float* d_initial_state,
+                                     const int32_t* cu_seqlens, const void* saved, size_t saved_bytes, void* dq, void* dk_out, void* dv_out, float* d_initial_state,
                                      int64_t N, int64_t S, int32_t H, int32_t Hk, int32_t dk, int32_t dv, void* workspace,
                                      size_t workspace_bytes, int32_t dtype, void* stream);
 int q38moe_linear_attention_step(const void* q, const void* k, const void* v, const int64_t* strides, const float* log_decay,

@@ -1894,46 +1894,52 @@ static int check_linattn(int64_t N, int64_t S, int32_t H, int32_t Hk, int32_t dk
   return Q38MOE_OK;
 }
 
-// How a call's sequences are cut, and the parts of its workspace: the plan (packed), the states between segments, and (backwards,
-// shared heads) one fp32 gradient for each head.
+// How a call's sequences are cut, and the parts of its workspace: the plan (packed), the states between segments (forwards: may
+// be the caller's instead), and (backwards, shared heads) fp32 gradients of each head.
 struct LinattnPlan {
   int L, nseg;
   int64_t tokens, segs;
-  size_t mid, grouped, bytes;
+  size_t states, mid, grouped, grouped_k, bytes;
 };
 static int linattn_plan(LinattnPlan& p, int64_t N, int64_t S, int32_t H, int32_t Hk, int32_t dk, int32_t dv, bool packed,
-                        bool backward) {
+                        bool backward, bool own_states) {
   p.tokens = packed ? S : N * S;
   p.L = q38::la_segment_tokens(p.tokens, N, H);
   p.nseg = packed ? 0 : (int)std::max<int64_t>(1, (S + p.L - 1) / p.L);
   p.segs = packed ? S / p.L + N : N * p.nseg;
   if (p.segs * H >= (int64_t)1 << 31) return fail(Q38MOE_EINVAL, "too many sequences and heads for one launch");
-  const size_t states = sizeof(float) * (size_t)(p.segs - N) * H * (size_t)q38::la_padded_state(dk, dv);
+  p.states = sizeof(float) * (size_t)(p.segs - N) * H * (size_t)q38::la_padded_state(dk, dv);
   const bool grouped = backward && H != Hk;
   p.mid = packed ? align_up(sizeof(int32_t) * (size_t)(3 * N + 1)) : 0;
-  p.grouped = p.mid + align_up(states);
-  p.bytes = p.grouped + (grouped ? sizeof(float) * (size_t)p.tokens * H * std::max(dk, dv) : 0);
+  p.grouped = p.mid + (own_states ? align_up(p.states) : 0);
+  p.grouped_k = align_up(sizeof(float) * (size_t)p.tokens * H * dv);
+  p.bytes = p.grouped + (grouped ? p.grouped_k + sizeof(float) * (size_t)p.tokens * H * dk : 0);
   return Q38MOE_OK;
 }
 
 int q38moe_linear_attention_workspace_bytes(int64_t N, int64_t S, int32_t H, int32_t Hk, int32_t dk, int32_t dv, int32_t packed,
-                                            int32_t backward, size_t* bytes) {
+                                            int32_t backward, size_t* bytes, size_t* saved_bytes) {
   g_err[0] = 0;
   if (bytes == nullptr) return fail(Q38MOE_EINVAL, "bytes must not be NULL");
   Q38_CHECK(check_linattn(N, S, H, Hk, dk, dv, Q38MOE_BF16));
   LinattnPlan p;
-  Q38_CHECK(linattn_plan(p, N, S, H, Hk, dk, dv, packed != 0, backward != 0));
+  Q38_CHECK(linattn_plan(p, N, S, H, Hk, dk, dv, packed != 0, backward != 0, true));
   *bytes = p.bytes;
+  if (saved_bytes != nullptr) *saved_bytes = p.states;
   return Q38MOE_OK;
 }
 
 // Checks, the plan, and what every pass over the tokens shares.
-static int linattn_start(LinattnPlan& p, q38::LaArgs& a, const float* log_decay, const int32_t* cu_seqlens, int64_t N, int64_t S,
-                         int32_t H, int32_t Hk, int32_t dk, int32_t dv, bool backward, void* workspace,
-                         size_t workspace_bytes, int32_t dtype, hipStream_t st) {
+static int linattn_start(LinattnPlan& p, q38::LaArgs& a, const float* log_decay, const int32_t* cu_seqlens, const void* saved,
+                         size_t saved_bytes, int64_t N, int64_t S, int32_t H, int32_t Hk, int32_t dk, int32_t dv,
+                         bool backward, void* workspace, size_t workspace_bytes, int32_t dtype, hipStream_t st) {
   Q38_CHECK(check_linattn(N, S, H, Hk, dk, dv, dtype));
   if (log_decay == nullptr) return fail(Q38MOE_EINVAL, "log_decay must not be NULL");
-  Q38_CHECK(linattn_plan(p, N, S, H, Hk, dk, dv, cu_seqlens != nullptr, backward));
+  Q38_CHECK(linattn_plan(p, N, S, H, Hk, dk, dv, cu_seqlens != nullptr, backward, backward || saved == nullptr));
+  if (saved != nullptr) {
+    Q38_CHECK(check_ptr(saved, "saved"));
+    if (saved_bytes < p.states) return fail(Q38MOE_EWORKSPACE, "saved needs %zu bytes, got %zu", p.states, saved_bytes);
+  }
   if (p.bytes > 0) {
     Q38_CHECK(check_ptr(workspace, "workspace"));
     if (workspace_bytes < p.bytes)
@@ -1955,8 +1961,9 @@ static q38::LaTensor la_tensor(const void* p, const int64_t* strides, int div) {
 
 int q38moe_linear_attention_forward(const void* q, const void* k, const void* v, const int64_t* strides, const float* log_decay,
                                     float scale, const float* initial_state, const int32_t* cu_seqlens, void* out,
-                                    float* final_state, int64_t N, int64_t S, int32_t H, int32_t Hk, int32_t dk, int32_t dv,
-                                    void* workspace, size_t workspace_bytes, int32_t dtype, void* stream) {
+                                    float* final_state, void* saved, size_t saved_bytes, int64_t N, int64_t S, int32_t H,
+                                    int32_t Hk, int32_t dk, int32_t dv, void* workspace, size_t workspace_bytes, int32_t dtype,
+                                    void* stream) {
   g_err[0] = 0;
   Q38_CHECK(check_strides(strides, 9, dtype));
   LinattnPlan p;
@@ -1970,7 +1977,9 @@ int q38moe_linear_attention_forward(const void* q, const void* k, const void* v,
     Q38_CHECK(check_ptr(out, "out"));
   }
   hipStream_t st = static_cast<hipStream_t>(stream);
-  Q38_CHECK(linattn_start(p, a, log_decay, cu_seqlens, N, S, H, Hk, dk, dv, false, workspace, workspace_bytes, dtype, st));
+  Q38_CHECK(linattn_start(p, a, log_decay, cu_seqlens, saved, saved_bytes, N, S, H, Hk, dk, dv, false, workspace, workspace_bytes,
+                          dtype, st));
+  if (saved != nullptr) a.mid = static_cast<float*>(saved);
   const int G = H / Hk;
   a.q = la_tensor(q, strides, 1);
   a.k = la_tensor(k, strides + 3, G);
@@ -1981,7 +1990,7 @@ int q38moe_linear_attention_forward(const void* q, const void* k, const void* v,
   a.intra = a.inter = scale, a.gain = 1.0f, a.lag = 0;
   a.dk = dk, a.dv = dv;
   const bool bf16 = dtype == Q38MOE_BF16;
-  Q38_HIP(q38::launch_la(a, p.segs, false, bf16, st), "linear attention launch");
+  Q38_HIP(q38::launch_la(a, p.segs, true, bf16, st), "linear attention launch");
   if (a.plan != nullptr && S > 0)
     Q38_HIP(q38::launch_la_gap(out, a.plan, (int)N, S, H * dv * (int)elem_size(dtype), st), "linear attention launch");
   return Q38MOE_OK;
@@ -1989,7 +1998,7 @@ int q38moe_linear_attention_forward(const void* q, const void* k, const void* v,
 
 int q38moe_linear_attention_backward(const void* d_out, const float* d_final_state, const void* q, const void* k, const void* v,
                                      const int64_t* strides, const float* log_decay, float scale, const float* initial_state,
-                                     const int32_t* cu_seqlens, void* dq, void* dk_out, void* dv_out, float* d_initial_state,
+                                     const int32_t* cu_seqlens, const void* saved, size_t saved_bytes, void* dq, void* dk_out, void* dv_out, float* d_initial_state,
                                      int64_t N, int64_t S, int32_t H, int32_t Hk, int32_t dk, int32_t dv, void* workspace,
                                      size_t workspace_bytes, int32_t dtype, void* stream) {
   g_err[0] = 0;
@@ -2008,47 +2017,70 @@ int q38moe_linear_attention_backward(const void* d_out, const float* d_final_sta
     Q38_CHECK(check_opt_ptr(dv_out, "dv"));
   }
   hipStream_t st = static_cast<hipStream_t>(stream);
-  Q38_CHECK(linattn_start(p, a, log_decay, cu_seqlens, N, S, H, Hk, dk, dv, true, workspace, workspace_bytes, dtype, st));
+  Q38_CHECK(linattn_start(p, a, log_decay, cu_seqlens, saved, saved_bytes, N, S, H, Hk, dk, dv, true, workspace, workspace_bytes,
+                          dtype, st));
   const int G = H / Hk;
   const bool bf16 = dtype == Q38MOE_BF16;
-  float* per_head = reinterpret_cast<float*>(static_cast<char*>(workspace) + p.grouped);
+  if (d_initial_state != nullptr && dv_out == nullptr && p.tokens > 0)
+    return fail(Q38MOE_EINVAL, "the initial state's gradient comes with dv");
+  char* const per_head = static_cast<char*>(workspace) + p.grouped;
   const int64_t do_strides[3] = {S * (int64_t)H * dv, (int64_t)H * dv, dv};
   const q38::LaTensor tq = la_tensor(q, strides, 1), tk = la_tensor(k, strides + 3, G), tv = la_tensor(v, strides + 6, G),
                       tdo = la_tensor(d_out, do_strides, 1);
-  // One pass with its results in `out`, the heads that share one added where it has Hk of them.
-  auto pass = [&](void* out, int d, bool shared, bool backwards) -> int {
-    const bool grouped = shared && G > 1;
-    a.o = grouped ? per_head : out;
-    a.o_f32 = grouped || !bf16;
-    a.oh = d, a.ot = (int64_t)H * d, a.ob = S * a.ot;
-    Q38_HIP(q38::launch_la(a, p.segs, backwards, bf16, st), "linear attention backward launch");
-    if (grouped) Q38_HIP(q38::launch_la_group(per_head, out, p.tokens * Hk, G, d, bf16, st), "linear attention backward launch");
-    if (a.plan != nullptr && S > 0)
+  // Results of Hk heads: added from those of each, which went to the workspace; then zeros for tokens of no sequence.
+  auto finish = [&](void* out, const char* heads, int d, bool shared) -> int {
+    if (out == nullptr || p.tokens == 0) return Q38MOE_OK;
+    if (shared && G > 1)
+      Q38_HIP(q38::launch_la_group(reinterpret_cast<const float*>(heads), out, p.tokens * Hk, G, d, bf16, st),
+              "linear attention backward launch");
+    if (a.plan != nullptr)
       Q38_HIP(q38::launch_la_gap(out, a.plan, (int)N, S, (shared ? Hk : H) * d * (int)elem_size(dtype), st),
               "linear attention backward launch");
     return Q38MOE_OK;
   };
+  auto results = [&](q38::LaArgs& b, void* out, char* heads, int d, bool shared) {
+    b.o = shared && G > 1 && out != nullptr ? heads : out;
+    b.o_f32 = (shared && G > 1) || !bf16;
+    b.oh = d, b.ot = (int64_t)H * d, b.ob = S * b.ot;
+  };
   if (dq != nullptr) {
-    a.q = tdo, a.k = tv, a.v = tk, a.dk = dv, a.dv = dk;
-    a.s0 = initial_state, a.s1 = nullptr, a.turned = true;
-    a.intra = a.inter = scale, a.gain = 1.0f, a.lag = 0;
-    Q38_CHECK(pass(dq, dk, false, false));
+    q38::LaArgs b = a;
+    results(b, dq, nullptr, dk, false);
+    b.q = tdo, b.k = tv, b.v = tk, b.dk = dv, b.dv = dk;
+    b.s0 = initial_state, b.turned = true;
+    b.intra = b.inter = scale, b.gain = 1.0f;
+    if (saved != nullptr) b.mid = static_cast<float*>(const_cast<void*>(saved)), b.mid_turned = true;
+    Q38_HIP(q38::launch_la(b, p.segs, saved == nullptr, bf16, st), "linear attention backward launch");
+    Q38_CHECK(finish(dq, nullptr, dk, false));
   }
+  if (dk_out == nullptr && dv_out == nullptr && d_initial_state == nullptr) return Q38MOE_OK;
+  char *const v_heads = per_head, *const k_heads = per_head + p.grouped_k;
   a.intra = a.gain = scale, a.inter = 1.0f, a.lag = 1;
   a.s0 = d_final_state;
-  if (dk_out != nullptr) {
-    a.q = tv, a.k = tdo, a.v = tq, a.dk = dv, a.dv = dk;
-    a.s1 = nullptr, a.turned = true;
-    Q38_CHECK(pass(dk_out, dk, true, true));
+  if (bf16) {
+    q38::LaBackArgs b;
+    results(a, dv_out, v_heads, dv, true);
+    b.dv_out = a.o;
+    results(a, dk_out, k_heads, dk, true);
+    b.dk_out = a.o;
+    a.k = tq, a.v = tdo, a.dk = dk, a.dv = dv, a.s1 = d_initial_state;
+    b.s = a, b.k = tk, b.v = tv;
+    Q38_HIP(q38::launch_la_back_bf16(b, p.segs, st), "linear attention backward launch");
+  } else {
+    if (dk_out != nullptr) {
+      q38::LaArgs b = a;
+      b.q = tv, b.k = tdo, b.v = tq, b.dk = dv, b.dv = dk, b.turned = true;
+      results(b, dk_out, k_heads, dk, true);
+      Q38_HIP(q38::launch_la_backwards_f32(b, p.segs, st), "linear attention backward launch");
+    }
+    if (dv_out != nullptr || d_initial_state != nullptr) {
+      a.q = tk, a.k = tq, a.v = tdo, a.dk = dk, a.dv = dv, a.s1 = d_initial_state;
+      results(a, dv_out, v_heads, dv, true);
+      Q38_HIP(q38::launch_la_backwards_f32(a, p.segs, st), "linear attention backward launch");
+    }
   }
-  if (dv_out != nullptr || (p.tokens == 0 && d_initial_state != nullptr)) {
-    a.q = tk, a.k = tq, a.v = tdo, a.dk = dk, a.dv = dv;
-    a.s1 = d_initial_state, a.turned = false;
-    Q38_CHECK(pass(dv_out, dv, true, true));
-  } else if (d_initial_state != nullptr) {
-    return fail(Q38MOE_EINVAL, "the initial state's gradient comes with dv");
-  }
-  return Q38MOE_OK;
+  Q38_CHECK(finish(dk_out, k_heads, dk, true));
+  return finish(dv_out, v_heads, dv, true);
 }
 
 int q38moe_linear_attention_step(const void* q, const void* k, const void* v, const int64_t* strides, const float* log_decay,

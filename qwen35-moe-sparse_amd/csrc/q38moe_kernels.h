@@ -276,7 +276,8 @@ struct LaTensor {
 };
 // One pass: o_i = intra sum_{j <= i} e^{g (i - j)} (q_i . k_j) v_j + inter e^{g (i + 1 - lag)} S^T q_i and S = e^{g L} S + gain
 // sum_j e^{g (L - 1 - j + lag)} k_j v_j^T, tokens taken forwards or backwards. s0, s1 (may be NULL): the caller's states [N, H, dk, dv],
-// turned: [N, H, dv, dk]. mid: a state per segment of L tokens. plan (packed sequences) or NULL (N sequences of S tokens, nseg
+// turned: [N, H, dv, dk]. mid: a state per segment of L tokens with another behind it; mid_turned: as a call with dk and dv
+// exchanged left it. plan (packed sequences) or NULL (N sequences of S tokens, nseg
 // segments each).
 struct LaArgs {
   LaTensor q, k, v;
@@ -287,7 +288,14 @@ struct LaArgs {
   const int32_t* plan;
   float intra, inter, gain;
   int lag, N, S, H, dk, dv, L, nseg;
-  bool o_f32, turned;
+  bool o_f32, turned, mid_turned;
+};
+// dk and dv together, bf16: s is the pass that makes dv's state (k = q, v = dO; its q and o unused), and its strides
+// those of dense results [.., H, dk] and [.., H, dv] (either may be NULL).
+struct LaBackArgs {
+  LaArgs s;
+  LaTensor k, v;
+  void *dk_out, *dv_out;
 };
 struct LaStepArgs {
   LaTensor q, k, v;
@@ -303,7 +311,10 @@ int la_segment_tokens(int64_t T, int64_t N, int H);
 int64_t la_padded_state(int dk, int dv);  // elements of a state in mid
 hipError_t launch_la_plan(const int32_t* cu, int32_t* plan, int N, int S, int L, hipStream_t st);
 hipError_t launch_la_gap(void* o, const int32_t* plan, int N, int64_t T, int row_bytes, hipStream_t st);
-hipError_t launch_la(const LaArgs& a, int64_t segs, bool backwards, bool bf16, hipStream_t st);
+// Forwards; states: fills a.mid first (else it is as an earlier call over the same tokens left it).
+hipError_t launch_la(const LaArgs& a, int64_t segs, bool states, bool bf16, hipStream_t st);
+hipError_t launch_la_backwards_f32(const LaArgs& a, int64_t segs, hipStream_t st);
+hipError_t launch_la_back_bf16(const LaBackArgs& a, int64_t segs, hipStream_t st);
 hipError_t launch_la_group(const float* x, void* out, int64_t rows, int G, int d, bool bf16, hipStream_t st);
 hipError_t launch_la_step(const LaStepArgs& a, bool bf16, hipStream_t st);
 

@@ -155,7 +155,8 @@ __global__ __launch_bounds__(256) void la_gap_kernel(void* o, const int32_t* __r
 // 64 rows of features on their way from memory to LDS, zero behind the last row and the last feature.
 template <int BYTES, int THREADS>  // of a row of the tile
 struct LaStage {
-  static constexpr int COLS = BYTES / 16, N = LA_C * COLS / THREADS, ROWS = THREADS / COLS;
+  static constexpr int COLS = BYTES / 16, N = (LA_C * COLS + THREADS - 1) / THREADS, ROWS = THREADS / COLS;
+  static constexpr bool EVEN = N * ROWS == LA_C;
   u32x4_t r[N];
   const uint8_t* at;  // the thread's first piece of the next 64 rows
   int64_t step;       // bytes from row to row, negative backwards
@@ -180,12 +181,14 @@ struct LaStage {
     const bool swap = SWAP && (row & 1);
 #pragma unroll
     for (int i = 0; i < N; ++i)
-      *reinterpret_cast<u32x4_t*>(lds + la_at(row + ROWS * i, col, BYTES)) =
-          swap ? u32x4_t{r[i][2], r[i][3], r[i][0], r[i][1]} : r[i];
+      if (EVEN || row + ROWS * i < LA_C)
+        *reinterpret_cast<u32x4_t*>(lds + la_at(row + ROWS * i, col, BYTES)) =
+            swap ? u32x4_t{r[i][2], r[i][3], r[i][0], r[i][1]} : r[i];
   }
   // The next 64 rows straight into a tile, asynchronously. Places behind the last row or feature get others of the same kind,
   // since a copy cannot leave zeros: rows that are not stored, and features that meet zeros of the state and of the keys.
   __device__ __forceinline__ void copy(int tid, uint8_t* lds, int rows, int bytes) {
+    static_assert(EVEN, "every thread copies");
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const int row = tid / COLS + ROWS * i, col = la_at(row, tid % COLS, 0) >> 4;
@@ -215,6 +218,13 @@ __device__ __forceinline__ int afresh(int x) {
   return x;
 }
 
+// Where a.mid has row `row`, column `col` of a state with NA tiles of rows.
+template <bool BF16, int NA>
+__device__ __forceinline__ int la_place_of(int row, int col) {
+  const int i = BF16 ? 2 * (row >> 5) + ((row >> 2) & 1) : row >> 4, q = BF16 ? (row >> 3) & 3 : (row >> 2) & 3;
+  return (((col >> 4) * NA + i) * 64 + 16 * q + (col & 15)) * 4 + (row & 3);
+}
+
 // Waves on a SIMD that the LDS of la_kernel's workgroups allows, at most 4: the limit of its registers.
 constexpr int la_waves(bool bf16, int dk, int dv, bool out) {
   return bf16 ? (out && dk == 128 && dv == 64 ? 2 : 4) : out && dk == 128 && dv == 64 ? 1 : 2;
@@ -233,12 +243,80 @@ __device__ __forceinline__ int la_row(int i, int q) {
   return BF16 ? 32 * (i >> 1) + 8 * q + 4 * (i & 1) : 16 * i + 4 * q;
 }
 
+// bf16: one unit's scores, weighted and rounded, as an operand. KEYS_SWAPPED: the keys' odd rows lie with the halves of their columns
+// exchanged. row_at: see la_kernel.
+template <int BYTES, bool KEYS_SWAPPED>
+__device__ __forceinline__ u32x4_t la_scores(const uint8_t* keys, const uint8_t* queries, int unit, int lr, int lq,
+                                             const int* row_at, float intra, const float2* tab) {
+  const int t = la_unit_queries(unit), u = la_unit_keys(unit);
+  auto key = [&](const uint8_t* at) {
+    const u32x4_t k = *reinterpret_cast<const u32x4_t*>(at);
+    return KEYS_SWAPPED && (lr & 1) ? u32x4_t{k[2], k[3], k[0], k[1]} : k;
+  };
+  f32x4_t P[2];
+  P[0] = P[1] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+  for (int s = 0; s < BYTES / 64; ++s) {
+    const uint8_t* x = keys + row_at[s & 1] + 128 * (s >> 1) + 32 * BYTES * u;
+    const u32x4_t q = *reinterpret_cast<const u32x4_t*>(queries + row_at[s & 1] + 128 * (s >> 1) + 16 * BYTES * t);
+    P[0] = mfma16x16x32(key(x), q, P[0]);
+    if (2 * u + 1 <= t) P[1] = mfma16x16x32(key(x + 16 * BYTES), q, P[1]);
+  }
+#pragma unroll
+  for (int k = 0; k < 2; ++k)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int n = 16 * (t - 2 * u - k) + lr - 4 * lq - e;  // tokens between key and query
+      P[k][e] = n >= 0 ? P[k][e] * (intra * tab[max(n, 0)].x) : 0.0f;
+    }
+  return la_pack(P[0], P[1]);
+}
+
+// bf16: S = e^{g rows} S + the chunk's k v^T. v: the wave's column's tokens as operands; k: the row-major tile of BYTES a row, its
+// odd rows' halves exchanged. The weighted values are split into three bf16 parts.
+template <int BYTES, int NA>
+__device__ __forceinline__ void la_add(f32x4_t (&S)[NA], const uint8_t* keys, const u32x4_t (&v)[2], float2 full, const float* add,
+                                       const int* column_at, int lq) {
+#pragma unroll
+  for (int i = 0; i < NA; ++i)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) S[i][e] = fmaf(S[i][e], full.x, S[i][e] * full.y);
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    __builtin_amdgcn_sched_barrier(0);
+    u32x4_t part[3];
+#pragma unroll
+    for (int z = 0; z < 4; ++z) {
+      const int n = 32 * u + 16 * (z >> 1) + 4 * lq + 2 * (z & 1);  // token of the first of the two
+      float x0, x1;
+      unpack_bf16x2(v[u][z], x0, x1);
+      x0 *= add[n];
+      x1 *= add[n + 1];
+#pragma unroll
+      for (int y = 0; y < 3; ++y) {
+        const uint32_t b0 = __float_as_uint(x0), b1 = __float_as_uint(x1);
+        part[y][z] = __builtin_amdgcn_perm(b1, b0, 0x07060302u);  // the high halves
+        x0 -= __uint_as_float(b0 & 0xffff0000u);
+        x1 -= __uint_as_float(b1 & 0xffff0000u);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < NA; ++i) {
+      // The reads of few rows at a time: more of them in flight would push the loop's state out of the registers.
+      if (i % 2 == 0) __builtin_amdgcn_sched_barrier(0);
+      const u32x4_t k = la_column<BYTES>(keys + (column_at[(i >> 1) & 1] ^ (8 * (i & 1))) + 128 * (i >> 2) + 32 * BYTES * u);
+#pragma unroll
+      for (int y = 0; y < 3; ++y) S[i] = mfma16x16x32(k, part[y], S[i]);
+    }
+  }
+}
+
 // One segment of one head; DV / 16 waves. Wave w has columns 16 w .. of the state and of the outputs for all 64 queries of a
 // chunk (outputs as [column, query] tiles), and some of the scores' six [32 keys, 16 queries] units, which go through LDS. The
 // state stays in accumulators, which, rounded, are the operand that queries read (la_row). A column's tokens come out of the
 // transposing LDS read in the order in which an accumulator holds the scores' keys, once for the outputs and for the state.
 // Two barriers a chunk: tiles and scores are read behind one, scores and the next tiles written behind the other.
-template <bool BF16, int DK, int DV, int PARTS, bool REV, bool OUT>
+template <bool BF16, int DK, int DV, bool REV, bool OUT>
 __global__ __launch_bounds__(4 * DV, la_waves(BF16, DK, DV, OUT)) void la_kernel(LaArgs a) {
   constexpr int ES = BF16 ? 2 : 4, KB = DK * ES, VB = DV * ES, NA = DK / 16, W = DV / 16, THREADS = 4 * DV;
   __shared__ __attribute__((aligned(16))) uint8_t Ks[LA_C * KB];
@@ -278,7 +356,11 @@ __global__ __launch_bounds__(4 * DV, la_waves(BF16, DK, DV, OUT)) void la_kernel
   for (int i = 0; i < NA; ++i) {
     S[i] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
     if (!OUT) continue;
-    if (p.s > 0) {
+    if (p.s > 0 && a.mid_turned) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        S[i][e] = a.mid[((slot - 1) * a.H + h) * (DK * DV) + la_place_of<BF16, DV / 16>(16 * w + lr, la_row<BF16>(i, lq) + e)];
+    } else if (p.s > 0) {
       S[i] = *mid(slot - 1, i);
     } else if (a.s0 != nullptr) {
 #pragma unroll
@@ -327,42 +409,29 @@ __global__ __launch_bounds__(4 * DV, la_waves(BF16, DK, DV, OUT)) void la_kernel
     if constexpr (OUT) {
       // Scores of queries 16 t + lr with keys 32 u + {4 lq .., 16 + 4 lq ..}, weighted.
       for (int unit = w; unit < LA_UNITS; unit += W) {
-        const int t = la_unit_queries(unit), u = la_unit_keys(unit);
-        f32x4_t P[2];
-        P[0] = P[1] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+        if constexpr (BF16) {
+          *reinterpret_cast<u32x4_t*>(Ps + (unit * 64 + lane) * 16) =
+              la_scores<KB, true>(Ks, Q, unit, lr, lq, row_at, a.intra, tab);
+        } else {
+          const int t = la_unit_queries(unit), u = la_unit_keys(unit);
 #pragma unroll
-        for (int s = 0; s < KB / 64; ++s) {
-          const uint8_t* x = Ks + row_at[s & 1] + 128 * (s >> 1) + 32 * KB * u;
-          if constexpr (BF16) {
-            const u32x4_t q = *reinterpret_cast<const u32x4_t*>(Q + row_at[s & 1] + 128 * (s >> 1) + 16 * KB * t);
-            auto key = [&](const uint8_t* at) {  // odd rows lie with their halves exchanged
-              const u32x4_t k = *reinterpret_cast<const u32x4_t*>(at);
-              return lr & 1 ? u32x4_t{k[2], k[3], k[0], k[1]} : k;
-            };
-            P[0] = mfma16x16x32(key(x), q, P[0]);
-            if (2 * u + 1 <= t) P[1] = mfma16x16x32(key(x + 16 * KB), q, P[1]);
-          } else {
-            const f32x4_t q = *reinterpret_cast<const f32x4_t*>(Q + row_at[s & 1] + 128 * (s >> 1) + 16 * KB * t);
-            const f32x4_t c = *reinterpret_cast<const f32x4_t*>(x), d = *reinterpret_cast<const f32x4_t*>(x + 16 * KB);
+          for (int k = 0; k < 2; ++k) {
+            f32x4_t P = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int s = 0; s < KB / 64; ++s) {
+              const int at = row_at[s & 1] + 128 * (s >> 1);
+              const f32x4_t x = *reinterpret_cast<const f32x4_t*>(Ks + at + 16 * KB * (2 * u + k));
+              const f32x4_t y = *reinterpret_cast<const f32x4_t*>(Q + at + 16 * KB * t);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) P = mfma16x16x4(x[e], y[e], P);
+            }
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              P[0] = mfma16x16x4(c[e], q[e], P[0]);
-              P[1] = mfma16x16x4(d[e], q[e], P[1]);
+              const int n = 16 * (t - 2 * u - k) + lr - 4 * lq - e;  // tokens between key and query
+              P[e] = n >= 0 ? P[e] * (a.intra * tab[max(n, 0)].x) : 0.0f;
             }
+            *reinterpret_cast<f32x4_t*>(Ps + ((2 * unit + k) * 64 + lane) * 16) = P;
           }
-        }
-#pragma unroll
-        for (int k = 0; k < 2; ++k)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int n = 16 * (t - 2 * u - k) + lr - 4 * lq - e;  // tokens between key and query
-            P[k][e] = n >= 0 ? P[k][e] * (a.intra * tab[max(n, 0)].x) : 0.0f;
-          }
-        if constexpr (BF16) {
-          *reinterpret_cast<u32x4_t*>(Ps + (unit * 64 + lane) * 16) = la_pack(P[0], P[1]);
-        } else {
-          *reinterpret_cast<f32x4_t*>(Ps + (2 * unit * 64 + lane) * 16) = P[0];
-          *reinterpret_cast<f32x4_t*>(Ps + ((2 * unit + 1) * 64 + lane) * 16) = P[1];
         }
       }
       // What the queries read from the state.
@@ -403,39 +472,13 @@ __global__ __launch_bounds__(4 * DV, la_waves(BF16, DK, DV, OUT)) void la_kernel
     if (more || keep) {
       const float2 full = tab[rows];
       const float* add = put + LA_C - rows;  // zero behind the last row
-#pragma unroll
-      for (int i = 0; i < NA; ++i)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) S[i][e] = fmaf(S[i][e], full.x, S[i][e] * full.y);
       if constexpr (BF16) {
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          __builtin_amdgcn_sched_barrier(0);
-          u32x4_t part[PARTS];
-#pragma unroll
-          for (int z = 0; z < 4; ++z) {
-            const int n = 32 * u + 16 * (z >> 1) + 4 * lq + 2 * (z & 1);  // token of the first of the two
-            float x0, x1;
-            unpack_bf16x2(v[u][z], x0, x1);
-            x0 *= add[n];
-            x1 *= add[n + 1];
-#pragma unroll
-            for (int y = 0; y < PARTS; ++y) {
-              const uint32_t b0 = __float_as_uint(x0), b1 = __float_as_uint(x1);
-              part[y][z] = __builtin_amdgcn_perm(b1, b0, 0x07060302u);  // the high halves
-              x0 -= __uint_as_float(b0 & 0xffff0000u);
-              x1 -= __uint_as_float(b1 & 0xffff0000u);
-            }
-          }
-#pragma unroll
-          for (int i = 0; i < NA; ++i) {
-            if (i % 4 == 0) __builtin_amdgcn_sched_barrier(0);
-            const u32x4_t k = la_column<KB>(Ks + (column_at[(i >> 1) & 1] ^ (8 * (i & 1))) + 128 * (i >> 2) + 32 * KB * u);
-#pragma unroll
-            for (int y = 0; y < PARTS; ++y) S[i] = mfma16x16x32(k, part[y], S[i]);
-          }
-        }
+        la_add<KB>(S, Ks, v, full, add, column_at, lq);
       } else {
+#pragma unroll
+        for (int i = 0; i < NA; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) S[i][e] = fmaf(S[i][e], full.x, S[i][e] * full.y);
 #pragma unroll
         for (int t = 0; t < 4; ++t)
 #pragma unroll
@@ -490,6 +533,173 @@ __global__ __launch_bounds__(4 * DV, la_waves(BF16, DK, DV, OUT)) void la_kernel
       }
     }
   }
+}
+
+// dk and dv of one segment of one head together, bf16, backwards in time with T = the gradient of the state [dk, dv]:
+//   dv_j = scale sum_{i >= j} e^{g (i - j)} (k_j . q_i) dO_i + e^{g j'} T^T k_j     (j' tokens from the chunk's start, backwards)
+//   dk_j = scale sum_{i >= j} e^{g (i - j)} (v_j . dO_i) q_i + e^{g j'} T v_j
+// DV / 16 waves make dv and hold T as la_kernel's hold S; DK / 16 more make dk and read T, rounded, from LDS, where the first
+// ones leave it once a chunk. One pass over q, k, v and dO instead of two over three of them each, and T made once:
+// 4 x 4096 tokens, 16 heads of 128 (MI355X): see la_run_back.
+template <int DK, int DV>
+__global__ __launch_bounds__(4 * (DK + DV), DK == DV ? 4 : 3) void la_back_kernel(LaBackArgs a) {
+  constexpr int KB = DK * 2, VB = DV * 2, NA = DK / 16, WV = DV / 16, WK = DK / 16, THREADS = 4 * (DK + DV);
+  __shared__ __attribute__((aligned(16))) uint8_t Qs[LA_C * KB], Ks[LA_C * KB], Vs[LA_C * VB], Ds[LA_C * VB];
+  __shared__ __attribute__((aligned(16))) uint8_t Ts[DV * KB];
+  __shared__ __attribute__((aligned(16))) uint8_t Ps[2][LA_UNITS * 1024];
+  __shared__ float2 tab[LA_C + 1];
+  __shared__ float put[2 * LA_C];
+  const int tid = threadIdx.x;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const bool first_waves = w < WV;
+  const int wc = first_waves ? w : w - WV;  // columns 16 wc .. of dv or dk
+  const int seg = (int)(blockIdx.x / a.s.H), h = (int)(blockIdx.x % a.s.H);
+  const LaPlace p = la_place<true>(a.s, seg);
+  if (!p.there) return;
+  const double g = (double)a.s.g[h];
+  if (tid <= LA_C) tab[tid] = la_decay2(g, tid);
+  if (tid < 2 * LA_C) put[tid] = tid < LA_C ? a.s.gain * la_decay2(g, LA_C - tid).x : 0.0f;
+  const int64_t first = a.s.plan == nullptr ? 0 : p.start;
+  const int64_t sb = a.s.plan == nullptr ? p.seq : 0;
+  const int begin = p.s * a.s.L, end = min(p.len, begin + a.s.L);
+  const bool keep = p.s == p.nseg - 1 && a.s.s1 != nullptr;
+  auto start = [&](auto& stage, const LaTensor& t) {
+    const uint8_t* base = static_cast<const uint8_t*>(t.p) + 2 * (sb * t.sb + first * t.st + (int64_t)(h / t.div) * t.sh);
+    stage.start(base + (int64_t)(p.len - 1) * t.st * 2, -t.st * 2, begin);
+  };
+  LaStage<KB, THREADS> qst, kst;
+  LaStage<VB, THREADS> vst, dst;
+  start(qst, a.s.k);
+  start(dst, a.s.v);
+  start(kst, a.k);
+  start(vst, a.v);
+  auto fetch = [&](int rows) {
+    const int tid = afresh((int)threadIdx.x);
+    qst.load(tid, rows, a.s.dk * 2);
+    kst.load(tid, rows, a.s.dk * 2);
+    vst.load(tid, rows, a.s.dv * 2);
+    dst.load(tid, rows, a.s.dv * 2);
+  };
+  auto stage = [&]() {
+    const int tid = afresh((int)threadIdx.x);
+    qst.template store<true>(tid, Qs);
+    kst.template store<false>(tid, Ks);
+    vst.template store<false>(tid, Vs);
+    dst.template store<false>(tid, Ds);
+  };
+
+  f32x4_t T[NA];  // first waves: rows la_row(i, lq) .., column 16 w + lr
+  const int64_t user = ((int64_t)p.seq * a.s.H + h) * a.s.dk * a.s.dv + 16 * w + (tid & 15);
+  {
+    const int lane = tid & 63, lr = lane & 15, lq = lane >> 4;
+#pragma unroll
+    for (int i = 0; i < NA; ++i) {
+      T[i] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+      if (!first_waves) continue;
+      if (p.s > 0) {
+        T[i] = *reinterpret_cast<const f32x4_t*>(a.s.mid + ((la_slot(a.s, p.seq) + p.s - 1) * a.s.H + h) * (DK * DV) +
+                                                 ((w * NA + i) * 64 + lane) * 4);
+      } else if (a.s.s0 != nullptr) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int row = la_row<true>(i, lq) + e;
+          if (row < a.s.dk && 16 * w + lr < a.s.dv) T[i][e] = a.s.s0[user + row * a.s.dv];
+        }
+      }
+    }
+  }
+  auto publish = [&](int lr, int lq) {  // as [dv][dk]
+#pragma unroll
+    for (int u = 0; u < NA / 2; ++u)
+      *reinterpret_cast<u32x4_t*>(Ts + la_at(16 * wc + lr, 4 * u + lq, KB)) = la_pack(T[2 * u], T[2 * u + 1]);
+  };
+  if (begin < end) {
+    fetch(min(LA_C, end - begin));
+    stage();
+    if (first_waves) publish(tid & 15, (tid >> 4) & 3);
+  }
+  for (int j0 = begin; j0 < end; j0 += LA_C) {
+    const int rows = min(LA_C, end - j0);
+    const bool more = j0 + LA_C < end;
+    __syncthreads();
+    if (more) fetch(min(LA_C, end - j0 - LA_C));
+    const int lane = afresh(tid & 63), lr = lane & 15, lq = lane >> 4;
+    f32x4_t o[4];
+    u32x4_t v[2];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) o[t] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    if (first_waves) {
+      const int row_at[2] = {la_at(lr, lq, KB), la_at(lr, 4 + lq, KB)};
+      int column_at[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) column_at[i] = la_at(4 * lq + (lr >> 2), 4 * i + (lr & 3), KB) + 8 * ((lr >> 2) & 1);
+      const int value_at = la_at(4 * lq + (lr >> 2), 2 * wc + ((lr & 3) >> 1), VB) + 8 * (lr & 1);
+      for (int unit = wc; unit < LA_UNITS; unit += WV)
+        *reinterpret_cast<u32x4_t*>(Ps[0] + (unit * 64 + lane) * 16) =
+            la_scores<KB, true>(Qs, Ks, unit, lr, lq, row_at, a.s.intra, tab);
+#pragma unroll
+      for (int s = 0; s < KB / 64; ++s) {
+        const u32x4_t x = la_pack(T[2 * s], T[2 * s + 1]);
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+          o[t] = mfma16x16x32(x, *reinterpret_cast<const u32x4_t*>(Ks + row_at[s & 1] + 128 * (s >> 1) + 16 * KB * t), o[t]);
+      }
+#pragma unroll
+      for (int u = 0; u < 2; ++u) v[u] = la_column<VB>(Ds + value_at + 32 * VB * u);
+      if (more || keep) la_add<KB>(T, Qs, v, tab[rows], put + LA_C - rows, column_at, lq);
+    } else {
+      const int row_at[2] = {la_at(lr, lq, VB), la_at(lr, 4 + lq, VB)};
+      const int value_at = la_at(4 * lq + (lr >> 2), 2 * wc + ((lr & 3) >> 1), KB) + 8 * ((lr ^ (lr >> 2)) & 1);
+      // Row 16 wc + lr of T, columns 32 s + 8 lq .. + 3 and the 4 behind them.
+      int state_at[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) state_at[i] = la_at(8 * lq + 4 * i + (lr >> 2), 2 * wc + ((lr & 3) >> 1), KB) + 8 * (lr & 1);
+      for (int unit = wc; unit < LA_UNITS; unit += WK)
+        *reinterpret_cast<u32x4_t*>(Ps[1] + (unit * 64 + lane) * 16) =
+            la_scores<VB, false>(Ds, Vs, unit, lr, lq, row_at, a.s.intra, tab);
+#pragma unroll
+      for (int s = 0; s < VB / 64; ++s) {
+        const uint2 x = la_read_tr(Ts + state_at[0] + 32 * KB * s), y = la_read_tr(Ts + state_at[1] + 32 * KB * s);
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+          o[t] = mfma16x16x32(u32x4_t{x.x, x.y, y.x, y.y},
+                              *reinterpret_cast<const u32x4_t*>(Vs + row_at[s & 1] + 128 * (s >> 1) + 16 * VB * t), o[t]);
+      }
+#pragma unroll
+      for (int u = 0; u < 2; ++u) v[u] = la_column<KB>(Qs + value_at + 32 * KB * u);
+    }
+    __syncthreads();
+    if (more) {
+      stage();
+      if (first_waves) publish(lr, lq);
+    }
+    const uint8_t* const P = Ps[first_waves ? 0 : 1];
+    const int c = 16 * wc + 4 * lq, d = first_waves ? a.s.dv : a.s.dk;
+    void* const to = first_waves ? a.dv_out : a.dk_out;
+    const int64_t ot = (int64_t)a.s.H * d, out = sb * a.s.S * ot + (first + p.len - 1 - j0 - lr) * ot + (int64_t)h * d + c;
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      o[t] = o[t] * tab[16 * t + lr].x;
+#pragma unroll
+      for (int u = 0; u <= t / 2; ++u)
+        o[t] = mfma16x16x32(v[u], *reinterpret_cast<const u32x4_t*>(P + (la_unit(t, u) * 64 + lane) * 16), o[t]);
+      if (j0 + 16 * t + lr >= end || c >= d || to == nullptr) continue;
+      if (a.s.o_f32)
+        *reinterpret_cast<f32x4_t*>(static_cast<float*>(to) + out - 16 * t * ot) = o[t];
+      else
+        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(to) + out - 16 * t * ot) =
+            make_uint2(pack_bf16x2(o[t][0], o[t][1]), pack_bf16x2(o[t][2], o[t][3]));
+    }
+  }
+  if (!keep || !first_waves) return;
+  const int lr = tid & 15, lq = (tid >> 4) & 3;
+#pragma unroll
+  for (int i = 0; i < NA; ++i)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int row = la_row<true>(i, lq) + e;
+      if (row < a.s.dk && 16 * w + lr < a.s.dv) a.s.s1[user + row * a.s.dv] = T[i][e];
+    }
 }
 
 // mid[s] = e^{g L} (the state before segment s) + mid[s]: the state behind every segment but a sequence's last. A thread has 4
@@ -604,34 +814,71 @@ __global__ __launch_bounds__(256) void la_step_kernel(LaStepArgs a) {
   }
 }
 
-template <bool BF16, int DK, int DV, int PARTS, bool REV>
-hipError_t la_run(const LaArgs& a, int64_t segs, hipStream_t st) {
+// What every segment adds to the state, and the states between them, into a.mid.
+template <bool BF16, int DK, int DV, bool REV>
+hipError_t la_states(const LaArgs& a, int64_t segs, hipStream_t st) {
   const int64_t inner = segs - a.N;  // segments with another behind them, at most
-  if (inner > 0) {
-    hipLaunchKernelGGL((la_kernel<BF16, DK, DV, PARTS, REV, false>), dim3((unsigned)(inner * a.H)), dim3(4 * DV), 0, st, a);
-    hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return e;
-    hipLaunchKernelGGL((la_carry_kernel<BF16, DK, DV>), dim3((unsigned)(a.N * a.H), DK * DV / 1024), dim3(256), 0, st, a);
-    e = hipGetLastError();
-    if (e != hipSuccess) return e;
-  }
-  hipLaunchKernelGGL((la_kernel<BF16, DK, DV, PARTS, REV, true>), dim3((unsigned)(segs * a.H)), dim3(4 * DV), 0, st, a);
+  if (inner == 0) return hipSuccess;
+  hipLaunchKernelGGL((la_kernel<BF16, DK, DV, REV, false>), dim3((unsigned)(inner * a.H)), dim3(4 * DV), 0, st, a);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  hipLaunchKernelGGL((la_carry_kernel<BF16, DK, DV>), dim3((unsigned)(a.N * a.H), DK * DV / 1024), dim3(256), 0, st, a);
   return hipGetLastError();
 }
 
-template <bool BF16, int PARTS, bool REV>
-hipError_t la_run_d(const LaArgs& a, int64_t segs, hipStream_t st) {
-  if (a.dk <= 64)
-    return a.dv <= 64 ? la_run<BF16, 64, 64, PARTS, REV>(a, segs, st) : la_run<BF16, 64, 128, PARTS, REV>(a, segs, st);
-  return a.dv <= 64 ? la_run<BF16, 128, 64, PARTS, REV>(a, segs, st) : la_run<BF16, 128, 128, PARTS, REV>(a, segs, st);
+template <bool BF16, int DK, int DV, bool REV>
+hipError_t la_run(const LaArgs& a, int64_t segs, bool states, hipStream_t st) {
+  if (states) {
+    const hipError_t e = la_states<BF16, DK, DV, REV>(a, segs, st);
+    if (e != hipSuccess) return e;
+  }
+  hipLaunchKernelGGL((la_kernel<BF16, DK, DV, REV, true>), dim3((unsigned)(segs * a.H)), dim3(4 * DV), 0, st, a);
+  return hipGetLastError();
 }
 
-// A state that is an output is made of three bf16 parts (24 bits); one that only queries read, rounded to 8 bits, of two.
-template <bool REV>
-hipError_t la_run_p(const LaArgs& a, int64_t segs, bool bf16, hipStream_t st) {
-  if (!bf16) return la_run_d<false, 1, REV>(a, segs, st);
-  return la_run_d<true, 3, REV>(a, segs, st);
+template <int DK, int DV>
+hipError_t la_run_back(const LaBackArgs& a, int64_t segs, hipStream_t st) {
+  const hipError_t e = la_states<true, DK, DV, true>(a.s, segs, st);
+  if (e != hipSuccess) return e;
+  hipLaunchKernelGGL((la_back_kernel<DK, DV>), dim3((unsigned)(segs * a.s.H)), dim3(4 * (DK + DV)), 0, st, a);
+  return hipGetLastError();
 }
+
+// Calls f<DK, DV>(): the widths up to 64 or 128.
+template <class F>
+hipError_t la_widths(int dk, int dv, F f) {
+  if (dk <= 64) return dv <= 64 ? f.template operator()<64, 64>() : f.template operator()<64, 128>();
+  return dv <= 64 ? f.template operator()<128, 64>() : f.template operator()<128, 128>();
+}
+
+struct LaForwards {
+  const LaArgs& a;
+  int64_t segs;
+  bool states, bf16;
+  hipStream_t st;
+  template <int DK, int DV>
+  hipError_t operator()() const {
+    return bf16 ? la_run<true, DK, DV, false>(a, segs, states, st) : la_run<false, DK, DV, false>(a, segs, states, st);
+  }
+};
+struct LaBackwards {
+  const LaArgs& a;
+  int64_t segs;
+  hipStream_t st;
+  template <int DK, int DV>
+  hipError_t operator()() const {
+    return la_run<false, DK, DV, true>(a, segs, true, st);
+  }
+};
+struct LaBackBoth {
+  const LaBackArgs& a;
+  int64_t segs;
+  hipStream_t st;
+  template <int DK, int DV>
+  hipError_t operator()() const {
+    return la_run_back<DK, DV>(a, segs, st);
+  }
+};
 
 }  // namespace
 
@@ -654,8 +901,16 @@ hipError_t launch_la_gap(void* o, const int32_t* plan, int N, int64_t T, int row
   return hipGetLastError();
 }
 
-hipError_t launch_la(const LaArgs& a, int64_t segs, bool backwards, bool bf16, hipStream_t st) {
-  return backwards ? la_run_p<true>(a, segs, bf16, st) : la_run_p<false>(a, segs, bf16, st);
+hipError_t launch_la(const LaArgs& a, int64_t segs, bool states, bool bf16, hipStream_t st) {
+  return la_widths(a.dk, a.dv, LaForwards{a, segs, states, bf16, st});
+}
+
+hipError_t launch_la_backwards_f32(const LaArgs& a, int64_t segs, hipStream_t st) {
+  return la_widths(a.dk, a.dv, LaBackwards{a, segs, st});
+}
+
+hipError_t launch_la_back_bf16(const LaBackArgs& a, int64_t segs, hipStream_t st) {
+  return la_widths(a.s.dk, a.s.dv, LaBackBoth{a, segs, st});
 }
 
 hipError_t launch_la_group(const float* x, void* out, int64_t rows, int G, int d, bool bf16, hipStream_t st) {

@@ -331,26 +331,28 @@ def qk_norm_rope(q, k, q_norm, k_norm, positions, inv_freq, axes=None, eps=1e-6,
 
 
 class HipLinearAttention(torch.autograd.Function):
-    """Kept are the operands; the backward pass makes the states again (q38moe_linear_attention_forward, _backward)."""
+    """Kept are the operands and the states between segments of the sequences, at most 64 KB for every 64 tokens of a head and
+    about 32 MB where there are many (q38moe_linear_attention_forward, _backward)."""
 
     @staticmethod
     def forward(ctx, q, k, v, log_decay, scale, initial_state, cu_seqlens, return_state):
         ctx.set_materialize_grads(False)
-        ctx.save_for_backward(q, k, v, log_decay, initial_state, cu_seqlens)
+        out, state, saved = ops.linear_attention(q, k, v, log_decay, scale, initial_state, cu_seqlens, return_state, save=True)
+        ctx.save_for_backward(q, k, v, log_decay, initial_state, cu_seqlens, saved)
         ctx.scale = scale
-        return ops.linear_attention(q, k, v, log_decay, scale, initial_state, cu_seqlens, return_state)
+        return out, state
 
     @staticmethod
     @once_differentiable
     def backward(ctx, d_out, d_state):
-        q, k, v, g, S0, cu = ctx.saved_tensors
+        q, k, v, g, S0, cu, saved = ctx.saved_tensors
         needs = ctx.needs_input_grad
         if (d_out is None and d_state is None) or not any(needs):
             return (None,) * 8
         d_out = (torch.zeros(*q.shape[:3], v.shape[3], dtype=q.dtype, device=q.device) if d_out is None
                  else d_out.contiguous())
         dq, dk, dv, ds = ops.linear_attention_backward(d_out, None if d_state is None else d_state.contiguous(), q, k, v, g,
-                                                       ctx.scale, S0, cu, need_state=needs[5])
+                                                       ctx.scale, S0, cu, need_state=needs[5], saved=saved)
         return (dq if needs[0] else None, dk if needs[1] else None, dv if needs[2] else None, None, None, ds, None, None)
 
 

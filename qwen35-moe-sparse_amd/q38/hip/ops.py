@@ -1339,9 +1339,9 @@ class _LinearAttention:
         return (self.q.data_ptr(), self.k.data_ptr(), self.v.data_ptr(), self.strides, self.g.data_ptr(), self.scale,
                 None if self.S0 is None else self.S0.data_ptr(), self.cu.data_ptr() if self.packed else None)
 
-    def workspace(self, backward):
-        n = _linear_attention_workspace_bytes(*self.shape, self.packed, backward, self.dev)
-        return torch.empty(n, dtype=torch.uint8, device=self.dev)
+    def bytes(self, backward):
+        """(workspace, saved states)"""
+        return _linear_attention_bytes(*self.shape, self.packed, backward, self.dev)
 
 
 def _decay(log_decay, H, dev):
@@ -1354,47 +1354,54 @@ def _state(t, name, shape, dev):
 
 
 @functools.lru_cache(maxsize=512)
-def _linear_attention_workspace_bytes(N, S, H, Hk, dk, dv, packed, backward, device):
-    n = ctypes.c_size_t()
-    check(lib.q38moe_linear_attention_workspace_bytes(N, S, H, Hk, dk, dv, packed, backward, ctypes.byref(n)),
-          "q38moe_linear_attention_workspace_bytes")
-    return n.value
+def _linear_attention_bytes(N, S, H, Hk, dk, dv, packed, backward, device):
+    n, saved = ctypes.c_size_t(), ctypes.c_size_t()
+    check(lib.q38moe_linear_attention_workspace_bytes(N, S, H, Hk, dk, dv, packed, backward, ctypes.byref(n),
+                                                      ctypes.byref(saved)), "q38moe_linear_attention_workspace_bytes")
+    return n.value, saved.value
 
 
-def linear_attention(q, k, v, log_decay, scale=None, initial_state=None, cu_seqlens=None, return_state=False):
+def linear_attention(q, k, v, log_decay, scale=None, initial_state=None, cu_seqlens=None, return_state=False, save=False):
     """Linear attention with a decay for each head (q38moe_linear_attention_forward): see ``autograd.linear_attention``.
-    Returns (out [B,S,H,dv], final state [N,H,dk,dv] fp32 or None)."""
+    Returns (out [B,S,H,dv], final state [N,H,dk,dv] fp32 or None), and with save what ``linear_attention_backward`` of the
+    same operands takes as ``saved``."""
     a = _LinearAttention(q, k, v, log_decay, scale, initial_state, cu_seqlens)
     N, S, H, _, dk, dv = a.shape
     out = torch.empty(q.shape[0], S, H, dv, dtype=a.dt, device=a.dev)
     state = torch.empty(N, H, dk, dv, dtype=torch.float32, device=a.dev) if return_state else None
     with _on(a.dev):
-        ws = a.workspace(False)
+        n, states = a.bytes(False)
+        ws = torch.empty(n, dtype=torch.uint8, device=a.dev)
+        saved = torch.empty(states, dtype=torch.uint8, device=a.dev) if save and states else None
         check(lib.q38moe_linear_attention_forward(*a.call(), out.data_ptr(), None if state is None else state.data_ptr(),
-                                                  *a.shape, ws.data_ptr(), ws.numel(), _DTYPES[a.dt],
-                                                  _raw_stream(a.dev.index)), "q38moe_linear_attention_forward")
-    return out, state
+                                                  None if saved is None else saved.data_ptr(), states, *a.shape,
+                                                  ws.data_ptr(), n, _DTYPES[a.dt], _raw_stream(a.dev.index)),
+              "q38moe_linear_attention_forward")
+    return (out, state, saved) if save else (out, state)
 
 
 def linear_attention_backward(d_out, d_final_state, q, k, v, log_decay, scale=None, initial_state=None, cu_seqlens=None,
-                              need_state=False):
+                              need_state=False, saved=None):
     """Gradients (dq, dk, dv, d initial_state or None) of ``linear_attention`` for those of its output and its final state
-    (None: zero)."""
+    (None: zero). saved: what the forward pass kept (None: it is made again)."""
     a = _LinearAttention(q, k, v, log_decay, scale, initial_state, cu_seqlens)
     N, S, H, Hk, dk, dv = a.shape
     B = q.shape[0]
     _heads(_same(d_out, "d_out", a.dt, (B, S, H, dv)), "d_out", a.dt, a.dev)
     d_out = d_out if d_out.data_ptr() % 16 == 0 else d_out.clone()
     _state(d_final_state, "d_final_state", (N, H, dk, dv), a.dev)
+    n, states = a.bytes(True)
+    if saved is not None:
+        _heads(_same(saved, "saved", torch.uint8, (states,)), "saved", torch.uint8, a.dev)
     dq, dk_, dv_ = (torch.empty(B, S, h, d, dtype=a.dt, device=a.dev) for h, d in ((H, dk), (Hk, dk), (Hk, dv)))
     ds = torch.empty(N, H, dk, dv, dtype=torch.float32, device=a.dev) if need_state else None
     with _on(a.dev):
-        ws = a.workspace(True)
+        ws = torch.empty(n, dtype=torch.uint8, device=a.dev)
         check(lib.q38moe_linear_attention_backward(d_out.data_ptr(),
                                                    None if d_final_state is None else d_final_state.data_ptr(), *a.call(),
-                                                   dq.data_ptr(), dk_.data_ptr(), dv_.data_ptr(),
-                                                   None if ds is None else ds.data_ptr(), *a.shape, ws.data_ptr(),
-                                                   ws.numel(), _DTYPES[a.dt], _raw_stream(a.dev.index)),
+                                                   None if saved is None else saved.data_ptr(), states, dq.data_ptr(),
+                                                   dk_.data_ptr(), dv_.data_ptr(), None if ds is None else ds.data_ptr(),
+                                                   *a.shape, ws.data_ptr(), n, _DTYPES[a.dt], _raw_stream(a.dev.index)),
               "q38moe_linear_attention_backward")
     return dq, dk_, dv_, ds
 

@@ -93,7 +93,7 @@ def test_linear_attention_abi_arguments():
 
     def shape(N=2, S=100, H=4, Hk=2, dk=64, dv=64, packed=0, backward=0):
         n = ctypes.c_size_t()
-        rc = lib.q38moe_linear_attention_workspace_bytes(N, S, H, Hk, dk, dv, packed, backward, ctypes.byref(n))
+        rc = lib.q38moe_linear_attention_workspace_bytes(N, S, H, Hk, dk, dv, packed, backward, ctypes.byref(n), None)
         return rc if rc else n.value
 
     assert shape(N=-1) == -1 and says("N must be")
@@ -102,7 +102,7 @@ def test_linear_attention_abi_arguments():
     assert shape(dk=60) == -1 and says("dk must be") and shape(dk=136) == -1 and shape(dk=0) == -1
     assert shape(dv=4) == -1 and says("dv must be")
     assert shape(N=1 << 24, S=1, H=128, Hk=1) == -1 and says("too many")
-    assert shape() == 0                                    # one segment each: nothing to keep
+    assert shape(S=64) == 0                                # one segment each: nothing to keep
     assert shape(packed=1) >= 4 * 7                        # the plan
     assert shape(S=65536, N=1) > 0
     assert shape(backward=1) >= 2 * 100 * 4 * 64 * 4       # a gradient for each head that shares
@@ -111,9 +111,10 @@ def test_linear_attention_abi_arguments():
 
     nine = (ctypes.c_int64 * 9)(25600, 256, 64, 12800, 128, 64, 12800, 128, 64)
 
-    def fwd(q=p, v=p, strides=nine, g=p, cu=None, out=p, N=2, S=100, H=4, ws=p, n=1 << 40, dtype=1):
-        return lib.q38moe_linear_attention_forward(q, p, v, strides, g, 1.0, None, cu, out, None, N, S, H, 2, 64, 64, ws, n,
-                                                   dtype, None)
+    def fwd(q=p, v=p, strides=nine, g=p, cu=None, out=p, N=2, S=100, H=4, ws=p, n=1 << 40, dtype=1, saved=None,
+            sn=0):
+        return lib.q38moe_linear_attention_forward(q, p, v, strides, g, 1.0, None, cu, out, None, saved, sn, N, S, H, 2, 64,
+                                                   64, ws, n, dtype, None)
 
     assert fwd(dtype=7) == -1
     assert fwd(strides=None) == -1 and says("strides")
@@ -124,10 +125,13 @@ def test_linear_attention_abi_arguments():
     assert fwd(N=0, S=8, cu=p) == -1 and says("need a sequence")
     assert fwd(N=1, S=65536, ws=None) == -1 and says("workspace must")
     assert fwd(N=1, S=65536, n=16) == -2 and says("workspace needs")
+    assert fwd(N=1, S=65536, saved=ctypes.c_void_p(8), sn=1 << 40) == -1 and says("saved must be 16-byte")
+    assert fwd(N=1, S=65536, saved=p, sn=16) == -2 and says("saved needs")
     assert fwd(N=0) == 0
 
     def back(do=p, dv=p, ds=None):
-        return lib.q38moe_linear_attention_backward(do, None, p, p, p, nine, p, 1.0, None, None, None, None, dv, ds, 2, 100, 4, 2, 64,
+        return lib.q38moe_linear_attention_backward(do, None, p, p, p, nine, p, 1.0, None, None, None, 0, None, None, dv, ds,
+                                                    2, 100, 4, 2, 64,
                                                     64, p, 1 << 40, 1, None)
 
     assert back(do=None) == -1 and says("d_out")
