@@ -618,7 +618,7 @@ int q38moe_qk_norm_rope_backward(const void* d_q_out, const void* d_k_out, const
  * twice. out [B,H,dv].
  */
 int q38moe_linear_attention_workspace_bytes(int64_t N, int64_t S, int32_t H, int32_t Hk, int32_t dk, int32_t dv, int32_t packed,
-                                            int32_t backward, size_t* bytes, size_t* saved_bytes);
+                                            int32_t backward, int32_t dtype, size_t* bytes, size_t* saved_bytes);
 int q38moe_linear_attention_forward(const void* q, const void* k, const void* v, const int64_t* strides, const float* log_decay,
                                     float scale, const float* initial_state, const int32_t* cu_seqlens, void* out,
                                     float* final_state, void* saved, size_t saved_bytes, int64_t N, int64_t S, int32_t H,

@@ -1894,38 +1894,53 @@ static int check_linattn(int64_t N, int64_t S, int32_t H, int32_t Hk, int32_t dk
   return Q38MOE_OK;
 }
 
-// How a call's sequences are cut, and the parts of its workspace: the plan (packed), the states between segments (forwards: may
-// be the caller's instead), and (backwards, shared heads) fp32 gradients of each head.
-struct LinattnPlan {
+// How sequences are cut into segments, and the bytes of the states between those.
+struct LinattnCut {
   int L, nseg;
-  int64_t tokens, segs;
-  size_t states, mid, grouped, grouped_k, bytes;
+  int64_t segs;
+  size_t states;
+};
+static int linattn_cut(LinattnCut& c, int64_t N, int64_t S, int32_t H, int32_t dk, int32_t dv, bool packed, int per_cu) {
+  c.L = q38::la_segment_tokens(N, S, packed, H, per_cu);
+  c.nseg = packed ? 0 : (int)std::max<int64_t>(1, (S + c.L - 1) / c.L);
+  c.segs = packed ? S / c.L + N : N * c.nseg;
+  if (c.segs * H + S / 64 >= (int64_t)1 << 31) return fail(Q38MOE_EINVAL, "too many sequences and heads for one launch");
+  c.states = sizeof(float) * (size_t)(c.segs - N) * H * (size_t)q38::la_padded_state(dk, dv);
+  return Q38MOE_OK;
+}
+
+// The cuts of a call (back: of dk and dv in one pass, whose workgroups are larger; packed sequences have one plan and so one cut)
+// and the parts of its workspace: the plan (packed), the states (forwards: may be the caller's instead), and (backwards, shared
+// heads) fp32 gradients of each head.
+struct LinattnPlan {
+  LinattnCut cut, back;
+  int64_t tokens;
+  size_t mid, grouped, grouped_k, bytes;
 };
 static int linattn_plan(LinattnPlan& p, int64_t N, int64_t S, int32_t H, int32_t Hk, int32_t dk, int32_t dv, bool packed,
-                        bool backward, bool own_states) {
+                        bool backward, bool own_states, int32_t dtype) {
+  const bool bf16 = dtype == Q38MOE_BF16;
   p.tokens = packed ? S : N * S;
-  p.L = q38::la_segment_tokens(p.tokens, N, H);
-  p.nseg = packed ? 0 : (int)std::max<int64_t>(1, (S + p.L - 1) / p.L);
-  p.segs = packed ? S / p.L + N : N * p.nseg;
-  if (p.segs * H >= (int64_t)1 << 31) return fail(Q38MOE_EINVAL, "too many sequences and heads for one launch");
-  p.states = sizeof(float) * (size_t)(p.segs - N) * H * (size_t)q38::la_padded_state(dk, dv);
+  Q38_CHECK(linattn_cut(p.cut, N, S, H, dk, dv, packed, q38::la_per_cu(bf16, dk, dv, false)));
+  p.back = p.cut;
+  if (bf16 && !packed) Q38_CHECK(linattn_cut(p.back, N, S, H, dk, dv, packed, q38::la_per_cu(bf16, dk, dv, true)));
   const bool grouped = backward && H != Hk;
   p.mid = packed ? align_up(sizeof(int32_t) * (size_t)(3 * N + 1)) : 0;
-  p.grouped = p.mid + (own_states ? align_up(p.states) : 0);
+  p.grouped = p.mid + (own_states ? align_up(backward ? std::max(p.cut.states, p.back.states) : p.cut.states) : 0);
   p.grouped_k = align_up(sizeof(float) * (size_t)p.tokens * H * dv);
   p.bytes = p.grouped + (grouped ? p.grouped_k + sizeof(float) * (size_t)p.tokens * H * dk : 0);
   return Q38MOE_OK;
 }
 
 int q38moe_linear_attention_workspace_bytes(int64_t N, int64_t S, int32_t H, int32_t Hk, int32_t dk, int32_t dv, int32_t packed,
-                                            int32_t backward, size_t* bytes, size_t* saved_bytes) {
+                                            int32_t backward, int32_t dtype, size_t* bytes, size_t* saved_bytes) {
   g_err[0] = 0;
   if (bytes == nullptr) return fail(Q38MOE_EINVAL, "bytes must not be NULL");
-  Q38_CHECK(check_linattn(N, S, H, Hk, dk, dv, Q38MOE_BF16));
+  Q38_CHECK(check_linattn(N, S, H, Hk, dk, dv, dtype));
   LinattnPlan p;
-  Q38_CHECK(linattn_plan(p, N, S, H, Hk, dk, dv, packed != 0, backward != 0, true));
+  Q38_CHECK(linattn_plan(p, N, S, H, Hk, dk, dv, packed != 0, backward != 0, true, dtype));
   *bytes = p.bytes;
-  if (saved_bytes != nullptr) *saved_bytes = p.states;
+  if (saved_bytes != nullptr) *saved_bytes = p.cut.states;
   return Q38MOE_OK;
 }
 
@@ -1935,10 +1950,11 @@ static int linattn_start(LinattnPlan& p, q38::LaArgs& a, const float* log_decay,
                          bool backward, void* workspace, size_t workspace_bytes, int32_t dtype, hipStream_t st) {
   Q38_CHECK(check_linattn(N, S, H, Hk, dk, dv, dtype));
   if (log_decay == nullptr) return fail(Q38MOE_EINVAL, "log_decay must not be NULL");
-  Q38_CHECK(linattn_plan(p, N, S, H, Hk, dk, dv, cu_seqlens != nullptr, backward, backward || saved == nullptr));
+  Q38_CHECK(linattn_plan(p, N, S, H, Hk, dk, dv, cu_seqlens != nullptr, backward, backward || saved == nullptr, dtype));
   if (saved != nullptr) {
     Q38_CHECK(check_ptr(saved, "saved"));
-    if (saved_bytes < p.states) return fail(Q38MOE_EWORKSPACE, "saved needs %zu bytes, got %zu", p.states, saved_bytes);
+    if (saved_bytes < p.cut.states)
+      return fail(Q38MOE_EWORKSPACE, "saved needs %zu bytes, got %zu", p.cut.states, saved_bytes);
   }
   if (p.bytes > 0) {
     Q38_CHECK(check_ptr(workspace, "workspace"));
@@ -1948,11 +1964,11 @@ static int linattn_start(LinattnPlan& p, q38::LaArgs& a, const float* log_decay,
   a = {};
   a.g = log_decay;
   a.mid = reinterpret_cast<float*>(static_cast<char*>(workspace) + p.mid);
-  a.N = (int)N, a.S = (int)S, a.H = H, a.L = p.L, a.nseg = p.nseg;
+  a.N = (int)N, a.S = (int)S, a.H = H, a.L = p.cut.L, a.nseg = p.cut.nseg, a.segs = (int)p.cut.segs;
   (void)hipGetLastError();
   if (cu_seqlens != nullptr) {
     a.plan = static_cast<const int32_t*>(workspace);
-    Q38_HIP(q38::launch_la_plan(cu_seqlens, static_cast<int32_t*>(workspace), (int)N, (int)S, p.L, st), "segments launch");
+    Q38_HIP(q38::launch_la_plan(cu_seqlens, static_cast<int32_t*>(workspace), (int)N, (int)S, p.cut.L, st), "segments launch");
   }
   return Q38MOE_OK;
 }
@@ -1990,9 +2006,7 @@ int q38moe_linear_attention_forward(const void* q, const void* k, const void* v,
   a.intra = a.inter = scale, a.gain = 1.0f, a.lag = 0;
   a.dk = dk, a.dv = dv;
   const bool bf16 = dtype == Q38MOE_BF16;
-  Q38_HIP(q38::launch_la(a, p.segs, true, bf16, st), "linear attention launch");
-  if (a.plan != nullptr && S > 0)
-    Q38_HIP(q38::launch_la_gap(out, a.plan, (int)N, S, H * dv * (int)elem_size(dtype), st), "linear attention launch");
+  Q38_HIP(q38::launch_la(a, true, bf16, st), "linear attention launch");
   return Q38MOE_OK;
 }
 
@@ -2027,15 +2041,11 @@ int q38moe_linear_attention_backward(const void* d_out, const float* d_final_sta
   const int64_t do_strides[3] = {S * (int64_t)H * dv, (int64_t)H * dv, dv};
   const q38::LaTensor tq = la_tensor(q, strides, 1), tk = la_tensor(k, strides + 3, G), tv = la_tensor(v, strides + 6, G),
                       tdo = la_tensor(d_out, do_strides, 1);
-  // Results of Hk heads: added from those of each, which went to the workspace; then zeros for tokens of no sequence.
-  auto finish = [&](void* out, const char* heads, int d, bool shared) -> int {
-    if (out == nullptr || p.tokens == 0) return Q38MOE_OK;
-    if (shared && G > 1)
-      Q38_HIP(q38::launch_la_group(reinterpret_cast<const float*>(heads), out, p.tokens * Hk, G, d, bf16, st),
-              "linear attention backward launch");
-    if (a.plan != nullptr)
-      Q38_HIP(q38::launch_la_gap(out, a.plan, (int)N, S, (shared ? Hk : H) * d * (int)elem_size(dtype), st),
-              "linear attention backward launch");
+  // Results of Hk heads: added from those of each, which went to the workspace.
+  auto finish = [&](void* out, const char* heads, int d) -> int {
+    if (out == nullptr || p.tokens == 0 || G == 1) return Q38MOE_OK;
+    Q38_HIP(q38::launch_la_group(reinterpret_cast<const float*>(heads), out, p.tokens * Hk, G, d, bf16, st),
+            "linear attention backward launch");
     return Q38MOE_OK;
   };
   auto results = [&](q38::LaArgs& b, void* out, char* heads, int d, bool shared) {
@@ -2050,8 +2060,7 @@ int q38moe_linear_attention_backward(const void* d_out, const float* d_final_sta
     b.s0 = initial_state, b.turned = true;
     b.intra = b.inter = scale, b.gain = 1.0f;
     if (saved != nullptr) b.mid = static_cast<float*>(const_cast<void*>(saved)), b.mid_turned = true;
-    Q38_HIP(q38::launch_la(b, p.segs, saved == nullptr, bf16, st), "linear attention backward launch");
-    Q38_CHECK(finish(dq, nullptr, dk, false));
+    Q38_HIP(q38::launch_la(b, saved == nullptr, bf16, st), "linear attention backward launch");
   }
   if (dk_out == nullptr && dv_out == nullptr && d_initial_state == nullptr) return Q38MOE_OK;
   char *const v_heads = per_head, *const k_heads = per_head + p.grouped_k;
@@ -2064,23 +2073,24 @@ int q38moe_linear_attention_backward(const void* d_out, const float* d_final_sta
     results(a, dk_out, k_heads, dk, true);
     b.dk_out = a.o;
     a.k = tq, a.v = tdo, a.dk = dk, a.dv = dv, a.s1 = d_initial_state;
+    a.L = p.back.L, a.nseg = p.back.nseg, a.segs = (int)p.back.segs;
     b.s = a, b.k = tk, b.v = tv;
-    Q38_HIP(q38::launch_la_back_bf16(b, p.segs, st), "linear attention backward launch");
+    Q38_HIP(q38::launch_la_back_bf16(b, st), "linear attention backward launch");
   } else {
     if (dk_out != nullptr) {
       q38::LaArgs b = a;
       b.q = tv, b.k = tdo, b.v = tq, b.dk = dv, b.dv = dk, b.turned = true;
       results(b, dk_out, k_heads, dk, true);
-      Q38_HIP(q38::launch_la_backwards_f32(b, p.segs, st), "linear attention backward launch");
+      Q38_HIP(q38::launch_la_backwards_f32(b, st), "linear attention backward launch");
     }
     if (dv_out != nullptr || d_initial_state != nullptr) {
       a.q = tk, a.k = tq, a.v = tdo, a.dk = dk, a.dv = dv, a.s1 = d_initial_state;
       results(a, dv_out, v_heads, dv, true);
-      Q38_HIP(q38::launch_la_backwards_f32(a, p.segs, st), "linear attention backward launch");
+      Q38_HIP(q38::launch_la_backwards_f32(a, st), "linear attention backward launch");
     }
   }
-  Q38_CHECK(finish(dk_out, k_heads, dk, true));
-  return finish(dv_out, v_heads, dv, true);
+  Q38_CHECK(finish(dk_out, k_heads, dk));
+  return finish(dv_out, v_heads, dv);
 }
 
 int q38moe_linear_attention_step(const void* q, const void* k, const void* v, const int64_t* strides, const float* log_decay,

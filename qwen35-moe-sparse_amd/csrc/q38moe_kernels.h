@@ -278,7 +278,7 @@ struct LaTensor {
 // sum_j e^{g (L - 1 - j + lag)} k_j v_j^T, tokens taken forwards or backwards. s0, s1 (may be NULL): the caller's states [N, H, dk, dv],
 // turned: [N, H, dv, dk]. mid: a state per segment of L tokens with another behind it; mid_turned: as a call with dk and dv
 // exchanged left it. plan (packed sequences) or NULL (N sequences of S tokens, nseg
-// segments each).
+// segments each); segs: at most, of all sequences.
 struct LaArgs {
   LaTensor q, k, v;
   void* o;
@@ -287,7 +287,7 @@ struct LaArgs {
   float *s1, *mid;
   const int32_t* plan;
   float intra, inter, gain;
-  int lag, N, S, H, dk, dv, L, nseg;
+  int lag, N, S, H, dk, dv, L, nseg, segs;
   bool o_f32, turned, mid_turned;
 };
 // dk and dv together, bf16: s is the pass that makes dv's state (k = q, v = dO; its q and o unused), and its strides
@@ -307,14 +307,14 @@ struct LaStepArgs {
   int64_t B, pool;
   int H, dk, dv;
 };
-int la_segment_tokens(int64_t T, int64_t N, int H);
+int la_segment_tokens(int64_t N, int64_t S, bool packed, int H, int per_cu);
+int la_per_cu(bool bf16, int dk, int dv, bool back);
 int64_t la_padded_state(int dk, int dv);  // elements of a state in mid
 hipError_t launch_la_plan(const int32_t* cu, int32_t* plan, int N, int S, int L, hipStream_t st);
-hipError_t launch_la_gap(void* o, const int32_t* plan, int N, int64_t T, int row_bytes, hipStream_t st);
 // Forwards; states: fills a.mid first (else it is as an earlier call over the same tokens left it).
-hipError_t launch_la(const LaArgs& a, int64_t segs, bool states, bool bf16, hipStream_t st);
-hipError_t launch_la_backwards_f32(const LaArgs& a, int64_t segs, hipStream_t st);
-hipError_t launch_la_back_bf16(const LaBackArgs& a, int64_t segs, hipStream_t st);
+hipError_t launch_la(const LaArgs& a, bool states, bool bf16, hipStream_t st);
+hipError_t launch_la_backwards_f32(const LaArgs& a, hipStream_t st);
+hipError_t launch_la_back_bf16(const LaBackArgs& a, hipStream_t st);
 hipError_t launch_la_group(const float* x, void* out, int64_t rows, int G, int d, bool bf16, hipStream_t st);
 hipError_t launch_la_step(const LaStepArgs& a, bool bf16, hipStream_t st);
 

@@ -68,11 +68,13 @@ __device__ __forceinline__ LaPlace la_place(const LaArgs& a, int seg) {
   const int32_t* first = a.plan;
   auto before = [&](int n) { return OUT ? first[n] : first[n] - n; };
   p.there = seg < before(a.N);
-  int lo = 0, hi = a.N - 1;  // the last sequence that starts at or before seg
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (before(mid) <= seg) lo = mid;
-    else hi = mid - 1;
+  // The last sequence that starts at or before seg: the wave's lanes look at 64 places at once.
+  int lo = 0;
+  for (int step = a.N; step > 1;) {
+    const int each = (step + 63) / 64, n = lo + each * ((int)threadIdx.x & 63);
+    const uint64_t at = ballot64(n < min(lo + step, a.N) && before(n) <= seg);
+    lo += each * max(0, 63 - __builtin_clzll(at | 1));
+    step = each;
   }
   p.seq = lo;
   p.s = seg - before(lo);
@@ -142,13 +144,15 @@ __global__ __launch_bounds__(1024) void la_plan_kernel(const int32_t* __restrict
   }
 }
 
-// Rows of [T, heads, dv] that belong to no sequence: zeros.
-__global__ __launch_bounds__(256) void la_gap_kernel(void* o, const int32_t* __restrict__ plan, int N, int64_t T, int row_bytes) {
-  const int64_t from = plan[N + 1], to = plan[N + 1 + N - 1] + plan[2 * N + 1 + N - 1];
-  const int per = row_bytes / 16;
-  for (int64_t r = (int64_t)blockIdx.x * 64; r < min((int64_t)(blockIdx.x + 1) * 64, T); ++r) {
+// Rows 64 block .. of `out` (row_bytes each) that belong to no packed sequence: zeros. The workgroups behind those of the
+// segments do this.
+__device__ __forceinline__ void la_gap(const LaArgs& a, void* out, int row_bytes, int block) {
+  const int32_t* start = a.plan + a.N + 1;
+  const int from = start[0], to = start[a.N - 1] + start[2 * a.N - 1], per = row_bytes / 16;
+  for (int r = 64 * block; r < min(64 * (block + 1), a.S); ++r) {
     if (r >= from && r < to) continue;
-    for (int c = threadIdx.x; c < per; c += 256) st16(static_cast<uint8_t*>(o) + r * row_bytes + 16 * c, u32x4_t{0, 0, 0, 0});
+    for (int c = threadIdx.x; c < per; c += blockDim.x)
+      st16(static_cast<uint8_t*>(out) + (int64_t)r * row_bytes + 16 * c, u32x4_t{0, 0, 0, 0});
   }
 }
 
@@ -327,6 +331,10 @@ __global__ __launch_bounds__(4 * DV, la_waves(BF16, DK, DV, OUT)) void la_kernel
   __shared__ float put[2 * LA_C];   // what a token adds to the state with: of a chunk's 64, then zeros
   const int tid = threadIdx.x, lane = tid & 63, lr = lane & 15, lq = lane >> 4;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  if (OUT && blockIdx.x >= (unsigned)a.segs * a.H) {
+    la_gap(a, a.o, a.H * a.dv * (a.o_f32 ? 4 : ES), blockIdx.x - a.segs * a.H);
+    return;
+  }
   const int seg = (int)(blockIdx.x / a.H), h = (int)(blockIdx.x % a.H);
   const LaPlace p = la_place<OUT>(a, seg);
   if (!p.there) return;
@@ -553,6 +561,12 @@ __global__ __launch_bounds__(4 * (DK + DV), DK == DV ? 4 : 3) void la_back_kerne
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const bool first_waves = w < WV;
   const int wc = first_waves ? w : w - WV;  // columns 16 wc .. of dv or dk
+  if (blockIdx.x >= (unsigned)a.s.segs * a.s.H) {
+    const int block = blockIdx.x - a.s.segs * a.s.H, es = a.s.o_f32 ? 4 : 2;
+    if (a.dk_out != nullptr) la_gap(a.s, a.dk_out, a.s.H * a.s.dk * es, block);
+    if (a.dv_out != nullptr) la_gap(a.s, a.dv_out, a.s.H * a.s.dv * es, block);
+    return;
+  }
   const int seg = (int)(blockIdx.x / a.s.H), h = (int)(blockIdx.x % a.s.H);
   const LaPlace p = la_place<true>(a.s, seg);
   if (!p.there) return;
@@ -814,10 +828,12 @@ __global__ __launch_bounds__(256) void la_step_kernel(LaStepArgs a) {
   }
 }
 
+unsigned la_blocks(const LaArgs& a) { return (unsigned)a.segs * a.H + (a.plan != nullptr ? (unsigned)(a.S + 63) / 64 : 0); }
+
 // What every segment adds to the state, and the states between them, into a.mid.
 template <bool BF16, int DK, int DV, bool REV>
-hipError_t la_states(const LaArgs& a, int64_t segs, hipStream_t st) {
-  const int64_t inner = segs - a.N;  // segments with another behind them, at most
+hipError_t la_states(const LaArgs& a, hipStream_t st) {
+  const int64_t inner = a.segs - a.N;  // segments with another behind them, at most
   if (inner == 0) return hipSuccess;
   hipLaunchKernelGGL((la_kernel<BF16, DK, DV, REV, false>), dim3((unsigned)(inner * a.H)), dim3(4 * DV), 0, st, a);
   const hipError_t e = hipGetLastError();
@@ -827,20 +843,20 @@ hipError_t la_states(const LaArgs& a, int64_t segs, hipStream_t st) {
 }
 
 template <bool BF16, int DK, int DV, bool REV>
-hipError_t la_run(const LaArgs& a, int64_t segs, bool states, hipStream_t st) {
+hipError_t la_run(const LaArgs& a, bool states, hipStream_t st) {
   if (states) {
-    const hipError_t e = la_states<BF16, DK, DV, REV>(a, segs, st);
+    const hipError_t e = la_states<BF16, DK, DV, REV>(a, st);
     if (e != hipSuccess) return e;
   }
-  hipLaunchKernelGGL((la_kernel<BF16, DK, DV, REV, true>), dim3((unsigned)(segs * a.H)), dim3(4 * DV), 0, st, a);
+  hipLaunchKernelGGL((la_kernel<BF16, DK, DV, REV, true>), dim3(la_blocks(a)), dim3(4 * DV), 0, st, a);
   return hipGetLastError();
 }
 
 template <int DK, int DV>
-hipError_t la_run_back(const LaBackArgs& a, int64_t segs, hipStream_t st) {
-  const hipError_t e = la_states<true, DK, DV, true>(a.s, segs, st);
+hipError_t la_run_back(const LaBackArgs& a, hipStream_t st) {
+  const hipError_t e = la_states<true, DK, DV, true>(a.s, st);
   if (e != hipSuccess) return e;
-  hipLaunchKernelGGL((la_back_kernel<DK, DV>), dim3((unsigned)(segs * a.s.H)), dim3(4 * (DK + DV)), 0, st, a);
+  hipLaunchKernelGGL((la_back_kernel<DK, DV>), dim3(la_blocks(a.s)), dim3(4 * (DK + DV)), 0, st, a);
   return hipGetLastError();
 }
 
@@ -853,40 +869,46 @@ hipError_t la_widths(int dk, int dv, F f) {
 
 struct LaForwards {
   const LaArgs& a;
-  int64_t segs;
   bool states, bf16;
   hipStream_t st;
   template <int DK, int DV>
   hipError_t operator()() const {
-    return bf16 ? la_run<true, DK, DV, false>(a, segs, states, st) : la_run<false, DK, DV, false>(a, segs, states, st);
+    return bf16 ? la_run<true, DK, DV, false>(a, states, st) : la_run<false, DK, DV, false>(a, states, st);
   }
 };
 struct LaBackwards {
   const LaArgs& a;
-  int64_t segs;
   hipStream_t st;
   template <int DK, int DV>
   hipError_t operator()() const {
-    return la_run<false, DK, DV, true>(a, segs, true, st);
+    return la_run<false, DK, DV, true>(a, true, st);
   }
 };
 struct LaBackBoth {
   const LaBackArgs& a;
-  int64_t segs;
   hipStream_t st;
   template <int DK, int DV>
   hipError_t operator()() const {
-    return la_run_back<DK, DV>(a, segs, st);
+    return la_run_back<DK, DV>(a, st);
   }
 };
 
 }  // namespace
 
-int la_segment_tokens(int64_t T, int64_t N, int H) {
-  // As many segments as give every CU two workgroups.
-  const int64_t want = std::max<int64_t>(1, 2 * (int64_t)device_cus() / H);
-  const int64_t chunks = (T + LA_C * want - 1) / (LA_C * want);
-  return (int)std::min<int64_t>(std::max<int64_t>(chunks, 1), 1 << 20) * LA_C;
+// As long segments as still give every CU the workgroups that it holds, `per_cu`: more segments cost more states to write and read
+// (64 KB at widths of 128, as much as 64 tokens' queries to outputs), fewer leave CUs idle. Of packed sequences half a
+// segment each is taken to be lost to their ends. 4 x 4096 tokens x 16 heads of 128 forward and back with 1, 2, 4, 8 a CU:
+// 341, 339, 395, 513 us; 65536 tokens forward 447, 400, 433, 484.
+int la_segment_tokens(int64_t N, int64_t S, bool packed, int H, int per_cu) {
+  const int64_t want = std::max<int64_t>(1, (int64_t)per_cu * device_cus() / H), chunks = std::max<int64_t>(1, (S + LA_C - 1) / LA_C);
+  const int64_t n = packed ? std::max({want - N / 2, want / 2, (int64_t)1}) : std::max<int64_t>(1, want / std::max<int64_t>(1, N));
+  return (int)((chunks + n - 1) / n) * LA_C;
+}
+
+// Workgroups of la_kernel, or of la_back_kernel, on a CU, by their LDS and registers.
+int la_per_cu(bool bf16, int dk, int dv, bool back) {
+  const bool narrow = dk <= 64 && dv <= 64;
+  return back ? (narrow ? 2 : 1) : bf16 ? (narrow ? 4 : 2) : narrow ? 2 : 1;
 }
 
 int64_t la_padded_state(int dk, int dv) { return (int64_t)(dk <= 64 ? 64 : 128) * (dv <= 64 ? 64 : 128); }
@@ -896,21 +918,16 @@ hipError_t launch_la_plan(const int32_t* cu, int32_t* plan, int N, int S, int L,
   return hipGetLastError();
 }
 
-hipError_t launch_la_gap(void* o, const int32_t* plan, int N, int64_t T, int row_bytes, hipStream_t st) {
-  hipLaunchKernelGGL(la_gap_kernel, dim3((unsigned)((T + 63) / 64)), dim3(256), 0, st, o, plan, N, T, row_bytes);
-  return hipGetLastError();
+hipError_t launch_la(const LaArgs& a, bool states, bool bf16, hipStream_t st) {
+  return la_widths(a.dk, a.dv, LaForwards{a, states, bf16, st});
 }
 
-hipError_t launch_la(const LaArgs& a, int64_t segs, bool states, bool bf16, hipStream_t st) {
-  return la_widths(a.dk, a.dv, LaForwards{a, segs, states, bf16, st});
+hipError_t launch_la_backwards_f32(const LaArgs& a, hipStream_t st) {
+  return la_widths(a.dk, a.dv, LaBackwards{a, st});
 }
 
-hipError_t launch_la_backwards_f32(const LaArgs& a, int64_t segs, hipStream_t st) {
-  return la_widths(a.dk, a.dv, LaBackwards{a, segs, st});
-}
-
-hipError_t launch_la_back_bf16(const LaBackArgs& a, int64_t segs, hipStream_t st) {
-  return la_widths(a.s.dk, a.s.dv, LaBackBoth{a, segs, st});
+hipError_t launch_la_back_bf16(const LaBackArgs& a, hipStream_t st) {
+  return la_widths(a.s.dk, a.s.dv, LaBackBoth{a, st});
 }
 
 hipError_t launch_la_group(const float* x, void* out, int64_t rows, int G, int d, bool bf16, hipStream_t st) {

@@ -102,7 +102,7 @@ SIGNATURES = {
     "q38moe_qk_norm_rope_workspace_bytes": (_c_int, [_c_i64] + [_c_i32] * 4 + [ctypes.POINTER(_c_size)]),
     "q38moe_qk_norm_rope_backward": (_c_int, [_vp] * 7 + [_c_i32, _vp, _c_i32, _vp, _c_i32] + [_vp] * 5 + [_c_i64] +
                                      [_c_i32] * 4 + [ctypes.c_float, _vp, _c_size, _c_i32, _vp]),
-    "q38moe_linear_attention_workspace_bytes": (_c_int, [_c_i64] * 2 + [_c_i32] * 6 + [ctypes.POINTER(_c_size)] * 2),
+    "q38moe_linear_attention_workspace_bytes": (_c_int, [_c_i64] * 2 + [_c_i32] * 7 + [ctypes.POINTER(_c_size)] * 2),
     "q38moe_linear_attention_forward": (_c_int, [_vp] * 5 + [ctypes.c_float] + [_vp] * 5 + [_c_size] + [_c_i64] * 2 + [_c_i32] * 4 +
                                         [_vp, _c_size, _c_i32, _vp]),
     "q38moe_linear_attention_backward": (_c_int, [_vp] * 7 + [ctypes.c_float] + [_vp] * 3 + [_c_size] + [_vp] * 4 + [_c_i64] * 2 + [_c_i32] * 4 +

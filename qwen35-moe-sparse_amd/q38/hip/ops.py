@@ -1341,7 +1341,7 @@ class _LinearAttention:
 
     def bytes(self, backward):
         """(workspace, saved states)"""
-        return _linear_attention_bytes(*self.shape, self.packed, backward, self.dev)
+        return _linear_attention_bytes(*self.shape, self.packed, backward, self.dt, self.dev)
 
 
 def _decay(log_decay, H, dev):
@@ -1354,9 +1354,9 @@ def _state(t, name, shape, dev):
 
 
 @functools.lru_cache(maxsize=512)
-def _linear_attention_bytes(N, S, H, Hk, dk, dv, packed, backward, device):
+def _linear_attention_bytes(N, S, H, Hk, dk, dv, packed, backward, dt, device):
     n, saved = ctypes.c_size_t(), ctypes.c_size_t()
-    check(lib.q38moe_linear_attention_workspace_bytes(N, S, H, Hk, dk, dv, packed, backward, ctypes.byref(n),
+    check(lib.q38moe_linear_attention_workspace_bytes(N, S, H, Hk, dk, dv, packed, backward, _DTYPES[dt], ctypes.byref(n),
                                                       ctypes.byref(saved)), "q38moe_linear_attention_workspace_bytes")
     return n.value, saved.value
 

@@ -93,7 +93,7 @@ def test_linear_attention_abi_arguments():
 
     def shape(N=2, S=100, H=4, Hk=2, dk=64, dv=64, packed=0, backward=0):
         n = ctypes.c_size_t()
-        rc = lib.q38moe_linear_attention_workspace_bytes(N, S, H, Hk, dk, dv, packed, backward, ctypes.byref(n), None)
+        rc = lib.q38moe_linear_attention_workspace_bytes(N, S, H, Hk, dk, dv, packed, backward, 1, ctypes.byref(n), None)
         return rc if rc else n.value
 
     assert shape(N=-1) == -1 and says("N must be")
