@@ -308,9 +308,11 @@ class HipQkNormRope(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, d_q_out, d_k_out):
-        grads = ops.qk_norm_rope_backward(d_q_out.contiguous(), d_k_out.contiguous(), *ctx.saved_tensors, *ctx.rest,
-                                          need_norms=ctx.needs_input_grad[2:4])
-        return *(g if need else None for g, need in zip(grads, ctx.needs_input_grad)), None, None, None, None, None
+        # The gradients have the outputs' types, shapes and device: autograd sees to that, and the forward has looked at the rest.
+        saved, needs = ctx.saved_tensors, ctx.needs_input_grad
+        dq, dk, dwq, dwk = ops._qk_norm_rope_backward(d_q_out.contiguous(), d_k_out.contiguous(), *saved, *ctx.rest, needs[2:4],
+                                                      saved[0].device)
+        return dq if needs[0] else None, dk if needs[1] else None, dwq, dwk, None, None, None, None, None
 
 
 def qk_norm_rope(q, k, q_norm, k_norm, positions, inv_freq, axes=None, eps=1e-6, unit_offset=True):
@@ -325,7 +327,9 @@ def qk_norm_rope(q, k, q_norm, k_norm, positions, inv_freq, axes=None, eps=1e-6,
     if _bf16_autocast():
         q, k, q_norm, k_norm = (t if t is None else t.to(torch.bfloat16) for t in (q, k, q_norm, k_norm))
     positions = positions.contiguous()
-    if _recorded(*(t for t in (q, k, q_norm, k_norm) if t is not None)):
+    if forward_ad._current_level >= 0 or (torch.is_grad_enabled() and (
+            q.requires_grad or k.requires_grad or (q_norm is not None and q_norm.requires_grad)
+            or (k_norm is not None and k_norm.requires_grad))):
         return HipQkNormRope.apply(q, k, q_norm, k_norm, positions, inv_freq, axes, eps, unit_offset)
     return ops.qk_norm_rope(q, k, q_norm, k_norm, positions, inv_freq, axes, eps, unit_offset)
 
@@ -351,8 +355,8 @@ class HipLinearAttention(torch.autograd.Function):
             return (None,) * 8
         d_out = (torch.zeros(*q.shape[:3], v.shape[3], dtype=q.dtype, device=q.device) if d_out is None
                  else d_out.contiguous())
-        dq, dk, dv, ds = ops.linear_attention_backward(d_out, None if d_state is None else d_state.contiguous(), q, k, v, g,
-                                                       ctx.scale, S0, cu, need_state=needs[5], saved=saved)
+        dq, dk, dv, ds = ops._linear_attention_backward(d_out, None if d_state is None else d_state.contiguous(), q, k, v, g,
+                                                        ctx.scale, S0, cu, needs[5], saved, q.device)
         return (dq if needs[0] else None, dk if needs[1] else None, dv if needs[2] else None, None, None, ds, None, None)
 
 
@@ -373,6 +377,8 @@ def linear_attention(q, k, v, log_decay, scale=None, initial_state=None, cu_seql
         q, k, v = (t.to(torch.bfloat16) for t in (q, k, v))
     if initial_state is not None:
         initial_state = initial_state.contiguous()
-    if _recorded(*((q, k, v) if initial_state is None else (q, k, v, initial_state))):
+    if forward_ad._current_level >= 0 or (torch.is_grad_enabled() and (
+            q.requires_grad or k.requires_grad or v.requires_grad
+            or (initial_state is not None and initial_state.requires_grad))):
         return HipLinearAttention.apply(q, k, v, log_decay, scale, initial_state, cu_seqlens, return_state)
     return ops.linear_attention(q, k, v, log_decay, scale, initial_state, cu_seqlens, return_state)

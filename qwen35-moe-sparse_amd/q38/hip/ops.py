@@ -1156,25 +1156,24 @@ def _collect_rows(rows, plan, w, pw):
 
 
 # ---- a token mixer with a carried state: normed and rotated heads, linear attention, its step ----------------------
+# What a call's shapes, strides and types say is looked at once for each and kept (_rope_plan, _mix_plan, _step_plan):
+# looking again at every call costs the host as much as the launches.
 
-def _rows16(t, lead):
-    """t with its first ``lead`` dimensions in place, or a copy of it, whose last dimension is dense and whose rows start on
-    16-byte boundaries."""
-    size = t.element_size()
-    if t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(s * size % 16 == 0 for s in t.stride()[:lead]):
-        return t
-    t = t.contiguous()
-    return t if t.data_ptr() % 16 == 0 else t.clone()
+def _tensors(**named):
+    for name, t in named.items():
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{name} must be a tensor, got {type(t)}")
 
 
-def _heads(t, name, dt, dev, dims=None):
-    if not isinstance(t, torch.Tensor) or t.dtype != dt:
-        raise TypeError(f"{name} must be {dt}, got {getattr(t, 'dtype', type(t))}")
-    if t.device != dev:
-        raise RuntimeError(f"{name} must be on {dev}, got {t.device}")
-    if dims is not None and t.dim() != dims:
-        raise ValueError(f"{name} must have {dims} dims, got shape {tuple(t.shape)}")
-    return t
+def _one_gpu(q, *others):
+    """q's device, which must be that of the others (None: left out) and a GPU."""
+    at = q.get_device()
+    if at < 0:
+        raise RuntimeError("q must be a CUDA/HIP tensor")
+    for t in others:
+        if t is not None and t.get_device() != at:
+            raise RuntimeError(f"every tensor must be on {q.device}, got one on {t.device}")
+    return q.device
 
 
 def _head_dim(d, name, most):
@@ -1182,10 +1181,36 @@ def _head_dim(d, name, most):
         raise ValueError(f"{name} must be a multiple of 8 up to {most}, got {d}")
 
 
-def _on_gpu(t, name):
-    if t.device.type != "cuda":
-        raise RuntimeError(f"{name} must be a CUDA/HIP tensor")
-    return t.device
+def _float_type(dt, name):
+    if dt not in _DTYPES:
+        raise TypeError(f"{name} must be a bf16 or fp32 tensor, got {dt}")
+    return 2 if dt == torch.bfloat16 else 4
+
+
+def _rows_stride(shape, stride, size):
+    """Strides (row, head) of rows [..., heads, d] whose leading dimensions run on as one and that start on 16-byte boundaries;
+    None where they do not."""
+    if 0 in shape:
+        return 0, 0
+    row, span = 0, None
+    for n, s in zip(shape[-3::-1], stride[-3::-1]):
+        if n == 1:
+            continue
+        if span is None:
+            row = s
+        elif s != span:
+            return None
+        span = s * n
+    head = stride[-2] if shape[-2] > 1 else 0
+    if stride[-1] != 1 or row * size % 16 or head * size % 16:
+        return None
+    return row, head
+
+
+def _dense(t):
+    """A copy of t that the kernels take."""
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
 def rope_axis_map(sections, interleaved=True, device=None):
@@ -1205,67 +1230,89 @@ def rope_axis_map(sections, interleaved=True, device=None):
     return torch.tensor(found, dtype=torch.int32, device=device)
 
 
-class _Rope:
-    """The checked operands of a rotation: q [T,H,d] and k [T,KV,d] (views where they can be), the rest of the C call."""
+@functools.lru_cache(maxsize=1024)
+def _rope_plan(dt, k_dt, qs, ks, q_stride, k_stride, norms, pos, pos_dt, freqs, freq_dt, axes, axes_dt):
+    """((T, H, KV, d, rot), number of axes, strides as C takes them or None where q or k has to be copied)."""
+    size = _float_type(dt, "q")
+    if k_dt != dt:
+        raise TypeError(f"k must be {dt}, got {k_dt}")
+    if len(qs) < 2 or len(ks) != len(qs) or ks[:-2] != qs[:-2] or ks[-1] != qs[-1] or 0 in (qs[-2], ks[-2]):
+        raise ValueError(f"q [..., H, d] and k [..., KV, d] do not match: {tuple(qs)} and {tuple(ks)}")
+    lead, (H, d), KV = tuple(qs[:-2]), qs[-2:], ks[-2]
+    _head_dim(d, "the head width", 256)
+    for name, shape, w_dt in norms:
+        if w_dt != dt:
+            raise TypeError(f"{name} must be {dt}, got {w_dt}")
+        if shape != (d,):
+            raise ValueError(f"{name} must be ({d},), got {tuple(shape)}")
+    if freq_dt != torch.float32:
+        raise TypeError(f"inv_freq must be {torch.float32}, got {freq_dt}")
+    rot = 2 * math.prod(freqs)
+    if len(freqs) != 1 or rot > d or rot % 8:
+        raise ValueError(f"inv_freq must hold a multiple of 4 frequencies up to {d // 2}, got {tuple(freqs)}")
+    if pos_dt not in (torch.int32, torch.int64):
+        raise TypeError(f"positions must be int32 or int64, got {pos_dt}")
+    n = 1
+    if axes is None:
+        if pos != lead:
+            raise ValueError(f"positions must be {lead}, got {tuple(pos)}")
+    else:
+        if axes_dt != torch.int32 or axes != (rot // 2,):
+            raise ValueError(f"axes must be int32 [{rot // 2}], got {axes_dt} {tuple(axes)}")
+        if len(pos) != len(lead) + 1 or pos[1:] != lead or not 1 <= pos[0] <= 4:
+            raise ValueError(f"positions must be [1 to 4 axes, *{lead}], got {tuple(pos)}")
+        n = pos[0]
+    q_row, k_row = _rows_stride(qs, q_stride, size), _rows_stride(ks, k_stride, size)
+    strides = None if q_row is None or k_row is None else (ctypes.c_int64 * 4)(*q_row, *k_row)
+    return (math.prod(lead), H, KV, d, rot), n, strides
 
-    __slots__ = ("q", "k", "T", "H", "KV", "d", "rot", "dt", "dev", "strides", "head", "tail")
 
-    def __init__(self, q, k, q_norm, k_norm, positions, inv_freq, axes, eps, unit_offset):
-        dt = self.dt = _fdt(q, "q")
-        dev = self.dev = _on_gpu(q, "q")
-        _heads(k, "k", dt, dev)
-        if q.dim() < 2 or k.dim() != q.dim() or k.shape[:-2] != q.shape[:-2] or k.shape[-1] != q.shape[-1]:
-            raise ValueError(f"q [..., H, d] and k [..., KV, d] do not match: {tuple(q.shape)} and {tuple(k.shape)}")
-        lead = q.shape[:-2]
-        H, d = q.shape[-2:]
-        KV = k.shape[-2]
-        _head_dim(d, "the head width", 256)
-        self.T, self.H, self.KV, self.d = math.prod(lead), H, KV, d
-        for w, name in ((q_norm, "q_norm"), (k_norm, "k_norm")):
-            if w is not None:
-                _same(w, name, dt, (d,))
-                _heads(w, name, dt, dev)
-        _need(inv_freq, "inv_freq", dtype=torch.float32, ndim=1)
-        rot = self.rot = 2 * inv_freq.shape[0]
-        if rot > d or rot % 8:
-            raise ValueError(f"inv_freq must hold a multiple of 4 frequencies up to {d // 2}, got {inv_freq.shape[0]}")
-        _need(positions, "positions", dtype=None)
-        if positions.dtype not in (torch.int32, torch.int64):
-            raise TypeError(f"positions must be int32 or int64, got {positions.dtype}")
-        n = 1
-        if axes is None:
-            if positions.shape != lead:
-                raise ValueError(f"positions must be {tuple(lead)}, got {tuple(positions.shape)}")
-        else:
-            _same(axes, "axes", torch.int32, (rot // 2,))
-            if positions.dim() != q.dim() - 1 or positions.shape[1:] != lead or not 1 <= positions.shape[0] <= 4:
-                raise ValueError(f"positions must be [1 to 4 axes, {', '.join(map(str, lead))}], got {tuple(positions.shape)}")
-            n = positions.shape[0]
-        if inv_freq.device != dev or positions.device != dev or (axes is not None and axes.device != dev):
-            raise RuntimeError("q, positions, inv_freq and axes must be on one device")
-        q, k = (_rows16(t.reshape(self.T, t.shape[-2], d), 2) for t in (q, k))
-        self.q, self.k = q, k
-        self.strides = (ctypes.c_int64 * 4)(q.stride(0), q.stride(1), k.stride(0), k.stride(1))
-        self.head = (q.data_ptr(), k.data_ptr(), self.strides, None if q_norm is None else q_norm.data_ptr(),
-                     None if k_norm is None else k_norm.data_ptr(), bool(unit_offset), positions.data_ptr(),
-                     positions.dtype == torch.int64, None if axes is None else axes.data_ptr(), n, inv_freq.data_ptr())
-        self.tail = (self.T, H, KV, d, rot, eps)
+def _rope_operands(q, k, q_norm, k_norm, positions, inv_freq, axes, unit_offset):
+    """q and k (copies where the kernels cannot take them as they lie), the sizes and the first arguments of the C calls."""
+    norms = ()
+    if q_norm is not None:
+        norms += (("q_norm", q_norm.shape, q_norm.dtype),)
+    if k_norm is not None:
+        norms += (("k_norm", k_norm.shape, k_norm.dtype),)
+    rest = (norms, positions.shape, positions.dtype, inv_freq.shape, inv_freq.dtype, None if axes is None else axes.shape,
+            None if axes is None else axes.dtype)
+    sizes, n, strides = _rope_plan(q.dtype, k.dtype, q.shape, k.shape, q.stride(), k.stride(), *rest)
+    pq, pk = q.data_ptr(), k.data_ptr()
+    if strides is None or (pq | pk) & 15:
+        q, k = _dense(q), _dense(k)
+        _, _, strides = _rope_plan(q.dtype, k.dtype, q.shape, k.shape, q.stride(), k.stride(), *rest)
+        pq, pk = q.data_ptr(), k.data_ptr()
+    return q, k, sizes, (pq, pk, strides, None if q_norm is None else q_norm.data_ptr(),
+                         None if k_norm is None else k_norm.data_ptr(), unit_offset, positions.data_ptr(),
+                         positions.dtype == torch.int64, None if axes is None else axes.data_ptr(), n, inv_freq.data_ptr())
 
 
 def _norm_weight(w):
     """A norm's weight (or None) as the kernels take it."""
-    return w if w is None or (w.is_contiguous() and w.data_ptr() % 16 == 0) else w.contiguous().clone()
+    return w if w is None or (w.is_contiguous() and w.data_ptr() % 16 == 0) else _dense(w)
+
+
+def _rope_check(q, k, q_norm, k_norm, positions, inv_freq, axes):
+    """What shapes and types leave open: tensors, one GPU, positions, frequencies and axes contiguous."""
+    _tensors(q=q, k=k, positions=positions, inv_freq=inv_freq)
+    _float_type(q.dtype, "q")
+    dev = _one_gpu(q, k, q_norm, k_norm, positions, inv_freq, axes)
+    if not (positions.is_contiguous() and inv_freq.is_contiguous() and (axes is None or axes.is_contiguous())):
+        raise ValueError("positions, inv_freq and axes must be contiguous")
+    return dev
 
 
 def qk_norm_rope(q, k, q_norm, k_norm, positions, inv_freq, axes=None, eps=1e-6, unit_offset=True):
     """RMS norm of every query and key head and rotation by position in one pass (q38moe_qk_norm_rope): see
     ``autograd.qk_norm_rope``. Returns contiguous (q [..., H, d], k [..., KV, d])."""
+    dev = _rope_check(q, k, q_norm, k_norm, positions, inv_freq, axes)
     q_norm, k_norm = _norm_weight(q_norm), _norm_weight(k_norm)
-    p = _Rope(q, k, q_norm, k_norm, positions, inv_freq, axes, eps, unit_offset)
-    qo, ko = torch.empty(q.shape, dtype=p.dt, device=p.dev), torch.empty(k.shape, dtype=p.dt, device=p.dev)
-    with _on(p.dev):
-        check(lib.q38moe_qk_norm_rope(*p.head, qo.data_ptr(), ko.data_ptr(), *p.tail, _DTYPES[p.dt],
-                                      _raw_stream(p.dev.index)), "q38moe_qk_norm_rope")
+    q, k, sizes, head = _rope_operands(q, k, q_norm, k_norm, positions, inv_freq, axes, unit_offset)
+    dt = q.dtype
+    qo, ko = torch.empty(q.shape, dtype=dt, device=dev), torch.empty(k.shape, dtype=dt, device=dev)
+    with _on(dev):
+        check(lib.q38moe_qk_norm_rope(*head, qo.data_ptr(), ko.data_ptr(), *sizes, eps, _DTYPES[dt],
+                                      _raw_stream(dev.index)), "q38moe_qk_norm_rope")
     return qo, ko
 
 
@@ -1281,102 +1328,141 @@ def qk_norm_rope_backward(d_q_out, d_k_out, q, k, q_norm, k_norm, positions, inv
                           unit_offset=True, need_norms=(True, True)):
     """Gradients (dq, dk, d q_norm, d k_norm) of ``qk_norm_rope``'s outputs for theirs; the weights' are None where there is no
     weight or need_norms says so."""
+    dev = _rope_check(q, k, q_norm, k_norm, positions, inv_freq, axes)
+    _tensors(d_q_out=d_q_out, d_k_out=d_k_out)
+    _one_gpu(q, d_q_out, d_k_out)
+    _same(d_q_out, "d_q_out", q.dtype, q.shape)
+    _same(d_k_out, "d_k_out", q.dtype, k.shape)
+    return _qk_norm_rope_backward(d_q_out, d_k_out, q, k, q_norm, k_norm, positions, inv_freq, axes, eps, unit_offset, need_norms,
+                                  dev)
+
+
+def _qk_norm_rope_backward(d_q_out, d_k_out, q, k, q_norm, k_norm, positions, inv_freq, axes, eps, unit_offset, need_norms, dev):
+    """qk_norm_rope_backward of operands that have been looked at."""
     q_norm, k_norm = _norm_weight(q_norm), _norm_weight(k_norm)
-    p = _Rope(q, k, q_norm, k_norm, positions, inv_freq, axes, eps, unit_offset)
-    for g, t, name in ((d_q_out, q, "d_q_out"), (d_k_out, k, "d_k_out")):
-        _heads(_same(g, name, p.dt, t.shape), name, p.dt, p.dev)
-    d_q_out, d_k_out = (g if g.data_ptr() % 16 == 0 else g.clone() for g in (d_q_out, d_k_out))
-    dq, dk = torch.empty(q.shape, dtype=p.dt, device=p.dev), torch.empty(k.shape, dtype=p.dt, device=p.dev)
+    q, k, sizes, head = _rope_operands(q, k, q_norm, k_norm, positions, inv_freq, axes, unit_offset)
+    pdq, pdk = d_q_out.data_ptr(), d_k_out.data_ptr()
+    if (pdq | pdk) & 15:
+        d_q_out, d_k_out = _dense(d_q_out), _dense(d_k_out)
+        pdq, pdk = d_q_out.data_ptr(), d_k_out.data_ptr()
+    dt = q.dtype
+    dq, dk = torch.empty(q.shape, dtype=dt, device=dev), torch.empty(k.shape, dtype=dt, device=dev)
     dwq = torch.empty_like(q_norm) if q_norm is not None and need_norms[0] else None
     dwk = torch.empty_like(k_norm) if k_norm is not None and need_norms[1] else None
-    with _on(p.dev):
+    with _on(dev):
         ws, n = None, 0
         if dwq is not None or dwk is not None:
-            n = _rope_workspace_bytes(p.T, p.H, p.KV, p.d, p.rot, p.dev)
-            ws = torch.empty(n, dtype=torch.uint8, device=p.dev)
-        check(lib.q38moe_qk_norm_rope_backward(d_q_out.data_ptr(), d_k_out.data_ptr(), *p.head, dq.data_ptr(), dk.data_ptr(),
+            n = _rope_workspace_bytes(*sizes, dev)
+            ws = torch.empty(n, dtype=torch.uint8, device=dev)
+        check(lib.q38moe_qk_norm_rope_backward(pdq, pdk, *head, dq.data_ptr(), dk.data_ptr(),
                                                None if dwq is None else dwq.data_ptr(),
-                                               None if dwk is None else dwk.data_ptr(), *p.tail,
-                                               None if ws is None else ws.data_ptr(), n, _DTYPES[p.dt],
-                                               _raw_stream(p.dev.index)), "q38moe_qk_norm_rope_backward")
+                                               None if dwk is None else dwk.data_ptr(), *sizes, eps,
+                                               None if ws is None else ws.data_ptr(), n, _DTYPES[dt],
+                                               _raw_stream(dev.index)), "q38moe_qk_norm_rope_backward")
     return dq, dk, dwq, dwk
 
 
-class _LinearAttention:
-    """The checked operands of a linear attention call."""
-
-    __slots__ = ("q", "k", "v", "g", "cu", "shape", "dt", "dev", "scale", "strides", "S0", "packed")
-
-    def __init__(self, q, k, v, log_decay, scale, initial_state, cu_seqlens):
-        dt = self.dt = _fdt(q, "q")
-        dev = self.dev = _on_gpu(q, "q")
-        _heads(q, "q", dt, dev, 4)
-        _heads(k, "k", dt, dev, 4)
-        _heads(v, "v", dt, dev, 4)
-        B, S, H, dk = q.shape
-        Hk, dv = v.shape[2:]
-        if k.shape != (B, S, Hk, dk) or v.shape[:2] != (B, S) or Hk < 1 or H % Hk:
-            raise ValueError(f"q [B,S,H,dk], k [B,S,Hk,dk], v [B,S,Hk,dv] do not match: {tuple(q.shape)}, {tuple(k.shape)}, "
-                             f"{tuple(v.shape)}")
-        _head_dim(dk, "dk", 128)
-        _head_dim(dv, "dv", 128)
-        self.packed = cu_seqlens is not None
-        N = B
-        if self.packed:
-            _heads(_need(cu_seqlens, "cu_seqlens", dtype=torch.int32, ndim=1), "cu_seqlens", torch.int32, dev)
-            N = cu_seqlens.shape[0] - 1
-            if B != 1 or N < 1:
-                raise ValueError(f"packed sequences are one row of tokens and at least two offsets, got {B} rows and "
-                                 f"{cu_seqlens.shape[0]} offsets")
-        self.g, self.cu = _decay(log_decay, H, dev), cu_seqlens
-        self.scale = dk ** -0.5 if scale is None else float(scale)
-        self.shape = (N, S, H, Hk, dk, dv)
-        self.S0 = _state(initial_state, "initial_state", (N, H, dk, dv), dev)
-        q, k, v = self.q, self.k, self.v = _rows16(q, 3), _rows16(k, 3), _rows16(v, 3)
-        self.strides = (ctypes.c_int64 * 9)(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3])
-
-    def call(self):
-        return (self.q.data_ptr(), self.k.data_ptr(), self.v.data_ptr(), self.strides, self.g.data_ptr(), self.scale,
-                None if self.S0 is None else self.S0.data_ptr(), self.cu.data_ptr() if self.packed else None)
-
-    def bytes(self, backward):
-        """(workspace, saved states)"""
-        return _linear_attention_bytes(*self.shape, self.packed, backward, self.dt, self.dev)
+def _mix_strides(named, size, dims):
+    """The first ``dims`` strides of every (shape, stride), or None where a tensor has to be copied."""
+    found = []
+    for shape, stride in named:
+        kept = [0 if n <= 1 else s for n, s in zip(shape[:dims], stride)]
+        if 0 not in shape and (stride[-1] != 1 or any(s * size % 16 for s in kept)):
+            return None
+        found += kept
+    return (ctypes.c_int64 * len(found))(*found)
 
 
-def _decay(log_decay, H, dev):
-    _same(log_decay, "log_decay", torch.float32, (H,))
-    return _heads(log_decay, "log_decay", torch.float32, dev)
+@functools.lru_cache(maxsize=1024)
+def _mix_plan(dt, k_dt, v_dt, qs, ks, vs, q_stride, k_stride, v_stride, g, g_dt, S0, S0_dt, cu, cu_dt, device):
+    """((N, S, H, Hk, dk, dv), strides or None, (workspace, saved states) forwards, the same backwards)."""
+    size = _float_type(dt, "q")
+    if k_dt != dt or v_dt != dt:
+        raise TypeError(f"k and v must be {dt}, got {k_dt} and {v_dt}")
+    if not len(qs) == len(ks) == len(vs) == 4:
+        raise ValueError(f"q, k and v must have 4 dims, got {tuple(qs)}, {tuple(ks)}, {tuple(vs)}")
+    B, S, H, dk = qs
+    Hk, dv = vs[2:]
+    if ks != (B, S, Hk, dk) or vs[:2] != (B, S) or Hk < 1 or H < 1 or H % Hk:
+        raise ValueError(f"q [B,S,H,dk], k [B,S,Hk,dk], v [B,S,Hk,dv] do not match: {tuple(qs)}, {tuple(ks)}, {tuple(vs)}")
+    _head_dim(dk, "dk", 128)
+    _head_dim(dv, "dv", 128)
+    _decay_like(g, g_dt, H)
+    N = B
+    if cu is not None:
+        if cu_dt != torch.int32 or len(cu) != 1:
+            raise TypeError(f"cu_seqlens must be int32 [N+1], got {cu_dt} {tuple(cu)}")
+        N = cu[0] - 1
+        if B != 1 or N < 1:
+            raise ValueError(f"packed sequences are one row of tokens and at least two offsets, got {B} rows and {cu[0]} offsets")
+    if S0 is not None:
+        _state_like("initial_state", S0, S0_dt, (N, H, dk, dv))
+    shape = (N, S, H, Hk, dk, dv)
+    both = []
+    for backward in (False, True):
+        n, saved = ctypes.c_size_t(), ctypes.c_size_t()
+        check(lib.q38moe_linear_attention_workspace_bytes(*shape, cu is not None, backward, _DTYPES[dt], ctypes.byref(n),
+                                                          ctypes.byref(saved)), "q38moe_linear_attention_workspace_bytes")
+        both.append((n.value, saved.value))
+    return shape, _mix_strides(((qs, q_stride), (ks, k_stride), (vs, v_stride)), size, 3), *both
 
 
-def _state(t, name, shape, dev):
-    return None if t is None else _heads(_same(t, name, torch.float32, shape), name, torch.float32, dev)
+def _decay_like(g, g_dt, H):
+    if g_dt != torch.float32 or g != (H,):
+        raise ValueError(f"log_decay must be fp32 [{H}], got {g_dt} {tuple(g)}")
 
 
-@functools.lru_cache(maxsize=512)
-def _linear_attention_bytes(N, S, H, Hk, dk, dv, packed, backward, dt, device):
-    n, saved = ctypes.c_size_t(), ctypes.c_size_t()
-    check(lib.q38moe_linear_attention_workspace_bytes(N, S, H, Hk, dk, dv, packed, backward, _DTYPES[dt], ctypes.byref(n),
-                                                      ctypes.byref(saved)), "q38moe_linear_attention_workspace_bytes")
-    return n.value, saved.value
+def _state_like(name, shape, dt, want):
+    if dt != torch.float32 or shape != want:
+        raise ValueError(f"{name} must be fp32 {want}, got {dt} {tuple(shape)}")
+
+
+def _mix_operands(q, k, v, log_decay, scale, initial_state, cu_seqlens):
+    """(shape, workspaces, the C calls' arguments for the operands, what has to live until they are made)."""
+    rest = (log_decay.shape, log_decay.dtype, None if initial_state is None else initial_state.shape,
+            None if initial_state is None else initial_state.dtype, None if cu_seqlens is None else cu_seqlens.shape,
+            None if cu_seqlens is None else cu_seqlens.dtype, q.device)
+    plan = _mix_plan(q.dtype, k.dtype, v.dtype, q.shape, k.shape, v.shape, q.stride(), k.stride(), v.stride(), *rest)
+    pq, pk, pv = q.data_ptr(), k.data_ptr(), v.data_ptr()
+    if plan[1] is None or (pq | pk | pv) & 15:
+        q, k, v = _dense(q), _dense(k), _dense(v)
+        plan = _mix_plan(q.dtype, k.dtype, v.dtype, q.shape, k.shape, v.shape, q.stride(), k.stride(), v.stride(), *rest)
+        pq, pk, pv = q.data_ptr(), k.data_ptr(), v.data_ptr()
+    shape, strides, forwards, backwards = plan
+    return shape, forwards, backwards, (pq, pk, pv, strides, log_decay.data_ptr(),
+                                        shape[4] ** -0.5 if scale is None else scale,
+                                        None if initial_state is None else initial_state.data_ptr(),
+                                        None if cu_seqlens is None else cu_seqlens.data_ptr()), (q, k, v)
+
+
+def _mix_check(q, k, v, log_decay, initial_state, cu_seqlens):
+    _tensors(q=q, k=k, v=v, log_decay=log_decay)
+    _float_type(q.dtype, "q")
+    dev = _one_gpu(q, k, v, log_decay, initial_state, cu_seqlens)
+    for t in (log_decay, initial_state, cu_seqlens):
+        if t is not None and not t.is_contiguous():
+            raise ValueError("log_decay, initial_state and cu_seqlens must be contiguous")
+    return dev
 
 
 def linear_attention(q, k, v, log_decay, scale=None, initial_state=None, cu_seqlens=None, return_state=False, save=False):
     """Linear attention with a decay for each head (q38moe_linear_attention_forward): see ``autograd.linear_attention``.
     Returns (out [B,S,H,dv], final state [N,H,dk,dv] fp32 or None), and with save what ``linear_attention_backward`` of the
     same operands takes as ``saved``."""
-    a = _LinearAttention(q, k, v, log_decay, scale, initial_state, cu_seqlens)
-    N, S, H, _, dk, dv = a.shape
-    out = torch.empty(q.shape[0], S, H, dv, dtype=a.dt, device=a.dev)
-    state = torch.empty(N, H, dk, dv, dtype=torch.float32, device=a.dev) if return_state else None
-    with _on(a.dev):
-        n, states = a.bytes(False)
-        ws = torch.empty(n, dtype=torch.uint8, device=a.dev)
-        saved = torch.empty(states, dtype=torch.uint8, device=a.dev) if save and states else None
-        check(lib.q38moe_linear_attention_forward(*a.call(), out.data_ptr(), None if state is None else state.data_ptr(),
-                                                  None if saved is None else saved.data_ptr(), states, *a.shape,
-                                                  ws.data_ptr(), n, _DTYPES[a.dt], _raw_stream(a.dev.index)),
-              "q38moe_linear_attention_forward")
+    dev = _mix_check(q, k, v, log_decay, initial_state, cu_seqlens)
+    B = q.shape[0]
+    shape, (n, states), _, args, _alive = _mix_operands(q, k, v, log_decay, scale, initial_state, cu_seqlens)
+    N, S, H, _, dk, dv = shape
+    dt = q.dtype
+    out = torch.empty((B, S, H, dv), dtype=dt, device=dev)
+    state = torch.empty((N, H, dk, dv), dtype=torch.float32, device=dev) if return_state else None
+    saved = torch.empty(states, dtype=torch.uint8, device=dev) if save and states else None
+    with _on(dev):
+        ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
+        check(lib.q38moe_linear_attention_forward(*args, out.data_ptr(), None if state is None else state.data_ptr(),
+                                                  None if saved is None else saved.data_ptr(), states, *shape,
+                                                  None if ws is None else ws.data_ptr(), n, _DTYPES[dt],
+                                                  _raw_stream(dev.index)), "q38moe_linear_attention_forward")
     return (out, state, saved) if save else (out, state)
 
 
@@ -1384,26 +1470,67 @@ def linear_attention_backward(d_out, d_final_state, q, k, v, log_decay, scale=No
                               need_state=False, saved=None):
     """Gradients (dq, dk, dv, d initial_state or None) of ``linear_attention`` for those of its output and its final state
     (None: zero). saved: what the forward pass kept (None: it is made again)."""
-    a = _LinearAttention(q, k, v, log_decay, scale, initial_state, cu_seqlens)
-    N, S, H, Hk, dk, dv = a.shape
-    B = q.shape[0]
-    _heads(_same(d_out, "d_out", a.dt, (B, S, H, dv)), "d_out", a.dt, a.dev)
-    d_out = d_out if d_out.data_ptr() % 16 == 0 else d_out.clone()
-    _state(d_final_state, "d_final_state", (N, H, dk, dv), a.dev)
-    n, states = a.bytes(True)
+    dev = _mix_check(q, k, v, log_decay, initial_state, cu_seqlens)
+    _tensors(d_out=d_out)
+    _one_gpu(q, d_out, d_final_state, saved)
+    (N, S, H, _, dk, dv), _, (_, states), _, _ = _mix_operands(q, k, v, log_decay, scale, initial_state, cu_seqlens)
+    _same(d_out, "d_out", q.dtype, (q.shape[0], S, H, dv))
+    if d_final_state is not None:
+        _state_like("d_final_state", d_final_state.shape, d_final_state.dtype, (N, H, dk, dv))
+        _need(d_final_state, "d_final_state", dtype=None)
     if saved is not None:
-        _heads(_same(saved, "saved", torch.uint8, (states,)), "saved", torch.uint8, a.dev)
-    dq, dk_, dv_ = (torch.empty(B, S, h, d, dtype=a.dt, device=a.dev) for h, d in ((H, dk), (Hk, dk), (Hk, dv)))
-    ds = torch.empty(N, H, dk, dv, dtype=torch.float32, device=a.dev) if need_state else None
-    with _on(a.dev):
-        ws = torch.empty(n, dtype=torch.uint8, device=a.dev)
+        _same(saved, "saved", torch.uint8, (states,))
+    return _linear_attention_backward(d_out, d_final_state, q, k, v, log_decay, scale, initial_state, cu_seqlens, need_state, saved,
+                                      dev)
+
+
+def _linear_attention_backward(d_out, d_final_state, q, k, v, log_decay, scale, initial_state, cu_seqlens, need_state, saved, dev):
+    """linear_attention_backward of operands that have been looked at."""
+    B = q.shape[0]
+    shape, _, (n, states), args, _alive = _mix_operands(q, k, v, log_decay, scale, initial_state, cu_seqlens)
+    N, S, H, Hk, dk, dv = shape
+    dt = q.dtype
+    if d_out.data_ptr() & 15:
+        d_out = d_out.clone()
+    dq = torch.empty((B, S, H, dk), dtype=dt, device=dev)
+    dk_ = torch.empty((B, S, Hk, dk), dtype=dt, device=dev)
+    dv_ = torch.empty((B, S, Hk, dv), dtype=dt, device=dev)
+    ds = torch.empty((N, H, dk, dv), dtype=torch.float32, device=dev) if need_state else None
+    with _on(dev):
+        ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
         check(lib.q38moe_linear_attention_backward(d_out.data_ptr(),
-                                                   None if d_final_state is None else d_final_state.data_ptr(), *a.call(),
+                                                   None if d_final_state is None else d_final_state.data_ptr(), *args,
                                                    None if saved is None else saved.data_ptr(), states, dq.data_ptr(),
-                                                   dk_.data_ptr(), dv_.data_ptr(), None if ds is None else ds.data_ptr(),
-                                                   *a.shape, ws.data_ptr(), n, _DTYPES[a.dt], _raw_stream(a.dev.index)),
-              "q38moe_linear_attention_backward")
+                                                   dk_.data_ptr(), dv_.data_ptr(), None if ds is None else ds.data_ptr(), *shape,
+                                                   None if ws is None else ws.data_ptr(), n, _DTYPES[dt],
+                                                   _raw_stream(dev.index)), "q38moe_linear_attention_backward")
     return dq, dk_, dv_, ds
+
+
+@functools.lru_cache(maxsize=1024)
+def _step_plan(dt, k_dt, v_dt, qs, ks, vs, q_stride, k_stride, v_stride, state, state_dt, g, g_dt, slots, slots_dt):
+    """((B, pool, H, Hk, dk, dv), strides or None)."""
+    size = _float_type(dt, "q")
+    if k_dt != dt or v_dt != dt:
+        raise TypeError(f"k and v must be {dt}, got {k_dt} and {v_dt}")
+    if not len(qs) == len(ks) == len(vs) == 3:
+        raise ValueError(f"q, k and v must have 3 dims, got {tuple(qs)}, {tuple(ks)}, {tuple(vs)}")
+    B, H, dk = qs
+    Hk, dv = vs[1:]
+    if ks != (B, Hk, dk) or vs[0] != B or Hk < 1 or H < 1 or H % Hk:
+        raise ValueError(f"q [B,H,dk], k [B,Hk,dk], v [B,Hk,dv] do not match: {tuple(qs)}, {tuple(ks)}, {tuple(vs)}")
+    _head_dim(dk, "dk", 128)
+    _head_dim(dv, "dv", 128)
+    if len(state) != 4:
+        raise ValueError(f"state must be [pool,{H},{dk},{dv}], got {tuple(state)}")
+    _state_like("state", state, state_dt, (state[0], H, dk, dv))
+    _decay_like(g, g_dt, H)
+    if slots is not None:
+        if slots_dt != torch.int32 or slots != (B,):
+            raise ValueError(f"slots must be int32 [{B}], got {slots_dt} {tuple(slots)}")
+    elif state[0] < B:
+        raise ValueError(f"without slots state must hold {B} sequences, got {state[0]}")
+    return (B, state[0], H, Hk, dk, dv), _mix_strides(((qs, q_stride), (ks, k_stride), (vs, v_stride)), size, 2)
 
 
 def linear_attention_step(q, k, v, state, log_decay, scale=None, slots=None):
@@ -1411,35 +1538,24 @@ def linear_attention_step(q, k, v, state, log_decay, scale=None, slots=None):
     [B,Hk,dv] (bf16 or fp32), the states [pool,H,dk,dv] (fp32, contiguous) updated in place. Sequence b has the state
     slots[b] (int32 [B]; without slots the state b); a slot outside the pool is none: nothing is updated and the output is zero.
     No slot may occur twice. scale: dk^-1/2 unless given. Returns out [B,H,dv]; no gradients."""
-    dt = _fdt(q, "q")
-    dev = _on_gpu(q, "q")
-    _heads(q, "q", dt, dev, 3)
-    _heads(k, "k", dt, dev, 3)
-    _heads(v, "v", dt, dev, 3)
-    B, H, dk = q.shape
-    Hk, dv = v.shape[1:]
-    if k.shape != (B, Hk, dk) or v.shape[0] != B or Hk < 1 or H % Hk:
-        raise ValueError(f"q [B,H,dk], k [B,Hk,dk], v [B,Hk,dv] do not match: {tuple(q.shape)}, {tuple(k.shape)}, "
-                         f"{tuple(v.shape)}")
-    _head_dim(dk, "dk", 128)
-    _head_dim(dv, "dv", 128)
-    _heads(_need(state, "state", dtype=torch.float32, ndim=4), "state", torch.float32, dev)
-    pool = state.shape[0]
-    if state.shape[1:] != (H, dk, dv):
-        raise ValueError(f"state must be [pool,{H},{dk},{dv}], got {tuple(state.shape)}")
-    if slots is not None:
-        _heads(_same(slots, "slots", torch.int32, (B,)), "slots", torch.int32, dev)
-    elif pool < B:
-        raise ValueError(f"without slots state must hold {B} sequences, got {pool}")
-    g = _decay(log_decay, H, dev)
-    q, k, v = _rows16(q, 2), _rows16(k, 2), _rows16(v, 2)
-    out = torch.empty(B, H, dv, dtype=dt, device=dev)
-    strides = (ctypes.c_int64 * 6)(*q.stride()[:2], *k.stride()[:2], *v.stride()[:2])
+    _tensors(q=q, k=k, v=v, state=state, log_decay=log_decay)
+    _float_type(q.dtype, "q")
+    dev = _one_gpu(q, k, v, state, log_decay, slots)
+    if not (state.is_contiguous() and log_decay.is_contiguous() and (slots is None or slots.is_contiguous())):
+        raise ValueError("state, log_decay and slots must be contiguous")
+    rest = (state.shape, state.dtype, log_decay.shape, log_decay.dtype, None if slots is None else slots.shape,
+            None if slots is None else slots.dtype)
+    sizes, strides = _step_plan(q.dtype, k.dtype, v.dtype, q.shape, k.shape, v.shape, q.stride(), k.stride(), v.stride(), *rest)
+    if strides is None or (q.data_ptr() | k.data_ptr() | v.data_ptr()) & 15:
+        q, k, v = _dense(q), _dense(k), _dense(v)
+        _, strides = _step_plan(q.dtype, k.dtype, v.dtype, q.shape, k.shape, v.shape, q.stride(), k.stride(), v.stride(), *rest)
+    B, _, H, _, dk, dv = sizes
+    dt = q.dtype
+    out = torch.empty((B, H, dv), dtype=dt, device=dev)
     with _on(dev):
-        check(lib.q38moe_linear_attention_step(q.data_ptr(), k.data_ptr(), v.data_ptr(), strides, g.data_ptr(),
-                                               dk ** -0.5 if scale is None else float(scale), state.data_ptr(),
-                                               None if slots is None else slots.data_ptr(), out.data_ptr(), B, pool, H, Hk,
-                                               dk, dv, _DTYPES[dt], _raw_stream(dev.index)),
-              "q38moe_linear_attention_step")
+        check(lib.q38moe_linear_attention_step(q.data_ptr(), k.data_ptr(), v.data_ptr(), strides, log_decay.data_ptr(),
+                                               dk ** -0.5 if scale is None else scale, state.data_ptr(),
+                                               None if slots is None else slots.data_ptr(), out.data_ptr(), *sizes,
+                                               _DTYPES[dt], _raw_stream(dev.index)), "q38moe_linear_attention_step")
     torch.autograd.graph.increment_version(state)
     return out
