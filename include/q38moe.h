@@ -611,7 +611,7 @@ int q38moe_qk_norm_rope_backward(const void* d_q_out, const void* d_k_out, const
  * tokens of no sequence get zeros. strides (host): sequence, token and head strides of q, k, v in elements, multiples of 16
  * bytes (the sequences' unused with cu_seqlens). dk and dv multiples of 8 up to 128. Backward: from d_out (contiguous) and
  * d_final_state (NULL: zero) the gradients that are not NULL, contiguous; d_initial_state only with dv. A token's NaN or
- * infinity may reach the outputs of its chunk, up to 63 tokens before it. Workspace contents arbitrary. saved (NULL: not kept):
+ * infinity reaches no earlier token's output; an infinity may come out of a state as a NaN. Workspace contents arbitrary. saved (NULL: not kept):
  * saved_bytes of states that the forward pass leaves and the backward pass of the same call takes (NULL: it makes them again).
  * step: one token of B sequences, q [B,H,dk], k [B,Hk,dk], v [B,Hk,dv] (strides: sequence and head of each), states updated in
  * place: state [pool,H,dk,dv], sequence b in slots[b] (NULL: b). A slot outside [0, pool) is none: out is zero. No slot may occur

@@ -315,6 +315,85 @@ __device__ __forceinline__ void la_add(f32x4_t (&S)[NA], const uint8_t* keys, co
   }
 }
 
+// A score of a later key is zero, but zero times a NaN or an infinity among its values is a NaN. So values that are not finite are
+// looked for, once a chunk, and where there are any their terms are added one by one, of keys at or before the query alone, and
+// zeros take their place for the product (la_weigh_infinite).
+__device__ __forceinline__ bool la_any_infinite(const u32x4_t (&v)[2]) {
+  uint32_t any = 0;
+#pragma unroll
+  for (int u = 0; u < 2; ++u)
+#pragma unroll
+    for (int z = 0; z < 4; ++z) any |= (v[u][z] & 0x7f807f80u) + 0x00800080u;  // carries out of an exponent of ones
+  return ballot64((any & 0x80008000u) != 0) != 0;
+}
+__device__ __forceinline__ bool la_any_infinite(const f32x4_t (&v)[4]) {
+  uint32_t any = 0;
+#pragma unroll
+  for (int t = 0; t < 4; ++t)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) any |= (__float_as_uint(v[t][e]) & 0x7f800000u) + 0x00800000u;
+  return ballot64((any & 0x80000000u) != 0) != 0;
+}
+__device__ __forceinline__ bool la_infinite(float x) { return !(fabsf(x) <= 3.402823466e38f); }
+
+// o[t] += the terms of values that are not finite. value(n, c): token n's value of column c of the wave's 16, where the lane at
+// 16 ((n / 4) % 4) + c holds it; score(t, n): that of token n for query 16 t + lr.
+template <class Value, class Score>
+__device__ __forceinline__ void la_weigh_infinite(f32x4_t (&o)[4], int lr, int lq, Value value, Score score) {
+#pragma unroll 1
+  for (int n = 0; n < LA_C; ++n)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float x = value(n, 4 * lq + e);
+      if (!la_infinite(x)) continue;
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+        if (n <= 16 * t + lr) o[t][e] += score(t, n) * x;
+    }
+}
+__device__ __forceinline__ void la_weigh_infinite(f32x4_t (&o)[4], u32x4_t (&v)[2], const uint8_t* scores, int lr, int lq) {
+  la_weigh_infinite(
+      o, lr, lq,
+      [&](int n, int c) {
+        const int z = 2 * ((n >> 4) & 1) + ((n >> 1) & 1);
+        const u32x4_t x = n < 32 ? u32x4_t(v[0]) : u32x4_t(v[1]);
+        const uint32_t word = __shfl(z == 0 ? x[0] : z == 1 ? x[1] : z == 2 ? x[2] : x[3], 16 * ((n >> 2) & 3) + c);
+        return __uint_as_float(n & 1 ? word & 0xffff0000u : word << 16);
+      },
+      [&](int t, int n) {
+        const int unit = t == 3 ? n >> 5 : t == 2 ? 2 + 3 * (n >> 5) : 4 - t, lane = 16 * ((n >> 2) & 3) + lr;
+        const uint8_t* at = scores + (unit * 64 + lane) * 16 + 8 * ((n >> 4) & 1) + 2 * (n & 3);
+        return bf16_to_f32(*reinterpret_cast<const uint16_t*>(at));
+      });
+#pragma unroll
+  for (int u = 0; u < 2; ++u)
+#pragma unroll
+    for (int z = 0; z < 4; ++z) {
+      const uint32_t x = v[u][z];
+      v[u][z] = ((x & 0x7f80u) == 0x7f80u ? 0u : x & 0xffffu) | ((x & 0x7f800000u) == 0x7f800000u ? 0u : x & 0xffff0000u);
+    }
+}
+__device__ __forceinline__ void la_weigh_infinite(f32x4_t (&o)[4], f32x4_t (&v)[4], const uint8_t* scores, int lr, int lq) {
+  la_weigh_infinite(
+      o, lr, lq,
+      [&](int n, int c) {
+        uint32_t word = 0;  // by masks: an index that varies would put the values into memory
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) word |= n >> 4 == t && (n & 3) == e ? __float_as_uint(v[t][e]) : 0u;
+        return __uint_as_float(__shfl(word, 16 * ((n >> 2) & 3) + c));
+      },
+      [&](int t, int n) {
+        const int k = n >> 4, unit = t == 3 ? k >> 1 : t == 2 ? 2 + 3 * (k >> 1) : 4 - t, lane = 16 * ((n >> 2) & 3) + lr;
+        return *reinterpret_cast<const float*>(scores + ((2 * unit + (k & 1)) * 64 + lane) * 16 + 4 * (n & 3));
+      });
+#pragma unroll
+  for (int t = 0; t < 4; ++t)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[t][e] = la_infinite(v[t][e]) ? 0.0f : v[t][e];
+}
+
 // One segment of one head; DV / 16 waves. Wave w has columns 16 w .. of the state and of the outputs for all 64 queries of a
 // chunk (outputs as [column, query] tiles), and some of the scores' six [32 keys, 16 queries] units, which go through LDS. The
 // state stays in accumulators, which, rounded, are the operand that queries read (la_row). A column's tokens come out of the
@@ -503,6 +582,11 @@ __global__ __launch_bounds__(4 * DV, la_waves(BF16, DK, DV, OUT)) void la_kernel
     if (more) stage();
     if constexpr (OUT) {
       const int c = 16 * w + 4 * lq;
+      if constexpr (BF16) {
+        if (__builtin_expect(la_any_infinite(v), 0)) la_weigh_infinite(o, v, Ps, lr, lq);
+      } else {
+        if (__builtin_expect(la_any_infinite(vf), 0)) la_weigh_infinite(o, vf, Ps, lr, lq);
+      }
       const int64_t out = sb * a.ob + (first + (REV ? p.len - 1 - j0 - lr : j0 + lr)) * a.ot + (int64_t)h * a.oh + c;
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
@@ -688,12 +772,14 @@ __global__ __launch_bounds__(4 * (DK + DV), DK == DV ? 4 : 3) void la_back_kerne
       if (first_waves) publish(lr, lq);
     }
     const uint8_t* const P = Ps[first_waves ? 0 : 1];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) o[t] = o[t] * tab[16 * t + lr].x;
+    if (__builtin_expect(la_any_infinite(v), 0)) la_weigh_infinite(o, v, P, lr, lq);
     const int c = 16 * wc + 4 * lq, d = first_waves ? a.s.dv : a.s.dk;
     void* const to = first_waves ? a.dv_out : a.dk_out;
     const int64_t ot = (int64_t)a.s.H * d, out = sb * a.s.S * ot + (first + p.len - 1 - j0 - lr) * ot + (int64_t)h * d + c;
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
-      o[t] = o[t] * tab[16 * t + lr].x;
 #pragma unroll
       for (int u = 0; u <= t / 2; ++u)
         o[t] = mfma16x16x32(v[u], *reinterpret_cast<const u32x4_t*>(P + (la_unit(t, u) * 64 + lane) * 16), o[t]);

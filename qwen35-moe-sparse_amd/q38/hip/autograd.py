@@ -370,7 +370,7 @@ def linear_attention(q, k, v, log_decay, scale=None, initial_state=None, cu_seql
     cu_seqlens[n] to cu_seqlens[n+1]; tokens of no sequence come out zero, a sequence without tokens keeps its state. States are fp32
     throughout; bf16 operands of the matrix units are rounded once (scores, and the state as queries read it). Gradients flow
     to q, k, v and initial_state, not to log_decay. ``ops.linear_attention_step`` goes on one token at a time. A NaN or infinity
-    at a token may reach up to 63 tokens before it. Under bf16 autocast q, k and v are cast to bf16."""
+    reaches no earlier token's output; an infinity may come out of a state as a NaN. Under bf16 autocast q, k and v are cast to bf16."""
     if log_decay.requires_grad and torch.is_grad_enabled():
         raise ValueError("log_decay has no gradient here: pass log_decay.detach()")
     if _bf16_autocast():

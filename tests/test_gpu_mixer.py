@@ -567,3 +567,136 @@ def test_autocast(gpu):
     assert a.dtype == b.dtype == out.dtype == torch.bfloat16
     grads = torch.autograd.grad(out, leaves, do.bfloat16())
     assert all(t.dtype == torch.float32 and bool(t.isfinite().all()) for t in grads)
+
+
+# ---- values that are not finite, long offsets, other devices' streams -------------------------
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+@pytest.mark.parametrize("dk,dv", [(64, 64), (128, 128), (64, 128)])
+def test_nothing_reaches_back(gpu, dtype, bad, dk, dv):
+    """A NaN or infinity at a token changes no bit of what earlier tokens give, in its own chunk neither, and in the gradients of
+    no later one; a value's stays in its column."""
+    from q38.hip import autograd
+    S, H, Hk = 200, 4, 2
+    q, k, v, g, S0, do, _ = _mix_inputs(gpu, 1, S, H, Hk, dk, dv, dtype)
+
+    def run(q, k, v, do):
+        leaves = [t.clone().requires_grad_(True) for t in (q, k, v)]
+        out, last = autograd.linear_attention(*leaves, g, initial_state=S0, return_state=True)
+        return (out.detach(), last.detach(), *torch.autograd.grad(out, leaves, do))
+
+    clean = run(q, k, v, do)
+    for at in (0, 15, 16, 77, 100, 127, 128, 199):
+        for i, name in enumerate("qkv"):
+            ins = [t.clone() for t in (q, k, v)]
+            ins[i][0, at, -1, 3] = bad  # of the last head
+            got = run(*ins, do)
+            before = got[0][:, :at], clean[0][:, :at]
+            assert torch.equal(*before), (name, at)
+            assert torch.equal(got[0][:, :, :1], clean[0][:, :, :1]), (name, at)  # another head
+            if name == "q":
+                assert torch.equal(got[0][:, at + 1:], clean[0][:, at + 1:]) and torch.equal(got[1], clean[1])
+            if name == "v":
+                rest = [c for c in range(dv) if c != 3]
+                assert torch.equal(got[0][..., rest], clean[0][..., rest]) and torch.equal(got[1][..., rest], clean[1][..., rest])
+                assert not bool(got[0][0, at, -1, 3].isfinite())
+        d = do.clone()
+        d[0, at, -1, 5] = bad
+        got = run(q, k, v, d)
+        assert torch.equal(got[2][:, :at], clean[2][:, :at]), at               # dq: its own token and the ones behind none
+        assert torch.equal(got[2][:, at + 1:], clean[2][:, at + 1:]), at
+        for j in (3, 4):                                                       # dk, dv: tokens at or before it
+            assert torch.equal(got[j][:, at + 1:], clean[j][:, at + 1:]), (j, at)
+        assert not bool(got[4][0, at, -1].isfinite().all())
+
+
+def test_decays_at_the_ends(gpu):
+    """log_decay 0 forgets nothing, -inf all but the token itself, -200 nearly so (e^-200 is a float's zero)."""
+    from q38.hip import autograd, ops
+    q, k, v, _, S0, _, _ = _mix_inputs(gpu, 1, 150, 4, 4, 64, 64, torch.float32)
+    g = torch.tensor([0.0, float("-inf"), -200.0, -1e-7], device=gpu)
+    out, last = autograd.linear_attention(q, k, v, g, initial_state=S0, return_state=True)
+    own = (q * k).sum(-1, keepdim=True) * v / 8.0
+    for h in (1, 2):
+        torch.testing.assert_close(out[:, :, h], own[:, :, h], rtol=1e-5, atol=1e-5)
+        torch.testing.assert_close(last[0, h], k[0, -1, h][:, None] * v[0, -1, h][None], rtol=1e-6, atol=1e-6)
+    for h in (0, 3):
+        *want, state, size = _sum64(_heads(q[0])[h:h + 1], _heads(k[0])[h:h + 1], _heads(v[0])[h:h + 1], g[h:h + 1],
+                                    S0[0, h:h + 1], 0.125, 0.125, 1.0, 0)
+        _check(out[0, :, h:h + 1], want, torch.float32, 64, f"head {h}")
+        _check_state(last[0, h:h + 1], state, size, 64, 150, f"state {h}")
+    state = S0.clone()
+    o = ops.linear_attention_step(q[:, 0], k[:, 0], v[:, 0], state, g)
+    torch.testing.assert_close(o, out[:, 0], rtol=1e-5, atol=1e-5)
+
+
+def test_slow_decay_over_a_long_sequence(gpu):
+    """A decay of 1e-5 over 40000 tokens: the state remembers all of them, and is as near to float64 as sums of that many terms
+    in fp32 are (64-token sums, one rounded decay a chunk: errors of both signs, so 16 u (n)^1/2 of the terms' size and
+    not n u)."""
+    from q38.hip import ops
+    S = 40000
+    q, k, v, _, _, _, _ = _mix_inputs(gpu, 1, S, 2, 2, 64, 64, torch.bfloat16, state=False)
+    k, v = k.abs(), v.abs()  # no cancellation: a decay that is off in one direction would show
+    g = torch.tensor([-1e-5, -3e-6], device=gpu)
+    _, last = ops.linear_attention(q, k, v, g, return_state=True)
+    w = torch.exp(g.double()[:, None] * torch.arange(S - 1, -1, -1, device=gpu).double())
+    exact = torch.stack([(k[0, :, h].double() * w[h][:, None]).t().contiguous() @ v[0, :, h].double() for h in range(2)])
+    err = float(((last[0].double() - exact) / exact).abs().max())
+    assert err <= 16 * U * math.sqrt(S / 64), err
+
+
+def test_offsets_past_32_bits(gpu):
+    """Tokens 2^25 elements apart (5 GB from the first to the last), and outputs of more than 2^31 elements."""
+    from q38.hip import ops
+    far = torch.empty(70 << 25, dtype=torch.bfloat16, device=gpu)
+    q, k, v, g, S0, _, _ = _mix_inputs(gpu, 1, 70, 2, 1, 64, 64, torch.bfloat16)
+    parts = []
+    for i, t in enumerate((q, k, v)):
+        x = far.as_strided(t.shape, (0, 1 << 25, 64, 1), 256 * i)
+        x.copy_(t)
+        parts.append(x)
+    for a, b in zip(ops.linear_attention(*parts, g, initial_state=S0, return_state=True),
+                    ops.linear_attention(q, k, v, g, initial_state=S0, return_state=True)):
+        assert torch.equal(a, b)
+    w, inv, pos = torch.zeros(64, dtype=torch.bfloat16, device=gpu), torch.ones(8, device=gpu), torch.arange(70, device=gpu)
+    for a, b in zip(ops.qk_norm_rope(parts[0][0], parts[1][0], w, w, pos, inv), ops.qk_norm_rope(q[0], k[0], w, w, pos, inv)):
+        assert torch.equal(a, b)
+    del far, parts
+    T, H = (1 << 20) + 70, 32
+    r = torch.Generator(device=gpu).manual_seed(1)
+    q = torch.empty(T, H, 64, dtype=torch.bfloat16, device=gpu)
+    q[-70:] = _randn(r, 70, H, 64, dtype=torch.bfloat16)
+    q[:-70] = 0
+    k = _randn(r, T, 1, 64, dtype=torch.bfloat16)
+    pos = torch.arange(T, device=gpu)
+    qo, ko = ops.qk_norm_rope(q, k, w, w, pos, inv)
+    a, b = ops.qk_norm_rope(q[-70:], k[-70:], w, w, pos[-70:].contiguous(), inv)
+    assert torch.equal(qo[-70:], a) and torch.equal(ko[-70:], b)
+    del qo
+    g = torch.full((H,), -0.5, device=gpu)
+    out, last = ops.linear_attention(q[None], k[None], k[None], g, return_state=True)
+    # e^-35 of what is before the last 70 tokens is left at their end, e^-0.5 .. at their start: from the state of the 500 before.
+    _, S0 = ops.linear_attention(q[None, -570:-70], k[None, -570:-70], k[None, -570:-70], g, return_state=True)
+    x = _heads(k[-70:], H)
+    *want, state, size = _sum64(_heads(q[-70:]), x, x, g, S0[0], 0.125, 0.125, 1.0, 0)
+    # The call's chunks lie otherwise than the reference's: a score rounded there is a state rounded here, of the same size.
+    outs, rounded, terms = want
+    bound = 2 * (64 + 64 + 20) * U * terms + 2.0 ** -8 * (terms + outs.abs()) * 1.01
+    _within(out[0, -70:], outs.transpose(0, 1), bound.transpose(0, 1), "out")
+    _check_state(last[0], state, size, 64, 570, "state")
+
+
+def test_current_device_is_not_needed(gpu):
+    """Tensors that another stream made are used in that order on the current one; a call inside torch.inference_mode."""
+    from q38.hip import autograd, ops
+    q, k, v, g, S0, _, _ = _mix_inputs(gpu, 1, 90, 2, 2, 64, 64, torch.bfloat16)
+    want = ops.linear_attention(q, k, v, g, initial_state=S0)[0]
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s), torch.inference_mode():
+        q2, k2, v2 = q * 1, k * 1, v * 1
+        got = autograd.linear_attention(q2, k2, v2, g, initial_state=S0)[0]
+    torch.cuda.current_stream().wait_stream(s)
+    assert torch.equal(got, want)
