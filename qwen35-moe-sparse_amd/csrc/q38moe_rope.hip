@@ -223,22 +223,23 @@ __global__ __launch_bounds__(ROPE_THREADS) void rope_backward_kernel(RopeArgs p,
   }
 }
 
-// dw[which][c] = sum over blocks of partial[block][which][c], in fp64: 16 columns a block, 16 threads each.
+// dw[which][c] = sum over blocks of partial[block][which][c], in fp64: 16 columns a block, 64 threads each (16 threads: 4.8 us
+// where these take 3, of 1024 blocks' sums).
 template <bool BF16>
-__global__ __launch_bounds__(256) void rope_dw_kernel(const float* __restrict__ partial, int blocks, int d, void* dwq, void* dwk) {
-  __shared__ double s[16][17];
+__global__ __launch_bounds__(1024) void rope_dw_kernel(const float* __restrict__ partial, int blocks, int d, void* dwq, void* dwk) {
+  __shared__ double s[64][17];
   const int which = blockIdx.y, c = blockIdx.x * 16 + threadIdx.x % 16, g = threadIdx.x / 16;
   double v = 0.0;
   if (c < d) {
 #pragma unroll 8
-    for (int b = g; b < blocks; b += 16) v += (double)partial[((int64_t)b * 2 + which) * d + c];
+    for (int b = g; b < blocks; b += 64) v += (double)partial[((int64_t)b * 2 + which) * d + c];
   }
   s[g][threadIdx.x % 16] = v;
   __syncthreads();
   void* dst = which == 0 ? dwq : dwk;
   if (threadIdx.x < 16 && c < d && dst != nullptr) {
     double sum = 0.0;
-    for (int r = 0; r < 16; ++r) sum += s[r][threadIdx.x];
+    for (int r = 0; r < 64; ++r) sum += s[r][threadIdx.x];
     if (BF16) static_cast<uint16_t*>(dst)[c] = (uint16_t)f32_to_bf16_rne((float)sum);
     else static_cast<float*>(dst)[c] = (float)sum;
   }
@@ -297,8 +298,8 @@ hipError_t launch_rope_backward(RopeArgs p, const void* dyq, const void* dyk, fl
   }
   if (dwq == nullptr && dwk == nullptr) return hipSuccess;
   const dim3 grid((unsigned)((p.d + 15) / 16), 2);
-  if (bf16) hipLaunchKernelGGL(rope_dw_kernel<true>, grid, dim3(256), 0, st, partial, blocks, p.d, dwq, dwk);
-  else hipLaunchKernelGGL(rope_dw_kernel<false>, grid, dim3(256), 0, st, partial, blocks, p.d, dwq, dwk);
+  if (bf16) hipLaunchKernelGGL(rope_dw_kernel<true>, grid, dim3(1024), 0, st, partial, blocks, p.d, dwq, dwk);
+  else hipLaunchKernelGGL(rope_dw_kernel<false>, grid, dim3(1024), 0, st, partial, blocks, p.d, dwq, dwk);
   return hipGetLastError();
 }
 
