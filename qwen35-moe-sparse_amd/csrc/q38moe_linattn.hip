@@ -37,11 +37,16 @@ __device__ __forceinline__ f32x4_t mfma16x16x4(float a, float b, f32x4_t c) {
   return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
 }
 
-// Byte of 16-byte column `col` of row `row` in a tile of rows of `bytes` bytes. The low three bits of the column are mixed with
-// the row's, so that 8 rows' same column, and 4 rows' same pair of columns, lie in different banks.
-__device__ __forceinline__ int la_at(int row, int col, int bytes) {
-  return row * bytes + ((col ^ (((row & 3) << 1) | ((row >> 2) & 1))) << 4);
-}
+// A tile of rows of BYTES bytes: where row `row` has its 16-byte column `col`. The columns are mixed with the row so that the
+// lanes that a read serves at once (16 bytes: rows 0-3 and 12-15 of a column and 4-11 of the next; 8 bytes, transposing: two
+// columns of 8 rows, or four half ones; 4 bytes, fp32: one column of rows 4 apart) find their data in different banks. Half columns
+// of bf16 tiles are exchanged in every other row where `swapped` says so (la_row's reads).
+template <bool BF16, int BYTES>
+struct LaTile {
+  static __device__ __forceinline__ int key(int row) { return !BF16 ? row & 15 : BYTES == 128 ? row & 6 : 2 * (row & 7); }
+  static __device__ __forceinline__ int at(int row, int col) { return row * BYTES + ((col ^ key(row)) << 4); }
+  static __device__ __forceinline__ bool swapped(int row) { return (BYTES == 128 ? row >> 1 : row) & 1; }
+};
 
 // e^{g n} to 24 + 24 bits.
 __device__ __forceinline__ float2 la_decay2(double g, int64_t n) {
@@ -157,8 +162,9 @@ __device__ __forceinline__ void la_gap(const LaArgs& a, void* out, int row_bytes
 }
 
 // 64 rows of features on their way from memory to LDS, zero behind the last row and the last feature.
-template <int BYTES, int THREADS>  // of a row of the tile
+template <bool BF16, int BYTES, int THREADS>
 struct LaStage {
+  using Tile = LaTile<BF16, BYTES>;
   static constexpr int COLS = BYTES / 16, N = (LA_C * COLS + THREADS - 1) / THREADS, ROWS = THREADS / COLS;
   static constexpr bool EVEN = N * ROWS == LA_C;
   u32x4_t r[N];
@@ -181,12 +187,12 @@ struct LaStage {
   template <bool SWAP>
   __device__ __forceinline__ void store(int tid, uint8_t* lds) const {
     const int row = tid / COLS, col = tid % COLS;
-    static_assert(ROWS % 2 == 0, "the rows of a thread are all even or all odd");
-    const bool swap = SWAP && (row & 1);
+    static_assert(ROWS % 4 == 0, "the rows of a thread are all swapped or none");
+    const bool swap = SWAP && Tile::swapped(row);
 #pragma unroll
     for (int i = 0; i < N; ++i)
       if (EVEN || row + ROWS * i < LA_C)
-        *reinterpret_cast<u32x4_t*>(lds + la_at(row + ROWS * i, col, BYTES)) =
+        *reinterpret_cast<u32x4_t*>(lds + Tile::at(row + ROWS * i, col)) =
             swap ? u32x4_t{r[i][2], r[i][3], r[i][0], r[i][1]} : r[i];
   }
   // The next 64 rows straight into a tile, asynchronously. Places behind the last row or feature get others of the same kind,
@@ -195,7 +201,7 @@ struct LaStage {
     static_assert(EVEN, "every thread copies");
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int row = tid / COLS + ROWS * i, col = la_at(row, tid % COLS, 0) >> 4;
+      const int row = tid / COLS + ROWS * i, col = tid % COLS ^ Tile::key(row);
       load_lds16(at + (min(row, rows - 1) - tid / COLS) * step + 16 * (min(col, bytes / 16 - 1) - tid % COLS),
                  lds + 16 * (THREADS * i + (tid & ~63)));
     }
@@ -251,18 +257,18 @@ __device__ __forceinline__ int la_row(int i, int q) {
 // exchanged. row_at: see la_kernel.
 template <int BYTES, bool KEYS_SWAPPED>
 __device__ __forceinline__ u32x4_t la_scores(const uint8_t* keys, const uint8_t* queries, int unit, int lr, int lq,
-                                             const int* row_at, float intra, const float2* tab) {
+                                             int row_at, float intra, const float2* tab) {
   const int t = la_unit_queries(unit), u = la_unit_keys(unit);
   auto key = [&](const uint8_t* at) {
     const u32x4_t k = *reinterpret_cast<const u32x4_t*>(at);
-    return KEYS_SWAPPED && (lr & 1) ? u32x4_t{k[2], k[3], k[0], k[1]} : k;
+    return KEYS_SWAPPED && LaTile<true, BYTES>::swapped(lr) ? u32x4_t{k[2], k[3], k[0], k[1]} : k;
   };
   f32x4_t P[2];
   P[0] = P[1] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
   for (int s = 0; s < BYTES / 64; ++s) {
-    const uint8_t* x = keys + row_at[s & 1] + 128 * (s >> 1) + 32 * BYTES * u;
-    const u32x4_t q = *reinterpret_cast<const u32x4_t*>(queries + row_at[s & 1] + 128 * (s >> 1) + 16 * BYTES * t);
+    const uint8_t* x = keys + (row_at ^ (64 * s)) + 32 * BYTES * u;
+    const u32x4_t q = *reinterpret_cast<const u32x4_t*>(queries + (row_at ^ (64 * s)) + 16 * BYTES * t);
     P[0] = mfma16x16x32(key(x), q, P[0]);
     if (2 * u + 1 <= t) P[1] = mfma16x16x32(key(x + 16 * BYTES), q, P[1]);
   }
@@ -280,7 +286,7 @@ __device__ __forceinline__ u32x4_t la_scores(const uint8_t* keys, const uint8_t*
 // odd rows' halves exchanged. The weighted values are split into three bf16 parts.
 template <int BYTES, int NA>
 __device__ __forceinline__ void la_add(f32x4_t (&S)[NA], const uint8_t* keys, const u32x4_t (&v)[2], float2 full, const float* add,
-                                       const int* column_at, int lq) {
+                                       int column_at, int lq) {
 #pragma unroll
   for (int i = 0; i < NA; ++i)
 #pragma unroll
@@ -308,7 +314,7 @@ __device__ __forceinline__ void la_add(f32x4_t (&S)[NA], const uint8_t* keys, co
     for (int i = 0; i < NA; ++i) {
       // The reads of few rows at a time: more of them in flight would push the loop's state out of the registers.
       if (i % 2 == 0) __builtin_amdgcn_sched_barrier(0);
-      const u32x4_t k = la_column<BYTES>(keys + (column_at[(i >> 1) & 1] ^ (8 * (i & 1))) + 128 * (i >> 2) + 32 * BYTES * u);
+      const u32x4_t k = la_column<BYTES>(keys + (column_at ^ (64 * (i >> 1) + 8 * (i & 1))) + 32 * BYTES * u);
 #pragma unroll
       for (int y = 0; y < 3; ++y) S[i] = mfma16x16x32(k, part[y], S[i]);
     }
@@ -427,8 +433,8 @@ __global__ __launch_bounds__(4 * DV, la_waves(BF16, DK, DV, OUT)) void la_kernel
   const int begin = p.s * a.L, end = min(p.len, begin + a.L);
   const bool last = p.s == p.nseg - 1, keep = !OUT || (last && a.s1 != nullptr);
 
-  LaStage<KB, THREADS> kst, qst;
-  LaStage<VB, THREADS> vst;
+  LaStage<BF16, KB, THREADS> kst, qst;
+  LaStage<BF16, VB, THREADS> vst;
   start(kst, a.k, begin);
   start(vst, a.v, begin);
   if (OUT) start(qst, a.q, begin);
@@ -484,13 +490,13 @@ __global__ __launch_bounds__(4 * DV, la_waves(BF16, DK, DV, OUT)) void la_kernel
     if (more) fetch(min(LA_C, end - j0 - LA_C), Qs[par ^ 1]);
     const uint8_t* const Q = Qs[par];
     const int lane = afresh(tid & 63), lr = lane & 15, lq = lane >> 4;
-    // Row 16 t + lr, column 4 s + lq of a tile of KB bytes a row: row_at[s & 1] + 128 (s >> 1) + 16 KB t.
-    const int row_at[2] = {la_at(lr, lq, KB), la_at(lr, 4 + lq, KB)};
-    // bf16: rows 4 lq + lr / 4, features row_of(i, lr / 4, 0) for lr % 4: column_at[i / 2 % 2] ^ 8 (i % 2), + 128 (i / 4).
-    int column_at[2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) column_at[i] = la_at(4 * lq + (lr >> 2), 4 * i + (lr & 3), KB) + 8 * ((lr >> 2) & 1);
-    const int value_at = la_at(4 * lq + (lr >> 2), 2 * w + ((lr & 3) >> 1), VB) + 8 * (lr & 1);
+    using KeyTile = LaTile<BF16, KB>;
+    using ValueTile = LaTile<BF16, VB>;
+    // Row 16 t + lr, column 4 s + lq: row_at ^ 64 (s % 4), + 256 (s / 4), + 16 KB t.
+    const int row_at = KeyTile::at(lr, lq);
+    // bf16: rows 4 lq + lr / 4, features la_row(i, lr % 4) ..: column_at ^ (64 (i / 2) + 8 (i % 2)).
+    const int column_at = KeyTile::at(4 * lq + (lr >> 2), lr & 3) + 8 * KeyTile::swapped(lr >> 2);
+    const int value_at = ValueTile::at(4 * lq + (lr >> 2), 2 * w + ((lr & 3) >> 1)) + 8 * (lr & 1);
     f32x4_t o[4];  // [query tile]
     if constexpr (OUT) {
       // Scores of queries 16 t + lr with keys 32 u + {4 lq .., 16 + 4 lq ..}, weighted.
@@ -505,7 +511,7 @@ __global__ __launch_bounds__(4 * DV, la_waves(BF16, DK, DV, OUT)) void la_kernel
             f32x4_t P = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int s = 0; s < KB / 64; ++s) {
-              const int at = row_at[s & 1] + 128 * (s >> 1);
+              const int at = (row_at ^ (64 * (s & 3))) + 256 * (s >> 2);
               const f32x4_t x = *reinterpret_cast<const f32x4_t*>(Ks + at + 16 * KB * (2 * u + k));
               const f32x4_t y = *reinterpret_cast<const f32x4_t*>(Q + at + 16 * KB * t);
 #pragma unroll
@@ -529,7 +535,7 @@ __global__ __launch_bounds__(4 * DV, la_waves(BF16, DK, DV, OUT)) void la_kernel
         if constexpr (BF16) x = la_pack(S[2 * s], S[2 * s + 1]);
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
-          const u32x4_t y = *reinterpret_cast<const u32x4_t*>(Q + row_at[s & 1] + 128 * (s >> 1) + 16 * KB * t);
+          const u32x4_t y = *reinterpret_cast<const u32x4_t*>(Q + (row_at ^ (64 * (s & 3))) + 256 * (s >> 2) + 16 * KB * t);
           if constexpr (BF16) {
             o[t] = mfma16x16x32(x, y, o[t]);
           } else {
@@ -553,7 +559,7 @@ __global__ __launch_bounds__(4 * DV, la_waves(BF16, DK, DV, OUT)) void la_kernel
       for (int t = 0; t < 4; ++t)
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          vf[t][e] = *reinterpret_cast<const float*>(Vs + la_at(16 * t + 4 * lq + e, 4 * w + (lr >> 2), VB) + 4 * (lr & 3));
+          vf[t][e] = *reinterpret_cast<const float*>(Vs + ValueTile::at(16 * t + 4 * lq + e, 4 * w + (lr >> 2)) + 4 * (lr & 3));
     }
     if (more || keep) {
       const float2 full = tab[rows];
@@ -573,7 +579,7 @@ __global__ __launch_bounds__(4 * DV, la_waves(BF16, DK, DV, OUT)) void la_kernel
             const float x = vf[t][e] * add[n];
 #pragma unroll
             for (int i = 0; i < NA; ++i)
-              S[i] = mfma16x16x4(*reinterpret_cast<const float*>(Ks + la_at(n, 4 * i + (lr >> 2), KB) + 4 * (lr & 3)), x, S[i]);
+              S[i] = mfma16x16x4(*reinterpret_cast<const float*>(Ks + KeyTile::at(n, 4 * i + (lr >> 2)) + 4 * (lr & 3)), x, S[i]);
           }
       }
     }
@@ -661,8 +667,10 @@ __global__ __launch_bounds__(4 * (DK + DV), DK == DV ? 4 : 3) void la_back_kerne
     const uint8_t* base = static_cast<const uint8_t*>(t.p) + 2 * (sb * t.sb + first * t.st + (int64_t)(h / t.div) * t.sh);
     stage.start(base + (int64_t)(p.len - 1) * t.st * 2, -t.st * 2, begin);
   };
-  LaStage<KB, THREADS> qst, kst;
-  LaStage<VB, THREADS> vst, dst;
+  using KeyTile = LaTile<true, KB>;
+  using ValueTile = LaTile<true, VB>;
+  LaStage<true, KB, THREADS> qst, kst;
+  LaStage<true, VB, THREADS> vst, dst;
   start(qst, a.s.k);
   start(dst, a.s.v);
   start(kst, a.k);
@@ -706,10 +714,12 @@ __global__ __launch_bounds__(4 * (DK + DV), DK == DV ? 4 : 3) void la_back_kerne
   const double g = (double)a.s.g[h];
   if (tid <= LA_C) tab[tid] = la_decay2(g, tid);
   if (tid < 2 * LA_C) put[tid] = tid < LA_C ? a.s.gain * la_decay2(g, LA_C - tid).x : 0.0f;
-  auto publish = [&](int lr, int lq) {  // as [dv][dk]
+  // Ts is [dv][dk]; rows 8 apart, which its transposing reads take together, are mixed as those 4 apart of other tiles are.
+  auto state = [&](int row, int col) { return row * KB + ((col ^ KeyTile::key((row & 3) | ((row >> 1) & 4))) << 4); };
+  auto publish = [&](int lr, int lq) {
 #pragma unroll
     for (int u = 0; u < NA / 2; ++u)
-      *reinterpret_cast<u32x4_t*>(Ts + la_at(16 * wc + lr, 4 * u + lq, KB)) = la_pack(T[2 * u], T[2 * u + 1]);
+      *reinterpret_cast<u32x4_t*>(Ts + state(16 * wc + lr, 4 * u + lq)) = la_pack(T[2 * u], T[2 * u + 1]);
   };
   if (begin < end) {
     stage();
@@ -726,11 +736,9 @@ __global__ __launch_bounds__(4 * (DK + DV), DK == DV ? 4 : 3) void la_back_kerne
 #pragma unroll
     for (int t = 0; t < 4; ++t) o[t] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
     if (first_waves) {
-      const int row_at[2] = {la_at(lr, lq, KB), la_at(lr, 4 + lq, KB)};
-      int column_at[2];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) column_at[i] = la_at(4 * lq + (lr >> 2), 4 * i + (lr & 3), KB) + 8 * ((lr >> 2) & 1);
-      const int value_at = la_at(4 * lq + (lr >> 2), 2 * wc + ((lr & 3) >> 1), VB) + 8 * (lr & 1);
+      const int row_at = KeyTile::at(lr, lq);
+      const int column_at = KeyTile::at(4 * lq + (lr >> 2), lr & 3) + 8 * KeyTile::swapped(lr >> 2);
+      const int value_at = ValueTile::at(4 * lq + (lr >> 2), 2 * wc + ((lr & 3) >> 1)) + 8 * (lr & 1);
       for (int unit = wc; unit < LA_UNITS; unit += WV)
         *reinterpret_cast<u32x4_t*>(Ps[0] + (unit * 64 + lane) * 16) =
             la_scores<KB, true>(Qs, Ks, unit, lr, lq, row_at, a.s.intra, tab);
@@ -739,18 +747,19 @@ __global__ __launch_bounds__(4 * (DK + DV), DK == DV ? 4 : 3) void la_back_kerne
         const u32x4_t x = la_pack(T[2 * s], T[2 * s + 1]);
 #pragma unroll
         for (int t = 0; t < 4; ++t)
-          o[t] = mfma16x16x32(x, *reinterpret_cast<const u32x4_t*>(Ks + row_at[s & 1] + 128 * (s >> 1) + 16 * KB * t), o[t]);
+          o[t] = mfma16x16x32(x, *reinterpret_cast<const u32x4_t*>(Ks + (row_at ^ (64 * s)) + 16 * KB * t), o[t]);
       }
 #pragma unroll
       for (int u = 0; u < 2; ++u) v[u] = la_column<VB>(Ds + value_at + 32 * VB * u);
       if (more || keep) la_add<KB>(T, Qs, v, tab[rows], put + LA_C - rows, column_at, lq);
     } else {
-      const int row_at[2] = {la_at(lr, lq, VB), la_at(lr, 4 + lq, VB)};
-      const int value_at = la_at(4 * lq + (lr >> 2), 2 * wc + ((lr & 3) >> 1), KB) + 8 * ((lr ^ (lr >> 2)) & 1);
+      const int row_at = ValueTile::at(lr, lq);
+      const int value_at =
+          KeyTile::at(4 * lq + (lr >> 2), 2 * wc + ((lr & 3) >> 1)) + 8 * ((lr & 1) ^ KeyTile::swapped(lr >> 2));
       // Row 16 wc + lr of T, columns 32 s + 8 lq .. + 3 and the 4 behind them.
       int state_at[2];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) state_at[i] = la_at(8 * lq + 4 * i + (lr >> 2), 2 * wc + ((lr & 3) >> 1), KB) + 8 * (lr & 1);
+      for (int i = 0; i < 2; ++i) state_at[i] = state(8 * lq + 4 * i + (lr >> 2), 2 * wc + ((lr & 3) >> 1)) + 8 * (lr & 1);
       for (int unit = wc; unit < LA_UNITS; unit += WK)
         *reinterpret_cast<u32x4_t*>(Ps[1] + (unit * 64 + lane) * 16) =
             la_scores<VB, false>(Ds, Vs, unit, lr, lq, row_at, a.s.intra, tab);
@@ -760,7 +769,7 @@ __global__ __launch_bounds__(4 * (DK + DV), DK == DV ? 4 : 3) void la_back_kerne
 #pragma unroll
         for (int t = 0; t < 4; ++t)
           o[t] = mfma16x16x32(u32x4_t{x.x, x.y, y.x, y.y},
-                              *reinterpret_cast<const u32x4_t*>(Vs + row_at[s & 1] + 128 * (s >> 1) + 16 * VB * t), o[t]);
+                              *reinterpret_cast<const u32x4_t*>(Vs + (row_at ^ (64 * s)) + 16 * VB * t), o[t]);
       }
 #pragma unroll
       for (int u = 0; u < 2; ++u) v[u] = la_column<KB>(Qs + value_at + 32 * KB * u);
