@@ -321,6 +321,13 @@ __device__ __forceinline__ void la_add(f32x4_t (&S)[NA], const uint8_t* keys, co
   }
 }
 
+// The (segment, head) of workgroup b of n: neighbours run on one XCD (b runs on XCD b % 8), so that heads which share keys and values
+// find them in its L2 (39 heads on 13 of 64: 25.0 -> 23.2 us; heads of their own: no difference).
+__device__ __forceinline__ unsigned la_unit_of(unsigned b, unsigned n) {
+  const unsigned x = b % 8, i = b / 8;
+  return x * (n / 8) + min(x, n % 8) + i;
+}
+
 // A score of a later key is zero, but zero times a NaN or an infinity among its values is a NaN. So values that are not finite are
 // looked for, once a chunk, and where there are any their terms are added one by one, of keys at or before the query alone, and
 // zeros take their place for the product (la_weigh_infinite).
@@ -420,7 +427,8 @@ __global__ __launch_bounds__(4 * DV, la_waves(BF16, DK, DV, OUT)) void la_kernel
     la_gap(a, a.o, a.H * a.dv * (a.o_f32 ? 4 : ES), blockIdx.x - a.segs * a.H);
     return;
   }
-  const int seg = (int)(blockIdx.x / a.H), h = (int)(blockIdx.x % a.H);
+  const unsigned unit = la_unit_of(blockIdx.x, OUT ? (unsigned)a.segs * a.H : gridDim.x);
+  const int seg = (int)(unit / a.H), h = (int)(unit % a.H);
   const LaPlace p = la_place<OUT>(a, seg);
   if (!p.there) return;
   const int64_t first = a.plan == nullptr ? 0 : p.start;
@@ -656,7 +664,8 @@ __global__ __launch_bounds__(4 * (DK + DV), DK == DV ? 4 : 3) void la_back_kerne
     if (a.dv_out != nullptr) la_gap(a.s, a.dv_out, a.s.H * a.s.dv * es, block);
     return;
   }
-  const int seg = (int)(blockIdx.x / a.s.H), h = (int)(blockIdx.x % a.s.H);
+  const unsigned unit = la_unit_of(blockIdx.x, (unsigned)a.s.segs * a.s.H);
+  const int seg = (int)(unit / a.s.H), h = (int)(unit % a.s.H);
   const LaPlace p = la_place<true>(a.s, seg);
   if (!p.there) return;
   const int64_t first = a.s.plan == nullptr ? 0 : p.start;
