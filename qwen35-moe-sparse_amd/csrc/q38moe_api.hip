@@ -1900,11 +1900,12 @@ struct LinattnCut {
   int64_t segs;
   size_t states;
 };
-static int linattn_cut(LinattnCut& c, int64_t N, int64_t S, int32_t H, int32_t dk, int32_t dv, bool packed, int per_cu) {
-  c.L = q38::la_segment_tokens(N, S, packed, H, per_cu);
+static int linattn_cut(LinattnCut& c, int64_t N, int64_t S, int32_t H, int32_t dk, int32_t dv, bool packed, bool bf16,
+                       bool back) {
+  c.L = q38::la_segment_tokens(N, S, packed, H, bf16, dk, dv, back);
   c.nseg = packed ? 0 : (int)std::max<int64_t>(1, (S + c.L - 1) / c.L);
   c.segs = packed ? S / c.L + N : N * c.nseg;
-  if (c.segs * H + S / 64 >= (int64_t)1 << 31) return fail(Q38MOE_EINVAL, "too many sequences and heads for one launch");
+  if (c.segs * H + 8 * (int64_t)H + S / 64 >= (int64_t)1 << 31) return fail(Q38MOE_EINVAL, "too many sequences and heads for one launch");
   c.states = sizeof(float) * (size_t)(c.segs - N) * H * (size_t)q38::la_padded_state(dk, dv);
   return Q38MOE_OK;
 }
@@ -1921,9 +1922,9 @@ static int linattn_plan(LinattnPlan& p, int64_t N, int64_t S, int32_t H, int32_t
                         bool backward, bool own_states, int32_t dtype) {
   const bool bf16 = dtype == Q38MOE_BF16;
   p.tokens = packed ? S : N * S;
-  Q38_CHECK(linattn_cut(p.cut, N, S, H, dk, dv, packed, q38::la_per_cu(bf16, dk, dv, false)));
+  Q38_CHECK(linattn_cut(p.cut, N, S, H, dk, dv, packed, bf16, false));
   p.back = p.cut;
-  if (bf16 && !packed) Q38_CHECK(linattn_cut(p.back, N, S, H, dk, dv, packed, q38::la_per_cu(bf16, dk, dv, true)));
+  if (bf16 && !packed) Q38_CHECK(linattn_cut(p.back, N, S, H, dk, dv, packed, bf16, true));
   const bool grouped = backward && H != Hk;
   p.mid = packed ? align_up(sizeof(int32_t) * (size_t)(3 * N + 1)) : 0;
   p.grouped = p.mid + (own_states ? align_up(backward ? std::max(p.cut.states, p.back.states) : p.cut.states) : 0);
@@ -1964,7 +1965,7 @@ static int linattn_start(LinattnPlan& p, q38::LaArgs& a, const float* log_decay,
   a = {};
   a.g = log_decay;
   a.mid = reinterpret_cast<float*>(static_cast<char*>(workspace) + p.mid);
-  a.N = (int)N, a.S = (int)S, a.H = H, a.L = p.cut.L, a.nseg = p.cut.nseg, a.segs = (int)p.cut.segs;
+  a.N = (int)N, a.S = (int)S, a.H = H, a.group = H / Hk, a.L = p.cut.L, a.nseg = p.cut.nseg, a.segs = (int)p.cut.segs;
   (void)hipGetLastError();
   if (cu_seqlens != nullptr) {
     a.plan = static_cast<const int32_t*>(workspace);

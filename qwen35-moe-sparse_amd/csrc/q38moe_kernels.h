@@ -278,7 +278,8 @@ struct LaTensor {
 // sum_j e^{g (L - 1 - j + lag)} k_j v_j^T, tokens taken forwards or backwards. s0, s1 (may be NULL): the caller's states [N, H, dk, dv],
 // turned: [N, H, dv, dk]. mid: a state per segment of L tokens with another behind it; mid_turned: as a call with dk and dv
 // exchanged left it. plan (packed sequences) or NULL (N sequences of S tokens, nseg
-// segments each); segs: at most, of all sequences.
+// segments each); segs: at most, of all sequences. group: heads that
+// share keys and values.
 struct LaArgs {
   LaTensor q, k, v;
   void* o;
@@ -287,7 +288,7 @@ struct LaArgs {
   float *s1, *mid;
   const int32_t* plan;
   float intra, inter, gain;
-  int lag, N, S, H, dk, dv, L, nseg, segs;
+  int lag, N, S, H, group, dk, dv, L, nseg, segs;
   bool o_f32, turned, mid_turned;
 };
 // dk and dv together, bf16: s is the pass that makes dv's state (k = q, v = dO; its q and o unused), and its strides
@@ -307,8 +308,7 @@ struct LaStepArgs {
   int64_t B, pool;
   int H, dk, dv;
 };
-int la_segment_tokens(int64_t N, int64_t S, bool packed, int H, int per_cu);
-int la_per_cu(bool bf16, int dk, int dv, bool back);
+int la_segment_tokens(int64_t N, int64_t S, bool packed, int H, bool bf16, int dk, int dv, bool back);
 int64_t la_padded_state(int dk, int dv);  // elements of a state in mid
 hipError_t launch_la_plan(const int32_t* cu, int32_t* plan, int N, int S, int L, hipStream_t st);
 // Forwards; states: fills a.mid first (else it is as an earlier call over the same tokens left it).

@@ -81,11 +81,12 @@ __device__ __forceinline__ LaPlace la_place(const LaArgs& a, int seg) {
     lo += each * max(0, 63 - __builtin_clzll(at | 1));
     step = each;
   }
+  lo = __builtin_amdgcn_readfirstlane(lo);
   p.seq = lo;
-  p.s = seg - before(lo);
-  p.nseg = first[lo + 1] - first[lo];
-  p.start = a.plan[a.N + 1 + lo];
-  p.len = a.plan[2 * a.N + 1 + lo];
+  p.s = __builtin_amdgcn_readfirstlane(seg - before(lo));
+  p.nseg = __builtin_amdgcn_readfirstlane(first[lo + 1] - first[lo]);
+  p.start = __builtin_amdgcn_readfirstlane(a.plan[a.N + 1 + lo]);
+  p.len = __builtin_amdgcn_readfirstlane(a.plan[2 * a.N + 1 + lo]);
   return p;
 }
 // The place in a.mid of the state behind the sequence's first segment.
@@ -228,13 +229,6 @@ __device__ __forceinline__ int afresh(int x) {
   return x;
 }
 
-// Where a.mid has row `row`, column `col` of a state with NA tiles of rows.
-template <bool BF16, int NA>
-__device__ __forceinline__ int la_place_of(int row, int col) {
-  const int i = BF16 ? 2 * (row >> 5) + ((row >> 2) & 1) : row >> 4, q = BF16 ? (row >> 3) & 3 : (row >> 2) & 3;
-  return (((col >> 4) * NA + i) * 64 + 16 * q + (col & 15)) * 4 + (row & 3);
-}
-
 // Waves on a SIMD that the LDS of la_kernel's workgroups allows, at most 4: the limit of its registers.
 constexpr int la_waves(bool bf16, int dk, int dv, bool out) {
   return bf16 ? (out && dk == 128 && dv == 64 ? 2 : 4) : out && dk == 128 && dv == 64 ? 1 : 2;
@@ -321,16 +315,28 @@ __device__ __forceinline__ void la_add(f32x4_t (&S)[NA], const uint8_t* keys, co
   }
 }
 
-// The (segment, head) of workgroup b of n: neighbours run on one XCD (b runs on XCD b % 8), so that heads which share keys and values
-// find them in its L2 (39 heads on 13 of 64: 25.0 -> 23.2 us; heads of their own: no difference).
-__device__ __forceinline__ unsigned la_unit_of(unsigned b, unsigned n) {
-  const unsigned x = b % 8, i = b / 8;
-  return x * (n / 8) + min(x, n % 8) + i;
+// The segment and the head of workgroup b. Heads that share keys and values run on one XCD (b runs on XCD b % 8) and find them in
+// its L2 (39 heads on 13 of 64, 2 x 2049 tokens: 25.0 -> 23.2 us). Ordinary heads are spread over the XCDs, each head's segments
+// on few of them, so that its states are found there too.
+struct LaUnit {
+  int seg, h, shared;  // the head, and the one that it shares keys and values with others in
+};
+__device__ __forceinline__ LaUnit la_unit_of(const LaArgs& a, unsigned b) {
+  const unsigned G = a.group, Hk = G == 1 ? a.H : a.H / G, i = b / 8, j = G == 1 ? i : i / G, u = 8 * j + b % 8, seg = u / Hk;
+  const int shared = (int)(u - seg * Hk);
+  return {(int)seg, (int)(shared * G + (i - j * G)), shared};
+}
+__host__ __device__ __forceinline__ unsigned la_units(const LaArgs& a, unsigned segs) {
+  return (segs * (a.H / a.group) + 7) / 8 * 8 * a.group;
 }
 
 // A score of a later key is zero, but zero times a NaN or an infinity among its values is a NaN. So values that are not finite are
 // looked for, once a chunk, and where there are any their terms are added one by one, of keys at or before the query alone, and
-// zeros take their place for the product (la_weigh_infinite).
+// zeros take their place for the product (la_weigh_infinite). A wave that has just added them to its columns of the state need
+// look at one row of that alone: each is a sum over all of the column's values.
+__device__ __forceinline__ bool la_any_infinite(float x) {
+  return ballot64((__float_as_uint(x) & 0x7f800000u) == 0x7f800000u) != 0;
+}
 __device__ __forceinline__ bool la_any_infinite(const u32x4_t (&v)[2]) {
   uint32_t any = 0;
 #pragma unroll
@@ -364,7 +370,16 @@ __device__ __forceinline__ void la_weigh_infinite(f32x4_t (&o)[4], int lr, int l
         if (n <= 16 * t + lr) o[t][e] += score(t, n) * x;
     }
 }
-__device__ __forceinline__ void la_weigh_infinite(f32x4_t (&o)[4], u32x4_t (&v)[2], const uint8_t* scores, int lr, int lq) {
+// bf16: o[t] += scores times values.
+__device__ __forceinline__ void la_weigh(f32x4_t (&o)[4], const u32x4_t (&v)[2], const uint8_t* scores, int lane) {
+#pragma unroll
+  for (int t = 0; t < 4; ++t)
+#pragma unroll
+    for (int u = 0; u <= t / 2; ++u)
+      o[t] = mfma16x16x32(v[u], *reinterpret_cast<const u32x4_t*>(scores + (la_unit(t, u) * 64 + lane) * 16), o[t]);
+}
+__device__ __forceinline__ void la_weigh_infinite(f32x4_t (&o)[4], u32x4_t (&v)[2], const uint8_t* scores, int lane) {
+  const int lr = lane & 15, lq = lane >> 4;
   la_weigh_infinite(
       o, lr, lq,
       [&](int n, int c) {
@@ -386,7 +401,19 @@ __device__ __forceinline__ void la_weigh_infinite(f32x4_t (&o)[4], u32x4_t (&v)[
       v[u][z] = ((x & 0x7f80u) == 0x7f80u ? 0u : x & 0xffffu) | ((x & 0x7f800000u) == 0x7f800000u ? 0u : x & 0xffff0000u);
     }
 }
-__device__ __forceinline__ void la_weigh_infinite(f32x4_t (&o)[4], f32x4_t (&v)[4], const uint8_t* scores, int lr, int lq) {
+// The same in fp32.
+__device__ __forceinline__ void la_weigh(f32x4_t (&o)[4], const f32x4_t (&v)[4], const uint8_t* scores, int lane) {
+#pragma unroll
+  for (int t = 0; t < 4; ++t)
+#pragma unroll
+    for (int k = 0; k <= t; ++k) {
+      const f32x4_t s = *reinterpret_cast<const f32x4_t*>(scores + ((2 * la_unit(t, k / 2) + k % 2) * 64 + lane) * 16);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[t] = mfma16x16x4(v[k][e], s[e], o[t]);
+    }
+}
+__device__ __forceinline__ void la_weigh_infinite(f32x4_t (&o)[4], f32x4_t (&v)[4], const uint8_t* scores, int lane) {
+  const int lr = lane & 15, lq = lane >> 4;
   la_weigh_infinite(
       o, lr, lq,
       [&](int n, int c) {
@@ -407,6 +434,31 @@ __device__ __forceinline__ void la_weigh_infinite(f32x4_t (&o)[4], f32x4_t (&v)[
     for (int e = 0; e < 4; ++e) v[t][e] = la_infinite(v[t][e]) ? 0.0f : v[t][e];
 }
 
+// tab[n] = e^{g n} for n <= 64; put[n] = what token n of a whole chunk adds to the state with, gain e^{g (63 - n + lag)}, then zeros.
+__device__ __forceinline__ void la_tables(float2* tab, float* put, double g, float gain, int lag, int tid) {
+  if (tid <= LA_C) tab[tid] = la_decay2(g, tid);
+  if (tid >= 128 && tid < 256) put[tid - 128] = tid - 128 < LA_C ? gain * la_decay2(g, LA_C - 1 - (tid - 128) + lag).x : 0.0f;
+}
+
+// Where the caller's state has the lane's element e of tile i, column col: [dk][dv], or [dv][dk] with turned; -1 outside of it.
+template <bool BF16>
+__device__ __forceinline__ int la_user(const LaArgs& a, int i, int e, int lq, int col) {
+  const int row = la_row<BF16>(0, lq), more = la_row<BF16>(i, 0) + e;  // row + more
+  const int at = a.turned ? col * a.dk + row + more : row * a.dv + col + more * a.dv;
+  return row + more < a.dk && col < a.dv ? at : -1;
+}
+
+// The same of a state in a.mid that a call with dk and dv exchanged left, in tiles of NA rows: from the lane's own part, of row
+// 16 w + lr and columns la_row(0, lq) .., by what i and e add.
+template <bool BF16, int NA>
+__device__ __forceinline__ int la_turned(int i, int e, int w, int lr, int lq) {
+  const int row = 16 * w + lr;
+  const int tile = BF16 ? 2 * (row >> 5) + ((row >> 2) & 1) : row >> 4, q = BF16 ? (row >> 3) & 3 : (row >> 2) & 3;
+  const int own = (64 * tile + 16 * q) * 4 + (row & 3);
+  return BF16 ? own + (lq >> 1) * (256 * NA) + 32 * (lq & 1) + (i >> 1) * (512 * NA) + 16 * (i & 1) + 4 * e
+              : own + 16 * lq + i * (256 * NA) + 4 * e;
+}
+
 // One segment of one head; DV / 16 waves. Wave w has columns 16 w .. of the state and of the outputs for all 64 queries of a
 // chunk (outputs as [column, query] tiles), and some of the scores' six [32 keys, 16 queries] units, which go through LDS. The
 // state stays in accumulators, which, rounded, are the operand that queries read (la_row). A column's tokens come out of the
@@ -423,18 +475,19 @@ __global__ __launch_bounds__(4 * DV, la_waves(BF16, DK, DV, OUT)) void la_kernel
   __shared__ float put[2 * LA_C];   // what a token adds to the state with: of a chunk's 64, then zeros
   const int tid = threadIdx.x, lane = tid & 63, lr = lane & 15, lq = lane >> 4;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
-  if (OUT && blockIdx.x >= (unsigned)a.segs * a.H) {
-    la_gap(a, a.o, a.H * a.dv * (a.o_f32 ? 4 : ES), blockIdx.x - a.segs * a.H);
+  if (OUT && blockIdx.x >= la_units(a, a.segs)) {
+    la_gap(a, a.o, a.H * a.dv * (a.o_f32 ? 4 : ES), blockIdx.x - la_units(a, a.segs));
     return;
   }
-  const unsigned unit = la_unit_of(blockIdx.x, OUT ? (unsigned)a.segs * a.H : gridDim.x);
-  const int seg = (int)(unit / a.H), h = (int)(unit % a.H);
+  const LaUnit unit = la_unit_of(a, blockIdx.x);
+  const int seg = unit.seg, h = unit.h;
+  if (seg >= (OUT ? a.segs : a.segs - a.N)) return;
   const LaPlace p = la_place<OUT>(a, seg);
   if (!p.there) return;
   const int64_t first = a.plan == nullptr ? 0 : p.start;
   const int64_t sb = a.plan == nullptr ? p.seq : 0;
   auto start = [&](auto& stage, const LaTensor& t, int j0) {
-    const uint8_t* base = static_cast<const uint8_t*>(t.p) + ES * (sb * t.sb + first * t.st + (int64_t)(h / t.div) * t.sh);
+    const uint8_t* base = static_cast<const uint8_t*>(t.p) + ES * (sb * t.sb + first * t.st + (int64_t)(t.div == 1 ? h : unit.shared) * t.sh);
     if (REV) stage.start(base + (int64_t)(p.len - 1) * t.st * ES, -t.st * ES, j0);
     else stage.start(base, t.st * ES, j0);
   };
@@ -452,38 +505,36 @@ __global__ __launch_bounds__(4 * DV, la_waves(BF16, DK, DV, OUT)) void la_kernel
     kst.load(tid, rows, a.dk * ES);
     vst.load(tid, rows, a.dv * ES);
   };
-  // The first tiles are on their way while the state is read and the decays are made.
-  if (begin < end) fetch(min(LA_C, end - begin), Qs[0]);
+  const double g = (double)a.g[h];
   // Rows la_row(i, lq) .. + 3, column 16 w + lr.
   f32x4_t S[NA];
-  const int64_t slot = la_slot(a, p.seq) + p.s;
-  auto mid = [&](int64_t s, int i) {
-    return reinterpret_cast<f32x4_t*>(a.mid + (s * a.H + h) * (DK * DV) + ((w * NA + i) * 64 + lane) * 4);
-  };
-  // Row and column of the caller's state, whose rows may lie as columns.
-  const int64_t user = ((int64_t)p.seq * a.H + h) * a.dk * a.dv + (16 * w + lr) * (a.turned ? a.dk : 1);
-  const int user_row = a.turned ? 1 : a.dv;
+  const float* before = a.mid + ((la_slot(a, p.seq) + p.s - 1) * a.H + h) * (DK * DV);
+  const int64_t user = ((int64_t)p.seq * a.H + h) * a.dk * a.dv;
+  if (OUT && p.s > 0 && a.mid_turned) {
 #pragma unroll
-  for (int i = 0; i < NA; ++i) {
-    S[i] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-    if (!OUT) continue;
-    if (p.s > 0 && a.mid_turned) {
+    for (int i = 0; i < NA; ++i)
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        S[i][e] = a.mid[((slot - 1) * a.H + h) * (DK * DV) + la_place_of<BF16, DV / 16>(16 * w + lr, la_row<BF16>(i, lq) + e)];
-    } else if (p.s > 0) {
-      S[i] = *mid(slot - 1, i);
-    } else if (a.s0 != nullptr) {
+      for (int e = 0; e < 4; ++e) S[i][e] = before[la_turned<BF16, DV / 16>(i, e, w, lr, lq)];
+  } else if (OUT && p.s > 0) {
+#pragma unroll
+    for (int i = 0; i < NA; ++i) S[i] = *reinterpret_cast<const f32x4_t*>(before + ((w * NA + i) * 64 + lane) * 4);
+  } else if (OUT && a.s0 != nullptr) {
+#pragma unroll
+    for (int i = 0; i < NA; ++i)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const int row = la_row<BF16>(i, lq) + e;
-        if (row < a.dk && 16 * w + lr < a.dv) S[i][e] = a.s0[user + row * user_row];
+        const int at = la_user<BF16>(a, i, e, lq, 16 * w + lr);
+        const float x = (a.s0 + user)[max(at, 0)];
+        S[i][e] = at >= 0 ? x : 0.0f;
       }
-    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < NA; ++i) S[i] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
   }
-  const double g = (double)a.g[h];
-  if (tid <= LA_C) tab[tid] = la_decay2(g, tid);
-  if (tid < 2 * LA_C) put[tid] = tid < LA_C ? a.gain * la_decay2(g, LA_C - 1 - tid + a.lag).x : 0.0f;
+  // The first tiles are on their way while the decays are made (before the state, which is waited for first: 2048 tokens x 16
+  // heads of 128 take 42.4 us, so 40.2).
+  if (begin < end) fetch(min(LA_C, end - begin), Qs[0]);
+  la_tables(tab, put, g, a.gain, a.lag, tid);
   auto stage = [&]() {
     const int tid = afresh((int)threadIdx.x);
     kst.template store<BF16>(tid, Ks);
@@ -594,27 +645,19 @@ __global__ __launch_bounds__(4 * DV, la_waves(BF16, DK, DV, OUT)) void la_kernel
     __syncthreads();
     if (more) stage();
     if constexpr (OUT) {
+      const int lane = afresh((int)threadIdx.x) & 63, lr = lane & 15, lq = lane >> 4;
       const int c = 16 * w + 4 * lq;
       if constexpr (BF16) {
-        if (__builtin_expect(la_any_infinite(v), 0)) la_weigh_infinite(o, v, Ps, lr, lq);
+        if (__builtin_expect(more || keep ? la_any_infinite(S[0][0]) : la_any_infinite(v), 0)) la_weigh_infinite(o, v, Ps, lane);
+        la_weigh(o, v, Ps, lane);
       } else {
-        if (__builtin_expect(la_any_infinite(vf), 0)) la_weigh_infinite(o, vf, Ps, lr, lq);
+        if (__builtin_expect(more || keep ? la_any_infinite(S[0][0]) : la_any_infinite(vf), 0))
+          la_weigh_infinite(o, vf, Ps, lane);
+        la_weigh(o, vf, Ps, lane);
       }
       const int64_t out = sb * a.ob + (first + (REV ? p.len - 1 - j0 - lr : j0 + lr)) * a.ot + (int64_t)h * a.oh + c;
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
-        if constexpr (BF16) {
-#pragma unroll
-          for (int u = 0; u <= t / 2; ++u)
-            o[t] = mfma16x16x32(v[u], *reinterpret_cast<const u32x4_t*>(Ps + (la_unit(t, u) * 64 + lane) * 16), o[t]);
-        } else {
-#pragma unroll
-          for (int k = 0; k <= t; ++k) {
-            const f32x4_t s = *reinterpret_cast<const f32x4_t*>(Ps + ((2 * la_unit(t, k / 2) + k % 2) * 64 + lane) * 16);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o[t] = mfma16x16x4(vf[k][e], s[e], o[t]);
-          }
-        }
         if (j0 + 16 * t + lr >= end || c >= a.dv) continue;
         const int64_t to = out + (int64_t)(REV ? -(16 * t) : 16 * t) * a.ot;
         if (BF16 && !a.o_f32)
@@ -626,15 +669,16 @@ __global__ __launch_bounds__(4 * DV, la_waves(BF16, DK, DV, OUT)) void la_kernel
     }
   }
   if (!keep) return;
+  const int own = afresh(tid & 63);
 #pragma unroll
   for (int i = 0; i < NA; ++i) {
     if (!OUT) {
-      *mid(slot, i) = S[i];
+      *reinterpret_cast<f32x4_t*>(a.mid + ((la_slot(a, p.seq) + p.s) * a.H + h) * (DK * DV) + ((w * NA + i) * 64 + own) * 4) = S[i];
     } else {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const int row = la_row<BF16>(i, lq) + e;
-        if (row < a.dk && 16 * w + lr < a.dv) a.s1[user + row * user_row] = S[i][e];
+        const int at = la_user<BF16>(a, i, e, own >> 4, 16 * w + (own & 15));
+        if (at >= 0) (a.s1 + user)[at] = S[i][e];
       }
     }
   }
@@ -658,14 +702,15 @@ __global__ __launch_bounds__(4 * (DK + DV), DK == DV ? 4 : 3) void la_back_kerne
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const bool first_waves = w < WV;
   const int wc = first_waves ? w : w - WV;  // columns 16 wc .. of dv or dk
-  if (blockIdx.x >= (unsigned)a.s.segs * a.s.H) {
-    const int block = blockIdx.x - a.s.segs * a.s.H, es = a.s.o_f32 ? 4 : 2;
+  if (blockIdx.x >= la_units(a.s, a.s.segs)) {
+    const int block = blockIdx.x - la_units(a.s, a.s.segs), es = a.s.o_f32 ? 4 : 2;
     if (a.dk_out != nullptr) la_gap(a.s, a.dk_out, a.s.H * a.s.dk * es, block);
     if (a.dv_out != nullptr) la_gap(a.s, a.dv_out, a.s.H * a.s.dv * es, block);
     return;
   }
-  const unsigned unit = la_unit_of(blockIdx.x, (unsigned)a.s.segs * a.s.H);
-  const int seg = (int)(unit / a.s.H), h = (int)(unit % a.s.H);
+  const LaUnit unit = la_unit_of(a.s, blockIdx.x);
+  const int seg = unit.seg, h = unit.h;
+  if (seg >= a.s.segs) return;
   const LaPlace p = la_place<true>(a.s, seg);
   if (!p.there) return;
   const int64_t first = a.s.plan == nullptr ? 0 : p.start;
@@ -673,7 +718,7 @@ __global__ __launch_bounds__(4 * (DK + DV), DK == DV ? 4 : 3) void la_back_kerne
   const int begin = p.s * a.s.L, end = min(p.len, begin + a.s.L);
   const bool keep = p.s == p.nseg - 1 && a.s.s1 != nullptr;
   auto start = [&](auto& stage, const LaTensor& t) {
-    const uint8_t* base = static_cast<const uint8_t*>(t.p) + 2 * (sb * t.sb + first * t.st + (int64_t)(h / t.div) * t.sh);
+    const uint8_t* base = static_cast<const uint8_t*>(t.p) + 2 * (sb * t.sb + first * t.st + (int64_t)(t.div == 1 ? h : unit.shared) * t.sh);
     stage.start(base + (int64_t)(p.len - 1) * t.st * 2, -t.st * 2, begin);
   };
   using KeyTile = LaTile<true, KB>;
@@ -698,31 +743,32 @@ __global__ __launch_bounds__(4 * (DK + DV), DK == DV ? 4 : 3) void la_back_kerne
     vst.template store<false>(tid, Vs);
     dst.template store<false>(tid, Ds);
   };
+  const double g = (double)a.s.g[h];
   if (begin < end) fetch(min(LA_C, end - begin));
 
   f32x4_t T[NA];  // first waves: rows la_row(i, lq) .., column 16 w + lr
-  const int64_t user = ((int64_t)p.seq * a.s.H + h) * a.s.dk * a.s.dv + 16 * w + (tid & 15);
+  const int64_t user = ((int64_t)p.seq * a.s.H + h) * a.s.dk * a.s.dv;
   {
     const int lane = tid & 63, lr = lane & 15, lq = lane >> 4;
+    if (first_waves && p.s > 0) {
+      const float* before = a.s.mid + ((la_slot(a.s, p.seq) + p.s - 1) * a.s.H + h) * (DK * DV);
 #pragma unroll
-    for (int i = 0; i < NA; ++i) {
-      T[i] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-      if (!first_waves) continue;
-      if (p.s > 0) {
-        T[i] = *reinterpret_cast<const f32x4_t*>(a.s.mid + ((la_slot(a.s, p.seq) + p.s - 1) * a.s.H + h) * (DK * DV) +
-                                                 ((w * NA + i) * 64 + lane) * 4);
-      } else if (a.s.s0 != nullptr) {
+      for (int i = 0; i < NA; ++i) T[i] = *reinterpret_cast<const f32x4_t*>(before + ((w * NA + i) * 64 + lane) * 4);
+    } else if (first_waves && a.s.s0 != nullptr) {
+#pragma unroll
+      for (int i = 0; i < NA; ++i)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const int row = la_row<true>(i, lq) + e;
-          if (row < a.s.dk && 16 * w + lr < a.s.dv) T[i][e] = a.s.s0[user + row * a.s.dv];
+          const int at = la_user<true>(a.s, i, e, lq, 16 * w + lr);
+          const float x = (a.s.s0 + user)[max(at, 0)];
+          T[i][e] = at >= 0 ? x : 0.0f;
         }
-      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < NA; ++i) T[i] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
     }
   }
-  const double g = (double)a.s.g[h];
-  if (tid <= LA_C) tab[tid] = la_decay2(g, tid);
-  if (tid < 2 * LA_C) put[tid] = tid < LA_C ? a.s.gain * la_decay2(g, LA_C - tid).x : 0.0f;
+  la_tables(tab, put, g, a.s.gain, 1, tid);
   // Ts is [dv][dk]; rows 8 apart, which its transposing reads take together, are mixed as those 4 apart of other tiles are.
   auto state = [&](int row, int col) { return row * KB + ((col ^ KeyTile::key((row & 3) | ((row >> 1) & 4))) << 4); };
   auto publish = [&](int lr, int lq) {
@@ -788,19 +834,19 @@ __global__ __launch_bounds__(4 * (DK + DV), DK == DV ? 4 : 3) void la_back_kerne
       stage();
       if (first_waves) publish(lr, lq);
     }
+    const int me = afresh((int)threadIdx.x) & 63, mr = me & 15, mq = me >> 4;
     const uint8_t* const P = Ps[first_waves ? 0 : 1];
 #pragma unroll
-    for (int t = 0; t < 4; ++t) o[t] = o[t] * tab[16 * t + lr].x;
-    if (__builtin_expect(la_any_infinite(v), 0)) la_weigh_infinite(o, v, P, lr, lq);
-    const int c = 16 * wc + 4 * lq, d = first_waves ? a.s.dv : a.s.dk;
+    for (int t = 0; t < 4; ++t) o[t] = o[t] * tab[16 * t + mr].x;
+    if (__builtin_expect(first_waves && (more || keep) ? la_any_infinite(T[0][0]) : la_any_infinite(v), 0))
+      la_weigh_infinite(o, v, P, me);
+    la_weigh(o, v, P, me);
+    const int c = 16 * wc + 4 * mq, d = first_waves ? a.s.dv : a.s.dk;
     void* const to = first_waves ? a.dv_out : a.dk_out;
-    const int64_t ot = (int64_t)a.s.H * d, out = sb * a.s.S * ot + (first + p.len - 1 - j0 - lr) * ot + (int64_t)h * d + c;
+    const int64_t ot = (int64_t)a.s.H * d, out = sb * a.s.S * ot + (first + p.len - 1 - j0 - mr) * ot + (int64_t)h * d + c;
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
-#pragma unroll
-      for (int u = 0; u <= t / 2; ++u)
-        o[t] = mfma16x16x32(v[u], *reinterpret_cast<const u32x4_t*>(P + (la_unit(t, u) * 64 + lane) * 16), o[t]);
-      if (j0 + 16 * t + lr >= end || c >= d || to == nullptr) continue;
+      if (j0 + 16 * t + mr >= end || c >= d || to == nullptr) continue;
       if (a.s.o_f32)
         *reinterpret_cast<f32x4_t*>(static_cast<float*>(to) + out - 16 * t * ot) = o[t];
       else
@@ -809,13 +855,13 @@ __global__ __launch_bounds__(4 * (DK + DV), DK == DV ? 4 : 3) void la_back_kerne
     }
   }
   if (!keep || !first_waves) return;
-  const int lr = tid & 15, lq = (tid >> 4) & 3;
+  const int own = afresh(tid & 63);
 #pragma unroll
   for (int i = 0; i < NA; ++i)
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const int row = la_row<true>(i, lq) + e;
-      if (row < a.s.dk && 16 * w + lr < a.s.dv) a.s.s1[user + row * a.s.dv] = T[i][e];
+      const int at = la_user<true>(a.s, i, e, own >> 4, 16 * w + (own & 15));
+      if (at >= 0) (a.s.s1 + user)[at] = T[i][e];
     }
 }
 
@@ -931,14 +977,14 @@ __global__ __launch_bounds__(256) void la_step_kernel(LaStepArgs a) {
   }
 }
 
-unsigned la_blocks(const LaArgs& a) { return (unsigned)a.segs * a.H + (a.plan != nullptr ? (unsigned)(a.S + 63) / 64 : 0); }
+unsigned la_blocks(const LaArgs& a) { return la_units(a, a.segs) + (a.plan != nullptr ? (unsigned)(a.S + 63) / 64 : 0); }
 
 // What every segment adds to the state, and the states between them, into a.mid.
 template <bool BF16, int DK, int DV, bool REV>
 hipError_t la_states(const LaArgs& a, hipStream_t st) {
   const int64_t inner = a.segs - a.N;  // segments with another behind them, at most
   if (inner == 0) return hipSuccess;
-  hipLaunchKernelGGL((la_kernel<BF16, DK, DV, REV, false>), dim3((unsigned)(inner * a.H)), dim3(4 * DV), 0, st, a);
+  hipLaunchKernelGGL((la_kernel<BF16, DK, DV, REV, false>), dim3(la_units(a, (unsigned)inner)), dim3(4 * DV), 0, st, a);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
   hipLaunchKernelGGL((la_carry_kernel<BF16, DK, DV>), dim3((unsigned)(a.N * a.H), DK * DV / 1024), dim3(256), 0, st, a);
@@ -998,23 +1044,25 @@ struct LaBackBoth {
 
 }  // namespace
 
-// As long segments as still give every CU the workgroups that it holds, `per_cu`: more segments cost more states to write and read
-// (64 KB at widths of 128, as much as 64 tokens' queries to outputs), fewer leave CUs idle. Of packed sequences half a
-// segment each is taken to be lost to their ends. 4 x 4096 tokens x 16 heads of 128 forward and back with 1, 2, 4, 8 a CU:
-// 341, 339, 395, 513 us; 65536 tokens forward 447, 400, 433, 484.
-int la_segment_tokens(int64_t N, int64_t S, bool packed, int H, int per_cu) {
-  const int64_t want = std::max<int64_t>(1, (int64_t)per_cu * device_cus() / H), chunks = std::max<int64_t>(1, (S + LA_C - 1) / LA_C);
-  // A sequence of two chunks is quicker in one launch than in three: 128 tokens x 16 heads of 128 take 15.0 us, and 17.8 in two
-  // segments; 192 take 19.0 and 18.3.
-  if (!packed && chunks <= 2) return 2 * LA_C;
-  const int64_t n = packed ? std::max({want - N / 2, want / 2, (int64_t)1}) : std::max<int64_t>(1, want / std::max<int64_t>(1, N));
-  return (int)((chunks + n - 1) / n) * LA_C;
-}
-
-// Workgroups of la_kernel, or of la_back_kernel, on a CU, by their LDS and registers.
-int la_per_cu(bool bf16, int dk, int dv, bool back) {
+// Workgroups of la_kernel, or (back) of la_back_kernel, that a CU holds, by their LDS and registers.
+static int la_per_cu(bool bf16, int dk, int dv, bool back) {
   const bool narrow = dk <= 64 && dv <= 64;
   return back ? (narrow ? 2 : 1) : bf16 ? (narrow ? 4 : 2) : narrow ? 2 : 1;
+}
+
+// As long segments as still give every CU the workgroups that it holds: more segments cost more states to write and read (64 KB
+// at widths of 128, as much as 64 tokens' queries to outputs), fewer leave CUs idle. Of packed sequences half a segment each is
+// taken to be lost to their ends. 4 x 4096 tokens x 16 heads of 128 forward and back with 1, 2, 4, 8 a CU: 341, 339, 395,
+// 513 us; 65536 tokens forward 447, 400, 433, 484.
+int la_segment_tokens(int64_t N, int64_t S, bool packed, int H, bool bf16, int dk, int dv, bool back) {
+  const int per_cu = la_per_cu(bf16, dk, dv, back);
+  const int64_t want = std::max<int64_t>(1, (int64_t)per_cu * device_cus() / H), chunks = std::max<int64_t>(1, (S + LA_C - 1) / LA_C);
+  // Two chunks are quicker in one launch than in three but for wide fp32, whose chunk takes longest. 128 tokens x 16 heads
+  // forward in one and in two segments: bf16 of 128 15.0 and 17.8 us, fp32 of 64 16.8 and 18.0, fp32 of 128 32.1 and 31.9 (and
+  // back 77.7 and 69.5). Three chunks of bf16: 19.0 and 18.3.
+  if (!packed && chunks <= 2 && (bf16 || (dk <= 64 && dv <= 64))) return 2 * LA_C;
+  const int64_t n = packed ? std::max({want - N / 2, want / 2, (int64_t)1}) : std::max<int64_t>(1, want / std::max<int64_t>(1, N));
+  return (int)((chunks + n - 1) / n) * LA_C;
 }
 
 int64_t la_padded_state(int dk, int dv) { return (int64_t)(dk <= 64 ? 64 : 128) * (dv <= 64 ? 64 : 128); }
