@@ -866,7 +866,8 @@ __global__ __launch_bounds__(4 * (DK + DV), DK == DV ? 4 : 3) void la_back_kerne
 }
 
 // mid[s] = e^{g L} (the state before segment s) + mid[s]: the state behind every segment but a sequence's last. A thread has 4
-// elements of one state; reads run LA_AHEAD segments ahead.
+// elements of one state, and the reads of the next LA_AHEAD segments are on their way while those of the last are added (31
+// segments of 16 heads of 128: 14.2 -> 11.1 us, 65 MB at 5.9 TB/s).
 constexpr int LA_AHEAD = 8;
 template <bool BF16, int DK, int DV>
 __global__ __launch_bounds__(256) void la_carry_kernel(LaArgs a) {
@@ -889,18 +890,27 @@ __global__ __launch_bounds__(256) void la_carry_kernel(LaArgs a) {
   }
   f32x4_t* p = reinterpret_cast<f32x4_t*>(a.mid + (slot * a.H + h) * (DK * DV) + 4 * idx);
   const int64_t step = (int64_t)a.H * DK * DV / 4;
-  for (int s = 0; s < n; s += LA_AHEAD) {
-    f32x4_t x[LA_AHEAD];
+  f32x4_t x[2][LA_AHEAD];
+  auto read = [&](f32x4_t (&to)[LA_AHEAD], int s) {
 #pragma unroll
     for (int u = 0; u < LA_AHEAD; ++u)
-      if (s + u < n) x[u] = p[(s + u) * step];
+      if (s + u < n) to[u] = p[(s + u) * step];
+  };
+  auto write = [&](f32x4_t (&from)[LA_AHEAD], int s) {
 #pragma unroll
     for (int u = 0; u < LA_AHEAD; ++u) {
       if (s + u >= n) break;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) S[e] = fmaf(S[e], whole.x, fmaf(S[e], whole.y, x[u][e]));
+      for (int e = 0; e < 4; ++e) S[e] = fmaf(S[e], whole.x, fmaf(S[e], whole.y, from[u][e]));
       p[(s + u) * step] = S;
     }
+  };
+  read(x[0], 0);
+  for (int s = 0; s < n; s += 2 * LA_AHEAD) {
+    read(x[1], s + LA_AHEAD);
+    write(x[0], s);
+    read(x[0], s + 2 * LA_AHEAD);
+    write(x[1], s + LA_AHEAD);
   }
 }
 
@@ -1057,12 +1067,16 @@ static int la_per_cu(bool bf16, int dk, int dv, bool back) {
 int la_segment_tokens(int64_t N, int64_t S, bool packed, int H, bool bf16, int dk, int dv, bool back) {
   const int per_cu = la_per_cu(bf16, dk, dv, back);
   const int64_t want = std::max<int64_t>(1, (int64_t)per_cu * device_cus() / H), chunks = std::max<int64_t>(1, (S + LA_C - 1) / LA_C);
-  // Two chunks are quicker in one launch than in three but for wide fp32, whose chunk takes longest. 128 tokens x 16 heads
-  // forward in one and in two segments: bf16 of 128 15.0 and 17.8 us, fp32 of 64 16.8 and 18.0, fp32 of 128 32.1 and 31.9 (and
-  // back 77.7 and 69.5). Three chunks of bf16: 19.0 and 18.3.
-  if (!packed && chunks <= 2 && (bf16 || (dk <= 64 && dv <= 64))) return 2 * LA_C;
+  // Two chunks of bf16 are quicker in one launch than in three, of fp32, which take longer, not. 128 tokens x 16 heads of 128
+  // forward in one and in two segments: bf16 15.0 and 17.8 us, fp32 32.1 and 31.9 (and back 77.7 and 69.5). Three chunks of bf16:
+  // 19.0 and 18.3.
+  if (!packed && bf16 && chunks <= 2) return 2 * LA_C;
   const int64_t n = packed ? std::max({want - N / 2, want / 2, (int64_t)1}) : std::max<int64_t>(1, want / std::max<int64_t>(1, N));
-  return (int)((chunks + n - 1) / n) * LA_C;
+  // A segment of one chunk costs twice its bytes in states, which pays while half of the workgroups' places are empty (of
+  // la_back_kernel's to the last one): 1024 tokens x 16 heads of 128 forward with one and two chunks a segment 23.7 and 25.5 us,
+  // 2048 tokens 37.0 and 32.0, of 64 4096 tokens 29.1 and 24.9.
+  const bool two = !packed && bf16 && !back && 2 * chunks > n;
+  return (int)std::max<int64_t>(two ? 2 : 1, (chunks + n - 1) / n) * LA_C;
 }
 
 int64_t la_padded_state(int dk, int dv) { return (int64_t)(dk <= 64 ? 64 : 128) * (dv <= 64 ? 64 : 128); }
