@@ -1061,9 +1061,8 @@ static int la_per_cu(bool bf16, int dk, int dv, bool back) {
 }
 
 // As long segments as still give every CU the workgroups that it holds: more segments cost more states to write and read (64 KB
-// at widths of 128, as much as 64 tokens' queries to outputs), fewer leave CUs idle. Of packed sequences half a segment each is
-// taken to be lost to their ends. 4 x 4096 tokens x 16 heads of 128 forward and back with 1, 2, 4, 8 a CU: 341, 339, 395,
-// 513 us; 65536 tokens forward 447, 400, 433, 484.
+// at widths of 128, as much as 64 tokens' queries to outputs), fewer leave CUs idle. 4 x 4096 tokens x 16 heads of 128 forward
+// and back with 1, 2, 4, 8 a CU: 341, 339, 395, 513 us; 65536 tokens forward 447, 400, 433, 484.
 int la_segment_tokens(int64_t N, int64_t S, bool packed, int H, bool bf16, int dk, int dv, bool back) {
   const int per_cu = la_per_cu(bf16, dk, dv, back);
   const int64_t want = std::max<int64_t>(1, (int64_t)per_cu * device_cus() / H), chunks = std::max<int64_t>(1, (S + LA_C - 1) / LA_C);
@@ -1071,7 +1070,13 @@ int la_segment_tokens(int64_t N, int64_t S, bool packed, int H, bool bf16, int d
   // forward in one and in two segments: bf16 15.0 and 17.8 us, fp32 32.1 and 31.9 (and back 77.7 and 69.5). Three chunks of bf16:
   // 19.0 and 18.3.
   if (!packed && bf16 && chunks <= 2) return 2 * LA_C;
-  const int64_t n = packed ? std::max({want - N / 2, want / 2, (int64_t)1}) : std::max<int64_t>(1, want / std::max<int64_t>(1, N));
+  // Packed: sequences end inside of segments, half a one each, so these are made longer, up to a third; twice as long where the
+  // sequences alone fill the CUs and few of them have a second segment. 16 heads of 128 forward with n = want, 3/4, 1/2 of it, the
+  // mean of eight drawn sets: 8191 tokens in 8 sequences 84, 79, 84 us, in 23 83, 77, 85, in 100 95, 94, 84; 32768 in 12 258, 246,
+  // 287, in 120 260, 249, 231; in 3 with want - 1 and 3/4 of it 244, 263.
+  const int64_t n = !packed         ? std::max<int64_t>(1, want / std::max<int64_t>(1, N))
+                    : N >= 2 * want ? std::max<int64_t>(1, want / 2)
+                                    : std::max({want - N / 2, want * 3 / 4, (int64_t)1});
   // A segment of one chunk costs twice its bytes in states, which pays while half of the workgroups' places are empty (of
   // la_back_kernel's to the last one): 1024 tokens x 16 heads of 128 forward with one and two chunks a segment 23.7 and 25.5 us,
   // 2048 tokens 37.0 and 32.0, of 64 4096 tokens 29.1 and 24.9.
