@@ -434,7 +434,8 @@ __device__ __forceinline__ void la_weigh_infinite(f32x4_t (&o)[4], f32x4_t (&v)[
     for (int e = 0; e < 4; ++e) v[t][e] = la_infinite(v[t][e]) ? 0.0f : v[t][e];
 }
 
-// tab[n] = e^{g n} for n <= 64; put[n] = what token n of a whole chunk adds to the state with, gain e^{g (63 - n + lag)}, then zeros.
+// tab[n] = e^{g n} for n <= 64; put[n] = what token n of a whole chunk adds to the state with, gain e^{g (63 - n + lag)}, then
+// zeros.
 __device__ __forceinline__ void la_tables(float2* tab, float* put, double g, float gain, int lag, int tid) {
   if (tid <= LA_C) tab[tid] = la_decay2(g, tid);
   if (tid >= 128 && tid < 256) put[tid - 128] = tid - 128 < LA_C ? gain * la_decay2(g, LA_C - 1 - (tid - 128) + lag).x : 0.0f;
@@ -464,6 +465,8 @@ __device__ __forceinline__ int la_turned(int i, int e, int w, int lr, int lq) {
 // state stays in accumulators, which, rounded, are the operand that queries read (la_row). A column's tokens come out of the
 // transposing LDS read in the order in which an accumulator holds the scores' keys, once for the outputs and for the state.
 // Two barriers a chunk: tiles and scores are read behind one, scores and the next tiles written behind the other.
+// Memory-bound: 4 x 4096 tokens x 16 heads of 128 bf16 (MI355X) take 68 us with OUT (302 MB, 4.4 TB/s; a large copy reaches
+// 5.1) and 36 us without (163 MB, 4.5 TB/s). fp32 is bound by its matrix instructions and the reads of their operands.
 template <bool BF16, int DK, int DV, bool REV, bool OUT>
 __global__ __launch_bounds__(4 * DV, la_waves(BF16, DK, DV, OUT)) void la_kernel(LaArgs a) {
   constexpr int ES = BF16 ? 2 : 4, KB = DK * ES, VB = DV * ES, NA = DK / 16, W = DV / 16, THREADS = 4 * DV;
@@ -487,7 +490,8 @@ __global__ __launch_bounds__(4 * DV, la_waves(BF16, DK, DV, OUT)) void la_kernel
   const int64_t first = a.plan == nullptr ? 0 : p.start;
   const int64_t sb = a.plan == nullptr ? p.seq : 0;
   auto start = [&](auto& stage, const LaTensor& t, int j0) {
-    const uint8_t* base = static_cast<const uint8_t*>(t.p) + ES * (sb * t.sb + first * t.st + (int64_t)(t.div == 1 ? h : unit.shared) * t.sh);
+    const int head = t.div == 1 ? h : unit.shared;
+    const uint8_t* base = static_cast<const uint8_t*>(t.p) + ES * (sb * t.sb + first * t.st + (int64_t)head * t.sh);
     if (REV) stage.start(base + (int64_t)(p.len - 1) * t.st * ES, -t.st * ES, j0);
     else stage.start(base, t.st * ES, j0);
   };
@@ -689,7 +693,7 @@ __global__ __launch_bounds__(4 * DV, la_waves(BF16, DK, DV, OUT)) void la_kernel
 //   dk_j = scale sum_{i >= j} e^{g (i - j)} (v_j . dO_i) q_i + e^{g j'} T v_j
 // DV / 16 waves make dv and hold T as la_kernel's hold S; DK / 16 more make dk and read T, rounded, from LDS, where the first
 // ones leave it once a chunk. One pass over q, k, v and dO instead of two over three of them each, and T made once:
-// 4 x 4096 tokens, 16 heads of 128 (MI355X): see la_run_back.
+// 4 x 4096 tokens x 16 heads of 128 (MI355X) take 103 us (419 MB, 4.1 TB/s), two passes of la_kernel 2 x 68 and another carry.
 template <int DK, int DV>
 __global__ __launch_bounds__(4 * (DK + DV), DK == DV ? 4 : 3) void la_back_kernel(LaBackArgs a) {
   constexpr int KB = DK * 2, VB = DV * 2, NA = DK / 16, WV = DV / 16, WK = DK / 16, THREADS = 4 * (DK + DV);
@@ -718,7 +722,8 @@ __global__ __launch_bounds__(4 * (DK + DV), DK == DV ? 4 : 3) void la_back_kerne
   const int begin = p.s * a.s.L, end = min(p.len, begin + a.s.L);
   const bool keep = p.s == p.nseg - 1 && a.s.s1 != nullptr;
   auto start = [&](auto& stage, const LaTensor& t) {
-    const uint8_t* base = static_cast<const uint8_t*>(t.p) + 2 * (sb * t.sb + first * t.st + (int64_t)(t.div == 1 ? h : unit.shared) * t.sh);
+    const int head = t.div == 1 ? h : unit.shared;
+    const uint8_t* base = static_cast<const uint8_t*>(t.p) + 2 * (sb * t.sb + first * t.st + (int64_t)head * t.sh);
     stage.start(base + (int64_t)(p.len - 1) * t.st * 2, -t.st * 2, begin);
   };
   using KeyTile = LaTile<true, KB>;
@@ -916,7 +921,8 @@ __global__ __launch_bounds__(256) void la_carry_kernel(LaArgs a) {
 
 // out[t][hk][c] = sum over the G heads that share hk of x[t][hk G + i][c], fp32 in, one rounding.
 template <bool BF16>
-__global__ __launch_bounds__(256) void la_group_kernel(const float* __restrict__ x, void* __restrict__ out, int64_t n4, int G, int d4) {
+__global__ __launch_bounds__(256) void la_group_kernel(const float* __restrict__ x, void* __restrict__ out, int64_t n4, int G,
+                                                       int d4) {
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n4; i += (int64_t)gridDim.x * 256) {
     const int64_t row = i / d4;
     const int c = (int)(i - row * d4);
@@ -930,7 +936,7 @@ __global__ __launch_bounds__(256) void la_group_kernel(const float* __restrict__
 }
 
 // One token: S = e^g S + k v^T in place, o = scale S^T q. Workgroup: 32 columns of one state, thread: 4 columns of every 32nd
-// row; HBM-bound, 8 bytes per element of the states.
+// row; HBM-bound, 8 bytes per element of the states: 256 sequences x 16 heads of 128 x 128 take 113 us (541 MB, 4.8 TB/s).
 template <bool BF16>
 __global__ __launch_bounds__(256) void la_step_kernel(LaStepArgs a) {
   constexpr int ES = BF16 ? 2 : 4;
@@ -948,7 +954,13 @@ __global__ __launch_bounds__(256) void la_step_kernel(LaStepArgs a) {
     return BF16 ? bf16_to_f32(*reinterpret_cast<const uint16_t*>(at)) : *reinterpret_cast<const float*>(at);
   };
   f32x4_t o = {0.0f, 0.0f, 0.0f, 0.0f};
-  if (slot >= 0 && slot < a.pool) {
+  bool mine = slot >= 0 && slot < a.pool;
+  if (a.slots != nullptr) {  // not one that an earlier sequence has: both would write it (without this look 94 us, with it 97)
+    bool before = false;
+    for (int64_t n = tid; n < b; n += 256) before |= a.slots[n] == slot;
+    mine &= !__syncthreads_or(before);
+  }
+  if (mine) {
     const float lam = (float)exp((double)a.g[h]);
     f32x4_t v = {0.0f, 0.0f, 0.0f, 0.0f};
     if (there) {
@@ -1065,7 +1077,8 @@ static int la_per_cu(bool bf16, int dk, int dv, bool back) {
 // and back with 1, 2, 4, 8 a CU: 341, 339, 395, 513 us; 65536 tokens forward 447, 400, 433, 484.
 int la_segment_tokens(int64_t N, int64_t S, bool packed, int H, bool bf16, int dk, int dv, bool back) {
   const int per_cu = la_per_cu(bf16, dk, dv, back);
-  const int64_t want = std::max<int64_t>(1, (int64_t)per_cu * device_cus() / H), chunks = std::max<int64_t>(1, (S + LA_C - 1) / LA_C);
+  const int64_t want = std::max<int64_t>(1, (int64_t)per_cu * device_cus() / H);
+  const int64_t chunks = std::max<int64_t>(1, (S + LA_C - 1) / LA_C);
   // Two chunks of bf16 are quicker in one launch than in three, of fp32, which take longer, not. 128 tokens x 16 heads of 128
   // forward in one and in two segments: bf16 15.0 and 17.8 us, fp32 32.1 and 31.9 (and back 77.7 and 69.5). Three chunks of bf16:
   // 19.0 and 18.3.

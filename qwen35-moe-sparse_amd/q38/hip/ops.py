@@ -1536,8 +1536,8 @@ def _step_plan(dt, k_dt, v_dt, qs, ks, vs, q_stride, k_stride, v_stride, state, 
 def linear_attention_step(q, k, v, state, log_decay, scale=None, slots=None):
     """One token of every sequence through ``linear_attention`` (q38moe_linear_attention_step): q [B,H,dk], k [B,Hk,dk], v
     [B,Hk,dv] (bf16 or fp32), the states [pool,H,dk,dv] (fp32, contiguous) updated in place. Sequence b has the state
-    slots[b] (int32 [B]; without slots the state b); a slot outside the pool is none: nothing is updated and the output is zero.
-    No slot may occur twice. scale: dk^-1/2 unless given. Returns out [B,H,dv]; no gradients."""
+    slots[b] (int32 [B]; without slots the state b); a slot outside the pool, or that of an earlier sequence, is none: nothing
+    is updated and the output is zero. scale: dk^-1/2 unless given. Returns out [B,H,dv]; no gradients."""
     _tensors(q=q, k=k, v=v, state=state, log_decay=log_decay)
     _float_type(q.dtype, "q")
     dev = _one_gpu(q, k, v, state, log_decay, slots)

@@ -444,6 +444,23 @@ def test_step(gpu, dtype, B, H, Hk, dk, dv, pool):
         _within(out[b], o, e + vh * (o.abs() + e) + 1e-37, "out")
 
 
+@pytest.mark.parametrize("B,again", [(2, (0, 1)), (301, (3, 300)), (301, (12, 13))])
+def test_step_with_a_slot_twice(gpu, B, again):
+    """The sequence that names a slot first has it; the other gets zero, and nothing else changes: bits as without the other."""
+    from q38.hip import ops
+    r = torch.Generator(device=gpu).manual_seed(B)
+    q, k, v = (_randn(r, B, 2, 64, dtype=torch.bfloat16) for _ in range(3))
+    state = _randn(r, B + 4, 2, 64, 64)
+    g = -torch.rand(2, generator=r, device=gpu)
+    slots = torch.randperm(B + 4, generator=r, device=gpu)[:B].int()
+    twice, without = slots.clone(), slots.clone()
+    twice[again[1]], without[again[1]] = slots[again[0]], -1
+    a, b = state.clone(), state.clone()
+    assert torch.equal(ops.linear_attention_step(q, k, v, a, g, slots=twice),
+                       ops.linear_attention_step(q, k, v, b, g, slots=without))
+    assert torch.equal(a, b)
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_prompt_then_tokens(gpu, dtype):
     """As they are used: a fused projection's heads normed and rotated, the prompts through linear attention, then token by token
