@@ -626,9 +626,10 @@ int q38moe_linear_attention_forward(const void* q, const void* k, const void* v,
                                     void* stream);
 int q38moe_linear_attention_backward(const void* d_out, const float* d_final_state, const void* q, const void* k, const void* v,
                                      const int64_t* strides, const float* log_decay, float scale, const float* initial_state,
-                                     const int32_t* cu_seqlens, const void* saved, size_t saved_bytes, void* dq, void* dk_out, void* dv_out, float* d_initial_state,
-                                     int64_t N, int64_t S, int32_t H, int32_t Hk, int32_t dk, int32_t dv, void* workspace,
-                                     size_t workspace_bytes, int32_t dtype, void* stream);
+                                     const int32_t* cu_seqlens, const void* saved, size_t saved_bytes, void* dq, void* dk_out,
+                                     void* dv_out, float* d_initial_state, int64_t N, int64_t S, int32_t H, int32_t Hk,
+                                     int32_t dk, int32_t dv, void* workspace, size_t workspace_bytes, int32_t dtype,
+                                     void* stream);
 int q38moe_linear_attention_step(const void* q, const void* k, const void* v, const int64_t* strides, const float* log_decay,
                                  float scale, float* state, const int32_t* slots, void* out, int64_t B, int64_t pool, int32_t H,
                                  int32_t Hk, int32_t dk, int32_t dv, int32_t dtype, void* stream);

@@ -2013,8 +2013,8 @@ int q38moe_linear_attention_forward(const void* q, const void* k, const void* v,
 
 int q38moe_linear_attention_backward(const void* d_out, const float* d_final_state, const void* q, const void* k, const void* v,
                                      const int64_t* strides, const float* log_decay, float scale, const float* initial_state,
-                                     const int32_t* cu_seqlens, const void* saved, size_t saved_bytes, void* dq, void* dk_out, void* dv_out, float* d_initial_state,
-                                     int64_t N, int64_t S, int32_t H, int32_t Hk, int32_t dk, int32_t dv, void* workspace,
+                                     const int32_t* cu_seqlens, const void* saved, size_t saved_bytes, void* dq, void* dk_out,
+                                     void* dv_out, float* d_initial_state, int64_t N, int64_t S, int32_t H, int32_t Hk, int32_t dk, int32_t dv, void* workspace,
                                      size_t workspace_bytes, int32_t dtype, void* stream) {
   g_err[0] = 0;
   Q38_CHECK(check_strides(strides, 9, dtype));
@@ -2042,13 +2042,6 @@ int q38moe_linear_attention_backward(const void* d_out, const float* d_final_sta
   const int64_t do_strides[3] = {S * (int64_t)H * dv, (int64_t)H * dv, dv};
   const q38::LaTensor tq = la_tensor(q, strides, 1), tk = la_tensor(k, strides + 3, G), tv = la_tensor(v, strides + 6, G),
                       tdo = la_tensor(d_out, do_strides, 1);
-  // Results of Hk heads: added from those of each, which went to the workspace.
-  auto finish = [&](void* out, const char* heads, int d) -> int {
-    if (out == nullptr || p.tokens == 0 || G == 1) return Q38MOE_OK;
-    Q38_HIP(q38::launch_la_group(reinterpret_cast<const float*>(heads), out, p.tokens * Hk, G, d, bf16, st),
-            "linear attention backward launch");
-    return Q38MOE_OK;
-  };
   auto results = [&](q38::LaArgs& b, void* out, char* heads, int d, bool shared) {
     b.o = shared && G > 1 && out != nullptr ? heads : out;
     b.o_f32 = (shared && G > 1) || !bf16;
@@ -2090,8 +2083,12 @@ int q38moe_linear_attention_backward(const void* d_out, const float* d_final_sta
       Q38_HIP(q38::launch_la_backwards_f32(a, st), "linear attention backward launch");
     }
   }
-  Q38_CHECK(finish(dk_out, k_heads, dk));
-  return finish(dv_out, v_heads, dv);
+  // Results of Hk heads: added from those of each, which went to the workspace.
+  if (G > 1)
+    Q38_HIP(q38::launch_la_group({reinterpret_cast<const float*>(k_heads), dk_out, dk},
+                                 {reinterpret_cast<const float*>(v_heads), dv_out, dv}, p.tokens * Hk, G, bf16, st),
+            "linear attention backward launch");
+  return Q38MOE_OK;
 }
 
 int q38moe_linear_attention_step(const void* q, const void* k, const void* v, const int64_t* strides, const float* log_decay,

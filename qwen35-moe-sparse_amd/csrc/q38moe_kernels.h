@@ -277,9 +277,8 @@ struct LaTensor {
 // One pass: o_i = intra sum_{j <= i} e^{g (i - j)} (q_i . k_j) v_j + inter e^{g (i + 1 - lag)} S^T q_i and S = e^{g L} S + gain
 // sum_j e^{g (L - 1 - j + lag)} k_j v_j^T, tokens taken forwards or backwards. s0, s1 (may be NULL): the caller's states [N, H, dk, dv],
 // turned: [N, H, dv, dk]. mid: a state per segment of L tokens with another behind it; mid_turned: as a call with dk and dv
-// exchanged left it. plan (packed sequences) or NULL (N sequences of S tokens, nseg
-// segments each); segs: at most, of all sequences. group: heads that
-// share keys and values.
+// exchanged left it. plan (packed sequences) or NULL (N sequences of S tokens, nseg segments each); segs: at most, of all
+// sequences. group: heads that share keys and values.
 struct LaArgs {
   LaTensor q, k, v;
   void* o;
@@ -315,7 +314,13 @@ hipError_t launch_la_plan(const int32_t* cu, int32_t* plan, int N, int S, int L,
 hipError_t launch_la(const LaArgs& a, bool states, bool bf16, hipStream_t st);
 hipError_t launch_la_backwards_f32(const LaArgs& a, hipStream_t st);
 hipError_t launch_la_back_bf16(const LaBackArgs& a, hipStream_t st);
-hipError_t launch_la_group(const float* x, void* out, int64_t rows, int G, int d, bool bf16, hipStream_t st);
+// Gradients [rows, G, d] of heads that share one, added to out [rows, d]; two of them, out NULL: not this one.
+struct LaGroup {
+  const float* x;
+  void* out;
+  int d;
+};
+hipError_t launch_la_group(const LaGroup& a, const LaGroup& b, int64_t rows, int G, bool bf16, hipStream_t st);
 hipError_t launch_la_step(const LaStepArgs& a, bool bf16, hipStream_t st);
 
 }  // namespace q38

@@ -919,19 +919,20 @@ __global__ __launch_bounds__(256) void la_carry_kernel(LaArgs a) {
   }
 }
 
-// out[t][hk][c] = sum over the G heads that share hk of x[t][hk G + i][c], fp32 in, one rounding.
+// out[t][hk][c] = sum over the G heads that share hk of x[t][hk G + i][c], fp32 in, one rounding; of two such in one launch.
 template <bool BF16>
-__global__ __launch_bounds__(256) void la_group_kernel(const float* __restrict__ x, void* __restrict__ out, int64_t n4, int G,
-                                                       int d4) {
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n4; i += (int64_t)gridDim.x * 256) {
+__global__ __launch_bounds__(256) void la_group_kernel(LaGroup a, LaGroup b, int64_t rows, int G) {
+  const LaGroup g = blockIdx.y == 0 ? a : b;
+  const int d4 = g.d / 4;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < rows * d4; i += (int64_t)gridDim.x * 256) {
     const int64_t row = i / d4;
     const int c = (int)(i - row * d4);
     f32x4_t s = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int j = 0; j < G; ++j) s += *reinterpret_cast<const f32x4_t*>(x + ((row * G + j) * d4 + c) * 4);
+    for (int j = 0; j < G; ++j) s += *reinterpret_cast<const f32x4_t*>(g.x + ((row * G + j) * d4 + c) * 4);
     if (BF16)
-      *reinterpret_cast<uint2*>(static_cast<uint16_t*>(out) + 4 * i) = make_uint2(pack_bf16x2(s[0], s[1]), pack_bf16x2(s[2], s[3]));
+      *reinterpret_cast<uint2*>(static_cast<uint16_t*>(g.out) + 4 * i) = make_uint2(pack_bf16x2(s[0], s[1]), pack_bf16x2(s[2], s[3]));
     else
-      *reinterpret_cast<f32x4_t*>(static_cast<float*>(out) + 4 * i) = s;
+      *reinterpret_cast<f32x4_t*>(static_cast<float*>(g.out) + 4 * i) = s;
   }
 }
 
@@ -1116,12 +1117,14 @@ hipError_t launch_la_back_bf16(const LaBackArgs& a, hipStream_t st) {
   return la_widths(a.s.dk, a.s.dv, LaBackBoth{a, st});
 }
 
-hipError_t launch_la_group(const float* x, void* out, int64_t rows, int G, int d, bool bf16, hipStream_t st) {
-  const int64_t n4 = rows * (d / 4);
-  const dim3 grid((unsigned)std::min<int64_t>((n4 + 255) / 256, 16 * (int64_t)device_cus()));
-  if (n4 == 0) return hipSuccess;
-  if (bf16) hipLaunchKernelGGL(la_group_kernel<true>, grid, dim3(256), 0, st, x, out, n4, G, d / 4);
-  else hipLaunchKernelGGL(la_group_kernel<false>, grid, dim3(256), 0, st, x, out, n4, G, d / 4);
+hipError_t launch_la_group(const LaGroup& a, const LaGroup& b, int64_t rows, int G, bool bf16, hipStream_t st) {
+  const LaGroup first = a.out != nullptr ? a : b;
+  const int both = a.out != nullptr && b.out != nullptr;
+  const int64_t n4 = rows * ((both ? std::max(a.d, b.d) : first.d) / 4);
+  if (first.out == nullptr || n4 == 0) return hipSuccess;
+  const dim3 grid((unsigned)std::min<int64_t>((n4 + 255) / 256, 16 * (int64_t)device_cus()), 1 + both);
+  if (bf16) hipLaunchKernelGGL(la_group_kernel<true>, grid, dim3(256), 0, st, first, b, rows, G);
+  else hipLaunchKernelGGL(la_group_kernel<false>, grid, dim3(256), 0, st, first, b, rows, G);
   return hipGetLastError();
 }
 
