@@ -12,8 +12,10 @@
 // to the state, la_carry_kernel runs over the segments, la_kernel<OUT = true> goes through the chunks of each with the state
 // in its accumulators.
 //
-// bf16 roundings: the weighted scores and the state that queries read, each once, as operands of the matrix units; what
-// goes into the state itself is split into three bf16 parts (24 bits), so that the state is as exact as in fp32.
+// bf16 roundings: the state that queries read, once, as an operand of the matrix units (16384 values' errors, which average out).
+// The weighted scores are split into two bf16 parts (16 bits): where a call has few of them, their errors would not, and all of an
+// output row shares its score's (a token alone was 0.0027 off, 0.0017 now, the rounding of the result; 1 to 2 % in time). What goes
+// into the state itself is split into three parts (24 bits), so that the state is as exact as in fp32.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -247,11 +249,12 @@ __device__ __forceinline__ int la_row(int i, int q) {
   return BF16 ? 32 * (i >> 1) + 8 * q + 4 * (i & 1) : 16 * i + 4 * q;
 }
 
-// bf16: one unit's scores, weighted and rounded, as an operand. KEYS_SWAPPED: the keys' odd rows lie with the halves of their columns
-// exchanged. row_at: see la_kernel.
+// bf16: one unit's scores, weighted, to `to` as operands: rounded, and behind the units what that left. KEYS_SWAPPED: the keys' odd
+// rows lie with the halves of their columns exchanged. row_at: see la_kernel.
+constexpr int LA_SCORES = LA_UNITS * 1024;
 template <int BYTES, bool KEYS_SWAPPED>
-__device__ __forceinline__ u32x4_t la_scores(const uint8_t* keys, const uint8_t* queries, int unit, int lr, int lq,
-                                             int row_at, float intra, const float2* tab) {
+__device__ __forceinline__ void la_scores(const uint8_t* keys, const uint8_t* queries, uint8_t* to, int unit, int lr, int lq,
+                                          int row_at, float intra, const float2* tab) {
   const int t = la_unit_queries(unit), u = la_unit_keys(unit);
   auto key = [&](const uint8_t* at) {
     const u32x4_t k = *reinterpret_cast<const u32x4_t*>(at);
@@ -273,7 +276,19 @@ __device__ __forceinline__ u32x4_t la_scores(const uint8_t* keys, const uint8_t*
       const int n = 16 * (t - 2 * u - k) + lr - 4 * lq - e;  // tokens between key and query
       P[k][e] = n >= 0 ? P[k][e] * (intra * tab[max(n, 0)].x) : 0.0f;
     }
-  return la_pack(P[0], P[1]);
+  const u32x4_t high = la_pack(P[0], P[1]);
+#pragma unroll
+  for (int z = 0; z < 4; ++z) {
+    float x0, x1;
+    unpack_bf16x2(high[z], x0, x1);
+    const int e = 2 * (z & 1);
+    const float y0 = P[z >> 1][e] - x0, y1 = P[z >> 1][e + 1] - x1;
+    P[z >> 1][e] = y0 == y0 ? y0 : 0.0f;  // an infinity leaves nothing
+    P[z >> 1][e + 1] = y1 == y1 ? y1 : 0.0f;
+  }
+  uint8_t* const at = to + (unit * 64 + 16 * lq + lr) * 16;
+  *reinterpret_cast<u32x4_t*>(at) = high;
+  *reinterpret_cast<u32x4_t*>(at + LA_SCORES) = la_pack(P[0], P[1]);
 }
 
 // bf16: S = e^{g rows} S + the chunk's k v^T. v: the wave's column's tokens as operands; k: the row-major tile of BYTES a row, its
@@ -376,7 +391,9 @@ __device__ __forceinline__ void la_weigh(f32x4_t (&o)[4], const u32x4_t (&v)[2],
   for (int t = 0; t < 4; ++t)
 #pragma unroll
     for (int u = 0; u <= t / 2; ++u)
-      o[t] = mfma16x16x32(v[u], *reinterpret_cast<const u32x4_t*>(scores + (la_unit(t, u) * 64 + lane) * 16), o[t]);
+#pragma unroll
+      for (int part = 0; part < 2 * LA_SCORES; part += LA_SCORES)
+        o[t] = mfma16x16x32(v[u], *reinterpret_cast<const u32x4_t*>(scores + (la_unit(t, u) * 64 + lane) * 16 + part), o[t]);
 }
 __device__ __forceinline__ void la_weigh_infinite(f32x4_t (&o)[4], u32x4_t (&v)[2], const uint8_t* scores, int lane) {
   const int lr = lane & 15, lq = lane >> 4;
@@ -391,7 +408,8 @@ __device__ __forceinline__ void la_weigh_infinite(f32x4_t (&o)[4], u32x4_t (&v)[
       [&](int t, int n) {
         const int unit = t == 3 ? n >> 5 : t == 2 ? 2 + 3 * (n >> 5) : 4 - t, lane = 16 * ((n >> 2) & 3) + lr;
         const uint8_t* at = scores + (unit * 64 + lane) * 16 + 8 * ((n >> 4) & 1) + 2 * (n & 3);
-        return bf16_to_f32(*reinterpret_cast<const uint16_t*>(at));
+        auto part = [](const uint8_t* x) { return bf16_to_f32(*reinterpret_cast<const uint16_t*>(x)); };
+        return part(at) + part(at + LA_SCORES);
       });
 #pragma unroll
   for (int u = 0; u < 2; ++u)
@@ -472,8 +490,11 @@ __global__ __launch_bounds__(4 * DV, la_waves(BF16, DK, DV, OUT)) void la_kernel
   constexpr int ES = BF16 ? 2 : 4, KB = DK * ES, VB = DV * ES, NA = DK / 16, W = DV / 16, THREADS = 4 * DV;
   __shared__ __attribute__((aligned(16))) uint8_t Ks[LA_C * KB];
   __shared__ __attribute__((aligned(16))) uint8_t Vs[LA_C * VB];
-  __shared__ __attribute__((aligned(16))) uint8_t Qs[2][OUT ? LA_C * KB : 16];
-  __shared__ __attribute__((aligned(16))) uint8_t Ps[OUT ? LA_UNITS * 512 * ES : 16];
+  // Queries go straight to LDS, to the other of two tiles; narrow ones through registers like keys and values, so that four
+  // workgroups' LDS fit on a CU.
+  constexpr bool COPY = !(BF16 && DK == 64 && DV == 64);
+  __shared__ __attribute__((aligned(16))) uint8_t Qs[1 + COPY][OUT ? LA_C * KB : 16];
+  __shared__ __attribute__((aligned(16))) uint8_t Ps[OUT ? 2 * LA_SCORES : 16];
   __shared__ float2 tab[LA_C + 1];  // e^{g n} to 48 bits
   __shared__ float put[2 * LA_C];   // what a token adds to the state with: of a chunk's 64, then zeros
   const int tid = threadIdx.x, lane = tid & 63, lr = lane & 15, lq = lane >> 4;
@@ -505,7 +526,8 @@ __global__ __launch_bounds__(4 * DV, la_waves(BF16, DK, DV, OUT)) void la_kernel
   if (OUT) start(qst, a.q, begin);
   auto fetch = [&](int rows, uint8_t* queries) {
     const int tid = afresh((int)threadIdx.x);
-    if (OUT) qst.copy(tid, queries, rows, a.dk * ES);  // first: done when the others are
+    if (OUT && COPY) qst.copy(tid, queries, rows, a.dk * ES);  // first: done when the others are
+    if (OUT && !COPY) qst.load(tid, rows, a.dk * ES);
     kst.load(tid, rows, a.dk * ES);
     vst.load(tid, rows, a.dv * ES);
   };
@@ -543,15 +565,16 @@ __global__ __launch_bounds__(4 * DV, la_waves(BF16, DK, DV, OUT)) void la_kernel
     const int tid = afresh((int)threadIdx.x);
     kst.template store<BF16>(tid, Ks);
     vst.template store<false>(tid, Vs);
-    wait_vmcnt0();  // the queries' copy
+    if (OUT && !COPY) qst.template store<false>(tid, Qs[0]);
+    if (OUT && COPY) wait_vmcnt0();  // the queries' copy
   };
   if (begin < end) stage();
   for (int j0 = begin, par = 0; j0 < end; j0 += LA_C, par ^= 1) {
     const int rows = min(LA_C, end - j0);
     const bool more = j0 + LA_C < end;
     __syncthreads();
-    if (more) fetch(min(LA_C, end - j0 - LA_C), Qs[par ^ 1]);
-    const uint8_t* const Q = Qs[par];
+    if (more) fetch(min(LA_C, end - j0 - LA_C), Qs[COPY ? par ^ 1 : 0]);
+    const uint8_t* const Q = Qs[COPY ? par : 0];
     const int lane = afresh(tid & 63), lr = lane & 15, lq = lane >> 4;
     using KeyTile = LaTile<BF16, KB>;
     using ValueTile = LaTile<BF16, VB>;
@@ -565,8 +588,7 @@ __global__ __launch_bounds__(4 * DV, la_waves(BF16, DK, DV, OUT)) void la_kernel
       // Scores of queries 16 t + lr with keys 32 u + {4 lq .., 16 + 4 lq ..}, weighted.
       for (int unit = w; unit < LA_UNITS; unit += W) {
         if constexpr (BF16) {
-          *reinterpret_cast<u32x4_t*>(Ps + (unit * 64 + lane) * 16) =
-              la_scores<KB, true>(Ks, Q, unit, lr, lq, row_at, a.intra, tab);
+          la_scores<KB, true>(Ks, Q, Ps, unit, lr, lq, row_at, a.intra, tab);
         } else {
           const int t = la_unit_queries(unit), u = la_unit_keys(unit);
 #pragma unroll
@@ -699,7 +721,7 @@ __global__ __launch_bounds__(4 * (DK + DV), DK == DV ? 4 : 3) void la_back_kerne
   constexpr int KB = DK * 2, VB = DV * 2, NA = DK / 16, WV = DV / 16, WK = DK / 16, THREADS = 4 * (DK + DV);
   __shared__ __attribute__((aligned(16))) uint8_t Qs[LA_C * KB], Ks[LA_C * KB], Vs[LA_C * VB], Ds[LA_C * VB];
   __shared__ __attribute__((aligned(16))) uint8_t Ts[DV * KB];
-  __shared__ __attribute__((aligned(16))) uint8_t Ps[2][LA_UNITS * 1024];
+  __shared__ __attribute__((aligned(16))) uint8_t Ps[2][2 * LA_SCORES];
   __shared__ float2 tab[LA_C + 1];
   __shared__ float put[2 * LA_C];
   const int tid = threadIdx.x;
@@ -800,8 +822,7 @@ __global__ __launch_bounds__(4 * (DK + DV), DK == DV ? 4 : 3) void la_back_kerne
       const int column_at = KeyTile::at(4 * lq + (lr >> 2), lr & 3) + 8 * KeyTile::swapped(lr >> 2);
       const int value_at = ValueTile::at(4 * lq + (lr >> 2), 2 * wc + ((lr & 3) >> 1)) + 8 * (lr & 1);
       for (int unit = wc; unit < LA_UNITS; unit += WV)
-        *reinterpret_cast<u32x4_t*>(Ps[0] + (unit * 64 + lane) * 16) =
-            la_scores<KB, true>(Qs, Ks, unit, lr, lq, row_at, a.s.intra, tab);
+        la_scores<KB, true>(Qs, Ks, Ps[0], unit, lr, lq, row_at, a.s.intra, tab);
 #pragma unroll
       for (int s = 0; s < KB / 64; ++s) {
         const u32x4_t x = la_pack(T[2 * s], T[2 * s + 1]);
@@ -821,8 +842,7 @@ __global__ __launch_bounds__(4 * (DK + DV), DK == DV ? 4 : 3) void la_back_kerne
 #pragma unroll
       for (int i = 0; i < 2; ++i) state_at[i] = state(8 * lq + 4 * i + (lr >> 2), 2 * wc + ((lr & 3) >> 1)) + 8 * (lr & 1);
       for (int unit = wc; unit < LA_UNITS; unit += WK)
-        *reinterpret_cast<u32x4_t*>(Ps[1] + (unit * 64 + lane) * 16) =
-            la_scores<VB, false>(Ds, Vs, unit, lr, lq, row_at, a.s.intra, tab);
+        la_scores<VB, false>(Ds, Vs, Ps[1], unit, lr, lq, row_at, a.s.intra, tab);
 #pragma unroll
       for (int s = 0; s < VB / 64; ++s) {
         const uint2 x = la_read_tr(Ts + state_at[0] + 32 * KB * s), y = la_read_tr(Ts + state_at[1] + 32 * KB * s);
@@ -930,7 +950,8 @@ __global__ __launch_bounds__(256) void la_group_kernel(LaGroup a, LaGroup b, int
     f32x4_t s = {0.0f, 0.0f, 0.0f, 0.0f};
     for (int j = 0; j < G; ++j) s += *reinterpret_cast<const f32x4_t*>(g.x + ((row * G + j) * d4 + c) * 4);
     if (BF16)
-      *reinterpret_cast<uint2*>(static_cast<uint16_t*>(g.out) + 4 * i) = make_uint2(pack_bf16x2(s[0], s[1]), pack_bf16x2(s[2], s[3]));
+      *reinterpret_cast<uint2*>(static_cast<uint16_t*>(g.out) + 4 * i) =
+          make_uint2(pack_bf16x2(s[0], s[1]), pack_bf16x2(s[2], s[3]));
     else
       *reinterpret_cast<f32x4_t*>(static_cast<float*>(g.out) + 4 * i) = s;
   }
