@@ -715,7 +715,7 @@ __global__ __launch_bounds__(4 * DV, la_waves(BF16, DK, DV, OUT)) void la_kernel
 //   dk_j = scale sum_{i >= j} e^{g (i - j)} (v_j . dO_i) q_i + e^{g j'} T v_j
 // DV / 16 waves make dv and hold T as la_kernel's hold S; DK / 16 more make dk and read T, rounded, from LDS, where the first
 // ones leave it once a chunk. One pass over q, k, v and dO instead of two over three of them each, and T made once:
-// 4 x 4096 tokens x 16 heads of 128 (MI355X) take 103 us (419 MB, 4.1 TB/s), two passes of la_kernel 2 x 68 and another carry.
+// 4 x 4096 tokens x 16 heads of 128 (MI355X) take 110 us (419 MB, 3.8 TB/s), two passes of la_kernel 2 x 68 and another carry.
 template <int DK, int DV>
 __global__ __launch_bounds__(4 * (DK + DV), DK == DV ? 4 : 3) void la_back_kernel(LaBackArgs a) {
   constexpr int KB = DK * 2, VB = DV * 2, NA = DK / 16, WV = DV / 16, WK = DK / 16, THREADS = 4 * (DK + DV);
