@@ -332,6 +332,24 @@ def test_linear_attention_packed(gpu, dtype, lens, tail, H, Hk, dk, dv, state):
         _check_sequence(dtype, 0.3, q[0, r], k[0, r], v[0, r], g, S0[n] if state else None, do[0, r], dS[n], got)
 
 
+# Many heads make segments of several chunks: of the 256 CUs each has few of a head's.
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("B,S,H,Hk,dk,dv", [(1, 1500, 128, 64, 128, 128), (2, 2049, 64, 64, 64, 64), (1, 777, 96, 96, 64, 128),
+                                            (1, 1100, 64, 16, 128, 64)])
+def test_linear_attention_of_many_heads(gpu, dtype, B, S, H, Hk, dk, dv):
+    print(f"many heads {dtype} B={B} S={S} H={H} Hk={Hk} dk={dk} dv={dv}", flush=True)
+    test_linear_attention(gpu, dtype, B, S, H, Hk, dk, dv, True)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("lens,tail,H,Hk,dk,dv", [
+    ([700, 0, 1, 640, 65, 2], 9, 128, 128, 128, 128),                    # few sequences, and the rule for
+    ([3, 900, 1, 128, 0, 257] + [31] * 20 + [384], 0, 96, 48, 64, 64),   # more of them than the CUs need
+])
+def test_linear_attention_packed_of_many_heads(gpu, dtype, lens, tail, H, Hk, dk, dv):
+    test_linear_attention_packed(gpu, dtype, lens, tail, H, Hk, dk, dv, True)
+
+
 def test_linear_attention_offsets_out_of_order(gpu):
     """Offsets past the row or out of order are brought in: each sequence what lies between the largest offset so far and the
     next, within the row; the rest zeros."""
@@ -590,12 +608,14 @@ def test_autocast(gpu):
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("bad", [float("nan"), float("inf")])
-@pytest.mark.parametrize("dk,dv", [(64, 64), (128, 128), (64, 128)])
-def test_nothing_reaches_back(gpu, dtype, bad, dk, dv):
+@pytest.mark.parametrize("dk,dv,S,H,Hk,places", [
+    (64, 64, 200, 4, 2, (0, 15, 16, 77, 100, 127, 128, 199)), (128, 128, 200, 4, 2, (0, 15, 16, 77, 100, 127, 128, 199)),
+    (64, 128, 200, 4, 2, (0, 15, 16, 77, 100, 127, 128, 199)), (128, 128, 700, 128, 64, (1, 130, 463)),
+    (64, 64, 700, 128, 128, (77, 300))])   # many heads: segments of several chunks
+def test_nothing_reaches_back(gpu, dtype, bad, dk, dv, S, H, Hk, places):
     """A NaN or infinity at a token changes no bit of what earlier tokens give, in its own chunk neither, and in the gradients of
     no later one; a value's stays in its column."""
     from q38.hip import autograd
-    S, H, Hk = 200, 4, 2
     q, k, v, g, S0, do, _ = _mix_inputs(gpu, 1, S, H, Hk, dk, dv, dtype)
 
     def run(q, k, v, do):
@@ -604,7 +624,7 @@ def test_nothing_reaches_back(gpu, dtype, bad, dk, dv):
         return (out.detach(), last.detach(), *torch.autograd.grad(out, leaves, do))
 
     clean = run(q, k, v, do)
-    for at in (0, 15, 16, 77, 100, 127, 128, 199):
+    for at in places:
         for i, name in enumerate("qkv"):
             ins = [t.clone() for t in (q, k, v)]
             ins[i][0, at, -1, 3] = bad  # of the last head
