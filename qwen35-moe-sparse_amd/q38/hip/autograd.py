@@ -28,6 +28,8 @@ whose padded path then runs its bmm in bf16) are cast to bf16 by differentiable 
 the output comes back in hidden_states' dtype, so their gradients arrive in their own dtype. Indices
 are int32/int64 as in the forward.
 """
+import functools
+
 import torch
 from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
@@ -296,22 +298,33 @@ def combine(rows, topk_w, plan):
     return ops.collect_rows(rows, plan, topk_w)
 
 
+def _once(backward):
+    """once_differentiable, whose own work is only done where a graph of the gradients is asked for."""
+    refused = once_differentiable(backward)
+
+    @functools.wraps(backward)
+    def run(ctx, *grads):
+        return refused(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+    return run
+
+
 class HipQkNormRope(torch.autograd.Function):
     """Kept are the operands alone: the backward pass makes the norms and the turns again (q38moe_qk_norm_rope, _backward)."""
 
     @staticmethod
     def forward(ctx, q, k, q_norm, k_norm, positions, inv_freq, axes, eps, unit_offset):
         ctx.save_for_backward(q, k, q_norm, k_norm, positions, inv_freq, axes)
-        ctx.rest = eps, unit_offset
-        return ops.qk_norm_rope(q, k, q_norm, k_norm, positions, inv_freq, axes, eps, unit_offset)
+        *out, made = ops._qk_norm_rope(q, k, q_norm, k_norm, positions, inv_freq, axes, eps, unit_offset)
+        ctx.rest = eps, unit_offset, made
+        return tuple(out)
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, d_q_out, d_k_out):
         # The gradients have the outputs' types, shapes and device: autograd sees to that, and the forward has looked at the rest.
-        saved, needs = ctx.saved_tensors, ctx.needs_input_grad
-        dq, dk, dwq, dwk = ops._qk_norm_rope_backward(d_q_out.contiguous(), d_k_out.contiguous(), *saved, *ctx.rest, needs[2:4],
-                                                      saved[0].device)
+        saved, needs, (eps, unit_offset, made) = ctx.saved_tensors, ctx.needs_input_grad, ctx.rest
+        dq, dk, dwq, dwk = ops._qk_norm_rope_backward(d_q_out.contiguous(), d_k_out.contiguous(), *saved, eps, unit_offset,
+                                                      needs[2:4], saved[0].device, made)
         return dq if needs[0] else None, dk if needs[1] else None, dwq, dwk, None, None, None, None, None
 
 
@@ -341,22 +354,23 @@ class HipLinearAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, log_decay, scale, initial_state, cu_seqlens, return_state):
         ctx.set_materialize_grads(False)
-        out, state, saved = ops.linear_attention(q, k, v, log_decay, scale, initial_state, cu_seqlens, return_state, save=True)
+        out, state, saved, made = ops._linear_attention(q, k, v, log_decay, scale, initial_state, cu_seqlens, return_state, True)
         ctx.save_for_backward(q, k, v, log_decay, initial_state, cu_seqlens, saved)
-        ctx.scale = scale
+        ctx.rest = scale, made
         return out, state
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, d_out, d_state):
         q, k, v, g, S0, cu, saved = ctx.saved_tensors
         needs = ctx.needs_input_grad
         if (d_out is None and d_state is None) or not any(needs):
             return (None,) * 8
+        scale, made = ctx.rest
         d_out = (torch.zeros(*q.shape[:3], v.shape[3], dtype=q.dtype, device=q.device) if d_out is None
                  else d_out.contiguous())
         dq, dk, dv, ds = ops._linear_attention_backward(d_out, None if d_state is None else d_state.contiguous(), q, k, v, g,
-                                                        ctx.scale, S0, cu, needs[5], saved, q.device)
+                                                        scale, S0, cu, needs[5], saved, q.device, made)
         return (dq if needs[0] else None, dk if needs[1] else None, dv if needs[2] else None, None, None, ds, None, None)
 
 

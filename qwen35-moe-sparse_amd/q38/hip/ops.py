@@ -1207,6 +1207,11 @@ def _rows_stride(shape, stride, size):
     return row, head
 
 
+def _empty_like(t):
+    """torch.empty of t's shape, type and device, contiguous; sooner where t is."""
+    return torch.empty_like(t) if t.is_contiguous() else torch.empty(t.shape, dtype=t.dtype, device=t.device)
+
+
 def _dense(t):
     """A copy of t that the kernels take."""
     t = t.contiguous()
@@ -1305,15 +1310,21 @@ def _rope_check(q, k, q_norm, k_norm, positions, inv_freq, axes):
 def qk_norm_rope(q, k, q_norm, k_norm, positions, inv_freq, axes=None, eps=1e-6, unit_offset=True):
     """RMS norm of every query and key head and rotation by position in one pass (q38moe_qk_norm_rope): see
     ``autograd.qk_norm_rope``. Returns contiguous (q [..., H, d], k [..., KV, d])."""
+    return _qk_norm_rope(q, k, q_norm, k_norm, positions, inv_freq, axes, eps, unit_offset)[:2]
+
+
+def _qk_norm_rope(q, k, q_norm, k_norm, positions, inv_freq, axes, eps, unit_offset):
+    """qk_norm_rope, and what a backward pass of the same operands need not look at again (None where one had to be copied)."""
     dev = _rope_check(q, k, q_norm, k_norm, positions, inv_freq, axes)
+    given = q, k, q_norm, k_norm
     q_norm, k_norm = _norm_weight(q_norm), _norm_weight(k_norm)
     q, k, sizes, head = _rope_operands(q, k, q_norm, k_norm, positions, inv_freq, axes, unit_offset)
-    dt = q.dtype
-    qo, ko = torch.empty(q.shape, dtype=dt, device=dev), torch.empty(k.shape, dtype=dt, device=dev)
+    qo, ko = _empty_like(q), _empty_like(k)
     with _on(dev):
-        check(lib.q38moe_qk_norm_rope(*head, qo.data_ptr(), ko.data_ptr(), *sizes, eps, _DTYPES[dt],
+        check(lib.q38moe_qk_norm_rope(*head, qo.data_ptr(), ko.data_ptr(), *sizes, eps, _DTYPES[q.dtype],
                                       _raw_stream(dev.index)), "q38moe_qk_norm_rope")
-    return qo, ko
+    as_given = q is given[0] and k is given[1] and q_norm is given[2] and k_norm is given[3]
+    return qo, ko, (q.stride(), k.stride(), sizes, head) if as_given else None
 
 
 @functools.lru_cache(maxsize=512)
@@ -1337,16 +1348,27 @@ def qk_norm_rope_backward(d_q_out, d_k_out, q, k, q_norm, k_norm, positions, inv
                                   dev)
 
 
-def _qk_norm_rope_backward(d_q_out, d_k_out, q, k, q_norm, k_norm, positions, inv_freq, axes, eps, unit_offset, need_norms, dev):
-    """qk_norm_rope_backward of operands that have been looked at."""
-    q_norm, k_norm = _norm_weight(q_norm), _norm_weight(k_norm)
-    q, k, sizes, head = _rope_operands(q, k, q_norm, k_norm, positions, inv_freq, axes, unit_offset)
+def _at(t):
+    return None if t is None else t.data_ptr()
+
+
+def _qk_norm_rope_backward(d_q_out, d_k_out, q, k, q_norm, k_norm, positions, inv_freq, axes, eps, unit_offset, need_norms, dev,
+                           made=None):
+    """qk_norm_rope_backward of operands that have been looked at; made: by _qk_norm_rope, for them if they lie where they lay. (The
+    backward pass runs in a thread of its own, where every object that the forward pass has touched too is slow to reach.)"""
+    if made is not None:
+        q_stride, k_stride, sizes, head = made
+        (pq, pk, _, pwq, pwk, _, p_pos, _, p_axes, _, p_freq) = head
+    if made is None or not (q.data_ptr() == pq and k.data_ptr() == pk and _at(q_norm) == pwq and _at(k_norm) == pwk
+                            and positions.data_ptr() == p_pos and _at(axes) == p_axes and inv_freq.data_ptr() == p_freq
+                            and q.stride() == q_stride and k.stride() == k_stride):
+        q_norm, k_norm = _norm_weight(q_norm), _norm_weight(k_norm)
+        q, k, sizes, head = _rope_operands(q, k, q_norm, k_norm, positions, inv_freq, axes, unit_offset)
     pdq, pdk = d_q_out.data_ptr(), d_k_out.data_ptr()
     if (pdq | pdk) & 15:
         d_q_out, d_k_out = _dense(d_q_out), _dense(d_k_out)
         pdq, pdk = d_q_out.data_ptr(), d_k_out.data_ptr()
-    dt = q.dtype
-    dq, dk = torch.empty(q.shape, dtype=dt, device=dev), torch.empty(k.shape, dtype=dt, device=dev)
+    dq, dk = torch.empty_like(d_q_out), torch.empty_like(d_k_out)
     dwq = torch.empty_like(q_norm) if q_norm is not None and need_norms[0] else None
     dwk = torch.empty_like(k_norm) if k_norm is not None and need_norms[1] else None
     with _on(dev):
@@ -1357,7 +1379,7 @@ def _qk_norm_rope_backward(d_q_out, d_k_out, q, k, q_norm, k_norm, positions, in
         check(lib.q38moe_qk_norm_rope_backward(pdq, pdk, *head, dq.data_ptr(), dk.data_ptr(),
                                                None if dwq is None else dwq.data_ptr(),
                                                None if dwk is None else dwk.data_ptr(), *sizes, eps,
-                                               None if ws is None else ws.data_ptr(), n, _DTYPES[dt],
+                                               None if ws is None else ws.data_ptr(), n, _DTYPES[d_q_out.dtype],
                                                _raw_stream(dev.index)), "q38moe_qk_norm_rope_backward")
     return dq, dk, dwq, dwk
 
@@ -1449,21 +1471,25 @@ def linear_attention(q, k, v, log_decay, scale=None, initial_state=None, cu_seql
     """Linear attention with a decay for each head (q38moe_linear_attention_forward): see ``autograd.linear_attention``.
     Returns (out [B,S,H,dv], final state [N,H,dk,dv] fp32 or None), and with save what ``linear_attention_backward`` of the
     same operands takes as ``saved``."""
+    return _linear_attention(q, k, v, log_decay, scale, initial_state, cu_seqlens, return_state, save)[:2 + save]
+
+
+def _linear_attention(q, k, v, log_decay, scale, initial_state, cu_seqlens, return_state, save):
+    """(out, state, saved, what a backward pass of the same operands need not look at again, None where one had to be copied)."""
     dev = _mix_check(q, k, v, log_decay, initial_state, cu_seqlens)
-    B = q.shape[0]
-    shape, (n, states), _, args, _alive = _mix_operands(q, k, v, log_decay, scale, initial_state, cu_seqlens)
+    shape, (n, states), backwards, args, used = _mix_operands(q, k, v, log_decay, scale, initial_state, cu_seqlens)
     N, S, H, _, dk, dv = shape
-    dt = q.dtype
-    out = torch.empty((B, S, H, dv), dtype=dt, device=dev)
+    out = _empty_like(q) if dk == dv else torch.empty((*q.shape[:3], dv), dtype=q.dtype, device=dev)
     state = torch.empty((N, H, dk, dv), dtype=torch.float32, device=dev) if return_state else None
     saved = torch.empty(states, dtype=torch.uint8, device=dev) if save and states else None
     with _on(dev):
         ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
         check(lib.q38moe_linear_attention_forward(*args, out.data_ptr(), None if state is None else state.data_ptr(),
                                                   None if saved is None else saved.data_ptr(), states, *shape,
-                                                  None if ws is None else ws.data_ptr(), n, _DTYPES[dt],
+                                                  None if ws is None else ws.data_ptr(), n, _DTYPES[q.dtype],
                                                   _raw_stream(dev.index)), "q38moe_linear_attention_forward")
-    return (out, state, saved) if save else (out, state)
+    as_given = used[0] is q and used[1] is k and used[2] is v
+    return out, state, saved, (q.stride(), k.stride(), v.stride(), shape, backwards, args) if as_given else None
 
 
 def linear_attention_backward(d_out, d_final_state, q, k, v, log_decay, scale=None, initial_state=None, cu_seqlens=None,
@@ -1484,17 +1510,21 @@ def linear_attention_backward(d_out, d_final_state, q, k, v, log_decay, scale=No
                                       dev)
 
 
-def _linear_attention_backward(d_out, d_final_state, q, k, v, log_decay, scale, initial_state, cu_seqlens, need_state, saved, dev):
-    """linear_attention_backward of operands that have been looked at."""
-    B = q.shape[0]
-    shape, _, (n, states), args, _alive = _mix_operands(q, k, v, log_decay, scale, initial_state, cu_seqlens)
-    N, S, H, Hk, dk, dv = shape
-    dt = q.dtype
+def _linear_attention_backward(d_out, d_final_state, q, k, v, log_decay, scale, initial_state, cu_seqlens, need_state, saved, dev,
+                               made=None):
+    """linear_attention_backward of operands that have been looked at; made: by _linear_attention, for them if they lie where they
+    lay (see _qk_norm_rope_backward)."""
+    if made is not None:
+        q_stride, k_stride, v_stride, shape, (n, states), args = made
+        pq, pk, pv, _, p_g, _, p_S0, p_cu = args
+    if made is None or not (q.data_ptr() == pq and k.data_ptr() == pk and v.data_ptr() == pv and log_decay.data_ptr() == p_g
+                            and _at(initial_state) == p_S0 and _at(cu_seqlens) == p_cu and q.stride() == q_stride
+                            and k.stride() == k_stride and v.stride() == v_stride):
+        shape, _, (n, states), args, _alive = _mix_operands(q, k, v, log_decay, scale, initial_state, cu_seqlens)
+    N, _, H, _, dk, dv = shape
     if d_out.data_ptr() & 15:
         d_out = d_out.clone()
-    dq = torch.empty((B, S, H, dk), dtype=dt, device=dev)
-    dk_ = torch.empty((B, S, Hk, dk), dtype=dt, device=dev)
-    dv_ = torch.empty((B, S, Hk, dv), dtype=dt, device=dev)
+    dq, dk_, dv_ = _empty_like(q), _empty_like(k), _empty_like(v)
     ds = torch.empty((N, H, dk, dv), dtype=torch.float32, device=dev) if need_state else None
     with _on(dev):
         ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
@@ -1502,7 +1532,7 @@ def _linear_attention_backward(d_out, d_final_state, q, k, v, log_decay, scale, 
                                                    None if d_final_state is None else d_final_state.data_ptr(), *args,
                                                    None if saved is None else saved.data_ptr(), states, dq.data_ptr(),
                                                    dk_.data_ptr(), dv_.data_ptr(), None if ds is None else ds.data_ptr(), *shape,
-                                                   None if ws is None else ws.data_ptr(), n, _DTYPES[dt],
+                                                   None if ws is None else ws.data_ptr(), n, _DTYPES[q.dtype],
                                                    _raw_stream(dev.index)), "q38moe_linear_attention_backward")
     return dq, dk_, dv_, ds
 

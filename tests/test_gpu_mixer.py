@@ -7,8 +7,8 @@ sum of d: 3 (d + 40) u of the sizes of their terms. An angle in 64 bits is itsel
 these references, and in the kernel position * inv_freq, times 1 / 2 pi and that constant's own rounding. Four together make
 1e-11 at a position of 10^4 and 5e-4 at 2^40, where it is most of a bf16 rounding.
 
-Linear attention: within a chunk of 64 tokens a bf16 call rounds the weighted scores once (v of each) and the state that
-queries read once (v of each element), then the result (v). The fp32 sums have dk, 64 and, through the state, all earlier
+Linear attention: within a chunk of 64 tokens a bf16 call keeps the weighted scores in two parts (v^2 of each; v is counted) and
+rounds the state that queries read once (v of each element), then the result (v). The fp32 sums have dk, 64 and, through the state, all earlier
 tokens as terms: 2 (dk + 64 + n + 20) u of the sum of all terms' sizes, n the number of chunks (within a chunk 64 terms more; decays
 are rounded once a chunk). States are not rounded to bf16 at all. The gradients are the same sums with the roles exchanged."""
 import math
@@ -588,6 +588,50 @@ def test_two_streams(gpu):
     for i in range(2):
         for one in got[i]:
             assert all(torch.equal(a, b) for a, b in zip(one, want[i]))
+
+
+def test_gradients_are_taken_once(gpu):
+    """With create_graph the gradients are the same bits and have no gradient themselves; forward-mode tangents are refused."""
+    from q38.hip import autograd
+    q, k, v, g, _, do, _ = _mix_inputs(gpu, 1, 70, 2, 2, 64, 64, torch.float32, state=False)
+    pos, inv = torch.arange(70, device=gpu)[None], torch.rand(8, device=gpu)
+    for call in (lambda q, k: autograd.qk_norm_rope(q, k, None, None, pos, inv)[0],
+                 lambda q, k: autograd.linear_attention(q, k, v, g)[0]):
+        leaves = [t.clone().requires_grad_(True) for t in (q, k)]
+        once = torch.autograd.grad(call(*leaves), leaves, do)
+        twice = torch.autograd.grad(call(*leaves), leaves, do, create_graph=True)
+        assert all(torch.equal(a, b) for a, b in zip(once, twice))
+        with pytest.raises(RuntimeError):  # no graph of them
+            torch.autograd.grad(twice[0].sum(), leaves, allow_unused=True)
+        with torch.autograd.forward_ad.dual_level(), pytest.raises(RuntimeError):
+            call(torch.autograd.forward_ad.make_dual(q, torch.ones_like(q)), k)
+
+
+def test_saved_tensors_that_were_moved(gpu):
+    """Under hooks that keep saved tensors elsewhere (other places and strides in the backward pass): the same bits."""
+    from q38.hip import autograd
+    g = torch.Generator(device=gpu).manual_seed(9)
+    fused = _randn(g, 2, 100, 4 + 2 + 2, 64, dtype=torch.bfloat16)
+    w = _randn(g, 2, 64, dtype=torch.bfloat16)
+    pos, inv = torch.arange(100, device=gpu).repeat(2, 1), torch.rand(8, generator=g, device=gpu)
+    decay = -torch.rand(4, generator=g, device=gpu)
+
+    def run():
+        x = fused.clone().requires_grad_(True)
+        wq, wk = (t.clone().requires_grad_(True) for t in w)
+        q, k = autograd.qk_norm_rope(x[..., :4, :], x[..., 4:6, :], wq, wk, pos, inv)
+        out, _ = autograd.linear_attention(q, k, x[..., 6:, :], decay)
+        return out, lambda: torch.autograd.grad(out, (x, wq, wk), torch.ones_like(out))
+
+    want, grads = run()
+    want = want, *grads()
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: (t.device, t.cpu()), lambda kept: kept[1].to(kept[0])):
+        got, grads = run()
+        junk = [_randn(g, 2, 100, n, 64, dtype=torch.bfloat16) for n in (2, 4, 8)]
+        got = got, *grads()
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+    del junk
 
 
 def test_autocast(gpu):
