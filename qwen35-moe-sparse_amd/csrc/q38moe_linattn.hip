@@ -12,10 +12,11 @@
 // to the state, la_carry_kernel runs over the segments, la_kernel<OUT = true> goes through the chunks of each with the state
 // in its accumulators.
 //
-// bf16 roundings: the state that queries read, once, as an operand of the matrix units (16384 values' errors, which average out).
-// The weighted scores are split into two bf16 parts (16 bits): where a call has few of them, their errors would not, and all of an
-// output row shares its score's (a token alone was 0.0027 off, 0.0017 now, the rounding of the result; 1 to 2 % in time). What goes
-// into the state itself is split into three parts (24 bits), so that the state is as exact as in fp32.
+// bf16 roundings: the weighted scores and the state that queries read are operands of the matrix units in two bf16 parts (16
+// bits: off by 2^-16 of themselves at most, where rounding a result leaves 2^-8 of that): a result is as near to exact as its own
+// rounding. With the state in one part it was 0.0021 off (norm of the error over the result's), so 0.0017, for 4 x 4096 tokens x 16
+// heads of 128 forward and back in 346 us, not 331. What goes into the state itself is split into three parts (24 bits), so that
+// the state is as exact as in fp32.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -224,6 +225,19 @@ __device__ __forceinline__ u32x4_t la_pack(f32x4_t x, f32x4_t y) {
   return u32x4_t{pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3])};
 }
 
+// What la_pack(x, y) left, rounded. An infinity leaves a NaN.
+__device__ __forceinline__ u32x4_t la_left(f32x4_t x, f32x4_t y, u32x4_t packed) {
+#pragma unroll
+  for (int z = 0; z < 4; ++z) {
+    float x0, x1;
+    unpack_bf16x2(packed[z], x0, x1);
+    f32x4_t& of = z < 2 ? x : y;
+    of[2 * (z & 1)] -= x0;
+    of[2 * (z & 1) + 1] -= x1;
+  }
+  return la_pack(x, y);
+}
+
 // x, but not as the compiler knows it: what follows from it is made again in every chunk rather than kept in registers that
 // the loop lacks.
 __device__ __forceinline__ int afresh(int x) {
@@ -269,12 +283,21 @@ __device__ __forceinline__ void la_scores(const uint8_t* keys, const uint8_t* qu
     P[0] = mfma16x16x32(key(x), q, P[0]);
     if (2 * u + 1 <= t) P[1] = mfma16x16x32(key(x + 16 * BYTES), q, P[1]);
   }
+  float decay[2][4];
+#pragma unroll
+  for (int k = 0; k < 2; ++k)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) decay[k][e] = tab[max(16 * (t - 2 * u - k) + lr - 4 * lq - e, 0)].x;
+#pragma unroll
+  for (int k = 0; k < 2; ++k)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) asm volatile("" : "+v"(decay[k][e]));  // all at once, none behind a branch on its place
 #pragma unroll
   for (int k = 0; k < 2; ++k)
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const int n = 16 * (t - 2 * u - k) + lr - 4 * lq - e;  // tokens between key and query
-      P[k][e] = n >= 0 ? P[k][e] * (intra * tab[max(n, 0)].x) : 0.0f;
+      P[k][e] = n >= 0 ? P[k][e] * (intra * decay[k][e]) : 0.0f;
     }
   const u32x4_t high = la_pack(P[0], P[1]);
 #pragma unroll
@@ -370,6 +393,11 @@ __device__ __forceinline__ bool la_any_infinite(const f32x4_t (&v)[4]) {
 }
 __device__ __forceinline__ bool la_infinite(float x) { return !(fabsf(x) <= 3.402823466e38f); }
 
+// x of that lane of the wave (__shfl would keep the lane's own number in a register all through the loop).
+__device__ __forceinline__ uint32_t la_lane(uint32_t x, int lane) {
+  return (uint32_t)__builtin_amdgcn_ds_bpermute(4 * lane, (int)x);
+}
+
 // o[t] += the terms of values that are not finite. value(n, c): token n's value of column c of the wave's 16, where the lane at
 // 16 ((n / 4) % 4) + c holds it; score(t, n): that of token n for query 16 t + lr.
 template <class Value, class Score>
@@ -402,7 +430,7 @@ __device__ __forceinline__ void la_weigh_infinite(f32x4_t (&o)[4], u32x4_t (&v)[
       [&](int n, int c) {
         const int z = 2 * ((n >> 4) & 1) + ((n >> 1) & 1);
         const u32x4_t x = n < 32 ? u32x4_t(v[0]) : u32x4_t(v[1]);
-        const uint32_t word = __shfl(z == 0 ? x[0] : z == 1 ? x[1] : z == 2 ? x[2] : x[3], 16 * ((n >> 2) & 3) + c);
+        const uint32_t word = la_lane(z == 0 ? x[0] : z == 1 ? x[1] : z == 2 ? x[2] : x[3], 16 * ((n >> 2) & 3) + c);
         return __uint_as_float(n & 1 ? word & 0xffff0000u : word << 16);
       },
       [&](int t, int n) {
@@ -440,7 +468,7 @@ __device__ __forceinline__ void la_weigh_infinite(f32x4_t (&o)[4], f32x4_t (&v)[
         for (int t = 0; t < 4; ++t)
 #pragma unroll
           for (int e = 0; e < 4; ++e) word |= n >> 4 == t && (n & 3) == e ? __float_as_uint(v[t][e]) : 0u;
-        return __uint_as_float(__shfl(word, 16 * ((n >> 2) & 3) + c));
+        return __uint_as_float(la_lane(word, 16 * ((n >> 2) & 3) + c));
       },
       [&](int t, int n) {
         const int k = n >> 4, unit = t == 3 ? k >> 1 : t == 2 ? 2 + 3 * (k >> 1) : 4 - t, lane = 16 * ((n >> 2) & 3) + lr;
@@ -524,12 +552,14 @@ __global__ __launch_bounds__(4 * DV, la_waves(BF16, DK, DV, OUT)) void la_kernel
   start(kst, a.k, begin);
   start(vst, a.v, begin);
   if (OUT) start(qst, a.q, begin);
-  auto fetch = [&](int rows, uint8_t* queries) {
+  auto fetch = [&](int rows) {
     const int tid = afresh((int)threadIdx.x);
-    if (OUT && COPY) qst.copy(tid, queries, rows, a.dk * ES);  // first: done when the others are
     if (OUT && !COPY) qst.load(tid, rows, a.dk * ES);
     kst.load(tid, rows, a.dk * ES);
     vst.load(tid, rows, a.dv * ES);
+  };
+  auto copy = [&](int rows, uint8_t* queries) {
+    if (OUT && COPY) qst.copy(afresh((int)threadIdx.x), queries, rows, a.dk * ES);
   };
   const double g = (double)a.g[h];
   // Rows la_row(i, lq) .. + 3, column 16 w + lr.
@@ -559,7 +589,10 @@ __global__ __launch_bounds__(4 * DV, la_waves(BF16, DK, DV, OUT)) void la_kernel
   }
   // The first tiles are on their way while the decays are made (before the state, which is waited for first: 2048 tokens x 16
   // heads of 128 take 42.4 us, so 40.2).
-  if (begin < end) fetch(min(LA_C, end - begin), Qs[0]);
+  if (begin < end) {
+    copy(min(LA_C, end - begin), Qs[0]);
+    fetch(min(LA_C, end - begin));
+  }
   la_tables(tab, put, g, a.gain, a.lag, tid);
   auto stage = [&]() {
     const int tid = afresh((int)threadIdx.x);
@@ -573,7 +606,7 @@ __global__ __launch_bounds__(4 * DV, la_waves(BF16, DK, DV, OUT)) void la_kernel
     const int rows = min(LA_C, end - j0);
     const bool more = j0 + LA_C < end;
     __syncthreads();
-    if (more) fetch(min(LA_C, end - j0 - LA_C), Qs[COPY ? par ^ 1 : 0]);
+    if (more) fetch(min(LA_C, end - j0 - LA_C));
     const uint8_t* const Q = Qs[COPY ? par : 0];
     const int lane = afresh(tid & 63), lr = lane & 15, lq = lane >> 4;
     using KeyTile = LaTile<BF16, KB>;
@@ -616,13 +649,13 @@ __global__ __launch_bounds__(4 * DV, la_waves(BF16, DK, DV, OUT)) void la_kernel
       for (int t = 0; t < 4; ++t) o[t] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
       for (int s = 0; s < KB / 64; ++s) {
-        u32x4_t x;
-        if constexpr (BF16) x = la_pack(S[2 * s], S[2 * s + 1]);
+        u32x4_t x, left;
+        if constexpr (BF16) x = la_pack(S[2 * s], S[2 * s + 1]), left = la_left(S[2 * s], S[2 * s + 1], x);
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
           const u32x4_t y = *reinterpret_cast<const u32x4_t*>(Q + (row_at ^ (64 * (s & 3))) + 256 * (s >> 2) + 16 * KB * t);
           if constexpr (BF16) {
-            o[t] = mfma16x16x32(x, y, o[t]);
+            o[t] = mfma16x16x32(left, y, mfma16x16x32(x, y, o[t]));
           } else {
             const f32x4_t yf = __builtin_bit_cast(f32x4_t, y);
 #pragma unroll
@@ -632,6 +665,8 @@ __global__ __launch_bounds__(4 * DV, la_waves(BF16, DK, DV, OUT)) void la_kernel
       }
 #pragma unroll
       for (int t = 0; t < 4; ++t) o[t] = o[t] * (a.inter * tab[16 * t + lr + 1 - a.lag].x);
+      // Behind this chunk's reads of queries: a read of either tile waits for copies under way.
+      if (more) copy(min(LA_C, end - j0 - LA_C), Qs[COPY ? par ^ 1 : 0]);
     }
     // The wave's columns of the values: bf16 as operands, tokens 32 u + {4 lq .., 16 + 4 lq ..}; fp32 tokens 16 t + 4 lq .. .
     u32x4_t v[2];
@@ -713,14 +748,14 @@ __global__ __launch_bounds__(4 * DV, la_waves(BF16, DK, DV, OUT)) void la_kernel
 // dk and dv of one segment of one head together, bf16, backwards in time with T = the gradient of the state [dk, dv]:
 //   dv_j = scale sum_{i >= j} e^{g (i - j)} (k_j . q_i) dO_i + e^{g j'} T^T k_j     (j' tokens from the chunk's start, backwards)
 //   dk_j = scale sum_{i >= j} e^{g (i - j)} (v_j . dO_i) q_i + e^{g j'} T v_j
-// DV / 16 waves make dv and hold T as la_kernel's hold S; DK / 16 more make dk and read T, rounded, from LDS, where the first
-// ones leave it once a chunk. One pass over q, k, v and dO instead of two over three of them each, and T made once:
+// DV / 16 waves make dv and hold T as la_kernel's hold S; DK / 16 more make dk and read T, in two bf16 parts, from LDS, where the
+// first ones leave it once a chunk. One pass over q, k, v and dO instead of two over three of them each, and T made once:
 // 4 x 4096 tokens x 16 heads of 128 (MI355X) take 110 us (419 MB, 3.8 TB/s), two passes of la_kernel 2 x 68 and another carry.
 template <int DK, int DV>
 __global__ __launch_bounds__(4 * (DK + DV), DK == DV ? 4 : 3) void la_back_kernel(LaBackArgs a) {
   constexpr int KB = DK * 2, VB = DV * 2, NA = DK / 16, WV = DV / 16, WK = DK / 16, THREADS = 4 * (DK + DV);
   __shared__ __attribute__((aligned(16))) uint8_t Qs[LA_C * KB], Ks[LA_C * KB], Vs[LA_C * VB], Ds[LA_C * VB];
-  __shared__ __attribute__((aligned(16))) uint8_t Ts[DV * KB];
+  __shared__ __attribute__((aligned(16))) uint8_t Ts[2][DV * KB];
   __shared__ __attribute__((aligned(16))) uint8_t Ps[2][2 * LA_SCORES];
   __shared__ float2 tab[LA_C + 1];
   __shared__ float put[2 * LA_C];
@@ -796,12 +831,15 @@ __global__ __launch_bounds__(4 * (DK + DV), DK == DV ? 4 : 3) void la_back_kerne
     }
   }
   la_tables(tab, put, g, a.s.gain, 1, tid);
-  // Ts is [dv][dk]; rows 8 apart, which its transposing reads take together, are mixed as those 4 apart of other tiles are.
+  // Ts is [dv][dk], two parts; rows 8 apart, which its transposing reads take together, are mixed as those 4 apart of other tiles are.
   auto state = [&](int row, int col) { return row * KB + ((col ^ KeyTile::key((row & 3) | ((row >> 1) & 4))) << 4); };
   auto publish = [&](int lr, int lq) {
 #pragma unroll
-    for (int u = 0; u < NA / 2; ++u)
-      *reinterpret_cast<u32x4_t*>(Ts + state(16 * wc + lr, 4 * u + lq)) = la_pack(T[2 * u], T[2 * u + 1]);
+    for (int u = 0; u < NA / 2; ++u) {
+      const u32x4_t x = la_pack(T[2 * u], T[2 * u + 1]);
+      *reinterpret_cast<u32x4_t*>(Ts[0] + state(16 * wc + lr, 4 * u + lq)) = x;
+      *reinterpret_cast<u32x4_t*>(Ts[1] + state(16 * wc + lr, 4 * u + lq)) = la_left(T[2 * u], T[2 * u + 1], x);
+    }
   };
   if (begin < end) {
     stage();
@@ -825,10 +863,14 @@ __global__ __launch_bounds__(4 * (DK + DV), DK == DV ? 4 : 3) void la_back_kerne
         la_scores<KB, true>(Qs, Ks, Ps[0], unit, lr, lq, row_at, a.s.intra, tab);
 #pragma unroll
       for (int s = 0; s < KB / 64; ++s) {
-        const u32x4_t x = la_pack(T[2 * s], T[2 * s + 1]);
+        // T as the wave itself published it: reads cost less than making it again.
+        const u32x4_t x = *reinterpret_cast<const u32x4_t*>(Ts[0] + state(16 * wc + lr, 4 * s + lq));
+        const u32x4_t left = *reinterpret_cast<const u32x4_t*>(Ts[1] + state(16 * wc + lr, 4 * s + lq));
 #pragma unroll
-        for (int t = 0; t < 4; ++t)
-          o[t] = mfma16x16x32(x, *reinterpret_cast<const u32x4_t*>(Ks + (row_at ^ (64 * s)) + 16 * KB * t), o[t]);
+        for (int t = 0; t < 4; ++t) {
+          const u32x4_t y = *reinterpret_cast<const u32x4_t*>(Ks + (row_at ^ (64 * s)) + 16 * KB * t);
+          o[t] = mfma16x16x32(left, y, mfma16x16x32(x, y, o[t]));
+        }
       }
 #pragma unroll
       for (int u = 0; u < 2; ++u) v[u] = la_column<VB>(Ds + value_at + 32 * VB * u);
@@ -845,11 +887,17 @@ __global__ __launch_bounds__(4 * (DK + DV), DK == DV ? 4 : 3) void la_back_kerne
         la_scores<VB, false>(Ds, Vs, Ps[1], unit, lr, lq, row_at, a.s.intra, tab);
 #pragma unroll
       for (int s = 0; s < VB / 64; ++s) {
-        const uint2 x = la_read_tr(Ts + state_at[0] + 32 * KB * s), y = la_read_tr(Ts + state_at[1] + 32 * KB * s);
+        u32x4_t x[2];
 #pragma unroll
-        for (int t = 0; t < 4; ++t)
-          o[t] = mfma16x16x32(u32x4_t{x.x, x.y, y.x, y.y},
-                              *reinterpret_cast<const u32x4_t*>(Vs + (row_at ^ (64 * s)) + 16 * VB * t), o[t]);
+        for (int part = 0; part < 2; ++part) {
+          const uint2 a = la_read_tr(Ts[part] + state_at[0] + 32 * KB * s), b = la_read_tr(Ts[part] + state_at[1] + 32 * KB * s);
+          x[part] = u32x4_t{a.x, a.y, b.x, b.y};
+        }
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          const u32x4_t y = *reinterpret_cast<const u32x4_t*>(Vs + (row_at ^ (64 * s)) + 16 * VB * t);
+          o[t] = mfma16x16x32(x[1], y, mfma16x16x32(x[0], y, o[t]));
+        }
       }
 #pragma unroll
       for (int u = 0; u < 2; ++u) v[u] = la_column<KB>(Qs + value_at + 32 * KB * u);

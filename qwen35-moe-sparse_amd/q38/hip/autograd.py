@@ -382,7 +382,7 @@ def linear_attention(q, k, v, log_decay, scale=None, initial_state=None, cu_seql
     from, and with return_state the states after the last tokens come back: (out [B,S,H,dv], state or None). N is B, or, with
     cu_seqlens (int32 [N+1] on the GPU, B = 1), the row holds N sequences one behind the other, n being the tokens
     cu_seqlens[n] to cu_seqlens[n+1]; tokens of no sequence come out zero, a sequence without tokens keeps its state. States are fp32
-    throughout; of the bf16 operands that it makes itself, the state as queries read it is rounded once. Gradients flow
+    throughout; bf16 operands that it makes itself, scores and the state as queries read it, keep 16 bits. Gradients flow
     to q, k, v and initial_state, not to log_decay. ``ops.linear_attention_step`` goes on one token at a time. A NaN or infinity
     reaches no earlier token's output; an infinity may come out of a state as a NaN. Under bf16 autocast q, k and v are cast to bf16."""
     if log_decay.requires_grad and torch.is_grad_enabled():

@@ -1,0 +1,77 @@
+"""How exact the token mixer is where its results are not: the roundings that test_gpu_mixer.py's bounds leave room for.
+
+bf16: the weighted scores and the state that queries read are operands in two bf16 parts. The first leaves at most v of a
+value (v = 2^-8, half a step), the second v of that: v^2 of every score and of every element of the state, beside the fp32 sums
+and v for the rounding of the result. An operand of one part is v off: most where a result is small beside its terms."""
+import pytest
+import torch
+
+import test_gpu_mixer as mixer
+from test_gpu_mixer import U, _sum64, _within
+
+V = 2.0 ** -8
+
+
+def _sharp(got, want, dtype, dk, name, group=1):
+    """mixer._check with v^2 of each score and element of the state in the place of v."""
+    out, rounded, terms = want
+    H, S, d = out.shape
+    v = torch.finfo(dtype).eps / 2
+    bound = 2 * (dk + 64 + S / 64 + 20 + group) * U * terms + (v * v * rounded * (1 + v) if dtype == torch.bfloat16 else 0)
+    out, bound = (t.view(H // group, group, S, d).sum(1).transpose(0, 1) for t in (out, bound))
+    _within(got, out, bound + v * (out.abs() + bound) + 1e-37, name)
+
+
+def _parts(x, n):
+    """x as the sum of n bf16 numbers."""
+    got = torch.zeros_like(x)
+    for _ in range(n):
+        got = got + (x - got).bfloat16().double()
+    return got
+
+
+def _emulated(q, k, v, g, S0, scale, of_scores, of_state):
+    """The chunked sums in float64 with operands of so many parts, rounded to bf16; [S,H,.] in, [S,H,dv] out."""
+    q, k, v = (t.double().transpose(0, 1) for t in (q, k, v))
+    g, state, outs = g.double()[:, None, None], S0.double(), []
+    for j0 in range(0, q.shape[1], 64):
+        a, b, c = (t[:, j0:j0 + 64] for t in (q, k, v))
+        n = a.shape[1]
+        at = torch.arange(n)
+        gap = at[:, None] - at[None, :]
+        s = a @ b.transpose(1, 2) * torch.where(gap >= 0, torch.exp(g * gap.clamp(min=0)), torch.zeros((), dtype=torch.float64))
+        outs.append(_parts(s * scale, of_scores) @ c + torch.exp(g * (at[:, None] + 1)) * scale * (a @ _parts(state, of_state)))
+        state = torch.exp(g * n) * state + (b * torch.exp(g * (n - 1 - at[:, None]))).transpose(1, 2) @ c
+    return torch.cat(outs, 1).transpose(0, 1).bfloat16()
+
+
+@pytest.mark.parametrize("dk,dv", [(8, 8), (64, 64), (128, 128)])
+def test_the_bound_sees_a_part_less(dk, dv):
+    """On the CPU: sums with operands of two parts are within the bound, with one part of either they are not."""
+    q, k, v, g, S0, _, _ = mixer._mix_inputs(torch.device("cpu"), 1, 200, 4, 4, dk, dv, torch.bfloat16)
+    scale = dk ** -0.5
+    want = _sum64(*(t[0].transpose(0, 1) for t in (q, k, v)), g, S0[0], scale, scale, 1.0, 0)[:3]
+    args = q[0], k[0], v[0], g, S0[0], scale
+    _sharp(_emulated(*args, 2, 2), want, torch.bfloat16, dk, "two parts")
+    for parts in ((1, 2), (2, 1)):
+        with pytest.raises(AssertionError, match="of the bound"):
+            _sharp(_emulated(*args, *parts), want, torch.bfloat16, dk, "one part")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,S,H,Hk,dk,dv,state", [
+    (2, 1, 2, 1, 64, 64, True), (1, 70, 4, 4, 8, 8, True), (2, 300, 4, 2, 64, 64, True), (1, 300, 4, 2, 64, 128, True),
+    (1, 300, 4, 2, 128, 64, True), (2, 300, 4, 4, 128, 128, True), (1, 640, 4, 1, 48, 80, False), (1, 1500, 128, 64, 128, 128, True),
+])
+def test_operands_in_two_parts(gpu, monkeypatch, B, S, H, Hk, dk, dv, state):
+    """Outputs and every gradient."""
+    monkeypatch.setattr(mixer, "_check", _sharp)
+    mixer.test_linear_attention(gpu, torch.bfloat16, B, S, H, Hk, dk, dv, state)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lens,tail,H,Hk,dk,dv", [([100, 600, 3, 64, 0, 200], 37, 4, 2, 64, 64),
+                                                  ([700, 0, 1, 640, 65, 2], 9, 128, 128, 128, 128)])
+def test_operands_in_two_parts_packed(gpu, monkeypatch, lens, tail, H, Hk, dk, dv):
+    monkeypatch.setattr(mixer, "_check", _sharp)
+    mixer.test_linear_attention_packed(gpu, torch.bfloat16, lens, tail, H, Hk, dk, dv, True)
