@@ -1031,7 +1031,9 @@ __global__ __launch_bounds__(256) void la_step_kernel(LaStepArgs a) {
     mine &= !__syncthreads_or(before);
   }
   if (mine) {
-    const float lam = (float)exp((double)a.g[h]);
+    // In two floats: one is off by up to 2^-25 of the state in the same direction at every token, which adds up (after 20000 tokens of
+    // g = -1e-5 3e-4, and below -3e-8 nothing would be forgotten at all).
+    const float2 lam = la_decay2((double)a.g[h], 1);
     f32x4_t v = {0.0f, 0.0f, 0.0f, 0.0f};
     if (there) {
 #pragma unroll
@@ -1045,7 +1047,7 @@ __global__ __launch_bounds__(256) void la_step_kernel(LaStepArgs a) {
       const float k = load1(a.k, r), q = load1(a.q, r);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        s[e] = fmaf(s[e], lam, k * v[e]);
+        s[e] = fmaf(s[e], lam.x, fmaf(s[e], lam.y, k * v[e]));
         o[e] = fmaf(s[e], q, o[e]);
       }
       *reinterpret_cast<f32x4_t*>(S + (int64_t)r * a.dv) = s;

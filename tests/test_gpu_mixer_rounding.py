@@ -75,3 +75,28 @@ def test_operands_in_two_parts(gpu, monkeypatch, B, S, H, Hk, dk, dv, state):
 def test_operands_in_two_parts_packed(gpu, monkeypatch, lens, tail, H, Hk, dk, dv):
     monkeypatch.setattr(mixer, "_check", _sharp)
     mixer.test_linear_attention_packed(gpu, torch.bfloat16, lens, tail, H, Hk, dk, dv, True)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_many_steps_of_a_slow_decay(gpu, dtype):
+    """20000 single tokens with decays next to 1, everything positive, against float64. A step rounds the state twice (u of it
+    each, one sign or the other: a walk of at most 2 u (n/3)^1/2 as a standard deviation, 5 of them make 6 u n^1/2). A decay in one float
+    is off the same way every time, which makes 25 u n^1/2 or more of each of these."""
+    from q38.hip import ops
+    n, d = 20000, 32
+    decay = torch.tensor([-1e-5, -3e-6, -1e-7, -2e-8], device=gpu)
+    r = torch.Generator(device=gpu).manual_seed(4)
+    q, k, v = (torch.randn(n, 4, d, generator=r, device=gpu).abs().to(dtype) for _ in range(3))
+    state = 1e4 * (0.5 + torch.rand(1, 4, d, d, generator=r, device=gpu))
+    exact = torch.exp(decay.double() * n)[:, None, None] * state[0].double()
+    left = torch.exp(decay.double()[:, None] * torch.arange(n - 1, -1, -1, device=gpu))[..., None]
+    exact += (k.double().transpose(0, 1) * left).transpose(1, 2).contiguous() @ v.double().transpose(0, 1).contiguous()
+    for t in range(n):
+        out = ops.linear_attention_step(q[t:t + 1], k[t:t + 1], v[t:t + 1], state, decay)
+    torch.cuda.synchronize()
+    bound = 6 * U * n ** 0.5
+    _within(state[0], exact, bound * exact, "state")
+    o = (q[-1].double()[:, None] @ exact)[:, 0] * d ** -0.5
+    half = torch.finfo(dtype).eps / 2
+    _within(out[0], o, (bound + (d + 12) * U + half) * (1 + half) * o, "out")
