@@ -100,3 +100,57 @@ def test_many_steps_of_a_slow_decay(gpu, dtype):
     o = (q[-1].double()[:, None] @ exact)[:, 0] * d ** -0.5
     half = torch.finfo(dtype).eps / 2
     _within(out[0], o, (bound + (d + 12) * U + half) * (1 + half) * o, "out")
+
+
+# ---- decays over many chunks and segments -------------------------------------------------------
+
+def _midway(tokens):
+    """A log_decay near -1e-5 whose e^{g tokens} lies next to the middle between two floats."""
+    g = (-1e-5 * (1 + 1e-4 * torch.arange(2000, dtype=torch.float64))).float().double()
+    x = torch.exp(g * tokens)
+    return float(g[(x - x.float().double()).abs().argmax()])
+
+
+def _decayed(S, g, tokens, times, low):
+    """S e^{g tokens times} with a rounding to fp32 each time, the decay in two floats or (not low) in one."""
+    x = torch.exp(torch.tensor(g, dtype=torch.float64) * tokens)
+    hi = x.float().double()
+    lo = (x - hi).float().double() if low else 0.0
+    for _ in range(times):
+        S = (S.double() * hi + (S.double() * lo).float().double()).float()
+    return S
+
+
+# A rounding (u of the state, either sign) each time: 5 standard deviations of the walk, u (n/3)^1/2, are 3 u n^1/2. What
+# test_decay_alone_over_many_chunks runs is rounded up to 260 times: by 256 segments and 4 chunks of the last, or by 256 chunks.
+DECAY_BOUND = 3 * U * 260 ** 0.5
+
+
+@pytest.mark.parametrize("tokens,times", [(64, 256), (256, 256), (512, 128)])
+def test_the_bound_sees_a_decay_in_one_float(tokens, times):
+    """On the CPU, for every length of segments that the next test runs and its number of them: what that allows is more than two
+    floats leave and less than one does."""
+    g, S = _midway(tokens), 1.0 + torch.rand(64, 64, generator=torch.Generator().manual_seed(1))
+    exact = S.double() * torch.exp(torch.tensor(g, dtype=torch.float64) * tokens * times)
+    off = [float(((_decayed(S, g, tokens, times, low).double() - exact) / exact).abs().max()) for low in (True, False)]
+    assert off[0] < 0.8 * DECAY_BOUND and DECAY_BOUND < 0.8 * off[1], (off[0] / U, off[1] / U, DECAY_BOUND / U)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("S,H,d", [(65536, 4, 64),                        # 256 segments of 256 tokens or 128 of 512
+                                   (16384, 1024, 8), (16384, 512, 128)])  # so many heads that a segment has all 256 chunks
+def test_decay_alone_over_many_chunks(gpu, dtype, S, H, d):
+    """Keys and values of zero: the last state is e^{gS} of the first, and the gradients' likewise, through every chunk's and every
+    segment's decay and nothing else, with decays that one float rounds by half a step."""
+    from q38.hip import ops
+    g = torch.tensor([_midway(n) for n in (64, 128, 256, 512)], device=gpu).repeat(H // 4)
+    r = torch.Generator(device=gpu).manual_seed(2)
+    S0, dS = (1.0 + torch.rand(1, H, d, d, generator=r, device=gpu) for _ in range(2))
+    x = torch.zeros(1, S, 1, d, dtype=dtype, device=gpu).expand(1, S, H, d)
+    out, last = ops.linear_attention(x, x, x, g, initial_state=S0, return_state=True)
+    assert not bool(out[0, :, :4].any())
+    left = torch.exp(g.double() * S)[:, None, None]
+    _within(last[0], S0[0].double() * left, DECAY_BOUND * S0[0].double() * left, "state")
+    ds = ops.linear_attention_backward(out.zero_(), dS, x, x, x, g, initial_state=S0, need_state=True)[3]
+    _within(ds[0], dS[0].double() * left, DECAY_BOUND * dS[0].double() * left, "ds")
