@@ -13,6 +13,7 @@ import functools
 import math
 
 import torch
+from torch.autograd import forward_ad
 
 from ._lib import BF16, FP32, TILING_PERSISTENT, TILING_SMALL, check, lib
 
@@ -1567,10 +1568,17 @@ def linear_attention_step(q, k, v, state, log_decay, scale=None, slots=None):
     """One token of every sequence through ``linear_attention`` (q38moe_linear_attention_step): q [B,H,dk], k [B,Hk,dk], v
     [B,Hk,dv] (bf16 or fp32), the states [pool,H,dk,dv] (fp32, contiguous) updated in place. Sequence b has the state
     slots[b] (int32 [B]; without slots the state b); a slot outside the pool, or that of an earlier sequence, is none: nothing
-    is updated and the output is zero. scale: dk^-1/2 unless given. Returns out [B,H,dv]; no gradients."""
+    is updated and the output is zero. scale: dk^-1/2 unless given. Returns out [B,H,dv]. It has no gradient: operands that
+    require one are refused unless gradients are off (torch.no_grad), and forward-mode tangents always."""
     _tensors(q=q, k=k, v=v, state=state, log_decay=log_decay)
     _float_type(q.dtype, "q")
     dev = _one_gpu(q, k, v, state, log_decay, slots)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or state.requires_grad
+                                    or log_decay.requires_grad):
+        raise ValueError("linear_attention_step has no gradient: pass detached tensors, or call it under torch.no_grad()")
+    if forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None
+                                              for t in (q, k, v, state, log_decay)):
+        raise ValueError("linear_attention_step has no forward-mode derivative")
     if not (state.is_contiguous() and log_decay.is_contiguous() and (slots is None or slots.is_contiguous())):
         raise ValueError("state, log_decay and slots must be contiguous")
     rest = (state.shape, state.dtype, log_decay.shape, log_decay.dtype, None if slots is None else slots.shape,

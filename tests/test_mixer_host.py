@@ -153,3 +153,37 @@ def test_linear_attention_abi_arguments():
     assert step(q=None) == -1 and says("q must not")
     assert step(g=None) == -1 and says("log_decay")
     assert step(B=0) == 0
+
+
+def test_step_refuses_gradients(monkeypatch):
+    """Operands that want a gradient or carry a tangent are refused; not under no_grad."""
+    from q38.hip import ops
+    names = ("q", "k", "v", "state", "log_decay")
+
+    def operands():
+        x = torch.zeros(4, 2, 64)
+        return dict(q=x, k=x.clone(), v=x.clone(), state=torch.zeros(4, 2, 64, 64), log_decay=torch.zeros(2))
+
+    def refused(args, text):
+        with monkeypatch.context() as m:  # as if the tensors were on a GPU
+            m.setattr(ops, "_one_gpu", lambda *tensors: tensors[0].device)
+            with pytest.raises(ValueError, match=text):
+                ops.linear_attention_step(**args)
+
+    def passed_on(args):
+        with pytest.raises(RuntimeError, match="CUDA/HIP tensor"):
+            ops.linear_attention_step(**args)
+
+    for name in names:
+        args = operands()
+        args[name].requires_grad_(True)
+        refused(args, "has no gradient")
+        with torch.no_grad():
+            passed_on(args)
+        args[name] = args[name] * 1.0  # a state that a prompt has left, say
+        refused(args, "has no gradient")
+        args = operands()
+        with torch.autograd.forward_ad.dual_level():
+            passed_on(args)
+            args[name] = torch.autograd.forward_ad.make_dual(args[name], torch.ones_like(args[name]))
+            refused(args, "forward-mode")
