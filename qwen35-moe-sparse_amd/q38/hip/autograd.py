@@ -336,7 +336,9 @@ def qk_norm_rope(q, k, q_norm, k_norm, positions, inv_freq, axes=None, eps=1e-6,
     bits, so far positions keep their angles). positions: int32 or int64 of q's leading shape, or, with axes (int32
     [len(inv_freq)], see ``ops.rope_axis_map``), [number of axes, ...] with frequency i turning by axis axes[i]: time, height and
     width of images and video. fp32 throughout and one rounding. Returns (q, k), contiguous; gradients flow to q, k and the
-    weights. Under bf16 autocast q, k and the weights are cast to bf16."""
+    weights, not to inv_freq. Under bf16 autocast q, k and the weights are cast to bf16."""
+    if inv_freq.requires_grad and torch.is_grad_enabled():
+        raise ValueError("inv_freq has no gradient here: pass inv_freq.detach()")
     if _bf16_autocast():
         q, k, q_norm, k_norm = (t if t is None else t.to(torch.bfloat16) for t in (q, k, q_norm, k_norm))
     positions = positions.contiguous()

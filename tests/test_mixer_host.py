@@ -187,3 +187,15 @@ def test_step_refuses_gradients(monkeypatch):
             passed_on(args)
             args[name] = torch.autograd.forward_ad.make_dual(args[name], torch.ones_like(args[name]))
             refused(args, "forward-mode")
+
+
+def test_rope_refuses_a_gradient_of_the_frequencies():
+    from q38.hip import autograd
+    q, k = torch.zeros(4, 2, 64), torch.zeros(4, 1, 64)
+    args = q, k, None, None, torch.arange(4), torch.ones(8, requires_grad=True)
+    with pytest.raises(ValueError, match="inv_freq has no gradient"):
+        autograd.qk_norm_rope(*args)
+    with pytest.raises(ValueError, match="inv_freq has no gradient"):
+        autograd.qk_norm_rope(*args[:5], args[5] * 1.0)
+    with torch.no_grad(), pytest.raises(RuntimeError, match="CUDA/HIP tensor"):
+        autograd.qk_norm_rope(*args)
