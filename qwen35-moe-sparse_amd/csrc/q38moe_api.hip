@@ -1900,12 +1900,17 @@ struct LinattnCut {
   int64_t segs;
   size_t states;
 };
+// A launch's thread ids have 32 bits.
+static int check_launch(int64_t blocks, int64_t threads) {
+  return blocks * threads >= (int64_t)1 << 32 ? fail(Q38MOE_EINVAL, "too many sequences and heads for one launch") : Q38MOE_OK;
+}
+// threads: of the largest workgroup that the call launches.
 static int linattn_cut(LinattnCut& c, int64_t N, int64_t S, int32_t H, int32_t dk, int32_t dv, bool packed, bool bf16,
-                       bool back) {
+                       bool back, int threads) {
   c.L = q38::la_segment_tokens(N, S, packed, H, bf16, dk, dv, back);
   c.nseg = packed ? 0 : (int)std::max<int64_t>(1, (S + c.L - 1) / c.L);
   c.segs = packed ? S / c.L + N : N * c.nseg;
-  if (c.segs * H + 8 * (int64_t)H + S / 64 >= (int64_t)1 << 31) return fail(Q38MOE_EINVAL, "too many sequences and heads for one launch");
+  Q38_CHECK(check_launch(c.segs * H + 8 * (int64_t)H + S / 64, threads));
   c.states = sizeof(float) * (size_t)(c.segs - N) * H * (size_t)q38::la_padded_state(dk, dv);
   return Q38MOE_OK;
 }
@@ -1922,9 +1927,11 @@ static int linattn_plan(LinattnPlan& p, int64_t N, int64_t S, int32_t H, int32_t
                         bool backward, bool own_states, int32_t dtype) {
   const bool bf16 = dtype == Q38MOE_BF16;
   p.tokens = packed ? S : N * S;
-  Q38_CHECK(linattn_cut(p.cut, N, S, H, dk, dv, packed, bf16, false));
+  const int wk = dk <= 64 ? 256 : 512, wv = dv <= 64 ? 256 : 512;  // 4 threads for each column of a padded state
+  const int threads = !backward ? wv : bf16 ? wk + wv : std::max(wk, wv);
+  Q38_CHECK(linattn_cut(p.cut, N, S, H, dk, dv, packed, bf16, false, threads));
   p.back = p.cut;
-  if (bf16 && !packed) Q38_CHECK(linattn_cut(p.back, N, S, H, dk, dv, packed, bf16, true));
+  if (bf16 && !packed) Q38_CHECK(linattn_cut(p.back, N, S, H, dk, dv, packed, bf16, true, threads));
   const bool grouped = backward && H != Hk;
   p.mid = packed ? align_up(sizeof(int32_t) * (size_t)(3 * N + 1)) : 0;
   p.grouped = p.mid + (own_states ? align_up(backward ? std::max(p.cut.states, p.back.states) : p.cut.states) : 0);
@@ -2097,7 +2104,7 @@ int q38moe_linear_attention_step(const void* q, const void* k, const void* v, co
   g_err[0] = 0;
   Q38_CHECK(check_linattn(B, 1, H, Hk, dk, dv, dtype));
   Q38_CHECK(check_strides(strides, 6, dtype));
-  if (B * H * ((dv + 31) / 32) >= (int64_t)1 << 31) return fail(Q38MOE_EINVAL, "too many sequences and heads for one launch");
+  Q38_CHECK(check_launch(B * H * ((dv + 31) / 32), 256));
   if (pool < 0) return fail(Q38MOE_EINVAL, "pool must be >= 0 (got %lld)", (long long)pool);
   if (slots == nullptr && B > pool)
     return fail(Q38MOE_EINVAL, "without slots the pool must hold every sequence (B=%lld, pool=%lld)", (long long)B, (long long)pool);

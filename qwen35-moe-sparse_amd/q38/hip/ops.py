@@ -1398,7 +1398,7 @@ def _mix_strides(named, size, dims):
 
 @functools.lru_cache(maxsize=1024)
 def _mix_plan(dt, k_dt, v_dt, qs, ks, vs, q_stride, k_stride, v_stride, g, g_dt, S0, S0_dt, cu, cu_dt, device):
-    """((N, S, H, Hk, dk, dv), strides or None, (workspace, saved states) forwards, the same backwards)."""
+    """((N, S, H, Hk, dk, dv), strides or None, (workspace, saved states) forwards)."""
     size = _float_type(dt, "q")
     if k_dt != dt or v_dt != dt:
         raise TypeError(f"k and v must be {dt}, got {k_dt} and {v_dt}")
@@ -1421,13 +1421,18 @@ def _mix_plan(dt, k_dt, v_dt, qs, ks, vs, q_stride, k_stride, v_stride, g, g_dt,
     if S0 is not None:
         _state_like("initial_state", S0, S0_dt, (N, H, dk, dv))
     shape = (N, S, H, Hk, dk, dv)
-    both = []
-    for backward in (False, True):
-        n, saved = ctypes.c_size_t(), ctypes.c_size_t()
-        check(lib.q38moe_linear_attention_workspace_bytes(*shape, cu is not None, backward, _DTYPES[dt], ctypes.byref(n),
+    return (shape, _mix_strides(((qs, q_stride), (ks, k_stride), (vs, v_stride)), size, 3),
+            _mix_bytes(shape, cu is not None, False, dt, device))
+
+
+@functools.lru_cache(maxsize=1024)
+def _mix_bytes(shape, packed, backward, dt, device):
+    """(workspace, saved states) of a call forwards or backwards, which takes fewer sequences and heads."""
+    n, saved = ctypes.c_size_t(), ctypes.c_size_t()
+    with _on(device):
+        check(lib.q38moe_linear_attention_workspace_bytes(*shape, packed, backward, _DTYPES[dt], ctypes.byref(n),
                                                           ctypes.byref(saved)), "q38moe_linear_attention_workspace_bytes")
-        both.append((n.value, saved.value))
-    return shape, _mix_strides(((qs, q_stride), (ks, k_stride), (vs, v_stride)), size, 3), *both
+    return n.value, saved.value
 
 
 def _decay_like(g, g_dt, H):
@@ -1441,7 +1446,7 @@ def _state_like(name, shape, dt, want):
 
 
 def _mix_operands(q, k, v, log_decay, scale, initial_state, cu_seqlens):
-    """(shape, workspaces, the C calls' arguments for the operands, what has to live until they are made)."""
+    """(shape, forward workspace, the C calls' arguments for the operands, what has to live until they are made)."""
     rest = (log_decay.shape, log_decay.dtype, None if initial_state is None else initial_state.shape,
             None if initial_state is None else initial_state.dtype, None if cu_seqlens is None else cu_seqlens.shape,
             None if cu_seqlens is None else cu_seqlens.dtype, q.device)
@@ -1451,11 +1456,11 @@ def _mix_operands(q, k, v, log_decay, scale, initial_state, cu_seqlens):
         q, k, v = _dense(q), _dense(k), _dense(v)
         plan = _mix_plan(q.dtype, k.dtype, v.dtype, q.shape, k.shape, v.shape, q.stride(), k.stride(), v.stride(), *rest)
         pq, pk, pv = q.data_ptr(), k.data_ptr(), v.data_ptr()
-    shape, strides, forwards, backwards = plan
-    return shape, forwards, backwards, (pq, pk, pv, strides, log_decay.data_ptr(),
-                                        shape[4] ** -0.5 if scale is None else scale,
-                                        None if initial_state is None else initial_state.data_ptr(),
-                                        None if cu_seqlens is None else cu_seqlens.data_ptr()), (q, k, v)
+    shape, strides, forwards = plan
+    return shape, forwards, (pq, pk, pv, strides, log_decay.data_ptr(),
+                             shape[4] ** -0.5 if scale is None else scale,
+                             None if initial_state is None else initial_state.data_ptr(),
+                             None if cu_seqlens is None else cu_seqlens.data_ptr()), (q, k, v)
 
 
 def _mix_check(q, k, v, log_decay, initial_state, cu_seqlens):
@@ -1478,7 +1483,8 @@ def linear_attention(q, k, v, log_decay, scale=None, initial_state=None, cu_seql
 def _linear_attention(q, k, v, log_decay, scale, initial_state, cu_seqlens, return_state, save):
     """(out, state, saved, what a backward pass of the same operands need not look at again, None where one had to be copied)."""
     dev = _mix_check(q, k, v, log_decay, initial_state, cu_seqlens)
-    shape, (n, states), backwards, args, used = _mix_operands(q, k, v, log_decay, scale, initial_state, cu_seqlens)
+    shape, (n, states), args, used = _mix_operands(q, k, v, log_decay, scale, initial_state, cu_seqlens)
+    backwards = _mix_bytes(shape, cu_seqlens is not None, True, q.dtype, q.device) if save else None
     N, S, H, _, dk, dv = shape
     out = _empty_like(q) if dk == dv else torch.empty((*q.shape[:3], dv), dtype=q.dtype, device=dev)
     state = torch.empty((N, H, dk, dv), dtype=torch.float32, device=dev) if return_state else None
@@ -1500,7 +1506,7 @@ def linear_attention_backward(d_out, d_final_state, q, k, v, log_decay, scale=No
     dev = _mix_check(q, k, v, log_decay, initial_state, cu_seqlens)
     _tensors(d_out=d_out)
     _one_gpu(q, d_out, d_final_state, saved)
-    (N, S, H, _, dk, dv), _, (_, states), _, _ = _mix_operands(q, k, v, log_decay, scale, initial_state, cu_seqlens)
+    (N, S, H, _, dk, dv), (_, states), _, _ = _mix_operands(q, k, v, log_decay, scale, initial_state, cu_seqlens)
     _same(d_out, "d_out", q.dtype, (q.shape[0], S, H, dv))
     if d_final_state is not None:
         _state_like("d_final_state", d_final_state.shape, d_final_state.dtype, (N, H, dk, dv))
@@ -1521,7 +1527,8 @@ def _linear_attention_backward(d_out, d_final_state, q, k, v, log_decay, scale, 
     if made is None or not (q.data_ptr() == pq and k.data_ptr() == pk and v.data_ptr() == pv and log_decay.data_ptr() == p_g
                             and _at(initial_state) == p_S0 and _at(cu_seqlens) == p_cu and q.stride() == q_stride
                             and k.stride() == k_stride and v.stride() == v_stride):
-        shape, _, (n, states), args, _alive = _mix_operands(q, k, v, log_decay, scale, initial_state, cu_seqlens)
+        shape, _, args, _alive = _mix_operands(q, k, v, log_decay, scale, initial_state, cu_seqlens)
+        n, states = _mix_bytes(shape, cu_seqlens is not None, True, q.dtype, q.device)
     N, _, H, _, dk, dv = shape
     if d_out.data_ptr() & 15:
         d_out = d_out.clone()

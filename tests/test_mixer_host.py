@@ -199,3 +199,28 @@ def test_rope_refuses_a_gradient_of_the_frequencies():
         autograd.qk_norm_rope(*args[:5], args[5] * 1.0)
     with torch.no_grad(), pytest.raises(RuntimeError, match="CUDA/HIP tensor"):
         autograd.qk_norm_rope(*args)
+
+
+def test_as_many_workgroups_as_a_launch_takes():
+    """A launch's thread ids have 32 bits: workgroups of 4 threads for each column of a padded state (64 or 128), of both dk and dv
+    backwards in bf16, of 256 in a step. Refused from there on, before anything is launched, and not below."""
+    m = _lib()
+    lib, n = m.lib, ctypes.c_size_t()
+
+    def query(N, H, dk, dv, dtype, backward, packed=0):
+        S = N if packed else 1
+        return lib.q38moe_linear_attention_workspace_bytes(N, S, H, H, dk, dv, packed, backward, dtype, ctypes.byref(n), None)
+
+    for dk, dv, dtype, backward, threads in [(128, 128, m.BF16, 0, 512), (64, 64, m.BF16, 0, 256), (128, 64, m.BF16, 0, 256),
+                                             (64, 128, m.FP32, 0, 512), (128, 128, m.BF16, 1, 1024), (64, 64, m.BF16, 1, 512),
+                                             (128, 64, m.BF16, 1, 768), (128, 64, m.FP32, 1, 512), (64, 64, m.FP32, 1, 256)]:
+        for H in (16, 3):
+            most = (1 << 32) // threads // H  # one-token sequences
+            assert query(most + 1, H, dk, dv, dtype, backward) == -1, (dk, dv, dtype, backward, H)
+            assert b"too many" in lib.q38moe_last_error()
+            assert query(most - 64, H, dk, dv, dtype, backward) == 0, (dk, dv, dtype, backward, H)
+    assert query(1 << 19, 16, 128, 128, 1, 0, packed=1) == -1 and query(1 << 18, 16, 128, 128, 1, 0, packed=1) == 0
+
+    six, p = (ctypes.c_int64 * 6)(*([64] * 6)), ctypes.c_void_p(1 << 20)
+    assert lib.q38moe_linear_attention_step(p, p, p, six, p, 1.0, p, p, p, 1 << 20, 1 << 20, 8, 8, 64, 64, 1, None) == -1
+    assert b"too many" in lib.q38moe_last_error()
