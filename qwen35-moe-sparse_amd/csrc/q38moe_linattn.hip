@@ -1025,10 +1025,18 @@ __global__ __launch_bounds__(256) void la_step_kernel(LaStepArgs a) {
   };
   f32x4_t o = {0.0f, 0.0f, 0.0f, 0.0f};
   bool mine = slot >= 0 && slot < a.pool;
-  if (a.slots != nullptr) {  // not one that an earlier sequence has: both would write it (without this look 94 us, with it 97)
+  // Not one that an earlier sequence has: both would write it. 1024 slots are looked at at once: 4096 sequences x 16 heads of 128
+  // take 1903 us, 1910 without slots (256 at a time 1937), 4096 x 2 of 64 49 and 42 (55), 16384 x 2 of 64 348 and 193 (473): all
+  // workgroups' looks grow with the square of the sequences, and beyond some thousands of few and narrow heads they show.
+  if (mine && a.slots != nullptr) {
     bool before = false;
-    for (int64_t n = tid; n < b; n += 256) before |= a.slots[n] == slot;
-    mine &= !__syncthreads_or(before);
+    const int32_t *at = a.slots + tid, *const end = a.slots + b;
+    for (; at + 3 * 256 < end; at += 4 * 256) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) before |= at[256 * i] == (int32_t)slot;
+    }
+    for (; at < end; at += 256) before |= *at == (int32_t)slot;
+    mine = !__syncthreads_or(before);
   }
   if (mine) {
     // In two floats: one is off by up to 2^-25 of the state in the same direction at every token, which adds up (after 20000 tokens of
