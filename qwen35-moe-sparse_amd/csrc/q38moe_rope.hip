@@ -6,7 +6,8 @@
 // and back, with dn the rotation of dy by -a, g = dn w', xh = x rstd:
 //   dx = rstd (g - xh mean(g xh)),  dw = sum over tokens and heads of dn xh.
 // fp32 throughout, one rounding of each result. The angle is a product in 64 bits, reduced to a fraction of a turn there
-// (in 32 bits a position of 10^6 leaves an angle uncertain by 0.06); its sine and cosine are fp32.
+// (in 32 bits a position of 10^6 leaves an angle uncertain by 0.06); its sine and cosine are those of an fp32 fraction of a turn
+// and of what it leaves of the angle (which alone is up to 2^-23, and all of a sine near half a turn).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -54,7 +55,10 @@ __device__ __forceinline__ void rope_turns(const RopeArgs& p, int64_t t0, int n,
       const double pos = p.pos64 ? (double)static_cast<const int64_t*>(p.pos)[at] : (double)static_cast<const int32_t*>(p.pos)[at];
       double turn = pos * (double)p.inv_freq[i] * 0.15915494309189533577;
       turn -= rint(turn);
-      sincospif(2.0f * (float)turn, &cs.y, &cs.x);
+      const float near = (float)turn, more = (float)(6.283185307179586 * (turn - (double)near));
+      float s, c;
+      sincospif(2.0f * near, &s, &c);
+      cs = make_float2(fmaf(-more, s, c), fmaf(more, c, s));  // the rest of the angle, at most 2^-23: to the first order
     }
     turns[u] = cs;
   }

@@ -154,3 +154,26 @@ def test_decay_alone_over_many_chunks(gpu, dtype, S, H, d):
     _within(last[0], S0[0].double() * left, DECAY_BOUND * S0[0].double() * left, "state")
     ds = ops.linear_attention_backward(out.zero_(), dS, x, x, x, g, initial_state=S0, need_state=True)[3]
     _within(ds[0], dS[0].double() * left, DECAY_BOUND * dS[0].double() * left, "ds")
+
+
+# ---- rotation -----------------------------------------------------------------------------------
+
+@pytest.mark.gpu
+def test_turns_near_their_zeros(gpu):
+    """Sines and cosines themselves, as the rotation of (1, 0) in fp32, at angles next to multiples of a quarter turn, where one of the
+    two is all that the angle's rounding leaves. The functions' 2 ulp (4 u), what the angle adds to them (u, and u for the product), and
+    the rotation's own rounding (u) of each; the angle's four roundings in 64 bits are absolute."""
+    from q38.hip import ops
+    # Whole numbers next to n quarter turns: numerators of convergents of pi / 2 and multiples of them.
+    at = [1, 2, 3, 11, 22, 33, 44, 355, 710, 1065, 52174, 104348, 260515, 521030, 1042060]
+    pos = torch.tensor(at + [5, 17, 100, 4097], device=gpu)
+    T, d = pos.numel(), 64
+    inv = torch.ones(d // 2, device=gpu)
+    inv[1:] = 0.5 ** torch.arange(1, d // 2, device=gpu)  # exact fractions of them
+    x = torch.zeros(T, 1, d, device=gpu)
+    x[..., :d // 2] = 1.0
+    q, k = ops.qk_norm_rope(x, x, None, None, pos, inv)
+    angle = pos.double()[:, None] * inv.double()
+    exact = torch.cat([angle.cos(), angle.sin()], -1)[:, None]
+    _within(q, exact, 7 * U * exact.abs() + 4 * 2.0 ** -53 * torch.cat([angle, angle], -1)[:, None], "turn")
+    assert torch.equal(q, k)
