@@ -508,11 +508,12 @@ __device__ __forceinline__ int la_turned(int i, int e, int w, int lr, int lq) {
 
 // One segment of one head; DV / 16 waves. Wave w has columns 16 w .. of the state and of the outputs for all 64 queries of a
 // chunk (outputs as [column, query] tiles), and some of the scores' six [32 keys, 16 queries] units, which go through LDS. The
-// state stays in accumulators, which, rounded, are the operand that queries read (la_row). A column's tokens come out of the
+// state stays in accumulators, which, in two bf16 parts, are the operand that queries read (la_row). A column's tokens come out of the
 // transposing LDS read in the order in which an accumulator holds the scores' keys, once for the outputs and for the state.
 // Two barriers a chunk: tiles and scores are read behind one, scores and the next tiles written behind the other.
-// Memory-bound: 4 x 4096 tokens x 16 heads of 128 bf16 (MI355X) take 68 us with OUT (302 MB, 4.4 TB/s; a large copy reaches
-// 5.1) and 36 us without (163 MB, 4.5 TB/s). fp32 is bound by its matrix instructions and the reads of their operands.
+// 4 x 4096 tokens x 16 heads of 128 bf16 (MI355X; median, and least, of 27 passes) take 86 (75) us with OUT (302 MB, 3.5 TB/s; a large
+// copy reaches 5.1), 41 (36) without (163 MB, 4.0 TB/s): bound by memory and vector instructions, which are busy 62 % of the time,
+// the matrix units 33 % (60 and 35 without; counters at 65536 tokens). fp32: 267 and 119 us, matrix units busy 58 and 35 %.
 template <bool BF16, int DK, int DV, bool REV, bool OUT>
 __global__ __launch_bounds__(4 * DV, la_waves(BF16, DK, DV, OUT)) void la_kernel(LaArgs a) {
   constexpr int ES = BF16 ? 2 : 4, KB = DK * ES, VB = DV * ES, NA = DK / 16, W = DV / 16, THREADS = 4 * DV;
@@ -750,7 +751,8 @@ __global__ __launch_bounds__(4 * DV, la_waves(BF16, DK, DV, OUT)) void la_kernel
 //   dk_j = scale sum_{i >= j} e^{g (i - j)} (v_j . dO_i) q_i + e^{g j'} T v_j
 // DV / 16 waves make dv and hold T as la_kernel's hold S; DK / 16 more make dk and read T, in two bf16 parts, from LDS, where the
 // first ones leave it once a chunk. One pass over q, k, v and dO instead of two over three of them each, and T made once:
-// 4 x 4096 tokens x 16 heads of 128 (MI355X) take 110 us (419 MB, 3.8 TB/s), two passes of la_kernel 2 x 68 and another carry.
+// 4 x 4096 tokens x 16 heads of 128 (MI355X; median, and least, of 27 passes) take 139 (121) us (419 MB, 3.0 TB/s; vector units busy
+// 47 % of the time, matrix units 27), two passes of la_kernel 2 x 86 and another carry.
 template <int DK, int DV>
 __global__ __launch_bounds__(4 * (DK + DV), DK == DV ? 4 : 3) void la_back_kernel(LaBackArgs a) {
   constexpr int KB = DK * 2, VB = DV * 2, NA = DK / 16, WV = DV / 16, WK = DK / 16, THREADS = 4 * (DK + DV);
@@ -940,7 +942,7 @@ __global__ __launch_bounds__(4 * (DK + DV), DK == DV ? 4 : 3) void la_back_kerne
 
 // mid[s] = e^{g L} (the state before segment s) + mid[s]: the state behind every segment but a sequence's last. A thread has 4
 // elements of one state, and the reads of the next LA_AHEAD segments are on their way while those of the last are added (31
-// segments of 16 heads of 128: 14.2 -> 11.1 us, 65 MB at 5.9 TB/s).
+// segments of 16 heads of 128 without 14.2 us, with 11.1; the median of 27 passes of 65536 tokens 12.7, 65 MB at 5.1 TB/s).
 constexpr int LA_AHEAD = 8;
 template <bool BF16, int DK, int DV>
 __global__ __launch_bounds__(256) void la_carry_kernel(LaArgs a) {
@@ -1006,7 +1008,8 @@ __global__ __launch_bounds__(256) void la_group_kernel(LaGroup a, LaGroup b, int
 }
 
 // One token: S = e^g S + k v^T in place, o = scale S^T q. Workgroup: 32 columns of one state, thread: 4 columns of every 32nd
-// row; HBM-bound, 8 bytes per element of the states: 256 sequences x 16 heads of 128 x 128 take 113 us (541 MB, 4.8 TB/s).
+// row; HBM-bound, 8 bytes per element of the states: 256 sequences x 16 heads of 128 x 128, a pool of 320, take 116 us (median; 541
+// MB, 4.7 TB/s).
 template <bool BF16>
 __global__ __launch_bounds__(256) void la_step_kernel(LaStepArgs a) {
   constexpr int ES = BF16 ? 2 : 4;
@@ -1153,26 +1156,28 @@ static int la_per_cu(bool bf16, int dk, int dv, bool back) {
 }
 
 // As long segments as still give every CU the workgroups that it holds: more segments cost more states to write and read (64 KB
-// at widths of 128, as much as 64 tokens' queries to outputs), fewer leave CUs idle. 4 x 4096 tokens x 16 heads of 128 forward
-// and back with 1, 2, 4, 8 a CU: 341, 339, 395, 513 us; 65536 tokens forward 447, 400, 433, 484.
+// at widths of 128, as much as 64 tokens' queries to outputs), fewer leave CUs idle. 16 heads with half, all, twice and four times
+// as many as a CU holds: 4 x 4096 tokens of 128 bf16 forward and back 462, 359, 390, 458 us, 65536 tokens forward 473, 425, 444, 473,
+// of 64 195, 220, 238, 263 (289 with a quarter); 16384 tokens fp32 forward of 128 694, 367, 368, 384, of 64 161, 133, 141.
 int la_segment_tokens(int64_t N, int64_t S, bool packed, int H, bool bf16, int dk, int dv, bool back) {
   const int per_cu = la_per_cu(bf16, dk, dv, back);
   const int64_t want = std::max<int64_t>(1, (int64_t)per_cu * device_cus() / H);
   const int64_t chunks = std::max<int64_t>(1, (S + LA_C - 1) / LA_C);
   // Two chunks of bf16 are quicker in one launch than in three, of fp32, which take longer, not. 128 tokens x 16 heads of 128
-  // forward in one and in two segments: bf16 15.0 and 17.8 us, fp32 32.1 and 31.9 (and back 77.7 and 69.5). Three chunks of bf16:
-  // 19.0 and 18.3.
+  // forward in one and in two segments: bf16 15.2 and 17.3 us, fp32 34.6 and 31.5 (and back 107 and 84); of 64 10.3 and 12.8, 17.5 and
+  // 17.6 (59 and 53). Three chunks of bf16 in one and in three: 19.8 and 17.7, of 64 13.4 and 12.9.
   if (!packed && bf16 && chunks <= 2) return 2 * LA_C;
   // Packed: sequences end inside of segments, half a one each, so these are made longer, up to a third; twice as long where the
-  // sequences alone fill the CUs and few of them have a second segment. 16 heads of 128 forward with n = want, 3/4, 1/2 of it, the
-  // mean of eight drawn sets: 8191 tokens in 8 sequences 84, 79, 84 us, in 23 83, 77, 85, in 100 95, 94, 84; 32768 in 12 258, 246,
-  // 287, in 120 260, 249, 231; in 3 with want - 1 and 3/4 of it 244, 263.
+  // sequences alone fill the CUs and few of them have a second segment. 16 heads of 128 forward with n = want, 3/4, 1/2 of it and by
+  // the rule, the mean of eight drawn sets: 8191 tokens in 8 sequences 88, 83, 90, 79 us, in 23 84, 79, 89, 79, in 100 97, 96, 88, 88;
+  // 32768 in 3 247, 270, 293, 235, in 12 264, 265, 303, 254, in 120 261, 254, 234, 234. Of 64: 8191 in 23 44, 41, 42, 42 (fp32 98,
+  // 95, 114, 95), 32768 in 12 111, 105, 114, 102, in 120 116, 120, 133, 121.
   const int64_t n = !packed         ? std::max<int64_t>(1, want / std::max<int64_t>(1, N))
                     : N >= 2 * want ? std::max<int64_t>(1, want / 2)
                                     : std::max({want - N / 2, want * 3 / 4, (int64_t)1});
   // A segment of one chunk costs twice its bytes in states, which pays while half of the workgroups' places are empty (of
-  // la_back_kernel's to the last one): 1024 tokens x 16 heads of 128 forward with one and two chunks a segment 23.7 and 25.5 us,
-  // 2048 tokens 37.0 and 32.0, of 64 4096 tokens 29.1 and 24.9.
+  // la_back_kernel's to the last one): 1024 tokens x 16 heads of 128 forward with one and two chunks a segment 26.2 and 27.5 us,
+  // 2048 tokens 38.3 and 33.2, of 64 4096 tokens 30.3 and 25.9.
   const bool two = !packed && bf16 && !back && 2 * chunks > n;
   return (int)std::max<int64_t>(two ? 2 : 1, (chunks + n - 1) / n) * LA_C;
 }

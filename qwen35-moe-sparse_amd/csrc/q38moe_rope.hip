@@ -94,8 +94,8 @@ __device__ __forceinline__ float head_sum(float v) {
 }
 
 // One block per p.tokens tokens, LPH lanes per head (d / 8 up to a power of two), every head of a token in turn: the turns of
-// a token are made once for all of its heads. HBM-bound: 16384 tokens x 40 heads of 64 bf16 take 39 us (168 MB, 4.3 TB/s; a large
-// copy reaches 5.1), 4097 x 18 of 256 18.5 us (76 MB, 4.1 TB/s).
+// a token are made once for all of its heads. HBM-bound: 16384 tokens x 40 heads of 64 bf16 take 40 us (median; 168 MB, 4.2 TB/s; a
+// large copy reaches 5.1), 4097 x 18 of 256 19.0 us (76 MB, 4.0 TB/s).
 template <bool BF16, int LPH>
 __global__ __launch_bounds__(ROPE_THREADS) void rope_kernel(RopeArgs p) {
   __shared__ float2 turns[ROPE_TURNS];
@@ -146,7 +146,7 @@ __global__ __launch_bounds__(ROPE_THREADS) void rope_kernel(RopeArgs p) {
 
 // The gradients: blocks take groups of p.tokens tokens in turn; a lane keeps the weights' gradients of its 8 features, the
 // block's go to partial[block][2][d] and rope_dw_kernel adds them in a fixed order. HBM-bound: 16384 tokens x 40 heads of 64 bf16
-// take 57 us (252 MB, 4.4 TB/s); 6 and 8 blocks a CU instead of 4, and two rows at a time, take as long.
+// take 58 us (median; 252 MB, 4.3 TB/s); 6 and 8 blocks a CU instead of 4, and two rows at a time, take as long.
 template <bool BF16, int LPH>
 __global__ __launch_bounds__(ROPE_THREADS) void rope_backward_kernel(RopeArgs p, const void* __restrict__ dyq,
                                                                      const void* __restrict__ dyk, float* __restrict__ partial) {
