@@ -1900,9 +1900,12 @@ struct LinattnCut {
   int64_t segs;
   size_t states;
 };
-// A launch's thread ids have 32 bits.
-static int check_launch(int64_t blocks, int64_t threads) {
-  return blocks * threads >= (int64_t)1 << 32 ? fail(Q38MOE_EINVAL, "too many sequences and heads for one launch") : Q38MOE_OK;
+// parts workgroups for each of H heads, and more: a launch's thread ids have 32 bits.
+static int check_launch(int64_t parts, int64_t H, int64_t more, int64_t threads) {
+  const int64_t most = 0xffffffff / threads;
+  if (parts > most / H || parts * H + more > most)
+    return fail(Q38MOE_EINVAL, "too many sequences and heads for one launch");
+  return Q38MOE_OK;
 }
 // threads: of the largest workgroup that the call launches.
 static int linattn_cut(LinattnCut& c, int64_t N, int64_t S, int32_t H, int32_t dk, int32_t dv, bool packed, bool bf16,
@@ -1910,7 +1913,7 @@ static int linattn_cut(LinattnCut& c, int64_t N, int64_t S, int32_t H, int32_t d
   c.L = q38::la_segment_tokens(N, S, packed, H, bf16, dk, dv, back);
   c.nseg = packed ? 0 : (int)std::max<int64_t>(1, (S + c.L - 1) / c.L);
   c.segs = packed ? S / c.L + N : N * c.nseg;
-  Q38_CHECK(check_launch(c.segs * H + 8 * (int64_t)H + S / 64, threads));
+  Q38_CHECK(check_launch(c.segs, H, 8 * (int64_t)H + S / 64, threads));
   c.states = sizeof(float) * (size_t)(c.segs - N) * H * (size_t)q38::la_padded_state(dk, dv);
   return Q38MOE_OK;
 }
@@ -2104,7 +2107,7 @@ int q38moe_linear_attention_step(const void* q, const void* k, const void* v, co
   g_err[0] = 0;
   Q38_CHECK(check_linattn(B, 1, H, Hk, dk, dv, dtype));
   Q38_CHECK(check_strides(strides, 6, dtype));
-  Q38_CHECK(check_launch(B * H * ((dv + 31) / 32), 256));
+  Q38_CHECK(check_launch(B * ((dv + 31) / 32), H, 0, 256));
   if (pool < 0) return fail(Q38MOE_EINVAL, "pool must be >= 0 (got %lld)", (long long)pool);
   if (slots == nullptr && B > pool)
     return fail(Q38MOE_EINVAL, "without slots the pool must hold every sequence (B=%lld, pool=%lld)", (long long)B, (long long)pool);

@@ -219,6 +219,10 @@ def test_as_many_workgroups_as_a_launch_takes():
             assert query(most + 1, H, dk, dv, dtype, backward) == -1, (dk, dv, dtype, backward, H)
             assert b"too many" in lib.q38moe_last_error()
             assert query(most - 64, H, dk, dv, dtype, backward) == 0, (dk, dv, dtype, backward, H)
+    for H in (1 << 20, 1 << 29, 1 << 30, (1 << 31) - 1):  # nor where the product passes 64 bits
+        assert query(1 << 24, H, 128, 128, m.BF16, 1) == -1 and b"too many" in lib.q38moe_last_error(), H
+    assert lib.q38moe_linear_attention_workspace_bytes(1 << 24, 1 << 30, (1 << 31) - 1, 1, 128, 128, 0, 0, m.BF16, ctypes.byref(n),
+                                                       None) == -1 and b"too many" in lib.q38moe_last_error()
     assert query(1 << 19, 16, 128, 128, 1, 0, packed=1) == -1 and query(1 << 18, 16, 128, 128, 1, 0, packed=1) == 0
 
     six, p = (ctypes.c_int64 * 6)(*([64] * 6)), ctypes.c_void_p(1 << 20)
