@@ -615,8 +615,8 @@ int q38moe_qk_norm_rope_backward(const void* d_q_out, const void* d_k_out, const
  * saved_bytes of states that the forward pass leaves and the backward pass of the same call takes (NULL: it makes them again).
  * step: one token of B sequences, q [B,H,dk], k [B,Hk,dk], v [B,Hk,dv] (strides: sequence and head of each), states updated in
  * place: state [pool,H,dk,dv], sequence b in slots[b] (NULL: b). A slot outside [0, pool), or that of an earlier sequence, is
- * none: out is zero. out [B,H,dv]. A call launches at most 2^32 threads: a segment of a head takes 4 for each column of its padded
- * state (64 or 128; backwards in bf16 of dk and dv together), a step 256 for 32 columns; beyond that it is refused.
+ * none: out is zero. out [B,H,dv]. A launch has fewer than 2^32 threads: a segment of a head takes 4 for each column of its padded
+ * state (64 or 128; backwards in bf16 of dk and dv together), a step 256 for 32 columns; a call of more is refused.
  */
 int q38moe_linear_attention_workspace_bytes(int64_t N, int64_t S, int32_t H, int32_t Hk, int32_t dk, int32_t dv, int32_t packed,
                                             int32_t backward, int32_t dtype, size_t* bytes, size_t* saved_bytes);
